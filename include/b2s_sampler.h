@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define B2S_ABI_VERSION 5
+#define B2S_ABI_VERSION 6
 
 /* return codes */
 #define B2S_OK 0
@@ -52,6 +52,7 @@ extern "C" {
 #define B2S_STATUS_WAIT_TIMEOUT 4u  /* a bounded device wait gave up; the row returned PAD */
 #define B2S_STATUS_COUNT_LIMIT 8u   /* a token repeated more than alpha_len-1 times; its count was clamped */
 #define B2S_STATUS_SHARD_INCOMPLETE 16u /* a shard's candidate list overflowed `cap` or failed; the row returned PAD */
+#define B2S_STATUS_TOKEN_RANGE 32u  /* a token id >= vocab was taken as no token (log probabilities) */
 
 /* flags */
 #define B2S_FLAG_FORCE_GENERAL 1 /* take the exact radix-select path even when the candidate path applies */
@@ -291,6 +292,120 @@ int b2s_repetition_penalty(const void* x, int32_t x_dtype, int32_t rows, int32_t
                            const int64_t* history, int32_t window, int64_t history_row_stride, const float* alpha,
                            int32_t alpha_len, int32_t alpha_row_stride, float* out, int64_t out_row_stride,
                            uint32_t* status, void* stream);
+
+/*
+ * Log probabilities of given tokens (ABI 6; no counterpart in the reference, whose call sites stop at the token).
+ * With z = logits / temperature per row: logprob = z[token] - logsumexp(z), entropy = -sum p log p, rank = how many
+ * ids come before the token in (value descending, id ascending) order (NaN above every number), and the first `top`
+ * ids of that order with their log probabilities ([rows, top], 0 <= top <= 32, top <= vocab).  A token < 0 (PAD) or
+ * >= vocab is no token: logprob 0, rank -1 (>= vocab also sets B2S_STATUS_TOKEN_RANGE).  A row that is -inf throughout
+ * has logprob -inf and entropy 0; NaN or +inf in a row makes its logprobs and entropy NaN.  tokens may be NULL (no
+ * tokens), and logprob, entropy, rank, stats and status are optional outputs; stats ([rows][4] fp32, 16-byte
+ * aligned) is what b2s_token_logprobs_grad needs.  Rows may lie any row_stride >= vocab elements apart.
+ */
+int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, int32_t vocab, int64_t row_stride,
+                       const int64_t* tokens, float temperature, int32_t top, float* logprob, float* entropy,
+                       int64_t* rank, int64_t* top_ids, float* top_logprobs, float* stats, uint32_t* status,
+                       void* stream);
+
+/*
+ * The gradient of sum grad_logprob[r] logprob[r] + grad_entropy[r] entropy[r] with respect to the logits, in their
+ * type (ABI 6): ((grad_logprob ([i = token] - p_i) - grad_entropy p_i (log p_i + entropy)) / temperature.  Either
+ * gradient may be NULL (zero).  0 for a row that is -inf throughout; a row without a token has no logprob part.
+ */
+int b2s_token_logprobs_grad(const void* logits, int32_t logits_dtype, int32_t rows, int32_t vocab, int64_t row_stride,
+                            const int64_t* tokens, float temperature, const float* stats, const float* grad_logprob,
+                            const float* grad_entropy, void* grad_logits, int64_t grad_row_stride, void* stream);
+
+/*
+ * The same straight from hidden rows and a language-model head (ABI 6): logits = hidden[rows, hidden_dim] x
+ * head[vocab, hidden_dim]^T in fp32 on the tensor cores, never rounded to bf16 and never written.  hidden_dim a
+ * multiple of 8; rows of hidden and head 16-byte aligned.  `workspace`: device memory of at least the bytes that
+ * b2s_lmhead_logprobs_workspace gives, 16-byte aligned, free again once the call's work is done.
+ * The gradient recomputes the logits tile by tile and writes their gradient once, in bf16, to its workspace (rows x
+ * vocab x 2 bytes), then grad_hidden = dz x head and grad_head = dz^T x hidden (bf16, contiguous, either may be NULL).
+ * status gets B2S_STATUS_TOKEN_RANGE and B2S_STATUS_WAIT_TIMEOUT.
+ */
+typedef struct b2s_lmhead_args {
+    const void* hidden;        /* [rows, hidden_dim] bf16 */
+    int64_t hidden_row_stride; /* elements, a multiple of 8 */
+    const void* head;          /* [vocab, hidden_dim] bf16 */
+    int64_t head_row_stride;   /* elements, a multiple of 8 */
+    int32_t hidden_dim;
+    int32_t vocab;
+    int32_t rows;
+    float temperature;
+    const int64_t* tokens;     /* [rows] */
+    void* workspace;
+    int64_t workspace_bytes;
+    uint32_t* status;          /* optional */
+} b2s_lmhead_args;
+int b2s_lmhead_logprobs_workspace(int32_t rows, int32_t vocab, int32_t hidden_dim, int64_t* bytes);
+int b2s_lmhead_logprobs(const b2s_lmhead_args* args, float* logprob, float* entropy, float* stats, void* stream);
+int b2s_lmhead_logprobs_grad_workspace(int32_t rows, int32_t vocab, int32_t hidden_dim, int64_t* bytes);
+int b2s_lmhead_logprobs_grad(const b2s_lmhead_args* args, const float* stats, const float* grad_logprob,
+                             const float* grad_entropy, void* grad_hidden, void* grad_head, void* stream);
+
+/*
+ * Projection with everything in its epilogue (ABI 6): out = act(x[rows, in] x weight[out, in]^T + bias) + residual,
+ * bf16 in and out, fp32 in between, rounded once.  in_features a multiple of 8, rows of x and weight 16-byte aligned;
+ * bias (16-byte aligned), residual and preact are optional; preact receives x weight^T + bias in bf16, which
+ * b2s_linear_grad needs when there is an activation.  `workspace`: b2s_linear_workspace bytes (may be 0).
+ */
+#define B2S_ACT_NONE 0
+#define B2S_ACT_RELU 1
+#define B2S_ACT_GELU 2 /* 0.5 z (1 + erf(z / sqrt 2)) */
+#define B2S_ACT_SILU 3
+typedef struct b2s_linear_args {
+    const void* x;
+    int64_t x_row_stride;
+    const void* weight;
+    int64_t weight_row_stride;
+    int32_t rows;
+    int32_t in_features;
+    int32_t out_features;
+    int32_t activation;
+    const void* bias;
+    const void* residual;
+    int64_t residual_row_stride;
+    void* out;
+    int64_t out_row_stride;
+    void* preact;
+    int64_t preact_row_stride; /* a multiple of 8 */
+    void* workspace;
+    int64_t workspace_bytes;
+    uint32_t* status;
+} b2s_linear_args;
+int b2s_linear_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes);
+int b2s_linear(const b2s_linear_args* args, void* stream);
+
+/*
+ * The projection's gradient (ABI 6): dz = grad_out act'(preact), grad_x = dz x weight, grad_weight = dz^T x, grad_bias
+ * = the sum of dz over the rows, each optional, bf16, contiguous (the residual's gradient is grad_out itself).  Sums
+ * are taken in a fixed order: the same call gives the same bits.
+ */
+typedef struct b2s_linear_grad_args {
+    const void* grad_out;
+    int64_t grad_out_row_stride;
+    const void* x;
+    int64_t x_row_stride;
+    const void* weight;
+    int64_t weight_row_stride;
+    const void* preact; /* needed with an activation */
+    int64_t preact_row_stride;
+    int32_t rows;
+    int32_t in_features;
+    int32_t out_features;
+    int32_t activation;
+    void* grad_x;
+    void* grad_weight;
+    void* grad_bias;
+    void* workspace;
+    int64_t workspace_bytes;
+    uint32_t* status;
+} b2s_linear_grad_args;
+int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes);
+int b2s_linear_grad(const b2s_linear_grad_args* args, void* stream);
 
 /* Human-readable text of a B2S_ERR_* code, and of the last CUDA error seen by this library. */
 const char* b2s_error_string(int code);

@@ -50,6 +50,40 @@ class HeadArgs(ctypes.Structure):
     ]
 
 
+class LMHeadArgs(ctypes.Structure):
+    """b2s_lmhead_args of include/b2s_sampler.h."""
+    _fields_ = [
+        ("hidden", ctypes.c_void_p), ("hidden_row_stride", ctypes.c_int64), ("head", ctypes.c_void_p),
+        ("head_row_stride", ctypes.c_int64), ("hidden_dim", ctypes.c_int32), ("vocab", ctypes.c_int32),
+        ("rows", ctypes.c_int32), ("temperature", ctypes.c_float), ("tokens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    """b2s_linear_args of include/b2s_sampler.h."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_row_stride", ctypes.c_int64), ("weight", ctypes.c_void_p),
+        ("weight_row_stride", ctypes.c_int64), ("rows", ctypes.c_int32), ("in_features", ctypes.c_int32),
+        ("out_features", ctypes.c_int32), ("activation", ctypes.c_int32), ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p), ("residual_row_stride", ctypes.c_int64), ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64), ("preact", ctypes.c_void_p), ("preact_row_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p),
+    ]
+
+
+class LinearGradArgs(ctypes.Structure):
+    """b2s_linear_grad_args of include/b2s_sampler.h."""
+    _fields_ = [
+        ("grad_out", ctypes.c_void_p), ("grad_out_row_stride", ctypes.c_int64), ("x", ctypes.c_void_p),
+        ("x_row_stride", ctypes.c_int64), ("weight", ctypes.c_void_p), ("weight_row_stride", ctypes.c_int64),
+        ("preact", ctypes.c_void_p), ("preact_row_stride", ctypes.c_int64), ("rows", ctypes.c_int32),
+        ("in_features", ctypes.c_int32), ("out_features", ctypes.c_int32), ("activation", ctypes.c_int32),
+        ("grad_x", ctypes.c_void_p), ("grad_weight", ctypes.c_void_p), ("grad_bias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p),
+    ]
+
+
 # every entry point of include/b2s_sampler.h with its ctypes signature
 CAPI_SIGNATURES = {
     "b2s_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), ctypes.c_void_p]),
@@ -79,6 +113,28 @@ CAPI_SIGNATURES = {
                                               ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                               ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
     "b2s_expf_spec": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "b2s_token_logprobs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                          ctypes.c_int64, ctypes.c_void_p, ctypes.c_float, ctypes.c_int32,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "b2s_token_logprobs_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                               ctypes.c_int64, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
+                                               ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                               ctypes.c_void_p]),
+    "b2s_lmhead_logprobs_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                                     ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_lmhead_logprobs": (ctypes.c_int, [ctypes.POINTER(LMHeadArgs), ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_void_p, ctypes.c_void_p]),
+    "b2s_lmhead_logprobs_grad_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                                          ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_lmhead_logprobs_grad": (ctypes.c_int, [ctypes.POINTER(LMHeadArgs), ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "b2s_linear_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                            ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
+    "b2s_linear_grad_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                                 ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_linear_grad": (ctypes.c_int, [ctypes.POINTER(LinearGradArgs), ctypes.c_void_p]),
     "b2s_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "b2s_last_cuda_error": (ctypes.c_char_p, []),
     "b2s_abi_version": (ctypes.c_int, []),

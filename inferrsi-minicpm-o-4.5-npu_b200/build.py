@@ -24,9 +24,9 @@ LIB = PKG / "libb2s.so"
 OPS = BUILD / "b2s_torch_ops.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = [CSRC / "b2s_sampler.cu", CSRC / "b2s_resident.cu", CSRC / "b2s_short.cu", CSRC / "b2s_shard.cu",
-              CSRC / "b2s_lmhead.cu"]
+              CSRC / "b2s_lmhead.cu", CSRC / "b2s_logprobs.cu", CSRC / "b2s_gemm.cu"]
 CU_HEADERS = [CSRC / "b2s_device.cuh", CSRC / "b2s_list.cuh", CSRC / "b2s_row.cuh", CSRC / "b2s_rowpaths.cuh",
-              CSRC / "b2s_head.cuh", INCLUDE / "b2s_sampler.h"]
+              CSRC / "b2s_head.cuh", CSRC / "b2s_logprobs.cuh", CSRC / "b2s_gemm.cuh", INCLUDE / "b2s_sampler.h"]
 
 
 def _nvcc() -> str:

@@ -1,0 +1,178 @@
+// The running softmax statistics the log-probability kernels share (logits rows and the head's epilogue).
+// See b2s_logprobs.cu for the formulas; everything is in base 2, c = log2(e) / T.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "b2s_device.cuh"
+
+namespace b2s {
+
+// m: maximum of the raw values (NaN once one was seen); S = sum 2^y, U = sum 2^y y with y relative to ref(m).
+struct LpState {
+    float m, S, U;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// y of x against the maximum m: fma(x, c, -fl(m c)), or (x - m) c where m c overflows; never below -200 (2^-200 is
+// nothing beside the maximum's 1, and 0 * -inf would be NaN).
+__device__ __forceinline__ float lp_y(float x, float m, float c) {
+    const float R = __fmul_rn(m, c);
+    const float y = fabsf(R) <= 3.0e38f ? __fmaf_rn(x, c, -R) : __fmul_rn(__fsub_rn(x, m), c);
+    return fmaxf(y, -200.0f);
+}
+
+// The shift of y when the maximum goes from `from` to `to` >= from (both finite).
+__device__ __forceinline__ float lp_shift(float from, float to, float c) {
+    const float Rf = __fmul_rn(from, c), Rt = __fmul_rn(to, c);
+    const float d = fabsf(Rf) <= 3.0e38f && fabsf(Rt) <= 3.0e38f ? __fsub_rn(Rf, Rt) : __fmul_rn(__fsub_rn(from, to), c);
+    return fmaxf(d, -400.0f);
+}
+
+// The state moved to the maximum m (s.m <= m, m neither NaN nor infinite).
+__device__ __forceinline__ void lp_rescale(LpState& s, float m, float c) {
+    if (s.m == f_ninf()) {
+        s.m = m;
+        return;  // S = U = 0
+    }
+    const float d = lp_shift(s.m, m, c), f = ex2(d);
+    s.U = f * __fmaf_rn(d, s.S, s.U);
+    s.S = f * s.S;
+    s.m = m;
+}
+
+__device__ __forceinline__ LpState lp_merge(LpState a, LpState b, float c) {
+    const float m = fmax_nan(a.m, b.m);
+    LpState r;
+    r.m = m;
+    r.S = r.U = 0.0f;
+    if (!(fabsf(m) <= 3.402823466e38f)) return r;  // NaN, +inf, or nothing but -inf
+    if (a.m != f_ninf()) {
+        lp_rescale(a, m, c);
+        r.S += a.S;
+        r.U += a.U;
+    }
+    if (b.m != f_ninf()) {
+        lp_rescale(b, m, c);
+        r.S += b.S;
+        r.U += b.U;
+    }
+    return r;
+}
+
+__device__ __forceinline__ void lp_warp_merge(LpState& s, float c) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        LpState t;
+        t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+        t.S = __shfl_xor_sync(0xffffffffu, s.S, o);
+        t.U = __shfl_xor_sync(0xffffffffu, s.U, o);
+        s = lp_merge(s, t, c);
+    }
+}
+
+// N elements at once, any values.
+template <int N>
+__device__ __forceinline__ void lp_add_many(LpState& s, const float (&x)[N], float c) {
+    float bm = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) bm = fmax_nan(bm, x[j]);
+    const float m = fmax_nan(s.m, bm);
+    if (!(fabsf(m) <= 3.402823466e38f)) {  // NaN or +inf so far (the row's outcome), or nothing but -inf
+        s.m = m;
+        return;
+    }
+    if (m > s.m) lp_rescale(s, m, c);
+    const float R = __fmul_rn(s.m, c);
+    float S = 0.0f, U = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float y = __fmaf_rn(x[j], c, -R), e = ex2(y);
+        S += e;
+        U = __fmaf_rn(e, y, U);
+    }
+    if (!(fabsf(U) <= 3.0e38f)) {  // a masked element (0 * -inf), or a reference that overflows
+        S = U = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float y = lp_y(x[j], s.m, c), e = x[j] == f_ninf() ? 0.0f : ex2(y);
+            S += e;
+            U = __fmaf_rn(e, y, U);
+        }
+    }
+    s.S += S;
+    s.U += U;
+}
+
+__device__ __forceinline__ void lp_add(LpState& s, float x, float c) {
+    const float v[1] = {x};
+    lp_add_many<1>(s, v, c);
+}
+
+// What the outputs need of a whole row.
+struct LpFinal {
+    float m, R, log2S, entropy;
+};
+
+__device__ __forceinline__ LpFinal lp_final(const LpState& s, float c) {
+    LpFinal f;
+    f.m = s.m;
+    f.R = __fmul_rn(s.m, c);
+    if (s.m == f_ninf()) {  // nothing left: probability 0 everywhere
+        f.log2S = 0.0f;
+        f.entropy = 0.0f;
+    } else if (!(fabsf(s.m) <= 3.402823466e38f)) {
+        f.m = f.log2S = f.entropy = __int_as_float(0x7fffffff);
+    } else {
+        f.log2S = log2f(s.S);
+        f.entropy = fmaxf((f.log2S - s.U / s.S) * 0.693147180559945309f, 0.0f);
+    }
+    return f;
+}
+
+// log p of the value x of a row.
+__device__ __forceinline__ float lp_value(float x, const LpFinal& f, float c) {
+    if (f.m != f.m) return f.m;
+    if (x == f_ninf()) return x;
+    const float y = fabsf(f.R) <= 3.0e38f ? __fmaf_rn(x, c, -f.R) : __fmul_rn(__fsub_rn(x, f.m), c);
+    // a value so low that y overflows in base 2 may still be a number in base e (log2 S is nothing beside it)
+    if (!(fabsf(y) <= 3.0e38f)) return __fmul_rn(__fsub_rn(x, f.m), c * 0.693147180559945309f);
+    return (y - f.log2S) * 0.693147180559945309f;
+}
+
+// The gradient of g_lp logprob + g_h entropy with respect to one value of a row.
+struct LpGrad {
+    float m, R, log2S, H, glp, gh, scale, inv_t;
+    int t;
+    // st: the forward's (m, R, log2S, entropy); the row's token or -1 (no gradient through logprob)
+    __device__ __forceinline__ LpGrad(float4 st, int tok, float g_lp, float g_h, float it)
+        : m(st.x), R(st.y), log2S(st.z), H(st.w), glp(tok >= 0 ? g_lp : 0.0f), gh(g_h), inv_t(it), t(tok) {
+        if (m == f_ninf()) glp = gh = 0.0f;  // nothing left
+        scale = -(glp + gh * H);
+    }
+    __device__ __forceinline__ float at(float x, int id, float c) const {
+        float y = fabsf(R) <= 3.0e38f ? __fmaf_rn(x, c, -R) : __fmul_rn(__fsub_rn(x, m), c);
+        y = m == f_ninf() ? -400.0f : fmax_nan(y - log2S, -400.0f);  // log2 p, kept finite where p is 0
+        const float p = ex2(y);
+        // -p (glp + gh H + gh log p) + [id = t] glp
+        float d = p * __fmaf_rn(-gh * 0.693147180559945309f, y, scale);
+        if (id == t) d += glp;
+        return d * inv_t;
+    }
+};
+
+// Host side: the scale log2(e) / T rounded once.
+inline float lp_scale(float temperature) { return (float)(1.4426950408889634 / (double)temperature); }
+// Temperatures whose scale is a normal number well inside fp32.
+inline bool lp_temperature_ok(float t) { return t >= 1e-6f && t <= 1e6f; }
+
+cudaError_t device_sms(int* sms);  // multiprocessors of the current device
+
+}  // namespace b2s

@@ -1549,6 +1549,29 @@ static EncodeTiledFn encode_tiled_fn() {
     return fn;
 }
 
+}  // extern "C"
+
+namespace b2s {
+// A 2-D bf16 tensor map: `inner` contiguous elements per row, `outer` rows `outer_stride` elements apart, boxes of
+// [box_outer x box_inner] in the 128-byte swizzle, elements outside read as zero.
+int tensor_map_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t outer_stride, int box_inner,
+                  int box_outer) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return cuda_fail(cudaErrorNotSupported);
+    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+    const cuuint64_t strides[1] = {(cuuint64_t)outer_stride * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? B2S_OK
+               : B2S_ERR_INVALID;
+}
+}  // namespace b2s
+
+extern "C" {
+
 int b2s_head_sample(const b2s_head_args* h, const b2s_sample_args* a, void* stream) {
     using namespace b2s;
     if (!h || !a || !h->hidden || !h->head || !h->logits || !h->sync) return B2S_ERR_INVALID;

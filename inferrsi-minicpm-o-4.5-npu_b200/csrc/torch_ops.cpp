@@ -548,6 +548,320 @@ Tensor uniform_meta(const Tensor& seeds, const Tensor&, const optional<Tensor>&,
     return at::empty(seeds.sizes(), seeds.options().dtype(at::kFloat));
 }
 
+uint32_t* status_ptr(const optional<Tensor>& status, const Tensor& like) {
+    if (!status.has_value() || !status->defined()) return nullptr;
+    TORCH_CHECK(status->is_cuda() && status->device() == like.device() && status->scalar_type() == at::kInt &&
+                    status->numel() == 1,
+                "status must be a 1-element int32 tensor on ", like.device());
+    return reinterpret_cast<uint32_t*>(status->data_ptr<int32_t>());
+}
+
+void check_same(const Tensor& t, const Tensor& like, at::ScalarType st, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
+    TORCH_CHECK(t.scalar_type() == st, name, " must be ", c10::toString(st), ", got ", t.scalar_type());
+}
+
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.size(1), 1); }
+// A [rows, n] tensor whose rows are contiguous and do not overlap (a copy where they are not).
+Tensor plain_rows(const Tensor& t) {
+    if ((t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1))) return t;
+    return t.contiguous();
+}
+// The same with rows on 16-byte boundaries (a copy where they are not); n is a multiple of 8.
+Tensor aligned_rows(const Tensor& t) {
+    Tensor p = plain_rows(t);
+    if ((p.size(0) > 1 && p.stride(0) % 8 != 0) || (reinterpret_cast<uintptr_t>(p.data_ptr()) & 15) != 0)
+        p = p.clone(at::MemoryFormat::Contiguous);
+    return p;
+}
+// A [rows] fp32 gradient as the kernels read it (the engine hands over expanded ones).
+Tensor grad_vector(const optional<Tensor>& t, const Tensor& like, int64_t rows, const char* name) {
+    if (!t.has_value() || !t->defined()) return Tensor();
+    check_same(*t, like, at::kFloat, name);
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == rows, name, " must be [rows]");
+    return t->contiguous();
+}
+float* opt_f(Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<float>() : nullptr; }
+
+int logits_dtype(const Tensor& logits) {
+    TORCH_CHECK(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16,
+                "logits must be float32 or bfloat16");
+    return logits.scalar_type() == at::kBFloat16 ? B2S_DTYPE_BF16 : B2S_DTYPE_F32;
+}
+
+void check_tokens(const Tensor& tokens, const Tensor& like, int64_t rows) {
+    check_same(tokens, like, at::kLong, "tokens");
+    TORCH_CHECK(tokens.dim() == 1 && tokens.size(0) == rows && tokens.is_contiguous(),
+                "tokens must be contiguous int64 [rows]");
+}
+
+// Log probabilities of given tokens from logits rows; stats ([B, 4], for the gradient) only where asked for.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_cuda(const Tensor& logits,
+                                                                               const Tensor& tokens, double temperature,
+                                                                               int64_t top, bool want_stats,
+                                                                               const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(logits.device());
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be CUDA [rows, vocab]");
+    const int dt = logits_dtype(logits);
+    const int64_t B = logits.size(0), V = logits.size(1);
+    TORCH_CHECK(B <= INT32_MAX && V <= INT32_MAX && top <= INT32_MAX, "more than 2^31 - 1 rows or ids");
+    check_tokens(tokens, logits, B);
+    const Tensor x = plain_rows(logits);
+    auto of = x.options().dtype(at::kFloat), oi = x.options().dtype(at::kLong);
+    Tensor lp = at::empty({B}, of), ent = at::empty({B}, of), rank = at::empty({B}, oi);
+    Tensor ids = at::empty({B, top}, oi), vals = at::empty({B, top}, of);
+    Tensor stats = at::empty({want_stats ? B : 0, 4}, of);
+    check_rc(b2s_token_logprobs(x.data_ptr(), dt, (int32_t)B, (int32_t)V, row_stride(x), tokens.data_ptr<int64_t>(),
+                                (float)temperature, (int32_t)top, lp.data_ptr<float>(), ent.data_ptr<float>(),
+                                rank.data_ptr<int64_t>(), top ? ids.data_ptr<int64_t>() : nullptr,
+                                top ? vals.data_ptr<float>() : nullptr, opt_f(stats), status_ptr(status, logits),
+                                at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_token_logprobs");
+    return {lp, ent, rank, ids, vals, stats};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_meta(const Tensor& logits, const Tensor&,
+                                                                               double, int64_t top, bool want_stats,
+                                                                               const optional<Tensor>&) {
+    const int64_t B = logits.size(0);
+    auto of = logits.options().dtype(at::kFloat), oi = logits.options().dtype(at::kLong);
+    return {at::empty({B}, of), at::empty({B}, of), at::empty({B}, oi), at::empty({B, top}, oi),
+            at::empty({B, top}, of), at::empty({want_stats ? B : 0, 4}, of)};
+}
+
+Tensor token_logprobs_grad_cuda(const Tensor& logits, const Tensor& tokens, const Tensor& stats,
+                                const optional<Tensor>& g_lp, const optional<Tensor>& g_ent, double temperature) {
+    c10::cuda::CUDAGuard guard(logits.device());
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be CUDA [rows, vocab]");
+    const int dt = logits_dtype(logits);
+    const int64_t B = logits.size(0), V = logits.size(1);
+    check_tokens(tokens, logits, B);
+    check_same(stats, logits, at::kFloat, "stats");
+    TORCH_CHECK(stats.is_contiguous() && stats.numel() == 4 * B, "stats must be contiguous [rows, 4]");
+    const Tensor x = plain_rows(logits);
+    Tensor gl = grad_vector(g_lp, logits, B, "grad_logprob"), ge = grad_vector(g_ent, logits, B, "grad_entropy");
+    Tensor out = at::empty({B, V}, x.options());
+    check_rc(b2s_token_logprobs_grad(x.data_ptr(), dt, (int32_t)B, (int32_t)V, row_stride(x),
+                                     tokens.data_ptr<int64_t>(), (float)temperature, stats.data_ptr<float>(),
+                                     opt_f(gl), opt_f(ge), out.data_ptr(), V,
+                                     at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_token_logprobs_grad");
+    return out;
+}
+
+Tensor token_logprobs_grad_meta(const Tensor& logits, const Tensor&, const Tensor&, const optional<Tensor>&,
+                                const optional<Tensor>&, double) {
+    return at::empty({logits.size(0), logits.size(1)}, logits.options());
+}
+
+// Checks of a head product's operands; hidden / head come back with rows on 16-byte boundaries.
+b2s_lmhead_args head_args(Tensor& hidden, Tensor& head, const Tensor& tokens, double temperature,
+                          const optional<Tensor>& status) {
+    TORCH_CHECK(hidden.is_cuda(), "hidden must be a CUDA tensor");
+    check_same(hidden, hidden, at::kBFloat16, "hidden");
+    check_same(head, hidden, at::kBFloat16, "head");
+    TORCH_CHECK(hidden.dim() == 2 && head.dim() == 2 && head.size(1) == hidden.size(1),
+                "hidden [rows, hidden_dim] and head [vocab, hidden_dim] do not fit");
+    TORCH_CHECK(hidden.size(1) % 8 == 0 && hidden.size(1) >= 8, "hidden_dim must be a multiple of 8");
+    TORCH_CHECK(hidden.size(0) <= INT32_MAX && head.size(0) <= INT32_MAX && hidden.size(1) <= INT32_MAX,
+                "a size is beyond 2^31 - 1");
+    check_tokens(tokens, hidden, hidden.size(0));
+    hidden = aligned_rows(hidden);
+    head = aligned_rows(head);
+    b2s_lmhead_args a;
+    memset(&a, 0, sizeof(a));
+    a.hidden = hidden.data_ptr();
+    a.hidden_row_stride = row_stride(hidden);
+    a.head = head.data_ptr();
+    a.head_row_stride = row_stride(head);
+    a.hidden_dim = (int32_t)hidden.size(1);
+    a.vocab = (int32_t)head.size(0);
+    a.rows = (int32_t)hidden.size(0);
+    a.temperature = (float)temperature;
+    a.tokens = tokens.data_ptr<int64_t>();
+    a.status = status_ptr(status, hidden);
+    return a;
+}
+
+Tensor workspace(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+
+// Log probabilities of given tokens straight from a head.
+std::tuple<Tensor, Tensor, Tensor> lmhead_logprobs_cuda(const Tensor& hidden_, const Tensor& head_,
+                                                        const Tensor& tokens, double temperature, bool want_stats,
+                                                        const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(hidden_.device());
+    Tensor hidden = hidden_, head = head_;
+    b2s_lmhead_args a = head_args(hidden, head, tokens, temperature, status);
+    auto of = hidden.options().dtype(at::kFloat);
+    Tensor lp = at::empty({a.rows}, of), ent = at::empty({a.rows}, of);
+    Tensor stats = at::empty({want_stats ? a.rows : 0, 4}, of);
+    check_rc(b2s_lmhead_logprobs_workspace(a.rows, a.vocab, a.hidden_dim, &a.workspace_bytes),
+             "b2s_lmhead_logprobs_workspace");
+    Tensor ws = workspace(a.workspace_bytes, hidden);
+    a.workspace = ws.data_ptr();
+    check_rc(b2s_lmhead_logprobs(&a, lp.data_ptr<float>(), ent.data_ptr<float>(), opt_f(stats),
+                                 at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_lmhead_logprobs");
+    return {lp, ent, stats};
+}
+
+std::tuple<Tensor, Tensor, Tensor> lmhead_logprobs_meta(const Tensor& hidden, const Tensor&, const Tensor&, double,
+                                                        bool want_stats, const optional<Tensor>&) {
+    const int64_t B = hidden.size(0);
+    auto of = hidden.options().dtype(at::kFloat);
+    return {at::empty({B}, of), at::empty({B}, of), at::empty({want_stats ? B : 0, 4}, of)};
+}
+
+std::tuple<Tensor, Tensor> lmhead_logprobs_grad_cuda(const Tensor& hidden_, const Tensor& head_, const Tensor& tokens,
+                                                     const Tensor& stats, const optional<Tensor>& g_lp,
+                                                     const optional<Tensor>& g_ent, double temperature,
+                                                     bool want_hidden, bool want_head, const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(hidden_.device());
+    Tensor hidden = hidden_, head = head_;
+    b2s_lmhead_args a = head_args(hidden, head, tokens, temperature, status);
+    check_same(stats, hidden, at::kFloat, "stats");
+    TORCH_CHECK(stats.is_contiguous() && stats.numel() == 4 * (int64_t)a.rows, "stats must be contiguous [rows, 4]");
+    Tensor gl = grad_vector(g_lp, hidden, a.rows, "grad_logprob"), ge = grad_vector(g_ent, hidden, a.rows, "grad_entropy");
+    Tensor dh = at::empty({want_hidden ? a.rows : 0, a.hidden_dim}, hidden.options());
+    Tensor dw = at::empty({want_head ? a.vocab : 0, a.hidden_dim}, hidden.options());
+    if (!want_hidden && !want_head) return {dh, dw};
+    check_rc(b2s_lmhead_logprobs_grad_workspace(a.rows, a.vocab, a.hidden_dim, &a.workspace_bytes),
+             "b2s_lmhead_logprobs_grad_workspace");
+    Tensor ws = workspace(a.workspace_bytes, hidden);
+    a.workspace = ws.data_ptr();
+    check_rc(b2s_lmhead_logprobs_grad(&a, stats.data_ptr<float>(), opt_f(gl), opt_f(ge),
+                                      want_hidden ? dh.data_ptr() : nullptr, want_head ? dw.data_ptr() : nullptr,
+                                      at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_lmhead_logprobs_grad");
+    return {dh, dw};
+}
+
+std::tuple<Tensor, Tensor> lmhead_logprobs_grad_meta(const Tensor& hidden, const Tensor& head, const Tensor&,
+                                                     const Tensor&, const optional<Tensor>&, const optional<Tensor>&,
+                                                     double, bool want_hidden, bool want_head, const optional<Tensor>&) {
+    return {at::empty({want_hidden ? hidden.size(0) : 0, hidden.size(1)}, hidden.options()),
+            at::empty({want_head ? head.size(0) : 0, head.size(1)}, hidden.options())};
+}
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// act(x weight^T + bias) + residual on [rows, in] x; the pre-activation ([rows, out rounded up to 8]) where asked for.
+std::tuple<Tensor, Tensor> linear_cuda(const Tensor& x_, const Tensor& weight_, const optional<Tensor>& bias,
+                                       const optional<Tensor>& residual, int64_t activation, bool want_preact,
+                                       const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(x_.device());
+    TORCH_CHECK(x_.is_cuda() && x_.dim() == 2 && weight_.dim() == 2 && x_.size(1) == weight_.size(1),
+                "x must be CUDA [rows, in] and weight [out, in]");
+    check_same(x_, x_, at::kBFloat16, "x");
+    check_same(weight_, x_, at::kBFloat16, "weight");
+    TORCH_CHECK(x_.size(1) >= 8 && x_.size(1) % 8 == 0, "in must be a multiple of 8");
+    TORCH_CHECK(x_.size(0) <= INT32_MAX && x_.size(1) <= INT32_MAX && weight_.size(0) <= INT32_MAX,
+                "a size is beyond 2^31 - 1");
+    const Tensor x = aligned_rows(x_), weight = aligned_rows(weight_);
+    const int64_t R = x.size(0), N = weight.size(0);
+    Tensor b, r;
+    if (bias.has_value() && bias->defined()) {
+        check_same(*bias, x, at::kBFloat16, "bias");
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "bias must be [out]");
+        b = bias->contiguous();
+        if (reinterpret_cast<uintptr_t>(b.data_ptr()) & 15) b = b.clone();
+    }
+    if (residual.has_value() && residual->defined()) {
+        check_same(*residual, x, at::kBFloat16, "residual");
+        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == R && residual->size(1) == N,
+                    "residual must be [rows, out]");
+        r = plain_rows(*residual);
+    }
+    Tensor out = at::empty({R, N}, x.options());
+    Tensor pre = at::empty({want_preact ? R : 0, round8(N)}, x.options());
+    b2s_linear_args a;
+    memset(&a, 0, sizeof(a));
+    a.x = x.data_ptr();
+    a.x_row_stride = row_stride(x);
+    a.weight = weight.data_ptr();
+    a.weight_row_stride = row_stride(weight);
+    a.rows = (int32_t)R;
+    a.in_features = (int32_t)x.size(1);
+    a.out_features = (int32_t)N;
+    a.activation = (int32_t)activation;
+    a.bias = b.defined() ? b.data_ptr() : nullptr;
+    a.residual = r.defined() ? r.data_ptr() : nullptr;
+    a.residual_row_stride = r.defined() ? row_stride(r) : 0;
+    a.out = out.data_ptr();
+    a.out_row_stride = N;
+    a.preact = want_preact ? pre.data_ptr() : nullptr;
+    a.preact_row_stride = round8(N);
+    check_rc(b2s_linear_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes), "b2s_linear_workspace");
+    Tensor ws;
+    if (a.workspace_bytes) {
+        ws = workspace(a.workspace_bytes, x);
+        a.workspace = ws.data_ptr();
+    }
+    a.status = status_ptr(status, x);
+    check_rc(b2s_linear(&a, at::cuda::getCurrentCUDAStream().stream()), "b2s_linear");
+    return {out, pre};
+}
+
+std::tuple<Tensor, Tensor> linear_meta(const Tensor& x, const Tensor& weight, const optional<Tensor>&,
+                                       const optional<Tensor>&, int64_t, bool want_preact, const optional<Tensor>&) {
+    return {at::empty({x.size(0), weight.size(0)}, x.options()),
+            at::empty({want_preact ? x.size(0) : 0, round8(weight.size(0))}, x.options())};
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_grad_cuda(const Tensor& grad_out, const Tensor& x_, const Tensor& weight_,
+                                                    const optional<Tensor>& preact, int64_t activation, bool want_x,
+                                                    bool want_weight, bool want_bias, const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(x_.device());
+    TORCH_CHECK(x_.is_cuda() && x_.dim() == 2 && weight_.dim() == 2 && x_.size(1) == weight_.size(1),
+                "x must be CUDA [rows, in] and weight [out, in]");
+    check_same(x_, x_, at::kBFloat16, "x");
+    check_same(weight_, x_, at::kBFloat16, "weight");
+    check_same(grad_out, x_, at::kBFloat16, "grad_out");
+    const int64_t R = x_.size(0), K = x_.size(1), N = weight_.size(0);
+    TORCH_CHECK(grad_out.dim() == 2 && grad_out.size(0) == R && grad_out.size(1) == N, "grad_out must be [rows, out]");
+    const Tensor x = aligned_rows(x_), weight = aligned_rows(weight_), g = plain_rows(grad_out);
+    Tensor dx = at::empty({want_x ? R : 0, K}, x.options()), dw = at::empty({want_weight ? N : 0, K}, x.options());
+    Tensor db = at::empty({want_bias ? N : 0}, x.options());
+    b2s_linear_grad_args a;
+    memset(&a, 0, sizeof(a));
+    a.grad_out = g.data_ptr();
+    a.grad_out_row_stride = row_stride(g);
+    a.x = x.data_ptr();
+    a.x_row_stride = row_stride(x);
+    a.weight = weight.data_ptr();
+    a.weight_row_stride = row_stride(weight);
+    if (activation != B2S_ACT_NONE) {
+        TORCH_CHECK(preact.has_value() && preact->defined(), "preact is needed with an activation");
+        check_same(*preact, x, at::kBFloat16, "preact");
+        TORCH_CHECK(preact->dim() == 2 && preact->size(0) == R && preact->size(1) == round8(N) && preact->is_contiguous(),
+                    "preact must be what linear gave");
+        a.preact = preact->data_ptr();
+        a.preact_row_stride = round8(N);
+    }
+    a.rows = (int32_t)R;
+    a.in_features = (int32_t)K;
+    a.out_features = (int32_t)N;
+    a.activation = (int32_t)activation;
+    a.grad_x = want_x ? dx.data_ptr() : nullptr;
+    a.grad_weight = want_weight ? dw.data_ptr() : nullptr;
+    a.grad_bias = want_bias ? db.data_ptr() : nullptr;
+    check_rc(b2s_linear_grad_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes),
+             "b2s_linear_grad_workspace");
+    Tensor ws = workspace(a.workspace_bytes, x);
+    a.workspace = ws.data_ptr();
+    a.status = status_ptr(status, x);
+    check_rc(b2s_linear_grad(&a, at::cuda::getCurrentCUDAStream().stream()), "b2s_linear_grad");
+    return {dx, dw, db};
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_grad_meta(const Tensor&, const Tensor& x, const Tensor& weight,
+                                                    const optional<Tensor>&, int64_t, bool want_x, bool want_weight,
+                                                    bool want_bias, const optional<Tensor>&) {
+    const int64_t K = x.size(1), N = weight.size(0);
+    return {at::empty({want_x ? x.size(0) : 0, K}, x.options()), at::empty({want_weight ? N : 0, K}, x.options()),
+            at::empty({want_bias ? N : 0}, x.options())};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(minicpmo_sampler, m) {
@@ -594,6 +908,25 @@ TORCH_LIBRARY(minicpmo_sampler, m) {
         "shard_resolve(Tensor logits, Tensor? history, Tensor? steps, Tensor? alpha, Tensor? row_temperature, "
         "Tensor? status, Tensor pending, Tensor merged, float temperature, float presence_penalty, "
         "float frequency_penalty, int eos, int min_new_tokens, int offset, int shard) -> Tensor");
+    m.def(
+        "token_logprobs(Tensor logits, Tensor tokens, float temperature, int top, bool want_stats, Tensor? status) -> "
+        "(Tensor logprob, Tensor entropy, Tensor rank, Tensor top_ids, Tensor top_logprobs, Tensor stats)");
+    m.def(
+        "token_logprobs_grad(Tensor logits, Tensor tokens, Tensor stats, Tensor? grad_logprob, Tensor? grad_entropy, "
+        "float temperature) -> Tensor");
+    m.def(
+        "lmhead_logprobs(Tensor hidden, Tensor head, Tensor tokens, float temperature, bool want_stats, "
+        "Tensor? status) -> (Tensor logprob, Tensor entropy, Tensor stats)");
+    m.def(
+        "lmhead_logprobs_grad(Tensor hidden, Tensor head, Tensor tokens, Tensor stats, Tensor? grad_logprob, "
+        "Tensor? grad_entropy, float temperature, bool want_hidden, bool want_head, Tensor? status) -> "
+        "(Tensor grad_hidden, Tensor grad_head)");
+    m.def(
+        "linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int activation, bool want_preact, "
+        "Tensor? status) -> (Tensor out, Tensor preact)");
+    m.def(
+        "linear_grad(Tensor grad_out, Tensor x, Tensor weight, Tensor? preact, int activation, bool want_x, "
+        "bool want_weight, bool want_bias, Tensor? status) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias)");
 }
 
 TORCH_LIBRARY_IMPL(minicpmo_sampler, CUDA, m) {
@@ -609,6 +942,12 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, CUDA, m) {
     m.impl("shard_candidates", &shard_candidates_cuda);
     m.impl("shard_merge", &shard_merge_cuda);
     m.impl("shard_resolve", &shard_resolve_cuda);
+    m.impl("token_logprobs", &token_logprobs_cuda);
+    m.impl("token_logprobs_grad", &token_logprobs_grad_cuda);
+    m.impl("lmhead_logprobs", &lmhead_logprobs_cuda);
+    m.impl("lmhead_logprobs_grad", &lmhead_logprobs_grad_cuda);
+    m.impl("linear", &linear_cuda);
+    m.impl("linear_grad", &linear_grad_cuda);
 }
 
 TORCH_LIBRARY_IMPL(minicpmo_sampler, Meta, m) {
@@ -624,4 +963,10 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, Meta, m) {
     m.impl("shard_candidates", &shard_candidates_meta);
     m.impl("shard_merge", &shard_merge_meta);
     m.impl("shard_resolve", &shard_resolve_meta);
+    m.impl("token_logprobs", &token_logprobs_meta);
+    m.impl("token_logprobs_grad", &token_logprobs_grad_meta);
+    m.impl("lmhead_logprobs", &lmhead_logprobs_meta);
+    m.impl("lmhead_logprobs_grad", &lmhead_logprobs_grad_meta);
+    m.impl("linear", &linear_meta);
+    m.impl("linear_grad", &linear_grad_meta);
 }
