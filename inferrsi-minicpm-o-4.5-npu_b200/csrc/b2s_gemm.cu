@@ -15,60 +15,141 @@ int tensor_map_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t out
 
 namespace {
 
+// Tile t (TM rows each) of the order that takes GM_GROUP x 128 rows at a time.
+template <int TM>
 __device__ __forceinline__ void tile_of(const GemmArgs& a, int64_t t, int* mt, int* nt) {
-    const int64_t per = (int64_t)GM_GROUP * a.tiles_n;
+    constexpr int GROUP = GM_GROUP * GM_M / TM;
+    const int64_t per = (int64_t)GROUP * a.tiles_n;
     const int g = (int)(t / per), in = (int)(t % per);
-    const int gm = min(GM_GROUP, a.tiles_m - g * GM_GROUP);
-    *mt = g * GM_GROUP + in % gm;
+    const int gm = min(GROUP, a.tiles_m - g * GROUP);
+    *mt = g * GROUP + in % gm;
     *nt = in / gm;
 }
 
-// The epilogue of one thread's row of a tile: columns [n0, n0 + TN) from tensor memory at `tm`.
-template <int TN, int EPI>
-__device__ __forceinline__ void epilogue_row(const GemmArgs& a, uint32_t tm, int row, int n0, int nt) {
+// The i-th piece of work of CTA (or pair) c of G: a tile and its k blocks [kb0, kb1); slot: where its sums go, -1 for a whole tile.
+struct Piece {
+    int64_t tile;
+    int kb0, kb1, slot;
+};
+template <int CG>
+__device__ __forceinline__ bool piece_at(const GemmArgs& a, int i, Piece* p) {
+    const int c = (int)blockIdx.x / CG, G = (int)gridDim.x / CG;
+    p->kb0 = 0;
+    p->kb1 = a.nkb;
+    p->slot = -1;
+    if (i < a.waves) {
+        p->tile = (int64_t)i * G + c;
+        return true;
+    }
+    const int64_t u = (int64_t)(i - a.waves) * G + c;
+    if (u >= (int64_t)a.rest * a.split) return false;
+    p->tile = (int64_t)a.waves * G + u % a.rest;
+    if (a.split > 1) {
+        p->kb0 = (int)(u / a.rest) * a.chunk;
+        p->kb1 = min(a.nkb, p->kb0 + a.chunk);
+        p->slot = (int)u;
+    }
+    return true;
+}
+
+// The epilogue of one warp's 32 rows of a tile: columns [n0, n0 + TN) from tensor memory at `tm` (lane = row).
+template <int TM, int TN, int EPI>
+__device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, int row0, int n0, int nt, int slot,
+                                              unsigned char* st) {
+    const int lane = threadIdx.x & 31, row = row0 + lane;
     const bool live = row < a.M;
-    if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
-        unsigned char* out = static_cast<unsigned char*>(a.out) + (int64_t)row * a.out_stride * 2;
+    const int rows = min(32, a.M - row0);  // <= 0: a warp past the last row
+    if constexpr (EPI != EPI_LSE) {
+        if (slot >= 0) {  // part of a split tile: its fp32 sums as they are
+            const int held = min(a.M, TM);
+            float* dst = a.partial + (int64_t)slot * held * TN + (int64_t)(row0 % TM) * TN;
 #pragma unroll 1
-        for (int q = 0; q < TN / 32; ++q) {
-            float v[32];
-            tmem_ld32(tm + 32u * q, v);
-            const int n = n0 + 32 * q;
-            if (live && n < a.N) {
+            for (int q = 0; q < TN / 32; ++q) {
+                float v[32];
+                tmem_ld32(tm + 32u * q, v);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int ng = n + 8 * g;
-                    if (ng < a.N) {
-                        float* w = v + 8 * g;
-                        if constexpr (EPI == EPI_LINEAR) {
-                            if (a.bias) {
-                                float b[8];
-                                load8(a.bias, ng, a.N, true, b);
+                for (int j = 0; j < 8; ++j)
+                    *stage_at(st, lane, j) = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                                        __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                __syncwarp();
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) w[j] += b[j];
-                            }
-                            // the saved pre-activation is bf16, like the tensors around it: the slope taken from it
-                            // is off by half a bf16 step of z times the activation's curvature, less than dz's own
-                            // rounding to the tensor cores' bf16
-                            if (a.preact)
-                                store8(static_cast<unsigned char*>(a.preact) + (int64_t)row * a.pre_stride * 2, ng, a.N,
-                                       true, w);
-                            if (a.act != ACT_NONE) {
+                for (int i = 0; i < 8; ++i) {
+                    const int r = 4 * i + (lane >> 3), c = lane & 7;
+                    if (r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)r * TN + 32 * q + 4 * c) = *stage_at(st, r, c);
+                }
+                __syncwarp();
+            }
+            return;
+        }
+    }
+    if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
+        unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride;
+        const unsigned short* res = static_cast<const unsigned short*>(a.residual) + (int64_t)row0 * a.res_stride;
+        const bool with_res = EPI == EPI_LINEAR && a.residual;
+        uint4 rq[8];
+        auto fetch = [&](int n) {  // the next block's residual, in flight meanwhile
+            if (with_res && a.res_vec && n + 64 <= a.N) block_fetch(rq, res + n, a.res_stride, rows);
+        };
+        fetch(n0);
+#pragma unroll 1
+        for (int q = 0; q < TN / 64; ++q) {
+            const int n = n0 + 64 * q, cols = a.N - n;
+            if (cols <= 0) break;
+            if (with_res) {
+                if (a.res_vec && cols >= 64) {
+                    block_put(st, rq);
+                    if (q + 1 < TN / 64) fetch(n + 64);
+                } else {
+                    block_load(st, res + n, a.res_stride, rows, cols);
+                }
+                __syncwarp();
+            }
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                float v[32];
+                tmem_ld32(tm + 64u * q + 32u * h, v);
+                if constexpr (EPI == EPI_LINEAR) {
+                    if (a.bias) {
+                        const int nb = n + 32 * h + lane;
+                        const float b = nb < a.N ? bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + nb)) : 0.0f;
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) w[j] = act_apply(w[j], a.act);
-                            }
-                            if (a.residual) {
-                                float r[8];
-                                load8(static_cast<const unsigned char*>(a.residual) + (int64_t)row * a.res_stride * 2,
-                                      ng, a.N, a.res_vec, r);
+                        for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
+                    }
+                    // the saved pre-activation is bf16, like the tensors around it: the slope taken from it is off by
+                    // half a bf16 step of z times the activation's curvature, less than dz's own rounding to the
+                    // tensor cores' bf16
+                    if (a.preact) stage_half(st + 4096, h, v);
+                    if (a.act == ACT_RELU) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) w[j] += r[j];
+                        for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_RELU>(v[j]);
+                    } else if (a.act == ACT_GELU) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_GELU>(v[j]);
+                    } else if (a.act == ACT_SILU) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_SILU>(v[j]);
+                    }
+                    if (with_res) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint4 u = *stage_at(st, lane, 4 * h + j);
+                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                v[8 * j + 2 * k] += __uint_as_float(w[k] << 16);
+                                v[8 * j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
                             }
                         }
-                        store8(out, ng, a.N, a.out_vec, w);
                     }
                 }
+                stage_half(st, h, v);  // this lane's own row: nobody else reads it before the barrier
             }
+            __syncwarp();
+            block_store(st, out + n, a.out_stride, rows, cols, a.out_vec);
+            if (EPI == EPI_LINEAR && a.preact)
+                block_store(st + 4096, static_cast<unsigned short*>(a.preact) + (int64_t)row0 * a.pre_stride + n,
+                            a.pre_stride, rows, cols, true);
+            __syncwarp();
         }
     } else if constexpr (EPI == EPI_LSE) {
         const int64_t tok = live ? a.tokens[row] : -1;
@@ -77,63 +158,68 @@ __device__ __forceinline__ void epilogue_row(const GemmArgs& a, uint32_t tm, int
         s.S = s.U = 0.0f;
 #pragma unroll 1
         for (int q = 0; q < TN / 32; ++q) {
+            const int n = n0 + 32 * q;
+            if (n >= a.N) break;
             float v[32];
             tmem_ld32(tm + 32u * q, v);
-            const int n = n0 + 32 * q;
-            if (n < a.N) {
-                if (tok >= n && tok < min(n + 32, a.N)) {
-                    float tv = v[0];
+            if (tok >= n && tok < min(n + 32, a.N)) {
+                float tv = v[0];
 #pragma unroll
-                    for (int j = 1; j < 32; ++j) tv = tok == n + j ? v[j] : tv;
-                    a.token_value[row] = tv;
-                }
-                if (n + 32 > a.N) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = n + j < a.N ? v[j] : f_ninf();
-                }
-                lp_add_many<32>(s, v, a.c);
+                for (int j = 1; j < 32; ++j) tv = tok == n + j ? v[j] : tv;
+                a.token_value[row] = tv;
             }
+            if (n + 32 > a.N) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = n + j < a.N ? v[j] : f_ninf();
+            }
+            lp_add_any<32>(s, v, a.c);
         }
         if (live) a.part[(int64_t)row * a.tiles_n + nt] = make_float4(s.m, s.S, s.U, 0.0f);
     } else {
         const int64_t tok = live ? a.tokens[row] : -1;
-        const float4 st = live ? a.stats[row] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const LpGrad g(st, tok >= 0 && tok < a.N ? (int)tok : -1, live && a.g_lp ? a.g_lp[row] : 0.0f,
+        const float4 stt = live ? a.stats[row] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const LpGrad g(stt, tok >= 0 && tok < a.N ? (int)tok : -1, live && a.g_lp ? a.g_lp[row] : 0.0f,
                        live && a.g_h ? a.g_h[row] : 0.0f, a.inv_t);
-        unsigned char* out = static_cast<unsigned char*>(a.out) + (int64_t)row * a.out_stride * 2;
+        unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride;
 #pragma unroll 1
-        for (int q = 0; q < TN / 32; ++q) {
-            float v[32];
-            tmem_ld32(tm + 32u * q, v);
-            const int n = n0 + 32 * q;
-            if (live && n < a.N) {
+        for (int q = 0; q < TN / 64; ++q) {
+            const int n = n0 + 64 * q, cols = a.N - n;
+            if (cols <= 0) break;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                float v[32];
+                tmem_ld32(tm + 64u * q + 32u * h, v);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = g.at(v[j], n + j, a.c);
+                for (int j = 0; j < 32; ++j) v[j] = g.at(v[j], n + 32 * h + j, a.c);
                 // dz is rounded to bf16 once: it is the tensor cores' operand in both gradient products
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n + 8 * j < a.N) store8(out, n + 8 * j, a.N, a.out_vec, v + 8 * j);
+                stage_half(st, h, v);
             }
+            __syncwarp();
+            block_store(st, out + n, a.out_stride, rows, cols, true);
+            __syncwarp();
         }
     }
 }
 
-template <int TN, bool AMN, bool BMN, int EPI>
+template <int CG, int TN, bool AMN, bool BMN, int EPI>
 __global__ void __launch_bounds__(GM_THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                 const __grid_constant__ GemmArgs a) {
-    constexpr int ST = gm_stages(TN);
-    constexpr uint32_t STAGE = gm_stage_bytes(TN);
+    constexpr int TM = CG * GM_M, BN = TN / CG;  // rows of a tile; this CTA's columns of B
+    constexpr int ST = gm_stages(CG, TN);
+    constexpr uint32_t STAGE = gm_stage_bytes(CG, TN);
     constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)AMN << 15) | ((uint32_t)BMN << 16) |
-                               ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(GM_M >> 4) << 24);
+                               ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
     extern __shared__ __align__(128) unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
     const uint32_t base_u = smem_u32(smem_raw);
     unsigned char* sm = smem_raw + (((base_u + 1023u) & ~1023u) - base_u);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + ST * STAGE);
+    unsigned char* staging = sm + ST * STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + GM_STAGING);  // the first CTA's serves both
     uint64_t* empty = full + ST;
     uint64_t* tfull = empty + ST;   // [2] an accumulator is complete
-    uint64_t* tempty = tfull + 2;   // [2] an accumulator has been read
+    uint64_t* tempty = tfull + 2;   // [2] an accumulator has been read (the first CTA's, by both)
     uint64_t* drain = tempty + 2;   // every MMA issued has completed (only after a failure)
     uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
@@ -149,7 +235,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], 128);
+            mbar_init(&tempty[s], 128 * CG);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -157,106 +243,150 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         *issued = 0;
         *consumed = 0;
     }
-    if (warp == 5) tmem_alloc(tslot, 2 * TN);
+    if (warp == 5) {
+        if constexpr (CG == 2) tmem_alloc_pair(tslot, 2 * TN);
+        else tmem_alloc(tslot, 2 * TN);
+    }
     tc_fence_before();
     __syncthreads();
+    if constexpr (CG == 2) {  // the partner's mbarriers exist before anything signals them
+        cluster_arrive_release();
+        cluster_wait();
+    }
     tc_fence_after();
     const uint32_t tmem = *tslot;
     pdl_wait_then_release();
 
-    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+    // The loading and the issuing warp run their loops converged, one lane elected where something is issued: with the
+    // loops inside a one-lane branch a k block cost the issuing thread 580 clocks, more than its MMAs' 512.
     if (warp == 4) {
-        if (lane == 0) {  // loads
-            int it = 0;
-            bool ok = true;
-            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                int mt, nt;
-                tile_of(a, t, &mt, &nt);
-                for (int kb = 0; kb < a.nkb; ++kb, ++it) {
-                    const int s = it % ST;
-                    if (it >= ST && !mbar_wait_bounded(&empty[s], (uint32_t)(it / ST - 1) & 1u, HEAD_WAIT_NS)) {
-                        *fail = 1;
-                        ok = false;
-                        break;
-                    }
-                    if (*fail) {
-                        ok = false;
-                        break;
-                    }
+        int s = 0, it = 0;
+        uint32_t ph = 1;  // parity of `empty`'s last phase: the first round finds every stage free
+        bool ok = true;
+        const uint32_t bar0 = CG == 2 ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
+        Piece p;
+        for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
+            int mt, nt;
+            tile_of<TM>(a, p.tile, &mt, &nt);
+            const int m0 = mt * TM + (int)rank * GM_M, n0 = nt * TN + (int)rank * BN;
+            for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
+                if (!gm_wait<false>(&empty[s], ph)) {
+                    *fail = 1;
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
                     unsigned char* sa = sm + s * STAGE;
                     unsigned char* sb = sa + GM_A_BYTES;
-                    mbar_arrive_expect_tx(&full[s], STAGE);  // parts outside the tensors are filled with zeros
+                    // parts outside the tensors are filled with zeros and count as bytes
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * STAGE);
+                    auto load = [&](unsigned char* dst, const CUtensorMap* map, int x, int y) {
+                        if constexpr (CG == 2) tma_load_2d_pair(dst, map, x, y, bar0 + 8u * s);
+                        else tma_load_2d(dst, map, x, y, &full[s]);
+                    };
                     if constexpr (AMN) {
 #pragma unroll
-                        for (int j = 0; j < GM_M / 64; ++j)
-                            tma_load_2d(sa + 8192 * j, &amap, mt * GM_M + 64 * j, kb * GM_KB, &full[s]);
+                        for (int j = 0; j < GM_M / 64; ++j) load(sa + 8192 * j, &amap, m0 + 64 * j, kb * GM_KB);
                     } else {
-                        tma_load_2d(sa, &amap, kb * GM_KB, mt * GM_M, &full[s]);
+                        load(sa, &amap, kb * GM_KB, m0);
                     }
                     if constexpr (BMN) {
 #pragma unroll
-                        for (int j = 0; j < TN / 64; ++j)
-                            tma_load_2d(sb + 8192 * j, &bmap, nt * TN + 64 * j, kb * GM_KB, &full[s]);
+                        for (int j = 0; j < BN / 64; ++j) load(sb + 8192 * j, &bmap, n0 + 64 * j, kb * GM_KB);
                     } else {
-                        tma_load_2d(sb, &bmap, kb * GM_KB, nt * TN, &full[s]);
+                        load(sb, &bmap, kb * GM_KB, n0);
                     }
                 }
+                __syncwarp();
+                if (++s == ST) {
+                    s = 0;
+                    ph ^= 1;
+                }
             }
-            *issued = it;
         }
+        if (lane == 0) *issued = it;
+        // the first CTA's last signals to this CTA's `empty` have landed before it leaves
+        if (CG == 2 && ok)
+            for (int k = it > ST ? it - ST : 0; k < it; ++k)
+                if (!gm_wait<false>(&empty[k % ST], (uint32_t)(k / ST) & 1u)) {
+                    *fail = 1;
+                    break;
+                }
     } else if (warp == 5) {
-        if (lane == 0) {  // MMAs
-            int it = 0, i = 0;
+        if (rank == 0) {  // MMAs
+            int s = 0, it = 0;
+            uint32_t ph = 0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
+            const uint64_t da0 = AMN ? umma_desc_mn128(smem_u32(sm)) : umma_desc_sw128(smem_u32(sm));
+            const uint64_t db0 = BMN ? umma_desc_mn128(smem_u32(sm) + GM_A_BYTES) : umma_desc_sw128(smem_u32(sm) + GM_A_BYTES);
+            auto commit = [&](uint64_t* bar) {
+                if constexpr (CG == 2) umma_commit_pair(bar);
+                else umma_commit(bar);
+            };
+            Piece p;
+            for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
                 const int acc = i & 1;
-                if (i >= 2 && !mbar_wait_bounded(&tempty[acc], (uint32_t)(i / 2 - 1) & 1u, HEAD_WAIT_NS)) {
+                if (i >= 2 && !gm_wait<CG == 2>(&tempty[acc], (uint32_t)(i / 2 - 1) & 1u)) {
                     *fail = 1;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)(acc * TN);
-                for (int kb = 0; kb < a.nkb; ++kb) {
-                    const int s = it % ST;
-                    if (*fail || !mbar_wait_bounded(&full[s], (uint32_t)(it / ST) & 1u, HEAD_WAIT_NS)) {
+                uint32_t more = 0;
+                for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
+                    if (!gm_wait<false>(&full[s], ph)) {
                         *fail = 1;
                         ok = false;
                         break;
                     }
-                    ++it;
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(sm + s * STAGE), b0 = a0 + GM_A_BYTES;
+                    if (elect_one()) {
+                        // a stage is STAGE bytes on, a step of 16 k 32 bytes (k contiguous) or 2 KB, in units of 16
+                        const uint64_t da = da0 + (uint32_t)s * (STAGE >> 4), db = db0 + (uint32_t)s * (STAGE >> 4);
 #pragma unroll
-                    for (int k = 0; k < GM_KB / 16; ++k)
-                        umma_bf16(d, AMN ? umma_desc_mn128(a0 + 2048u * k) : umma_desc_sw128(a0 + 32u * k),
-                                  BMN ? umma_desc_mn128(b0 + 2048u * k) : umma_desc_sw128(b0 + 32u * k), IDESC,
-                                  (kb | k) != 0 ? 1u : 0u);
-                    umma_commit(&empty[s]);
+                        for (int k = 0; k < GM_KB / 16; ++k) {
+                            if constexpr (CG == 2)
+                                umma_bf16_pair(d, da + (AMN ? 128 : 2) * k, db + (BMN ? 128 : 2) * k, IDESC, more);
+                            else
+                                umma_bf16(d, da + (AMN ? 128 : 2) * k, db + (BMN ? 128 : 2) * k, IDESC, more);
+                            more = 1;
+                        }
+                        commit(&empty[s]);
+                        if (kb + 1 == p.kb1) commit(&tfull[acc]);
+                    }
+                    more = 1;
+                    __syncwarp();
+                    if (++s == ST) {
+                        s = 0;
+                        ph ^= 1;
+                    }
                 }
-                if (ok) umma_commit(&tfull[acc]);
             }
-            *consumed = it;
+            if (lane == 0) *consumed = it;
             if (*fail) {
-                umma_commit(drain);
-                mbar_wait_bounded(drain, 0u, HEAD_WAIT_NS);
+                if (elect_one()) commit(drain);
+                __syncwarp();
+                gm_wait<false>(drain, 0u);
             }
         }
     } else {
-        int i = 0;
-        for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+        Piece p;
+        for (int i = 0; piece_at<CG>(a, i, &p); ++i) {
             int mt, nt;
-            tile_of(a, t, &mt, &nt);
+            tile_of<TM>(a, p.tile, &mt, &nt);
             const int acc = i & 1;
-            const bool ok = mbar_wait_bounded(&tfull[acc], (uint32_t)(i / 2) & 1u, HEAD_WAIT_NS);
+            const bool ok = gm_wait<false>(&tfull[acc], (uint32_t)(i / 2) & 1u);
             if (!__all_sync(0xffffffffu, ok) || *fail) {
                 *fail = 1;
                 break;
             }
             tc_fence_after();
-            epilogue_row<TN, EPI>(a, tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(acc * TN),
-                                  mt * GM_M + warp * 32 + lane, nt * TN, nt);
+            epilogue_rows<TM, TN, EPI>(a, tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(acc * TN),
+                                       mt * TM + (int)rank * GM_M + warp * 32, nt * TN, nt, p.slot,
+                                       staging + warp * 8192);
             tc_fence_before();
-            mbar_arrive(&tempty[acc]);
+            if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
+            else mbar_arrive(&tempty[acc]);
         }
     }
     __syncwarp();
@@ -264,30 +394,97 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
     __syncthreads();
     if (*fail && tid == 0) {
         if (a.status) atomicOr(a.status, B2S_STATUS_WAIT_TIMEOUT);
-        // loads issued but not seen landing still write this CTA's shared memory
-        for (int it = *consumed; it < *issued; ++it)
-            mbar_wait_bounded(&full[it % ST], (uint32_t)(it / ST) & 1u, HEAD_WAIT_NS);
+        // loads issued but not seen landing still write this CTA's shared memory: those that the first CTA counts are
+        // waited for, any other for a millisecond, a thousand times what a load takes
+        if (rank == 0)
+            for (int it = *consumed; it < *issued; ++it)
+                gm_wait<false>(&full[it % ST], (uint32_t)(it / ST) & 1u);
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000ull) {
+        }
+    }
+    if constexpr (CG == 2) {  // neither CTA leaves while the other may signal it or its MMAs read its shared memory
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait();
     }
     if (warp == 5) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * TN);
+        if constexpr (CG == 2) tmem_dealloc_pair(tmem, 2 * TN);
+        else tmem_dealloc(tmem, 2 * TN);
     }
 }
 
 template <typename... P, typename... A>
-cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, uint32_t smem, void* stream, A... args) {
+cudaError_t launch_cluster(void (*kernel)(P...), dim3 grid, int cluster, int threads, uint32_t smem, void* stream,
+                           A... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, uint32_t smem, void* stream, A... args) {
+    return launch_cluster(kernel, grid, 1, threads, smem, stream, args...);
+}
+
+// Adds a split tile's sums in k order and runs the epilogue: a thread per 4 columns of a row, grid.y = the split tiles.
+constexpr int FIX_NT = 256;
+template <int TM, int TN, int EPI>
+__global__ void __launch_bounds__(FIX_NT) gemm_join_kernel(const __grid_constant__ GemmArgs a, int G) {
+    pdl_wait_then_release();
+    int mt, nt;
+    tile_of<TM>(a, (int64_t)a.waves * G + blockIdx.y, &mt, &nt);
+    const int held = min(a.M, TM), rows = min(TM, a.M - mt * TM);
+    const int i = (int)blockIdx.x * FIX_NT + (int)threadIdx.x;
+    const int lr = i / (TN / 4), n = nt * TN + (i % (TN / 4)) * 4, row = mt * TM + lr;
+    if (lr >= rows || n >= a.N) return;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* part = a.partial + ((int64_t)blockIdx.y * held + lr) * TN + n - nt * TN;
+    const int64_t step = (int64_t)a.rest * held * TN;
+#pragma unroll 4
+    for (int s = 0; s < a.split; ++s) {
+        const float4 p = *reinterpret_cast<const float4*>(part + s * step);
+        v[0] += p.x;
+        v[1] += p.y;
+        v[2] += p.z;
+        v[3] += p.w;
+    }
+    unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row * a.out_stride + n;
+    const int cols = min(4, a.N - n);
+    if (EPI == EPI_LINEAR) {
+        const unsigned short* bias = static_cast<const unsigned short*>(a.bias);
+        const unsigned short* res = static_cast<const unsigned short*>(a.residual) + (int64_t)row * a.res_stride + n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j < cols) {
+                if (bias) v[j] += bf16_bits_to_f(__ldg(bias + n + j));
+                if (a.preact)
+                    (static_cast<__nv_bfloat16*>(a.preact) + (int64_t)row * a.pre_stride + n)[j] = __float2bfloat16_rn(v[j]);
+                v[j] = act_apply(v[j], a.act);
+                if (a.residual) v[j] += bf16_bits_to_f(__ldg(res + j));
+            }
+        }
+    }
+    if (a.out_vec && cols == 4) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < cols) out[j] = __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
+    }
 }
 
 // An operand of a product: rows of `k` elements `stride` apart (k contiguous), or, transposed, k rows of `m` elements.
@@ -296,44 +493,111 @@ struct Operand {
     int64_t stride;
 };
 
-template <int TN, bool AMN, bool BMN, int EPI>
-int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, void* stream) {
+// How a product is cut: CTAs per tile, columns per tile, CTAs (or pairs) at work, whole waves, the rest and the chunks
+// along k that the rest is cut into.
+struct Plan {
+    int cg, tn, G, waves, rest, split, chunk;
+    int64_t bytes;  // of the split's workspace
+};
+// The cheapest cut by estimated clocks.  A k block costs a CTA its MMAs (measured without loads: 530 clocks for 256 or
+// 128 columns alike, 290 for 64) or its stage's way from L2 (64 bytes a clock; rows outside A are not fetched); an
+// epilogue that nothing overlaps costs about 8 clocks a column; a split costs a second launch, about 5000 clocks, and
+// its sums' way out and back, about 3000 bytes a clock over all SMs.
+Plan plan_for(int M, int N, int64_t K, bool may_split, int sms) {
+    Plan best = {};
+    int64_t best_cost = INT64_MAX;
+    const int64_t nkb = (K + GM_KB - 1) / GM_KB;
+    auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    for (int cg = 2; cg >= 1; --cg) {
+        for (int tn = 256; tn >= (cg == 2 ? 128 : 64); tn >>= 1) {
+            if (cg == 2 && M <= GM_M) continue;  // half of the pair would have no rows
+            const int tm = cg * GM_M, U = sms / cg;
+            const int64_t tiles = ceil_div(M, tm) * ceil_div(N, tn);
+            const int64_t mma = tn == 64 ? 290 : 530, fill = 2 * ((M < GM_M ? M : GM_M) + tn / cg);
+            const int64_t kb_cost = mma > fill ? mma : fill;
+            Plan p = {};
+            p.cg = cg;
+            p.tn = tn;
+            p.G = (int)(tiles < U ? tiles : U);
+            p.waves = (int)(tiles / U);
+            p.rest = (int)(tiles % U);
+            p.split = 1;
+            p.chunk = (int)nkb;
+            int64_t cost = (p.waves + (p.rest ? 1 : 0)) * nkb * kb_cost;
+            if (may_split && p.rest) {
+                const int64_t held = M < tm ? M : tm;
+                for (int64_t want = 2; want <= nkb && want <= 64; ++want) {
+                    const int64_t chunk = ceil_div(nkb, want), split = ceil_div(nkb, chunk);
+                    const int64_t bytes = split * p.rest * held * tn * 4;
+                    const int64_t c = (p.waves * nkb + ceil_div(p.rest * split, U) * chunk) * kb_cost + 5000 + 2 * bytes / 3000;
+                    if (split > 1 && c < cost) {
+                        cost = c;
+                        p.split = (int)split;
+                        p.chunk = (int)chunk;
+                        p.bytes = bytes;
+                        p.G = (int)(p.waves || p.rest * split >= U ? U : p.rest * split);
+                    }
+                }
+            }
+            cost += 8 * tn;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = p;
+            }
+        }
+    }
+    return best;
+}
+
+// The plan on the current device (without one, where only sizes are asked for, on a B200's 148 multiprocessors).
+Plan plan_here(int M, int N, int64_t K, bool may_split) {
+    int sms = 0;
+    if (device_sms(&sms) != cudaSuccess || sms < 1) sms = 148;
+    return plan_for(M, N, K, may_split, sms);
+}
+
+template <int CG, int TN, bool AMN, bool BMN, int EPI>
+int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, const Plan& p, void* stream) {
+    constexpr int TM = CG * GM_M;
     CUtensorMap amap, bmap;
     int rc = AMN ? tensor_map_2d(&amap, A.base, a.M, K, A.stride, 64, GM_KB)
                  : tensor_map_2d(&amap, A.base, K, a.M, A.stride, GM_KB, GM_M);
     if (rc == B2S_OK)
         rc = BMN ? tensor_map_2d(&bmap, B.base, a.N, K, B.stride, 64, GM_KB)
-                 : tensor_map_2d(&bmap, B.base, K, a.N, B.stride, GM_KB, TN);
+                 : tensor_map_2d(&bmap, B.base, K, a.N, B.stride, GM_KB, TN / CG);
     if (rc != B2S_OK) return rc;
-    a.tiles_m = (a.M + GM_M - 1) / GM_M;
+    a.tiles_m = (a.M + TM - 1) / TM;
     a.tiles_n = (a.N + TN - 1) / TN;
     a.nkb = (int)((K + GM_KB - 1) / GM_KB);
-    int sms = 0;
-    cudaError_t e = device_sms(&sms);
+    a.waves = p.waves;
+    a.rest = p.rest;
+    a.split = p.split;
+    a.chunk = p.chunk;
+    const auto kernel = gemm_kernel<CG, TN, AMN, BMN, EPI>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gm_smem(CG, TN));
     if (e != cudaSuccess) return cuda_fail(e);
-    const auto kernel = gemm_kernel<TN, AMN, BMN, EPI>;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gm_smem(TN));
-    if (e != cudaSuccess) return cuda_fail(e);
-    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-    e = launch_pdl(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), GM_THREADS, gm_smem(TN), stream, amap, bmap, a);
+    e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, GM_THREADS, gm_smem(CG, TN), stream, amap, bmap, a);
+    if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
+        if (e == cudaSuccess && p.split > 1) {
+            const int held = a.M < TM ? a.M : TM;
+            e = launch_pdl(gemm_join_kernel<TM, TN, EPI>,
+                           dim3((unsigned)((held * (TN / 4) + FIX_NT - 1) / FIX_NT), (unsigned)p.rest), FIX_NT, 0, stream,
+                           a, p.G);
+        }
+    }
     return e == cudaSuccess ? B2S_OK : cuda_fail(e);
-}
-
-int tile_cols(int M, int N) {
-    int sms = 0;
-    if (device_sms(&sms) != cudaSuccess) sms = 148;
-    const int64_t mt = (M + GM_M - 1) / GM_M;
-    for (int tn = 256; tn > 64; tn >>= 1)
-        if (mt * ((N + tn - 1) / tn) >= sms) return tn;
-    return 64;
 }
 
 template <bool AMN, bool BMN, int EPI>
 int gemm(const Operand& A, const Operand& B, int64_t K, const GemmArgs& a, void* stream) {
-    switch (tile_cols(a.M, a.N)) {
-        case 256: return gemm_tn<256, AMN, BMN, EPI>(A, B, K, a, stream);
-        case 128: return gemm_tn<128, AMN, BMN, EPI>(A, B, K, a, stream);
-        default: return gemm_tn<64, AMN, BMN, EPI>(A, B, K, a, stream);
+    const Plan p = plan_here(a.M, a.N, K, EPI == EPI_LINEAR || EPI == EPI_STORE);
+    if (p.cg == 2)
+        return p.tn == 256 ? gemm_tn<2, 256, AMN, BMN, EPI>(A, B, K, a, p, stream)
+                           : gemm_tn<2, 128, AMN, BMN, EPI>(A, B, K, a, p, stream);
+    switch (p.tn) {
+        case 256: return gemm_tn<1, 256, AMN, BMN, EPI>(A, B, K, a, p, stream);
+        case 128: return gemm_tn<1, 128, AMN, BMN, EPI>(A, B, K, a, p, stream);
+        default: return gemm_tn<1, 64, AMN, BMN, EPI>(A, B, K, a, p, stream);
     }
 }
 
@@ -376,53 +640,65 @@ __global__ void __launch_bounds__(LM_NT) lmhead_merge_kernel(const float4* part,
 
 // ------------------------------------------------------------------ the projection's elementwise gradient
 
-// dz = dy act'(z) (bf16, rows dz_stride apart) and the sums of its columns over this CTA's rows: 32 groups of 8
-// columns x 8 rows in turn per CTA; the sums (fp32, of the unrounded dz) go to part[blockIdx.y][n], or, with one
+// dz = dy act'(z) (bf16, rows dz_stride apart) and the sums of its columns over this CTA's rows, E columns of a row per
+// thread: 8 where dy's rows are 16-byte aligned, else 1, so that a warp's loads stay whole lines.  32 threads cover 32 E
+// columns, the 8 warps take rows in turn; the sums (fp32, of the unrounded dz) go to part[blockIdx.y][n], or, with one
 // part, straight to the bias gradient.
 constexpr int DZ_NT = 256;
-__global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_t dy_stride, int dy_vec, const void* z,
+template <int E>
+__global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_t dy_stride, const void* z,
                                                           int64_t z_stride, int act, int rows, int N, int rows_per,
                                                           void* dz, int64_t dz_stride, float* part, void* db) {
     pdl_wait_then_release();
-    __shared__ float red[8][32][9];
+    __shared__ float red[8][32][E + 1];
     const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5;
-    const int n = (blockIdx.x * 32 + cg) * 8;
+    const int n = (blockIdx.x * 32 + cg) * E;
     const int r0 = blockIdx.y * rows_per, r1 = min(rows, r0 + rows_per);
-    float sum[8] = {};
+    float sum[E] = {};
     if (n < N) {
+#pragma unroll 4
         for (int r = r0 + rl; r < r1; r += 8) {
-            float g[8];
-            load8(static_cast<const unsigned char*>(dy) + (int64_t)r * dy_stride * 2, n, N, dy_vec, g);
-            if (act != ACT_NONE) {
-                float x[8];
-                load8(static_cast<const unsigned char*>(z) + (int64_t)r * z_stride * 2, n, N, true, x);
+            const unsigned short* gp = static_cast<const unsigned short*>(dy) + (int64_t)r * dy_stride;
+            const unsigned short* zp = static_cast<const unsigned short*>(z) + (int64_t)r * z_stride;
+            if constexpr (E == 8) {
+                float g[8];
+                load8(gp, n, N, true, g);
+                if (act != ACT_NONE) {
+                    float x[8];
+                    load8(zp, n, N, true, x);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] *= act_slope(x[j], act);
+                    for (int j = 0; j < 8; ++j) g[j] *= act_slope(x[j], act);
+                }
+                if (dz) store8(static_cast<unsigned short*>(dz) + (int64_t)r * dz_stride, n, N, true, g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += g[j];
+            } else {
+                float g = bf16_bits_to_f(__ldg(gp + n));
+                if (act != ACT_NONE) g *= act_slope(bf16_bits_to_f(__ldg(zp + n)), act);
+                if (dz) (static_cast<__nv_bfloat16*>(dz) + (int64_t)r * dz_stride)[n] = __float2bfloat16_rn(g);
+                sum[0] += g;
             }
-            if (dz) store8(static_cast<unsigned char*>(dz) + (int64_t)r * dz_stride * 2, n, N, true, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += g[j];
         }
     }
     if (!part && !db) return;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) red[rl][cg][j] = sum[j];
+    for (int j = 0; j < E; ++j) red[rl][cg][j] = sum[j];
     __syncthreads();
-    const int i = threadIdx.x, c = i >> 3, j = i & 7;  // one column per thread
+    const int i = threadIdx.x, c = i / E, j = i % E;  // one column per thread
+    const int col = blockIdx.x * 32 * E + i;
+    if (i >= 32 * E || col >= N) return;
     float s = red[0][c][j];
 #pragma unroll
     for (int k = 1; k < 8; ++k) s += red[k][c][j];
-    const int col = blockIdx.x * 256 + i;
-    if (col < N) {
-        if (part) part[(int64_t)blockIdx.y * N + col] = s;
-        else static_cast<__nv_bfloat16*>(db)[col] = __float2bfloat16_rn(s);
-    }
+    if (part) part[(int64_t)blockIdx.y * N + col] = s;
+    else static_cast<__nv_bfloat16*>(db)[col] = __float2bfloat16_rn(s);
 }
 __global__ void linear_db_kernel(const float* part, int parts, int N, void* db) {
     pdl_wait_then_release();
     const int n = blockIdx.x * blockDim.x + threadIdx.x;
     if (n >= N) return;
     float s = 0.0f;
+#pragma unroll 8
     for (int p = 0; p < parts; ++p) s += part[(int64_t)p * N + n];
     static_cast<__nv_bfloat16*>(db)[n] = __float2bfloat16_rn(s);
 }
@@ -454,7 +730,7 @@ extern "C" {
 int b2s_lmhead_logprobs_workspace(int32_t rows, int32_t vocab, int32_t hidden_dim, int64_t* bytes) {
     using namespace b2s;
     if (rows < 0 || vocab < 1 || hidden_dim < 8 || !bytes) return B2S_ERR_INVALID;
-    const int tn = tile_cols(rows, vocab);
+    const int tn = plan_here(rows > 0 ? rows : 1, vocab, hidden_dim, false).tn;
     *bytes = up((int64_t)rows * ((vocab + tn - 1) / tn) * 16 + (int64_t)rows * 4, 256);
     return B2S_OK;
 }
@@ -470,7 +746,7 @@ int b2s_lmhead_logprobs(const b2s_lmhead_args* h, float* logprob, float* entropy
     b2s_lmhead_logprobs_workspace(h->rows, h->vocab, h->hidden_dim, &need);
     if (!h->tokens || !h->workspace || h->workspace_bytes < need || !aligned16(h->workspace) || (stats && !aligned16(stats)))
         return B2S_ERR_INVALID;
-    const int tn = tile_cols(h->rows, h->vocab);
+    const int tn = plan_here(h->rows, h->vocab, h->hidden_dim, false).tn;
     const int tiles = (h->vocab + tn - 1) / tn;
     GemmArgs a;
     memset(&a, 0, sizeof(a));
@@ -493,7 +769,9 @@ int b2s_lmhead_logprobs(const b2s_lmhead_args* h, float* logprob, float* entropy
 int b2s_lmhead_logprobs_grad_workspace(int32_t rows, int32_t vocab, int32_t hidden_dim, int64_t* bytes) {
     using namespace b2s;
     if (rows < 0 || vocab < 1 || hidden_dim < 8 || !bytes) return B2S_ERR_INVALID;
-    *bytes = up((int64_t)rows * up(vocab, 8) * 2, 256);
+    const int64_t r = rows > 0 ? rows : 1;
+    const int64_t dh = plan_here((int)r, hidden_dim, vocab, true).bytes, dw = plan_here(vocab, hidden_dim, r, true).bytes;
+    *bytes = up(r * up(vocab, 8) * 2, 256) + up(dh > dw ? dh : dw, 256);
     return B2S_OK;
 }
 
@@ -539,6 +817,7 @@ int b2s_lmhead_logprobs_grad(const b2s_lmhead_args* h, const float* stats, const
     b.out_vec = 1;
     b.N = h->hidden_dim;
     b.out_stride = h->hidden_dim;
+    b.partial = reinterpret_cast<float*>(static_cast<unsigned char*>(h->workspace) + up((int64_t)h->rows * ldz * 2, 256));
     if (grad_hidden) {
         b.M = h->rows;
         b.out = grad_hidden;
@@ -554,8 +833,9 @@ int b2s_lmhead_logprobs_grad(const b2s_lmhead_args* h, const float* stats, const
 }
 
 int b2s_linear_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
+    using namespace b2s;
     if (rows < 0 || in_features < 8 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
-    *bytes = 0;
+    *bytes = rows ? plan_here(rows, out_features, in_features, true).bytes : 0;
     return B2S_OK;
 }
 
@@ -572,6 +852,9 @@ int b2s_linear(const b2s_linear_args* l, void* stream) {
         (l->preact && (!aligned16(l->preact) || l->preact_row_stride < l->out_features || l->preact_row_stride % 8)) ||
         ((reinterpret_cast<uintptr_t>(l->out) | reinterpret_cast<uintptr_t>(l->residual)) & 1))
         return B2S_ERR_INVALID;
+    int64_t need = 0;
+    b2s_linear_workspace(l->rows, l->in_features, l->out_features, &need);
+    if (need && (!l->workspace || l->workspace_bytes < need || !aligned16(l->workspace))) return B2S_ERR_INVALID;
     GemmArgs a;
     memset(&a, 0, sizeof(a));
     a.M = l->rows;
@@ -587,6 +870,7 @@ int b2s_linear(const b2s_linear_args* l, void* stream) {
     a.act = l->activation;
     a.preact = l->preact;
     a.pre_stride = l->preact_row_stride;
+    a.partial = static_cast<float*>(l->workspace);
     return gemm<false, false, EPI_LINEAR>({l->x, l->x_row_stride}, {l->weight, l->weight_row_stride}, l->in_features, a,
                                           stream);
 }
@@ -594,8 +878,11 @@ int b2s_linear(const b2s_linear_args* l, void* stream) {
 int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
     using namespace b2s;
     if (rows < 0 || in_features < 8 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
-    *bytes = up((int64_t)rows * up(out_features, 8) * 2, 256) +
-             up((int64_t)dz_parts(rows, out_features) * out_features * 4, 256);
+    const int64_t r = rows > 0 ? rows : 1;
+    const int64_t dx = plan_here((int)r, in_features, out_features, true).bytes;
+    const int64_t dw = plan_here(out_features, in_features, r, true).bytes;
+    *bytes = up(r * up(out_features, 8) * 2, 256) + up((int64_t)dz_parts((int)r, out_features) * out_features * 4, 256) +
+             up(dx > dw ? dx : dw, 256);
     return B2S_OK;
 }
 
@@ -628,15 +915,17 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
     const bool direct = l->activation == B2S_ACT_NONE && dy_vec;
     const bool products = l->grad_x || l->grad_weight;
     Operand dz = {l->workspace, ldz};
+    const int parts = dz_parts(l->rows, l->out_features);
+    float* part = reinterpret_cast<float*>(static_cast<unsigned char*>(l->workspace) + up((int64_t)l->rows * ldz * 2, 256));
     if (direct) dz = {l->grad_out, l->grad_out_row_stride};
     if ((products && !direct) || l->grad_bias) {
-        const int parts = dz_parts(l->rows, l->out_features);
-        float* part = reinterpret_cast<float*>(static_cast<unsigned char*>(l->workspace) + up((int64_t)l->rows * ldz * 2, 256));
         const int per = (l->rows + parts - 1) / parts;
         const bool two = l->grad_bias && parts > 1;
-        cudaError_t e = launch_pdl(linear_dz_kernel, dim3((unsigned)((l->out_features + 255) / 256), (unsigned)parts),
-                                   DZ_NT, 0, stream, l->grad_out, l->grad_out_row_stride, (int)dy_vec, l->preact,
-                                   l->preact_row_stride, (int)l->activation, (int)l->rows, (int)l->out_features, per,
+        const int width = dy_vec ? 256 : 32;  // columns per CTA
+        cudaError_t e = launch_pdl(dy_vec ? linear_dz_kernel<8> : linear_dz_kernel<1>,
+                                   dim3((unsigned)((l->out_features + width - 1) / width), (unsigned)parts), DZ_NT, 0,
+                                   stream, l->grad_out, l->grad_out_row_stride, l->preact, l->preact_row_stride,
+                                   (int)l->activation, (int)l->rows, (int)l->out_features, per,
                                    products && !direct ? l->workspace : nullptr, ldz, two ? part : nullptr,
                                    two ? nullptr : l->grad_bias);
         if (e == cudaSuccess && two)
@@ -650,6 +939,8 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
     b.out_vec = 1;
     b.N = l->in_features;
     b.out_stride = l->in_features;
+    b.partial = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(part) +
+                                         up((int64_t)parts * l->out_features * 4, 256));
     int rc = B2S_OK;
     if (l->grad_x) {
         b.M = l->rows;

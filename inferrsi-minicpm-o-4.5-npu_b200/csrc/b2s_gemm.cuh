@@ -4,11 +4,19 @@
 // gradient's transposed operand), without a transposed copy: the 128-byte swizzled shared-memory layouts of both
 // orders are fed to the same MMA through its descriptors.
 //
-// A persistent CTA takes tiles of 128 x TN in an order that keeps a group of row tiles together (so that a wave's
-// operands stay in L2).  Warp 4 fills a ring of stages by TMA, warp 5 issues the MMAs and the other four warps run the
-// epilogue of one tile on one half of tensor memory while the MMAs of the next fill the other half.  Every wait is
-// bounded; a wait that gives up ends all roles, waits (bounded) for copies and MMAs in flight, and sets
-// B2S_STATUS_WAIT_TIMEOUT.
+// A persistent CTA, or a pair of them (a cluster of two on one tile, cta_group::2), takes tiles of 128 or 256 x TN in an
+// order that keeps a group of row tiles together (so that a wave's operands stay in L2).  What bounds a large product is
+// the way from L2 to the SMs, about 64 bytes a clock each: a 128 x 256 tile of one CTA asks for 96 while its MMAs run
+// (48 KB per 512 clocks), so it keeps the tensor pipe 60 % busy; a pair holds 128 rows of A each and half of B's
+// columns, and asks for 64.  Warp 4 fills a ring of stages by TMA, warp 5 issues the MMAs and the other four warps run the
+// epilogue of one tile on one half of tensor memory while the MMAs of the next fill the other half.  Tiles that do not
+// fill a wave are split along k into equal chunks, all tiles' first chunks first (CTAs at work at the same time then
+// read the same k range of both operands, once from HBM); a chunk's fp32 sums go to a workspace, and a second kernel
+// adds them in k order and runs the epilogue, so the result does not depend on timing.  Rows go to and from global memory through a swizzled 4 KB block of shared memory per
+// warp, whole 128-byte lines at a time.  The epilogues are loops over 32 columns with short bodies: unrolled over a
+// tile, with every activation inlined per element, they ran from beyond the instruction cache and a 128 x 256 tile took
+// 17 to 47 us.  Every wait is bounded; a wait that gives up ends all roles,
+// waits (bounded) for copies and MMAs in flight, and sets B2S_STATUS_WAIT_TIMEOUT.
 #pragma once
 
 #include "b2s_head.cuh"
@@ -22,19 +30,25 @@ constexpr int GM_THREADS = 192;  // warps 0-3: epilogue (their tensor-memory qua
 constexpr int GM_GROUP = 16;     // row tiles taken together
 constexpr uint32_t GM_A_BYTES = GM_M * GM_KB * 2;
 
-__host__ __device__ constexpr uint32_t gm_b_bytes(int tn) { return (uint32_t)tn * GM_KB * 2; }
-__host__ __device__ constexpr uint32_t gm_stage_bytes(int tn) { return GM_A_BYTES + gm_b_bytes(tn); }
-// as many stages as fit 200 KB, at most 8
-__host__ __device__ constexpr int gm_stages(int tn) {
-    return (int)(200u * 1024u / gm_stage_bytes(tn)) > 8 ? 8 : (int)(200u * 1024u / gm_stage_bytes(tn));
+// A stage of one CTA: its 128 rows of A and its 1 / CG of the TN columns of B.
+__host__ __device__ constexpr uint32_t gm_stage_bytes(int cg, int tn) { return GM_A_BYTES + (uint32_t)(tn / cg) * GM_KB * 2; }
+constexpr uint32_t GM_STAGING = 4 * 8192;  // two blocks of 32 rows x 128 bytes per epilogue warp
+// as many stages as fit 192 KB, at most 8
+__host__ __device__ constexpr int gm_stages(int cg, int tn) {
+    return (int)(192u * 1024u / gm_stage_bytes(cg, tn)) > 8 ? 8 : (int)(192u * 1024u / gm_stage_bytes(cg, tn));
 }
-__host__ __device__ constexpr uint32_t gm_smem(int tn) { return 1024 + gm_stages(tn) * gm_stage_bytes(tn) + 256; }
+__host__ __device__ constexpr uint32_t gm_smem(int cg, int tn) {
+    return 1024 + gm_stages(cg, tn) * gm_stage_bytes(cg, tn) + GM_STAGING + 256;
+}
 
 enum { EPI_LINEAR = 0, EPI_LSE = 1, EPI_DZ = 2, EPI_STORE = 3 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
 
 struct GemmArgs {
     int M, N, nkb, tiles_m, tiles_n;
+    // full waves of whole tiles, then `rest` tiles in `split` chunks of `chunk` k blocks each (split 1: whole tiles)
+    int waves, rest, split, chunk;
+    float* partial;  // split > 1: [split][rest][min(M, rows of a tile)][TN] fp32
     uint32_t* status;
     // EPI_LINEAR, EPI_STORE, EPI_DZ: the output [M, N] bf16
     void* out;
@@ -58,17 +72,40 @@ struct GemmArgs {
     const float* g_h;
 };
 
-__device__ __forceinline__ float act_apply(float z, int act) {
-    if (act == ACT_RELU) return fmax_nan(z, 0.0f);
-    if (act == ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.707106781186547524f));
-    if (act == ACT_SILU) return __fdividef(z, 1.0f + ex2(-1.44269504088896341f * z));
+// 2 (1 - Phi(|z|)) = erfc(|z| / sqrt 2) by Abramowitz and Stegun's 7.1.26 (absolute error 1.5e-7, less than a
+// thousandth of a bf16 step of the results), and e^(-z^2 / 2), which the slope needs too.
+__device__ __forceinline__ float gelu_tail(float z, float* e) {
+    const float a = fabsf(z), t = __fdividef(1.0f, __fmaf_rn(0.231641888f, a, 1.0f));  // 0.3275911 / sqrt 2
+    *e = ex2(-0.72134752044448170f * a * a);
+    float p = 1.061405429f;
+    p = __fmaf_rn(p, t, -1.453152027f);
+    p = __fmaf_rn(p, t, 1.421413741f);
+    p = __fmaf_rn(p, t, -0.284496736f);
+    p = __fmaf_rn(p, t, 0.254829592f);
+    return p * t * *e;
+}
+template <int ACT>
+__device__ __forceinline__ float act_apply(float z) {
+    if (ACT == ACT_RELU) return fmax_nan(z, 0.0f);
+    if (ACT == ACT_GELU) {
+        float e;
+        const float q = 0.5f * gelu_tail(z, &e);
+        return z * (z > 0.0f ? 1.0f - q : q);
+    }
+    if (ACT == ACT_SILU) return __fdividef(z, 1.0f + ex2(-1.44269504088896341f * z));
     return z;
+}
+__device__ __forceinline__ float act_apply(float z, int act) {
+    return act == ACT_RELU ? act_apply<ACT_RELU>(z)
+                           : act == ACT_GELU ? act_apply<ACT_GELU>(z) : act == ACT_SILU ? act_apply<ACT_SILU>(z) : z;
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
     if (act == ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (act == ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.707106781186547524f)) +
-               0.398942280401432678f * z * ex2(-0.72134752044448170f * z * z);
+    if (act == ACT_GELU) {
+        float e;
+        const float q = 0.5f * gelu_tail(z, &e);
+        return __fmaf_rn(0.398942280401432678f * z, e, z > 0.0f ? 1.0f - q : q);
+    }
     if (act == ACT_SILU) {
         const float s = __fdividef(1.0f, 1.0f + ex2(-1.44269504088896341f * z));
         return s * (1.0f + z * (1.0f - s));
@@ -84,7 +121,7 @@ __device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t saddr) {
 }
 
 // 32 lanes x 32 columns of fp32 from tensor memory (this warp's lane quarter), waited for.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&f)[32]) {
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* f) {
     uint32_t v[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -100,8 +137,138 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&f)[32]) {
     for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
 }
 
+// Waits for the phase of `bar` with the given parity, for at most GM_WAIT clocks (false then).  The bound is kept with
+// the SM's own clock: a read of the global timer costs more than a k block's MMAs, and a wait per k block that took it
+// held the products to 740 clocks per k block whatever the tile's width.
+constexpr long long GM_WAIT = 500ll * 1000 * 1000;  // about a quarter of a second
+template <bool CLUSTER>
+__device__ __forceinline__ bool gm_try(uint64_t* bar, uint32_t parity) {
+    if constexpr (!CLUSTER) return mbar_try_wait(bar, parity);
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity) {
+    if (gm_try<CLUSTER>(bar, parity)) return true;
+    const long long t0 = clock64();
+    do {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (gm_try<CLUSTER>(bar, parity)) return true;
+    } while (clock64() - t0 < GM_WAIT);
+    return false;
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p)::"memory");
+    return p != 0;
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// The pair's forms (cta_group::2): tensor memory allocated in both CTAs by a warp of each, MMAs issued by the first CTA
+// over both CTAs' shared memory (the same offsets) into both CTAs' tensor memory, completion signalled to the same
+// mbarrier in both, and loads into this CTA's shared memory that complete on an mbarrier of the first CTA.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(cluster_bar)
+        : "memory");
+}
+
+// 16-byte chunk j of row r in a warp's staging block: conflict-free both for a lane per row and for 8 lanes per row.
+__device__ __forceinline__ uint4* stage_at(unsigned char* st, int r, int j) {
+    return reinterpret_cast<uint4*>(st + r * 128 + ((j ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ unsigned short* stage_elem(unsigned char* st, int r, int e) {
+    return reinterpret_cast<unsigned short*>(st + r * 128 + (((e >> 3) ^ (r & 7)) << 4)) + (e & 7);
+}
+// A warp's block of 32 rows x 64 bf16 from its staging block to rows `stride` elements apart; `vec`: 16-byte aligned rows.
+__device__ __forceinline__ void block_store(unsigned char* st, void* base, int64_t stride, int rows, int cols, bool vec) {
+    const int lane = threadIdx.x & 31;
+    unsigned short* p = static_cast<unsigned short*>(base);
+    if (vec && cols >= 64) {
+        const int c = lane & 7;
+#pragma unroll 4
+        for (int r = lane >> 3; r < rows; r += 4) *reinterpret_cast<uint4*>(p + r * stride + 8 * c) = *stage_at(st, r, c);
+    } else {
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+            if (lane < cols) p[r * stride + lane] = *stage_elem(st, r, lane);
+            if (lane + 32 < cols) p[r * stride + lane + 32] = *stage_elem(st, r, lane + 32);
+        }
+    }
+}
+// The same the other way: fetched into registers (so that the loads can be in flight meanwhile) and put, or, for rows
+// that are not aligned and the last columns, loaded at once.
+__device__ __forceinline__ void block_fetch(uint4 (&q)[8], const void* base, int64_t stride, int rows) {
+    const int lane = threadIdx.x & 31, c = lane & 7;
+    const unsigned short* p = static_cast<const unsigned short*>(base);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        if (r < rows) q[i] = __ldg(reinterpret_cast<const uint4*>(p + r * stride + 8 * c));
+    }
+}
+__device__ __forceinline__ void block_put(unsigned char* st, const uint4 (&q)[8]) {
+    const int lane = threadIdx.x & 31, c = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *stage_at(st, 4 * i + (lane >> 3), c) = q[i];
+}
+__device__ __forceinline__ void block_load(unsigned char* st, const void* base, int64_t stride, int rows, int cols) {
+    const int lane = threadIdx.x & 31;
+    const unsigned short* p = static_cast<const unsigned short*>(base);
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+        if (lane < cols) *stage_elem(st, r, lane) = __ldg(p + r * stride + lane);
+        if (lane + 32 < cols) *stage_elem(st, r, lane + 32) = __ldg(p + r * stride + lane + 32);
+    }
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Half `h` (32 columns) of this lane's row into the staging block, each value rounded once to bf16 (the output's type).
+__device__ __forceinline__ void stage_half(unsigned char* st, int h, const float (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        *stage_at(st, lane, 4 * h + j) =
+            make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
+                       pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
 }
 
 // Up to 8 bf16 of a row from column n (N columns), `vec`: the row is 16-byte aligned and n a multiple of 8.

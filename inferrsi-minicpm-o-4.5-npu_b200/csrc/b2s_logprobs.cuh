@@ -111,6 +111,31 @@ __device__ __forceinline__ void lp_add_many(LpState& s, const float (&x)[N], flo
     s.U += U;
 }
 
+// The same without the second form: every y bounded below, the reference that overflows chosen per call.  Short code for
+// the products' epilogue, whose arithmetic the MMAs hide.
+template <int N>
+__device__ __forceinline__ void lp_add_any(LpState& s, const float (&x)[N], float c) {
+    float bm = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) bm = fmax_nan(bm, x[j]);
+    const float m = fmax_nan(s.m, bm);
+    if (!(fabsf(m) <= 3.402823466e38f)) {
+        s.m = m;
+        return;
+    }
+    if (m > s.m) lp_rescale(s, m, c);
+    const float R = __fmul_rn(s.m, c);
+    const bool far = !(fabsf(R) <= 3.0e38f);
+    const float mul = c, off = far ? s.m : R, pre = far ? 1.0f : c, post = far ? mul : 1.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        // fma(x, c, -R), or (x - m) c
+        const float y = fmaxf(__fmul_rn(__fmaf_rn(x[j], pre, -off), post), -200.0f), e = ex2(y);
+        s.S += e;
+        s.U = __fmaf_rn(e, y, s.U);
+    }
+}
+
 __device__ __forceinline__ void lp_add(LpState& s, float x, float c) {
     const float v[1] = {x};
     lp_add_many<1>(s, v, c);

@@ -50,7 +50,7 @@ def operands(n, k, m, seed):
 
 SIZES = [(1, 8, 1), (1, 4096, 768), (2, 768, 768), (3, 72, 5), (16, 4096, 768), (17, 640, 333), (64, 768, 6562),
          (100, 200, 129), (128, 64, 256), (129, 1000, 257), (513, 768, 1537), (1000, 256, 4096), (2050, 80, 64),
-         (31, 8192, 40)]
+         (31, 8192, 40), (1300, 2048, 4096)]
 
 
 @pytest.mark.parametrize("activation", [None, "relu", "gelu", "silu"])
