@@ -346,17 +346,17 @@ __device__ __forceinline__ int block_excl_scan_i(int v, int* red, int* total) {
 }
 
 // Radix select: the key of the k-th largest (1-based, 1 <= k <= n) of n keys produced by key(i), over 4
-// rounds of 8-bit digits, most significant first.  hist: 256 shared words; ctl: 2 shared words.
-template <typename KeyFn>
+// rounds of 8-bit digits, most significant first.  hist: 256 shared words; ctl: 2 shared words; THREADS: the CTA's.
+template <int THREADS = NT, typename KeyFn>
 __device__ uint32_t block_kth_largest(int n, int k, KeyFn key, uint32_t* hist, uint32_t* ctl) {
     uint32_t prefix = 0, mask = 0;
     int krem = k;
     const int tid = threadIdx.x;
     for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += NT) hist[i] = 0;
+        for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
         __syncthreads();
         // whole warps iterate together so equal digits can be aggregated (one atomic per distinct digit)
-        for (int base = 0; base < n; base += NT) {
+        for (int base = 0; base < n; base += THREADS) {
             const int i = base + tid;
             uint32_t d = 256u;
             if (i < n) {

@@ -52,19 +52,30 @@ __device__ __forceinline__ bool piece_at(const GemmArgs& a, int i, Piece* p) {
     return true;
 }
 
-// The epilogue of one warp's 32 rows of a tile: columns [n0, n0 + TN) from tensor memory at `tm` (lane = row).
+// Whether a block of 32 columns from n is copied as 16-byte vectors.
+__device__ __forceinline__ bool vec_block(const GemmArgs& a, int n, int aligned) { return aligned && n + 32 <= a.N; }
+// The residual's block of 32 columns from n of the 32 rows from row0.
+__device__ __forceinline__ void residual_fetch(const GemmArgs& a, uint32_t (&q)[16], int row0, int n) {
+    if (a.residual && n < a.N)
+        block_fetch(q, static_cast<const unsigned short*>(a.residual) + (int64_t)row0 * a.res_stride + n, a.res_stride,
+                    a.M - row0, a.N - n, vec_block(a, n, a.res_vec));
+}
+
+// The epilogue of one warp: 32 rows of a tile, columns [n0, n0 + COLS) from tensor memory at `tm` (lane = row).  `rq`:
+// the residual's first block.
 template <int TM, int TN, int EPI>
-__device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, int row0, int n0, int nt, int slot,
-                                              unsigned char* st) {
+__device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, int row0, int n0, int half, int nt, int slot,
+                                              unsigned char* st, uint32_t (&rq)[16]) {
+    constexpr int COLS = TN / 2;
     const int lane = threadIdx.x & 31, row = row0 + lane;
     const bool live = row < a.M;
     const int rows = min(32, a.M - row0);  // <= 0: a warp past the last row
-    if constexpr (EPI != EPI_LSE) {
-        if (slot >= 0) {  // part of a split tile: its fp32 sums as they are
+    if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
+        if (slot >= 0) {  // a chunk of a split tile: its fp32 sums as they are
             const int held = min(a.M, TM);
-            float* dst = a.partial + (int64_t)slot * held * TN + (int64_t)(row0 % TM) * TN;
+            float* dst = a.partial + ((int64_t)slot * held + row0 % TM) * TN + n0 - nt * TN;
 #pragma unroll 1
-            for (int q = 0; q < TN / 32; ++q) {
+            for (int q = 0; q < COLS / 32; ++q) {
                 float v[32];
                 tmem_ld32(tm + 32u * q, v);
 #pragma unroll
@@ -81,74 +92,57 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
             }
             return;
         }
-    }
-    if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
         unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride;
-        const unsigned short* res = static_cast<const unsigned short*>(a.residual) + (int64_t)row0 * a.res_stride;
         const bool with_res = EPI == EPI_LINEAR && a.residual;
-        uint4 rq[8];
-        auto fetch = [&](int n) {  // the next block's residual, in flight meanwhile
-            if (with_res && a.res_vec && n + 64 <= a.N) block_fetch(rq, res + n, a.res_stride, rows);
-        };
-        fetch(n0);
 #pragma unroll 1
-        for (int q = 0; q < TN / 64; ++q) {
-            const int n = n0 + 64 * q, cols = a.N - n;
+        for (int q = 0; q < COLS / 32; ++q) {
+            const int n = n0 + 32 * q, cols = a.N - n;
             if (cols <= 0) break;
             if (with_res) {
-                if (a.res_vec && cols >= 64) {
-                    block_put(st, rq);
-                    if (q + 1 < TN / 64) fetch(n + 64);
-                } else {
-                    block_load(st, res + n, a.res_stride, rows, cols);
-                }
+                block_put(st, rq, vec_block(a, n, a.res_vec));
+                if (q + 1 < COLS / 32) residual_fetch(a, rq, row0, n + 32);  // in flight under this block
                 __syncwarp();
             }
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                float v[32];
-                tmem_ld32(tm + 64u * q + 32u * h, v);
-                if constexpr (EPI == EPI_LINEAR) {
-                    if (a.bias) {
-                        const int nb = n + 32 * h + lane;
-                        const float b = nb < a.N ? bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + nb)) : 0.0f;
+            float v[32];
+            tmem_ld32(tm + 32u * q, v);
+            if constexpr (EPI == EPI_LINEAR) {
+                if (a.bias) {
+                    const float b = lane < cols ? bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + n + lane)) : 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
-                    }
-                    // the saved pre-activation is bf16, like the tensors around it: the slope taken from it is off by
-                    // half a bf16 step of z times the activation's curvature, less than dz's own rounding to the
-                    // tensor cores' bf16
-                    if (a.preact) stage_half(st + 4096, h, v);
-                    if (a.act == ACT_RELU) {
+                    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
+                }
+                // the saved pre-activation is bf16, like the tensors around it: the slope taken from it is off by half a
+                // bf16 step of z times the activation's curvature, less than dz's own rounding to the tensor cores' bf16
+                if (a.preact) stage_row(st, 4, v);
+                if (a.act == ACT_RELU) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_RELU>(v[j]);
-                    } else if (a.act == ACT_GELU) {
+                    for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_RELU>(v[j]);
+                } else if (a.act == ACT_GELU) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_GELU>(v[j]);
-                    } else if (a.act == ACT_SILU) {
+                    for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_GELU>(v[j]);
+                } else if (a.act == ACT_SILU) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_SILU>(v[j]);
-                    }
-                    if (with_res) {
+                    for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_SILU>(v[j]);
+                }
+                if (with_res) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint4 u = *stage_at(st, lane, 4 * h + j);
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 u = *stage_at(st, lane, j);
+                        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                v[8 * j + 2 * k] += __uint_as_float(w[k] << 16);
-                                v[8 * j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
-                            }
+                        for (int k = 0; k < 4; ++k) {
+                            v[8 * j + 2 * k] += __uint_as_float(w[k] << 16);
+                            v[8 * j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
                         }
                     }
                 }
-                stage_half(st, h, v);  // this lane's own row: nobody else reads it before the barrier
             }
+            stage_row(st, 0, v);  // over this lane's own row of the residual
             __syncwarp();
-            block_store(st, out + n, a.out_stride, rows, cols, a.out_vec);
+            block_store(st, 0, out + n, a.out_stride, rows, cols, vec_block(a, n, a.out_vec));
             if (EPI == EPI_LINEAR && a.preact)
-                block_store(st + 4096, static_cast<unsigned short*>(a.preact) + (int64_t)row0 * a.pre_stride + n,
-                            a.pre_stride, rows, cols, true);
+                block_store(st, 4, static_cast<unsigned short*>(a.preact) + (int64_t)row0 * a.pre_stride + n, a.pre_stride,
+                            rows, cols, vec_block(a, n, 1));
             __syncwarp();
         }
     } else if constexpr (EPI == EPI_LSE) {
@@ -157,7 +151,7 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
         s.m = f_ninf();
         s.S = s.U = 0.0f;
 #pragma unroll 1
-        for (int q = 0; q < TN / 32; ++q) {
+        for (int q = 0; q < COLS / 32; ++q) {
             const int n = n0 + 32 * q;
             if (n >= a.N) break;
             float v[32];
@@ -174,7 +168,7 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
             }
             lp_add_any<32>(s, v, a.c);
         }
-        if (live) a.part[(int64_t)row * a.tiles_n + nt] = make_float4(s.m, s.S, s.U, 0.0f);
+        if (live) a.part[((int64_t)row * a.tiles_n + nt) * 2 + half] = make_float4(s.m, s.S, s.U, 0.0f);
     } else {
         const int64_t tok = live ? a.tokens[row] : -1;
         const float4 stt = live ? a.stats[row] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -182,20 +176,17 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
                        live && a.g_h ? a.g_h[row] : 0.0f, a.inv_t);
         unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride;
 #pragma unroll 1
-        for (int q = 0; q < TN / 64; ++q) {
-            const int n = n0 + 64 * q, cols = a.N - n;
+        for (int q = 0; q < COLS / 32; ++q) {
+            const int n = n0 + 32 * q, cols = a.N - n;
             if (cols <= 0) break;
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                float v[32];
-                tmem_ld32(tm + 64u * q + 32u * h, v);
+            float v[32];
+            tmem_ld32(tm + 32u * q, v);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = g.at(v[j], n + 32 * h + j, a.c);
-                // dz is rounded to bf16 once: it is the tensor cores' operand in both gradient products
-                stage_half(st, h, v);
-            }
+            for (int j = 0; j < 32; ++j) v[j] = g.at(v[j], n + j, a.c);
+            // dz is rounded to bf16 once: it is the tensor cores' operand in both gradient products
+            stage_row(st, 0, v);
             __syncwarp();
-            block_store(st, out + n, a.out_stride, rows, cols, true);
+            block_store(st, 0, out + n, a.out_stride, rows, cols, vec_block(a, n, 1));
             __syncwarp();
         }
     }
@@ -235,7 +226,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], 128 * CG);
+            mbar_init(&tempty[s], 32 * GM_EPI * CG);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -243,7 +234,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         *issued = 0;
         *consumed = 0;
     }
-    if (warp == 5) {
+    if (warp == GM_EPI + 1) {
         if constexpr (CG == 2) tmem_alloc_pair(tslot, 2 * TN);
         else tmem_alloc(tslot, 2 * TN);
     }
@@ -259,7 +250,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
 
     // The loading and the issuing warp run their loops converged, one lane elected where something is issued: with the
     // loops inside a one-lane branch a k block cost the issuing thread 580 clocks, more than its MMAs' 512.
-    if (warp == 4) {
+    if (warp == GM_EPI) {
         int s = 0, it = 0;
         uint32_t ph = 1;  // parity of `empty`'s last phase: the first round finds every stage free
         bool ok = true;
@@ -312,7 +303,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                     *fail = 1;
                     break;
                 }
-    } else if (warp == 5) {
+    } else if (warp == GM_EPI + 1) {
         if (rank == 0) {  // MMAs
             int s = 0, it = 0;
             uint32_t ph = 0;
@@ -374,16 +365,18 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         for (int i = 0; piece_at<CG>(a, i, &p); ++i) {
             int mt, nt;
             tile_of<TM>(a, p.tile, &mt, &nt);
-            const int acc = i & 1;
+            const int acc = i & 1, half = warp >> 2;
+            const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32, n0 = nt * TN + half * (TN / 2);
+            uint32_t rq[16];
+            if (EPI == EPI_LINEAR && p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
             const bool ok = gm_wait<false>(&tfull[acc], (uint32_t)(i / 2) & 1u);
             if (!__all_sync(0xffffffffu, ok) || *fail) {
                 *fail = 1;
                 break;
             }
             tc_fence_after();
-            epilogue_rows<TM, TN, EPI>(a, tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(acc * TN),
-                                       mt * TM + (int)rank * GM_M + warp * 32, nt * TN, nt, p.slot,
-                                       staging + warp * 8192);
+            epilogue_rows<TM, TN, EPI>(a, tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(acc * TN + half * (TN / 2)),
+                                       row0, n0, half, nt, p.slot, staging + warp * 4096, rq);
             tc_fence_before();
             if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
             else mbar_arrive(&tempty[acc]);
@@ -408,7 +401,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         cluster_arrive_release();
         cluster_wait();
     }
-    if (warp == 5) {
+    if (warp == GM_EPI + 1) {
         tc_fence_after();
         if constexpr (CG == 2) tmem_dealloc_pair(tmem, 2 * TN);
         else tmem_dealloc(tmem, 2 * TN);
@@ -731,7 +724,7 @@ int b2s_lmhead_logprobs_workspace(int32_t rows, int32_t vocab, int32_t hidden_di
     using namespace b2s;
     if (rows < 0 || vocab < 1 || hidden_dim < 8 || !bytes) return B2S_ERR_INVALID;
     const int tn = plan_here(rows > 0 ? rows : 1, vocab, hidden_dim, false).tn;
-    *bytes = up((int64_t)rows * ((vocab + tn - 1) / tn) * 16 + (int64_t)rows * 4, 256);
+    *bytes = up((int64_t)rows * ((vocab + tn - 1) / tn) * 32 + (int64_t)rows * 4, 256);
     return B2S_OK;
 }
 
@@ -747,7 +740,7 @@ int b2s_lmhead_logprobs(const b2s_lmhead_args* h, float* logprob, float* entropy
     if (!h->tokens || !h->workspace || h->workspace_bytes < need || !aligned16(h->workspace) || (stats && !aligned16(stats)))
         return B2S_ERR_INVALID;
     const int tn = plan_here(h->rows, h->vocab, h->hidden_dim, false).tn;
-    const int tiles = (h->vocab + tn - 1) / tn;
+    const int tiles = 2 * ((h->vocab + tn - 1) / tn);  // states per row: two halves of each column tile
     GemmArgs a;
     memset(&a, 0, sizeof(a));
     a.M = h->rows;

@@ -8,7 +8,7 @@
 // order that keeps a group of row tiles together (so that a wave's operands stay in L2).  What bounds a large product is
 // the way from L2 to the SMs, about 64 bytes a clock each: a 128 x 256 tile of one CTA asks for 96 while its MMAs run
 // (48 KB per 512 clocks), so it keeps the tensor pipe 60 % busy; a pair holds 128 rows of A each and half of B's
-// columns, and asks for 64.  Warp 4 fills a ring of stages by TMA, warp 5 issues the MMAs and the other four warps run the
+// columns, and asks for 64.  Warp 8 fills a ring of stages by TMA, warp 9 issues the MMAs and eight warps run the
 // epilogue of one tile on one half of tensor memory while the MMAs of the next fill the other half.  Tiles that do not
 // fill a wave are split along k into equal chunks, all tiles' first chunks first (CTAs at work at the same time then
 // read the same k range of both operands, once from HBM); a chunk's fp32 sums go to a workspace, and a second kernel
@@ -26,13 +26,14 @@ namespace b2s {
 
 constexpr int GM_M = 128;        // rows of a tile: the MMA's M, one accumulator lane each
 constexpr int GM_KB = 64;        // k per stage: one 128-byte row of the swizzle
-constexpr int GM_THREADS = 192;  // warps 0-3: epilogue (their tensor-memory quarter), 4: loads, 5: MMAs
+constexpr int GM_EPI = 8;        // epilogue warps: warp w has tensor-memory quarter w % 4 and half w / 4 of the columns
+constexpr int GM_THREADS = 32 * GM_EPI + 64;
 constexpr int GM_GROUP = 16;     // row tiles taken together
 constexpr uint32_t GM_A_BYTES = GM_M * GM_KB * 2;
 
 // A stage of one CTA: its 128 rows of A and its 1 / CG of the TN columns of B.
 __host__ __device__ constexpr uint32_t gm_stage_bytes(int cg, int tn) { return GM_A_BYTES + (uint32_t)(tn / cg) * GM_KB * 2; }
-constexpr uint32_t GM_STAGING = 4 * 8192;  // two blocks of 32 rows x 128 bytes per epilogue warp
+constexpr uint32_t GM_STAGING = GM_EPI * 4096;  // per epilogue warp: 32 rows x (64 bytes of output, 64 of pre-activation)
 // as many stages as fit 192 KB, at most 8
 __host__ __device__ constexpr int gm_stages(int cg, int tn) {
     return (int)(192u * 1024u / gm_stage_bytes(cg, tn)) > 8 ? 8 : (int)(192u * 1024u / gm_stage_bytes(cg, tn));
@@ -62,7 +63,7 @@ struct GemmArgs {
     int act;
     void* preact;
     int64_t pre_stride;
-    // EPI_LSE: per row and column tile (m, S, U), the token's value; EPI_DZ: the gradient's inputs
+    // EPI_LSE: per row and half of a column tile (m, S, U), the token's value; EPI_DZ: the gradient's inputs
     float c, inv_t;
     const int64_t* tokens;
     float4* part;
@@ -209,64 +210,105 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
         : "memory");
 }
 
-// 16-byte chunk j of row r in a warp's staging block: conflict-free both for a lane per row and for 8 lanes per row.
+// 16-byte chunk j of row r in a warp's staging block (chunks 0-3: the output or the residual, 4-7: the pre-activation):
+// conflict-free for a lane per row, and for the copies below, whose 8 lanes of a phase hold rows r and r + 4.
 __device__ __forceinline__ uint4* stage_at(unsigned char* st, int r, int j) {
     return reinterpret_cast<uint4*>(st + r * 128 + ((j ^ (r & 7)) << 4));
 }
-__device__ __forceinline__ unsigned short* stage_elem(unsigned char* st, int r, int e) {
-    return reinterpret_cast<unsigned short*>(st + r * 128 + (((e >> 3) ^ (r & 7)) << 4)) + (e & 7);
+// The 4-byte word of columns 2 w, 2 w + 1 of row r, from chunk `base`.
+__device__ __forceinline__ uint32_t* stage_word(unsigned char* st, int r, int base, int w) {
+    return reinterpret_cast<uint32_t*>(st + r * 128 + (((base + (w >> 2)) ^ (r & 7)) << 4)) + (w & 3);
 }
-// A warp's block of 32 rows x 64 bf16 from its staging block to rows `stride` elements apart; `vec`: 16-byte aligned rows.
-__device__ __forceinline__ void block_store(unsigned char* st, void* base, int64_t stride, int rows, int cols, bool vec) {
+// Copies between a staging block and 32 rows x 32 bf16 of global memory, rows `stride` elements apart.  `vec` (16-byte
+// aligned rows, all 32 columns there): 4 lanes per row, 8 rows at a time; else 16 lanes per row, 2 columns each.
+__device__ __forceinline__ int vec_row(int i) {
+    const int rr = (threadIdx.x & 31) >> 2;
+    return 8 * i + (rr & 1) * 4 + (rr >> 1);
+}
+__device__ __forceinline__ void block_store(unsigned char* st, int base, void* out, int64_t stride, int rows, int cols,
+                                            bool vec) {
     const int lane = threadIdx.x & 31;
-    unsigned short* p = static_cast<unsigned short*>(base);
-    if (vec && cols >= 64) {
-        const int c = lane & 7;
-#pragma unroll 4
-        for (int r = lane >> 3; r < rows; r += 4) *reinterpret_cast<uint4*>(p + r * stride + 8 * c) = *stage_at(st, r, c);
+    unsigned short* p = static_cast<unsigned short*>(out);
+    if (vec) {
+        const int c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = vec_row(i);
+            if (r < rows) *reinterpret_cast<uint4*>(p + r * stride + 8 * c) = *stage_at(st, r, base + c);
+        }
     } else {
+        // whole 4-byte words where the row starts on one, else words one column on, the ends by themselves; the two rows of
+        // a step have the same parity, so a warp takes one of the two ways
+        const int w = lane & 15, left = cols - 2 * w;
 #pragma unroll 4
-        for (int r = 0; r < rows; ++r) {
-            if (lane < cols) p[r * stride + lane] = *stage_elem(st, r, lane);
-            if (lane + 32 < cols) p[r * stride + lane + 32] = *stage_elem(st, r, lane + 32);
+        for (int i = 0; i < 16; ++i) {
+            const int r = 4 * (i >> 1) + (i & 1) + 2 * (lane >> 4);
+            const uint32_t v = *stage_word(st, r, base, w);
+            const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1, 16);
+            unsigned short* q = p + r * stride + 2 * w;
+            if (r < rows) {
+                if ((reinterpret_cast<uintptr_t>(q) & 2) == 0) {
+                    if (left >= 2) *reinterpret_cast<uint32_t*>(q) = v;
+                    else if (left == 1) q[0] = (unsigned short)v;
+                } else {
+                    if (w == 0) q[0] = (unsigned short)v;  // a block has a first column
+                    if (w < 15 && left >= 3) *reinterpret_cast<uint32_t*>(q + 1) = v >> 16 | next << 16;
+                    else if (left >= 2) q[1] = (unsigned short)(v >> 16);
+                }
+            }
         }
     }
 }
-// The same the other way: fetched into registers (so that the loads can be in flight meanwhile) and put, or, for rows
-// that are not aligned and the last columns, loaded at once.
-__device__ __forceinline__ void block_fetch(uint4 (&q)[8], const void* base, int64_t stride, int rows) {
-    const int lane = threadIdx.x & 31, c = lane & 7;
-    const unsigned short* p = static_cast<const unsigned short*>(base);
+// A block of the residual into registers, in flight until it is put into the staging block.
+__device__ __forceinline__ void block_fetch(uint32_t (&q)[16], const void* in, int64_t stride, int rows, int cols, bool vec) {
+    const int lane = threadIdx.x & 31;
+    const unsigned short* p = static_cast<const unsigned short*>(in);
+    if (vec) {
+        const int c = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        if (r < rows) q[i] = __ldg(reinterpret_cast<const uint4*>(p + r * stride + 8 * c));
+        for (int i = 0; i < 4; ++i) {
+            const int r = vec_row(i);
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (r < rows) u = __ldg(reinterpret_cast<const uint4*>(p + r * stride + 8 * c));
+            q[4 * i] = u.x;
+            q[4 * i + 1] = u.y;
+            q[4 * i + 2] = u.z;
+            q[4 * i + 3] = u.w;
+        }
+    } else {
+        const int w = lane & 15, left = cols - 2 * w;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = 2 * i + (lane >> 4);
+            const unsigned short* g = p + r * stride + 2 * w;
+            uint32_t lo = 0, hi = 0;
+            if (r < rows && left >= 1) lo = __ldg(g);
+            if (r < rows && left >= 2) hi = __ldg(g + 1);
+            q[i] = lo | hi << 16;
+        }
     }
 }
-__device__ __forceinline__ void block_put(unsigned char* st, const uint4 (&q)[8]) {
-    const int lane = threadIdx.x & 31, c = lane & 7;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) *stage_at(st, 4 * i + (lane >> 3), c) = q[i];
-}
-__device__ __forceinline__ void block_load(unsigned char* st, const void* base, int64_t stride, int rows, int cols) {
+__device__ __forceinline__ void block_put(unsigned char* st, const uint32_t (&q)[16], bool vec) {
     const int lane = threadIdx.x & 31;
-    const unsigned short* p = static_cast<const unsigned short*>(base);
-#pragma unroll 8
-    for (int r = 0; r < rows; ++r) {
-        if (lane < cols) *stage_elem(st, r, lane) = __ldg(p + r * stride + lane);
-        if (lane + 32 < cols) *stage_elem(st, r, lane + 32) = __ldg(p + r * stride + lane + 32);
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *stage_at(st, vec_row(i), lane & 3) = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) *stage_word(st, 2 * i + (lane >> 4), 0, lane & 15) = q[i];
     }
 }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Half `h` (32 columns) of this lane's row into the staging block, each value rounded once to bf16 (the output's type).
-__device__ __forceinline__ void stage_half(unsigned char* st, int h, const float (&v)[32]) {
+// This lane's row of 32 values into chunks `base` .. base + 3, each rounded once to bf16 (the output's type).
+__device__ __forceinline__ void stage_row(unsigned char* st, int base, const float (&v)[32]) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        *stage_at(st, lane, 4 * h + j) =
+        *stage_at(st, lane, base + j) =
             make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
                        pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
 }

@@ -10,13 +10,17 @@
 // y = (x - m) c instead.  A masked (-inf) element adds nothing; a row with nothing left has logprob -inf, entropy 0
 // and gradient 0; NaN or +inf anywhere makes the row NaN, as a softmax gives it.
 //
-// Forward, one pass over the row: a cluster of CTAs per row (several while rows are few), each thread streaming
-// 16-byte vectors.  The rank counts the elements before the token in (value descending, id ascending) order:
-// an element before the token counts when x >= x_t, i.e. x > pred(x_t), one after it when x > x_t, so a vector needs
-// one threshold.  Top alternatives: pass 1 leaves each thread's maximum; the top-th largest of the warps' largest
-// maxima bounds the CTA's top-th value from below; only the shares of threads that reach it are read again (from L2),
-// their elements above the bound listed and ordered by rank counting.  Lists that overflow (more ties than the list
-// holds) take an exact radix select over the CTA's part of the row.
+// Forward, one pass over the row by bulk copies into a ring of shared-memory chunks (a thread's registers do not bound
+// the bytes in flight), 128 threads per row where rows are many and short, else 512 and a cluster of CTAs per row while
+// rows are few.  Two elements share one packed fp32 operation, and a bf16 pair one maximum and one comparison: about 6
+// instructions an element, so that bf16 rows stay bound by HBM.  The rank counts the elements before the token in (value
+// descending, id ascending) order: an element before the token counts when x >= x_t, i.e. x > pred(x_t), one after it
+// when x > x_t, so a vector needs one threshold.  Top alternatives: pass 1 leaves each thread's maximum; the top-th
+// largest of the warps' largest maxima bounds the CTA's top-th value from below; only the shares of threads that reach
+// it are read again (from shared memory where the part fits, else from L2), their elements above the bound listed and
+// ordered by rank counting.  Where too few threads hold anything (short or masked rows) every finite element is listed
+// and the first masked ids fill what is missing.  Lists that overflow (more ties than the list holds) take an exact
+// radix select over the CTA's part of the row.
 //
 // Backward, elementwise: dx = (g_lp ([i = t] - p) - g_H p (log p + H)) / T with p = 2^(y - log2 S) recomputed from
 // the saved reference: one read and one write of the row.
@@ -50,15 +54,42 @@ cudaError_t device_sms(int* sms) {
 namespace {
 
 constexpr int LP_CAP = 512;      // candidate list entries per CTA
-constexpr int LP_GATHER = 4;     // thread maxima gathered per warp (16 warps x 4 = 64 >= the largest top)
+constexpr int LP_GATHER = 64;    // thread maxima gathered per CTA, at most
 constexpr int LP_MAX_TOP = 32;
-constexpr int LP_U = 4;          // vectors per thread and batch
+constexpr int LP_U = 4;          // vectors per thread and chunk
+constexpr uint64_t LP_WAIT_NS = 250ull * 1000 * 1000;
+
+// The largest float below x (x not NaN); NaN for -inf, whose "x > pred" must hold for every element.
+__device__ __forceinline__ float pred_float(float x) {
+    if (x == f_ninf()) return __int_as_float(0x7fffffff);
+    if (x == 0.0f) return __int_as_float((int)0x80000001u);
+    const int b = __float_as_int(x);
+    return __int_as_float(x > 0.0f ? b - 1 : b + 1);
+}
 
 template <typename E>
 struct LpElem;
 template <>
 struct LpElem<float> {
     static constexpr int EPV = 4;
+    typedef float Thr;
+    static __device__ __forceinline__ Thr threshold(float xt) { return xt; }
+    static __device__ __forceinline__ Thr threshold_before(float xt) { return pred_float(xt); }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+    static __device__ __forceinline__ float batch_max(const uint4 (&q)[LP_U]) {
+        float m = __uint_as_float(q[0].x);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            m = fmax_nan(m, fmax_nan(__uint_as_float(q[u].x), __uint_as_float(q[u].y)));
+            m = fmax_nan(m, fmax_nan(__uint_as_float(q[u].z), __uint_as_float(q[u].w)));
+        }
+        return m;
+    }
+    // elements above the threshold, or NaN
+    static __device__ __forceinline__ int count_above(uint4 q, Thr t) {
+        return !(__uint_as_float(q.x) <= t) + !(__uint_as_float(q.y) <= t) + !(__uint_as_float(q.z) <= t) +
+               !(__uint_as_float(q.w) <= t);
+    }
     static __device__ __forceinline__ float ld(const void* p, int64_t i) { return __ldg(static_cast<const float*>(p) + i); }
     static __device__ __forceinline__ void unpack(uint4 q, float (&x)[4]) {
         x[0] = __uint_as_float(q.x); x[1] = __uint_as_float(q.y); x[2] = __uint_as_float(q.z); x[3] = __uint_as_float(q.w);
@@ -71,6 +102,35 @@ struct LpElem<float> {
 template <>
 struct LpElem<__nv_bfloat16> {
     static constexpr int EPV = 8;
+    typedef __nv_bfloat162 Thr;
+    static __device__ __forceinline__ __nv_bfloat162 as2(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ Thr both(uint32_t bits) { return as2(bits | bits << 16); }
+    static __device__ __forceinline__ Thr threshold(float xt) { return both(__float_as_uint(xt) >> 16); }
+    // the largest bf16 below xt; NaN for -inf
+    static __device__ __forceinline__ Thr threshold_before(float xt) {
+        const uint32_t b = __float_as_uint(xt) >> 16;
+        if (xt == f_ninf()) return both(0x7fffu);
+        if (xt == 0.0f) return both(0x8001u);
+        return both(xt > 0.0f ? b - 1u : b + 1u);
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+    static __device__ __forceinline__ float batch_max(const uint4 (&q)[LP_U]) {
+        __nv_bfloat162 m = as2(q[0].x);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            m = __hmax2_nan(m, __hmax2_nan(as2(q[u].x), as2(q[u].y)));
+            m = __hmax2_nan(m, __hmax2_nan(as2(q[u].z), as2(q[u].w)));
+        }
+        return fmax_nan(__low2float(m), __high2float(m));
+    }
+    // elements above the threshold, or NaN: a true comparison is a 0xffff half, whose low byte is -1
+    static __device__ __forceinline__ int count_above(uint4 q, Thr t) {
+        int n = __dp4a((int)__hgtu2_mask(as2(q.x), t), 0x00010001, 0);
+        n = __dp4a((int)__hgtu2_mask(as2(q.y), t), 0x00010001, n);
+        n = __dp4a((int)__hgtu2_mask(as2(q.z), t), 0x00010001, n);
+        n = __dp4a((int)__hgtu2_mask(as2(q.w), t), 0x00010001, n);
+        return -n;
+    }
     static __device__ __forceinline__ float ld(const void* p, int64_t i) {
         return bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(p) + i));
     }
@@ -105,21 +165,16 @@ __device__ __forceinline__ unsigned long long rank_word(float x, int id) {
 }
 __device__ __forceinline__ int word_id(unsigned long long w) { return (int)(0xffffffffu - (uint32_t)w); }
 
-// The largest float below x (x not NaN); NaN for -inf, whose "x > pred" must hold for every element.
-__device__ __forceinline__ float pred_float(float x) {
-    if (x == f_ninf()) return __int_as_float(0x7fffffff);
-    if (x == 0.0f) return __int_as_float((int)0x80000001u);
-    const int b = __float_as_int(x);
-    return __int_as_float(x > 0.0f ? b - 1 : b + 1);
-}
-
+template <int NTH>
 struct LpShared {
-    LpState warp[NWARP];
-    int count[NWARP];
-    int has_nan[NWARP];
-    uint32_t gather[NWARP * LP_GATHER];
-    int n_list;
-    int red[NWARP + 1];
+    static constexpr int WARPS = NTH / 32;
+    uint64_t full[16], empty[16];
+    float wmax[WARPS];
+    float wS[WARPS], wU[WARPS];
+    int wcount[WARPS];
+    uint32_t gather[LP_GATHER];
+    int n_list, failed;
+    int ties[WARPS];
     uint32_t hist[256];
     uint32_t ctl[2];
     unsigned long long list[LP_CAP];
@@ -131,7 +186,7 @@ struct LpShared {
 struct LpArgs {
     const void* logits;
     int64_t stride;
-    int V, per, top;
+    int V, per, top, stages;
     float c;
     const int64_t* tokens;
     float *logprob, *entropy;
@@ -141,31 +196,107 @@ struct LpArgs {
     uint32_t* status;
 };
 
+// A thread's running statistics: two lanes of S and U that packed operations add to.
+struct LpThread {
+    float m;
+    float2 S, U;
+};
+__device__ __forceinline__ void lp_thread_rescale(LpThread& s, float m, float c) {
+    if (s.m != f_ninf()) {
+        const float d = lp_shift(s.m, m, c), f = ex2(d);
+        s.U = make_float2(f * __fmaf_rn(d, s.S.x, s.U.x), f * __fmaf_rn(d, s.S.y, s.U.y));
+        s.S = make_float2(f * s.S.x, f * s.S.y);
+    }
+    s.m = m;
+}
+// One value, by the thread's first lane, whatever the reference.
+__device__ __forceinline__ void lp_thread_add(LpThread& s, float x, float c) {
+    const float m = fmax_nan(s.m, x);
+    if (!(fabsf(m) <= 3.402823466e38f)) {
+        s.m = m;
+        return;
+    }
+    if (m > s.m) lp_thread_rescale(s, m, c);
+    const float y = lp_y(x, s.m, c), e = ex2(y);
+    s.S.x += e;
+    s.U.x = __fmaf_rn(e, y, s.U.x);
+}
+// LP_U vectors whose maximum is bm: the maximum moved, then packed sums.
+template <typename E>
+__device__ __forceinline__ void lp_thread_batch(LpThread& s, const uint4 (&q)[LP_U], float bm, float c) {
+    if (!(bm <= s.m)) {  // larger, or NaN
+        const float m = fmax_nan(s.m, bm);
+        if (fabsf(m) <= 3.402823466e38f) lp_thread_rescale(s, m, c);
+        else s.m = m;
+    }
+    if (!(fabsf(s.m) <= 3.402823466e38f)) return;  // NaN or +inf (the row's outcome), or nothing but -inf so far
+    const float R = __fmul_rn(s.m, c);
+    if (fabsf(R) <= 3.0e38f) {
+        const float2 c2 = make_float2(c, c), r2 = make_float2(-R, -R);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            float x[LpElem<E>::EPV];
+            LpElem<E>::unpack(q[u], x);
+#pragma unroll
+            for (int j = 0; j < LpElem<E>::EPV; j += 2) {
+                float2 y = __ffma2_rn(make_float2(x[j], x[j + 1]), c2, r2);
+                y = make_float2(fmaxf(y.x, -200.0f), fmaxf(y.y, -200.0f));  // a masked element: 0 * -200
+                const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                s.S = __fadd2_rn(s.S, e);
+                s.U = __ffma2_rn(e, y, s.U);
+            }
+        }
+    } else {  // a reference that overflows: (x - m) c
+        const float2 c2 = make_float2(c, c), m2 = make_float2(-s.m, -s.m);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            float x[LpElem<E>::EPV];
+            LpElem<E>::unpack(q[u], x);
+#pragma unroll
+            for (int j = 0; j < LpElem<E>::EPV; j += 2) {
+                float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m2), c2);
+                y = make_float2(fmaxf(y.x, -200.0f), fmaxf(y.y, -200.0f));
+                const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                s.S = __fadd2_rn(s.S, e);
+                s.U = __ffma2_rn(e, y, s.U);
+            }
+        }
+    }
+}
+
 // The top `need` words of elements [0, n) of this CTA's part of the row (element i has id lo + i), exactly, whatever
 // the ties: the need-th largest value by radix select, then everything above it and the first ties in id order.
 // Every thread calls it; sh.list holds min(need, n) words afterwards.
-template <typename E>
-__device__ __noinline__ void exact_top(LpShared& sh, const void* rowp, int lo, int n, int need) {
-    const int tid = threadIdx.x;
+template <typename E, int NTH>
+__device__ __noinline__ void exact_top(LpShared<NTH>& sh, const void* rowp, int lo, int n, int need) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     need = min(need, n);
     auto key = [&](int i) { return rank_key(LpElem<E>::ld(rowp, lo + i)); };
     __syncthreads();
-    const uint32_t kth = block_kth_largest(n, need, key, sh.hist, sh.ctl);
+    const uint32_t kth = block_kth_largest<NTH>(n, need, key, sh.hist, sh.ctl);
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += NT) {
+    for (int i = tid; i < n; i += NTH) {
         const float x = LpElem<E>::ld(rowp, lo + i);
         if (rank_key(x) > kth) sh.list[atomicAdd(&sh.n_list, 1)] = rank_word(x, lo + i);  // fewer than need <= LP_CAP
     }
     __syncthreads();
     int have = sh.n_list;
-    for (int b = 0; b < n && have < need; b += NT) {
+    for (int b = 0; b < n && have < need; b += NTH) {
         const int i = b + tid;
         const float x = i < n ? LpElem<E>::ld(rowp, lo + i) : 0.0f;
-        const int tie = i < n && rank_key(x) == kth;
-        int total;
-        const int before = block_excl_scan_i(tie, sh.red, &total);
-        if (tie && have + before < need) sh.list[have + before] = rank_word(x, lo + i);
+        const bool tie = i < n && rank_key(x) == kth;
+        const uint32_t who = __ballot_sync(0xffffffffu, tie);
+        if (lane == 0) sh.ties[warp] = __popc(who);
+        __syncthreads();
+        int at = have, total = 0;
+#pragma unroll
+        for (int w = 0; w < NTH / 32; ++w) {
+            at += w < warp ? sh.ties[w] : 0;
+            total += sh.ties[w];
+        }
+        at += __popc(who & ((1u << lane) - 1u));
+        if (tie && at < need) sh.list[at] = rank_word(x, lo + i);
         have += total;
         __syncthreads();
     }
@@ -174,23 +305,99 @@ __device__ __noinline__ void exact_top(LpShared& sh, const void* rowp, int lo, i
 }
 
 // Orders n words (distinct) of `list` into out[0 .. top): out[k] the k-th largest, 0 where there are fewer.
+template <int NTH>
 __device__ __forceinline__ void order_words(const unsigned long long* list, int n, unsigned long long* out, int top) {
-    for (int k = threadIdx.x; k < top; k += NT)
+    for (int k = threadIdx.x; k < top; k += NTH)
         if (k >= n) out[k] = 0ull;
-    for (int i = threadIdx.x; i < n; i += NT) {
+    for (int i = threadIdx.x; i < n; i += NTH) {
         const unsigned long long w = list[i];
         int r = 0;
+#pragma unroll 4
         for (int j = 0; j < n; ++j) r += list[j] > w;
         if (r < top) out[r] = w;
     }
 }
 
-template <typename E, bool TOP>
-__global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const LpArgs a) {
-    constexpr int EPV = LpElem<E>::EPV;
-    constexpr int ES = 16 / EPV;
-    __shared__ LpShared sh;
-    pdl_wait_then_release();
+// The `top` best words of this CTA's part into sh.top.  tmax: this thread's maximum; vectors v of the interior belong to
+// thread v % NTH; `vec(v)` reads one (from shared memory or again from global memory).
+template <typename E, int NTH, typename Vec>
+__device__ __forceinline__ void part_top(LpShared<NTH>& sh, const LpArgs& a, const unsigned char* rowp, int lo, int n, int nh,
+                                         int nv, int nt, float tmax, Vec vec) {
+    constexpr int EPV = LpElem<E>::EPV, WARPS = NTH / 32;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hi = lo + n, i0 = lo + nh;
+    // the warps' largest thread maxima (0: none left), enough rounds for `top` of them and a few to spare
+    const int rounds = min(LP_GATHER / WARPS, (a.top + WARPS - 1) / WARPS + 2), gathered = rounds * WARPS;
+    const uint32_t mine = tmax == f_ninf() ? 0u : rank_key(tmax);
+    uint32_t k = mine;
+    for (int g = 0; g < rounds; ++g) {
+        const uint32_t mx = __reduce_max_sync(0xffffffffu, k);
+        if (lane == 0) sh.gather[warp * rounds + g] = mx;
+        const uint32_t who = __ballot_sync(0xffffffffu, k == mx);
+        if (lane == __ffs(who) - 1) k = 0u;
+    }
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
+    // tau: the top-th largest gathered maximum, each a distinct element, so at least `top` elements reach it; 0 where
+    // there are fewer: every element above -inf is listed then
+    const uint32_t g0 = lane < gathered ? sh.gather[lane] : 0u, g1 = 32 + lane < gathered ? sh.gather[32 + lane] : 0u;
+    int r0 = 0, r1 = 0;
+    for (int j = 0; j < gathered; ++j) {
+        const uint32_t o = sh.gather[j];
+        r0 += o > g0 || (o == g0 && j < lane);
+        r1 += o > g1 || (o == g1 && j < 32 + lane);
+    }
+    const uint32_t kth = __reduce_max_sync(0xffffffffu, r0 == a.top - 1 && lane < gathered           ? g0
+                                                        : r1 == a.top - 1 && 32 + lane < gathered ? g1
+                                                                                                  : 0u);
+    const uint32_t tau = kth ? kth : rank_key(f_ninf()) + 1u;
+    uint32_t hits = __ballot_sync(0xffffffffu, mine >= tau);
+    auto offer = [&](float x, int id) {
+        if (rank_key(x) >= tau) {
+            const int p = atomicAdd(&sh.n_list, 1);
+            if (p < LP_CAP) sh.list[p] = rank_word(x, id);
+        }
+    };
+    while (hits) {  // one warp per share
+        if (*reinterpret_cast<volatile int*>(&sh.n_list) > LP_CAP) break;  // the exact path will take it
+        const int h = (warp << 5) + __ffs(hits) - 1;
+        hits &= hits - 1;
+        for (int v = h + lane * NTH; v < nv; v += 32 * NTH) {
+            float x[EPV];
+            LpElem<E>::unpack(vec(v), x);
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) offer(x[j], i0 + v * EPV + j);
+        }
+        if (lane == 0 && h < nh) offer(LpElem<E>::ld(rowp, lo + h), lo + h);
+        if (lane == 0 && h >= 32 && h < 32 + nt) offer(LpElem<E>::ld(rowp, hi - nt + h - 32), hi - nt + h - 32);
+    }
+    __syncthreads();
+    if (sh.n_list > LP_CAP) {
+        exact_top<E, NTH>(sh, rowp, lo, n, a.top);
+    } else if (sh.n_list < a.top && warp == 0) {
+        // every finite element is listed; the masked ones follow in id order
+        int have = sh.n_list;
+        __syncwarp();
+        const int need = min(a.top, n);
+        for (int b = 0; b < n && have < need; b += 32) {
+            const bool tie = b + lane < n && LpElem<E>::ld(rowp, lo + b + lane) == f_ninf();
+            const uint32_t who = __ballot_sync(0xffffffffu, tie);
+            const int at = have + __popc(who & ((1u << lane) - 1u));
+            if (tie && at < need) sh.list[at] = rank_word(f_ninf(), lo + b + lane);
+            have = min(need, have + __popc(who));
+        }
+        if (lane == 0) sh.n_list = have;
+    }
+    __syncthreads();
+    order_words<NTH>(sh.list, sh.n_list, sh.top, a.top);
+}
+
+template <typename E, int NTH, bool TOP>
+__global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const LpArgs a) {
+    constexpr int EPV = LpElem<E>::EPV, ES = 16 / EPV, WARPS = NTH / 32;
+    constexpr int VPC = LP_U * NTH;  // vectors per chunk
+    __shared__ LpShared<NTH> sh;
+    extern __shared__ __align__(128) unsigned char ring[];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
     const int r = (int)(blockIdx.x / C);
@@ -198,156 +405,163 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const LpArgs a) {
     const unsigned char* rowp = static_cast<const unsigned char*>(a.logits) + (int64_t)r * a.stride * ES;
     const int lo = min(a.V, crank * a.per), hi = min(a.V, lo + a.per), n = hi - lo;
 
-    const int64_t tok = a.tokens ? a.tokens[r] : -1;
-    const bool has_tok = tok >= 0 && tok < a.V;
-    const int t = has_tok ? (int)tok : -1;
-    const float xt = has_tok ? LpElem<E>::ld(rowp, t) : 0.0f;
-    const float thr_after = xt, thr_before = pred_float(xt);
-
     // the 16-byte interior [v0, v0 + nv vectors) of the part, a ragged head and tail
     const uintptr_t A = reinterpret_cast<uintptr_t>(rowp) + (uintptr_t)lo * ES;
-    int nh = (int)(((16 - (A & 15)) & 15) / ES);
-    nh = min(nh, n);
+    const int nh = min(n, (int)(((16 - (A & 15)) & 15) / ES));
     const int nv = (n - nh) / EPV;
     const int i0 = lo + nh;             // id of the interior's first element
     const int nt = n - nh - nv * EPV;   // tail elements
     const uint4* vp = reinterpret_cast<const uint4*>(rowp + (int64_t)i0 * ES);
+    const int chunks = (nv + VPC - 1) / VPC;
+    auto load_chunk = [&](int k) {  // by one thread
+        const int s = k % a.stages, cnt = min(VPC, nv - k * VPC);
+        mbar_arrive_expect_tx(&sh.full[s], (uint32_t)cnt * 16u);
+        bulk_g2s(ring + (size_t)s * VPC * 16, vp + (int64_t)k * VPC, (uint32_t)cnt * 16u, &sh.full[s]);
+    };
+    if (tid == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            mbar_init(&sh.full[s], 1);
+            mbar_init(&sh.empty[s], WARPS);
+        }
+        fence_mbar_init();
+        sh.failed = 0;
+    }
+    pdl_wait_then_release();
+    if (tid == 0)
+        for (int k = 0; k < min(chunks, a.stages); ++k) load_chunk(k);
+    const int64_t tok = a.tokens ? a.tokens[r] : -1;
+    const bool has_tok = tok >= 0 && tok < a.V;
+    const int t = has_tok ? (int)tok : -1;
+    const float xt = has_tok ? LpElem<E>::ld(rowp, t) : 0.0f;
+    const typename LpElem<E>::Thr thr_after = LpElem<E>::threshold(xt), thr_before = LpElem<E>::threshold_before(xt);
+    const int tv = t >= i0 ? min(nv, (t - i0) / EPV) : 0;  // vectors below it lie before the token
 
-    LpState s;
+    LpThread s;
     s.m = f_ninf();
-    s.S = 0.0f;
-    s.U = 0.0f;
+    s.S = s.U = make_float2(0.0f, 0.0f);
     int cnt = 0;
     auto one = [&](float x, int id) {
-        lp_add(s, x, a.c);
-        cnt += !(x <= (id < t ? thr_before : thr_after)) && id != t;
+        lp_thread_add(s, x, a.c);
+        cnt += id != t && (x > xt || x != x || (id < t && x == xt));
     };
     if (tid < nh) one(LpElem<E>::ld(rowp, lo + tid), lo + tid);
     if (tid >= 32 && tid < 32 + nt) one(LpElem<E>::ld(rowp, hi - nt + tid - 32), hi - nt + tid - 32);
+    __syncthreads();  // the mbarriers are there
 
-    for (int b = tid; b < nv; b += LP_U * NT) {
+    int slot = 0;
+    uint32_t ph = 0;
+    for (int k = 0; k < chunks; ++k) {
+        // refill the chunk before this one: its readers have had a whole chunk's time
+        if (tid == 0 && k > 0 && k - 1 + a.stages < chunks) {
+            const int ps = (k - 1) % a.stages;
+            if (mbar_wait_bounded(&sh.empty[ps], (uint32_t)((k - 1) / a.stages) & 1u, LP_WAIT_NS)) load_chunk(k - 1 + a.stages);
+            else sh.failed = 1;
+        }
+        if (!mbar_wait_bounded(&sh.full[slot], ph, LP_WAIT_NS)) {
+            sh.failed = 1;
+            break;
+        }
+        const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)slot * VPC * 16);
         uint4 q[LP_U];
 #pragma unroll
-        for (int u = 0; u < LP_U; ++u)
-            if (b + u * NT < nv) q[u] = ldg_stream(vp + b + u * NT);
-#pragma unroll
         for (int u = 0; u < LP_U; ++u) {
-            const int v = b + u * NT;
-            if (v < nv) {
-                float x[EPV];
-                LpElem<E>::unpack(q[u], x);
-                lp_add_many<EPV>(s, x, a.c);
-                const int id = i0 + v * EPV;
-                if (t < id || t >= id + EPV) {
-                    const float thr = id < t ? thr_before : thr_after;
+            const int v = tid + u * NTH;
+            q[u] = k * VPC + v < nv ? buf[v] : LpElem<E>::nothing();
+        }
+        const float bm = LpElem<E>::batch_max(q);
+        lp_thread_batch<E>(s, q, bm, a.c);
+        // the vector that holds the token counts as behind it here
 #pragma unroll
-                    for (int j = 0; j < EPV; ++j) cnt += !(x[j] <= thr);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < EPV; ++j) cnt += !(x[j] <= (id + j < t ? thr_before : thr_after)) && id + j != t;
-                }
-            }
+        for (int u = 0; u < LP_U; ++u)
+            cnt += LpElem<E>::count_above(q[u], k * VPC + tid + u * NTH < tv ? thr_before : thr_after);
+        if (chunks > a.stages) {
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.empty[slot])) : "memory");
+        }
+        if (++slot == a.stages) {
+            slot = 0;
+            ph ^= 1;
         }
     }
-    // a NaN token: NaN compares false with everything, so every element was counted; the elements before it are the
-    // NaN ones with a smaller id
+    // the elements of the token's own vector before it that tie with it
+    if (tid == 0 && t >= i0 && t < i0 + nv * EPV)
+        for (int i = i0 + tv * EPV; i < t; ++i) cnt += LpElem<E>::ld(rowp, i) == xt;
+    // a NaN token compares false with everything, so every element was counted: the ones before it are the NaN ones with
+    // a smaller id
     if (has_tok && xt != xt) {
         cnt = 0;
-        for (int i = lo + tid; i < min(hi, t); i += NT) {
+        for (int i = lo + tid; i < min(hi, t); i += NTH) {
             const float x = LpElem<E>::ld(rowp, i);
             cnt += x != x;
         }
     }
-
     const float tmax = s.m;  // this thread's maximum (NaN if it saw one)
-    if (TOP) {
-        // the warp's LP_GATHER largest thread maxima (0: no such thread)
-        uint32_t k = tmax == f_ninf() ? 0u : rank_key(tmax);
-#pragma unroll
-        for (int g = 0; g < LP_GATHER; ++g) {
-            const uint32_t mx = __reduce_max_sync(0xffffffffu, k);
-            if (lane == 0) sh.gather[warp * LP_GATHER + g] = mx;
-            const uint32_t who = __ballot_sync(0xffffffffu, k == mx);
-            if (lane == __ffs(who) - 1) k = 0u;
-        }
-        if (tid == 0) sh.n_list = 0;
+
+    // the CTA's maximum (NaN wins), then sums relative to it
+    float m = s.m;
+    {
+        const uint32_t key = __reduce_max_sync(0xffffffffu, rank_key(m));
+        m = key == 0xffffffffu ? __int_as_float(0x7fffffff) : okey_to_f(key);
     }
-    // merge the warp's, then the CTA's states and counts
-    lp_warp_merge(s, a.c);
-    cnt = warp_sum_i(cnt);
+    if (lane == 0) sh.wmax[warp] = m;
+    __syncthreads();
+    m = sh.wmax[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) m = fmax_nan(m, sh.wmax[w]);
+    if (sh.failed) m = __int_as_float(0x7fffffff);
+    float S = 0.0f, U = 0.0f;
+    if (fabsf(m) <= 3.402823466e38f && s.m != f_ninf()) {
+        lp_thread_rescale(s, m, a.c);
+        S = s.S.x + s.S.y;
+        U = s.U.x + s.U.y;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        S += __shfl_xor_sync(0xffffffffu, S, o);
+        U += __shfl_xor_sync(0xffffffffu, U, o);
+    }
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
     if (lane == 0) {
-        sh.warp[warp] = s;
-        sh.count[warp] = cnt;
+        sh.wS[warp] = S;
+        sh.wU[warp] = U;
+        sh.wcount[warp] = cnt;
+    }
+    if (TOP) {
+        if (chunks <= a.stages && !sh.failed)
+            part_top<E, NTH>(sh, a, rowp, lo, n, nh, nv, nt, tmax,
+                             [&](int v) { return reinterpret_cast<const uint4*>(ring)[v]; });
+        else
+            part_top<E, NTH>(sh, a, rowp, lo, n, nh, nv, nt, tmax, [&](int v) { return ldg_stream(vp + v); });
     }
     __syncthreads();
-    if (warp == 0) {
-        LpState w;
-        w.m = f_ninf();
-        w.S = w.U = 0.0f;
-        int c2 = 0;
-        if (lane < NWARP) {
-            w = sh.warp[lane];
-            c2 = sh.count[lane];
-        }
-        lp_warp_merge(w, a.c);
-        c2 = warp_sum_i(c2);
-        if (lane == 0) {
+    LpState w;
+    w.m = m;
+    w.S = w.U = 0.0f;
+    int c2 = 0;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+        w.S += sh.wS[k];
+        w.U += sh.wU[k];
+        c2 += sh.wcount[k];
+    }
+    if (C > 1) {
+        if (tid == 0) {
             sh.total = w;
             sh.total_count = c2;
         }
-    }
-    if (TOP) {
-        // tau: the top-th largest gathered maximum, each a distinct element, so at least `top` elements reach it
-        const uint32_t g0 = sh.gather[lane], g1 = sh.gather[32 + lane];
-        int r0 = 0, r1 = 0;
-#pragma unroll 8
-        for (int j = 0; j < NWARP * LP_GATHER; ++j) {
-            const uint32_t o = sh.gather[j];
-            r0 += o > g0 || (o == g0 && j < lane);
-            r1 += o > g1 || (o == g1 && j < 32 + lane);
-        }
-        const uint32_t tau = __reduce_max_sync(0xffffffffu, r0 == a.top - 1 ? g0 : r1 == a.top - 1 ? g1 : 0u);
-        // pass 2: the shares whose maximum reaches tau, one warp per share
-        uint32_t hits = __ballot_sync(0xffffffffu, (tmax == f_ninf() ? 0u : rank_key(tmax)) >= tau);
-        auto offer = [&](float x, int id) {
-            if (rank_key(x) >= tau) {
-                const int p = atomicAdd(&sh.n_list, 1);
-                if (p < LP_CAP) sh.list[p] = rank_word(x, id);
+        cluster.sync();
+        if (crank == 0)
+            for (int k = 1; k < C; ++k) {
+                const LpShared<NTH>* o = cluster.map_shared_rank(&sh, k);
+                w = lp_merge(w, o->total, a.c);
+                c2 += o->total_count;
             }
-        };
-        while (hits) {
-            if (*reinterpret_cast<volatile int*>(&sh.n_list) > LP_CAP) break;  // the exact path will take it
-            const int h = (warp << 5) + __ffs(hits) - 1;
-            hits &= hits - 1;
-            for (int v = h + lane * NT; v < nv; v += 32 * NT) {
-                float x[EPV];
-                LpElem<E>::unpack(ldg_stream(vp + v), x);
-#pragma unroll
-                for (int j = 0; j < EPV; ++j) offer(x[j], i0 + v * EPV + j);
-            }
-            if (lane == 0 && h < nh) offer(LpElem<E>::ld(rowp, lo + h), lo + h);
-            if (lane == 0 && h >= 32 && h < 32 + nt) offer(LpElem<E>::ld(rowp, hi - nt + h - 32), hi - nt + h - 32);
-        }
-        __syncthreads();
-        if (sh.n_list > LP_CAP) exact_top<E>(sh, rowp, lo, n, a.top);
-        order_words(sh.list, sh.n_list, sh.top, a.top);
     }
-    if (C > 1) cluster.sync();
-    else __syncthreads();
-
     if (crank == 0) {
-        LpState w = sh.total;
-        int c2 = sh.total_count;
-        for (int k = 1; k < C; ++k) {
-            const LpShared* o = cluster.map_shared_rank(&sh, k);
-            w = lp_merge(w, o->total, a.c);
-            c2 += o->total_count;
-        }
         const LpFinal f = lp_final(w, a.c);
         if (tid == 0) {
-            float lp = 0.0f;
-            if (has_tok) lp = lp_value(xt, f, a.c);
-            if (a.logprob) a.logprob[r] = lp;
+            if (a.logprob) a.logprob[r] = has_tok ? lp_value(xt, f, a.c) : 0.0f;
             if (a.entropy) a.entropy[r] = f.entropy;
             if (a.rank) a.rank[r] = has_tok ? (int64_t)c2 : -1;
             if (a.stats) a.stats[r] = make_float4(f.m, f.R, f.log2S, f.entropy);
@@ -355,19 +569,16 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const LpArgs a) {
         }
         if (TOP) {
             // the cluster's lists (C x top words, each in order) into one
-            int n_all = 0;
+            int n_all = a.top;
+            const unsigned long long* src = sh.top;
             if (C > 1) {
-                __syncthreads();
-                for (int i = tid; i < C * a.top; i += NT) {
-                    const LpShared* o = cluster.map_shared_rank(&sh, i / a.top);
-                    sh.list[i] = o->top[i % a.top];
-                }
                 n_all = C * a.top;
+                for (int i = tid; i < n_all; i += NTH)
+                    sh.list[i] = cluster.map_shared_rank(&sh, i / a.top)->top[i % a.top];
+                src = sh.list;
                 __syncthreads();
             }
-            const unsigned long long* src = C > 1 ? sh.list : sh.top;
-            if (C == 1) n_all = a.top;
-            for (int i = tid; i < n_all; i += NT) {
+            for (int i = tid; i < n_all; i += NTH) {
                 const unsigned long long w64 = src[i];
                 int rk = i;
                 if (C > 1) {
@@ -375,11 +586,19 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const LpArgs a) {
                     for (int j = 0; j < n_all; ++j) rk += src[j] > w64;
                 }
                 if (w64 != 0ull && rk < a.top) {
-                    const int id = word_id(w64);
-                    a.top_ids[(int64_t)r * a.top + rk] = id;
-                    a.top_logprobs[(int64_t)r * a.top + rk] = lp_value(LpElem<E>::ld(rowp, id), f, a.c);
+                    const uint32_t key = (uint32_t)(w64 >> 32);
+                    const float x = key == 0xffffffffu ? __int_as_float(0x7fffffff) : okey_to_f(key);
+                    a.top_ids[(int64_t)r * a.top + rk] = word_id(w64);
+                    a.top_logprobs[(int64_t)r * a.top + rk] = lp_value(x, f, a.c);
                 }
             }
+        }
+    }
+    if (sh.failed && tid == 0) {  // copies still in flight write this CTA's shared memory: wait for them
+        if (a.status) atomicOr(a.status, B2S_STATUS_WAIT_TIMEOUT);
+        for (int s2 = 0; s2 < a.stages; ++s2) {
+            mbar_wait_bounded(&sh.full[s2], 0u, LP_WAIT_NS);
+            mbar_wait_bounded(&sh.full[s2], 1u, LP_WAIT_NS);
         }
     }
     if (C > 1) cluster.sync();  // the first CTA has read the others' shared memory
@@ -428,11 +647,12 @@ __global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void*
 }
 
 template <typename K, typename... Args>
-cudaError_t launch(K kernel, int64_t blocks, int threads, int cluster, void* stream, Args... args) {
+cudaError_t launch(K kernel, int64_t blocks, int threads, uint32_t smem, int cluster, void* stream, Args... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)blocks, 1, 1);
     cfg.blockDim = dim3((unsigned)threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -444,6 +664,21 @@ cudaError_t launch(K kernel, int64_t blocks, int threads, int cluster, void* str
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 0 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// The forward kernel on `rows` rows, C CTAs of NTH threads each; the ring holds the whole part where it fits, else as
+// many chunks as let two CTAs (1024 threads) share an SM's shared memory.
+template <typename E, int NTH, bool TOP>
+cudaError_t launch_rows(LpArgs a, int rows, int C, int es, void* stream) {
+    constexpr uint32_t CHUNK = LP_U * NTH * 16;
+    constexpr int MOST = NTH == 128 ? 12 : 3;  // 96 KB
+    a.per = ((a.V + C - 1) / C + 15) / 16 * 16;
+    const int chunks = (int)(((int64_t)a.per * es + CHUNK - 1) / CHUNK);
+    a.stages = chunks < 1 ? 1 : (chunks > MOST ? MOST : chunks);
+    const auto kernel = token_logprobs_kernel<E, NTH, TOP>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MOST * CHUNK));
+    if (e != cudaSuccess) return e;
+    return launch(kernel, (int64_t)rows * C, NTH, a.stages * CHUNK, C, stream, a);
 }
 
 }  // namespace
@@ -469,14 +704,10 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     int sms = 0;
     const cudaError_t de = device_sms(&sms);
     if (de != cudaSuccess) return cuda_fail(de);
-    int C = 1;
-    while (C < 8 && (int64_t)rows * C * 2 <= 2 * sms && (int64_t)vocab * es / (C * 2) >= 16 * 1024) C <<= 1;
-    const int per = ((vocab + C - 1) / C + 15) / 16 * 16;
     LpArgs a;
     a.logits = logits;
     a.stride = row_stride;
     a.V = vocab;
-    a.per = per;
     a.top = top;
     a.c = lp_scale(temperature);
     a.tokens = tokens;
@@ -488,11 +719,21 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     a.stats = reinterpret_cast<float4*>(stats);
     a.status = status;
     const bool bf = logits_dtype == B2S_DTYPE_BF16;
-    const cudaError_t e =
-        top ? (bf ? launch(token_logprobs_kernel<__nv_bfloat16, true>, (int64_t)rows * C, NT, C, stream, a)
-                  : launch(token_logprobs_kernel<float, true>, (int64_t)rows * C, NT, C, stream, a))
-            : (bf ? launch(token_logprobs_kernel<__nv_bfloat16, false>, (int64_t)rows * C, NT, C, stream, a)
-                  : launch(token_logprobs_kernel<float, false>, (int64_t)rows * C, NT, C, stream, a));
+    const int64_t row_bytes = (int64_t)vocab * es;
+    cudaError_t e;
+    if (rows >= 2 * sms && row_bytes <= 64 * 1024) {
+        e = top ? (bf ? launch_rows<__nv_bfloat16, 128, true>(a, rows, 1, es, stream)
+                      : launch_rows<float, 128, true>(a, rows, 1, es, stream))
+                : (bf ? launch_rows<__nv_bfloat16, 128, false>(a, rows, 1, es, stream)
+                      : launch_rows<float, 128, false>(a, rows, 1, es, stream));
+    } else {
+        int C = 1;
+        while (C < 8 && (int64_t)rows * C * 2 <= 2 * sms && row_bytes / (C * 2) >= 16 * 1024) C <<= 1;
+        e = top ? (bf ? launch_rows<__nv_bfloat16, 512, true>(a, rows, C, es, stream)
+                      : launch_rows<float, 512, true>(a, rows, C, es, stream))
+                : (bf ? launch_rows<__nv_bfloat16, 512, false>(a, rows, C, es, stream)
+                      : launch_rows<float, 512, false>(a, rows, C, es, stream));
+    }
     return e == cudaSuccess ? B2S_OK : cuda_fail(e);
 }
 
@@ -517,10 +758,10 @@ int b2s_token_logprobs_grad(const void* logits, int32_t logits_dtype, int32_t ro
     const float4* st = reinterpret_cast<const float4*>(stats);
     const cudaError_t e =
         logits_dtype == B2S_DTYPE_BF16
-            ? launch(token_logprobs_grad_kernel<__nv_bfloat16>, nch * rows, LPG_NT, 0, stream, logits, row_stride,
+            ? launch(token_logprobs_grad_kernel<__nv_bfloat16>, nch * rows, LPG_NT, 0u, 0, stream, logits, row_stride,
                      (int)vocab, chunk_vecs, (int)nch, tokens, c, inv, st, grad_logprob, grad_entropy, grad_logits,
                      grad_row_stride)
-            : launch(token_logprobs_grad_kernel<float>, nch * rows, LPG_NT, 0, stream, logits, row_stride, (int)vocab,
+            : launch(token_logprobs_grad_kernel<float>, nch * rows, LPG_NT, 0u, 0, stream, logits, row_stride, (int)vocab,
                      chunk_vecs, (int)nch, tokens, c, inv, st, grad_logprob, grad_entropy, grad_logits, grad_row_stride);
     return e == cudaSuccess ? B2S_OK : cuda_fail(e);
 }
