@@ -16,7 +16,7 @@ OPS = PKG / "_build" / "b2s_torch_ops.so"
 
 _lock = threading.Lock()
 _capi = None
-_ops_loaded = False
+_ops_loaded = None
 
 
 class SampleArgs(ctypes.Structure):
@@ -160,16 +160,18 @@ def capi() -> ctypes.CDLL:
 def ops():
     """``torch.ops.minicpmo_sampler`` with its CUDA kernels registered."""
     global _ops_loaded
+    if _ops_loaded is not None:
+        return _ops_loaded
     import torch
 
     capi()  # libb2s.so first (RTLD_GLOBAL): the op library links against it by soname
     with _lock:
-        if not _ops_loaded:
+        if _ops_loaded is None:
             if not OPS.exists():
                 raise RuntimeError(f"{OPS} is missing: build the torch op layer first (build.py)")
             torch.ops.load_library(str(OPS))
-            _ops_loaded = True
-    return torch.ops.minicpmo_sampler
+            _ops_loaded = torch.ops.minicpmo_sampler
+    return _ops_loaded
 
 
 def check(rc: int, what: str) -> None:

@@ -606,6 +606,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
 
 // dx for one chunk of a row per CTA.
 constexpr int LPG_NT = 256;
+constexpr int LPG_U = 4;  // vectors in flight per thread
 template <typename E>
 __global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void* logits, int64_t stride, int V,
                                                                      int chunk_vecs, int chunks, const int64_t* tokens,
@@ -630,19 +631,39 @@ __global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void*
         const int i = nh + nv * EPV + (int)threadIdx.x;
         if (i < V) LpElem<E>::st(outp, i, g.at(LpElem<E>::ld(rowp, i), i, c));
     }
-    const int v1 = min(nv, (ch + 1) * chunk_vecs);
-    for (int v = ch * chunk_vecs + (int)threadIdx.x; v < v1; v += LPG_NT) {
-        const int id = nh + v * EPV;
-        float x[EPV];
-        if (same) {
-            LpElem<E>::unpack(ldg_stream(reinterpret_cast<const uint4*>(rowp + (int64_t)id * ES)), x);
-        } else {
+    const int v1 = min(nv, (ch + 1) * chunk_vecs), tv = g.t >= nh ? (g.t - nh) / EPV : -1;
+    const uint4* vp = reinterpret_cast<const uint4*>(rowp + (int64_t)nh * ES);
+    for (int v0 = ch * chunk_vecs + (int)threadIdx.x; v0 < v1; v0 += LPG_U * LPG_NT) {
+        uint4 q[LPG_U];
 #pragma unroll
-            for (int j = 0; j < EPV; ++j) x[j] = LpElem<E>::ld(rowp, id + j);
+        for (int u = 0; u < LPG_U; ++u) {
+            const int v = v0 + u * LPG_NT;
+            if (v < v1) {
+                if (same) {
+                    q[u] = ldg_stream(vp + v);
+                } else {
+                    float x[EPV];
+#pragma unroll
+                    for (int j = 0; j < EPV; ++j) x[j] = LpElem<E>::ld(rowp, nh + v * EPV + j);
+                    q[u] = LpElem<E>::pack(x);  // the values themselves: nothing is rounded
+                }
+            }
         }
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) x[j] = g.at(x[j], id + j, c);
-        *reinterpret_cast<uint4*>(outp + (int64_t)id * ES) = LpElem<E>::pack(x);
+        for (int u = 0; u < LPG_U; ++u) {
+            const int v = v0 + u * LPG_NT;
+            if (v < v1) {
+                float x[EPV];
+                LpElem<E>::unpack(q[u], x);
+#pragma unroll
+                for (int j = 0; j < EPV; ++j) x[j] = g.rest(x[j], c);
+                if (v == tv) {
+#pragma unroll
+                    for (int j = 0; j < EPV; ++j) x[j] += nh + v * EPV + j == g.t ? g.bump : 0.0f;
+                }
+                __stcs(reinterpret_cast<uint4*>(outp + (int64_t)nh * ES) + v, LpElem<E>::pack(x));
+            }
+        }
     }
 }
 

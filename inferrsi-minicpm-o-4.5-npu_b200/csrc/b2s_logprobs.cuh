@@ -172,25 +172,33 @@ __device__ __forceinline__ float lp_value(float x, const LpFinal& f, float c) {
     return (y - f.log2S) * 0.693147180559945309f;
 }
 
-// The gradient of g_lp logprob + g_h entropy with respect to one value of a row.
+// The gradient of g_lp logprob + g_h entropy with respect to one value of a row:
+// (-p (g_lp + g_h H + g_h log p) + [id = token] g_lp) / T = p (scale + slope log2 p) + [id = token] bump.
 struct LpGrad {
-    float m, R, log2S, H, glp, gh, scale, inv_t;
+    float m, R, log2S, scale, slope, bump;
+    bool far;
     int t;
     // st: the forward's (m, R, log2S, entropy); the row's token or -1 (no gradient through logprob)
-    __device__ __forceinline__ LpGrad(float4 st, int tok, float g_lp, float g_h, float it)
-        : m(st.x), R(st.y), log2S(st.z), H(st.w), glp(tok >= 0 ? g_lp : 0.0f), gh(g_h), inv_t(it), t(tok) {
-        if (m == f_ninf()) glp = gh = 0.0f;  // nothing left
-        scale = -(glp + gh * H);
+    __device__ __forceinline__ LpGrad(float4 st, int tok, float g_lp, float g_h, float inv_t)
+        : m(st.x), R(st.y), log2S(st.z), t(tok) {
+        const bool none = m == f_ninf();  // nothing left: no gradient
+        const float glp = tok >= 0 && !none ? g_lp : 0.0f, gh = none ? 0.0f : g_h;
+        scale = -(glp + gh * st.w) * inv_t;
+        slope = -gh * 0.693147180559945309f * inv_t;
+        bump = glp * inv_t;
+        far = !(fabsf(R) <= 3.0e38f) && !none;
+        if (none) {
+            R = 0.0f;
+            log2S = 1000.0f;  // p = 0 for every value that is left: there is none
+        }
     }
-    __device__ __forceinline__ float at(float x, int id, float c) const {
-        float y = fabsf(R) <= 3.0e38f ? __fmaf_rn(x, c, -R) : __fmul_rn(__fsub_rn(x, m), c);
-        y = m == f_ninf() ? -400.0f : fmax_nan(y - log2S, -400.0f);  // log2 p, kept finite where p is 0
-        const float p = ex2(y);
-        // -p (glp + gh H + gh log p) + [id = t] glp
-        float d = p * __fmaf_rn(-gh * 0.693147180559945309f, y, scale);
-        if (id == t) d += glp;
-        return d * inv_t;
+    // without the token's own part
+    __device__ __forceinline__ float rest(float x, float c) const {
+        float y = far ? __fmul_rn(__fsub_rn(x, m), c) : __fmaf_rn(x, c, -R);
+        y = fmax_nan(y - log2S, -400.0f);  // log2 p, kept finite where p is 0
+        return ex2(y) * __fmaf_rn(slope, y, scale);
     }
+    __device__ __forceinline__ float at(float x, int id, float c) const { return rest(x, c) + (id == t ? bump : 0.0f); }
 };
 
 // Host side: the scale log2(e) / T rounded once.

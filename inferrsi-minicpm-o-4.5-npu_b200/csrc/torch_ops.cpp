@@ -3,8 +3,12 @@
 // without running anything.  Outputs come from the caching allocator (graph-capture pools included);
 // nothing here synchronises with the host.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -548,6 +552,11 @@ Tensor uniform_meta(const Tensor& seeds, const Tensor&, const optional<Tensor>&,
     return at::empty(seeds.sizes(), seeds.options().dtype(at::kFloat));
 }
 
+// An uninitialised tensor on the current device, straight from the caching allocator (without the dispatcher's way there).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType st, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, st, like.device(), c10::nullopt);
+}
+
 uint32_t* status_ptr(const optional<Tensor>& status, const Tensor& like) {
     if (!status.has_value() || !status->defined()) return nullptr;
     TORCH_CHECK(status->is_cuda() && status->device() == like.device() && status->scalar_type() == at::kInt &&
@@ -607,10 +616,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_cuda(c
     TORCH_CHECK(B <= INT32_MAX && V <= INT32_MAX && top <= INT32_MAX, "more than 2^31 - 1 rows or ids");
     check_tokens(tokens, logits, B);
     const Tensor x = plain_rows(logits);
-    auto of = x.options().dtype(at::kFloat), oi = x.options().dtype(at::kLong);
-    Tensor lp = at::empty({B}, of), ent = at::empty({B}, of), rank = at::empty({B}, oi);
-    Tensor ids = at::empty({B, top}, oi), vals = at::empty({B, top}, of);
-    Tensor stats = at::empty({want_stats ? B : 0, 4}, of);
+    Tensor lp = fresh({B}, at::kFloat, x), ent = fresh({B}, at::kFloat, x), rank = fresh({B}, at::kLong, x);
+    Tensor ids = fresh({B, top}, at::kLong, x), vals = fresh({B, top}, at::kFloat, x);
+    Tensor stats = fresh({want_stats ? B : 0, 4}, at::kFloat, x);
     check_rc(b2s_token_logprobs(x.data_ptr(), dt, (int32_t)B, (int32_t)V, row_stride(x), tokens.data_ptr<int64_t>(),
                                 (float)temperature, (int32_t)top, lp.data_ptr<float>(), ent.data_ptr<float>(),
                                 rank.data_ptr<int64_t>(), top ? ids.data_ptr<int64_t>() : nullptr,
@@ -640,7 +648,7 @@ Tensor token_logprobs_grad_cuda(const Tensor& logits, const Tensor& tokens, cons
     TORCH_CHECK(stats.is_contiguous() && stats.numel() == 4 * B, "stats must be contiguous [rows, 4]");
     const Tensor x = plain_rows(logits);
     Tensor gl = grad_vector(g_lp, logits, B, "grad_logprob"), ge = grad_vector(g_ent, logits, B, "grad_entropy");
-    Tensor out = at::empty({B, V}, x.options());
+    Tensor out = fresh({B, V}, x.scalar_type(), x);
     check_rc(b2s_token_logprobs_grad(x.data_ptr(), dt, (int32_t)B, (int32_t)V, row_stride(x),
                                      tokens.data_ptr<int64_t>(), (float)temperature, stats.data_ptr<float>(),
                                      opt_f(gl), opt_f(ge), out.data_ptr(), V,
@@ -683,7 +691,7 @@ b2s_lmhead_args head_args(Tensor& hidden, Tensor& head, const Tensor& tokens, do
     return a;
 }
 
-Tensor workspace(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+Tensor workspace(int64_t bytes, const Tensor& like) { return fresh({bytes}, at::kByte, like); }
 
 // Log probabilities of given tokens straight from a head.
 std::tuple<Tensor, Tensor, Tensor> lmhead_logprobs_cuda(const Tensor& hidden_, const Tensor& head_,
@@ -692,9 +700,8 @@ std::tuple<Tensor, Tensor, Tensor> lmhead_logprobs_cuda(const Tensor& hidden_, c
     c10::cuda::CUDAGuard guard(hidden_.device());
     Tensor hidden = hidden_, head = head_;
     b2s_lmhead_args a = head_args(hidden, head, tokens, temperature, status);
-    auto of = hidden.options().dtype(at::kFloat);
-    Tensor lp = at::empty({a.rows}, of), ent = at::empty({a.rows}, of);
-    Tensor stats = at::empty({want_stats ? a.rows : 0, 4}, of);
+    Tensor lp = fresh({a.rows}, at::kFloat, hidden), ent = fresh({a.rows}, at::kFloat, hidden);
+    Tensor stats = fresh({want_stats ? a.rows : 0, 4}, at::kFloat, hidden);
     check_rc(b2s_lmhead_logprobs_workspace(a.rows, a.vocab, a.hidden_dim, &a.workspace_bytes),
              "b2s_lmhead_logprobs_workspace");
     Tensor ws = workspace(a.workspace_bytes, hidden);
@@ -722,8 +729,8 @@ std::tuple<Tensor, Tensor> lmhead_logprobs_grad_cuda(const Tensor& hidden_, cons
     check_same(stats, hidden, at::kFloat, "stats");
     TORCH_CHECK(stats.is_contiguous() && stats.numel() == 4 * (int64_t)a.rows, "stats must be contiguous [rows, 4]");
     Tensor gl = grad_vector(g_lp, hidden, a.rows, "grad_logprob"), ge = grad_vector(g_ent, hidden, a.rows, "grad_entropy");
-    Tensor dh = at::empty({want_hidden ? a.rows : 0, a.hidden_dim}, hidden.options());
-    Tensor dw = at::empty({want_head ? a.vocab : 0, a.hidden_dim}, hidden.options());
+    Tensor dh = fresh({want_hidden ? a.rows : 0, a.hidden_dim}, at::kBFloat16, hidden);
+    Tensor dw = fresh({want_head ? a.vocab : 0, a.hidden_dim}, at::kBFloat16, hidden);
     if (!want_hidden && !want_head) return {dh, dw};
     check_rc(b2s_lmhead_logprobs_grad_workspace(a.rows, a.vocab, a.hidden_dim, &a.workspace_bytes),
              "b2s_lmhead_logprobs_grad_workspace");
@@ -772,8 +779,8 @@ std::tuple<Tensor, Tensor> linear_cuda(const Tensor& x_, const Tensor& weight_, 
                     "residual must be [rows, out]");
         r = plain_rows(*residual);
     }
-    Tensor out = at::empty({R, N}, x.options());
-    Tensor pre = at::empty({want_preact ? R : 0, round8(N)}, x.options());
+    Tensor out = fresh({R, N}, at::kBFloat16, x);
+    Tensor pre = fresh({want_preact ? R : 0, round8(N)}, at::kBFloat16, x);
     b2s_linear_args a;
     memset(&a, 0, sizeof(a));
     a.x = x.data_ptr();
@@ -820,8 +827,8 @@ std::tuple<Tensor, Tensor, Tensor> linear_grad_cuda(const Tensor& grad_out, cons
     const int64_t R = x_.size(0), K = x_.size(1), N = weight_.size(0);
     TORCH_CHECK(grad_out.dim() == 2 && grad_out.size(0) == R && grad_out.size(1) == N, "grad_out must be [rows, out]");
     const Tensor x = aligned_rows(x_), weight = aligned_rows(weight_), g = plain_rows(grad_out);
-    Tensor dx = at::empty({want_x ? R : 0, K}, x.options()), dw = at::empty({want_weight ? N : 0, K}, x.options());
-    Tensor db = at::empty({want_bias ? N : 0}, x.options());
+    Tensor dx = fresh({want_x ? R : 0, K}, at::kBFloat16, x), dw = fresh({want_weight ? N : 0, K}, at::kBFloat16, x);
+    Tensor db = fresh({want_bias ? N : 0}, at::kBFloat16, x);
     b2s_linear_grad_args a;
     memset(&a, 0, sizeof(a));
     a.grad_out = g.data_ptr();
@@ -860,6 +867,189 @@ std::tuple<Tensor, Tensor, Tensor> linear_grad_meta(const Tensor&, const Tensor&
     const int64_t K = x.size(1), N = weight.size(0);
     return {at::empty({want_x ? x.size(0) : 0, K}, x.options()), at::empty({want_weight ? N : 0, K}, x.options()),
             at::empty({want_bias ? N : 0}, x.options())};
+}
+
+// ------------------------------------------------------------------ gradients
+// The differentiable operators' Autograd kernels: nodes of torch's graph whose backward calls the gradient ops above.  A
+// call whose inputs need no gradient goes straight on to the CUDA kernel.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool needs_grad(const optional<Tensor>& t) { return t.has_value() && needs_grad(*t); }
+Tensor or_none(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+optional<Tensor> or_null(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+
+// The gradients have none of their own: under create_graph they carry a node that says so if it is ever run.
+void seal(variable_list& grads, const char* what) {
+    if (!at::GradMode::is_enabled()) return;
+    variable_list given;
+    for (const Tensor& g : grads)
+        if (g.defined()) given.push_back(g.detach().set_requires_grad(true));
+    if (given.empty()) return;
+    auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once",
+                                                                (int64_t)given.size());
+    variable_list sealed = (*node)(std::move(given));
+    size_t k = 0;
+    for (Tensor& g : grads)
+        if (g.defined()) g = sealed[k++];
+}
+
+// The operators below the Autograd key (CUDA, Meta, a tracer's fake tensors).
+template <typename F>
+c10::TypedOperatorHandle<F> op_handle(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+const auto& token_logprobs_op() {
+    static const auto op = op_handle<decltype(token_logprobs_cuda)>("minicpmo_sampler::token_logprobs");
+    return op;
+}
+const auto& token_logprobs_grad_op() {
+    static const auto op = op_handle<decltype(token_logprobs_grad_cuda)>("minicpmo_sampler::token_logprobs_grad");
+    return op;
+}
+const auto& lmhead_logprobs_op() {
+    static const auto op = op_handle<decltype(lmhead_logprobs_cuda)>("minicpmo_sampler::lmhead_logprobs");
+    return op;
+}
+const auto& lmhead_logprobs_grad_op() {
+    static const auto op = op_handle<decltype(lmhead_logprobs_grad_cuda)>("minicpmo_sampler::lmhead_logprobs_grad");
+    return op;
+}
+const auto& linear_op() {
+    static const auto op = op_handle<decltype(linear_cuda)>("minicpmo_sampler::linear");
+    return op;
+}
+const auto& linear_grad_op() {
+    static const auto op = op_handle<decltype(linear_grad_cuda)>("minicpmo_sampler::linear_grad");
+    return op;
+}
+
+struct TokenLogprobsNode : public torch::autograd::Function<TokenLogprobsNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, double temperature,
+                                 int64_t top, const optional<Tensor>& status) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [lp, ent, rank, ids, vals, stats] = token_logprobs_op().call(logits, tokens, temperature, top, true, status);
+        ctx->save_for_backward({logits, tokens, stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->mark_non_differentiable({rank, ids, vals, stats});
+        ctx->set_materialize_grads(false);
+        return {lp, ent, rank, ids, vals, stats};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(5);
+        if (!g[0].defined() && !g[1].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            out[0] = token_logprobs_grad_op().call(saved[0], saved[1], saved[2], or_null(g[0]), or_null(g[1]),
+                                                   ctx->saved_data["temperature"].toDouble());
+        }
+        seal(out, "token_logprobs");
+        return out;
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_autograd(const Tensor& logits,
+                                                                                   const Tensor& tokens,
+                                                                                   double temperature, int64_t top,
+                                                                                   bool want_stats,
+                                                                                   const optional<Tensor>& status) {
+    if (!at::GradMode::is_enabled() || !needs_grad(logits)) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return token_logprobs_op().call(logits, tokens, temperature, top, want_stats, status);
+    }
+    variable_list o = TokenLogprobsNode::apply(logits, tokens, temperature, top, status);
+    return {o[0], o[1], o[2], o[3], o[4], o[5]};
+}
+
+struct HeadLogprobsNode : public torch::autograd::Function<HeadLogprobsNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& head, const Tensor& tokens,
+                                 double temperature, const optional<Tensor>& status) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [lp, ent, stats] = lmhead_logprobs_op().call(hidden, head, tokens, temperature, true, status);
+        ctx->save_for_backward({hidden, head, tokens, stats, or_none(status)});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->mark_non_differentiable({stats});
+        ctx->set_materialize_grads(false);
+        return {lp, ent, stats};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(5);
+        if (!g[0].defined() && !g[1].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            auto [dh, dw] = lmhead_logprobs_grad_op().call(saved[0], saved[1], saved[2], saved[3], or_null(g[0]),
+                                                           or_null(g[1]), ctx->saved_data["temperature"].toDouble(),
+                                                           want_h, want_w, or_null(saved[4]));
+            if (want_h) out[0] = dh;
+            if (want_w) out[1] = dw;
+        }
+        seal(out, "lmhead_logprobs");
+        return out;
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor> lmhead_logprobs_autograd(const Tensor& hidden, const Tensor& head,
+                                                            const Tensor& tokens, double temperature, bool want_stats,
+                                                            const optional<Tensor>& status) {
+    if (!at::GradMode::is_enabled() || !(needs_grad(hidden) || needs_grad(head))) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return lmhead_logprobs_op().call(hidden, head, tokens, temperature, want_stats, status);
+    }
+    variable_list o = HeadLogprobsNode::apply(hidden, head, tokens, temperature, status);
+    return {o[0], o[1], o[2]};
+}
+
+struct LinearNode : public torch::autograd::Function<LinearNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
+                                 const optional<Tensor>& residual, int64_t activation, const optional<Tensor>& status) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [out, pre] = linear_op().call(x, weight, bias, residual, activation, activation != B2S_ACT_NONE, status);
+        ctx->save_for_backward({x, weight, activation != B2S_ACT_NONE ? pre : Tensor(), or_none(status)});
+        ctx->saved_data["activation"] = activation;
+        // the graph's edges are numbered over the tensors that were there
+        ctx->saved_data["bias"] = bias.has_value() && bias->defined();
+        ctx->saved_data["residual"] = residual.has_value() && residual->defined();
+        ctx->mark_non_differentiable({pre});
+        ctx->set_materialize_grads(false);
+        return {out, pre};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(6);
+        if (!g[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        const bool want_b = has_b && ctx->needs_input_grad(2);
+        if (want_x || want_w || want_b) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            auto [dx, dw, db] = linear_grad_op().call(g[0], saved[0], saved[1], or_null(saved[2]),
+                                                      ctx->saved_data["activation"].toInt(), want_x, want_w, want_b,
+                                                      or_null(saved[3]));
+            if (want_x) out[0] = dx;
+            if (want_w) out[1] = dw;
+            if (want_b) out[2] = db;
+        }
+        seal(out, "linear");
+        if (has_r && ctx->needs_input_grad(has_b ? 3 : 2)) out[3] = g[0];
+        return out;
+    }
+};
+
+std::tuple<Tensor, Tensor> linear_autograd(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
+                                           const optional<Tensor>& residual, int64_t activation, bool want_preact,
+                                           const optional<Tensor>& status) {
+    if (!at::GradMode::is_enabled() ||
+        !(needs_grad(x) || needs_grad(weight) || needs_grad(bias) || needs_grad(residual))) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return linear_op().call(x, weight, bias, residual, activation, want_preact, status);
+    }
+    variable_list o = LinearNode::apply(x, weight, bias, residual, activation, status);
+    return {o[0], o[1]};
 }
 
 }  // namespace
@@ -969,4 +1159,10 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, Meta, m) {
     m.impl("lmhead_logprobs_grad", &lmhead_logprobs_grad_meta);
     m.impl("linear", &linear_meta);
     m.impl("linear_grad", &linear_grad_meta);
+}
+
+TORCH_LIBRARY_IMPL(minicpmo_sampler, Autograd, m) {
+    m.impl("token_logprobs", &token_logprobs_autograd);
+    m.impl("lmhead_logprobs", &lmhead_logprobs_autograd);
+    m.impl("linear", &linear_autograd);
 }

@@ -22,7 +22,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 from . import talker_sampler as ts
@@ -53,27 +52,7 @@ def _check_temperature(t) -> float:
 def _check_tokens(tokens: torch.Tensor, rows: int) -> torch.Tensor:
     if tokens.dim() != 1 or tokens.shape[0] != rows or tokens.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"tokens must be int64 [{rows}], got {tokens.dtype} {tuple(tokens.shape)}")
-    return tokens.to(torch.int64).contiguous()
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, temperature, top, status):
-        lp, ent, rank, ids, vals, stats = _native.ops().token_logprobs(logits, tokens, temperature, top, True, status)
-        ctx.save_for_backward(logits, tokens, stats)
-        ctx.temperature = temperature
-        ctx.mark_non_differentiable(rank, ids, vals)
-        ctx.set_materialize_grads(False)
-        return lp, ent, rank, ids, vals
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, _rank, _ids, _vals):
-        if g_lp is None and g_ent is None:
-            return None, None, None, None, None
-        logits, tokens, stats = ctx.saved_tensors
-        return (_native.ops().token_logprobs_grad(logits, tokens, stats, g_lp, g_ent, ctx.temperature), None, None,
-                None, None)
+    return tokens if tokens.dtype == torch.int64 and tokens.is_contiguous() else tokens.to(torch.int64).contiguous()
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, temperature: float = 1.0,
@@ -87,32 +66,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
         raise ValueError(f"top must be within [0, {min(MAX_TOP, logits.shape[1])}], got {top}")
     temperature, top = _check_temperature(temperature), int(top)
     tokens = _check_tokens(tokens, logits.shape[0])
-    if torch.is_grad_enabled() and logits.requires_grad:
-        lp, ent, rank, ids, vals = _TokenLogprobs.apply(logits, tokens, temperature, top, status)
-    else:
-        lp, ent, rank, ids, vals, _ = _native.ops().token_logprobs(logits, tokens, temperature, top, False, status)
+    lp, ent, rank, ids, vals, _ = _native.ops().token_logprobs(logits, tokens, temperature, top, False, status)
     return TokenLogprobs(lp, ent, rank, ids if top else None, vals if top else None)
-
-
-class _HeadLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, head, tokens, temperature, status):
-        lp, ent, stats = _native.ops().lmhead_logprobs(hidden, head, tokens, temperature, True, status)
-        ctx.save_for_backward(hidden, head, tokens, stats)
-        ctx.temperature, ctx.status = temperature, status
-        ctx.set_materialize_grads(False)
-        return lp, ent
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent):
-        if g_lp is None and g_ent is None:
-            return None, None, None, None, None
-        hidden, head, tokens, stats = ctx.saved_tensors
-        want_h, want_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        dh, dw = _native.ops().lmhead_logprobs_grad(hidden, head, tokens, stats, g_lp, g_ent, ctx.temperature, want_h,
-                                                    want_w, ctx.status)
-        return dh if want_h else None, dw if want_w else None, None, None, None
 
 
 class LMHeadLogprobs:
@@ -136,7 +91,5 @@ class LMHeadLogprobs:
             raise ValueError(f"hidden must be bf16 [rows, {self.head.shape[1]}]")
         temperature = _check_temperature(temperature)
         tokens = _check_tokens(tokens, hidden.shape[0])
-        if torch.is_grad_enabled() and (hidden.requires_grad or self.head.requires_grad):
-            return HeadLogprobs(*_HeadLogprobs.apply(hidden, self.head, tokens, temperature, status))
         lp, ent, _ = _native.ops().lmhead_logprobs(hidden, self.head, tokens, temperature, False, status)
         return HeadLogprobs(lp, ent)

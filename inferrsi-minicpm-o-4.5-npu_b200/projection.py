@@ -13,33 +13,12 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 from . import talker_sampler as ts
 
 # the activations' C-ABI codes; "gelu" is the exact form, 0.5 z (1 + erf(z / sqrt 2))
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, status):
-        out, preact = _native.ops().linear(x, weight, bias, residual, act, act != 0, status)
-        ctx.save_for_backward(x, weight, preact if act else None)
-        ctx.act, ctx.status = act, status
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, weight, preact = ctx.saved_tensors
-        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if want_x or want_w or want_b:
-            dx, dw, db = _native.ops().linear_grad(g, x, weight, preact, ctx.act, want_x, want_w, want_b, ctx.status)
-        return (dx if want_x else None, dw if want_w else None, db if want_b else None, g if want_r else None, None,
-                None)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -66,8 +45,5 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     act = ACTIVATIONS[activation]
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     r2 = residual if residual is None or x.dim() == 2 else residual.reshape(-1, n)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias, r2)):
-        out = _Linear.apply(x2, weight, bias, r2, act, status)
-    else:
-        out, _ = _native.ops().linear(x2, weight, bias, r2, act, False, status)
+    out, _ = _native.ops().linear(x2, weight, bias, r2, act, False, status)
     return out if x.dim() == 2 else out.reshape(shape)
