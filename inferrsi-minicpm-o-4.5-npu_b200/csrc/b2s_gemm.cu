@@ -3,7 +3,7 @@
 // reference, whose call sites use F.linear.
 #include <string.h>
 
-#include <mutex>
+#include <atomic>
 
 #include "b2s_gemm.cuh"
 
@@ -567,8 +567,15 @@ int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, const Pla
     a.split = p.split;
     a.chunk = p.chunk;
     const auto kernel = gemm_kernel<CG, TN, AMN, BMN, EPI>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gm_smem(CG, TN));
+    static std::atomic<bool> set[64];  // the attribute is set once per device; racing callers set the same
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e);
+    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_relaxed)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gm_smem(CG, TN));
+        if (e != cudaSuccess) return cuda_fail(e);
+        if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
+    }
     e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, GM_THREADS, gm_smem(CG, TN), stream, amap, bmap, a);
     if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
         if (e == cudaSuccess && p.split > 1) {

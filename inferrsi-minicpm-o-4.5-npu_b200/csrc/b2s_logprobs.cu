@@ -15,17 +15,22 @@
 // rows are few.  Two elements share one packed fp32 operation, and a bf16 pair one maximum and one comparison: about 6
 // instructions an element, so that bf16 rows stay bound by HBM.  The rank counts the elements before the token in (value
 // descending, id ascending) order: an element before the token counts when x >= x_t, i.e. x > pred(x_t), one after it
-// when x > x_t, so a vector needs one threshold.  Top alternatives: pass 1 leaves each thread's maximum; the top-th
-// largest of the warps' largest maxima bounds the CTA's top-th value from below; only the shares of threads that reach
-// it are read again (from shared memory where the part fits, else from L2), their elements above the bound listed and
-// ordered by rank counting.  Where too few threads hold anything (short or masked rows) every finite element is listed
-// and the first masked ids fill what is missing.  Lists that overflow (more ties than the list holds) take an exact
-// radix select over the CTA's part of the row.
+// when x > x_t, so a vector needs one threshold.  Top alternatives: the
+// top-th largest of the warps' largest thread maxima bounds the CTA's top-th value from below (each is a distinct
+// element), and what reaches the bound is listed, element by element of the threads whose maximum does, and ordered by
+// rank counting.  Where the CTA's part of the row fits the ring this happens once, from shared memory, after the last
+// chunk.  Longer parts list on the way, with a bound from the first chunk that is taken again after 4, 16, .. chunks, so
+// that about 3 `top` elements are listed while what was read grows fourfold.  Where too few threads hold anything (short
+// or masked rows) every finite element is listed and the first masked ids fill what is missing.  A list that overflows is
+// made again in a second pass (L2) from a last bound, and where ties overflow that too, by an exact radix select.
 //
 // Backward, elementwise: dx = (g_lp ([i = t] - p) - g_H p (log p + H)) / T with p = 2^(y - log2 S) recomputed from
 // the saved reference: one read and one write of the row.
 #include <cooperative_groups.h>
 #include <string.h>
+
+#include <atomic>
+#include <type_traits>
 
 #include "../../include/b2s_sampler.h"
 #include "b2s_device.cuh"
@@ -85,12 +90,16 @@ struct LpElem<float> {
         }
         return m;
     }
+    static __device__ __forceinline__ float vec_max(uint4 q) {
+        return fmax_nan(fmax_nan(__uint_as_float(q.x), __uint_as_float(q.y)), fmax_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
+    }
     // elements above the threshold, or NaN
     static __device__ __forceinline__ int count_above(uint4 q, Thr t) {
         return !(__uint_as_float(q.x) <= t) + !(__uint_as_float(q.y) <= t) + !(__uint_as_float(q.z) <= t) +
                !(__uint_as_float(q.w) <= t);
     }
     static __device__ __forceinline__ float ld(const void* p, int64_t i) { return __ldg(static_cast<const float*>(p) + i); }
+    static __device__ __forceinline__ float ld_shared(const uint4* p, int j) { return reinterpret_cast<const float*>(p)[j]; }
     static __device__ __forceinline__ void unpack(uint4 q, float (&x)[4]) {
         x[0] = __uint_as_float(q.x); x[1] = __uint_as_float(q.y); x[2] = __uint_as_float(q.z); x[3] = __uint_as_float(q.w);
     }
@@ -123,6 +132,10 @@ struct LpElem<__nv_bfloat16> {
         }
         return fmax_nan(__low2float(m), __high2float(m));
     }
+    static __device__ __forceinline__ float vec_max(uint4 q) {
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(as2(q.x), as2(q.y)), __hmax2_nan(as2(q.z), as2(q.w)));
+        return fmax_nan(__low2float(m), __high2float(m));
+    }
     // elements above the threshold, or NaN: a true comparison is a 0xffff half, whose low byte is -1
     static __device__ __forceinline__ int count_above(uint4 q, Thr t) {
         int n = __dp4a((int)__hgtu2_mask(as2(q.x), t), 0x00010001, 0);
@@ -133,6 +146,9 @@ struct LpElem<__nv_bfloat16> {
     }
     static __device__ __forceinline__ float ld(const void* p, int64_t i) {
         return bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(p) + i));
+    }
+    static __device__ __forceinline__ float ld_shared(const uint4* p, int j) {
+        return bf16_bits_to_f(reinterpret_cast<const unsigned short*>(p)[j]);
     }
     static __device__ __forceinline__ void unpack(uint4 q, float (&x)[8]) {
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -165,21 +181,26 @@ __device__ __forceinline__ unsigned long long rank_word(float x, int id) {
 }
 __device__ __forceinline__ int word_id(unsigned long long w) { return (int)(0xffffffffu - (uint32_t)w); }
 
-template <int NTH>
-struct LpShared {
-    static constexpr int WARPS = NTH / 32;
-    uint64_t full[16], empty[16];
-    float wmax[WARPS];
-    float wS[WARPS], wU[WARPS];
-    int wcount[WARPS];
-    uint32_t gather[LP_GATHER];
-    int n_list, failed;
-    int ties[WARPS];
+struct LpLists {
+    alignas(16) uint32_t gather[LP_GATHER];
+    uint32_t bound;  // the last bound, 0: none
+    int n_list;
+    int ties[16];
     uint32_t hist[256];
     uint32_t ctl[2];
     unsigned long long list[LP_CAP];
     unsigned long long top[LP_MAX_TOP];  // this CTA's best, in order (0: none)
-    LpState total;                       // this CTA's state and count, read by the cluster's first CTA
+};
+struct LpNoLists {};
+template <int NTH, bool TOP>
+struct LpShared : std::conditional_t<TOP, LpLists, LpNoLists> {
+    static constexpr int WARPS = NTH / 32;
+    uint64_t full[6], empty[6];
+    float wmax[WARPS];
+    float wS[WARPS], wU[WARPS];
+    int wcount[WARPS];
+    int failed;
+    LpState total;  // this CTA's state and count, read by the cluster's first CTA
     int total_count;
 };
 
@@ -268,7 +289,7 @@ __device__ __forceinline__ void lp_thread_batch(LpThread& s, const uint4 (&q)[LP
 // the ties: the need-th largest value by radix select, then everything above it and the first ties in id order.
 // Every thread calls it; sh.list holds min(need, n) words afterwards.
 template <typename E, int NTH>
-__device__ __noinline__ void exact_top(LpShared<NTH>& sh, const void* rowp, int lo, int n, int need) {
+__device__ __noinline__ void exact_top(LpLists& sh, const void* rowp, int lo, int n, int need) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     need = min(need, n);
     auto key = [&](int i) { return rank_key(LpElem<E>::ld(rowp, lo + i)); };
@@ -304,81 +325,123 @@ __device__ __noinline__ void exact_top(LpShared<NTH>& sh, const void* rowp, int 
     __syncthreads();
 }
 
+// How many of the n words of `list` come before the i-th (i < n), by 8 lanes a word; the warp calls it converged.
+__device__ __forceinline__ int rank_of(const unsigned long long* list, int n, int i) {
+    const unsigned long long w = i < n ? list[i] : 0ull;
+    int r = 0;
+#pragma unroll 2
+    for (int j = threadIdx.x & 7; j < n; j += 8) r += list[j] > w;
+    r += __shfl_xor_sync(0xffffffffu, r, 1);
+    r += __shfl_xor_sync(0xffffffffu, r, 2);
+    return r + __shfl_xor_sync(0xffffffffu, r, 4);
+}
 // Orders n words (distinct) of `list` into out[0 .. top): out[k] the k-th largest, 0 where there are fewer.
 template <int NTH>
 __device__ __forceinline__ void order_words(const unsigned long long* list, int n, unsigned long long* out, int top) {
     for (int k = threadIdx.x; k < top; k += NTH)
         if (k >= n) out[k] = 0ull;
-    for (int i = threadIdx.x; i < n; i += NTH) {
-        const unsigned long long w = list[i];
-        int r = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) r += list[j] > w;
-        if (r < top) out[r] = w;
+    for (int b = 0; b < n; b += NTH / 8) {
+        const int i = b + (int)(threadIdx.x >> 3), r = rank_of(list, n, i);
+        if ((threadIdx.x & 7) == 0 && i < n && r < top) out[r] = list[i];
     }
 }
 
-// The `top` best words of this CTA's part into sh.top.  tmax: this thread's maximum; vectors v of the interior belong to
-// thread v % NTH; `vec(v)` reads one (from shared memory or again from global memory).
-template <typename E, int NTH, typename Vec>
-__device__ __forceinline__ void part_top(LpShared<NTH>& sh, const LpArgs& a, const unsigned char* rowp, int lo, int n, int nh,
-                                         int nv, int nt, float tmax, Vec vec) {
-    constexpr int EPV = LpElem<E>::EPV, WARPS = NTH / 32;
+// Whether a value reaches the bound (as a value: NaN does).
+__device__ __forceinline__ bool reaches(float x, float bound) { return !(x < bound); }
+__device__ __forceinline__ float bound_value(uint32_t bound) {
+    return bound == 0xffffffffu || bound > 0xff800000u ? __int_as_float(0x7f800000) : okey_to_f(bound);  // NaN only: +inf
+}
+
+// The bound (see above) from this thread's maximum so far: an order key that at least `top` elements reach, or, where
+// there are fewer maxima than that, the one above -inf's.  Every thread calls it.  A gathered word is a key without its
+// last 6 bits and the complement of its place, so that words differ; the bound they give is lower by less than 64 keys.
+// The first `warps` warps hold something.
+template <int NTH>
+__device__ __noinline__ float top_bound(LpLists& sh, int top, int warps, float tmax) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int hi = lo + n, i0 = lo + nh;
-    // the warps' largest thread maxima (0: none left), enough rounds for `top` of them and a few to spare
-    const int rounds = min(LP_GATHER / WARPS, (a.top + WARPS - 1) / WARPS + 2), gathered = rounds * WARPS;
-    const uint32_t mine = tmax == f_ninf() ? 0u : rank_key(tmax);
-    uint32_t k = mine;
-    for (int g = 0; g < rounds; ++g) {
+    // enough rounds for `top` maxima and a few to spare
+    const int rounds = min(LP_GATHER / warps, (top + warps - 1) / warps + 2), gathered = rounds * warps;
+    uint32_t k = tmax == f_ninf() ? 0u : rank_key(tmax);
+#pragma unroll 1
+    for (int g = 0; g < (warp < warps ? rounds : 0); ++g) {
         const uint32_t mx = __reduce_max_sync(0xffffffffu, k);
-        if (lane == 0) sh.gather[warp * rounds + g] = mx;
+        const int at = warp * rounds + g;
+        if (lane == 0) sh.gather[at] = (mx & ~63u) | (63u - (uint32_t)at);
         const uint32_t who = __ballot_sync(0xffffffffu, k == mx);
         if (lane == __ffs(who) - 1) k = 0u;
     }
-    if (tid == 0) sh.n_list = 0;
+    if (tid >= gathered && tid < LP_GATHER) sh.gather[tid] = 63u - (uint32_t)tid;
     __syncthreads();
-    // tau: the top-th largest gathered maximum, each a distinct element, so at least `top` elements reach it; 0 where
-    // there are fewer: every element above -inf is listed then
-    const uint32_t g0 = lane < gathered ? sh.gather[lane] : 0u, g1 = 32 + lane < gathered ? sh.gather[32 + lane] : 0u;
-    int r0 = 0, r1 = 0;
-    for (int j = 0; j < gathered; ++j) {
-        const uint32_t o = sh.gather[j];
-        r0 += o > g0 || (o == g0 && j < lane);
-        r1 += o > g1 || (o == g1 && j < 32 + lane);
-    }
-    const uint32_t kth = __reduce_max_sync(0xffffffffu, r0 == a.top - 1 && lane < gathered           ? g0
-                                                        : r1 == a.top - 1 && 32 + lane < gathered ? g1
-                                                                                                  : 0u);
-    const uint32_t tau = kth ? kth : rank_key(f_ninf()) + 1u;
-    uint32_t hits = __ballot_sync(0xffffffffu, mine >= tau);
-    auto offer = [&](float x, int id) {
-        if (rank_key(x) >= tau) {
-            const int p = atomicAdd(&sh.n_list, 1);
-            if (p < LP_CAP) sh.list[p] = rank_word(x, id);
+    if (tid < LP_GATHER) {
+        const uint32_t mine = sh.gather[tid];
+        int r = 0;
+#pragma unroll 8
+        for (int j = 0; j < LP_GATHER; j += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(&sh.gather[j]);
+            r += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
         }
-    };
-    while (hits) {  // one warp per share
-        if (*reinterpret_cast<volatile int*>(&sh.n_list) > LP_CAP) break;  // the exact path will take it
-        const int h = (warp << 5) + __ffs(hits) - 1;
-        hits &= hits - 1;
-        for (int v = h + lane * NTH; v < nv; v += 32 * NTH) {
-            float x[EPV];
-            LpElem<E>::unpack(vec(v), x);
-#pragma unroll
-            for (int j = 0; j < EPV; ++j) offer(x[j], i0 + v * EPV + j);
-        }
-        if (lane == 0 && h < nh) offer(LpElem<E>::ld(rowp, lo + h), lo + h);
-        if (lane == 0 && h >= 32 && h < 32 + nt) offer(LpElem<E>::ld(rowp, hi - nt + h - 32), hi - nt + h - 32);
+        if (r == top - 1) sh.bound = mine & ~63u;
     }
     __syncthreads();
-    if (sh.n_list > LP_CAP) {
-        exact_top<E, NTH>(sh, rowp, lo, n, a.top);
-    } else if (sh.n_list < a.top && warp == 0) {
+    return bound_value(sh.bound ? sh.bound : rank_key(f_ninf()) + 1u);
+}
+
+// Appends the lanes' elements that reach the bound, one shared atomic for all of them; the warp calls it converged.
+__device__ __forceinline__ void offer(LpLists& sh, float bound, bool there, float x, int id) {
+    const int lane = threadIdx.x & 31;
+    const bool pass = there && reaches(x, bound);
+    const uint32_t who = __ballot_sync(0xffffffffu, pass);
+    if (who == 0u) return;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&sh.n_list, __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+    if (pass && at < LP_CAP) sh.list[at] = rank_word(x, id);
+}
+template <typename E>
+__device__ __noinline__ void offer_vec(LpLists& sh, float bound, bool there, uint4 q, int id) {
+    if (!__any_sync(0xffffffffu, there && reaches(LpElem<E>::vec_max(q), bound))) return;
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {  // a word at a time, the next one moved to the front
+        if (LpElem<E>::EPV == 4) {
+            offer(sh, bound, there, __uint_as_float(q.x), id + j);
+        } else {
+            offer(sh, bound, there, __uint_as_float(q.x << 16), id + 2 * j);
+            offer(sh, bound, there, __uint_as_float(q.x & 0xffff0000u), id + 2 * j + 1);
+        }
+        q.x = q.y;
+        q.y = q.z;
+        q.z = q.w;
+    }
+}
+
+// The `top` best words of this CTA's part into sh.top, from the list (n_list entries offered).
+template <typename E, int NTH>
+__device__ __forceinline__ void finish_top(LpLists& sh, int top, int warps, float tmax, const unsigned char* rowp, int lo,
+                                           int n, int nh, int nv, const uint4* vp) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __syncthreads();
+    if (sh.n_list > LP_CAP) {  // again, with the bound that all maxima give
+        const float bound = top_bound<NTH>(sh, top, warps, tmax);
+        if (tid == 0) sh.n_list = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int b = warp * 32; b < nv; b += NTH) {
+            if (*reinterpret_cast<volatile int*>(&sh.n_list) > LP_CAP) break;
+            const int v = b + lane;
+            offer_vec<E>(sh, bound, v < nv, v < nv ? ldg_stream(vp + v) : LpElem<E>::nothing(), lo + nh + v * LpElem<E>::EPV);
+        }
+        if (warp == 0) {  // the ragged ends: fewer than 16 elements
+            const int tail = n - nh - nv * LpElem<E>::EPV;
+            const int i = lane < 16 ? (lane < nh ? lane : n) : (lane - 16 < tail ? n - tail + lane - 16 : n);
+            offer(sh, bound, i < n, i < n ? LpElem<E>::ld(rowp, lo + i) : 0.0f, lo + i);
+        }
+        __syncthreads();
+        if (sh.n_list > LP_CAP) exact_top<E, NTH>(sh, rowp, lo, n, top);
+    } else if (sh.n_list < top && warp == 0) {
         // every finite element is listed; the masked ones follow in id order
         int have = sh.n_list;
         __syncwarp();
-        const int need = min(a.top, n);
+        const int need = min(top, n);
         for (int b = 0; b < n && have < need; b += 32) {
             const bool tie = b + lane < n && LpElem<E>::ld(rowp, lo + b + lane) == f_ninf();
             const uint32_t who = __ballot_sync(0xffffffffu, tie);
@@ -389,14 +452,14 @@ __device__ __forceinline__ void part_top(LpShared<NTH>& sh, const LpArgs& a, con
         if (lane == 0) sh.n_list = have;
     }
     __syncthreads();
-    order_words<NTH>(sh.list, sh.n_list, sh.top, a.top);
+    order_words<NTH>(sh.list, sh.n_list, sh.top, top);
 }
 
 template <typename E, int NTH, bool TOP>
 __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const LpArgs a) {
     constexpr int EPV = LpElem<E>::EPV, ES = 16 / EPV, WARPS = NTH / 32;
     constexpr int VPC = LP_U * NTH;  // vectors per chunk
-    __shared__ LpShared<NTH> sh;
+    __shared__ LpShared<NTH, TOP> sh;
     extern __shared__ __align__(128) unsigned char ring[];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
@@ -425,6 +488,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         }
         fence_mbar_init();
         sh.failed = 0;
+        if constexpr (TOP) sh.n_list = sh.bound = 0;
     }
     pdl_wait_then_release();
     if (tid == 0)
@@ -450,30 +514,49 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
 
     int slot = 0;
     uint32_t ph = 0;
+    float bound = 0.0f;
+    const int warps = min(WARPS, (max(nv, 64) + 31) / 32);  // warps that hold something (the ragged ends: two)
+    bool bad = false;  // a wait gave up: nothing more is read, the barriers are still met
     for (int k = 0; k < chunks; ++k) {
         // refill the chunk before this one: its readers have had a whole chunk's time
-        if (tid == 0 && k > 0 && k - 1 + a.stages < chunks) {
+        if (tid == 0 && k > 0 && k - 1 + a.stages < chunks && !bad) {
             const int ps = (k - 1) % a.stages;
             if (mbar_wait_bounded(&sh.empty[ps], (uint32_t)((k - 1) / a.stages) & 1u, LP_WAIT_NS)) load_chunk(k - 1 + a.stages);
             else sh.failed = 1;
         }
-        if (!mbar_wait_bounded(&sh.full[slot], ph, LP_WAIT_NS)) {
+        if (!bad && !mbar_wait_bounded(&sh.full[slot], ph, LP_WAIT_NS)) {
             sh.failed = 1;
-            break;
+            bad = true;
         }
         const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)slot * VPC * 16);
-        uint4 q[LP_U];
+        const int left = bad ? 0 : nv - k * VPC;  // vectors of this chunk
+        float bm;
+        {
+            uint4 q[LP_U];
 #pragma unroll
-        for (int u = 0; u < LP_U; ++u) {
-            const int v = tid + u * NTH;
-            q[u] = k * VPC + v < nv ? buf[v] : LpElem<E>::nothing();
+            for (int u = 0; u < LP_U; ++u) {
+                const int v = tid + u * NTH;
+                q[u] = v < left ? buf[v] : LpElem<E>::nothing();
+            }
+            bm = LpElem<E>::batch_max(q);
+            lp_thread_batch<E>(s, q, bm, a.c);
+            // the vector that holds the token counts as behind it here
+#pragma unroll
+            for (int u = 0; u < LP_U; ++u)
+                cnt += LpElem<E>::count_above(q[u], k * VPC + tid + u * NTH < tv ? thr_before : thr_after);
         }
-        const float bm = LpElem<E>::batch_max(q);
-        lp_thread_batch<E>(s, q, bm, a.c);
-        // the vector that holds the token counts as behind it here
-#pragma unroll
-        for (int u = 0; u < LP_U; ++u)
-            cnt += LpElem<E>::count_above(q[u], k * VPC + tid + u * NTH < tv ? thr_before : thr_after);
+        if constexpr (TOP) {
+            if (chunks > a.stages) {
+                if (k == 0 || k == 3 || (k & 15) == 15) bound = top_bound<NTH>(sh, a.top, warps, s.m);
+                // the shares that reach it, an element per lane
+                for (uint32_t hits = __ballot_sync(0xffffffffu, reaches(bm, bound)); hits; hits &= hits - 1) {
+                    const int v = (tid & ~31) + __ffs(hits) - 1 + lane / EPV * NTH;
+                    const bool there = lane < LP_U * EPV && v < left;
+                    const float x = there ? LpElem<E>::ld_shared(buf + v, lane % EPV) : 0.0f;
+                    offer(sh, bound, there, x, i0 + (k * VPC + v) * EPV + lane % EPV);
+                }
+            }
+        }
         if (chunks > a.stages) {
             __syncwarp();
             if (lane == 0)
@@ -497,7 +580,27 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         }
     }
     const float tmax = s.m;  // this thread's maximum (NaN if it saw one)
-
+    if constexpr (TOP) {
+        if (chunks <= a.stages) {  // the whole part lies in shared memory
+            bound = top_bound<NTH>(sh, a.top, warps, tmax);
+            const uint4* buf = reinterpret_cast<const uint4*>(ring);
+            for (uint32_t hits = __ballot_sync(0xffffffffu, reaches(tmax, bound)); hits; hits &= hits - 1) {
+                // a vector of the thread's share per lane (at most 24), then the elements of those that reach it
+                const int v = (tid & ~31) + __ffs(hits) - 1 + lane * NTH;
+                const bool there = v < nv && !bad;
+                for (uint32_t vecs = __ballot_sync(0xffffffffu, there && reaches(LpElem<E>::vec_max(buf[there ? v : 0]), bound));
+                     vecs; vecs &= vecs - 1) {
+                    const int w = (tid & ~31) + __ffs(hits) - 1 + (__ffs(vecs) - 1) * NTH, j = lane & (EPV - 1);
+                    offer(sh, bound, lane < EPV, LpElem<E>::ld_shared(buf + w, j), i0 + w * EPV + j);
+                }
+            }
+        }
+        if (warp < 2) {  // the ragged ends
+            const bool head = tid < nh, tail = tid >= 32 && tid < 32 + nt;
+            const int id = head ? lo + tid : hi - nt + tid - 32;
+            offer(sh, bound, head || tail, head || tail ? LpElem<E>::ld(rowp, id) : 0.0f, id);
+        }
+    }
     // the CTA's maximum (NaN wins), then sums relative to it
     float m = s.m;
     {
@@ -527,13 +630,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         sh.wU[warp] = U;
         sh.wcount[warp] = cnt;
     }
-    if (TOP) {
-        if (chunks <= a.stages && !sh.failed)
-            part_top<E, NTH>(sh, a, rowp, lo, n, nh, nv, nt, tmax,
-                             [&](int v) { return reinterpret_cast<const uint4*>(ring)[v]; });
-        else
-            part_top<E, NTH>(sh, a, rowp, lo, n, nh, nv, nt, tmax, [&](int v) { return ldg_stream(vp + v); });
-    }
+    if constexpr (TOP) finish_top<E, NTH>(sh, a.top, warps, tmax, rowp, lo, n, nh, nv, vp);
     __syncthreads();
     LpState w;
     w.m = m;
@@ -553,7 +650,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         cluster.sync();
         if (crank == 0)
             for (int k = 1; k < C; ++k) {
-                const LpShared<NTH>* o = cluster.map_shared_rank(&sh, k);
+                const LpShared<NTH, TOP>* o = cluster.map_shared_rank(&sh, k);
                 w = lp_merge(w, o->total, a.c);
                 c2 += o->total_count;
             }
@@ -567,7 +664,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
             if (a.stats) a.stats[r] = make_float4(f.m, f.R, f.log2S, f.entropy);
             if (a.status && tok >= a.V) atomicOr(a.status, B2S_STATUS_TOKEN_RANGE);
         }
-        if (TOP) {
+        if constexpr (TOP) {
             // the cluster's lists (C x top words, each in order) into one
             int n_all = a.top;
             const unsigned long long* src = sh.top;
@@ -578,14 +675,10 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
                 src = sh.list;
                 __syncthreads();
             }
-            for (int i = tid; i < n_all; i += NTH) {
-                const unsigned long long w64 = src[i];
-                int rk = i;
-                if (C > 1) {
-                    rk = 0;
-                    for (int j = 0; j < n_all; ++j) rk += src[j] > w64;
-                }
-                if (w64 != 0ull && rk < a.top) {
+            for (int b = 0; b < n_all; b += NTH / 8) {
+                const int i = b + (tid >> 3), rk = C > 1 ? rank_of(src, n_all, i) : i;
+                const unsigned long long w64 = i < n_all ? src[i] : 0ull;
+                if ((tid & 7) == 0 && w64 != 0ull && rk < a.top) {
                     const uint32_t key = (uint32_t)(w64 >> 32);
                     const float x = key == 0xffffffffu ? __int_as_float(0x7fffffff) : okey_to_f(key);
                     a.top_ids[(int64_t)r * a.top + rk] = word_id(w64);
@@ -687,18 +780,26 @@ cudaError_t launch(K kernel, int64_t blocks, int threads, uint32_t smem, int clu
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// The forward kernel on `rows` rows, C CTAs of NTH threads each; the ring holds the whole part where it fits, else as
-// many chunks as let two CTAs (1024 threads) share an SM's shared memory.
+// The forward kernel on `rows` rows, C CTAs of NTH threads each.  A ring of three chunks keeps the copies going (96 KB of
+// 512 threads, 24 KB of 128: all 1024 threads that the registers allow fit an SM); with alternatives the whole part where
+// it fits 96 KB of 512 threads (192 where an SM has one CTA anyway) or 48 of 128 (four CTAs an SM).
 template <typename E, int NTH, bool TOP>
-cudaError_t launch_rows(LpArgs a, int rows, int C, int es, void* stream) {
+cudaError_t launch_rows(LpArgs a, int rows, int C, int es, int sms, void* stream) {
     constexpr uint32_t CHUNK = LP_U * NTH * 16;
-    constexpr int MOST = NTH == 128 ? 12 : 3;  // 96 KB
     a.per = ((a.V + C - 1) / C + 15) / 16 * 16;
     const int chunks = (int)(((int64_t)a.per * es + CHUNK - 1) / CHUNK);
-    a.stages = chunks < 1 ? 1 : (chunks > MOST ? MOST : chunks);
+    a.stages = chunks < 3 ? (chunks < 1 ? 1 : chunks) : 3;
+    if (TOP && chunks <= (NTH == 128 || (int64_t)rows * C <= sms ? 6 : 3)) a.stages = chunks < 1 ? 1 : chunks;
     const auto kernel = token_logprobs_kernel<E, NTH, TOP>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MOST * CHUNK));
+    static std::atomic<bool> set[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_relaxed)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(6 * CHUNK));
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
+    }
     return launch(kernel, (int64_t)rows * C, NTH, a.stages * CHUNK, C, stream, a);
 }
 
@@ -743,17 +844,17 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     const int64_t row_bytes = (int64_t)vocab * es;
     cudaError_t e;
     if (rows >= 2 * sms && row_bytes <= 64 * 1024) {
-        e = top ? (bf ? launch_rows<__nv_bfloat16, 128, true>(a, rows, 1, es, stream)
-                      : launch_rows<float, 128, true>(a, rows, 1, es, stream))
-                : (bf ? launch_rows<__nv_bfloat16, 128, false>(a, rows, 1, es, stream)
-                      : launch_rows<float, 128, false>(a, rows, 1, es, stream));
+        e = top ? (bf ? launch_rows<__nv_bfloat16, 128, true>(a, rows, 1, es, sms, stream)
+                      : launch_rows<float, 128, true>(a, rows, 1, es, sms, stream))
+                : (bf ? launch_rows<__nv_bfloat16, 128, false>(a, rows, 1, es, sms, stream)
+                      : launch_rows<float, 128, false>(a, rows, 1, es, sms, stream));
     } else {
         int C = 1;
         while (C < 8 && (int64_t)rows * C * 2 <= 2 * sms && row_bytes / (C * 2) >= 16 * 1024) C <<= 1;
-        e = top ? (bf ? launch_rows<__nv_bfloat16, 512, true>(a, rows, C, es, stream)
-                      : launch_rows<float, 512, true>(a, rows, C, es, stream))
-                : (bf ? launch_rows<__nv_bfloat16, 512, false>(a, rows, C, es, stream)
-                      : launch_rows<float, 512, false>(a, rows, C, es, stream));
+        e = top ? (bf ? launch_rows<__nv_bfloat16, 512, true>(a, rows, C, es, sms, stream)
+                      : launch_rows<float, 512, true>(a, rows, C, es, sms, stream))
+                : (bf ? launch_rows<__nv_bfloat16, 512, false>(a, rows, C, es, sms, stream)
+                      : launch_rows<float, 512, false>(a, rows, C, es, sms, stream));
     }
     return e == cudaSuccess ? B2S_OK : cuda_fail(e);
 }
