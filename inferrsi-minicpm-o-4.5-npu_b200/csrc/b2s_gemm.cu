@@ -64,13 +64,12 @@ __device__ __forceinline__ void residual_fetch(const GemmArgs& a, uint32_t (&q)[
 // The epilogue of one warp: 32 rows of a tile, columns [n0, n0 + COLS) from tensor memory at `tm` (lane = row).  `rq`:
 // the residual's first block.
 template <int TM, int TN, int EPI>
-__device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, int row0, int n0, int half, int nt, int slot,
+__device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, int row0, int n0, int nt, int slot,
                                               unsigned char* st, uint32_t (&rq)[16]) {
     constexpr int COLS = TN / 2;
-    const int lane = threadIdx.x & 31, row = row0 + lane;
-    const bool live = row < a.M;
+    const int lane = threadIdx.x & 31;
     const int rows = min(32, a.M - row0);  // <= 0: a warp past the last row
-    if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
+    {
         if (slot >= 0) {  // a chunk of a split tile: its fp32 sums as they are
             const int held = min(a.M, TM);
             float* dst = a.partial + ((int64_t)slot * held + row0 % TM) * TN + n0 - nt * TN;
@@ -145,49 +144,56 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
                             rows, cols, vec_block(a, n, 1));
             __syncwarp();
         }
-    } else if constexpr (EPI == EPI_LSE) {
-        const int64_t tok = live ? a.tokens[row] : -1;
+    }
+}
+
+// The head's epilogues: this lane's row of COLS fp32 logits (before the temperature) from column n0.
+template <int COLS, int EPI>
+__device__ __forceinline__ void epilogue_logits(const GemmArgs& a, const float (&v)[COLS], int row0, int n0, int half, int nt,
+                                                unsigned char* st) {
+    const int lane = threadIdx.x & 31, row = row0 + lane;
+    const bool live = row < a.M;
+    const int64_t tok = live ? a.tokens[row] : -1;
+    if constexpr (EPI == EPI_LSE) {
         LpState s;
         s.m = f_ninf();
         s.S = s.U = 0.0f;
-#pragma unroll 1
+        if (tok >= n0 && tok < min(n0 + COLS, a.N)) {
+            float tv = v[0];
+#pragma unroll
+            for (int j = 1; j < COLS; ++j) tv = tok == n0 + j ? v[j] : tv;
+            a.token_value[row] = tv;
+        }
+#pragma unroll
         for (int q = 0; q < COLS / 32; ++q) {
             const int n = n0 + 32 * q;
-            if (n >= a.N) break;
-            float v[32];
-            tmem_ld32(tm + 32u * q, v);
-            if (tok >= n && tok < min(n + 32, a.N)) {
-                float tv = v[0];
+            if (n < a.N) {
+                float x[32];
 #pragma unroll
-                for (int j = 1; j < 32; ++j) tv = tok == n + j ? v[j] : tv;
-                a.token_value[row] = tv;
+                for (int j = 0; j < 32; ++j) x[j] = n + j < a.N ? v[32 * q + j] : f_ninf();
+                lp_add_any<32>(s, x, a.c);
             }
-            if (n + 32 > a.N) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = n + j < a.N ? v[j] : f_ninf();
-            }
-            lp_add_any<32>(s, v, a.c);
         }
         if (live) a.part[((int64_t)row * a.tiles_n + nt) * 2 + half] = make_float4(s.m, s.S, s.U, 0.0f);
     } else {
-        const int64_t tok = live ? a.tokens[row] : -1;
+        const int rows = min(32, a.M - row0);
         const float4 stt = live ? a.stats[row] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const LpGrad g(stt, tok >= 0 && tok < a.N ? (int)tok : -1, live && a.g_lp ? a.g_lp[row] : 0.0f,
                        live && a.g_h ? a.g_h[row] : 0.0f, a.inv_t);
         unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride;
-#pragma unroll 1
+#pragma unroll
         for (int q = 0; q < COLS / 32; ++q) {
             const int n = n0 + 32 * q, cols = a.N - n;
-            if (cols <= 0) break;
-            float v[32];
-            tmem_ld32(tm + 32u * q, v);
+            if (cols > 0) {
+                float x[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = g.at(v[j], n + j, a.c);
-            // dz is rounded to bf16 once: it is the tensor cores' operand in both gradient products
-            stage_row(st, 0, v);
-            __syncwarp();
-            block_store(st, 0, out + n, a.out_stride, rows, cols, vec_block(a, n, 1));
-            __syncwarp();
+                for (int j = 0; j < 32; ++j) x[j] = g.at(v[32 * q + j], n + j, a.c);
+                // dz is rounded to bf16 once: it is the tensor cores' operand in both gradient products
+                stage_row(st, 0, x);
+                __syncwarp();
+                block_store(st, 0, out + n, a.out_stride, rows, cols, vec_block(a, n, 1));
+                __syncwarp();
+            }
         }
     }
 }
@@ -197,7 +203,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                 const __grid_constant__ GemmArgs a) {
     constexpr int TM = CG * GM_M, BN = TN / CG;  // rows of a tile; this CTA's columns of B
-    constexpr int ST = gm_stages(CG, TN);
+    constexpr int ST = gm_stages(CG, TN), SEGMENT = EPI == EPI_LSE || EPI == EPI_DZ ? GM_SEGMENT : 1 << 24;
     constexpr uint32_t STAGE = gm_stage_bytes(CG, TN);
     constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)AMN << 15) | ((uint32_t)BMN << 16) |
                                ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
@@ -315,41 +321,45 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                 else umma_commit(bar);
             };
             Piece p;
+            int g = 0;  // accumulators handed over
             for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
-                const int acc = i & 1;
-                if (i >= 2 && !gm_wait<CG == 2>(&tempty[acc], (uint32_t)(i / 2 - 1) & 1u)) {
-                    *fail = 1;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(acc * TN);
-                uint32_t more = 0;
-                for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
-                    if (!gm_wait<false>(&full[s], ph)) {
+                for (int k0 = p.kb0; ok && k0 < p.kb1; k0 += SEGMENT, ++g) {
+                    const int acc = g & 1, k1 = min(p.kb1, k0 + SEGMENT);
+                    if (g >= 2 && !gm_wait<CG == 2>(&tempty[acc], (uint32_t)(g / 2 - 1) & 1u)) {
                         *fail = 1;
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    if (elect_one()) {
-                        // a stage is STAGE bytes on, a step of 16 k 32 bytes (k contiguous) or 2 KB, in units of 16
-                        const uint64_t da = da0 + (uint32_t)s * (STAGE >> 4), db = db0 + (uint32_t)s * (STAGE >> 4);
-#pragma unroll
-                        for (int k = 0; k < GM_KB / 16; ++k) {
-                            if constexpr (CG == 2)
-                                umma_bf16_pair(d, da + (AMN ? 128 : 2) * k, db + (BMN ? 128 : 2) * k, IDESC, more);
-                            else
-                                umma_bf16(d, da + (AMN ? 128 : 2) * k, db + (BMN ? 128 : 2) * k, IDESC, more);
-                            more = 1;
+                    const uint32_t d = tmem + (uint32_t)(acc * TN);
+                    uint32_t more = 0;
+                    for (int kb = k0; kb < k1; ++kb, ++it) {
+                        if (!gm_wait<false>(&full[s], ph)) {
+                            *fail = 1;
+                            ok = false;
+                            break;
                         }
-                        commit(&empty[s]);
-                        if (kb + 1 == p.kb1) commit(&tfull[acc]);
-                    }
-                    more = 1;
-                    __syncwarp();
-                    if (++s == ST) {
-                        s = 0;
-                        ph ^= 1;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            // a stage is STAGE bytes on, a step of 16 k 32 bytes (k contiguous) or 2 KB, in units of 16
+                            const uint64_t da = da0 + (uint32_t)s * (STAGE >> 4), db = db0 + (uint32_t)s * (STAGE >> 4);
+#pragma unroll
+                            for (int k = 0; k < GM_KB / 16; ++k) {
+                                if constexpr (CG == 2)
+                                    umma_bf16_pair(d, da + (AMN ? 128 : 2) * k, db + (BMN ? 128 : 2) * k, IDESC, more);
+                                else
+                                    umma_bf16(d, da + (AMN ? 128 : 2) * k, db + (BMN ? 128 : 2) * k, IDESC, more);
+                                more = 1;
+                            }
+                            commit(&empty[s]);
+                            if (kb + 1 == k1) commit(&tfull[acc]);
+                        }
+                        more = 1;
+                        __syncwarp();
+                        if (++s == ST) {
+                            s = 0;
+                            ph ^= 1;
+                        }
                     }
                 }
             }
@@ -362,24 +372,52 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         }
     } else {
         Piece p;
-        for (int i = 0; piece_at<CG>(a, i, &p); ++i) {
+        int g = 0;
+        bool ok = true;
+        const int half = warp >> 2;
+        const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * (TN / 2));
+        auto take = [&]() {  // the next accumulator
+            ok = __all_sync(0xffffffffu, gm_wait<false>(&tfull[g & 1], (uint32_t)(g / 2) & 1u)) && !*fail;
+            if (!ok) *fail = 1;
+            tc_fence_after();
+            return ok;
+        };
+        auto give = [&]() {
+            tc_fence_before();
+            if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[g & 1]), 0));
+            else mbar_arrive(&tempty[g & 1]);
+            ++g;
+        };
+        for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
             int mt, nt;
             tile_of<TM>(a, p.tile, &mt, &nt);
-            const int acc = i & 1, half = warp >> 2;
             const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32, n0 = nt * TN + half * (TN / 2);
-            uint32_t rq[16];
-            if (EPI == EPI_LINEAR && p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
-            const bool ok = gm_wait<false>(&tfull[acc], (uint32_t)(i / 2) & 1u);
-            if (!__all_sync(0xffffffffu, ok) || *fail) {
-                *fail = 1;
-                break;
+            if constexpr (EPI == EPI_LSE || EPI == EPI_DZ) {
+                float v[TN / 2];
+                if (!take()) break;
+#pragma unroll
+                for (int q = 0; q < TN / 64; ++q) tmem_ld32(tm + (uint32_t)((g & 1) * TN + 32 * q), v + 32 * q);
+                give();
+#pragma unroll 1
+                for (int k0 = p.kb0 + SEGMENT; k0 < p.kb1; k0 += SEGMENT) {
+                    if (!take()) break;
+#pragma unroll
+                    for (int q = 0; q < TN / 32; ++q) {
+                        uint32_t x[16];
+                        tmem_ld16(tm + (uint32_t)((g & 1) * TN + 16 * q), x);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[16 * q + j] += __uint_as_float(x[j]);
+                    }
+                    give();
+                }
+                if (ok) epilogue_logits<TN / 2, EPI>(a, v, row0, n0, half, nt, staging + warp * 4096);
+            } else {
+                uint32_t rq[16];
+                if (EPI == EPI_LINEAR && p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
+                if (!take()) break;
+                epilogue_rows<TM, TN, EPI>(a, tm + (uint32_t)((g & 1) * TN), row0, n0, nt, p.slot, staging + warp * 4096, rq);
+                give();
             }
-            tc_fence_after();
-            epilogue_rows<TM, TN, EPI>(a, tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(acc * TN + half * (TN / 2)),
-                                       row0, n0, half, nt, p.slot, staging + warp * 4096, rq);
-            tc_fence_before();
-            if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
-            else mbar_arrive(&tempty[acc]);
         }
     }
     __syncwarp();

@@ -42,6 +42,11 @@ __host__ __device__ constexpr uint32_t gm_smem(int cg, int tn) {
     return 1024 + gm_stages(cg, tn) * gm_stage_bytes(cg, tn) + GM_STAGING + 256;
 }
 
+// The head's logits are handed over every 1024 k and added in registers: the tensor cores' fp32 accumulation loses about a
+// truncation per MMA of what is summed so far, which over 4096 k put the log probabilities 1.6e-6 off (relative), and by
+// quarters a quarter of that.
+constexpr int GM_SEGMENT = 1024 / GM_KB;
+
 enum { EPI_LINEAR = 0, EPI_LSE = 1, EPI_DZ = 2, EPI_STORE = 3 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
 

@@ -11,8 +11,8 @@
 // and gradient 0; NaN or +inf anywhere makes the row NaN, as a softmax gives it.
 //
 // Forward, one pass over the row by bulk copies into a ring of shared-memory chunks (a thread's registers do not bound
-// the bytes in flight), 128 threads per row where rows are many and short, else 512 and a cluster of CTAs per row while
-// rows are few.  Two elements share one packed fp32 operation, and a bf16 pair one maximum and one comparison: about 6
+// the bytes in flight), 128 or 256 threads per row where rows are many, else 512 and a cluster of CTAs per row while rows
+// are few.  Two elements share one packed fp32 operation, and a bf16 pair one maximum and one comparison: about 6
 // instructions an element, so that bf16 rows stay bound by HBM.  The rank counts the elements before the token in (value
 // descending, id ascending) order: an element before the token counts when x >= x_t, i.e. x > pred(x_t), one after it
 // when x > x_t, so a vector needs one threshold.  Top alternatives: the
@@ -781,8 +781,8 @@ cudaError_t launch(K kernel, int64_t blocks, int threads, uint32_t smem, int clu
 }
 
 // The forward kernel on `rows` rows, C CTAs of NTH threads each.  A ring of three chunks keeps the copies going (96 KB of
-// 512 threads, 24 KB of 128: all 1024 threads that the registers allow fit an SM); with alternatives the whole part where
-// it fits 96 KB of 512 threads (192 where an SM has one CTA anyway) or 48 of 128 (four CTAs an SM).
+// 512 threads, 48 of 256, 24 of 128: all 1024 threads that the registers allow fit an SM); with alternatives the whole
+// part where it fits those, 48 KB of 128 threads (four CTAs an SM), or 192 of 512 where an SM has one CTA anyway.
 template <typename E, int NTH, bool TOP>
 cudaError_t launch_rows(LpArgs a, int rows, int C, int es, int sms, void* stream) {
     constexpr uint32_t CHUNK = LP_U * NTH * 16;
@@ -843,11 +843,18 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     const bool bf = logits_dtype == B2S_DTYPE_BF16;
     const int64_t row_bytes = (int64_t)vocab * es;
     cudaError_t e;
+    // Many rows: a CTA each, of 128 threads up to 64 KB (1065 rows of 31 KB: 512 threads 13.3 us, 128 11.9) and of 256 beyond
+    // (2048 rows of 297 KB: 512 threads 142 us, 128 132, 256 129).  Few rows: clusters of 512 threads.
     if (rows >= 2 * sms && row_bytes <= 64 * 1024) {
         e = top ? (bf ? launch_rows<__nv_bfloat16, 128, true>(a, rows, 1, es, sms, stream)
                       : launch_rows<float, 128, true>(a, rows, 1, es, sms, stream))
                 : (bf ? launch_rows<__nv_bfloat16, 128, false>(a, rows, 1, es, sms, stream)
                       : launch_rows<float, 128, false>(a, rows, 1, es, sms, stream));
+    } else if (rows >= 2 * sms) {
+        e = top ? (bf ? launch_rows<__nv_bfloat16, 256, true>(a, rows, 1, es, sms, stream)
+                      : launch_rows<float, 256, true>(a, rows, 1, es, sms, stream))
+                : (bf ? launch_rows<__nv_bfloat16, 256, false>(a, rows, 1, es, sms, stream)
+                      : launch_rows<float, 256, false>(a, rows, 1, es, sms, stream));
     } else {
         int C = 1;
         while (C < 8 && (int64_t)rows * C * 2 <= 2 * sms && row_bytes / (C * 2) >= 16 * 1024) C <<= 1;
