@@ -557,7 +557,7 @@ Plan plan_for(int M, int N, int64_t K, bool may_split, int sms) {
             int64_t cost = (p.waves + (p.rest ? 1 : 0)) * nkb * kb_cost;
             if (may_split && p.rest) {
                 const int64_t held = M < tm ? M : tm;
-                for (int64_t want = 2; want <= nkb && want <= 64; ++want) {
+                for (int64_t want = 2; want <= nkb && want <= 64; want += want < 4 ? 1 : want / 2) {  // 2 3 4 6 9 13 19 28 42 63
                     const int64_t chunk = ceil_div(nkb, want), split = ceil_div(nkb, chunk);
                     const int64_t bytes = split * p.rest * held * tn * 4;
                     const int64_t c = (p.waves * nkb + ceil_div(p.rest * split, U) * chunk) * kb_cost + 5000 + 2 * bytes / 3000;
@@ -676,12 +676,96 @@ __global__ void __launch_bounds__(LM_NT) lmhead_merge_kernel(const float4* part,
     }
 }
 
+// ------------------------------------------------------------------ the projection of few rows
+
+// out = act(x w^T + bias) + residual for at most R rows: a CTA of 4 warps per F output features, which deal the k between
+// them 8 at a time, every lane 16-byte loads of the weight (read once, past L1) and of the rows (from L1), fp32 sums joined
+// by shuffles and through shared memory.  Bound by the weight's read: the tensor cores' path needs a split along k, two
+// launches and 128-row tiles for the same bytes.
+constexpr int ROWS_NT = 128;
+template <int R, int F>
+__global__ void __launch_bounds__(ROWS_NT) linear_rows_kernel(const __grid_constant__ GemmArgs a, const void* x,
+                                                              int64_t x_stride, const void* w, int64_t w_stride, int K) {
+    __shared__ float red[ROWS_NT / 32][R * F];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n0 = (int)blockIdx.x * F;
+    pdl_wait_then_release();
+    const uint4* wp[F];
+    const uint4* xp[R];
+#pragma unroll
+    for (int f = 0; f < F; ++f)  // rows and features past the end repeat the last one; they are not stored
+        wp[f] = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(w) + (int64_t)min(n0 + f, a.N - 1) * w_stride);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        xp[r] = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(x) + (int64_t)min(r, a.M - 1) * x_stride);
+    float2 acc[R][F];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int f = 0; f < F; ++f) acc[r][f] = make_float2(0.0f, 0.0f);
+    auto wide = [](uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); };
+#pragma unroll 4
+    for (int v = tid; v < K / 8; v += ROWS_NT) {
+        uint4 q[F];
+#pragma unroll
+        for (int f = 0; f < F; ++f) q[f] = ldg_stream(wp[f] + v);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint4 u = __ldg(xp[r] + v);
+            const float2 x0 = wide(u.x), x1 = wide(u.y), x2 = wide(u.z), x3 = wide(u.w);
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                acc[r][f] = __ffma2_rn(x0, wide(q[f].x), acc[r][f]);
+                acc[r][f] = __ffma2_rn(x1, wide(q[f].y), acc[r][f]);
+                acc[r][f] = __ffma2_rn(x2, wide(q[f].z), acc[r][f]);
+                acc[r][f] = __ffma2_rn(x3, wide(q[f].w), acc[r][f]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            float t = acc[r][f].x + acc[r][f].y;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (lane == 0) red[warp][r * F + f] = t;
+        }
+    __syncthreads();
+    if (tid < R * F) {
+        const int r = tid / F, n = n0 + tid % F;
+        if (r < a.M && n < a.N) {
+            float t = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+            if (a.bias) t += bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + n));
+            if (a.preact) static_cast<__nv_bfloat16*>(a.preact)[(int64_t)r * a.pre_stride + n] = __float2bfloat16_rn(t);
+            t = act_apply(t, a.act);
+            if (a.residual) t += bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.residual) + (int64_t)r * a.res_stride + n));
+            static_cast<__nv_bfloat16*>(a.out)[(int64_t)r * a.out_stride + n] = __float2bfloat16_rn(t);
+        }
+    }
+}
+// Which projections take it.  Against the tensor cores' path (us): 1 x 768 x 4096 3.5 : 11.1, 1 x 4096 x 4096 7.7 : 13.0,
+// 4 x 4096 x 4096 12.2 : 13.0, 8 x 768 x 4096 5.5 : 11.5, but 8 x 4096 x 4096 20.9 : 13.8 and 8 x 6562 x 768 14.2 : 10.2 (the
+// rows are read from L1 and unpacked once per two features).
+bool few_rows(int rows, int N, int64_t K) {
+    return rows <= 2 || (rows <= 4 && N * K <= 1 << 24) || (rows <= 8 && N <= 2048 && N * K <= 1 << 22);
+}
+cudaError_t linear_rows(const GemmArgs& a, const void* x, int64_t xs, const void* w, int64_t ws, int K, void* stream) {
+    auto go = [&](auto kernel, int F) {
+        return launch_pdl(kernel, dim3((unsigned)((a.N + F - 1) / F)), ROWS_NT, 0, stream, a, x, xs, w, ws, K);
+    };
+    if (a.M == 1) return go(linear_rows_kernel<1, 1>, 1);
+    if (a.M == 2) return go(linear_rows_kernel<2, 1>, 1);
+    if (a.M <= 4) return go(linear_rows_kernel<4, 2>, 2);
+    return go(linear_rows_kernel<8, 2>, 2);
+}
+
 // ------------------------------------------------------------------ the projection's elementwise gradient
 
 // dz = dy act'(z) (bf16, rows dz_stride apart) and the sums of its columns over this CTA's rows, E columns of a row per
-// thread: 8 where dy's rows are 16-byte aligned, else 1, so that a warp's loads stay whole lines.  32 threads cover 32 E
-// columns, the 8 warps take rows in turn; the sums (fp32, of the unrounded dz) go to part[blockIdx.y][n], or, with one
-// part, straight to the bias gradient.
+// thread: 8 where dy's rows are 16-byte aligned, else 2, z and dz (whose rows always are) still as whole words.  32 threads
+// cover 32 E columns, the 8 warps take rows in turn; the sums (fp32, of the unrounded dz) go to part[blockIdx.y][n], or,
+// with one part, straight to the bias gradient.
 constexpr int DZ_NT = 256;
 template <int E>
 __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_t dy_stride, const void* z,
@@ -696,26 +780,32 @@ __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_
     if (n < N) {
 #pragma unroll 4
         for (int r = r0 + rl; r < r1; r += 8) {
-            const unsigned short* gp = static_cast<const unsigned short*>(dy) + (int64_t)r * dy_stride;
-            const unsigned short* zp = static_cast<const unsigned short*>(z) + (int64_t)r * z_stride;
+            const unsigned short* gp = static_cast<const unsigned short*>(dy) + (int64_t)r * dy_stride + n;
+            const unsigned short* zp = static_cast<const unsigned short*>(z) + (int64_t)r * z_stride + n;
+            float g[E], x[E];
             if constexpr (E == 8) {
-                float g[8];
-                load8(gp, n, N, true, g);
-                if (act != ACT_NONE) {
-                    float x[8];
-                    load8(zp, n, N, true, x);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] *= act_slope(x[j], act);
-                }
-                if (dz) store8(static_cast<unsigned short*>(dz) + (int64_t)r * dz_stride, n, N, true, g);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum[j] += g[j];
+                load8(gp, 0, N - n, true, g);
+                if (act != ACT_NONE) load8(zp, 0, N - n, true, x);
             } else {
-                float g = bf16_bits_to_f(__ldg(gp + n));
-                if (act != ACT_NONE) g *= act_slope(bf16_bits_to_f(__ldg(zp + n)), act);
-                if (dz) (static_cast<__nv_bfloat16*>(dz) + (int64_t)r * dz_stride)[n] = __float2bfloat16_rn(g);
-                sum[0] += g;
+                g[0] = bf16_bits_to_f(__ldg(gp));
+                g[1] = n + 1 < N ? bf16_bits_to_f(__ldg(gp + 1)) : 0.0f;
+                if (act != ACT_NONE) {  // z's rows are padded to a multiple of 8
+                    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(zp));
+                    x[0] = __uint_as_float(w << 16);
+                    x[1] = __uint_as_float(w & 0xffff0000u);
+                }
             }
+            if (act != ACT_NONE) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) g[j] *= n + j < N ? act_slope(x[j], act) : 0.0f;
+            }
+            if (dz) {
+                unsigned short* o = static_cast<unsigned short*>(dz) + (int64_t)r * dz_stride + n;
+                if constexpr (E == 8) store8(o, 0, N - n, true, g);
+                else *reinterpret_cast<uint32_t*>(o) = pack_bf16(g[0], g[1]);  // dz's rows are padded likewise
+            }
+#pragma unroll
+            for (int j = 0; j < E; ++j) sum[j] += g[j];
         }
     }
     if (!part && !db) return;
@@ -744,8 +834,8 @@ __global__ void linear_db_kernel(const float* part, int parts, int N, void* db) 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 // parts of the rows whose column sums are taken separately: enough CTAs to fill the GPU, at least 64 rows each
-int dz_parts(int rows, int N) {
-    const int64_t cols = (N + 255) / 256;
+int dz_parts(int rows, int N, bool vec) {
+    const int64_t cols = vec ? (N + 255) / 256 : (N + 63) / 64;
     int64_t p = (4 * 148 + cols - 1) / cols;
     if (p > (rows + 63) / 64) p = (rows + 63) / 64;
     return (int)(p < 1 ? 1 : p);
@@ -873,7 +963,7 @@ int b2s_lmhead_logprobs_grad(const b2s_lmhead_args* h, const float* stats, const
 int b2s_linear_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
     using namespace b2s;
     if (rows < 0 || in_features < 8 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
-    *bytes = rows ? plan_here(rows, out_features, in_features, true).bytes : 0;
+    *bytes = rows && !few_rows(rows, out_features, in_features) ? plan_here(rows, out_features, in_features, true).bytes : 0;
     return B2S_OK;
 }
 
@@ -909,6 +999,10 @@ int b2s_linear(const b2s_linear_args* l, void* stream) {
     a.preact = l->preact;
     a.pre_stride = l->preact_row_stride;
     a.partial = static_cast<float*>(l->workspace);
+    if (few_rows(l->rows, l->out_features, l->in_features)) {
+        const cudaError_t e = linear_rows(a, l->x, l->x_row_stride, l->weight, l->weight_row_stride, l->in_features, stream);
+        return e == cudaSuccess ? B2S_OK : cuda_fail(e);
+    }
     return gemm<false, false, EPI_LINEAR>({l->x, l->x_row_stride}, {l->weight, l->weight_row_stride}, l->in_features, a,
                                           stream);
 }
@@ -919,7 +1013,7 @@ int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_fea
     const int64_t r = rows > 0 ? rows : 1;
     const int64_t dx = plan_here((int)r, in_features, out_features, true).bytes;
     const int64_t dw = plan_here(out_features, in_features, r, true).bytes;
-    *bytes = up(r * up(out_features, 8) * 2, 256) + up((int64_t)dz_parts((int)r, out_features) * out_features * 4, 256) +
+    *bytes = up(r * up(out_features, 8) * 2, 256) + up((int64_t)dz_parts((int)r, out_features, true) * out_features * 4, 256) +
              up(dx > dw ? dx : dw, 256);
     return B2S_OK;
 }
@@ -953,14 +1047,14 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
     const bool direct = l->activation == B2S_ACT_NONE && dy_vec;
     const bool products = l->grad_x || l->grad_weight;
     Operand dz = {l->workspace, ldz};
-    const int parts = dz_parts(l->rows, l->out_features);
+    const int parts = dz_parts(l->rows, l->out_features, dy_vec);  // at most what the workspace holds
     float* part = reinterpret_cast<float*>(static_cast<unsigned char*>(l->workspace) + up((int64_t)l->rows * ldz * 2, 256));
     if (direct) dz = {l->grad_out, l->grad_out_row_stride};
     if ((products && !direct) || l->grad_bias) {
         const int per = (l->rows + parts - 1) / parts;
         const bool two = l->grad_bias && parts > 1;
-        const int width = dy_vec ? 256 : 32;  // columns per CTA
-        cudaError_t e = launch_pdl(dy_vec ? linear_dz_kernel<8> : linear_dz_kernel<1>,
+        const int width = dy_vec ? 256 : 64;  // columns per CTA
+        cudaError_t e = launch_pdl(dy_vec ? linear_dz_kernel<8> : linear_dz_kernel<2>,
                                    dim3((unsigned)((l->out_features + width - 1) / width), (unsigned)parts), DZ_NT, 0,
                                    stream, l->grad_out, l->grad_out_row_stride, l->preact, l->preact_row_stride,
                                    (int)l->activation, (int)l->rows, (int)l->out_features, per,

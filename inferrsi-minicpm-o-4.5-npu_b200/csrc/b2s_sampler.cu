@@ -1546,6 +1546,11 @@ static EncodeTiledFn encode_tiled_fn() {
             q == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<EncodeTiledFn>(f);
     });
+    // The driver encodes for the calling thread's current context, which a thread has none of before its first runtime
+    // call (autograd's device threads, whose allocations come from a cache): binds the current device's once per thread.
+    static thread_local int bound = -1;
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev != bound && cudaSetDevice(dev) == cudaSuccess) bound = dev;
     return fn;
 }
 

@@ -477,6 +477,35 @@ def test_head_streams_and_graph(pkg):
     del g
 
 
+def test_calls_from_a_new_thread(pkg):
+    """A thread whose first CUDA work is the call itself (its allocations come from the cache), as autograd's device
+    threads are: the products' tensor maps need a current context."""
+    import threading
+
+    h, w, t, T = exact_operands(16, 300, 64, 9)
+    greedy = pkg.thinker_sampler.LMHeadArgmax(w, 16)
+    calls = {"head": lambda: pkg.logprobs.LMHeadLogprobs(w)(h, t, temperature=T).logprob,
+             "linear": lambda: pkg.projection.linear(h, w), "greedy": lambda: greedy(h),
+             "logits": lambda: pkg.logprobs.token_logprobs((h @ w.t()), t, top=3).logprob}
+    want = {k: f().clone() for k, f in calls.items()}
+    torch.cuda.synchronize()
+    for k, f in calls.items():
+        got = []
+
+        def run():
+            try:
+                got.append(f())
+            except Exception as e:  # reported below, in the test's own thread
+                got.append(e)
+
+        th = threading.Thread(target=run)
+        th.start()
+        th.join()
+        torch.cuda.synchronize()
+        assert isinstance(got[0], torch.Tensor), (k, got[0])
+        assert torch.equal(got[0], want[k]), k
+
+
 def test_head_agrees_with_logits(pkg):
     """The head's form and the logits' form of the same rows, and the greedy step: the argmax has the largest logprob."""
     h, w, _, T = exact_operands(33, 6562, 768, 8)
