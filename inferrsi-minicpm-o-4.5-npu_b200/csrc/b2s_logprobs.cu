@@ -189,7 +189,8 @@ struct LpLists {
     uint32_t hist[256];
     uint32_t ctl[2];
     unsigned long long list[LP_CAP];
-    unsigned long long top[LP_MAX_TOP];  // this CTA's best, in order (0: none)
+    unsigned long long top[LP_MAX_TOP];      // this CTA's best, in order (0: none)
+    unsigned long long all[8 * LP_MAX_TOP];  // the cluster's, in its first CTA
 };
 struct LpNoLists {};
 template <int NTH, bool TOP>
@@ -200,8 +201,8 @@ struct LpShared : std::conditional_t<TOP, LpLists, LpNoLists> {
     float wS[WARPS], wU[WARPS];
     int wcount[WARPS];
     int failed;
-    LpState total;  // this CTA's state and count, read by the cluster's first CTA
-    int total_count;
+    LpState total[8];  // the cluster's states and counts, in its first CTA
+    int total_count[8];
 };
 
 struct LpArgs {
@@ -481,6 +482,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         mbar_arrive_expect_tx(&sh.full[s], (uint32_t)cnt * 16u);
         bulk_g2s(ring + (size_t)s * VPC * 16, vp + (int64_t)k * VPC, (uint32_t)cnt * 16u, &sh.full[s]);
     };
+    if (C > 1) cluster_arrive_relaxed();  // waited for before the first store to another CTA
     if (tid == 0) {
         for (int s = 0; s < a.stages; ++s) {
             mbar_init(&sh.full[s], 1);
@@ -642,17 +644,23 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         w.U += sh.wU[k];
         c2 += sh.wcount[k];
     }
-    if (C > 1) {
+    if (C > 1) {  // every CTA hands its state, count and best words to the first one
+        __syncwarp();
+        cluster_wait();
+        LpShared<NTH, TOP>* first = cluster.map_shared_rank(&sh, 0);
         if (tid == 0) {
-            sh.total = w;
-            sh.total_count = c2;
+            first->total[crank] = w;
+            first->total_count[crank] = c2;
         }
-        cluster.sync();
+        if constexpr (TOP)
+            if (tid < a.top) first->all[crank * a.top + tid] = sh.top[tid];
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait();
         if (crank == 0)
             for (int k = 1; k < C; ++k) {
-                const LpShared<NTH, TOP>* o = cluster.map_shared_rank(&sh, k);
-                w = lp_merge(w, o->total, a.c);
-                c2 += o->total_count;
+                w = lp_merge(w, sh.total[k], a.c);
+                c2 += sh.total_count[k];
             }
     }
     if (crank == 0) {
@@ -666,15 +674,8 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         }
         if constexpr (TOP) {
             // the cluster's lists (C x top words, each in order) into one
-            int n_all = a.top;
-            const unsigned long long* src = sh.top;
-            if (C > 1) {
-                n_all = C * a.top;
-                for (int i = tid; i < n_all; i += NTH)
-                    sh.list[i] = cluster.map_shared_rank(&sh, i / a.top)->top[i % a.top];
-                src = sh.list;
-                __syncthreads();
-            }
+            const int n_all = C * a.top;
+            const unsigned long long* src = C > 1 ? sh.all : sh.top;
             for (int b = 0; b < n_all; b += NTH / 8) {
                 const int i = b + (tid >> 3), rk = C > 1 ? rank_of(src, n_all, i) : i;
                 const unsigned long long w64 = i < n_all ? src[i] : 0ull;
@@ -694,7 +695,6 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
             mbar_wait_bounded(&sh.full[s2], 1u, LP_WAIT_NS);
         }
     }
-    if (C > 1) cluster.sync();  // the first CTA has read the others' shared memory
 }
 
 // dx for one chunk of a row per CTA.
