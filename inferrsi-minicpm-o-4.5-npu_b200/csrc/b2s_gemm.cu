@@ -531,10 +531,12 @@ struct Plan {
     int64_t bytes;  // of the split's workspace
 };
 // The cheapest cut by estimated clocks.  A k block costs a CTA its MMAs (measured without loads: 530 clocks for 256 or
-// 128 columns alike, 290 for 64) or its stage's way from L2 (64 bytes a clock; rows outside A are not fetched); an
-// epilogue that nothing overlaps costs about 8 clocks a column; a split costs a second launch, about 5000 clocks, and
-// its sums' way out and back, about 3000 bytes a clock over all SMs.
-Plan plan_for(int M, int N, int64_t K, bool may_split, int sms) {
+// 128 columns alike, 290 for 64) or its stage's way from L2 (64 bytes a clock; rows outside A are not fetched).  An
+// epilogue costs 14 clocks a column where it only stores, 40 with the projection's bias, activation, residual and
+// pre-activation, and is hidden under the next tile's k blocks except the last one's.  A split costs a second launch,
+// about 9000 clocks with its wait, and its sums' way out and back, about 3000 bytes a clock over all SMs.
+Plan plan_for(int M, int N, int64_t K, int epi, int sms) {
+    const bool may_split = epi == EPI_LINEAR || epi == EPI_STORE;
     Plan best = {};
     int64_t best_cost = INT64_MAX;
     const int64_t nkb = (K + GM_KB - 1) / GM_KB;
@@ -554,13 +556,19 @@ Plan plan_for(int M, int N, int64_t K, bool may_split, int sms) {
             p.rest = (int)(tiles % U);
             p.split = 1;
             p.chunk = (int)nkb;
-            int64_t cost = (p.waves + (p.rest ? 1 : 0)) * nkb * kb_cost;
+            const int64_t tail = (epi == EPI_LINEAR ? 40 : 14) * tn;
+            auto tiles_cost = [&](int64_t rounds, int64_t nk) {
+                const int64_t mine = nk * kb_cost;
+                return rounds ? mine + (rounds - 1) * (mine > tail ? mine : tail) + tail : 0;
+            };
+            int64_t cost = tiles_cost(p.waves + (p.rest ? 1 : 0), nkb);
             if (may_split && p.rest) {
                 const int64_t held = M < tm ? M : tm;
                 for (int64_t want = 2; want <= nkb && want <= 64; want += want < 4 ? 1 : want / 2) {  // 2 3 4 6 9 13 19 28 42 63
                     const int64_t chunk = ceil_div(nkb, want), split = ceil_div(nkb, chunk);
                     const int64_t bytes = split * p.rest * held * tn * 4;
-                    const int64_t c = (p.waves * nkb + ceil_div(p.rest * split, U) * chunk) * kb_cost + 5000 + 2 * bytes / 3000;
+                    const int64_t c = tiles_cost(p.waves, nkb) + ceil_div(p.rest * split, U) * chunk * kb_cost + 14 * tn + 9000 +
+                                      2 * bytes / 3000;
                     if (split > 1 && c < cost) {
                         cost = c;
                         p.split = (int)split;
@@ -570,7 +578,6 @@ Plan plan_for(int M, int N, int64_t K, bool may_split, int sms) {
                     }
                 }
             }
-            cost += 8 * tn;
             if (cost < best_cost) {
                 best_cost = cost;
                 best = p;
@@ -581,10 +588,10 @@ Plan plan_for(int M, int N, int64_t K, bool may_split, int sms) {
 }
 
 // The plan on the current device (without one, where only sizes are asked for, on a B200's 148 multiprocessors).
-Plan plan_here(int M, int N, int64_t K, bool may_split) {
+Plan plan_here(int M, int N, int64_t K, int epi) {
     int sms = 0;
     if (device_sms(&sms) != cudaSuccess || sms < 1) sms = 148;
-    return plan_for(M, N, K, may_split, sms);
+    return plan_for(M, N, K, epi, sms);
 }
 
 template <int CG, int TN, bool AMN, bool BMN, int EPI>
@@ -628,7 +635,7 @@ int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, const Pla
 
 template <bool AMN, bool BMN, int EPI>
 int gemm(const Operand& A, const Operand& B, int64_t K, const GemmArgs& a, void* stream) {
-    const Plan p = plan_here(a.M, a.N, K, EPI == EPI_LINEAR || EPI == EPI_STORE);
+    const Plan p = plan_here(a.M, a.N, K, EPI);
     if (p.cg == 2)
         return p.tn == 256 ? gemm_tn<2, 256, AMN, BMN, EPI>(A, B, K, a, p, stream)
                            : gemm_tn<2, 128, AMN, BMN, EPI>(A, B, K, a, p, stream);
@@ -858,7 +865,7 @@ extern "C" {
 int b2s_lmhead_logprobs_workspace(int32_t rows, int32_t vocab, int32_t hidden_dim, int64_t* bytes) {
     using namespace b2s;
     if (rows < 0 || vocab < 1 || hidden_dim < 8 || !bytes) return B2S_ERR_INVALID;
-    const int tn = plan_here(rows > 0 ? rows : 1, vocab, hidden_dim, false).tn;
+    const int tn = plan_here(rows > 0 ? rows : 1, vocab, hidden_dim, EPI_LSE).tn;
     *bytes = up((int64_t)rows * ((vocab + tn - 1) / tn) * 32 + (int64_t)rows * 4, 256);
     return B2S_OK;
 }
@@ -874,7 +881,7 @@ int b2s_lmhead_logprobs(const b2s_lmhead_args* h, float* logprob, float* entropy
     b2s_lmhead_logprobs_workspace(h->rows, h->vocab, h->hidden_dim, &need);
     if (!h->tokens || !h->workspace || h->workspace_bytes < need || !aligned16(h->workspace) || (stats && !aligned16(stats)))
         return B2S_ERR_INVALID;
-    const int tn = plan_here(h->rows, h->vocab, h->hidden_dim, false).tn;
+    const int tn = plan_here(h->rows, h->vocab, h->hidden_dim, EPI_LSE).tn;
     const int tiles = 2 * ((h->vocab + tn - 1) / tn);  // states per row: two halves of each column tile
     GemmArgs a;
     memset(&a, 0, sizeof(a));
@@ -898,7 +905,7 @@ int b2s_lmhead_logprobs_grad_workspace(int32_t rows, int32_t vocab, int32_t hidd
     using namespace b2s;
     if (rows < 0 || vocab < 1 || hidden_dim < 8 || !bytes) return B2S_ERR_INVALID;
     const int64_t r = rows > 0 ? rows : 1;
-    const int64_t dh = plan_here((int)r, hidden_dim, vocab, true).bytes, dw = plan_here(vocab, hidden_dim, r, true).bytes;
+    const int64_t dh = plan_here((int)r, hidden_dim, vocab, EPI_STORE).bytes, dw = plan_here(vocab, hidden_dim, r, EPI_STORE).bytes;
     *bytes = up(r * up(vocab, 8) * 2, 256) + up(dh > dw ? dh : dw, 256);
     return B2S_OK;
 }
@@ -963,7 +970,7 @@ int b2s_lmhead_logprobs_grad(const b2s_lmhead_args* h, const float* stats, const
 int b2s_linear_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
     using namespace b2s;
     if (rows < 0 || in_features < 8 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
-    *bytes = rows && !few_rows(rows, out_features, in_features) ? plan_here(rows, out_features, in_features, true).bytes : 0;
+    *bytes = rows && !few_rows(rows, out_features, in_features) ? plan_here(rows, out_features, in_features, EPI_LINEAR).bytes : 0;
     return B2S_OK;
 }
 
@@ -1011,8 +1018,8 @@ int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_fea
     using namespace b2s;
     if (rows < 0 || in_features < 8 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
     const int64_t r = rows > 0 ? rows : 1;
-    const int64_t dx = plan_here((int)r, in_features, out_features, true).bytes;
-    const int64_t dw = plan_here(out_features, in_features, r, true).bytes;
+    const int64_t dx = plan_here((int)r, in_features, out_features, EPI_STORE).bytes;
+    const int64_t dw = plan_here(out_features, in_features, r, EPI_STORE).bytes;
     *bytes = up(r * up(out_features, 8) * 2, 256) + up((int64_t)dz_parts((int)r, out_features, true) * out_features * 4, 256) +
              up(dx > dw ? dx : dw, 256);
     return B2S_OK;
