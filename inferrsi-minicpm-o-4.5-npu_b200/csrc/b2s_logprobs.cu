@@ -61,6 +61,7 @@ namespace {
 constexpr int LP_CAP = 512;      // candidate list entries per CTA
 constexpr int LP_GATHER = 64;    // thread maxima gathered per CTA, at most
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_KEPT = 128;     // words of the histogram's room
 constexpr int LP_U = 4;          // vectors per thread and chunk
 constexpr uint64_t LP_WAIT_NS = 250ull * 1000 * 1000;
 
@@ -186,7 +187,7 @@ struct LpLists {
     uint32_t bound;  // the last bound, 0: none
     int n_list;
     int ties[16];
-    uint32_t hist[256];
+    alignas(16) uint32_t hist[256];
     uint32_t ctl[2];
     unsigned long long list[LP_CAP];
     unsigned long long top[LP_MAX_TOP];      // this CTA's best, in order (0: none)
@@ -453,7 +454,28 @@ __device__ __forceinline__ void finish_top(LpLists& sh, int top, int warps, floa
         if (lane == 0) sh.n_list = have;
     }
     __syncthreads();
-    order_words<NTH>(sh.list, sh.n_list, sh.top, top);
+    const unsigned long long* list = sh.list;
+    int listed = sh.n_list;
+    if (listed > 2 * top + 64) {  // listed on the way, with lower bounds: what the last one leaves, where that is less
+        const float bound = top_bound<NTH>(sh, top, warps, tmax);
+        if (tid == 0) sh.n_list = 0;
+        __syncthreads();
+        unsigned long long* kept = reinterpret_cast<unsigned long long*>(sh.hist);  // the radix select is done with it
+        const unsigned long long least = (unsigned long long)rank_key(bound) << 32;
+        for (int b = 0; b < listed; b += NTH) {
+            const unsigned long long w = b + tid < listed ? sh.list[b + tid] : 0ull;
+            if (w >= least) {
+                const int at = atomicAdd(&sh.n_list, 1);
+                if (at < LP_KEPT) kept[at] = w;
+            }
+        }
+        __syncthreads();
+        if (sh.n_list <= LP_KEPT) {
+            list = kept;
+            listed = sh.n_list;
+        }
+    }
+    order_words<NTH>(list, listed, sh.top, top);
 }
 
 template <typename E, int NTH, bool TOP>
@@ -844,8 +866,9 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     const int64_t row_bytes = (int64_t)vocab * es;
     cudaError_t e;
     // Many rows: a CTA each, of 128 threads up to 64 KB (1065 rows of 31 KB: 512 threads 13.3 us, 128 11.9) and of 256 beyond
-    // (2048 rows of 297 KB: 512 threads 142 us, 128 132, 256 129).  Few rows: clusters of 512 threads.
-    if (rows >= 2 * sms && row_bytes <= 64 * 1024) {
+    // (2048 rows of 297 KB: 512 threads 142 us, 128 132, 256 129).  With alternatives 256 from 24 KB on, which leaves an SM
+    // its 1024 threads beside whole rows in shared memory.  Few rows: clusters of 512 threads.
+    if (rows >= 2 * sms && row_bytes <= (top ? 24 : 64) * 1024) {
         e = top ? (bf ? launch_rows<__nv_bfloat16, 128, true>(a, rows, 1, es, sms, stream)
                       : launch_rows<float, 128, true>(a, rows, 1, es, sms, stream))
                 : (bf ? launch_rows<__nv_bfloat16, 128, false>(a, rows, 1, es, sms, stream)
