@@ -853,6 +853,7 @@ int check_head(const void* hidden, int64_t hstride, const void* head, int64_t ws
     if (rows < 0 || V < 1 || H < 8 || H % 8 || hstride < H || hstride % 8 || wstride < H || wstride % 8)
         return B2S_ERR_INVALID;
     if (!lp_temperature_ok(temperature)) return B2S_ERR_INVALID;
+    if (rows > LP_MAX_SIZE || V > LP_MAX_SIZE || H > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
     if (rows && (!hidden || !head || !aligned16(hidden) || !aligned16(head))) return B2S_ERR_INVALID;
     return B2S_OK;
 }
@@ -979,6 +980,7 @@ int b2s_linear(const b2s_linear_args* l, void* stream) {
     if (!l || l->rows < 0 || l->out_features < 1 || l->in_features < 8 || l->in_features % 8 || l->activation < 0 ||
         l->activation > B2S_ACT_SILU)
         return B2S_ERR_INVALID;
+    if (l->rows > LP_MAX_SIZE || l->in_features > LP_MAX_SIZE || l->out_features > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
     if (l->rows == 0) return B2S_OK;
     if (!l->x || !l->weight || !l->out || !aligned16(l->x) || !aligned16(l->weight) || l->x_row_stride < l->in_features ||
         l->x_row_stride % 8 || l->weight_row_stride < l->in_features || l->weight_row_stride % 8 ||
@@ -1030,6 +1032,7 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
     if (!l || l->rows < 0 || l->out_features < 1 || l->in_features < 8 || l->in_features % 8 || l->activation < 0 ||
         l->activation > B2S_ACT_SILU || (l->grad_weight && !aligned16(l->grad_weight)))
         return B2S_ERR_INVALID;
+    if (l->rows > LP_MAX_SIZE || l->in_features > LP_MAX_SIZE || l->out_features > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
     if (l->rows == 0) {  // sums over no rows
         cudaError_t e = cudaSuccess;
         if (l->grad_weight)

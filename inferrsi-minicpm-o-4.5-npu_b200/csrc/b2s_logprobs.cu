@@ -43,16 +43,16 @@ namespace b2s {
 int cuda_fail(cudaError_t e);
 
 cudaError_t device_sms(int* sms) {
-    static int cached[64] = {};  // 0: not asked yet; a device's count never changes, so racing writers agree
+    static std::atomic<int> cached[64];  // 0: not asked yet; a device's count never changes, so racing writers agree
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64 && cached[dev] > 0) {
-        *sms = cached[dev];
+    if (dev >= 0 && dev < 64 && cached[dev].load(std::memory_order_relaxed) > 0) {
+        *sms = cached[dev].load(std::memory_order_relaxed);
         return cudaSuccess;
     }
     e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess && dev >= 0 && dev < 64) cached[dev] = *sms;
+    if (e == cudaSuccess && dev >= 0 && dev < 64) cached[dev].store(*sms, std::memory_order_relaxed);
     return e;
 }
 
@@ -839,7 +839,7 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     if (logits_dtype != B2S_DTYPE_F32 && logits_dtype != B2S_DTYPE_BF16) return B2S_ERR_INVALID;
     if (!lp_temperature_ok(temperature)) return B2S_ERR_INVALID;
     if (top > vocab) return B2S_ERR_INVALID;
-    if (top > LP_MAX_TOP) return B2S_ERR_UNSUPPORTED;
+    if (top > LP_MAX_TOP || vocab > LP_MAX_SIZE || rows > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
     if (rows == 0) return B2S_OK;
     if (!logits || (top && (!top_ids || !top_logprobs)) || (stats && (reinterpret_cast<uintptr_t>(stats) & 15)))
         return B2S_ERR_INVALID;
@@ -896,6 +896,7 @@ int b2s_token_logprobs_grad(const void* logits, int32_t logits_dtype, int32_t ro
     if (rows < 0 || vocab < 1 || row_stride < vocab || grad_row_stride < vocab) return B2S_ERR_INVALID;
     if (logits_dtype != B2S_DTYPE_F32 && logits_dtype != B2S_DTYPE_BF16) return B2S_ERR_INVALID;
     if (!lp_temperature_ok(temperature)) return B2S_ERR_INVALID;
+    if (vocab > LP_MAX_SIZE || rows > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
     if (rows == 0) return B2S_OK;
     const int es = logits_dtype == B2S_DTYPE_BF16 ? 2 : 4;
     if (!logits || !stats || !grad_logits || (reinterpret_cast<uintptr_t>(stats) & 15) ||

@@ -206,6 +206,9 @@ inline float lp_scale(float temperature) { return (float)(1.4426950408889634 / (
 // Temperatures whose scale is a normal number well inside fp32.
 inline bool lp_temperature_ok(float t) { return t >= 1e-6f && t <= 1e6f; }
 
+// Rows, ids and features of a call: indices rounded up to a tile stay within 32 bits.
+constexpr int LP_MAX_SIZE = 0x7fffffff - 4096;
+
 cudaError_t device_sms(int* sms);  // multiprocessors of the current device
 
 }  // namespace b2s

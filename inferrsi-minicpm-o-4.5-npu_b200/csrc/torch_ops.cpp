@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -926,6 +927,21 @@ const auto& linear_grad_op() {
     return op;
 }
 
+// Under stream capture: a leaf whose gradient accumulator an eager graph on another stream keeps alive would tie the
+// captured backward pass to that stream, which invalidates the capture deep in the engine.  Said here instead.
+void check_capture(at::TensorList leaves) {
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    for (const Tensor& t : leaves) {
+        if (!needs_grad(t) || !t.is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+        if (!node) continue;
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t.get_device()).unwrap(),
+                    "a backward pass cannot be captured while an eager graph of the same leaves is alive: let its outputs go "
+                    "first (run the warm-up on a side stream and keep none of its results)");
+    }
+}
+
 struct TokenLogprobsNode : public torch::autograd::Function<TokenLogprobsNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, double temperature,
                                  int64_t top, const optional<Tensor>& status) {
@@ -960,6 +976,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_autogr
         at::AutoDispatchBelowADInplaceOrView below;
         return token_logprobs_op().call(logits, tokens, temperature, top, want_stats, status);
     }
+    check_capture({logits});
     variable_list o = TokenLogprobsNode::apply(logits, tokens, temperature, top, status);
     return {o[0], o[1], o[2], o[3], o[4], o[5]};
 }
@@ -1000,6 +1017,7 @@ std::tuple<Tensor, Tensor, Tensor> lmhead_logprobs_autograd(const Tensor& hidden
         at::AutoDispatchBelowADInplaceOrView below;
         return lmhead_logprobs_op().call(hidden, head, tokens, temperature, want_stats, status);
     }
+    check_capture({hidden, head});
     variable_list o = HeadLogprobsNode::apply(hidden, head, tokens, temperature, status);
     return {o[0], o[1], o[2]};
 }
@@ -1048,6 +1066,7 @@ std::tuple<Tensor, Tensor> linear_autograd(const Tensor& x, const Tensor& weight
         at::AutoDispatchBelowADInplaceOrView below;
         return linear_op().call(x, weight, bias, residual, activation, want_preact, status);
     }
+    check_capture({x, weight, or_none(bias), or_none(residual)});
     variable_list o = LinearNode::apply(x, weight, bias, residual, activation, status);
     return {o[0], o[1]};
 }

@@ -165,6 +165,38 @@ def test_masks_ties_and_special_values(pkg, V, dtype):
     assert torch.equal(r.rank, plain(x, t)[2])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V", [(300, 6000), (300, 14_001), (310, 40_003), (160, 160_001), (3, 160_001)])
+def test_rows_that_defeat_the_bound(pkg, n, V, dtype):
+    """Many rows (one CTA each, of either size), where the first chunk's bound is no help: ascending values, ties beyond
+    the list, a masked beginning, NaN by the hundred."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = (torch.randn(n, V, device=DEV, generator=g) * 2).to(dtype)
+    i = torch.arange(V, device=DEV)
+    ninf, nan = float("-inf"), float("nan")
+    kinds = [i.to(dtype), -i.to(dtype), torch.full((V,), 0.5, device=DEV, dtype=dtype), (i % 7).to(dtype),
+             torch.where(i < V - 100, ninf, 1.0).to(dtype), torch.where(i < V // 2, ninf, (i % 1000).float()).to(dtype),
+             torch.where(i % 9 == 0, nan, 1.0).to(dtype), torch.where(i == V - 1, 3.0, ninf).to(dtype),
+             torch.where(i % (V // 600 + 1) == 0, 9.0, -9.0).to(dtype), torch.full((V,), ninf, device=DEV, dtype=dtype)]
+    for r in range(n):
+        if r % 2 == 0 or n < 10:
+            x[r] = kinds[(r // 2 if n >= 10 else r) % len(kinds)]
+    t = torch.randint(0, V, (n,), device=DEV, generator=g)
+    for top in (32, 1, 5):
+        r = pkg.logprobs.token_logprobs(x, t, top=top)
+        lp, H, rank, ids, vals, _, _ = plain(x, t, 1.0, top)
+        assert torch.equal(r.rank, rank)
+        assert torch.equal(r.top_ids, ids)
+        close(r.logprob, lp, s_eps(V) + 4 * EPS * lp.abs())
+        close(r.entropy, H, 2 * s_eps(V) * (2 + H.abs()))
+        close(r.top_logprobs, vals, s_eps(V) + 4 * EPS * vals.abs())
+    if n < 10:  # every kind in turn where rows are split over CTAs
+        for k in range(len(kinds)):
+            y = kinds[k][None].expand(2, V).contiguous()
+            r = pkg.logprobs.token_logprobs(y, t[:2], top=32)
+            assert torch.equal(r.top_ids, plain(y, t[:2], 1.0, 32)[3])
+
+
 def test_no_token_rows_and_status(pkg):
     x, t = rows_of(6, 501, torch.float32, 5)
     st = torch.zeros(1, dtype=torch.int32, device=DEV)
@@ -475,6 +507,39 @@ def test_head_streams_and_graph(pkg):
     for a, b in zip(out, eager):
         assert torch.equal(a, b)
     del g
+
+
+def test_capture_beside_a_live_eager_graph_is_refused(pkg):
+    """A leaf whose eager graph is alive: torch's engine would tie the captured backward pass to the eager stream and
+    invalidate the capture; the operators say so instead, and work once the eager graph is gone."""
+    x, t = rows_of(5, 300, torch.float32, 1)
+    h, w, t2, T = exact_operands(5, 300, 64, 1)
+    lx, lh, lw = (v.clone().requires_grad_(True) for v in (x, h, w))
+    calls = ((lambda: pkg.logprobs.token_logprobs(lx, t).logprob, (lx,)),
+             (lambda: pkg.logprobs.LMHeadLogprobs(lw)(lh, t2, temperature=T).logprob, (lh, lw)),
+             (lambda: pkg.projection.linear(lh, lw), (lh, lw)))
+    for f, leaves in calls:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            y = f()
+            want = [v.clone() for v in torch.autograd.grad(y, leaves, torch.ones_like(y))]
+        torch.cuda.current_stream().wait_stream(s)
+        del y
+        alive = f()
+        one = torch.ones_like(alive)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), capture_error_mode="thread_local"):
+                f()
+        del alive
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, capture_error_mode="thread_local"):
+            y = f()
+            got = torch.autograd.grad(y, leaves, one)
+        g.replay()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        del g, y
 
 
 def test_calls_from_a_new_thread(pkg):

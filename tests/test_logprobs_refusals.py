@@ -33,6 +33,7 @@ def test_token_logprobs_arguments(pkg):
                 dict(logits=ctypes.c_void_p(0x10001)), dict(dtype=0, logits=ctypes.c_void_p(0x10002))):
         assert call(**bad) == 1, bad
     assert call(top=33) == 2
+    assert call(rows=0x7fffffff) == 2 and call(vocab=0x7fffffff, stride=0x7fffffff) == 2  # indices beyond 32 bits
 
     def grad(dtype=1, rows=4, vocab=100, stride=100, T=1.0, stats=FAKE[2], out=FAKE[3], ostride=100):
         return lib.b2s_token_logprobs_grad(FAKE[0], dtype, rows, vocab, stride, FAKE[1], T, stats, FAKE[4], None, out,
@@ -70,6 +71,9 @@ def test_head_more_arguments(pkg):
     lib, nat = pkg._native.capi(), pkg._native
     a = _head(nat)
     assert lib.b2s_lmhead_logprobs(None, FAKE[4], FAKE[5], None, None) == 1
+    for big in (dict(rows=0x7fffffff), dict(vocab=0x7ffffff8)):
+        assert lib.b2s_lmhead_logprobs(ctypes.byref(_head(nat, **big)), FAKE[4], FAKE[5], None, None) == 2
+    assert lib.b2s_linear(ctypes.byref(nat.LinearArgs(**{**LINEAR_OK, "rows": 0x7fffffff})), None) == 2
     assert lib.b2s_lmhead_logprobs(ctypes.byref(a), FAKE[4], FAKE[5], ctypes.c_void_p(0x10008), None) == 1
     assert lib.b2s_lmhead_logprobs(ctypes.byref(_head(nat, rows=0)), FAKE[4], FAKE[5], None, None) == 0
     assert lib.b2s_lmhead_logprobs_grad(ctypes.byref(a), None, FAKE[4], FAKE[5], FAKE[7], FAKE[8], None) == 1
