@@ -143,34 +143,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* f) {
     for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
 }
 
-// Waits for the phase of `bar` with the given parity, for at most GM_WAIT clocks (false then).  The bound is kept with
-// the SM's own clock: a read of the global timer costs more than a k block's MMAs, and a wait per k block that took it
-// held the products to 740 clocks per k block whatever the tile's width.
-constexpr long long GM_WAIT = 500ll * 1000 * 1000;  // about a quarter of a second
-template <bool CLUSTER>
-__device__ __forceinline__ bool gm_try(uint64_t* bar, uint32_t parity) {
-    if constexpr (!CLUSTER) return mbar_try_wait(bar, parity);
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-template <bool CLUSTER>
-__device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity) {
-    if (gm_try<CLUSTER>(bar, parity)) return true;
-    const long long t0 = clock64();
-    do {
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i)
-            if (gm_try<CLUSTER>(bar, parity)) return true;
-    } while (clock64() - t0 < GM_WAIT);
-    return false;
-}
-
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;

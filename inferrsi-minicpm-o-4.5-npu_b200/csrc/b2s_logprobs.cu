@@ -63,7 +63,6 @@ constexpr int LP_GATHER = 64;    // thread maxima gathered per CTA, at most
 constexpr int LP_MAX_TOP = 32;
 constexpr int LP_KEPT = 128;     // words of the histogram's room
 constexpr int LP_U = 4;          // vectors per thread and chunk
-constexpr uint64_t LP_WAIT_NS = 250ull * 1000 * 1000;
 
 // The largest float below x (x not NaN); NaN for -inf, whose "x > pred" must hold for every element.
 __device__ __forceinline__ float pred_float(float x) {
@@ -545,10 +544,10 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         // refill the chunk before this one: its readers have had a whole chunk's time
         if (tid == 0 && k > 0 && k - 1 + a.stages < chunks && !bad) {
             const int ps = (k - 1) % a.stages;
-            if (mbar_wait_bounded(&sh.empty[ps], (uint32_t)((k - 1) / a.stages) & 1u, LP_WAIT_NS)) load_chunk(k - 1 + a.stages);
+            if (gm_wait<false>(&sh.empty[ps], (uint32_t)((k - 1) / a.stages) & 1u)) load_chunk(k - 1 + a.stages);
             else sh.failed = 1;
         }
-        if (!bad && !mbar_wait_bounded(&sh.full[slot], ph, LP_WAIT_NS)) {
+        if (!bad && !gm_wait<false>(&sh.full[slot], ph)) {
             sh.failed = 1;
             bad = true;
         }
@@ -713,15 +712,15 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
     if (sh.failed && tid == 0) {  // copies still in flight write this CTA's shared memory: wait for them
         if (a.status) atomicOr(a.status, B2S_STATUS_WAIT_TIMEOUT);
         for (int s2 = 0; s2 < a.stages; ++s2) {
-            mbar_wait_bounded(&sh.full[s2], 0u, LP_WAIT_NS);
-            mbar_wait_bounded(&sh.full[s2], 1u, LP_WAIT_NS);
+            gm_wait<false>(&sh.full[s2], 0u);
+            gm_wait<false>(&sh.full[s2], 1u);
         }
     }
 }
 
 // dx for one chunk of a row per CTA.
 constexpr int LPG_NT = 256;
-constexpr int LPG_U = 4;  // vectors in flight per thread
+constexpr int LPG_U = 8;  // vectors in flight per thread
 template <typename E>
 __global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void* logits, int64_t stride, int V,
                                                                      int chunk_vecs, int chunks, const int64_t* tokens,

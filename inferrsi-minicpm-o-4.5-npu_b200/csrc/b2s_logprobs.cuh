@@ -1,5 +1,5 @@
-// The running softmax statistics the log-probability kernels share (logits rows and the head's epilogue).
-// See b2s_logprobs.cu for the formulas; everything is in base 2, c = log2(e) / T.
+// What the log-probability kernels share (logits rows and the head's epilogue): the running softmax statistics and a
+// bounded wait.  See b2s_logprobs.cu for the formulas; everything is in base 2, c = log2(e) / T.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -9,6 +9,34 @@
 #include "b2s_device.cuh"
 
 namespace b2s {
+
+// Waits for the phase of `bar` with the given parity, for at most GM_WAIT clocks (false then).  The bound is kept with
+// the SM's own clock: a read of the global timer costs more than a k block's MMAs, and a wait per k block that took it
+// held the products to 740 clocks per k block whatever the tile's width.
+constexpr long long GM_WAIT = 500ll * 1000 * 1000;  // about a quarter of a second
+template <bool CLUSTER>
+__device__ __forceinline__ bool gm_try(uint64_t* bar, uint32_t parity) {
+    if constexpr (!CLUSTER) return mbar_try_wait(bar, parity);
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity) {
+    if (gm_try<CLUSTER>(bar, parity)) return true;
+    const long long t0 = clock64();
+    do {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (gm_try<CLUSTER>(bar, parity)) return true;
+    } while (clock64() - t0 < GM_WAIT);
+    return false;
+}
 
 // m: maximum of the raw values (NaN once one was seen); S = sum 2^y, U = sum 2^y y with y relative to ref(m).
 struct LpState {
