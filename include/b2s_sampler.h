@@ -349,7 +349,7 @@ int b2s_lmhead_logprobs_grad(const b2s_lmhead_args* args, const float* stats, co
 /*
  * Projection with everything in its epilogue (ABI 6): out = act(x[rows, in] x weight[out, in]^T + bias) + residual,
  * bf16 in and out, fp32 in between, rounded once.  in_features a multiple of 8, rows of x and weight 16-byte aligned;
- * bias (16-byte aligned), residual and preact are optional; preact receives x weight^T + bias in bf16, which
+ * bias (16-byte aligned), residual and preact are optional; preact receives x weight^T + bias in fp16, which
  * b2s_linear_grad needs when there is an activation.  `workspace`: b2s_linear_workspace bytes (may be 0).
  */
 #define B2S_ACT_NONE 0

@@ -110,9 +110,7 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
                 }
-                // the saved pre-activation is bf16, like the tensors around it: the slope taken from it is off by half a
-                // bf16 step of z times the activation's curvature, less than dz's own rounding to the tensor cores' bf16
-                if (a.preact) stage_row(st, 4, v);
+                if (a.preact) stage_preact(st, v);
                 if (a.act == ACT_RELU) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_RELU>(v[j]);
@@ -503,7 +501,7 @@ __global__ void __launch_bounds__(FIX_NT) gemm_join_kernel(const __grid_constant
             if (j < cols) {
                 if (bias) v[j] += bf16_bits_to_f(__ldg(bias + n + j));
                 if (a.preact)
-                    (static_cast<__nv_bfloat16*>(a.preact) + (int64_t)row * a.pre_stride + n)[j] = __float2bfloat16_rn(v[j]);
+                    (static_cast<unsigned short*>(a.preact) + (int64_t)row * a.pre_stride + n)[j] = preact_bits(v[j]);
                 v[j] = act_apply(v[j], a.act);
                 if (a.residual) v[j] += bf16_bits_to_f(__ldg(res + j));
             }
@@ -744,7 +742,7 @@ __global__ void __launch_bounds__(ROWS_NT) linear_rows_kernel(const __grid_const
         if (r < a.M && n < a.N) {
             float t = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
             if (a.bias) t += bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + n));
-            if (a.preact) static_cast<__nv_bfloat16*>(a.preact)[(int64_t)r * a.pre_stride + n] = __float2bfloat16_rn(t);
+            if (a.preact) static_cast<unsigned short*>(a.preact)[(int64_t)r * a.pre_stride + n] = preact_bits(t);
             t = act_apply(t, a.act);
             if (a.residual) t += bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.residual) + (int64_t)r * a.res_stride + n));
             static_cast<__nv_bfloat16*>(a.out)[(int64_t)r * a.out_stride + n] = __float2bfloat16_rn(t);
@@ -792,14 +790,19 @@ __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_
             float g[E], x[E];
             if constexpr (E == 8) {
                 load8(gp, 0, N - n, true, g);
-                if (act != ACT_NONE) load8(zp, 0, N - n, true, x);
+                if (act != ACT_NONE) {  // z's rows are padded to a multiple of 8
+                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(zp));
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < E; ++j) x[j] = preact_value((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+                }
             } else {
                 g[0] = bf16_bits_to_f(__ldg(gp));
                 g[1] = n + 1 < N ? bf16_bits_to_f(__ldg(gp + 1)) : 0.0f;
-                if (act != ACT_NONE) {  // z's rows are padded to a multiple of 8
+                if (act != ACT_NONE) {
                     const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(zp));
-                    x[0] = __uint_as_float(w << 16);
-                    x[1] = __uint_as_float(w & 0xffff0000u);
+                    x[0] = preact_value((unsigned short)w);
+                    x[1] = preact_value((unsigned short)(w >> 16));
                 }
             }
             if (act != ACT_NONE) {

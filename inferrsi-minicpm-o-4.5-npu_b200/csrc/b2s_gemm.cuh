@@ -19,6 +19,8 @@
 // waits (bounded) for copies and MMAs in flight, and sets B2S_STATUS_WAIT_TIMEOUT.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "b2s_head.cuh"
 #include "b2s_logprobs.cuh"
 
@@ -105,7 +107,9 @@ __device__ __forceinline__ float act_apply(float z, int act) {
     return act == ACT_RELU ? act_apply<ACT_RELU>(z)
                            : act == ACT_GELU ? act_apply<ACT_GELU>(z) : act == ACT_SILU ? act_apply<ACT_SILU>(z) : z;
 }
+// The slope of a pre-activation that came back from fp16: past 65504 (infinite there) it is what it is at 6e4.
 __device__ __forceinline__ float act_slope(float z, int act) {
+    z = fabsf(z) > 6.0e4f ? copysignf(6.0e4f, z) : z;
     if (act == ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
     if (act == ACT_GELU) {
         float e;
@@ -288,6 +292,23 @@ __device__ __forceinline__ void stage_row(unsigned char* st, int base, const flo
         *stage_at(st, lane, base + j) =
             make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
                        pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
+}
+
+// The saved pre-activation is fp16: the slope taken from it is off by 2^-12 of z times the activation's curvature, an
+// eighth of what bf16 would add to dz's own rounding to the tensor cores' bf16, and slopes are flat long before fp16's
+// range ends.  A positive value below its range stays positive (the rectifier's slope asks for the sign).
+__device__ __forceinline__ unsigned short preact_bits(float z) {
+    const unsigned short h = __half_as_ushort(__float2half_rn(z));
+    return z > 0.0f && h == 0 ? 1 : h;
+}
+__device__ __forceinline__ float preact_value(unsigned short h) { return __half2float(__ushort_as_half(h)); }
+__device__ __forceinline__ void stage_preact(unsigned char* st, const float (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+    auto two = [](float a, float b) { return (uint32_t)preact_bits(a) | (uint32_t)preact_bits(b) << 16; };
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        *stage_at(st, lane, 4 + j) = make_uint4(two(v[8 * j], v[8 * j + 1]), two(v[8 * j + 2], v[8 * j + 3]),
+                                                two(v[8 * j + 4], v[8 * j + 5]), two(v[8 * j + 6], v[8 * j + 7]));
 }
 
 // Up to 8 bf16 of a row from column n (N columns), `vec`: the row is 16-byte aligned and n a multiple of 8.

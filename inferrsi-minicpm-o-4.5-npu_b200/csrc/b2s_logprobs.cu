@@ -556,17 +556,26 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         float bm;
         {
             uint4 q[LP_U];
+            if (left >= VPC) {
 #pragma unroll
-            for (int u = 0; u < LP_U; ++u) {
-                const int v = tid + u * NTH;
-                q[u] = v < left ? buf[v] : LpElem<E>::nothing();
+                for (int u = 0; u < LP_U; ++u) q[u] = buf[tid + u * NTH];
+            } else {
+#pragma unroll
+                for (int u = 0; u < LP_U; ++u) q[u] = tid + u * NTH < left ? buf[tid + u * NTH] : LpElem<E>::nothing();
             }
             bm = LpElem<E>::batch_max(q);
             lp_thread_batch<E>(s, q, bm, a.c);
             // the vector that holds the token counts as behind it here
+            const int before = tv - k * VPC;  // vectors of this chunk before it
+            if (before <= 0 || before >= VPC) {
+                const typename LpElem<E>::Thr thr = before <= 0 ? thr_after : thr_before;
 #pragma unroll
-            for (int u = 0; u < LP_U; ++u)
-                cnt += LpElem<E>::count_above(q[u], k * VPC + tid + u * NTH < tv ? thr_before : thr_after);
+                for (int u = 0; u < LP_U; ++u) cnt += LpElem<E>::count_above(q[u], thr);
+            } else {
+#pragma unroll
+                for (int u = 0; u < LP_U; ++u)
+                    cnt += LpElem<E>::count_above(q[u], tid + u * NTH < before ? thr_before : thr_after);
+            }
         }
         if constexpr (TOP) {
             if (chunks > a.stages) {

@@ -781,7 +781,7 @@ std::tuple<Tensor, Tensor> linear_cuda(const Tensor& x_, const Tensor& weight_, 
         r = plain_rows(*residual);
     }
     Tensor out = fresh({R, N}, at::kBFloat16, x);
-    Tensor pre = fresh({want_preact ? R : 0, round8(N)}, at::kBFloat16, x);
+    Tensor pre = fresh({want_preact ? R : 0, round8(N)}, at::kHalf, x);
     b2s_linear_args a;
     memset(&a, 0, sizeof(a));
     a.x = x.data_ptr();
@@ -813,7 +813,7 @@ std::tuple<Tensor, Tensor> linear_cuda(const Tensor& x_, const Tensor& weight_, 
 std::tuple<Tensor, Tensor> linear_meta(const Tensor& x, const Tensor& weight, const optional<Tensor>&,
                                        const optional<Tensor>&, int64_t, bool want_preact, const optional<Tensor>&) {
     return {at::empty({x.size(0), weight.size(0)}, x.options()),
-            at::empty({want_preact ? x.size(0) : 0, round8(weight.size(0))}, x.options())};
+            at::empty({want_preact ? x.size(0) : 0, round8(weight.size(0))}, x.options().dtype(at::kHalf))};
 }
 
 std::tuple<Tensor, Tensor, Tensor> linear_grad_cuda(const Tensor& grad_out, const Tensor& x_, const Tensor& weight_,
@@ -840,7 +840,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_grad_cuda(const Tensor& grad_out, cons
     a.weight_row_stride = row_stride(weight);
     if (activation != B2S_ACT_NONE) {
         TORCH_CHECK(preact.has_value() && preact->defined(), "preact is needed with an activation");
-        check_same(*preact, x, at::kBFloat16, "preact");
+        check_same(*preact, x, at::kHalf, "preact");
         TORCH_CHECK(preact->dim() == 2 && preact->size(0) == R && preact->size(1) == round8(N) && preact->is_contiguous(),
                     "preact must be what linear gave");
         a.preact = preact->data_ptr();

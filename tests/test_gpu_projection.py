@@ -3,8 +3,8 @@
 Operands are small multiples of 1/4 whose products and sums are exact in fp32, so that without a transcendental
 activation the output is the exact value rounded once and has to be equal bit for bit; with one, the activation's fp32
 error (a few 2^-24) can only move a value across a rounding border: half a step of bf16 (2^-8) and a little.  With an
-activation the gradient's slope is taken from a pre-activation rounded to bf16 (half a step of z times the curvature,
-below 0.5 for silu and 0.8 for gelu) and dz is rounded to bf16 as the products' operand.
+activation the gradient's slope is taken from a pre-activation rounded to 16 bits (at most half a step of bf16 of z times
+the curvature, below 0.5 for silu and 0.8 for gelu) and dz is rounded to bf16 as the products' operand.
 """
 
 import pytest
@@ -182,6 +182,11 @@ def test_nan_and_infinity_stay_in_their_rows(pkg):
     got = pkg.projection.linear(x3, w, b, activation="relu", residual=r)
     keep = torch.arange(140, device=DEV) != 130
     assert torch.equal(got[keep], want[keep])
+    zl = torch.tensor([[-3.0e38, -1.0e5, -6.0e4, 0.0, 1.0e-9, 6.0e4, 1.0e5, 3.0e38]], device=DEV).bfloat16().requires_grad_(True)
+    for act, low in (("gelu", 0.5), ("silu", 0.5), ("relu", 1.0)):  # slopes far out, and next to zero
+        d, = torch.autograd.grad(pkg.projection.linear(zl, torch.eye(8, device=DEV, dtype=torch.bfloat16), activation=act),
+                                 (zl,), torch.ones(1, 8, device=DEV, dtype=torch.bfloat16))
+        assert d[0].tolist() == [0.0, 0.0, 0.0, 0.0 if act == "relu" else 0.5, low, 1.0, 1.0, 1.0], act
     for act in ("gelu", "silu"):  # the tails: act(-large) = 0, act(large) = large
         z = torch.tensor([[-200.0, 200.0, -30000.0, 30000.0, 0.0, -3.0e38, 3.0e38, 1.0]], device=DEV).bfloat16()
         y = pkg.projection.linear(z, torch.eye(8, device=DEV, dtype=torch.bfloat16), activation=act)
