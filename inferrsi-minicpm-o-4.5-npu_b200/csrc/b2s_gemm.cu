@@ -408,7 +408,17 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                     }
                     give();
                 }
-                if (ok) epilogue_logits<TN / 2, EPI>(a, v, row0, n0, half, nt, staging + warp * 4096);
+                if (!ok) break;
+                if (EPI == EPI_LSE && p.slot >= 0) {  // a chunk of a split tile: fp32 sums, for lmhead_merge_kernel
+                    const int row = row0 + lane;
+                    float4* dst = reinterpret_cast<float4*>(a.partial + ((int64_t)p.slot * min(a.M, TM) + row) * TN + half * (TN / 2));
+                    if (row < a.M) {
+#pragma unroll
+                        for (int j = 0; j < TN / 8; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    }
+                } else {
+                    epilogue_logits<TN / 2, EPI>(a, v, row0, n0, half, nt, staging + warp * 4096);
+                }
             } else {
                 uint32_t rq[16];
                 if (EPI == EPI_LINEAR && p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
@@ -560,6 +570,15 @@ Plan plan_for(int M, int N, int64_t K, int epi, int sms) {
                 return rounds ? mine + (rounds - 1) * (mine > tail ? mine : tail) + tail : 0;
             };
             int64_t cost = tiles_cost(p.waves + (p.rest ? 1 : 0), nkb);
+            // The head's states cannot be joined across k; but where whole waves leave a handful of column tiles over (a step's
+            // 594 on 148 CTAs: two, which alone would stream their 4 MB at two SMs' rate), and one tile holds all rows,
+            // those are split 8 ways and lmhead_merge_kernel adds their logits.
+            if (epi == EPI_LSE && M <= GM_M && p.waves && p.rest && p.rest <= 16 && nkb >= 16) {
+                p.chunk = (int)ceil_div(nkb, 8);
+                p.split = (int)ceil_div(nkb, p.chunk);
+                p.bytes = (int64_t)p.split * p.rest * M * tn * 4;
+                cost = tiles_cost(p.waves, nkb) + ceil_div(p.rest * p.split, U) * p.chunk * kb_cost;
+            }
             if (may_split && p.rest) {
                 const int64_t held = M < tm ? M : tm;
                 for (int64_t want = 2; want <= nkb && want <= 64; want += want < 4 ? 1 : want / 2) {  // 2 3 4 6 9 13 19 28 42 63
@@ -646,19 +665,37 @@ int gemm(const Operand& A, const Operand& B, int64_t K, const GemmArgs& a, void*
 
 // ------------------------------------------------------------------ the head's log probabilities
 
-constexpr int LM_NT = 128;
-// One CTA per row: the column tiles' states into the row's outputs.
-__global__ void __launch_bounds__(LM_NT) lmhead_merge_kernel(const float4* part, int tiles, const float* token_value,
+constexpr int LM_NT = 256;
+// One CTA per row: the column tiles' states into the row's outputs, and the logits of the last `rest` tiles where those
+// were split along k (at most 128 rows): their chunks added in k order, then the columns' states like any other.
+__global__ void __launch_bounds__(LM_NT) lmhead_merge_kernel(const float4* part, int states, int stride, const float* partial,
+                                                             int rest, int split, int tn, int rows, const float* token_value,
                                                              const int64_t* tokens, int V, float c, float* logprob,
                                                              float* entropy, float4* stats, uint32_t* status) {
     pdl_wait_then_release();
     __shared__ LpState sw[LM_NT / 32];
+    __shared__ float tv;
     const int r = blockIdx.x, tid = threadIdx.x;
+    const int64_t tok = tokens[r];
+    const bool has = tok >= 0 && tok < V;
+    const int n0 = split > 1 ? (states / 2) * tn : V;  // first column of the split tiles
     LpState s;
     s.m = f_ninf();
     s.S = s.U = 0.0f;
-    for (int i = tid; i < tiles; i += LM_NT) {
-        const float4 p = part[(int64_t)r * tiles + i];
+    if (tid == 0 && has && tok < n0) tv = token_value[r];
+    const int64_t step = (int64_t)rest * rows * tn;
+    for (int n = n0 + tid; n < V; n += LM_NT) {
+        const int i = n - n0;
+        const float* p = partial + ((int64_t)(i / tn) * rows + r) * tn + i % tn;
+        float x = 0.0f;
+#pragma unroll 8
+        for (int k = 0; k < split; ++k) x += p[k * step];
+        if (n == tok) tv = x;
+        const float one[1] = {x};
+        lp_add_any<1>(s, one, c);
+    }
+    for (int i = tid; i < states; i += LM_NT) {
+        const float4 p = part[(int64_t)r * stride + i];
         LpState o;
         o.m = p.x;
         o.S = p.y;
@@ -668,16 +705,18 @@ __global__ void __launch_bounds__(LM_NT) lmhead_merge_kernel(const float4* part,
     lp_warp_merge(s, c);
     if ((tid & 31) == 0) sw[tid >> 5] = s;
     __syncthreads();
-    if (tid == 0) {
-#pragma unroll
-        for (int w = 1; w < LM_NT / 32; ++w) s = lp_merge(s, sw[w], c);
-        const LpFinal f = lp_final(s, c);
-        const int64_t tok = tokens[r];
-        const bool has = tok >= 0 && tok < V;
-        if (logprob) logprob[r] = has ? lp_value(token_value[r], f, c) : 0.0f;
-        if (entropy) entropy[r] = f.entropy;
-        if (stats) stats[r] = make_float4(f.m, f.R, f.log2S, f.entropy);
-        if (status && tok >= V) atomicOr(status, B2S_STATUS_TOKEN_RANGE);
+    if (tid < 32) {
+        s.m = f_ninf();
+        s.S = s.U = 0.0f;
+        if (tid < LM_NT / 32) s = sw[tid];
+        lp_warp_merge(s, c);
+        if (tid == 0) {
+            const LpFinal f = lp_final(s, c);
+            if (logprob) logprob[r] = has ? lp_value(tv, f, c) : 0.0f;
+            if (entropy) entropy[r] = f.entropy;
+            if (stats) stats[r] = make_float4(f.m, f.R, f.log2S, f.entropy);
+            if (status && tok >= V) atomicOr(status, B2S_STATUS_TOKEN_RANGE);
+        }
     }
 }
 
@@ -869,8 +908,8 @@ extern "C" {
 int b2s_lmhead_logprobs_workspace(int32_t rows, int32_t vocab, int32_t hidden_dim, int64_t* bytes) {
     using namespace b2s;
     if (rows < 0 || vocab < 1 || hidden_dim < 8 || !bytes) return B2S_ERR_INVALID;
-    const int tn = plan_here(rows > 0 ? rows : 1, vocab, hidden_dim, EPI_LSE).tn;
-    *bytes = up((int64_t)rows * ((vocab + tn - 1) / tn) * 32 + (int64_t)rows * 4, 256);
+    const Plan p = plan_here(rows > 0 ? rows : 1, vocab, hidden_dim, EPI_LSE);
+    *bytes = up((int64_t)rows * ((vocab + p.tn - 1) / p.tn) * 32 + (int64_t)rows * 4, 256) + p.bytes;
     return B2S_OK;
 }
 
@@ -885,8 +924,8 @@ int b2s_lmhead_logprobs(const b2s_lmhead_args* h, float* logprob, float* entropy
     b2s_lmhead_logprobs_workspace(h->rows, h->vocab, h->hidden_dim, &need);
     if (!h->tokens || !h->workspace || h->workspace_bytes < need || !aligned16(h->workspace) || (stats && !aligned16(stats)))
         return B2S_ERR_INVALID;
-    const int tn = plan_here(h->rows, h->vocab, h->hidden_dim, EPI_LSE).tn;
-    const int tiles = 2 * ((h->vocab + tn - 1) / tn);  // states per row: two halves of each column tile
+    const Plan p = plan_here(h->rows, h->vocab, h->hidden_dim, EPI_LSE);
+    const int tiles = (h->vocab + p.tn - 1) / p.tn, whole = p.split > 1 ? tiles - p.rest : tiles;
     GemmArgs a;
     memset(&a, 0, sizeof(a));
     a.M = h->rows;
@@ -894,14 +933,17 @@ int b2s_lmhead_logprobs(const b2s_lmhead_args* h, float* logprob, float* entropy
     a.status = h->status;
     a.c = lp_scale(h->temperature);
     a.tokens = h->tokens;
-    a.part = static_cast<float4*>(h->workspace);
-    a.token_value = reinterpret_cast<float*>(a.part + (int64_t)h->rows * tiles);
+    a.part = static_cast<float4*>(h->workspace);  // two states a row and column tile
+    a.token_value = reinterpret_cast<float*>(a.part + (int64_t)h->rows * tiles * 2);
+    a.partial = reinterpret_cast<float*>(static_cast<unsigned char*>(h->workspace) +
+                                         up((int64_t)h->rows * tiles * 32 + (int64_t)h->rows * 4, 256));
     rc = gemm<false, false, EPI_LSE>({h->hidden, h->hidden_row_stride}, {h->head, h->head_row_stride}, h->hidden_dim, a,
                                      stream);
     if (rc != B2S_OK) return rc;
     const cudaError_t e = launch_pdl(lmhead_merge_kernel, dim3((unsigned)h->rows), LM_NT, 0, stream,
-                                     (const float4*)a.part, tiles, (const float*)a.token_value, h->tokens,
-                                     (int)h->vocab, a.c, logprob, entropy, reinterpret_cast<float4*>(stats), h->status);
+                                     (const float4*)a.part, 2 * whole, 2 * tiles, (const float*)a.partial, p.rest, p.split,
+                                     p.tn, (int)h->rows, (const float*)a.token_value, h->tokens, (int)h->vocab, a.c, logprob,
+                                     entropy, reinterpret_cast<float4*>(stats), h->status);
     return e == cudaSuccess ? B2S_OK : cuda_fail(e);
 }
 

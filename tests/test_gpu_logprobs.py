@@ -357,7 +357,9 @@ def exact_operands(n, V, H, seed, scale=0.25):
 
 
 HEAD_SIZES = [(1, 1, 8), (1, 700, 64), (3, 64, 72), (5, 65, 8), (16, 6562, 768), (17, 1000, 1000), (64, 20_001, 256),
-              (127, 513, 128), (128, 512, 64), (129, 4096, 192), (300, 6561, 512), (2100, 777, 80), (40, 33_000, 768)]
+              (127, 513, 128), (128, 512, 64), (129, 4096, 192), (300, 6561, 512), (2100, 777, 80), (40, 33_000, 768),
+              # whole waves of column tiles and a few over, split along k
+              (3, 148 * 256 + 700, 1024), (100, 148 * 256 * 2 + 1, 1104)]
 
 
 @pytest.mark.parametrize("n,V,H", HEAD_SIZES)
