@@ -604,11 +604,28 @@ Plan plan_for(int M, int N, int64_t K, int epi, int sms) {
     return best;
 }
 
-// The plan on the current device (without one, where only sizes are asked for, on a B200's 148 multiprocessors).
+// The plan on the current device (without one, where only sizes are asked for, on a B200's 148 multiprocessors).  A plan
+// is a function of the sizes alone; each thread keeps its last few (making one takes the host about a microsecond, and a
+// gradient asks for five).
 Plan plan_here(int M, int N, int64_t K, int epi) {
+    struct Kept {
+        int M, N, epi, sms;
+        int64_t K;
+        Plan plan;
+    };
+    static thread_local Kept kept[16] = {};
     int sms = 0;
     if (device_sms(&sms) != cudaSuccess || sms < 1) sms = 148;
-    return plan_for(M, N, K, epi, sms);
+    Kept& k = kept[((unsigned)M * 31u + (unsigned)N * 17u + (unsigned)K * 7u + (unsigned)epi) % 16u];
+    if (k.M != M || k.N != N || k.K != K || k.epi != epi || k.sms != sms) {
+        k.plan = plan_for(M, N, K, epi, sms);
+        k.M = M;
+        k.N = N;
+        k.K = K;
+        k.epi = epi;
+        k.sms = sms;
+    }
+    return k.plan;
 }
 
 template <int CG, int TN, bool AMN, bool BMN, int EPI>

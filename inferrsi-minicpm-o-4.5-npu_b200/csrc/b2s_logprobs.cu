@@ -687,11 +687,27 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         __syncwarp();
         cluster_arrive_release();
         cluster_wait();
-        if (crank == 0)
-            for (int k = 1; k < C; ++k) {
-                w = lp_merge(w, sh.total[k], a.c);
-                c2 += sh.total_count[k];
+        if (crank == 0) {  // every warp for itself: the maximum, then one rescaling and a sum over the parts
+            LpState o;
+            o.m = f_ninf();
+            o.S = o.U = 0.0f;
+            c2 = 0;
+            if (lane < C) {
+                o = sh.total[lane];
+                c2 = sh.total_count[lane];
             }
+            const uint32_t key = __reduce_max_sync(0xffffffffu, rank_key(o.m));
+            w.m = key == 0xffffffffu ? __int_as_float(0x7fffffff) : okey_to_f(key);
+            if (fabsf(w.m) <= 3.402823466e38f && o.m != f_ninf()) lp_rescale(o, w.m, a.c);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) {
+                o.S += __shfl_xor_sync(0xffffffffu, o.S, d);
+                o.U += __shfl_xor_sync(0xffffffffu, o.U, d);
+            }
+            w.S = o.S;
+            w.U = o.U;
+            c2 = __reduce_add_sync(0xffffffffu, c2);
+        }
     }
     if (crank == 0) {
         const LpFinal f = lp_final(w, a.c);
