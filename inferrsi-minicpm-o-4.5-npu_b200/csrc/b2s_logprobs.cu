@@ -12,7 +12,7 @@
 //
 // Forward, one pass over the row by bulk copies into a ring of shared-memory chunks (a thread's registers do not bound
 // the bytes in flight), 128 or 256 threads per row where rows are many, else 512 and a cluster of CTAs per row while rows
-// are few.  Two elements share one packed fp32 operation, and a bf16 pair one maximum and one comparison: about 6
+// are few; many short rows without alternatives take a warp each, from registers.  Two elements share one packed fp32 operation, and a bf16 pair one maximum and one comparison: about 6
 // instructions an element, so that bf16 rows stay bound by HBM.  The rank counts the elements before the token in (value
 // descending, id ascending) order: an element before the token counts when x >= x_t, i.e. x > pred(x_t), one after it
 // when x > x_t, so a vector needs one threshold.  Top alternatives: the
@@ -743,6 +743,88 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
     }
 }
 
+// A warp per row, for many short rows without alternatives: no shared memory and no barriers, the next vectors in flight in
+// registers while the current ones are added.  Bound by latency and issue on the shortest rows, by HBM on the longest
+// (microseconds, a CTA of 128 threads per row / this kernel: 30000 rows of 1000 bf16 89.5 / 21.2, 8192 of 6562 bf16 40.3 /
+// 24.8, 4000 of 15000 fp32 46.9 / 40.4, 5.9 TB/s).  A lane adds up to a 64th of a row into each of its sums.
+constexpr int LPW_NT = 256;
+template <typename E>
+__global__ void __launch_bounds__(LPW_NT, 4) token_logprobs_warp_kernel(const LpArgs a, int rows) {
+    constexpr int EPV = LpElem<E>::EPV, ES = 16 / EPV;
+    pdl_wait_then_release();
+    const int r = (int)blockIdx.x * (LPW_NT / 32) + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= rows) return;
+    const unsigned char* rowp = static_cast<const unsigned char*>(a.logits) + (int64_t)r * a.stride * ES;
+    const int n = a.V, nh = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(rowp) & 15)) & 15) / ES));
+    const int nv = (n - nh) / EPV, nt = n - nh - nv * EPV;
+    const uint4* vp = reinterpret_cast<const uint4*>(rowp + (int64_t)nh * ES);
+    uint4 q[LP_U];
+    auto load = [&](int v0) {
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) q[u] = v0 + 32 * u + lane < nv ? ldg_stream(vp + v0 + 32 * u + lane) : LpElem<E>::nothing();
+    };
+    load(0);
+    const int64_t tok = a.tokens ? a.tokens[r] : -1;
+    const bool has_tok = tok >= 0 && tok < a.V;
+    const int t = has_tok ? (int)tok : -1;
+    const float xt = has_tok ? LpElem<E>::ld(rowp, t) : 0.0f;
+    const typename LpElem<E>::Thr thr_after = LpElem<E>::threshold(xt), thr_before = LpElem<E>::threshold_before(xt);
+    const int tv = t >= nh ? min(nv, (t - nh) / EPV) : 0;  // vectors below it lie before the token
+    LpThread s;
+    s.m = f_ninf();
+    s.S = s.U = make_float2(0.0f, 0.0f);
+    int cnt = 0;
+    const int end = lane < nh ? lane : (lane >= 16 && lane < 16 + nt ? n - nt + lane - 16 : -1);  // the ragged ends
+    if (end >= 0) {
+        const float x = LpElem<E>::ld(rowp, end);
+        lp_thread_add(s, x, a.c);
+        cnt += end != t && (x > xt || x != x || (end < t && x == xt));
+    }
+    for (int v0 = 0; v0 < nv; v0 += 32 * LP_U) {
+        uint4 now[LP_U];
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) now[u] = q[u];
+        load(v0 + 32 * LP_U);
+        lp_thread_batch<E>(s, now, LpElem<E>::batch_max(now), a.c);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)  // the vector that holds the token counts as behind it here
+            cnt += LpElem<E>::count_above(now[u], v0 + 32 * u + lane < tv ? thr_before : thr_after);
+    }
+    // the elements of the token's own vector before it that tie with it
+    const int i = nh + tv * EPV + lane;
+    if (t >= nh && t < nh + nv * EPV && i < t) cnt += LpElem<E>::ld(rowp, i) == xt;
+    if (has_tok && xt != xt) {  // a NaN token: the NaN elements before it
+        cnt = 0;
+        for (int j = lane; j < t; j += 32) {
+            const float x = LpElem<E>::ld(rowp, j);
+            cnt += x != x;
+        }
+    }
+    const uint32_t key = __reduce_max_sync(0xffffffffu, rank_key(s.m));
+    LpState w;
+    w.m = key == 0xffffffffu ? __int_as_float(0x7fffffff) : okey_to_f(key);
+    w.S = w.U = 0.0f;
+    if (fabsf(w.m) <= 3.402823466e38f && s.m != f_ninf()) {
+        lp_thread_rescale(s, w.m, a.c);
+        w.S = s.S.x + s.S.y;
+        w.U = s.U.x + s.U.y;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        w.S += __shfl_xor_sync(0xffffffffu, w.S, o);
+        w.U += __shfl_xor_sync(0xffffffffu, w.U, o);
+    }
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    const LpFinal f = lp_final(w, a.c);
+    if (lane == 0) {
+        if (a.logprob) a.logprob[r] = has_tok ? lp_value(xt, f, a.c) : 0.0f;
+        if (a.entropy) a.entropy[r] = f.entropy;
+        if (a.rank) a.rank[r] = has_tok ? (int64_t)cnt : -1;
+        if (a.stats) a.stats[r] = make_float4(f.m, f.R, f.log2S, f.entropy);
+        if (a.status && tok >= a.V) atomicOr(a.status, B2S_STATUS_TOKEN_RANGE);
+    }
+}
+
 // dx for one chunk of a row per CTA.
 constexpr int LPG_NT = 256;
 constexpr int LPG_U = 8;  // vectors in flight per thread
@@ -892,7 +974,15 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     // Many rows: a CTA each, of 128 threads up to 64 KB (1065 rows of 31 KB: 512 threads 13.3 us, 128 11.9) and of 256 beyond
     // (2048 rows of 297 KB: 512 threads 142 us, 128 132, 256 129).  With alternatives 256 from 24 KB on, which leaves an SM
     // its 1024 threads beside whole rows in shared memory.  Few rows: clusters of 512 threads.
-    if (rows >= 2 * sms && row_bytes <= (top ? 24 : 64) * 1024) {
+    //
+    // Without alternatives a warp per row once that fills the SMs' warps, or where a row is a few vectors per lane (a CTA / a
+    // warp: 300 rows of 700 bf16 3.4 / 2.9 us, 300 of 6562 4.4 / 6.5, 1200 of 6562 8.7 / 9.1, 2000 of 18664 20.5 / 20.3,
+    // 2000 of 30000 32.3 / 30.1, 4000 of 64000 107.4 / 106.6).
+    if (!top && ((rows >= 2 * sms && row_bytes <= 4 * 1024) || (rows >= 12 * sms && row_bytes <= 64 * 1024))) {
+        const int64_t blocks = ((int64_t)rows + LPW_NT / 32 - 1) / (LPW_NT / 32);
+        e = bf ? launch(token_logprobs_warp_kernel<__nv_bfloat16>, blocks, LPW_NT, 0u, 0, stream, a, (int)rows)
+               : launch(token_logprobs_warp_kernel<float>, blocks, LPW_NT, 0u, 0, stream, a, (int)rows);
+    } else if (rows >= 2 * sms && row_bytes <= (top ? 24 : 64) * 1024) {
         e = top ? (bf ? launch_rows<__nv_bfloat16, 128, true>(a, rows, 1, es, sms, stream)
                       : launch_rows<float, 128, true>(a, rows, 1, es, sms, stream))
                 : (bf ? launch_rows<__nv_bfloat16, 128, false>(a, rows, 1, es, sms, stream)

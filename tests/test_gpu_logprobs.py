@@ -197,6 +197,76 @@ def test_rows_that_defeat_the_bound(pkg, n, V, dtype):
             assert torch.equal(r.top_ids, plain(y, t[:2], 1.0, 32)[3])
 
 
+def warp_close(r, x, t, T):
+    """A warp per row: 32 lanes with two sums each add a 64th of the row into each, then as `check`."""
+    V = x.shape[1]
+    s = EPS * (V / 64 + 64)
+    lp, H, rank, _, _, _, _ = plain(x, t, T)
+    assert torch.equal(r.rank, rank)
+    close(r.logprob, lp, s + 4 * EPS * lp.abs())
+    close(r.entropy, H, 2 * s * (2 + H.abs()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V", [(300, 1), (301, 2), (303, 7), (307, 8), (299, 9), (300, 17), (300, 255), (300, 256),
+                                 (300, 700), (2000, 33), (1801, 1023), (1777, 2049), (1776, 6562), (1783, 16_001)])
+def test_many_short_rows(pkg, n, V, dtype):
+    """Rows that take a warp each, with a last CTA that has rows left over; tokens in the ragged ends too."""
+    for T, pad, shift in ((1.0, 0, 0), (0.7, 3, 1), (1.3, 8, 3), (1.0, 1, 0)):
+        x, t = rows_of(n, V, dtype, V + n, pad, shift)
+        t[::5] = torch.arange(t[::5].numel(), device=DEV) % min(V, 9)
+        t[1::5] = V - 1 - torch.arange(t[1::5].numel(), device=DEV) % min(V, 9)
+        t[2::50] = -1
+        warp_close(pkg.logprobs.token_logprobs(x, t, temperature=T), x, t, T)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,shift", [(320, 9, 0), (320, 700, 1), (1800, 700, 0), (1800, 6561, 0), (1800, 16_000, 3)])
+def test_many_short_rows_special_values(pkg, n, V, shift, dtype):
+    x, t = rows_of(n, V, dtype, V, 0, shift)
+    low, big = torch.finfo(dtype).min, torch.finfo(dtype).max
+    ninf, inf, nan = float("-inf"), float("inf"), float("nan")
+    i = torch.arange(V, device=DEV)
+
+    def only(where, value, rest=ninf):
+        return torch.where(where, value, rest).to(dtype)
+
+    kinds = [only(i < 0, 0.0), only(i == V // 2, 3.0), only(i < 0, 0.0, low), only(i >= V - 4, 1.0, low),
+             only(i >= 0, 0.25), only(i == V // 3, nan, 1.0), only(i == V // 3, inf, 1.0), only(i % 2 == 0, 0.5),
+             only(i >= 0, big), only(i < 3, big, 0.0), only(i % 2 == 0, 0.0, -0.0), i.to(dtype), -i.to(dtype),
+             (i % 7).to(dtype), only(i < 5, 2.0), only(i >= V // 2, nan, 1.0), only(i % 64 == 3, 50.0, -50.0)]
+    for r in range(n):
+        if r % 3:
+            x[r] = kinds[r % len(kinds)]
+    t[::4] = x[::4].float().argmax(1)
+    t[1::8] = V - 1
+    t[3::8] = V // 3
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    warp_close(pkg.logprobs.token_logprobs(x, t, status=st), x, t, 1.0)
+    assert int(st) == 0
+    t[n - 1] = V
+    r = pkg.logprobs.token_logprobs(x, t, status=st)
+    assert int(st) == 32 and float(r.logprob[n - 1]) == 0.0 and int(r.rank[n - 1]) == -1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,pad,shift", [(300, 33, 0, 0), (310, 700, 3, 1), (1800, 6562, 0, 0)])
+def test_many_short_rows_gradient(pkg, n, V, pad, shift, dtype):
+    x, t = rows_of(n, V, dtype, V, pad, shift)
+    x[0, ::2] = float("-inf")
+    t[0], t[1] = 1, -1
+    x[2] = float("-inf")
+    g = torch.Generator(device=DEV).manual_seed(7)
+    gl, gh = torch.randn(n, device=DEV, generator=g), torch.randn(n, device=DEV, generator=g)
+    leaf = x.detach().requires_grad_(True)
+    r = pkg.logprobs.token_logprobs(leaf, t, temperature=0.6)
+    d, = torch.autograd.grad((r.logprob, r.entropy), (leaf,), (gl, gh))
+    want, size = plain_grad(x, t, gl, gh, 0.6)
+    logp = plain(x, t, 0.6)[6]
+    rel = EPS * (V / 64 + 64) + 4 * EPS * torch.where(torch.isfinite(logp), logp.abs(), 0.0)
+    close(d, want, 2 * rel * size + HALF_STEP[dtype] * want.abs() + 2.0 ** -126)
+
+
 def test_no_token_rows_and_status(pkg):
     x, t = rows_of(6, 501, torch.float32, 5)
     st = torch.zeros(1, dtype=torch.int32, device=DEV)
