@@ -83,9 +83,15 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
                                                         __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = 4 * i + (lane >> 3), c = lane & 7;
-                    if (r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)r * TN + 32 * q + 4 * c) = *stage_at(st, r, c);
+                for (int h = 0; h < 32; h += 16) {  // read before it is stored, as in block_store
+                    uint4 u[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) u[i] = *stage_at(st, h + 4 * i + (lane >> 3), lane & 7);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = h + 4 * i + (lane >> 3);
+                        if (r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)r * TN + 32 * q + 4 * (lane & 7)) = u[i];
+                    }
                 }
                 __syncwarp();
             }

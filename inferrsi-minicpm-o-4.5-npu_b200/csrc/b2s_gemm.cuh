@@ -196,12 +196,14 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
 __device__ __forceinline__ uint4* stage_at(unsigned char* st, int r, int j) {
     return reinterpret_cast<uint4*>(st + r * 128 + ((j ^ (r & 7)) << 4));
 }
-// The 4-byte word of columns 2 w, 2 w + 1 of row r, from chunk `base`.
-__device__ __forceinline__ uint32_t* stage_word(unsigned char* st, int r, int base, int w) {
-    return reinterpret_cast<uint32_t*>(st + r * 128 + (((base + (w >> 2)) ^ (r & 7)) << 4)) + (w & 3);
+// The 4-byte word of columns 2 w, 2 w + 1 of row r.
+__device__ __forceinline__ uint32_t* stage_word(unsigned char* st, int r, int w) {
+    return reinterpret_cast<uint32_t*>(st + r * 128 + (((w >> 2) ^ (r & 7)) << 4)) + (w & 3);
 }
 // Copies between a staging block and 32 rows x 32 bf16 of global memory, rows `stride` elements apart.  `vec` (16-byte
-// aligned rows, all 32 columns there): 4 lanes per row, 8 rows at a time; else 16 lanes per row, 2 columns each.
+// aligned rows, all 32 columns there): 4 lanes per row, 8 rows at a time; else a column per lane.  What is read from the
+// block goes to registers before any of it is stored, as the compiler cannot tell that the two do not overlap and would wait
+// for each read by itself (4099 rows of 1537 columns out of 768: 20.0 against 15.2 us).
 __device__ __forceinline__ int vec_row(int i) {
     const int rr = (threadIdx.x & 31) >> 2;
     return 8 * i + (rr & 1) * 4 + (rr >> 1);
@@ -212,31 +214,26 @@ __device__ __forceinline__ void block_store(unsigned char* st, int base, void* o
     unsigned short* p = static_cast<unsigned short*>(out);
     if (vec) {
         const int c = lane & 3;
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *stage_at(st, vec_row(i), base + c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = vec_row(i);
-            if (r < rows) *reinterpret_cast<uint4*>(p + r * stride + 8 * c) = *stage_at(st, r, base + c);
+            if (r < rows) *reinterpret_cast<uint4*>(p + r * stride + 8 * c) = v[i];
         }
-    } else {
-        // whole 4-byte words where the row starts on one, else words one column on, the ends by themselves; the two rows of
-        // a step have the same parity, so a warp takes one of the two ways
-        const int w = lane & 15, left = cols - 2 * w;
-#pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-            const int r = 4 * (i >> 1) + (i & 1) + 2 * (lane >> 4);
-            const uint32_t v = *stage_word(st, r, base, w);
-            const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1, 16);
-            unsigned short* q = p + r * stride + 2 * w;
-            if (r < rows) {
-                if ((reinterpret_cast<uintptr_t>(q) & 2) == 0) {
-                    if (left >= 2) *reinterpret_cast<uint32_t*>(q) = v;
-                    else if (left == 1) q[0] = (unsigned short)v;
-                } else {
-                    if (w == 0) q[0] = (unsigned short)v;  // a block has a first column
-                    if (w < 15 && left >= 3) *reinterpret_cast<uint32_t*>(q + 1) = v >> 16 | next << 16;
-                    else if (left >= 2) q[1] = (unsigned short)(v >> 16);
-                }
-            }
+    } else if (lane < cols) {
+        const unsigned char* column = st + 2 * (lane & 7);
+        p += lane;
+#pragma unroll 1
+        for (int r = 0; r < 32; r += 8) {
+            unsigned short v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = *reinterpret_cast<const unsigned short*>(column + (r + k) * 128 + (((base + (lane >> 3)) ^ k) << 4));
+#pragma unroll
+            for (int k = 0; k < 8; ++k, p += stride)
+                if (r + k < rows) *p = v[k];
         }
     }
 }
@@ -277,7 +274,7 @@ __device__ __forceinline__ void block_put(unsigned char* st, const uint32_t (&q)
             *stage_at(st, vec_row(i), lane & 3) = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) *stage_word(st, 2 * i + (lane >> 4), 0, lane & 15) = q[i];
+        for (int i = 0; i < 16; ++i) *stage_word(st, 2 * i + (lane >> 4), lane & 15) = q[i];
     }
 }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
