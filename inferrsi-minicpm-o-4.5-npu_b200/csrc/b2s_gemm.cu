@@ -829,15 +829,17 @@ cudaError_t linear_rows(const GemmArgs& a, const void* x, int64_t xs, const void
 
 // ------------------------------------------------------------------ the projection's elementwise gradient
 
-// dz = dy act'(z) (bf16, rows dz_stride apart) and the sums of its columns over this CTA's rows, E columns of a row per
-// thread: 8 where dy's rows are 16-byte aligned, else 2, z and dz (whose rows always are) still as whole words.  32 threads
-// cover 32 E columns, the 8 warps take rows in turn; the sums (fp32, of the unrounded dz) go to part[blockIdx.y][n], or,
+// dz = dy act'(z) (bf16, rows dz_stride apart) and the sums of its columns over this CTA's rows, 8 columns of a row per
+// thread (z's and dz's rows are padded to that).  VEC: dy's rows are 16-byte aligned; else a row starts on a whole word or
+// half a word off, and a thread's 8 values are four words, or two halves and the three words between them.  32 threads
+// cover 256 columns, the 8 warps take rows in turn; the sums (fp32, of the unrounded dz) go to part[blockIdx.y][n], or,
 // with one part, straight to the bias gradient.
 constexpr int DZ_NT = 256;
-template <int E>
+template <bool VEC, int ACT>
 __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_t dy_stride, const void* z,
-                                                          int64_t z_stride, int act, int rows, int N, int rows_per,
+                                                          int64_t z_stride, int rows, int N, int rows_per,
                                                           void* dz, int64_t dz_stride, float* part, void* db) {
+    constexpr int E = 8;
     pdl_wait_then_release();
     __shared__ float red[8][32][E + 1];
     const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5;
@@ -850,32 +852,36 @@ __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_
             const unsigned short* gp = static_cast<const unsigned short*>(dy) + (int64_t)r * dy_stride + n;
             const unsigned short* zp = static_cast<const unsigned short*>(z) + (int64_t)r * z_stride + n;
             float g[E], x[E];
-            if constexpr (E == 8) {
-                load8(gp, 0, N - n, true, g);
-                if (act != ACT_NONE) {  // z's rows are padded to a multiple of 8
-                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(zp));
-                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int j = 0; j < E; ++j) x[j] = preact_value((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
-                }
+            if (VEC || n + E > N) {
+                load8(gp, 0, N - n, VEC, g);
             } else {
-                g[0] = bf16_bits_to_f(__ldg(gp));
-                g[1] = n + 1 < N ? bf16_bits_to_f(__ldg(gp + 1)) : 0.0f;
-                if (act != ACT_NONE) {
-                    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(zp));
-                    x[0] = preact_value((unsigned short)w);
-                    x[1] = preact_value((unsigned short)(w >> 16));
+                const bool half = reinterpret_cast<uintptr_t>(gp) & 2;
+                const uint32_t* mid = reinterpret_cast<const uint32_t*>(gp + (half ? 1 : 0));
+                uint32_t w[4] = {__ldg(mid), __ldg(mid + 1), __ldg(mid + 2), 0u};
+                if (half) {
+                    const uint32_t lo = __ldg(gp), hi = __ldg(gp + 7);
+                    w[3] = w[2] >> 16 | hi << 16;
+                    w[2] = __funnelshift_l(w[1], w[2], 16);
+                    w[1] = __funnelshift_l(w[0], w[1], 16);
+                    w[0] = lo | w[0] << 16;
+                } else {
+                    w[3] = __ldg(mid + 3);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    g[2 * j] = __uint_as_float(w[j] << 16);
+                    g[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
                 }
             }
-            if (act != ACT_NONE) {
+            if constexpr (ACT != ACT_NONE) {
+                const uint4 q = __ldg(reinterpret_cast<const uint4*>(zp));
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                for (int j = 0; j < E; ++j) g[j] *= n + j < N ? act_slope(x[j], act) : 0.0f;
+                for (int j = 0; j < E; ++j) x[j] = preact_value((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+#pragma unroll
+                for (int j = 0; j < E; ++j) g[j] *= n + j < N ? act_slope<ACT>(x[j]) : 0.0f;
             }
-            if (dz) {
-                unsigned short* o = static_cast<unsigned short*>(dz) + (int64_t)r * dz_stride + n;
-                if constexpr (E == 8) store8(o, 0, N - n, true, g);
-                else *reinterpret_cast<uint32_t*>(o) = pack_bf16(g[0], g[1]);  // dz's rows are padded likewise
-            }
+            if (dz) store8(static_cast<unsigned short*>(dz) + (int64_t)r * dz_stride + n, 0, N - n, true, g);
 #pragma unroll
             for (int j = 0; j < E; ++j) sum[j] += g[j];
         }
@@ -893,23 +899,31 @@ __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_
     if (part) part[(int64_t)blockIdx.y * N + col] = s;
     else static_cast<__nv_bfloat16*>(db)[col] = __float2bfloat16_rn(s);
 }
-__global__ void linear_db_kernel(const float* part, int parts, int N, void* db) {
+// db = the sums of the parts' sums, each of 8 warps taking an eighth of the parts of 32 columns.
+__global__ void __launch_bounds__(DZ_NT) linear_db_kernel(const float* part, int parts, int N, void* db) {
     pdl_wait_then_release();
-    const int n = blockIdx.x * blockDim.x + threadIdx.x;
-    if (n >= N) return;
+    __shared__ float red[8][32];
+    const int c = threadIdx.x & 31, w = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
     float s = 0.0f;
+    if (n < N) {
 #pragma unroll 8
-    for (int p = 0; p < parts; ++p) s += part[(int64_t)p * N + n];
+        for (int p = w; p < parts; p += 8) s += part[(int64_t)p * N + n];
+    }
+    red[w][c] = s;
+    __syncthreads();
+    if (w || n >= N) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += red[k][c];
     static_cast<__nv_bfloat16*>(db)[n] = __float2bfloat16_rn(s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
-// parts of the rows whose column sums are taken separately: enough CTAs to fill the GPU, at least 64 rows each
-int dz_parts(int rows, int N, bool vec) {
-    const int64_t cols = vec ? (N + 255) / 256 : (N + 63) / 64;
-    int64_t p = (4 * 148 + cols - 1) / cols;
-    if (p > (rows + 63) / 64) p = (rows + 63) / 64;
+// parts of the rows whose column sums are taken separately: one round of CTAs (four an SM), at least 32 rows each
+int dz_parts(int rows, int N) {
+    const int64_t cols = (N + 255) / 256;
+    int64_t p = 4 * 148 / cols;
+    if (p > (rows + 31) / 32) p = (rows + 31) / 32;
     return (int)(p < 1 ? 1 : p);
 }
 
@@ -1090,7 +1104,7 @@ int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_fea
     const int64_t r = rows > 0 ? rows : 1;
     const int64_t dx = plan_here((int)r, in_features, out_features, EPI_STORE).bytes;
     const int64_t dw = plan_here(out_features, in_features, r, EPI_STORE).bytes;
-    *bytes = up(r * up(out_features, 8) * 2, 256) + up((int64_t)dz_parts((int)r, out_features, true) * out_features * 4, 256) +
+    *bytes = up(r * up(out_features, 8) * 2, 256) + up((int64_t)dz_parts((int)r, out_features) * out_features * 4, 256) +
              up(dx > dw ? dx : dw, 256);
     return B2S_OK;
 }
@@ -1125,21 +1139,25 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
     const bool direct = l->activation == B2S_ACT_NONE && dy_vec;
     const bool products = l->grad_x || l->grad_weight;
     Operand dz = {l->workspace, ldz};
-    const int parts = dz_parts(l->rows, l->out_features, dy_vec);  // at most what the workspace holds
+    const int parts = dz_parts(l->rows, l->out_features);
     float* part = reinterpret_cast<float*>(static_cast<unsigned char*>(l->workspace) + up((int64_t)l->rows * ldz * 2, 256));
     if (direct) dz = {l->grad_out, l->grad_out_row_stride};
     if ((products && !direct) || l->grad_bias) {
         const int per = (l->rows + parts - 1) / parts;
         const bool two = l->grad_bias && parts > 1;
-        const int width = dy_vec ? 256 : 64;  // columns per CTA
-        cudaError_t e = launch_pdl(dy_vec ? linear_dz_kernel<8> : linear_dz_kernel<2>,
-                                   dim3((unsigned)((l->out_features + width - 1) / width), (unsigned)parts), DZ_NT, 0,
+        static constexpr decltype(&linear_dz_kernel<true, ACT_NONE>) kernels[2][4] = {
+            {linear_dz_kernel<false, ACT_NONE>, linear_dz_kernel<false, ACT_RELU>, linear_dz_kernel<false, ACT_GELU>,
+             linear_dz_kernel<false, ACT_SILU>},
+            {linear_dz_kernel<true, ACT_NONE>, linear_dz_kernel<true, ACT_RELU>, linear_dz_kernel<true, ACT_GELU>,
+             linear_dz_kernel<true, ACT_SILU>}};
+        cudaError_t e = launch_pdl(kernels[dy_vec][l->activation],
+                                   dim3((unsigned)((l->out_features + 255) / 256), (unsigned)parts), DZ_NT, 0,
                                    stream, l->grad_out, l->grad_out_row_stride, l->preact, l->preact_row_stride,
-                                   (int)l->activation, (int)l->rows, (int)l->out_features, per,
+                                   (int)l->rows, (int)l->out_features, per,
                                    products && !direct ? l->workspace : nullptr, ldz, two ? part : nullptr,
                                    two ? nullptr : l->grad_bias);
         if (e == cudaSuccess && two)
-            e = launch_pdl(linear_db_kernel, dim3((unsigned)((l->out_features + 127) / 128)), 128, 0, stream,
+            e = launch_pdl(linear_db_kernel, dim3((unsigned)((l->out_features + 31) / 32)), DZ_NT, 0, stream,
                            (const float*)part, parts, (int)l->out_features, l->grad_bias);
         if (e != cudaSuccess) return cuda_fail(e);
     }

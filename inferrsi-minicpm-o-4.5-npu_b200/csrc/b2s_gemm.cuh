@@ -108,15 +108,16 @@ __device__ __forceinline__ float act_apply(float z, int act) {
                            : act == ACT_GELU ? act_apply<ACT_GELU>(z) : act == ACT_SILU ? act_apply<ACT_SILU>(z) : z;
 }
 // The slope of a pre-activation that came back from fp16: past 65504 (infinite there) it is what it is at 6e4.
-__device__ __forceinline__ float act_slope(float z, int act) {
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
     z = fabsf(z) > 6.0e4f ? copysignf(6.0e4f, z) : z;
-    if (act == ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (act == ACT_GELU) {
+    if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+    if (ACT == ACT_GELU) {
         float e;
         const float q = 0.5f * gelu_tail(z, &e);
         return __fmaf_rn(0.398942280401432678f * z, e, z > 0.0f ? 1.0f - q : q);
     }
-    if (act == ACT_SILU) {
+    if (ACT == ACT_SILU) {
         const float s = __fdividef(1.0f, 1.0f + ex2(-1.44269504088896341f * z));
         return s * (1.0f + z * (1.0f - s));
     }
