@@ -94,6 +94,27 @@ def test_gradient(pkg, n, k, m, activation):
             assert bool(((got.double() - want).abs() <= tol * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs() + 2.0 ** -60).all())
 
 
+@pytest.mark.parametrize("activation", [None, "silu"])
+@pytest.mark.parametrize("shift,wide", [(1, 0), (2, 0), (3, 1), (0, 1), (1, 8), (5, 3)])
+def test_gradient_of_unaligned_rows(pkg, activation, shift, wide):
+    """The output's gradient (and the residual) off their 16-byte alignment: every element as from aligned rows."""
+    n, k, m = 301, 136, 520
+    x, w, b, r, dy = operands(n, k, m, 4)
+
+    def off(v):
+        buf = torch.full((n * (m + wide) + shift,), 77.0, device=DEV, dtype=torch.bfloat16)
+        view = buf[shift:].view(n, m + wide)[:, :m]
+        return view.copy_(v)
+
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+    y = pkg.projection.linear(*leaves, activation=activation, residual=r)
+    want = torch.autograd.grad(y, leaves, dy)
+    z = pkg.projection.linear(*leaves, activation=activation, residual=off(r))
+    assert torch.equal(y, z)
+    for got, exact in zip(torch.autograd.grad(z, leaves, off(dy)), want):
+        assert torch.equal(got, exact)
+
+
 @pytest.mark.parametrize("activation", [None, "relu", "gelu", "silu"])
 def test_each_gradient_alone_and_twice(pkg, activation):
     """Any subset of the inputs, the same bits each time."""
