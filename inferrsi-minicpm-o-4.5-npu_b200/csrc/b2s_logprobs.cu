@@ -825,11 +825,12 @@ __global__ void __launch_bounds__(LPW_NT, 4) token_logprobs_warp_kernel(const Lp
     }
 }
 
-// dx for one chunk of a row per CTA.
+// dx for one chunk of a row per G threads: a CTA (bound by HBM: 2048 x 151936 bf16 188 us, the copy's rate), or, for many
+// short rows, a whole row per warp.
 constexpr int LPG_NT = 256;
 constexpr int LPG_U = 8;  // vectors in flight per thread
-template <typename E>
-__global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void* logits, int64_t stride, int V,
+template <typename E, int G>
+__global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void* logits, int64_t stride, int rows, int V,
                                                                      int chunk_vecs, int chunks, const int64_t* tokens,
                                                                      float c, float inv_t, const float4* stats,
                                                                      const float* g_lp, const float* g_h, void* out,
@@ -837,7 +838,11 @@ __global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void*
     constexpr int EPV = LpElem<E>::EPV;
     constexpr int ES = 16 / EPV;
     pdl_wait_then_release();
-    const int r = (int)(blockIdx.x / chunks), ch = (int)(blockIdx.x % chunks);
+    int r = (int)(blockIdx.x / chunks), ch = (int)(blockIdx.x % chunks), tid = threadIdx.x;
+    if constexpr (G == 32) {  // a row per warp, in one chunk
+        r = (int)blockIdx.x * (LPG_NT / 32) + (int)(threadIdx.x >> 5), ch = 0, tid = threadIdx.x & 31;
+        if (r >= rows) return;
+    }
     const unsigned char* rowp = static_cast<const unsigned char*>(logits) + (int64_t)r * stride * ES;
     unsigned char* outp = static_cast<unsigned char*>(out) + (int64_t)r * ostride * ES;
     const float4 st = stats[r];
@@ -848,17 +853,17 @@ __global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void*
     const int nv = (V - nh) / EPV;
     const bool same = ((reinterpret_cast<uintptr_t>(rowp) - reinterpret_cast<uintptr_t>(outp)) & 15) == 0;
     if (ch == 0) {
-        if ((int)threadIdx.x < nh) LpElem<E>::st(outp, threadIdx.x, g.at(LpElem<E>::ld(rowp, threadIdx.x), threadIdx.x, c));
-        const int i = nh + nv * EPV + (int)threadIdx.x;
+        if (tid < nh) LpElem<E>::st(outp, tid, g.at(LpElem<E>::ld(rowp, tid), tid, c));
+        const int i = nh + nv * EPV + tid;
         if (i < V) LpElem<E>::st(outp, i, g.at(LpElem<E>::ld(rowp, i), i, c));
     }
     const int v1 = min(nv, (ch + 1) * chunk_vecs), tv = g.t >= nh ? (g.t - nh) / EPV : -1;
     const uint4* vp = reinterpret_cast<const uint4*>(rowp + (int64_t)nh * ES);
-    for (int v0 = ch * chunk_vecs + (int)threadIdx.x; v0 < v1; v0 += LPG_U * LPG_NT) {
+    for (int v0 = ch * chunk_vecs + tid; v0 < v1; v0 += LPG_U * G) {
         uint4 q[LPG_U];
 #pragma unroll
         for (int u = 0; u < LPG_U; ++u) {
-            const int v = v0 + u * LPG_NT;
+            const int v = v0 + u * G;
             if (v < v1) {
                 if (same) {
                     q[u] = ldg_stream(vp + v);
@@ -872,7 +877,7 @@ __global__ void __launch_bounds__(LPG_NT) token_logprobs_grad_kernel(const void*
         }
 #pragma unroll
         for (int u = 0; u < LPG_U; ++u) {
-            const int v = v0 + u * LPG_NT;
+            const int v = v0 + u * G;
             if (v < v1) {
                 float x[EPV];
                 LpElem<E>::unpack(q[u], x);
@@ -1017,19 +1022,29 @@ int b2s_token_logprobs_grad(const void* logits, int32_t logits_dtype, int32_t ro
         (reinterpret_cast<uintptr_t>(logits) & (es - 1)) || (reinterpret_cast<uintptr_t>(grad_logits) & (es - 1)))
         return B2S_ERR_INVALID;
     const int epv = 16 / es;
-    const int chunk_vecs = LPG_NT * 8;
-    const int64_t chunks = ((int64_t)vocab / epv + chunk_vecs - 1) / chunk_vecs;
+    int sms = 0;
+    const cudaError_t de = device_sms(&sms);
+    if (de != cudaSuccess) return cuda_fail(de);
+    const int64_t row_bytes = (int64_t)vocab * es;
+    // A CTA / a warp per row (us): 300 x 2040 bf16 3.6 / 3.9, 600 x 2040 4.3 / 4.0, 2000 x 4000 10.7 / 10.2, 2000 x 6562 13.0 /
+    // 15.3, 4000 x 6562 25.6 / 24.9, 8192 x 8000 53.1 / 49.8, 30000 x 1000 80.7 / 28.4, 8192 x 6562 fp32 65.2 / 72.7.
+    const bool warp = row_bytes <= 8 * 1024 ? rows >= 4 * sms : row_bytes <= 16 * 1024 && rows >= 24 * sms;
+    const int chunk_vecs = warp ? vocab / epv + 1 : LPG_NT * LPG_U;
+    const int64_t chunks = warp ? 1 : ((int64_t)vocab / epv + chunk_vecs - 1) / chunk_vecs;
     const int64_t nch = chunks < 1 ? 1 : chunks;
     if (nch * rows > INT32_MAX) return B2S_ERR_UNSUPPORTED;
     const float c = lp_scale(temperature), inv = (float)(1.0 / (double)temperature);
     const float4* st = reinterpret_cast<const float4*>(stats);
-    const cudaError_t e =
-        logits_dtype == B2S_DTYPE_BF16
-            ? launch(token_logprobs_grad_kernel<__nv_bfloat16>, nch * rows, LPG_NT, 0u, 0, stream, logits, row_stride,
-                     (int)vocab, chunk_vecs, (int)nch, tokens, c, inv, st, grad_logprob, grad_entropy, grad_logits,
-                     grad_row_stride)
-            : launch(token_logprobs_grad_kernel<float>, nch * rows, LPG_NT, 0u, 0, stream, logits, row_stride, (int)vocab,
-                     chunk_vecs, (int)nch, tokens, c, inv, st, grad_logprob, grad_entropy, grad_logits, grad_row_stride);
+    const int64_t per = warp ? LPG_NT / 32 : 1, blocks = (nch * rows + per - 1) / per;
+    auto go = [&](auto kernel) {
+        return launch(kernel, blocks, LPG_NT, 0u, 0, stream, logits, row_stride, (int)rows, (int)vocab, chunk_vecs, (int)nch,
+                      tokens, c, inv, st, grad_logprob, grad_entropy, grad_logits, grad_row_stride);
+    };
+    cudaError_t e;
+    if (logits_dtype == B2S_DTYPE_BF16)
+        e = warp ? go(token_logprobs_grad_kernel<__nv_bfloat16, 32>) : go(token_logprobs_grad_kernel<__nv_bfloat16, LPG_NT>);
+    else
+        e = warp ? go(token_logprobs_grad_kernel<float, 32>) : go(token_logprobs_grad_kernel<float, LPG_NT>);
     return e == cudaSuccess ? B2S_OK : cuda_fail(e);
 }
 

@@ -250,7 +250,9 @@ def test_many_short_rows_special_values(pkg, n, V, shift, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("n,V,pad,shift", [(300, 33, 0, 0), (310, 700, 3, 1), (1800, 6562, 0, 0)])
+@pytest.mark.parametrize("n,V,pad,shift", [(300, 33, 0, 0), (310, 700, 3, 1), (1800, 6562, 0, 0), (601, 1, 0, 0),
+                                           (605, 2, 1, 0), (593, 700, 0, 0), (603, 1023, 0, 0), (607, 2041, 3, 1),
+                                           (3553, 4000, 8, 5), (3555, 6562, 0, 0)])
 def test_many_short_rows_gradient(pkg, n, V, pad, shift, dtype):
     x, t = rows_of(n, V, dtype, V, pad, shift)
     x[0, ::2] = float("-inf")
