@@ -4,10 +4,9 @@
 // With z = x / T and c = log2(e) / T, everything is kept in base 2 around a reference R = fl(m c) of the running
 // maximum m: y_i = fma(x_i, c, -R) (one rounding of the exact x_i c - R, and R drops out of every difference, so R
 // need not be exact), S = sum 2^y, U = sum 2^y y.  Then logprob = (y_t - log2 S) ln 2 and the entropy
-// H = (log2 S - U / S) ln 2: U <= 0, so H is a sum of two non-negative terms and nothing cancels.  S and U are fp32
+// H = (log2 S - U / S) ln 2: U <= 0 but for R's rounding (at most 2^-5 of S), so that nothing cancels.  S and U are fp32
 // per thread (a few hundred terms each) and merged pairwise; a merge of two references shifts y by R_a - R_b.
-// Rows whose reference overflows (|m| c beyond fp32: a mask of the type's lowest value throughout) use
-// y = (x - m) c instead.  A masked (-inf) element adds nothing; a row with nothing left has logprob -inf, entropy 0
+// Beyond |R| = 2^20 (finite masks, logits by the million, small temperatures) y = (x - m) c instead (lp_far).  A masked (-inf) element adds nothing; a row with nothing left has logprob -inf, entropy 0
 // and gradient 0; NaN or +inf anywhere makes the row NaN, as a softmax gives it.
 //
 // Forward, one pass over the row by bulk copies into a ring of shared-memory chunks (a thread's registers do not bound
@@ -253,7 +252,7 @@ __device__ __forceinline__ void lp_thread_batch(LpThread& s, const uint4 (&q)[LP
     }
     if (!(fabsf(s.m) <= 3.402823466e38f)) return;  // NaN or +inf (the row's outcome), or nothing but -inf so far
     const float R = __fmul_rn(s.m, c);
-    if (fabsf(R) <= 3.0e38f) {
+    if (!lp_far(R)) {
         const float2 c2 = make_float2(c, c), r2 = make_float2(-R, -R);
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {
@@ -268,7 +267,7 @@ __device__ __forceinline__ void lp_thread_batch(LpThread& s, const uint4 (&q)[LP
                 s.U = __ffma2_rn(e, y, s.U);
             }
         }
-    } else {  // a reference that overflows: (x - m) c
+    } else {  // a reference far from zero: (x - m) c
         const float2 c2 = make_float2(c, c), m2 = make_float2(-s.m, -s.m);
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {

@@ -38,7 +38,7 @@ __device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity) {
     return false;
 }
 
-// m: maximum of the raw values (NaN once one was seen); S = sum 2^y, U = sum 2^y y with y relative to ref(m).
+// m: maximum of the raw values (NaN once one was seen); S = sum 2^y, U = sum 2^y y with y relative to m (lp_y).
 struct LpState {
     float m, S, U;
 };
@@ -49,18 +49,24 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// y of x against the maximum m: fma(x, c, -fl(m c)), or (x - m) c where m c overflows; never below -200 (2^-200 is
-// nothing beside the maximum's 1, and 0 * -inf would be NaN).
+// Whether a reference R = fl(m c) is far from zero.  Near, y = fma(x, c, -R) is one rounding of x c - R, and R's own
+// rounding, at most 2^-5, drops out of every difference.  Far, that rounding would be what 2^y is made of (it passes
+// fp32's exponents from |R| about 2^31 on, and R overflows beyond), so y = (x - m) c there, whose maximum is exactly 0.
+// Every user of a reference asks here, so that all of them take the same form.
+__device__ __forceinline__ bool lp_far(float R) { return !(fabsf(R) <= 1048576.0f); }
+
+// y of x against the maximum m; never below -200 (2^-200 is nothing beside the maximum's 1, and 0 * -inf would be NaN).
 __device__ __forceinline__ float lp_y(float x, float m, float c) {
     const float R = __fmul_rn(m, c);
-    const float y = fabsf(R) <= 3.0e38f ? __fmaf_rn(x, c, -R) : __fmul_rn(__fsub_rn(x, m), c);
+    const float y = lp_far(R) ? __fmul_rn(__fsub_rn(x, m), c) : __fmaf_rn(x, c, -R);
     return fmaxf(y, -200.0f);
 }
 
-// The shift of y when the maximum goes from `from` to `to` >= from (both finite).
+// The shift of y when the maximum goes from `from` to `to` >= from (both finite), each with its own form.
 __device__ __forceinline__ float lp_shift(float from, float to, float c) {
     const float Rf = __fmul_rn(from, c), Rt = __fmul_rn(to, c);
-    const float d = fabsf(Rf) <= 3.0e38f && fabsf(Rt) <= 3.0e38f ? __fsub_rn(Rf, Rt) : __fmul_rn(__fsub_rn(from, to), c);
+    const float d = lp_far(Rt) ? (lp_far(Rf) ? __fmul_rn(__fsub_rn(from, to), c) : -__fmaf_rn(to, c, -Rf))
+                               : (lp_far(Rf) ? __fmaf_rn(from, c, -Rt) : __fsub_rn(Rf, Rt));
     return fmaxf(d, -400.0f);
 }
 
@@ -126,7 +132,7 @@ __device__ __forceinline__ void lp_add_many(LpState& s, const float (&x)[N], flo
         S += e;
         U = __fmaf_rn(e, y, U);
     }
-    if (!(fabsf(U) <= 3.0e38f)) {  // a masked element (0 * -inf), or a reference that overflows
+    if (lp_far(R) || !(fabsf(U) <= 3.0e38f)) {  // a reference far from zero, or a masked element (0 * -inf)
         S = U = 0.0f;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -139,8 +145,8 @@ __device__ __forceinline__ void lp_add_many(LpState& s, const float (&x)[N], flo
     s.U += U;
 }
 
-// The same without the second form: every y bounded below, the reference that overflows chosen per call.  Short code for
-// the products' epilogue, whose arithmetic the MMAs hide.
+// The same without the second pass: every y bounded below, the form of y chosen per call.  Short code for the products'
+// epilogue, whose arithmetic the MMAs hide.
 template <int N>
 __device__ __forceinline__ void lp_add_any(LpState& s, const float (&x)[N], float c) {
     float bm = x[0];
@@ -153,7 +159,7 @@ __device__ __forceinline__ void lp_add_any(LpState& s, const float (&x)[N], floa
     }
     if (m > s.m) lp_rescale(s, m, c);
     const float R = __fmul_rn(s.m, c);
-    const bool far = !(fabsf(R) <= 3.0e38f);
+    const bool far = lp_far(R);
     const float mul = c, off = far ? s.m : R, pre = far ? 1.0f : c, post = far ? mul : 1.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -185,7 +191,7 @@ __device__ __forceinline__ LpFinal lp_final(const LpState& s, float c) {
         f.m = f.log2S = f.entropy = __int_as_float(0x7fffffff);
     } else {
         f.log2S = log2f(s.S);
-        f.entropy = fmaxf((f.log2S - s.U / s.S) * 0.693147180559945309f, 0.0f);
+        f.entropy = fmax_nan((f.log2S - s.U / s.S) * 0.693147180559945309f, 0.0f);
     }
     return f;
 }
@@ -194,10 +200,12 @@ __device__ __forceinline__ LpFinal lp_final(const LpState& s, float c) {
 __device__ __forceinline__ float lp_value(float x, const LpFinal& f, float c) {
     if (f.m != f.m) return f.m;
     if (x == f_ninf()) return x;
-    const float y = fabsf(f.R) <= 3.0e38f ? __fmaf_rn(x, c, -f.R) : __fmul_rn(__fsub_rn(x, f.m), c);
-    // a value so low that y overflows in base 2 may still be a number in base e (log2 S is nothing beside it)
-    if (!(fabsf(y) <= 3.0e38f)) return __fmul_rn(__fsub_rn(x, f.m), c * 0.693147180559945309f);
-    return (y - f.log2S) * 0.693147180559945309f;
+    const float y = lp_far(f.R) ? __fmul_rn(__fsub_rn(x, f.m), c) : __fmaf_rn(x, c, -f.R);
+    if (fabsf(y) <= 3.0e38f) return (y - f.log2S) * 0.693147180559945309f;
+    // a value so low that y overflows in base 2 may still be a number in base e (log2 S is nothing beside it), even where
+    // x - m overflows
+    const float ce = c * 0.693147180559945309f;
+    return ce <= 1.0f ? __fmaf_rn(x, ce, -__fmul_rn(f.m, ce)) : __fmul_rn(__fsub_rn(x, f.m), ce);
 }
 
 // The gradient of g_lp logprob + g_h entropy with respect to one value of a row:
@@ -214,7 +222,7 @@ struct LpGrad {
         scale = -(glp + gh * st.w) * inv_t;
         slope = -gh * 0.693147180559945309f * inv_t;
         bump = glp * inv_t;
-        far = !(fabsf(R) <= 3.0e38f) && !none;
+        far = lp_far(R) && !none;
         if (none) {
             R = 0.0f;
             log2S = 1000.0f;  // p = 0 for every value that is left: there is none
