@@ -936,8 +936,10 @@ const auto& linear_grad_op() {
 }
 
 // Under stream capture: a leaf whose gradient accumulator an eager graph on another stream keeps alive would tie the
-// captured backward pass to that stream, which invalidates the capture deep in the engine.  Said here instead.
+// captured backward pass to that stream, which invalidates the capture deep in the engine.  Said here instead.  Tracing
+// (Meta and fake tensors) works on machines without a driver, where there is nothing to ask.
 void check_capture(at::TensorList leaves) {
+    if (!at::hasCUDA()) return;
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
     for (const Tensor& t : leaves) {
         if (!needs_grad(t) || !t.is_leaf()) continue;
