@@ -880,6 +880,15 @@ using torch::autograd::variable_list;
 bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool needs_grad(const optional<Tensor>& t) { return t.has_value() && needs_grad(*t); }
 Tensor or_none(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+// A status word for the backward pass to add to.  Not among the saved tensors: it is an output, and callers that read and
+// clear it between the passes change it in place.
+void keep_status(AutogradContext* ctx, const optional<Tensor>& status) {
+    if (status.has_value() && status->defined()) ctx->saved_data["status"] = *status;
+}
+optional<Tensor> kept_status(AutogradContext* ctx) {
+    const auto it = ctx->saved_data.find("status");
+    return it == ctx->saved_data.end() ? optional<Tensor>() : optional<Tensor>(it->second.toTensor());
+}
 optional<Tensor> or_null(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
 
 // There is a backward pass only: an input that carries a tangent is refused, as the kernels would drop it.
@@ -997,7 +1006,8 @@ struct HeadLogprobsNode : public torch::autograd::Function<HeadLogprobsNode> {
                                  double temperature, const optional<Tensor>& status) {
         at::AutoDispatchBelowADInplaceOrView below;
         auto [lp, ent, stats] = lmhead_logprobs_op().call(hidden, head, tokens, temperature, true, status);
-        ctx->save_for_backward({hidden, head, tokens, stats, or_none(status)});
+        ctx->save_for_backward({hidden, head, tokens, stats});
+        keep_status(ctx, status);
         ctx->saved_data["temperature"] = temperature;
         ctx->mark_non_differentiable({stats});
         ctx->set_materialize_grads(false);
@@ -1012,7 +1022,7 @@ struct HeadLogprobsNode : public torch::autograd::Function<HeadLogprobsNode> {
             at::AutoDispatchBelowADInplaceOrView below;
             auto [dh, dw] = lmhead_logprobs_grad_op().call(saved[0], saved[1], saved[2], saved[3], or_null(g[0]),
                                                            or_null(g[1]), ctx->saved_data["temperature"].toDouble(),
-                                                           want_h, want_w, or_null(saved[4]));
+                                                           want_h, want_w, kept_status(ctx));
             if (want_h) out[0] = dh;
             if (want_w) out[1] = dw;
         }
@@ -1039,7 +1049,8 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
                                  const optional<Tensor>& residual, int64_t activation, const optional<Tensor>& status) {
         at::AutoDispatchBelowADInplaceOrView below;
         auto [out, pre] = linear_op().call(x, weight, bias, residual, activation, activation != B2S_ACT_NONE, status);
-        ctx->save_for_backward({x, weight, activation != B2S_ACT_NONE ? pre : Tensor(), or_none(status)});
+        ctx->save_for_backward({x, weight, activation != B2S_ACT_NONE ? pre : Tensor()});
+        keep_status(ctx, status);
         ctx->saved_data["activation"] = activation;
         // the graph's edges are numbered over the tensors that were there
         ctx->saved_data["bias"] = bias.has_value() && bias->defined();
@@ -1059,7 +1070,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
             at::AutoDispatchBelowADInplaceOrView below;
             auto [dx, dw, db] = linear_grad_op().call(g[0], saved[0], saved[1], or_null(saved[2]),
                                                       ctx->saved_data["activation"].toInt(), want_x, want_w, want_b,
-                                                      or_null(saved[3]));
+                                                      kept_status(ctx));
             if (want_x) out[0] = dx;
             if (want_w) out[1] = dw;
             if (want_b) out[2] = db;

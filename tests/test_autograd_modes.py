@@ -65,3 +65,18 @@ def test_traced_with_fake_tensors(pkg, name):
         f, inputs = calls(pkg._native.ops(), "cuda")[name]
         y = f(*[v.requires_grad_(True) for v in inputs])
     assert y.shape[0] == 3 and y.device.type == "cuda" and y.requires_grad
+
+
+def test_status_word_cleared_between_the_passes(pkg):
+    """The word is an output: reading and clearing it after a forward, or sharing it by two, leaves the backward alone."""
+    ops = pkg._native.ops()
+    st, t = meta(1, dtype=torch.int32), meta(3, dtype=torch.int64)
+    x, h, w = (v.requires_grad_(True) for v in (meta(3, 40, dtype=torch.float32), meta(3, 16), meta(40, 16)))
+    first = [ops.token_logprobs(x, t, 1.0, 0, False, st)[0], ops.lmhead_logprobs(h, w, t, 1.0, False, st)[0],
+             ops.linear(h, w, None, None, 2, False, st)[0]]
+    st.zero_()
+    second = [ops.lmhead_logprobs(h, w, t, 1.0, False, st)[0], ops.linear(h, w, None, None, 0, False, st)[0]]
+    st.zero_()
+    for y in first + second:
+        y.sum().backward()
+    assert h.grad.shape == h.shape and w.grad.shape == w.shape and x.grad.shape == x.shape
