@@ -892,11 +892,12 @@ optional<Tensor> kept_status(AutogradContext* ctx) {
 optional<Tensor> or_null(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
 
 // There is a backward pass only: an input that carries a tangent is refused, as the kernels would drop it.
-void refuse_tangents(at::TensorList inputs, const char* what) {
-    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-    for (const Tensor& t : inputs)
-        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what,
-                                    " has no forward-mode derivative");
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const optional<Tensor>& t) { return t.has_value() && has_tangent(*t); }
+template <typename... T>
+void refuse_tangents(const char* what, const T&... inputs) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...) || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), what,
+                                " has no forward-mode derivative");
 }
 
 // The gradients have none of their own: under create_graph they carry a node that says so if it is ever run.
@@ -991,7 +992,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_autogr
                                                                                    double temperature, int64_t top,
                                                                                    bool want_stats,
                                                                                    const optional<Tensor>& status) {
-    refuse_tangents({logits}, "token_logprobs");
+    refuse_tangents("token_logprobs", logits);
     if (!at::GradMode::is_enabled() || !needs_grad(logits)) {
         at::AutoDispatchBelowADInplaceOrView below;
         return token_logprobs_op().call(logits, tokens, temperature, top, want_stats, status);
@@ -1034,7 +1035,7 @@ struct HeadLogprobsNode : public torch::autograd::Function<HeadLogprobsNode> {
 std::tuple<Tensor, Tensor, Tensor> lmhead_logprobs_autograd(const Tensor& hidden, const Tensor& head,
                                                             const Tensor& tokens, double temperature, bool want_stats,
                                                             const optional<Tensor>& status) {
-    refuse_tangents({hidden, head}, "lmhead_logprobs");
+    refuse_tangents("lmhead_logprobs", hidden, head);
     if (!at::GradMode::is_enabled() || !(needs_grad(hidden) || needs_grad(head))) {
         at::AutoDispatchBelowADInplaceOrView below;
         return lmhead_logprobs_op().call(hidden, head, tokens, temperature, want_stats, status);
@@ -1084,7 +1085,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
 std::tuple<Tensor, Tensor> linear_autograd(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
                                            const optional<Tensor>& residual, int64_t activation, bool want_preact,
                                            const optional<Tensor>& status) {
-    refuse_tangents({x, weight, or_none(bias), or_none(residual)}, "linear");
+    refuse_tangents("linear", x, weight, bias, residual);
     if (!at::GradMode::is_enabled() ||
         !(needs_grad(x) || needs_grad(weight) || needs_grad(bias) || needs_grad(residual))) {
         at::AutoDispatchBelowADInplaceOrView below;
