@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define B2S_ABI_VERSION 6
+#define B2S_ABI_VERSION 7
 
 /* return codes */
 #define B2S_OK 0
@@ -49,7 +49,7 @@ extern "C" {
 /* bits of the device status word */
 #define B2S_STATUS_HISTORY_RANGE 1u /* a history id >= vocab was ignored (the row is still sampled) */
 #define B2S_STATUS_TOPK_LIMIT 2u    /* a row's top_k exceeded max_top_k; the row returned PAD */
-#define B2S_STATUS_WAIT_TIMEOUT 4u  /* a bounded device wait gave up; the row returned PAD */
+#define B2S_STATUS_WAIT_TIMEOUT 4u  /* a bounded device wait gave up; the row returned PAD (log probabilities, products: NaN) */
 #define B2S_STATUS_COUNT_LIMIT 8u   /* a token repeated more than alpha_len-1 times; its count was clamped */
 #define B2S_STATUS_SHARD_INCOMPLETE 16u /* a shard's candidate list overflowed `cap` or failed; the row returned PAD */
 #define B2S_STATUS_TOKEN_RANGE 32u  /* a token id >= vocab was taken as no token (log probabilities) */
@@ -406,6 +406,15 @@ typedef struct b2s_linear_grad_args {
 } b2s_linear_grad_args;
 int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes);
 int b2s_linear_grad(const b2s_linear_grad_args* args, void* stream);
+
+/*
+ * The bound of each device wait inside the log-probability and projection kernels, in SM clocks: sets it for the calls
+ * of this process that follow (clocks >= 0, at most the default of about a quarter of a second); a negative argument only
+ * asks.  previous (optional) gets the bound before.  A wait that gives up sets B2S_STATUS_WAIT_TIMEOUT and makes what was not finished NaN
+ * (ranks and ids of alternatives -1).  0: calls start no copies and no products and give up at once, which shows a caller
+ * what that looks like.  A captured call keeps the bound it was captured with.  (ABI 7)
+ */
+int b2s_wait_limit(int64_t clocks, int64_t* previous);
 
 /* Human-readable text of a B2S_ERR_* code, and of the last CUDA error seen by this library. */
 const char* b2s_error_string(int code);

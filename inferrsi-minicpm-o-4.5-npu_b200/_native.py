@@ -135,6 +135,7 @@ CAPI_SIGNATURES = {
     "b2s_linear_grad_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                                  ctypes.POINTER(ctypes.c_int64)]),
     "b2s_linear_grad": (ctypes.c_int, [ctypes.POINTER(LinearGradArgs), ctypes.c_void_p]),
+    "b2s_wait_limit": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)]),
     "b2s_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "b2s_last_cuda_error": (ctypes.c_char_p, []),
     "b2s_abi_version": (ctypes.c_int, []),

@@ -52,6 +52,11 @@ __device__ __forceinline__ bool piece_at(const GemmArgs& a, int i, Piece* p) {
     return true;
 }
 
+template <int N>
+__device__ __forceinline__ void fill_nan(float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = __int_as_float(0x7fffffff);
+}
 // Whether a block of 32 columns from n is copied as 16-byte vectors.
 __device__ __forceinline__ bool vec_block(const GemmArgs& a, int n, int aligned) { return aligned && n + 32 <= a.N; }
 // The residual's block of 32 columns from n of the 32 rows from row0.
@@ -62,9 +67,9 @@ __device__ __forceinline__ void residual_fetch(const GemmArgs& a, uint32_t (&q)[
 }
 
 // The epilogue of one warp: 32 rows of a tile, columns [n0, n0 + COLS) from tensor memory at `tm` (lane = row).  `rq`:
-// the residual's first block.
+// the residual's first block.  Not `good`: the accumulator was given up, and NaN takes its place.
 template <int TM, int TN, int EPI>
-__device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, int row0, int n0, int nt, int slot,
+__device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, bool good, int row0, int n0, int nt, int slot,
                                               unsigned char* st, uint32_t (&rq)[16]) {
     constexpr int COLS = TN / 2;
     const int lane = threadIdx.x & 31;
@@ -76,7 +81,8 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
 #pragma unroll 1
             for (int q = 0; q < COLS / 32; ++q) {
                 float v[32];
-                tmem_ld32(tm + 32u * q, v);
+                if (good) tmem_ld32(tm + 32u * q, v);
+                else fill_nan(v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     *stage_at(st, lane, j) = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
@@ -109,7 +115,8 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, in
                 __syncwarp();
             }
             float v[32];
-            tmem_ld32(tm + 32u * q, v);
+            if (good) tmem_ld32(tm + 32u * q, v);
+            else fill_nan(v);
             if constexpr (EPI == EPI_LINEAR) {
                 if (a.bias) {
                     const float b = lane < cols ? bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + n + lane)) : 0.0f;
@@ -263,7 +270,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
     if (warp == GM_EPI) {
         int s = 0, it = 0;
         uint32_t ph = 1;  // parity of `empty`'s last phase: the first round finds every stage free
-        bool ok = true;
+        bool ok = a.wait > 0;
         const uint32_t bar0 = CG == 2 ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
         Piece p;
         for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
@@ -271,7 +278,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
             tile_of<TM>(a, p.tile, &mt, &nt);
             const int m0 = mt * TM + (int)rank * GM_M, n0 = nt * TN + (int)rank * BN;
             for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
-                if (!gm_wait<false>(&empty[s], ph)) {
+                if (!__all_sync(0xffffffffu, gm_wait<false>(&empty[s], ph, a.wait))) {
                     *fail = 1;
                     ok = false;
                     break;
@@ -309,7 +316,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         // the first CTA's last signals to this CTA's `empty` have landed before it leaves
         if (CG == 2 && ok)
             for (int k = it > ST ? it - ST : 0; k < it; ++k)
-                if (!gm_wait<false>(&empty[k % ST], (uint32_t)(k / ST) & 1u)) {
+                if (!gm_wait<false>(&empty[k % ST], (uint32_t)(k / ST) & 1u, a.wait)) {
                     *fail = 1;
                     break;
                 }
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         if (rank == 0) {  // MMAs
             int s = 0, it = 0;
             uint32_t ph = 0;
-            bool ok = true;
+            bool ok = a.wait > 0;
             const uint64_t da0 = AMN ? umma_desc_mn128(smem_u32(sm)) : umma_desc_sw128(smem_u32(sm));
             const uint64_t db0 = BMN ? umma_desc_mn128(smem_u32(sm) + GM_A_BYTES) : umma_desc_sw128(smem_u32(sm) + GM_A_BYTES);
             auto commit = [&](uint64_t* bar) {
@@ -329,7 +336,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
             for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
                 for (int k0 = p.kb0; ok && k0 < p.kb1; k0 += SEGMENT, ++g) {
                     const int acc = g & 1, k1 = min(p.kb1, k0 + SEGMENT);
-                    if (g >= 2 && !gm_wait<CG == 2>(&tempty[acc], (uint32_t)(g / 2 - 1) & 1u)) {
+                    if (g >= 2 && !__all_sync(0xffffffffu, gm_wait<CG == 2>(&tempty[acc], (uint32_t)(g / 2 - 1) & 1u, a.wait))) {
                         *fail = 1;
                         ok = false;
                         break;
@@ -338,7 +345,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                     const uint32_t d = tmem + (uint32_t)(acc * TN);
                     uint32_t more = 0;
                     for (int kb = k0; kb < k1; ++kb, ++it) {
-                        if (!gm_wait<false>(&full[s], ph)) {
+                        if (!__all_sync(0xffffffffu, gm_wait<false>(&full[s], ph, a.wait))) {
                             *fail = 1;
                             ok = false;
                             break;
@@ -368,43 +375,41 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                 }
             }
             if (lane == 0) *consumed = it;
-            if (*fail) {
-                if (elect_one()) commit(drain);
-                __syncwarp();
-                gm_wait<false>(drain, 0u);
-            }
         }
     } else {
         Piece p;
         int g = 0;
-        bool ok = true;
+        bool ok = a.wait > 0;
+        if (!ok) *fail = 1;
         const int half = warp >> 2;
         const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * (TN / 2));
         auto take = [&]() {  // the next accumulator
-            ok = __all_sync(0xffffffffu, gm_wait<false>(&tfull[g & 1], (uint32_t)(g / 2) & 1u)) && !*fail;
+            ok = ok && __all_sync(0xffffffffu, gm_wait<false>(&tfull[g & 1], (uint32_t)(g / 2) & 1u, a.wait) && !*fail);
             if (!ok) *fail = 1;
             tc_fence_after();
             return ok;
         };
         auto give = [&]() {
+            if (!ok) return;
             tc_fence_before();
             if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[g & 1]), 0));
             else mbar_arrive(&tempty[g & 1]);
             ++g;
         };
-        for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
+        // once a wait gave up the pieces that are left take NaN without waiting
+        for (int i = 0; piece_at<CG>(a, i, &p); ++i) {
             int mt, nt;
             tile_of<TM>(a, p.tile, &mt, &nt);
             const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32, n0 = nt * TN + half * (TN / 2);
             if constexpr (EPI == EPI_LSE || EPI == EPI_DZ) {
                 float v[TN / 2];
-                if (!take()) break;
+                take();  // what was given up is read all the same: any values, replaced below
 #pragma unroll
                 for (int q = 0; q < TN / 64; ++q) tmem_ld32(tm + (uint32_t)((g & 1) * TN + 32 * q), v + 32 * q);
                 give();
 #pragma unroll 1
                 for (int k0 = p.kb0 + SEGMENT; k0 < p.kb1; k0 += SEGMENT) {
-                    if (!take()) break;
+                    take();
 #pragma unroll
                     for (int q = 0; q < TN / 32; ++q) {
                         uint32_t x[16];
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                     }
                     give();
                 }
-                if (!ok) break;
+                if (!ok) fill_nan(v);
                 if (EPI == EPI_LSE && p.slot >= 0) {  // a chunk of a split tile: fp32 sums, for lmhead_merge_kernel
                     const int row = row0 + lane;
                     float4* dst = reinterpret_cast<float4*>(a.partial + ((int64_t)p.slot * min(a.M, TM) + row) * TN + half * (TN / 2));
@@ -428,8 +433,8 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
             } else {
                 uint32_t rq[16];
                 if (EPI == EPI_LINEAR && p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
-                if (!take()) break;
-                epilogue_rows<TM, TN, EPI>(a, tm + (uint32_t)((g & 1) * TN), row0, n0, nt, p.slot, staging + warp * 4096, rq);
+                take();
+                epilogue_rows<TM, TN, EPI>(a, tm + (uint32_t)((g & 1) * TN), ok, row0, n0, nt, p.slot, staging + warp * 4096, rq);
                 give();
             }
         }
@@ -437,6 +442,15 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (*fail && warp == GM_EPI + 1 && rank == 0) {  // every MMA issued has completed
+        if (elect_one()) {
+            if constexpr (CG == 2) umma_commit_pair(drain);
+            else umma_commit(drain);
+        }
+        __syncwarp();
+        gm_wait<false>(drain, 0u);
+        tc_fence_before();
+    }
     if (*fail && tid == 0) {
         if (a.status) atomicOr(a.status, B2S_STATUS_WAIT_TIMEOUT);
         // loads issued but not seen landing still write this CTA's shared memory: those that the first CTA counts are
@@ -448,6 +462,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         while (globaltimer_ns() - t0 < 1000000ull) {
         }
     }
+    if (*fail) __syncthreads();  // the same for all: nothing writes it after the barrier above
     if constexpr (CG == 2) {  // neither CTA leaves while the other may signal it or its MMAs read its shared memory
         __syncwarp();
         cluster_arrive_release();
@@ -637,6 +652,7 @@ Plan plan_here(int M, int N, int64_t K, int epi) {
 template <int CG, int TN, bool AMN, bool BMN, int EPI>
 int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, const Plan& p, void* stream) {
     constexpr int TM = CG * GM_M;
+    a.wait = wait_limit();
     CUtensorMap amap, bmap;
     int rc = AMN ? tensor_map_2d(&amap, A.base, a.M, K, A.stride, 64, GM_KB)
                  : tensor_map_2d(&amap, A.base, K, a.M, A.stride, GM_KB, GM_M);

@@ -15,8 +15,9 @@
 // adds them in k order and runs the epilogue, so the result does not depend on timing.  Rows go to and from global memory through a swizzled 4 KB block of shared memory per
 // warp, whole 128-byte lines at a time.  The epilogues are loops over 32 columns with short bodies: unrolled over a
 // tile, with every activation inlined per element, they ran from beyond the instruction cache and a 128 x 256 tile took
-// 17 to 47 us.  Every wait is bounded; a wait that gives up ends all roles,
-// waits (bounded) for copies and MMAs in flight, and sets B2S_STATUS_WAIT_TIMEOUT.
+// 17 to 47 us.  Every wait is bounded; a wait that gives up ends the loads and the MMAs, makes NaN of every accumulator
+// that was not complete (in the output, or in the sums and states that the following kernels read, which make NaN of them
+// in turn), waits (bounded) for copies and MMAs in flight, and sets B2S_STATUS_WAIT_TIMEOUT.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -56,6 +57,7 @@ struct GemmArgs {
     int M, N, nkb, tiles_m, tiles_n;
     // full waves of whole tiles, then `rest` tiles in `split` chunks of `chunk` k blocks each (split 1: whole tiles)
     int waves, rest, split, chunk;
+    long long wait;  // clocks a wait takes at most; 0: nothing is loaded or multiplied and the product counts as given up
     float* partial;  // split > 1: [split][rest][min(M, rows of a tile)][TN] fp32
     uint32_t* status;
     // EPI_LINEAR, EPI_STORE, EPI_DZ: the output [M, N] bf16

@@ -55,6 +55,9 @@ cudaError_t device_sms(int* sms) {
     return e;
 }
 
+static std::atomic<long long> g_wait_limit{GM_WAIT};
+long long wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }
+
 namespace {
 
 constexpr int LP_CAP = 512;      // candidate list entries per CTA
@@ -200,6 +203,7 @@ struct LpShared : std::conditional_t<TOP, LpLists, LpNoLists> {
     float wS[WARPS], wU[WARPS];
     int wcount[WARPS];
     int failed;
+    int loaded;  // chunks asked for, by thread 0
     LpState total[8];  // the cluster's states and counts, in its first CTA
     int total_count[8];
 };
@@ -209,6 +213,7 @@ struct LpArgs {
     int64_t stride;
     int V, per, top, stages;
     float c;
+    long long wait;  // clocks a wait takes at most; 0: nothing is loaded and the rows count as given up
     const int64_t* tokens;
     float *logprob, *entropy;
     int64_t *rank, *top_ids;
@@ -501,6 +506,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         const int s = k % a.stages, cnt = min(VPC, nv - k * VPC);
         mbar_arrive_expect_tx(&sh.full[s], (uint32_t)cnt * 16u);
         bulk_g2s(ring + (size_t)s * VPC * 16, vp + (int64_t)k * VPC, (uint32_t)cnt * 16u, &sh.full[s]);
+        sh.loaded = k + 1;
     };
     if (C > 1) cluster_arrive_relaxed();  // waited for before the first store to another CTA
     if (tid == 0) {
@@ -509,11 +515,13 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
             mbar_init(&sh.empty[s], WARPS);
         }
         fence_mbar_init();
-        sh.failed = 0;
+        sh.failed = a.wait <= 0;
+        sh.loaded = 0;
         if constexpr (TOP) sh.n_list = sh.bound = 0;
     }
     pdl_wait_then_release();
-    if (tid == 0)
+    bool bad = a.wait <= 0;  // a wait gave up: nothing more is read, the barriers are still met
+    if (tid == 0 && !bad)
         for (int k = 0; k < min(chunks, a.stages); ++k) load_chunk(k);
     const int64_t tok = a.tokens ? a.tokens[r] : -1;
     const bool has_tok = tok >= 0 && tok < a.V;
@@ -538,15 +546,14 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
     uint32_t ph = 0;
     float bound = 0.0f;
     const int warps = min(WARPS, (max(nv, 64) + 31) / 32);  // warps that hold something (the ragged ends: two)
-    bool bad = false;  // a wait gave up: nothing more is read, the barriers are still met
     for (int k = 0; k < chunks; ++k) {
         // refill the chunk before this one: its readers have had a whole chunk's time
         if (tid == 0 && k > 0 && k - 1 + a.stages < chunks && !bad) {
             const int ps = (k - 1) % a.stages;
-            if (gm_wait<false>(&sh.empty[ps], (uint32_t)((k - 1) / a.stages) & 1u)) load_chunk(k - 1 + a.stages);
+            if (gm_wait<false>(&sh.empty[ps], (uint32_t)((k - 1) / a.stages) & 1u, a.wait)) load_chunk(k - 1 + a.stages);
             else sh.failed = 1;
         }
-        if (!bad && !gm_wait<false>(&sh.full[slot], ph)) {
+        if (!bad && !gm_wait<false>(&sh.full[slot], ph, a.wait)) {
             sh.failed = 1;
             bad = true;
         }
@@ -673,6 +680,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         w.U += sh.wU[k];
         c2 += sh.wcount[k];
     }
+    if (sh.failed) c2 = -1;
     if (C > 1) {  // every CTA hands its state, count and best words to the first one
         __syncwarp();
         cluster_wait();
@@ -705,7 +713,7 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
             }
             w.S = o.S;
             w.U = o.U;
-            c2 = __reduce_add_sync(0xffffffffu, c2);
+            c2 = __any_sync(0xffffffffu, c2 < 0) ? -1 : __reduce_add_sync(0xffffffffu, c2);
         }
     }
     if (crank == 0) {
@@ -718,8 +726,12 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
             if (a.status && tok >= a.V) atomicOr(a.status, B2S_STATUS_TOKEN_RANGE);
         }
         if constexpr (TOP) {
-            // the cluster's lists (C x top words, each in order) into one
-            const int n_all = C * a.top;
+            // the cluster's lists (C x top words, each in order) into one; no alternatives where a wait gave up
+            const int n_all = c2 < 0 ? 0 : C * a.top;
+            if (c2 < 0 && tid < a.top) {
+                a.top_ids[(int64_t)r * a.top + tid] = -1;
+                a.top_logprobs[(int64_t)r * a.top + tid] = __int_as_float(0x7fffffff);
+            }
             const unsigned long long* src = C > 1 ? sh.all : sh.top;
             for (int b = 0; b < n_all; b += NTH / 8) {
                 const int i = b + (tid >> 3), rk = C > 1 ? rank_of(src, n_all, i) : i;
@@ -735,10 +747,8 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
     }
     if (sh.failed && tid == 0) {  // copies still in flight write this CTA's shared memory: wait for them
         if (a.status) atomicOr(a.status, B2S_STATUS_WAIT_TIMEOUT);
-        for (int s2 = 0; s2 < a.stages; ++s2) {
-            gm_wait<false>(&sh.full[s2], 0u);
-            gm_wait<false>(&sh.full[s2], 1u);
-        }
+        for (int k = max(0, sh.loaded - a.stages); k < sh.loaded; ++k)
+            gm_wait<false>(&sh.full[k % a.stages], (uint32_t)(k / a.stages) & 1u);
     }
 }
 
@@ -940,6 +950,14 @@ cudaError_t launch_rows(LpArgs a, int rows, int C, int es, int sms, void* stream
 
 extern "C" {
 
+int b2s_wait_limit(int64_t clocks, int64_t* previous) {
+    using namespace b2s;
+    const long long before =
+        clocks < 0 ? wait_limit() : g_wait_limit.exchange(clocks < GM_WAIT ? clocks : GM_WAIT, std::memory_order_relaxed);
+    if (previous) *previous = before;
+    return B2S_OK;
+}
+
 int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, int32_t vocab, int64_t row_stride,
                        const int64_t* tokens, float temperature, int32_t top, float* logprob, float* entropy,
                        int64_t* rank, int64_t* top_ids, float* top_logprobs, float* stats, uint32_t* status,
@@ -964,6 +982,7 @@ int b2s_token_logprobs(const void* logits, int32_t logits_dtype, int32_t rows, i
     a.V = vocab;
     a.top = top;
     a.c = lp_scale(temperature);
+    a.wait = wait_limit();
     a.tokens = tokens;
     a.logprob = logprob;
     a.entropy = entropy;

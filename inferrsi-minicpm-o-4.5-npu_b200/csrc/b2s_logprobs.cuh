@@ -10,7 +10,7 @@
 
 namespace b2s {
 
-// Waits for the phase of `bar` with the given parity, for at most GM_WAIT clocks (false then).  The bound is kept with
+// Waits for the phase of `bar` with the given parity, for at most `limit` clocks (false then).  The bound is kept with
 // the SM's own clock: a read of the global timer costs more than a k block's MMAs, and a wait per k block that took it
 // held the products to 740 clocks per k block whatever the tile's width.
 constexpr long long GM_WAIT = 500ll * 1000 * 1000;  // about a quarter of a second
@@ -27,14 +27,14 @@ __device__ __forceinline__ bool gm_try(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 template <bool CLUSTER>
-__device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity, long long limit = GM_WAIT) {
     if (gm_try<CLUSTER>(bar, parity)) return true;
     const long long t0 = clock64();
     do {
 #pragma unroll 1
         for (int i = 0; i < 16; ++i)
             if (gm_try<CLUSTER>(bar, parity)) return true;
-    } while (clock64() - t0 < GM_WAIT);
+    } while (clock64() - t0 < limit);
     return false;
 }
 
@@ -246,5 +246,6 @@ inline bool lp_temperature_ok(float t) { return t >= 1e-6f && t <= 1e6f; }
 constexpr int LP_MAX_SIZE = 0x7fffffff - 4096;
 
 cudaError_t device_sms(int* sms);  // multiprocessors of the current device
+long long wait_limit();            // of the kernels' waits, in clocks (b2s_wait_limit); 0: they give up before they start
 
 }  // namespace b2s

@@ -14,7 +14,9 @@ A row that is -inf throughout has logprob -inf, entropy 0 and gradient 0; NaN or
 
 Both are differentiable through ``logprob`` and ``entropy`` (not through rank or alternatives, and once: there is no
 second derivative).  All calls are asynchronous, run on the current stream and can be captured in a CUDA graph; they
-keep no state between calls, so calls on several streams may overlap.
+keep no state between calls, so calls on several streams may overlap.  Waits inside the kernels are bounded
+(``b2s_wait_limit``): one that gives up, which a sound GPU never sees, makes what it left unfinished NaN, ranks and ids of
+alternatives -1, and sets 4 in ``status`` where there is one.
 """
 
 from __future__ import annotations

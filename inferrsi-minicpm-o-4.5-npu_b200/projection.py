@@ -5,7 +5,8 @@ the layers that feed a head -- as one tensor-core product with everything in its
 
 bf16 in and out, fp32 in between, rounded once.  Differentiable in x, weight, bias and residual (once).  Like the head
 products of this engine it takes CUDA tensors only, runs on the current stream, never synchronises, keeps no state
-between calls and can be captured in a CUDA graph.
+between calls and can be captured in a CUDA graph.  A device wait that gives up makes the unfinished outputs NaN and sets
+4 in ``status``.
 """
 
 from __future__ import annotations
