@@ -625,7 +625,13 @@ Plan plan_for(int M, int N, int64_t K, int epi, int sms) {
     return best;
 }
 
-// The plan on the current device (without one, where only sizes are asked for, on a B200's 148 multiprocessors).  A plan
+// Multiprocessors of the current device (without one, where only sizes are asked for, a B200's 148).
+int sms_here() {
+    int sms = 0;
+    return device_sms(&sms) == cudaSuccess && sms > 0 ? sms : 148;
+}
+
+// The plan on the current device.  A plan
 // is a function of the sizes alone; each thread keeps its last few (making one takes the host about a microsecond, and a
 // gradient asks for five).
 Plan plan_here(int M, int N, int64_t K, int epi) {
@@ -635,8 +641,7 @@ Plan plan_here(int M, int N, int64_t K, int epi) {
         Plan plan;
     };
     static thread_local Kept kept[16] = {};
-    int sms = 0;
-    if (device_sms(&sms) != cudaSuccess || sms < 1) sms = 148;
+    const int sms = sms_here();
     Kept& k = kept[((unsigned)M * 31u + (unsigned)N * 17u + (unsigned)K * 7u + (unsigned)epi) % 16u];
     if (k.M != M || k.N != N || k.K != K || k.epi != epi || k.sms != sms) {
         k.plan = plan_for(M, N, K, epi, sms);
@@ -938,7 +943,7 @@ int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 // parts of the rows whose column sums are taken separately: one round of CTAs (four an SM), at least 32 rows each
 int dz_parts(int rows, int N) {
     const int64_t cols = (N + 255) / 256;
-    int64_t p = 4 * 148 / cols;
+    int64_t p = 4 * sms_here() / cols;
     if (p > (rows + 31) / 32) p = (rows + 31) / 32;
     return (int)(p < 1 ? 1 : p);
 }

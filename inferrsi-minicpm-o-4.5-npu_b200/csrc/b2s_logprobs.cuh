@@ -112,41 +112,8 @@ __device__ __forceinline__ void lp_warp_merge(LpState& s, float c) {
     }
 }
 
-// N elements at once, any values.
-template <int N>
-__device__ __forceinline__ void lp_add_many(LpState& s, const float (&x)[N], float c) {
-    float bm = x[0];
-#pragma unroll
-    for (int j = 1; j < N; ++j) bm = fmax_nan(bm, x[j]);
-    const float m = fmax_nan(s.m, bm);
-    if (!(fabsf(m) <= 3.402823466e38f)) {  // NaN or +inf so far (the row's outcome), or nothing but -inf
-        s.m = m;
-        return;
-    }
-    if (m > s.m) lp_rescale(s, m, c);
-    const float R = __fmul_rn(s.m, c);
-    float S = 0.0f, U = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const float y = __fmaf_rn(x[j], c, -R), e = ex2(y);
-        S += e;
-        U = __fmaf_rn(e, y, U);
-    }
-    if (lp_far(R) || !(fabsf(U) <= 3.0e38f)) {  // a reference far from zero, or a masked element (0 * -inf)
-        S = U = 0.0f;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float y = lp_y(x[j], s.m, c), e = x[j] == f_ninf() ? 0.0f : ex2(y);
-            S += e;
-            U = __fmaf_rn(e, y, U);
-        }
-    }
-    s.S += S;
-    s.U += U;
-}
-
-// The same without the second pass: every y bounded below, the form of y chosen per call.  Short code for the products'
-// epilogue, whose arithmetic the MMAs hide.
+// N elements at once, any values: every y bounded below (a masked element adds 0), the form of y chosen per
+// call.  Short code for the products' epilogue, whose arithmetic the MMAs hide.
 template <int N>
 __device__ __forceinline__ void lp_add_any(LpState& s, const float (&x)[N], float c) {
     float bm = x[0];
@@ -168,11 +135,6 @@ __device__ __forceinline__ void lp_add_any(LpState& s, const float (&x)[N], floa
         s.S += e;
         s.U = __fmaf_rn(e, y, s.U);
     }
-}
-
-__device__ __forceinline__ void lp_add(LpState& s, float x, float c) {
-    const float v[1] = {x};
-    lp_add_many<1>(s, v, c);
 }
 
 // What the outputs need of a whole row.
