@@ -593,8 +593,13 @@ Plan plan_for(int M, int N, int64_t K, int epi, int sms) {
             int64_t cost = tiles_cost(p.waves + (p.rest ? 1 : 0), nkb);
             // The head's states cannot be joined across k; but where whole waves leave a handful of column tiles over (a step's
             // 594 on 148 CTAs: two, which alone would stream their 4 MB at two SMs' rate), and one tile holds all rows,
-            // those are split 8 ways and lmhead_merge_kernel adds their logits.
-            if (epi == EPI_LSE && M <= GM_M && p.waves && p.rest && p.rest <= 16 && nkb >= 16) {
+            // those are split 8 ways and lmhead_merge_kernel adds their logits.  That saves a tile's way from HBM, which
+            // grows with K, and costs the merge, which grows with the tiles and the rows.  Whole / split, us, 296 tiles and
+            // `rest` on 148 CTAs: K = 1024, 16 rows, rest 1 41.7 / 40.4, 2 41.5 / 42.8, 8 41.7 / 54.3; K = 2048, 16 rows,
+            // 2 70.6 / 68.4, 4 70.8 / 72.9; 128 rows, 1 67.1 / 66.2, 2 68.2 / 68.8; K = 4096, 16 rows, 2 126.5 / 111.1,
+            // 6 127.5 / 120.2, 10 127.3 / 126.9; 128 rows, 3 129.2 / 120.1, 6 129.1 / 128.2, 8 128.9 / 131.7; K = 8192,
+            // 16 rows, 10 243 / 223.
+            if (epi == EPI_LSE && M <= GM_M && p.waves && p.rest && p.rest * (M > 64 ? 16 : 8) <= nkb - 16) {
                 p.chunk = (int)ceil_div(nkb, 8);
                 p.split = (int)ceil_div(nkb, p.chunk);
                 p.bytes = (int64_t)p.split * p.rest * M * tn * 4;

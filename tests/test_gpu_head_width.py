@@ -11,7 +11,7 @@ The log probability has its own arithmetic beside it, 4 roundings of which the m
 import pytest
 import torch
 
-from tests.test_gpu_logprobs import DEV, EPS, close, plain_grad, s_eps
+from tests.test_gpu_logprobs import DEV, EPS, close, exact_operands, plain, plain_grad, s_eps
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,15 @@ def test_gradient(pkg, n, V, H):
         want = dz[:, v:v + 20_000].t() @ h.double()
         bound = tol[:, v:v + 20_000].t() @ h.double().abs()
         close(dw[v:v + 20_000], want, more * (bound * (1 + 2.0 ** -10) + 2.0 ** -8 * want.abs()) + 2.0 ** -100)
+
+
+@pytest.mark.parametrize("n,V,H", [(1, 148 * 256 + 300, 2304), (64, 148 * 256 + 1, 2056), (65, 148 * 256 + 5, 2048),
+                                   (128, 148 * 512 + 257, 3600), (33, 148 * 256 + 1500, 4096)])
+def test_left_over_column_tiles(pkg, n, V, H):
+    """Whole waves of column tiles and a few over, split along k: exact sums, tokens in the split tiles and outside."""
+    h, w, t, T = exact_operands(n, V, H, n + H)
+    t[::2] = V - 1 - torch.arange(t[::2].numel(), device=DEV) % (V - 148 * 256 * (V // (148 * 256)))
+    r = pkg.logprobs.LMHeadLogprobs(w)(h, t, temperature=T)
+    lp, ent = plain(h.double() @ w.double().t(), t, T)[:2]
+    close(r.logprob, lp, s_eps(V) + 4 * EPS * lp.abs())
+    close(r.entropy, ent, 2 * s_eps(V) * (2 + ent.abs()))

@@ -74,7 +74,7 @@ def test_logits(pkg, n, V, top, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,V,H", [(1, 700, 64), (16, 6562, 768), (100, 148 * 256 * 2 + 1, 1104), (300, 6561, 2056), (777, 6562, 768)])
+@pytest.mark.parametrize("n,V,H", [(1, 700, 64), (16, 6562, 768), (100, 148 * 256 * 2 + 1, 1104), (100, 148 * 256 + 1, 2056), (300, 6561, 2056), (777, 6562, 768)])
 def test_head(pkg, n, V, H):
     """Tiles of one CTA and of a pair, column tiles split along k; a given-up forward and a given-up gradient."""
     lp, lib = pkg.logprobs, pkg._native.capi()
