@@ -9,10 +9,13 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/b2s_sampler.h"
 
@@ -946,19 +949,40 @@ const auto& linear_grad_op() {
 }
 
 // Under stream capture: a leaf whose gradient accumulator an eager graph on another stream keeps alive would tie the
-// captured backward pass to that stream, which invalidates the capture deep in the engine.  Said here instead.  Tracing
+// captured backward pass to that stream, which invalidates the capture deep in the engine.  Said here instead, for leaves
+// that are inputs themselves and for those that inputs were made from on the capturing stream (a reshape, say).  Tracing
 // (Meta and fake tensors) works on machines without a driver, where there is nothing to ask.
-void check_capture(at::TensorList leaves) {
+void check_capture(at::TensorList inputs) {
+    using torch::autograd::Node;
     if (!at::hasCUDA()) return;
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
-    for (const Tensor& t : leaves) {
-        if (!needs_grad(t) || !t.is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-        if (!node) continue;
-        const auto stream = node->stream();
-        TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t.get_device()).unwrap(),
+    auto check = [](Node* accumulator, const c10::Stream& here) {
+        const auto stream = accumulator->stream();
+        TORCH_CHECK(!stream.has_value() || *stream == here,
                     "a backward pass cannot be captured while an eager graph of the same leaves is alive: let its outputs go "
                     "first (run the warm-up on a side stream and keep none of its results)");
+    };
+    std::unordered_set<Node*> seen;
+    std::vector<Node*> next;
+    for (const Tensor& t : inputs) {
+        if (!needs_grad(t) || !t.is_cuda()) continue;
+        const c10::Stream here = at::cuda::getCurrentCUDAStream(t.get_device()).unwrap();
+        if (t.is_leaf()) {
+            if (const auto node = torch::autograd::impl::try_get_grad_accumulator(t)) check(node.get(), here);
+            continue;
+        }
+        next.push_back(t.grad_fn().get());
+        while (!next.empty()) {
+            Node* node = next.back();
+            next.pop_back();
+            const auto stream = node->stream();
+            if (!seen.insert(node).second || (stream.has_value() && *stream != here)) continue;
+            for (const auto& edge : node->next_edges()) {
+                if (!edge.is_valid()) continue;
+                if (dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) check(edge.function.get(), here);
+                else next.push_back(edge.function.get());
+            }
+        }
     }
 }
 
