@@ -753,7 +753,8 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
 }
 
 // A warp per row, for many short rows without alternatives: no shared memory and no barriers, the next vectors in flight in
-// registers while the current ones are added.  Bound by latency and issue on the shortest rows, by HBM on the longest
+// registers while the current ones are added.  Bound by instruction issue on bf16 rows (120000 of 1000: issue active 77 %,
+// IPC 3.1, ALU 61 %, DRAM 33 %; 30000 of 6562: IPC 3.0, DRAM 53 %), by HBM on the longest fp32 ones
 // (microseconds, a CTA of 128 threads per row / this kernel: 30000 rows of 1000 bf16 89.5 / 21.2, 8192 of 6562 bf16 40.3 /
 // 24.8, 4000 of 15000 fp32 46.9 / 40.4, 5.9 TB/s).  A lane adds up to a 64th of a row into each of its sums.
 constexpr int LPW_NT = 256;
