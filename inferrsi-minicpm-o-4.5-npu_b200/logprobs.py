@@ -13,10 +13,10 @@ fp32).  A token of ``PAD`` (any id below 0, or one >= V) is no token: logprob 0,
 A row that is -inf throughout has logprob -inf, entropy 0 and gradient 0; NaN or +inf in a row makes it NaN.
 
 Both are differentiable through ``logprob`` and ``entropy`` (not through rank or alternatives, and once: there is no
-second derivative, and tangents are refused).  All calls are asynchronous, run on the current stream and can be captured in a CUDA graph; they
-keep no state between calls, so calls on several streams may overlap.  Waits inside the kernels are bounded
-(``b2s_wait_limit``): one that gives up, which a sound GPU never sees, makes what it left unfinished NaN, ranks and ids of
-alternatives -1, and sets 4 in ``status`` where there is one.
+second derivative, and tangents are refused).  All calls are asynchronous, run on the current stream and can be captured
+in a CUDA graph; they keep no state between calls, so calls on several streams may overlap.  Waits inside the kernels are
+bounded (``b2s_wait_limit``): one that gives up, which a sound GPU never sees, makes what it left unfinished NaN, ranks
+and ids of alternatives -1, and sets 4 in ``status`` where there is one.
 """
 
 from __future__ import annotations
