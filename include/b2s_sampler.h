@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define B2S_ABI_VERSION 7
+#define B2S_ABI_VERSION 8
 
 /* return codes */
 #define B2S_OK 0
@@ -52,7 +52,7 @@ extern "C" {
 #define B2S_STATUS_WAIT_TIMEOUT 4u  /* a bounded device wait gave up; the row returned PAD (log probabilities, products: NaN) */
 #define B2S_STATUS_COUNT_LIMIT 8u   /* a token repeated more than alpha_len-1 times; its count was clamped */
 #define B2S_STATUS_SHARD_INCOMPLETE 16u /* a shard's candidate list overflowed `cap` or failed; the row returned PAD */
-#define B2S_STATUS_TOKEN_RANGE 32u  /* a token id >= vocab was taken as no token (log probabilities) */
+#define B2S_STATUS_TOKEN_RANGE 32u  /* a token id >= vocab was taken as no token (log probabilities, embeddings) */
 
 /* flags */
 #define B2S_FLAG_FORCE_GENERAL 1 /* take the exact radix-select path even when the candidate path applies */
@@ -406,6 +406,73 @@ typedef struct b2s_linear_grad_args {
 } b2s_linear_grad_args;
 int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes);
 int b2s_linear_grad(const b2s_linear_grad_args* args, void* stream);
+
+/*
+ * Embedding lookup with a scale (ABI 8; no counterpart in the reference): out[i] = scale * table[tokens[i]], out [n, width]
+ * contiguous in the table's type (fp32 or bf16), rounded once.  A token < 0 (PAD) gives zeros, one >= vocab too and sets
+ * B2S_STATUS_TOKEN_RANGE.  Rows of the table may lie any row_stride >= width elements apart.
+ */
+int b2s_embedding(const int64_t* tokens, int32_t n, const void* table, int32_t dtype, int32_t vocab, int32_t width,
+                  int64_t row_stride, float scale, void* out, uint32_t* status, void* stream);
+
+/* The same from a microscaled 4-bit table (b2s_mx_quantize), out in bf16. */
+int b2s_embedding_mx(const int64_t* tokens, int32_t n, const void* codes, const void* scales, int32_t vocab, int32_t width,
+                     float scale, void* out, uint32_t* status, void* stream);
+
+/*
+ * The lookup's gradient (ABI 8): grad_table[v] = scale * the sum of grad_out's rows i with tokens[i] = v, in ascending
+ * order of i in fp32 (pieces of 32, those in order), rounded once; zeros for ids that do not occur.  grad_table [vocab,
+ * width] contiguous, `dtype` its and grad_out's.  The same call gives the same bits.
+ */
+int b2s_embedding_grad_workspace(int32_t n, int32_t vocab, int32_t width, int64_t* bytes);
+int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, int64_t grad_row_stride, int32_t dtype,
+                       int32_t vocab, int32_t width, float scale, void* grad_table, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
+/*
+ * Microscaled 4-bit matrices (ABI 8; OCP MX): blocks of 32 along a row share a scale 2^e, a byte e + 127 (255: NaN), e =
+ * max(floor(log2 max|x|) - 2, -127); an element is x 2^-e rounded to the nearest E2M1 value (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+ * their negatives), ties to even, saturated.  A block with NaN or an infinity has the scale NaN.
+ *   codes  [rows][ceil(k / 32)][16]: two elements a byte, the first in the low half, zeros past the row's end
+ *   scales [ceil(rows / 128)][ceil(k / 256)][1024]: of 128 rows x 8 blocks; the byte of (row, block) in a tile is at
+ *          (block / 4) * 512 + (row % 32) * 16 + (row / 32) * 4 + block % 4; zeros (anything but 255) past the matrix
+ * Both 16-byte aligned.  x and out are fp32 or bf16, rows any stride apart.
+ */
+int b2s_mx_quantize(const void* x, int32_t dtype, int32_t rows, int32_t k, int64_t row_stride, void* codes, void* scales,
+                    void* stream);
+int b2s_mx_dequantize(const void* codes, const void* scales, int32_t rows, int32_t k, int32_t dtype, void* out,
+                      int64_t out_row_stride, void* stream);
+
+/*
+ * Product of microscaled operands (ABI 8): out = act(x^ weight^T + bias) + residual; bias, residual and out bf16, fp32 in
+ * between, rounded once.  x is bf16 rows, quantised within the call, or already quantised (x NULL, x_codes and x_scales
+ * there).  bias, residual and preact (fp16, x^ weight^T + bias) are optional.  `workspace`: b2s_mx_linear_workspace bytes
+ * (may be 0), 16-byte aligned.
+ */
+typedef struct b2s_mx_linear_args {
+    const void* x;
+    int64_t x_row_stride;
+    const void* x_codes;
+    const void* x_scales;
+    const void* weight_codes;  /* [out_features, in_features] */
+    const void* weight_scales;
+    int32_t rows;
+    int32_t in_features;
+    int32_t out_features;
+    int32_t activation;
+    const void* bias;
+    const void* residual;
+    int64_t residual_row_stride;
+    void* out;
+    int64_t out_row_stride;
+    void* preact;
+    int64_t preact_row_stride; /* a multiple of 8 */
+    void* workspace;
+    int64_t workspace_bytes;
+    uint32_t* status;
+} b2s_mx_linear_args;
+int b2s_mx_linear_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes);
+int b2s_mx_linear(const b2s_mx_linear_args* args, void* stream);
 
 /*
  * The bound of each device wait inside the log-probability and projection kernels, in SM clocks: sets it for the calls

@@ -84,6 +84,19 @@ class LinearGradArgs(ctypes.Structure):
     ]
 
 
+class MxLinearArgs(ctypes.Structure):
+    """b2s_mx_linear_args of include/b2s_sampler.h."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_row_stride", ctypes.c_int64), ("x_codes", ctypes.c_void_p),
+        ("x_scales", ctypes.c_void_p), ("weight_codes", ctypes.c_void_p), ("weight_scales", ctypes.c_void_p),
+        ("rows", ctypes.c_int32), ("in_features", ctypes.c_int32), ("out_features", ctypes.c_int32),
+        ("activation", ctypes.c_int32), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+        ("residual_row_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64),
+        ("preact", ctypes.c_void_p), ("preact_row_stride", ctypes.c_int64), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p),
+    ]
+
+
 # every entry point of include/b2s_sampler.h with its ctypes signature
 CAPI_SIGNATURES = {
     "b2s_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), ctypes.c_void_p]),
@@ -135,6 +148,24 @@ CAPI_SIGNATURES = {
     "b2s_linear_grad_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                                  ctypes.POINTER(ctypes.c_int64)]),
     "b2s_linear_grad": (ctypes.c_int, [ctypes.POINTER(LinearGradArgs), ctypes.c_void_p]),
+    "b2s_embedding": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
+                                     ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p,
+                                     ctypes.c_void_p]),
+    "b2s_embedding_mx": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+                                        ctypes.c_int32, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p,
+                                        ctypes.c_void_p, ctypes.c_void_p]),
+    "b2s_embedding_grad_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                                    ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_embedding_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
+                                          ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_float,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "b2s_mx_quantize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64,
+                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "b2s_mx_dequantize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
+                                         ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "b2s_mx_linear_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                               ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_mx_linear": (ctypes.c_int, [ctypes.POINTER(MxLinearArgs), ctypes.c_void_p]),
     "b2s_wait_limit": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)]),
     "b2s_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "b2s_last_cuda_error": (ctypes.c_char_p, []),

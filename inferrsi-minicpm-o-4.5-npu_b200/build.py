@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -24,9 +25,11 @@ LIB = PKG / "libb2s.so"
 OPS = BUILD / "b2s_torch_ops.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = [CSRC / "b2s_sampler.cu", CSRC / "b2s_resident.cu", CSRC / "b2s_short.cu", CSRC / "b2s_shard.cu",
-              CSRC / "b2s_lmhead.cu", CSRC / "b2s_logprobs.cu", CSRC / "b2s_gemm.cu"]
+              CSRC / "b2s_lmhead.cu", CSRC / "b2s_logprobs.cu", CSRC / "b2s_gemm.cu", CSRC / "b2s_mx.cu",
+              CSRC / "b2s_embed.cu"]
 CU_HEADERS = [CSRC / "b2s_device.cuh", CSRC / "b2s_list.cuh", CSRC / "b2s_row.cuh", CSRC / "b2s_rowpaths.cuh",
-              CSRC / "b2s_head.cuh", CSRC / "b2s_logprobs.cuh", CSRC / "b2s_gemm.cuh", INCLUDE / "b2s_sampler.h"]
+              CSRC / "b2s_head.cuh", CSRC / "b2s_logprobs.cuh", CSRC / "b2s_gemm.cuh", CSRC / "b2s_launch.cuh",
+              CSRC / "b2s_mx.cuh", INCLUDE / "b2s_sampler.h"]
 
 
 def _nvcc() -> str:
@@ -47,18 +50,24 @@ def build_lib(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _stale(LIB, srcs + CU_HEADERS):
         return LIB
     BUILD.mkdir(exist_ok=True)
-    objs = []
-    for s in srcs:
+
+    def compile_one(s: Path) -> str:
         o = BUILD / (s.stem + ".o")
-        cmd = [_nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
-               f"-I{INCLUDE}", "-c", str(s), "-o", str(o)]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed for {s.name}:\n{r.stderr}")
-        if verbose:
-            print(r.stderr)
-        (BUILD / (s.stem + ".ptxas.txt")).write_text(r.stderr)
-        objs.append(str(o))
+        if force or _stale(o, [s, *CU_HEADERS]):
+            part = o.with_suffix(".o.tmp")
+            cmd = [_nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
+                   f"-I{INCLUDE}", "-c", str(s), "-o", str(part)]
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError(f"nvcc failed for {s.name}:\n{r.stderr}")
+            if verbose:
+                print(r.stderr)
+            (BUILD / (s.stem + ".ptxas.txt")).write_text(r.stderr)
+            os.replace(part, o)
+        return str(o)
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        objs = list(pool.map(compile_one, srcs))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [_nvcc(), *ARCH, "-shared", "-cudart", "static", "-Xlinker", "-soname=libb2s.so", "-o", str(tmp), *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -1,0 +1,428 @@
+// Microscaled 4-bit matrices (b2s_mx.cuh): quantisation, the way back, and the product of microscaled operands with bias,
+// activation and residual in its epilogue.  No counterpart in the reference.
+#include <string.h>
+
+#include "../../include/b2s_sampler.h"
+#include "b2s_gemm.cuh"
+#include "b2s_launch.cuh"
+#include "b2s_mx.cuh"
+
+namespace b2s {
+
+int cuda_fail(cudaError_t e);
+
+namespace {
+
+// ------------------------------------------------------------------ quantisation and back
+
+constexpr int MX_NT = 256;
+constexpr int MX_SEG = 256;  // elements of a row that a warp takes at a time: 8 a lane, the 8 blocks of a scale tile
+constexpr int MX_PER = 4;    // of those in flight
+
+// 8 elements of a row from column n (k columns) as fp32; zeros past the end.  VEC: 16-byte aligned rows.  Else the warp
+// loads a 32-element block at a time, an element a lane, and turns them round in shared memory.
+template <typename T>
+__device__ __forceinline__ float mx_value(const T* p);
+template <>
+__device__ __forceinline__ float mx_value(const float* p) { return __ldg(p); }
+template <>
+__device__ __forceinline__ float mx_value(const unsigned short* p) { return bf16_bits_to_f(__ldg(p)); }
+
+__device__ __forceinline__ void mx_load8(const float* p, float (&v)[8]) {
+    const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(p)), b = ldg_stream(reinterpret_cast<const uint4*>(p) + 1);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+}
+__device__ __forceinline__ void mx_load8(const unsigned short* p, float (&v)[8]) {
+    const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+}
+
+// grid: (a warp per row, MX_PER segments).  EIGHT: E4M3 codes, a byte each, and scales [blocks][rows]; else the 4-bit
+// layout, whose scale tiles' rows past the matrix get zeros.
+template <typename T, bool VEC, bool EIGHT>
+__global__ void __launch_bounds__(MX_NT) mx_quantize_kernel(const T* x, int64_t row_stride, int64_t rows, int k, uint8_t* codes,
+                                                            uint8_t* scales) {
+    constexpr int E = EIGHT ? 8 : 2;
+    __shared__ float turn[VEC ? 1 : MX_NT / 32][VEC ? 1 : MX_SEG];
+    pdl_wait_then_release();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = (int64_t)blockIdx.x * (MX_NT / 32) + warp, tiles = mx_tiles(k);
+    const int nb = (int)mx_blocks(k);
+    const bool live = r < rows;
+    if (!live && (EIGHT || r >= (rows + 127) / 128 * 128)) return;
+    const T* row = x + (live ? r : 0) * row_stride;
+    for (int64_t s0 = (int64_t)blockIdx.y * MX_PER; s0 < tiles; s0 += (int64_t)gridDim.y * MX_PER) {
+        float v[MX_PER][8];
+#pragma unroll
+        for (int j = 0; j < MX_PER; ++j) {
+            const int64_t n = (s0 + j) * MX_SEG + 8 * lane;
+            if (live && VEC && n + 8 <= k) {
+                mx_load8(row + n, v[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t at = VEC ? n + i : (s0 + j) * MX_SEG + 32 * i + lane;
+                    v[j][i] = live && at < k ? mx_value(row + at) : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < MX_PER; ++j) {
+            const int64_t tile = s0 + j;
+            if (tile >= tiles) break;
+            if constexpr (!VEC) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) turn[warp][32 * i + lane] = v[j][i];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(&turn[warp][8 * lane + i]);
+                    v[j][i] = q.x;
+                    v[j][i + 1] = q.y;
+                    v[j][i + 2] = q.z;
+                    v[j][i + 3] = q.w;
+                }
+            }
+            uint32_t most = 0;  // of the bits without the sign: NaN above everything
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[j][i]) & 0x7fffffffu);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const uint32_t code = mx_scale_code<E>(most);
+            const float inv = mx_inverse(code);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] *= inv;
+            const int block = (int)tile * 8 + (lane >> 2);
+            if constexpr (EIGHT) {
+                if (block < nb) {
+                    *reinterpret_cast<uint2*>(codes + (r * nb + block) * 32 + 8 * (lane & 3)) =
+                        make_uint2(mx_encode4_e4m3(v[j][0], v[j][1], v[j][2], v[j][3]), mx_encode4_e4m3(v[j][4], v[j][5], v[j][6], v[j][7]));
+                    if ((lane & 3) == 0) scales[(int64_t)block * rows + r] = (uint8_t)code;
+                }
+            } else {
+                uint32_t word = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xffffffffu, code, (lane & 16) + 4 * i) << (8 * i);
+                if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(r, block, tiles)) = word;
+                if (live && block < nb) *reinterpret_cast<uint32_t*>(codes + (r * nb + block) * 16 + 4 * (lane & 3)) = mx_encode8(v[j]);
+            }
+        }
+    }
+}
+
+template <typename T, bool EIGHT>
+__global__ void __launch_bounds__(MX_NT) mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k,
+                                                              T* out, int64_t out_stride, int vec) {
+    pdl_wait_then_release();
+    const int lane = threadIdx.x & 31;
+    const int64_t r = (int64_t)blockIdx.x * (MX_NT / 32) + (threadIdx.x >> 5), tiles = mx_tiles(k);
+    const int nb = (int)mx_blocks(k);
+    if (r >= rows) return;
+    for (int64_t s0 = (int64_t)blockIdx.y * MX_PER; s0 < tiles; s0 += (int64_t)gridDim.y * MX_PER) {
+        uint32_t c[MX_PER][2], f[MX_PER];
+#pragma unroll
+        for (int j = 0; j < MX_PER; ++j) {
+            const int block = (int)(s0 + j) * 8 + (lane >> 2);
+            c[j][0] = c[j][1] = f[j] = 0;
+            if (s0 + j < tiles && block < nb) {
+                if constexpr (EIGHT) {
+                    const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + (r * nb + block) * 32 + 8 * (lane & 3)));
+                    c[j][0] = q.x;
+                    c[j][1] = q.y;
+                    f[j] = __ldg(scales + (int64_t)block * rows + r);
+                } else {
+                    c[j][0] = __ldg(reinterpret_cast<const uint32_t*>(codes + (r * nb + block) * 16 + 4 * (lane & 3)));
+                    f[j] = __ldg(scales + mx_scale_at(r, block, tiles));
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < MX_PER; ++j) {
+            const int64_t n = (s0 + j) * MX_SEG + 8 * lane;
+            if (n >= k) break;
+            float v[8];
+            if constexpr (EIGHT) {
+                float a[4], b[4];
+                mx_decode4_e4m3(c[j][0], a);
+                mx_decode4_e4m3(c[j][1], b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = a[i];
+                    v[4 + i] = b[i];
+                }
+            } else {
+                mx_decode8(c[j][0], v);
+            }
+            const float s = mx_scale(f[j]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= s;
+            mx_store8(out + r * out_stride + n, (int)min((int64_t)8, k - n), vec, v);
+        }
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+dim3 mx_grid(int64_t rows, int64_t k) {
+    const int64_t y = (mx_tiles(k) + MX_PER - 1) / MX_PER;
+    return dim3((unsigned)((rows + MX_NT / 32 - 1) / (MX_NT / 32)), (unsigned)(y < 65535 ? y : 65535));
+}
+
+template <bool EIGHT>
+cudaError_t mx_quantize(const void* x, int dtype, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream) {
+    const int e = dtype == B2S_DTYPE_F32 ? 4 : 2;
+    const bool vec = aligned16(x) && row_stride * e % 16 == 0;
+    const dim3 grid = mx_grid(EIGHT ? rows : (rows + 127) / 128 * 128, k);
+    auto go = [&](auto kernel, auto* p) {
+        return launch_pdl(kernel, grid, MX_NT, 0, stream, p, row_stride, rows, k, static_cast<uint8_t*>(codes),
+                          static_cast<uint8_t*>(scales));
+    };
+    if (dtype == B2S_DTYPE_F32) {
+        const float* p = static_cast<const float*>(x);
+        return vec ? go(mx_quantize_kernel<float, true, EIGHT>, p) : go(mx_quantize_kernel<float, false, EIGHT>, p);
+    }
+    const unsigned short* p = static_cast<const unsigned short*>(x);
+    return vec ? go(mx_quantize_kernel<unsigned short, true, EIGHT>, p) : go(mx_quantize_kernel<unsigned short, false, EIGHT>, p);
+}
+template <bool EIGHT>
+cudaError_t mx_dequantize(const void* codes, const void* scales, int64_t rows, int k, int dtype, void* out, int64_t out_stride,
+                          void* stream) {
+    const int e = dtype == B2S_DTYPE_F32 ? 4 : 2;
+    const int vec = aligned16(out) && out_stride * e % 16 == 0;
+    auto go = [&](auto kernel, auto* p) {
+        return launch_pdl(kernel, mx_grid(rows, k), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
+                          static_cast<const uint8_t*>(scales), rows, k, p, out_stride, vec);
+    };
+    return dtype == B2S_DTYPE_F32 ? go(mx_dequantize_kernel<float, EIGHT>, static_cast<float*>(out))
+                                  : go(mx_dequantize_kernel<__nv_bfloat16, EIGHT>, static_cast<__nv_bfloat16*>(out));
+}
+
+// ------------------------------------------------------------------ the product of few rows
+
+// Each 4-bit code of a word as a byte, twice its value: {0, 1, 2, 3, 4, 6, 8, 12}, negative where bit 3 is set.
+__device__ __forceinline__ void mx_bytes(uint32_t c, int& lo, int& hi) {
+    auto four = [](uint32_t n) {  // the low four codes
+        const uint32_t pos = __byte_perm(0x03020100u, 0x0c080604u, n & 0x7777u);
+        const uint32_t neg = __byte_perm(0xfdfeff00u, 0xf4f8fafcu, n & 0x7777u);
+        const uint32_t mask = __byte_perm(0x0000ff00u, 0u, (n >> 3) & 0x1111u);
+        return (int)((pos & ~mask) | (neg & mask));
+    };
+    lo = four(c);
+    hi = four(c >> 16);
+}
+// 32 elements of x from column n as bytes, and their scale's factor (a quarter of it, for the two doubled operands).
+__device__ __forceinline__ float mx_block_bytes(const unsigned short* row, int n, int k, bool vec, int (&b)[8]) {
+    float v[4][8];
+    uint32_t most = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (vec && n + 8 * q + 8 <= k) {
+            mx_load8(row + n + 8 * q, v[q]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[q][i] = n + 8 * q + i < k ? mx_value(row + n + 8 * q + i) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[q][i]) & 0x7fffffffu);
+    }
+    const uint32_t code = mx_scale_code<2>(most);
+    const float inv = mx_inverse(code);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[q][i] *= inv;
+        mx_bytes(mx_encode8(v[q]), b[2 * q], b[2 * q + 1]);
+    }
+    return mx_scale(code) * 0.25f;
+}
+
+struct MxRowsArgs {
+    const unsigned short* x;  // bf16 rows, or null and the codes and scales of a quantised x
+    int64_t x_stride;
+    const uint8_t *xc, *xs;
+    const uint8_t *wc, *ws;
+    int M, N, K, act, x_vec, tpr;
+    const unsigned short *bias, *residual;
+    int64_t res_stride;
+    __half* preact;
+    int64_t pre_stride;
+    __nv_bfloat16* out;
+    int64_t out_stride;
+};
+
+// out = act(x^ w^T + b) + r for groups of at most R rows (grid.y), F features per group of `tpr` threads.  A thread takes
+// the blocks tpr apart: x's block as bytes in registers (quantised here: no launch of its own), a feature's 16 bytes of
+// codes as bytes, and integer dot products, exact within a block; blocks are added in fp32.
+constexpr int MXR_NT = 128;
+template <int R, int F>
+__global__ void __launch_bounds__(MXR_NT) mx_rows_kernel(const __grid_constant__ MxRowsArgs a) {
+    __shared__ float red[MXR_NT / 32][R * F];
+    pdl_wait_then_release();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = tid / a.tpr, n0 = ((int)blockIdx.x * (MXR_NT / a.tpr) + group) * F, r0 = (int)blockIdx.y * R;
+    const int nb = (int)mx_blocks(a.K);
+    const int64_t tiles = mx_tiles(a.K);
+    float acc[R][F];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int f = 0; f < F; ++f) acc[r][f] = 0.0f;
+    for (int b = tid % a.tpr; b < nb; b += a.tpr) {
+        uint4 w[F];
+        uint32_t ws[F];
+#pragma unroll
+        for (int f = 0; f < F; ++f) {  // features and rows past the end repeat the last one; they are not stored
+            const int64_t n = min(n0 + f, a.N - 1);
+            w[f] = ldg_stream(reinterpret_cast<const uint4*>(a.wc) + n * nb + b);
+            ws[f] = __ldg(a.ws + mx_scale_at(n, b, tiles));
+        }
+        int xb[R][8];
+        float xs[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t m = min(r0 + r, a.M - 1);
+            if (a.x) {
+                xs[r] = mx_block_bytes(a.x + m * a.x_stride, 32 * b, a.K, a.x_vec, xb[r]);
+            } else {
+                const uint4 q = __ldg(reinterpret_cast<const uint4*>(a.xc) + m * nb + b);
+                mx_bytes(q.x, xb[r][0], xb[r][1]);
+                mx_bytes(q.y, xb[r][2], xb[r][3]);
+                mx_bytes(q.z, xb[r][4], xb[r][5]);
+                mx_bytes(q.w, xb[r][6], xb[r][7]);
+                xs[r] = mx_scale(__ldg(a.xs + mx_scale_at(m, b, tiles))) * 0.25f;
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            int wb[8];
+            mx_bytes(w[f].x, wb[0], wb[1]);
+            mx_bytes(w[f].y, wb[2], wb[3]);
+            mx_bytes(w[f].z, wb[4], wb[5]);
+            mx_bytes(w[f].w, wb[6], wb[7]);
+            const float s = mx_scale(ws[f]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                int d = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d = __dp4a(wb[j], xb[r][j], d);
+                acc[r][f] = __fmaf_rn((float)d, xs[r] * s, acc[r][f]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            float t = acc[r][f];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (lane == 0) red[warp][r * F + f] = t;
+        }
+    __syncthreads();
+    const int per = a.tpr / 32;  // warps of a group
+    for (int i = tid; i < R * F * (MXR_NT / a.tpr); i += MXR_NT) {
+        const int g = i / (R * F), j = i % (R * F), m = r0 + j / F, n = ((int)blockIdx.x * (MXR_NT / a.tpr) + g) * F + j % F;
+        if (m >= a.M || n >= a.N) continue;
+        float t = red[g * per][j];
+        for (int k = 1; k < per; ++k) t += red[g * per + k][j];
+        if (a.bias) t += bf16_bits_to_f(__ldg(a.bias + n));
+        if (a.preact) a.preact[(int64_t)m * a.pre_stride + n] = __ushort_as_half(preact_bits(t));
+        t = act_apply(t, a.act);
+        if (a.residual) t += bf16_bits_to_f(__ldg(a.residual + (int64_t)m * a.res_stride + n));
+        a.out[(int64_t)m * a.out_stride + n] = __float2bfloat16_rn(t);
+    }
+}
+
+}  // namespace
+}  // namespace b2s
+
+extern "C" {
+
+int b2s_mx_quantize(const void* x, int32_t dtype, int32_t rows, int32_t k, int64_t row_stride, void* codes, void* scales,
+                    void* stream) {
+    using namespace b2s;
+    if (rows < 0 || k < 1 || row_stride < k || (dtype != B2S_DTYPE_F32 && dtype != B2S_DTYPE_BF16)) return B2S_ERR_INVALID;
+    if (rows > LP_MAX_SIZE || k > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
+    if (rows == 0) return B2S_OK;
+    if (!x || !codes || !scales || !aligned16(codes) || !aligned16(scales) ||
+        (reinterpret_cast<uintptr_t>(x) & (dtype == B2S_DTYPE_F32 ? 3 : 1)))
+        return B2S_ERR_INVALID;
+    const cudaError_t e = mx_quantize<false>(x, dtype, rows, k, row_stride, codes, scales, stream);
+    return e == cudaSuccess ? B2S_OK : cuda_fail(e);
+}
+
+int b2s_mx_dequantize(const void* codes, const void* scales, int32_t rows, int32_t k, int32_t dtype, void* out,
+                      int64_t out_row_stride, void* stream) {
+    using namespace b2s;
+    if (rows < 0 || k < 1 || out_row_stride < k || (dtype != B2S_DTYPE_F32 && dtype != B2S_DTYPE_BF16)) return B2S_ERR_INVALID;
+    if (rows > LP_MAX_SIZE || k > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
+    if (rows == 0) return B2S_OK;
+    if (!out || !codes || !scales || !aligned16(codes) || !aligned16(scales) ||
+        (reinterpret_cast<uintptr_t>(out) & (dtype == B2S_DTYPE_F32 ? 3 : 1)))
+        return B2S_ERR_INVALID;
+    const cudaError_t e = mx_dequantize<false>(codes, scales, rows, k, dtype, out, out_row_stride, stream);
+    return e == cudaSuccess ? B2S_OK : cuda_fail(e);
+}
+
+int b2s_mx_linear_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
+    using namespace b2s;
+    if (rows < 0 || in_features < 1 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
+    *bytes = 0;
+    return B2S_OK;
+}
+
+int b2s_mx_linear(const b2s_mx_linear_args* l, void* stream) {
+    using namespace b2s;
+    if (!l || l->rows < 0 || l->out_features < 1 || l->in_features < 1 || l->activation < 0 || l->activation > B2S_ACT_SILU)
+        return B2S_ERR_INVALID;
+    if (l->rows > LP_MAX_SIZE || l->in_features > LP_MAX_SIZE || l->out_features > LP_MAX_SIZE) return B2S_ERR_UNSUPPORTED;
+    if (l->rows == 0) return B2S_OK;
+    if (!l->x == !l->x_codes || !l->weight_codes || !l->weight_scales || !l->out || !aligned16(l->weight_codes) ||
+        !aligned16(l->weight_scales) || (l->x && l->x_row_stride < l->in_features) ||
+        (l->x_codes && (!l->x_scales || !aligned16(l->x_codes) || !aligned16(l->x_scales))) ||
+        l->out_row_stride < l->out_features || (l->residual && l->residual_row_stride < l->out_features) ||
+        (l->preact && (!aligned16(l->preact) || l->preact_row_stride < l->out_features || l->preact_row_stride % 8)) ||
+        ((reinterpret_cast<uintptr_t>(l->x) | reinterpret_cast<uintptr_t>(l->out) | reinterpret_cast<uintptr_t>(l->bias) |
+          reinterpret_cast<uintptr_t>(l->residual)) & 1))
+        return B2S_ERR_INVALID;
+    int64_t need = 0;
+    b2s_mx_linear_workspace(l->rows, l->in_features, l->out_features, &need);
+    if (need && (!l->workspace || l->workspace_bytes < need || !aligned16(l->workspace))) return B2S_ERR_INVALID;
+    MxRowsArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = static_cast<const unsigned short*>(l->x);
+    a.x_stride = l->x_row_stride;
+    a.x_vec = aligned16(l->x) && l->x_row_stride % 8 == 0;
+    a.xc = static_cast<const uint8_t*>(l->x_codes);
+    a.xs = static_cast<const uint8_t*>(l->x_scales);
+    a.wc = static_cast<const uint8_t*>(l->weight_codes);
+    a.ws = static_cast<const uint8_t*>(l->weight_scales);
+    a.M = l->rows;
+    a.N = l->out_features;
+    a.K = l->in_features;
+    a.act = l->activation;
+    a.bias = static_cast<const unsigned short*>(l->bias);
+    a.residual = static_cast<const unsigned short*>(l->residual);
+    a.res_stride = l->residual_row_stride;
+    a.preact = static_cast<__half*>(l->preact);
+    a.pre_stride = l->preact_row_stride;
+    a.out = static_cast<__nv_bfloat16*>(l->out);
+    a.out_stride = l->out_row_stride;
+    const int64_t nb = mx_blocks(a.K);
+    a.tpr = nb > 64 ? 128 : nb > 32 ? 64 : 32;
+    auto go = [&](auto kernel, int R, int F) {
+        const int64_t per = (int64_t)(MXR_NT / a.tpr) * F;
+        return launch_pdl(kernel, dim3((unsigned)((a.N + per - 1) / per), (unsigned)((a.M + R - 1) / R)), MXR_NT, 0, stream, a);
+    };
+    const cudaError_t e = a.M == 1 ? go(mx_rows_kernel<1, 4>, 1, 4) : a.M == 2 ? go(mx_rows_kernel<2, 4>, 2, 4) : go(mx_rows_kernel<4, 4>, 4, 4);
+    return e == cudaSuccess ? B2S_OK : cuda_fail(e);
+}
+
+}  // extern "C"

@@ -873,6 +873,250 @@ std::tuple<Tensor, Tensor, Tensor> linear_grad_meta(const Tensor&, const Tensor&
             at::empty({want_bias ? N : 0}, x.options())};
 }
 
+// ------------------------------------------------------------------ embeddings and microscaled matrices
+
+void check_table(const Tensor& table) {
+    TORCH_CHECK(table.is_cuda() && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1,
+                "table must be CUDA [vocab, width]");
+    TORCH_CHECK(table.scalar_type() == at::kFloat || table.scalar_type() == at::kBFloat16,
+                "table must be float32 or bfloat16");
+    TORCH_CHECK(table.size(0) <= INT32_MAX && table.size(1) <= INT32_MAX, "a size is beyond 2^31 - 1");
+}
+int32_t token_count(const Tensor& tokens, const Tensor& like) {
+    TORCH_CHECK(tokens.dim() == 1 && tokens.size(0) <= INT32_MAX, "tokens must be [n], n at most 2^31 - 1");
+    check_tokens(tokens, like, tokens.size(0));
+    return (int32_t)tokens.size(0);
+}
+
+Tensor embedding_cuda(const Tensor& tokens, const Tensor& table, double scale, const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(table.device());
+    check_table(table);
+    const int32_t n = token_count(tokens, table);
+    const Tensor t = plain_rows(table);
+    Tensor out = fresh({n, t.size(1)}, t.scalar_type(), t);
+    check_rc(b2s_embedding(tokens.data_ptr<int64_t>(), n, t.data_ptr(), logits_dtype(t), (int32_t)t.size(0),
+                           (int32_t)t.size(1), row_stride(t), (float)scale, out.data_ptr(), status_ptr(status, t),
+                           at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_embedding");
+    return out;
+}
+Tensor embedding_meta(const Tensor& tokens, const Tensor& table, double, const optional<Tensor>&) {
+    return at::empty({tokens.size(0), table.size(1)}, table.options());
+}
+
+// A 4-bit matrix of `k` columns: its rows.
+int32_t check_mx(const Tensor& codes, const Tensor& scales, int64_t k, const Tensor& like, const char* name) {
+    TORCH_CHECK(k >= 1 && k <= INT32_MAX, name, ": a row length out of range");
+    check_same(codes, like, at::kByte, name);
+    check_same(scales, like, at::kByte, name);
+    TORCH_CHECK(codes.dim() == 2 && codes.is_contiguous() && codes.size(1) == (k + 31) / 32 * 16 && codes.size(0) <= INT32_MAX,
+                name, ": codes must be contiguous uint8 [rows, ", (k + 31) / 32 * 16, "]");
+    TORCH_CHECK(scales.dim() == 3 && scales.is_contiguous() && scales.size(0) == (codes.size(0) + 127) / 128 &&
+                    scales.size(1) == (k + 255) / 256 && scales.size(2) == 1024,
+                name, ": scales must be contiguous uint8 [", (codes.size(0) + 127) / 128, ", ", (k + 255) / 256, ", 1024]");
+    TORCH_CHECK(((reinterpret_cast<uintptr_t>(codes.data_ptr()) | reinterpret_cast<uintptr_t>(scales.data_ptr())) & 15) == 0,
+                name, ": codes and scales must be 16-byte aligned");
+    return (int32_t)codes.size(0);
+}
+
+Tensor embedding_mx_cuda(const Tensor& tokens, const Tensor& codes, const Tensor& scales, int64_t width, double scale,
+                         const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(codes.device());
+    TORCH_CHECK(codes.is_cuda(), "codes must be a CUDA tensor");
+    const int32_t vocab = check_mx(codes, scales, width, codes, "table"), n = token_count(tokens, codes);
+    TORCH_CHECK(vocab >= 1, "table must have rows");
+    Tensor out = fresh({n, width}, at::kBFloat16, codes);
+    check_rc(b2s_embedding_mx(tokens.data_ptr<int64_t>(), n, codes.data_ptr(), scales.data_ptr(), vocab, (int32_t)width,
+                              (float)scale, out.data_ptr(), status_ptr(status, codes),
+                              at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_embedding_mx");
+    return out;
+}
+Tensor embedding_mx_meta(const Tensor& tokens, const Tensor& codes, const Tensor&, int64_t width, double,
+                         const optional<Tensor>&) {
+    return at::empty({tokens.size(0), width}, codes.options().dtype(at::kBFloat16));
+}
+
+Tensor embedding_grad_cuda(const Tensor& grad_out, const Tensor& tokens, int64_t vocab, double scale) {
+    c10::cuda::CUDAGuard guard(grad_out.device());
+    TORCH_CHECK(grad_out.is_cuda() && grad_out.dim() == 2, "grad_out must be CUDA [n, width]");
+    TORCH_CHECK(vocab >= 1 && vocab <= INT32_MAX && grad_out.size(1) >= 1 && grad_out.size(1) <= INT32_MAX,
+                "a size is out of range");
+    const int dt = logits_dtype(grad_out);
+    const int32_t n = token_count(tokens, grad_out), width = (int32_t)grad_out.size(1);
+    TORCH_CHECK(grad_out.size(0) == n, "grad_out must have a row per token");
+    const Tensor g = plain_rows(grad_out);
+    Tensor out = fresh({vocab, width}, g.scalar_type(), g);
+    int64_t bytes = 0;
+    check_rc(b2s_embedding_grad_workspace(n, (int32_t)vocab, width, &bytes), "b2s_embedding_grad_workspace");
+    Tensor ws = workspace(bytes, g);
+    check_rc(b2s_embedding_grad(tokens.data_ptr<int64_t>(), n, g.data_ptr(), row_stride(g), dt, (int32_t)vocab, width,
+                                (float)scale, out.data_ptr(), ws.data_ptr(), bytes,
+                                at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_embedding_grad");
+    return out;
+}
+Tensor embedding_grad_meta(const Tensor& grad_out, const Tensor&, int64_t vocab, double) {
+    return at::empty({vocab, grad_out.size(1)}, grad_out.options());
+}
+
+std::tuple<Tensor, Tensor> mx_quantize_cuda(const Tensor& x_) {
+    c10::cuda::CUDAGuard guard(x_.device());
+    TORCH_CHECK(x_.is_cuda() && x_.dim() == 2 && x_.size(1) >= 1, "x must be CUDA [rows, k]");
+    TORCH_CHECK(x_.size(0) <= INT32_MAX && x_.size(1) <= INT32_MAX, "a size is beyond 2^31 - 1");
+    const int dt = logits_dtype(x_);
+    const Tensor x = plain_rows(x_);
+    const int64_t R = x.size(0), K = x.size(1);
+    Tensor codes = fresh({R, (K + 31) / 32 * 16}, at::kByte, x), scales = fresh({(R + 127) / 128, (K + 255) / 256, 1024}, at::kByte, x);
+    check_rc(b2s_mx_quantize(x.data_ptr(), dt, (int32_t)R, (int32_t)K, row_stride(x), codes.data_ptr(), scales.data_ptr(),
+                             at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_mx_quantize");
+    return {codes, scales};
+}
+std::tuple<Tensor, Tensor> mx_quantize_meta(const Tensor& x) {
+    const int64_t R = x.size(0), K = x.size(1);
+    auto o = x.options().dtype(at::kByte);
+    return {at::empty({R, (K + 31) / 32 * 16}, o), at::empty({(R + 127) / 128, (K + 255) / 256, 1024}, o)};
+}
+
+Tensor mx_dequantize_cuda(const Tensor& codes, const Tensor& scales, int64_t k, at::ScalarType dtype) {
+    c10::cuda::CUDAGuard guard(codes.device());
+    TORCH_CHECK(codes.is_cuda(), "codes must be a CUDA tensor");
+    TORCH_CHECK(dtype == at::kFloat || dtype == at::kBFloat16, "dtype must be float32 or bfloat16");
+    const int32_t R = check_mx(codes, scales, k, codes, "x");
+    Tensor out = fresh({R, k}, dtype, codes);
+    check_rc(b2s_mx_dequantize(codes.data_ptr(), scales.data_ptr(), R, (int32_t)k,
+                               dtype == at::kFloat ? B2S_DTYPE_F32 : B2S_DTYPE_BF16, out.data_ptr(), k,
+                               at::cuda::getCurrentCUDAStream().stream()),
+             "b2s_mx_dequantize");
+    return out;
+}
+Tensor mx_dequantize_meta(const Tensor& codes, const Tensor&, int64_t k, at::ScalarType dtype) {
+    return at::empty({codes.size(0), k}, codes.options().dtype(dtype));
+}
+
+// act(x^ weight^T + bias) + residual: x bf16 [rows, in], or, with x_scales, an x's codes.
+std::tuple<Tensor, Tensor> mx_linear_cuda(const Tensor& x_, const optional<Tensor>& x_scales, const Tensor& codes,
+                                          const Tensor& scales, int64_t in_features, const optional<Tensor>& bias,
+                                          const optional<Tensor>& residual, int64_t activation, bool want_preact,
+                                          const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(x_.device());
+    TORCH_CHECK(x_.is_cuda() && x_.dim() == 2, "x must be CUDA [rows, in]");
+    b2s_mx_linear_args a;
+    memset(&a, 0, sizeof(a));
+    const int32_t N = check_mx(codes, scales, in_features, x_, "weight");
+    TORCH_CHECK(N >= 1 && x_.size(0) <= INT32_MAX, "a size is out of range");
+    const int64_t R = x_.size(0);
+    Tensor x = x_, b, r;
+    if (x_scales.has_value() && x_scales->defined()) {
+        check_mx(x_, *x_scales, in_features, x_, "x");
+        a.x_codes = x.data_ptr();
+        a.x_scales = x_scales->data_ptr();
+    } else {
+        check_same(x_, x_, at::kBFloat16, "x");
+        TORCH_CHECK(x_.size(1) == in_features, "x must be [rows, in]");
+        x = plain_rows(x_);
+        a.x = x.data_ptr();
+        a.x_row_stride = row_stride(x);
+    }
+    if (bias.has_value() && bias->defined()) {
+        check_same(*bias, x, at::kBFloat16, "bias");
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "bias must be [out]");
+        b = bias->contiguous();
+    }
+    if (residual.has_value() && residual->defined()) {
+        check_same(*residual, x, at::kBFloat16, "residual");
+        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == R && residual->size(1) == N,
+                    "residual must be [rows, out]");
+        r = plain_rows(*residual);
+    }
+    Tensor out = fresh({R, N}, at::kBFloat16, x);
+    Tensor pre = fresh({want_preact ? R : 0, round8(N)}, at::kHalf, x);
+    a.weight_codes = codes.data_ptr();
+    a.weight_scales = scales.data_ptr();
+    a.rows = (int32_t)R;
+    a.in_features = (int32_t)in_features;
+    a.out_features = N;
+    a.activation = (int32_t)activation;
+    a.bias = b.defined() ? b.data_ptr() : nullptr;
+    a.residual = r.defined() ? r.data_ptr() : nullptr;
+    a.residual_row_stride = r.defined() ? row_stride(r) : 0;
+    a.out = out.data_ptr();
+    a.out_row_stride = N;
+    a.preact = want_preact ? pre.data_ptr() : nullptr;
+    a.preact_row_stride = round8(N);
+    check_rc(b2s_mx_linear_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes), "b2s_mx_linear_workspace");
+    Tensor ws;
+    if (a.workspace_bytes) {
+        ws = workspace(a.workspace_bytes, x);
+        a.workspace = ws.data_ptr();
+    }
+    a.status = status_ptr(status, x);
+    check_rc(b2s_mx_linear(&a, at::cuda::getCurrentCUDAStream().stream()), "b2s_mx_linear");
+    return {out, pre};
+}
+std::tuple<Tensor, Tensor> mx_linear_meta(const Tensor& x, const optional<Tensor>&, const Tensor& codes, const Tensor&, int64_t,
+                                          const optional<Tensor>&, const optional<Tensor>&, int64_t, bool want_preact,
+                                          const optional<Tensor>&) {
+    return {at::empty({x.size(0), codes.size(0)}, x.options().dtype(at::kBFloat16)),
+            at::empty({want_preact ? x.size(0) : 0, round8(codes.size(0))}, x.options().dtype(at::kHalf))};
+}
+
+// Its gradient, straight through x's rounding: the weight is taken back to bf16 (exactly, but for scales near bf16's
+// smallest numbers) and the projection's gradient does the rest.  Rows of an odd length are filled up to 8.
+std::tuple<Tensor, Tensor> mx_linear_grad_cuda(const Tensor& grad_out, const Tensor& codes, const Tensor& scales,
+                                               int64_t in_features, const optional<Tensor>& preact, int64_t activation,
+                                               bool want_x, bool want_bias, const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(grad_out.device());
+    check_same(grad_out, grad_out, at::kBFloat16, "grad_out");
+    const int32_t N = check_mx(codes, scales, in_features, grad_out, "weight");
+    TORCH_CHECK(N >= 1 && grad_out.dim() == 2 && grad_out.size(1) == N && grad_out.size(0) <= INT32_MAX,
+                "grad_out must be [rows, out]");
+    const int64_t R = grad_out.size(0), K = round8(in_features);
+    TORCH_CHECK(K <= INT32_MAX, "a size is out of range");
+    const Tensor g = plain_rows(grad_out);
+    Tensor dx = fresh({want_x ? R : 0, K}, at::kBFloat16, g), db = fresh({want_bias ? N : 0}, at::kBFloat16, g), w;
+    b2s_linear_grad_args a;
+    memset(&a, 0, sizeof(a));
+    const auto stream = at::cuda::getCurrentCUDAStream().stream();
+    if (want_x && R) {
+        w = fresh({N, K}, at::kBFloat16, g);
+        check_rc(b2s_mx_dequantize(codes.data_ptr(), scales.data_ptr(), N, (int32_t)K, B2S_DTYPE_BF16, w.data_ptr(), K, stream),
+                 "b2s_mx_dequantize");
+        a.weight = w.data_ptr();
+        a.weight_row_stride = K;
+        a.grad_x = dx.data_ptr();
+    }
+    a.grad_out = g.data_ptr();
+    a.grad_out_row_stride = row_stride(g);
+    if (activation != B2S_ACT_NONE) {
+        TORCH_CHECK(preact.has_value() && preact->defined(), "preact is needed with an activation");
+        check_same(*preact, g, at::kHalf, "preact");
+        TORCH_CHECK(preact->dim() == 2 && preact->size(0) == R && preact->size(1) == round8(N) && preact->is_contiguous(),
+                    "preact must be what mx_linear gave");
+        a.preact = preact->data_ptr();
+        a.preact_row_stride = round8(N);
+    }
+    a.rows = (int32_t)R;
+    a.in_features = (int32_t)K;
+    a.out_features = N;
+    a.activation = (int32_t)activation;
+    a.grad_bias = want_bias ? db.data_ptr() : nullptr;
+    check_rc(b2s_linear_grad_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes),
+             "b2s_linear_grad_workspace");
+    Tensor ws = workspace(a.workspace_bytes, g);
+    a.workspace = ws.data_ptr();
+    a.status = status_ptr(status, g);
+    check_rc(b2s_linear_grad(&a, stream), "b2s_linear_grad");
+    return {K == in_features ? dx : dx.narrow(1, 0, in_features), db};
+}
+std::tuple<Tensor, Tensor> mx_linear_grad_meta(const Tensor& grad_out, const Tensor& codes, const Tensor&, int64_t in_features,
+                                               const optional<Tensor>&, int64_t, bool want_x, bool want_bias,
+                                               const optional<Tensor>&) {
+    return {at::empty({want_x ? grad_out.size(0) : 0, round8(in_features)}, grad_out.options()).narrow(1, 0, in_features),
+            at::empty({want_bias ? codes.size(0) : 0}, grad_out.options())};
+}
+
 // ------------------------------------------------------------------ gradients
 // The differentiable operators' Autograd kernels: nodes of torch's graph whose backward calls the gradient ops above.  A
 // call whose inputs need no gradient goes straight on to the CUDA kernel.
@@ -945,6 +1189,23 @@ const auto& linear_op() {
 }
 const auto& linear_grad_op() {
     static const auto op = op_handle<decltype(linear_grad_cuda)>("minicpmo_sampler::linear_grad");
+    return op;
+}
+
+const auto& embedding_op() {
+    static const auto op = op_handle<decltype(embedding_cuda)>("minicpmo_sampler::embedding");
+    return op;
+}
+const auto& embedding_grad_op() {
+    static const auto op = op_handle<decltype(embedding_grad_cuda)>("minicpmo_sampler::embedding_grad");
+    return op;
+}
+const auto& mx_linear_op() {
+    static const auto op = op_handle<decltype(mx_linear_cuda)>("minicpmo_sampler::mx_linear");
+    return op;
+}
+const auto& mx_linear_grad_op() {
+    static const auto op = op_handle<decltype(mx_linear_grad_cuda)>("minicpmo_sampler::mx_linear_grad");
     return op;
 }
 
@@ -1120,6 +1381,94 @@ std::tuple<Tensor, Tensor> linear_autograd(const Tensor& x, const Tensor& weight
     return {o[0], o[1]};
 }
 
+struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& table, double scale,
+                                 const optional<Tensor>& status) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        Tensor out = embedding_op().call(tokens, table, scale, status);
+        ctx->save_for_backward({tokens});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["vocab"] = table.size(0);
+        ctx->set_materialize_grads(false);
+        return {out};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(4);
+        if (!g[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            out[1] = embedding_grad_op().call(g[0], saved[0], ctx->saved_data["vocab"].toInt(),
+                                              ctx->saved_data["scale"].toDouble());
+        }
+        seal(out, "embedding");
+        return out;
+    }
+};
+
+Tensor embedding_autograd(const Tensor& tokens, const Tensor& table, double scale, const optional<Tensor>& status) {
+    refuse_tangents("embedding", table);
+    if (!at::GradMode::is_enabled() || !needs_grad(table)) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return embedding_op().call(tokens, table, scale, status);
+    }
+    check_capture({table});
+    return EmbeddingNode::apply(tokens, table, scale, status)[0];
+}
+
+struct MxLinearNode : public torch::autograd::Function<MxLinearNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& x_scales, const Tensor& codes,
+                                 const Tensor& scales, int64_t in_features, const optional<Tensor>& bias,
+                                 const optional<Tensor>& residual, int64_t activation, const optional<Tensor>& status) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [out, pre] = mx_linear_op().call(x, x_scales, codes, scales, in_features, bias, residual, activation,
+                                              activation != B2S_ACT_NONE, status);
+        ctx->save_for_backward({codes, scales, activation != B2S_ACT_NONE ? pre : Tensor()});
+        keep_status(ctx, status);
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["in"] = in_features;
+        // the graph's edges are numbered over the tensors that were there
+        ctx->saved_data["x_scales"] = x_scales.has_value() && x_scales->defined();
+        ctx->saved_data["bias"] = bias.has_value() && bias->defined();
+        ctx->saved_data["residual"] = residual.has_value() && residual->defined();
+        ctx->mark_non_differentiable({pre});
+        ctx->set_materialize_grads(false);
+        return {out, pre};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(9);
+        if (!g[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
+        int edge = ctx->saved_data["x_scales"].toBool() ? 4 : 3;  // of the bias, or what follows
+        const bool want_x = ctx->needs_input_grad(0), want_b = has_b && ctx->needs_input_grad(edge);
+        if (want_x || want_b) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            auto [dx, db] = mx_linear_grad_op().call(g[0], saved[0], saved[1], ctx->saved_data["in"].toInt(), or_null(saved[2]),
+                                                     ctx->saved_data["activation"].toInt(), want_x, want_b, kept_status(ctx));
+            if (want_x) out[0] = dx;
+            if (want_b) out[5] = db;
+        }
+        seal(out, "mx_linear");
+        if (has_r && ctx->needs_input_grad(edge + has_b)) out[6] = g[0];
+        return out;
+    }
+};
+
+std::tuple<Tensor, Tensor> mx_linear_autograd(const Tensor& x, const optional<Tensor>& x_scales, const Tensor& codes,
+                                              const Tensor& scales, int64_t in_features, const optional<Tensor>& bias,
+                                              const optional<Tensor>& residual, int64_t activation, bool want_preact,
+                                              const optional<Tensor>& status) {
+    refuse_tangents("mx_linear", x, bias, residual);
+    if (!at::GradMode::is_enabled() || !(needs_grad(x) || needs_grad(bias) || needs_grad(residual))) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return mx_linear_op().call(x, x_scales, codes, scales, in_features, bias, residual, activation, want_preact, status);
+    }
+    check_capture({x, or_none(bias), or_none(residual)});
+    variable_list o = MxLinearNode::apply(x, x_scales, codes, scales, in_features, bias, residual, activation, status);
+    return {o[0], o[1]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(minicpmo_sampler, m) {
@@ -1185,6 +1534,17 @@ TORCH_LIBRARY(minicpmo_sampler, m) {
     m.def(
         "linear_grad(Tensor grad_out, Tensor x, Tensor weight, Tensor? preact, int activation, bool want_x, "
         "bool want_weight, bool want_bias, Tensor? status) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias)");
+    m.def("embedding(Tensor tokens, Tensor table, float scale, Tensor? status) -> Tensor");
+    m.def("embedding_mx(Tensor tokens, Tensor codes, Tensor scales, int width, float scale, Tensor? status) -> Tensor");
+    m.def("embedding_grad(Tensor grad_out, Tensor tokens, int vocab, float scale) -> Tensor");
+    m.def("mx_quantize(Tensor x) -> (Tensor codes, Tensor scales)");
+    m.def("mx_dequantize(Tensor codes, Tensor scales, int k, ScalarType dtype) -> Tensor");
+    m.def(
+        "mx_linear(Tensor x, Tensor? x_scales, Tensor codes, Tensor scales, int in_features, Tensor? bias, Tensor? residual, "
+        "int activation, bool want_preact, Tensor? status) -> (Tensor out, Tensor preact)");
+    m.def(
+        "mx_linear_grad(Tensor grad_out, Tensor codes, Tensor scales, int in_features, Tensor? preact, int activation, "
+        "bool want_x, bool want_bias, Tensor? status) -> (Tensor grad_x, Tensor grad_bias)");
 }
 
 TORCH_LIBRARY_IMPL(minicpmo_sampler, CUDA, m) {
@@ -1206,6 +1566,13 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, CUDA, m) {
     m.impl("lmhead_logprobs_grad", &lmhead_logprobs_grad_cuda);
     m.impl("linear", &linear_cuda);
     m.impl("linear_grad", &linear_grad_cuda);
+    m.impl("embedding", &embedding_cuda);
+    m.impl("embedding_mx", &embedding_mx_cuda);
+    m.impl("embedding_grad", &embedding_grad_cuda);
+    m.impl("mx_quantize", &mx_quantize_cuda);
+    m.impl("mx_dequantize", &mx_dequantize_cuda);
+    m.impl("mx_linear", &mx_linear_cuda);
+    m.impl("mx_linear_grad", &mx_linear_grad_cuda);
 }
 
 TORCH_LIBRARY_IMPL(minicpmo_sampler, Meta, m) {
@@ -1227,10 +1594,19 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, Meta, m) {
     m.impl("lmhead_logprobs_grad", &lmhead_logprobs_grad_meta);
     m.impl("linear", &linear_meta);
     m.impl("linear_grad", &linear_grad_meta);
+    m.impl("embedding", &embedding_meta);
+    m.impl("embedding_mx", &embedding_mx_meta);
+    m.impl("embedding_grad", &embedding_grad_meta);
+    m.impl("mx_quantize", &mx_quantize_meta);
+    m.impl("mx_dequantize", &mx_dequantize_meta);
+    m.impl("mx_linear", &mx_linear_meta);
+    m.impl("mx_linear_grad", &mx_linear_grad_meta);
 }
 
 TORCH_LIBRARY_IMPL(minicpmo_sampler, Autograd, m) {
     m.impl("token_logprobs", &token_logprobs_autograd);
     m.impl("lmhead_logprobs", &lmhead_logprobs_autograd);
     m.impl("linear", &linear_autograd);
+    m.impl("embedding", &embedding_autograd);
+    m.impl("mx_linear", &mx_linear_autograd);
 }
