@@ -16,146 +16,31 @@ int tensor_map_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t out
 
 namespace {
 
-// Tile t (TM rows each) of the order that takes GM_GROUP x 128 rows at a time.
-template <int TM>
-__device__ __forceinline__ void tile_of(const GemmArgs& a, int64_t t, int* mt, int* nt) {
-    constexpr int GROUP = GM_GROUP * GM_M / TM;
-    const int64_t per = (int64_t)GROUP * a.tiles_n;
-    const int g = (int)(t / per), in = (int)(t % per);
-    const int gm = min(GROUP, a.tiles_m - g * GROUP);
-    *mt = g * GROUP + in % gm;
-    *nt = in / gm;
-}
-
-// The i-th piece of work of CTA (or pair) c of G: a tile and its k blocks [kb0, kb1); slot: where its sums go, -1 for a whole tile.
-struct Piece {
-    int64_t tile;
-    int kb0, kb1, slot;
-};
-template <int CG>
-__device__ __forceinline__ bool piece_at(const GemmArgs& a, int i, Piece* p) {
-    const int c = (int)blockIdx.x / CG, G = (int)gridDim.x / CG;
-    p->kb0 = 0;
-    p->kb1 = a.nkb;
-    p->slot = -1;
-    if (i < a.waves) {
-        p->tile = (int64_t)i * G + c;
-        return true;
-    }
-    const int64_t u = (int64_t)(i - a.waves) * G + c;
-    if (u >= (int64_t)a.rest * a.split) return false;
-    p->tile = (int64_t)a.waves * G + u % a.rest;
-    if (a.split > 1) {
-        p->kb0 = (int)(u / a.rest) * a.chunk;
-        p->kb1 = min(a.nkb, p->kb0 + a.chunk);
-        p->slot = (int)u;
-    }
-    return true;
-}
-
-template <int N>
-__device__ __forceinline__ void fill_nan(float (&v)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = __int_as_float(0x7fffffff);
-}
-// Whether a block of 32 columns from n is copied as 16-byte vectors.
-__device__ __forceinline__ bool vec_block(const GemmArgs& a, int n, int aligned) { return aligned && n + 32 <= a.N; }
-// The residual's block of 32 columns from n of the 32 rows from row0.
-__device__ __forceinline__ void residual_fetch(const GemmArgs& a, uint32_t (&q)[16], int row0, int n) {
-    if (a.residual && n < a.N)
-        block_fetch(q, static_cast<const unsigned short*>(a.residual) + (int64_t)row0 * a.res_stride + n, a.res_stride,
-                    a.M - row0, a.N - n, vec_block(a, n, a.res_vec));
-}
-
 // The epilogue of one warp: 32 rows of a tile, columns [n0, n0 + COLS) from tensor memory at `tm` (lane = row).  `rq`:
 // the residual's first block.  Not `good`: the accumulator was given up, and NaN takes its place.
 template <int TM, int TN, int EPI>
 __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, bool good, int row0, int n0, int nt, int slot,
                                               unsigned char* st, uint32_t (&rq)[16]) {
     constexpr int COLS = TN / 2;
-    const int lane = threadIdx.x & 31;
-    const int rows = min(32, a.M - row0);  // <= 0: a warp past the last row
-    {
-        if (slot >= 0) {  // a chunk of a split tile: its fp32 sums as they are
-            const int held = min(a.M, TM);
-            float* dst = a.partial + ((int64_t)slot * held + row0 % TM) * TN + n0 - nt * TN;
-#pragma unroll 1
-            for (int q = 0; q < COLS / 32; ++q) {
-                float v[32];
-                if (good) tmem_ld32(tm + 32u * q, v);
-                else fill_nan(v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    *stage_at(st, lane, j) = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                                                        __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-                __syncwarp();
-#pragma unroll
-                for (int h = 0; h < 32; h += 16) {  // read before it is stored, as in block_store
-                    uint4 u[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) u[i] = *stage_at(st, h + 4 * i + (lane >> 3), lane & 7);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = h + 4 * i + (lane >> 3);
-                        if (r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)r * TN + 32 * q + 4 * (lane & 7)) = u[i];
-                    }
-                }
-                __syncwarp();
-            }
-            return;
-        }
-        unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride;
-        const bool with_res = EPI == EPI_LINEAR && a.residual;
+    if (slot >= 0) {
 #pragma unroll 1
         for (int q = 0; q < COLS / 32; ++q) {
-            const int n = n0 + 32 * q, cols = a.N - n;
-            if (cols <= 0) break;
-            if (with_res) {
-                block_put(st, rq, vec_block(a, n, a.res_vec));
-                if (q + 1 < COLS / 32) residual_fetch(a, rq, row0, n + 32);  // in flight under this block
-                __syncwarp();
-            }
             float v[32];
             if (good) tmem_ld32(tm + 32u * q, v);
             else fill_nan(v);
-            if constexpr (EPI == EPI_LINEAR) {
-                if (a.bias) {
-                    const float b = lane < cols ? bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + n + lane)) : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
-                }
-                if (a.preact) stage_preact(st, v);
-                if (a.act == ACT_RELU) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_RELU>(v[j]);
-                } else if (a.act == ACT_GELU) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_GELU>(v[j]);
-                } else if (a.act == ACT_SILU) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_SILU>(v[j]);
-                }
-                if (with_res) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint4 u = *stage_at(st, lane, j);
-                        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            v[8 * j + 2 * k] += __uint_as_float(w[k] << 16);
-                            v[8 * j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
-                        }
-                    }
-                }
-            }
-            stage_row(st, 0, v);  // over this lane's own row of the residual
-            __syncwarp();
-            block_store(st, 0, out + n, a.out_stride, rows, cols, vec_block(a, n, a.out_vec));
-            if (EPI == EPI_LINEAR && a.preact)
-                block_store(st, 4, static_cast<unsigned short*>(a.preact) + (int64_t)row0 * a.pre_stride + n, a.pre_stride,
-                            rows, cols, vec_block(a, n, 1));
-            __syncwarp();
+            store_sums<TM, TN>(a, v, row0, n0 + 32 * q, nt, slot, st);
         }
+        return;
+    }
+#pragma unroll 1
+    for (int q = 0; q < COLS / 32; ++q) {
+        const int n = n0 + 32 * q;
+        if (n >= a.N) break;
+        if (EPI == EPI_LINEAR) residual_put(a, rq, row0, n, q + 1 < COLS / 32, st);
+        float v[32];
+        if (good) tmem_ld32(tm + 32u * q, v);
+        else fill_nan(v);
+        store_block<EPI>(a, v, row0, n, st);
     }
 }
 
@@ -476,65 +361,12 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
     }
 }
 
-// Adds a split tile's sums in k order and runs the epilogue: a thread per 4 columns of a row, grid.y = the split tiles.
-constexpr int FIX_NT = 256;
-template <int TM, int TN, int EPI>
-__global__ void __launch_bounds__(FIX_NT) gemm_join_kernel(const __grid_constant__ GemmArgs a, int G) {
-    pdl_wait_then_release();
-    int mt, nt;
-    tile_of<TM>(a, (int64_t)a.waves * G + blockIdx.y, &mt, &nt);
-    const int held = min(a.M, TM), rows = min(TM, a.M - mt * TM);
-    const int i = (int)blockIdx.x * FIX_NT + (int)threadIdx.x;
-    const int lr = i / (TN / 4), n = nt * TN + (i % (TN / 4)) * 4, row = mt * TM + lr;
-    if (lr >= rows || n >= a.N) return;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const float* part = a.partial + ((int64_t)blockIdx.y * held + lr) * TN + n - nt * TN;
-    const int64_t step = (int64_t)a.rest * held * TN;
-#pragma unroll 4
-    for (int s = 0; s < a.split; ++s) {
-        const float4 p = *reinterpret_cast<const float4*>(part + s * step);
-        v[0] += p.x;
-        v[1] += p.y;
-        v[2] += p.z;
-        v[3] += p.w;
-    }
-    unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row * a.out_stride + n;
-    const int cols = min(4, a.N - n);
-    if (EPI == EPI_LINEAR) {
-        const unsigned short* bias = static_cast<const unsigned short*>(a.bias);
-        const unsigned short* res = static_cast<const unsigned short*>(a.residual) + (int64_t)row * a.res_stride + n;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j < cols) {
-                if (bias) v[j] += bf16_bits_to_f(__ldg(bias + n + j));
-                if (a.preact)
-                    (static_cast<unsigned short*>(a.preact) + (int64_t)row * a.pre_stride + n)[j] = preact_bits(v[j]);
-                v[j] = act_apply(v[j], a.act);
-                if (a.residual) v[j] += bf16_bits_to_f(__ldg(res + j));
-            }
-        }
-    }
-    if (a.out_vec && cols == 4) {
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cols) out[j] = __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
-    }
-}
-
 // An operand of a product: rows of `k` elements `stride` apart (k contiguous), or, transposed, k rows of `m` elements.
 struct Operand {
     const void* base;
     int64_t stride;
 };
 
-// How a product is cut: CTAs per tile, columns per tile, CTAs (or pairs) at work, whole waves, the rest and the chunks
-// along k that the rest is cut into.
-struct Plan {
-    int cg, tn, G, waves, rest, split, chunk;
-    int64_t bytes;  // of the split's workspace
-};
 // The cheapest cut by estimated clocks.  A k block costs a CTA its MMAs (measured without loads: 530 clocks for 256 or
 // 128 columns alike, 290 for 64) or its stage's way from L2 (64 bytes a clock; rows outside A are not fetched).  An
 // epilogue costs 14 clocks a column where it only stores, 40 with the projection's bias, activation, residual and
@@ -606,6 +438,8 @@ Plan plan_for(int M, int N, int64_t K, int epi, int sms) {
     return best;
 }
 
+}  // namespace
+
 // Multiprocessors of the current device (without one, where only sizes are asked for, a B200's 148).
 int sms_here() {
     int sms = 0;
@@ -634,6 +468,8 @@ Plan plan_here(int M, int N, int64_t K, int epi) {
     }
     return k.plan;
 }
+
+namespace {
 
 template <int CG, int TN, bool AMN, bool BMN, int EPI>
 int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, const Plan& p, void* stream) {

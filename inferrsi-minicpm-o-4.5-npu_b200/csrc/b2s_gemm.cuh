@@ -293,7 +293,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 // This lane's row of 32 values into chunks `base` .. base + 3, each rounded once to bf16 (the output's type).
-__device__ __forceinline__ void stage_row(unsigned char* st, int base, const float (&v)[32]) {
+__device__ __forceinline__ void stage_row(unsigned char* st, int base, const float* v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -310,7 +310,7 @@ __device__ __forceinline__ unsigned short preact_bits(float z) {
     return z > 0.0f && h == 0 ? 1 : h;
 }
 __device__ __forceinline__ float preact_value(unsigned short h) { return __half2float(__ushort_as_half(h)); }
-__device__ __forceinline__ void stage_preact(unsigned char* st, const float (&v)[32]) {
+__device__ __forceinline__ void stage_preact(unsigned char* st, const float* v) {
     const int lane = threadIdx.x & 31;
     auto two = [](float a, float b) { return (uint32_t)preact_bits(a) | (uint32_t)preact_bits(b) << 16; };
 #pragma unroll
@@ -353,4 +353,189 @@ __device__ __forceinline__ void store8(void* row, int n, int N, bool vec, const 
     }
 }
 
+// How a product is cut: CTAs per tile, columns per tile, CTAs (or pairs) at work, whole waves, the rest and the chunks
+// along k that the rest is cut into.
+struct Plan {
+    int cg, tn, G, waves, rest, split, chunk;
+    int64_t bytes;  // of the split's workspace
+};
+int sms_here();
+Plan plan_here(int M, int N, int64_t K, int epi);
+
+namespace {
+
+// Tile t (TM rows each) of the order that takes GM_GROUP x 128 rows at a time.
+template <int TM>
+__device__ __forceinline__ void tile_of(const GemmArgs& a, int64_t t, int* mt, int* nt) {
+    constexpr int GROUP = GM_GROUP * GM_M / TM;
+    const int64_t per = (int64_t)GROUP * a.tiles_n;
+    const int g = (int)(t / per), in = (int)(t % per);
+    const int gm = min(GROUP, a.tiles_m - g * GROUP);
+    *mt = g * GROUP + in % gm;
+    *nt = in / gm;
+}
+
+// The i-th piece of work of CTA (or pair) c of G: a tile and its k blocks [kb0, kb1); slot: where its sums go, -1 for a whole tile.
+struct Piece {
+    int64_t tile;
+    int kb0, kb1, slot;
+};
+template <int CG>
+__device__ __forceinline__ bool piece_at(const GemmArgs& a, int i, Piece* p) {
+    const int c = (int)blockIdx.x / CG, G = (int)gridDim.x / CG;
+    p->kb0 = 0;
+    p->kb1 = a.nkb;
+    p->slot = -1;
+    if (i < a.waves) {
+        p->tile = (int64_t)i * G + c;
+        return true;
+    }
+    const int64_t u = (int64_t)(i - a.waves) * G + c;
+    if (u >= (int64_t)a.rest * a.split) return false;
+    p->tile = (int64_t)a.waves * G + u % a.rest;
+    if (a.split > 1) {
+        p->kb0 = (int)(u / a.rest) * a.chunk;
+        p->kb1 = min(a.nkb, p->kb0 + a.chunk);
+        p->slot = (int)u;
+    }
+    return true;
+}
+
+template <int N>
+__device__ __forceinline__ void fill_nan(float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = __int_as_float(0x7fffffff);
+}
+// Whether a block of 32 columns from n is copied as 16-byte vectors.
+__device__ __forceinline__ bool vec_block(const GemmArgs& a, int n, int aligned) { return aligned && n + 32 <= a.N; }
+// The residual's block of 32 columns from n of the 32 rows from row0.
+__device__ __forceinline__ void residual_fetch(const GemmArgs& a, uint32_t (&q)[16], int row0, int n) {
+    if (a.residual && n < a.N)
+        block_fetch(q, static_cast<const unsigned short*>(a.residual) + (int64_t)row0 * a.res_stride + n, a.res_stride,
+                    a.M - row0, a.N - n, vec_block(a, n, a.res_vec));
+}
+
+// A chunk of a split tile: 32 columns of its fp32 sums as they are.
+template <int TM, int TN>
+__device__ __forceinline__ void store_sums(const GemmArgs& a, const float* v, int row0, int n, int nt, int slot,
+                                           unsigned char* st) {
+    const int lane = threadIdx.x & 31, rows = min(32, a.M - row0);  // rows <= 0: a warp past the last row
+    float* dst = a.partial + ((int64_t)slot * min(a.M, TM) + row0 % TM) * TN + n - nt * TN;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        *stage_at(st, lane, j) = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                            __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {  // read before it is stored, as in block_store
+        uint4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = *stage_at(st, h + 4 * i + (lane >> 3), lane & 7);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = h + 4 * i + (lane >> 3);
+            if (r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)r * TN + 4 * (lane & 7)) = u[i];
+        }
+    }
+    __syncwarp();
+}
+// The residual's block of 32 columns from n into the staging block, and the next one's way here begun.
+__device__ __forceinline__ void residual_put(const GemmArgs& a, uint32_t (&rq)[16], int row0, int n, bool more, unsigned char* st) {
+    if (!a.residual) return;
+    block_put(st, rq, vec_block(a, n, a.res_vec));
+    if (more) residual_fetch(a, rq, row0, n + 32);  // in flight under this block
+    __syncwarp();
+}
+// This lane's row of 32 accumulated columns from n through the epilogue and to the output.
+template <int EPI>
+__device__ __forceinline__ void store_block(const GemmArgs& a, float* v, int row0, int n, unsigned char* st) {
+    const int lane = threadIdx.x & 31, rows = min(32, a.M - row0), cols = a.N - n;
+    if constexpr (EPI == EPI_LINEAR) {
+        if (a.bias) {
+            const float b = lane < cols ? bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + n + lane)) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
+        }
+        if (a.preact) stage_preact(st, v);
+        if (a.act == ACT_RELU) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_RELU>(v[j]);
+        } else if (a.act == ACT_GELU) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_GELU>(v[j]);
+        } else if (a.act == ACT_SILU) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_SILU>(v[j]);
+        }
+        if (a.residual) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint4 u = *stage_at(st, lane, j);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[8 * j + 2 * k] += __uint_as_float(w[k] << 16);
+                    v[8 * j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+                }
+            }
+        }
+    }
+    stage_row(st, 0, v);  // over this lane's own row of the residual
+    __syncwarp();
+    block_store(st, 0, static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride + n, a.out_stride, rows, cols,
+                vec_block(a, n, a.out_vec));
+    if (EPI == EPI_LINEAR && a.preact)
+        block_store(st, 4, static_cast<unsigned short*>(a.preact) + (int64_t)row0 * a.pre_stride + n, a.pre_stride, rows, cols,
+                    vec_block(a, n, 1));
+    __syncwarp();
+}
+
+// Adds a split tile's sums in k order and runs the epilogue: a thread per 4 columns of a row, grid.y = the split tiles.
+constexpr int FIX_NT = 256;
+template <int TM, int TN, int EPI>
+__global__ void __launch_bounds__(FIX_NT) gemm_join_kernel(const __grid_constant__ GemmArgs a, int G) {
+    pdl_wait_then_release();
+    int mt, nt;
+    tile_of<TM>(a, (int64_t)a.waves * G + blockIdx.y, &mt, &nt);
+    const int held = min(a.M, TM), rows = min(TM, a.M - mt * TM);
+    const int i = (int)blockIdx.x * FIX_NT + (int)threadIdx.x;
+    const int lr = i / (TN / 4), n = nt * TN + (i % (TN / 4)) * 4, row = mt * TM + lr;
+    if (lr >= rows || n >= a.N) return;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* part = a.partial + ((int64_t)blockIdx.y * held + lr) * TN + n - nt * TN;
+    const int64_t step = (int64_t)a.rest * held * TN;
+#pragma unroll 4
+    for (int s = 0; s < a.split; ++s) {
+        const float4 p = *reinterpret_cast<const float4*>(part + s * step);
+        v[0] += p.x;
+        v[1] += p.y;
+        v[2] += p.z;
+        v[3] += p.w;
+    }
+    unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row * a.out_stride + n;
+    const int cols = min(4, a.N - n);
+    if (EPI == EPI_LINEAR) {
+        const unsigned short* bias = static_cast<const unsigned short*>(a.bias);
+        const unsigned short* res = static_cast<const unsigned short*>(a.residual) + (int64_t)row * a.res_stride + n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j < cols) {
+                if (bias) v[j] += bf16_bits_to_f(__ldg(bias + n + j));
+                if (a.preact)
+                    (static_cast<unsigned short*>(a.preact) + (int64_t)row * a.pre_stride + n)[j] = preact_bits(v[j]);
+                v[j] = act_apply(v[j], a.act);
+                if (a.residual) v[j] += bf16_bits_to_f(__ldg(res + j));
+            }
+        }
+    }
+    if (a.out_vec && cols == 4) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < cols) out[j] = __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
+    }
+}
+
+}  // namespace
 }  // namespace b2s

@@ -10,6 +10,8 @@
 namespace b2s {
 
 int cuda_fail(cudaError_t e);
+Plan mx_plan(int M, int N, int64_t K);
+int mx_gemm(const MxOperand& A, const MxOperand& B, int64_t K, const GemmArgs& a, void* stream);
 
 namespace {
 
@@ -340,6 +342,25 @@ __global__ void __launch_bounds__(MXR_NT) mx_rows_kernel(const __grid_constant__
     }
 }
 
+cudaError_t mx_rows(const MxRowsArgs& a, void* stream) {
+    auto go = [&](auto kernel, int R, int F) {
+        const int64_t per = (int64_t)(MXR_NT / a.tpr) * F;
+        return launch_pdl(kernel, dim3((unsigned)((a.N + per - 1) / per), (unsigned)((a.M + R - 1) / R)), MXR_NT, 0, stream, a);
+    };
+    return a.M == 1 ? go(mx_rows_kernel<1, 4>, 1, 4) : a.M == 2 ? go(mx_rows_kernel<2, 4>, 2, 4) : go(mx_rows_kernel<4, 4>, 4, 4);
+}
+bool mx_few_rows(int rows) { return rows <= 4; }
+
+// The workspace of the tensor cores' path: x's codes and scales, then the sums of tiles that are split.
+struct MxWork {
+    int64_t scales, partial;
+};
+MxWork mx_work(int64_t rows, int64_t k) {
+    auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    const int64_t s = up(rows * mx_row_bytes(k));
+    return {s, s + (rows + 127) / 128 * mx_tiles(k) * 1024};
+}
+
 }  // namespace
 }  // namespace b2s
 
@@ -375,6 +396,10 @@ int b2s_mx_linear_workspace(int32_t rows, int32_t in_features, int32_t out_featu
     using namespace b2s;
     if (rows < 0 || in_features < 1 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
     *bytes = 0;
+    if (rows && !mx_few_rows(rows)) {
+        const MxWork w = mx_work(rows, in_features);
+        *bytes = w.partial + mx_plan(rows, out_features, in_features).bytes;
+    }
     return B2S_OK;
 }
 
@@ -395,34 +420,57 @@ int b2s_mx_linear(const b2s_mx_linear_args* l, void* stream) {
     int64_t need = 0;
     b2s_mx_linear_workspace(l->rows, l->in_features, l->out_features, &need);
     if (need && (!l->workspace || l->workspace_bytes < need || !aligned16(l->workspace))) return B2S_ERR_INVALID;
-    MxRowsArgs a;
+    if (mx_few_rows(l->rows)) {
+        MxRowsArgs a;
+        memset(&a, 0, sizeof(a));
+        a.x = static_cast<const unsigned short*>(l->x);
+        a.x_stride = l->x_row_stride;
+        a.x_vec = aligned16(l->x) && l->x_row_stride % 8 == 0;
+        a.xc = static_cast<const uint8_t*>(l->x_codes);
+        a.xs = static_cast<const uint8_t*>(l->x_scales);
+        a.wc = static_cast<const uint8_t*>(l->weight_codes);
+        a.ws = static_cast<const uint8_t*>(l->weight_scales);
+        a.M = l->rows;
+        a.N = l->out_features;
+        a.K = l->in_features;
+        a.act = l->activation;
+        a.bias = static_cast<const unsigned short*>(l->bias);
+        a.residual = static_cast<const unsigned short*>(l->residual);
+        a.res_stride = l->residual_row_stride;
+        a.preact = static_cast<__half*>(l->preact);
+        a.pre_stride = l->preact_row_stride;
+        a.out = static_cast<__nv_bfloat16*>(l->out);
+        a.out_stride = l->out_row_stride;
+        const int64_t nb = mx_blocks(a.K);
+        a.tpr = nb > 64 ? 128 : nb > 32 ? 64 : 32;
+        const cudaError_t e = mx_rows(a, stream);
+        return e == cudaSuccess ? B2S_OK : cuda_fail(e);
+    }
+    const MxWork w = mx_work(l->rows, l->in_features);
+    unsigned char* ws = static_cast<unsigned char*>(l->workspace);
+    MxOperand x = {l->x_codes, l->x_scales};
+    if (l->x) {
+        x = {ws, ws + w.scales};
+        const cudaError_t e = mx_quantize<false>(l->x, B2S_DTYPE_BF16, l->rows, l->in_features, l->x_row_stride, ws, ws + w.scales, stream);
+        if (e != cudaSuccess) return cuda_fail(e);
+    }
+    GemmArgs a;
     memset(&a, 0, sizeof(a));
-    a.x = static_cast<const unsigned short*>(l->x);
-    a.x_stride = l->x_row_stride;
-    a.x_vec = aligned16(l->x) && l->x_row_stride % 8 == 0;
-    a.xc = static_cast<const uint8_t*>(l->x_codes);
-    a.xs = static_cast<const uint8_t*>(l->x_scales);
-    a.wc = static_cast<const uint8_t*>(l->weight_codes);
-    a.ws = static_cast<const uint8_t*>(l->weight_scales);
     a.M = l->rows;
     a.N = l->out_features;
-    a.K = l->in_features;
-    a.act = l->activation;
-    a.bias = static_cast<const unsigned short*>(l->bias);
-    a.residual = static_cast<const unsigned short*>(l->residual);
-    a.res_stride = l->residual_row_stride;
-    a.preact = static_cast<__half*>(l->preact);
-    a.pre_stride = l->preact_row_stride;
-    a.out = static_cast<__nv_bfloat16*>(l->out);
+    a.status = l->status;
+    a.out = l->out;
     a.out_stride = l->out_row_stride;
-    const int64_t nb = mx_blocks(a.K);
-    a.tpr = nb > 64 ? 128 : nb > 32 ? 64 : 32;
-    auto go = [&](auto kernel, int R, int F) {
-        const int64_t per = (int64_t)(MXR_NT / a.tpr) * F;
-        return launch_pdl(kernel, dim3((unsigned)((a.N + per - 1) / per), (unsigned)((a.M + R - 1) / R)), MXR_NT, 0, stream, a);
-    };
-    const cudaError_t e = a.M == 1 ? go(mx_rows_kernel<1, 4>, 1, 4) : a.M == 2 ? go(mx_rows_kernel<2, 4>, 2, 4) : go(mx_rows_kernel<4, 4>, 4, 4);
-    return e == cudaSuccess ? B2S_OK : cuda_fail(e);
+    a.out_vec = aligned16(l->out) && l->out_row_stride % 8 == 0;
+    a.bias = l->bias;
+    a.residual = l->residual;
+    a.res_stride = l->residual_row_stride;
+    a.res_vec = aligned16(l->residual) && l->residual_row_stride % 8 == 0;
+    a.act = l->activation;
+    a.preact = l->preact;
+    a.pre_stride = l->preact_row_stride;
+    a.partial = reinterpret_cast<float*>(ws + w.partial);
+    return mx_gemm(x, {l->weight_codes, l->weight_scales}, l->in_features, a, stream);
 }
 
 }  // extern "C"

@@ -16,6 +16,12 @@ namespace b2s {
 
 constexpr int MX_BLOCK = 32;
 
+// A 4-bit matrix.
+struct MxOperand {
+    const void* codes;
+    const void* scales;
+};
+
 __host__ __device__ constexpr int64_t mx_blocks(int64_t k) { return (k + MX_BLOCK - 1) / MX_BLOCK; }
 __host__ __device__ constexpr int64_t mx_row_bytes(int64_t k) { return mx_blocks(k) * 16; }
 __host__ __device__ constexpr int64_t mx_tiles(int64_t k) { return (mx_blocks(k) + 7) / 8; }  // along a row

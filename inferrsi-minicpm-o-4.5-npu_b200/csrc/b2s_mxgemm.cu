@@ -1,0 +1,379 @@
+// The product of microscaled 4-bit operands on the tensor cores (sm_100a): D[m, n] = sum_k A[m, k] B[n, k] with
+// tcgen05.mma kind::mxf4, whose blocks of 32 k carry their scales into the multiplication, at four times bf16's rate; fp32
+// accumulation in tensor memory; bias, activation and residual in the epilogue.
+//
+// The shape is b2s_gemm.cuh's: persistent CTAs or pairs of them, a TMA ring, one loading and one issuing warp and eight
+// epilogue warps, tiles cut by the same plan (a stage of 256 k holds the same 128 bytes a row and takes the same clocks as
+// one of 64 k in bf16), chunks along k joined by a second kernel.  What is added: a stage brings 1 KB of scales for
+// each 128 rows, copied in the layout of the matrix's scale tiles, and the issuing warp has the tensor cores copy them from
+// shared to tensor memory (tcgen05.cp, each 512 bytes spread over 32 lanes and 4 columns, for all four lane quarters).
+// Each stage of the ring has its own columns there: when a stage is full again, the MMAs that read its scales are done.
+// 256 columns of accumulator leave no room for a second one beside the scales, so the epilogue takes an accumulator to
+// registers at once and gives it back before it does anything else.
+#include <string.h>
+
+#include <atomic>
+
+#include "../../include/b2s_sampler.h"
+#include "b2s_gemm.cuh"
+#include "b2s_launch.cuh"
+#include "b2s_mx.cuh"
+
+namespace b2s {
+
+int cuda_fail(cudaError_t e);
+int tensor_map_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t outer_stride, int box_inner,
+                  int box_outer);
+int tensor_map_words(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int box_inner, int box_outer);
+
+namespace {
+
+constexpr int MXG_KB = 256;  // k per stage: one 128-byte row of the swizzle
+// 128-row scale tiles of B that a tile of TN columns touches
+__host__ __device__ constexpr int mxg_btiles(int tn) { return tn > 128 ? tn / 128 : 1; }
+// A stage of one CTA: 128 rows of A, its share of B, A's scales (1 KB) and all of the tile's B's.
+__host__ __device__ constexpr uint32_t mxg_stage_bytes(int cg, int tn) {
+    return GM_A_BYTES + (uint32_t)(tn / cg) * 128 + 1024 + 1024 * mxg_btiles(tn);
+}
+__host__ __device__ constexpr int mxg_stages(int cg, int tn) {
+    return (int)(184u * 1024u / mxg_stage_bytes(cg, tn)) > 7 ? 7 : (int)(184u * 1024u / mxg_stage_bytes(cg, tn));
+}
+__host__ __device__ constexpr uint32_t mxg_smem(int cg, int tn) {
+    return 1024 + mxg_stages(cg, tn) * mxg_stage_bytes(cg, tn) + GM_STAGING + 256;
+}
+// Tensor memory: the accumulators, then each stage's scales: for each half of 128 k 4 columns of A's and 4 per tile of B's.
+__host__ __device__ constexpr int mxg_accs(int tn) { return tn == 256 ? 1 : 2; }
+__host__ __device__ constexpr int mxg_sf_cols(int tn) { return 8 + 8 * mxg_btiles(tn); }
+__host__ __device__ constexpr uint32_t mxg_tmem(int cg, int tn) {
+    return mxg_accs(tn) * tn + mxg_stages(cg, tn) * mxg_sf_cols(tn) > 256 ? 512 : 256;
+}
+
+// Shared-memory descriptor of 512 bytes of scales: 32 rows of 16 bytes, 8 rows at a time (128 bytes), no swizzle.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// To 4 columns of tensor memory, the same in each quarter of the lanes (of both CTAs, each from its own shared memory).
+template <int CG>
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+            : "memory");
+}
+
+template <int CG, int TN>
+__global__ void __launch_bounds__(GM_THREADS, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                   const __grid_constant__ CUtensorMap asmap, const __grid_constant__ CUtensorMap bsmap,
+                   const __grid_constant__ GemmArgs a) {
+    constexpr int TM = CG * GM_M, BN = TN / CG, ST = mxg_stages(CG, TN), BT = mxg_btiles(TN), ACCS = mxg_accs(TN);
+    constexpr uint32_t STAGE = mxg_stage_bytes(CG, TN), SFA = GM_A_BYTES + BN * 128, SFB = SFA + 1024;
+    constexpr uint32_t SF0 = ACCS * TN, SFC = mxg_sf_cols(TN);  // the scales' first column, columns a stage
+    // E2M1 operands (bits 7-9, 10-11 = 1), both K-major, N >> 3 at bit 17, E8M0 scales (bit 23), M >> 4 at bit 24; which two
+    // of a column's four scales A and B take at bits 29 and 4
+    constexpr uint32_t IDESC = (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | (1u << 23) | ((uint32_t)(TM >> 4) << 24);
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+    const uint32_t base_u = smem_u32(smem_raw);
+    unsigned char* sm = smem_raw + (((base_u + 1023u) & ~1023u) - base_u);
+    unsigned char* staging = sm + ST * STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + GM_STAGING);  // the first CTA's serves both
+    uint64_t* empty = full + ST;
+    uint64_t* tfull = empty + ST;      // [ACCS] an accumulator is complete
+    uint64_t* tempty = tfull + ACCS;   // [ACCS] an accumulator has been read (the first CTA's, by both)
+    uint64_t* drain = tempty + ACCS;   // every MMA issued has completed (only after a failure)
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
+    volatile int* issued = fail + 1;    // stage loads issued
+    volatile int* consumed = fail + 2;  // stage loads seen to land
+
+    if (tid == 0) {
+        prefetch_tensormap(&amap);
+        prefetch_tensormap(&bmap);
+        prefetch_tensormap(&asmap);
+        prefetch_tensormap(&bsmap);
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < ACCS; ++s) {
+            mbar_init(&tfull[s], 1);
+            mbar_init(&tempty[s], 32 * GM_EPI * CG);
+        }
+        mbar_init(drain, 1);
+        fence_mbar_init();
+        *fail = 0;
+        *issued = 0;
+        *consumed = 0;
+    }
+    if (warp == GM_EPI + 1) {
+        if constexpr (CG == 2) tmem_alloc_pair(tslot, mxg_tmem(CG, TN));
+        else tmem_alloc(tslot, mxg_tmem(CG, TN));
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) {  // the partner's mbarriers exist before anything signals them
+        cluster_arrive_release();
+        cluster_wait();
+    }
+    tc_fence_after();
+    const uint32_t tmem = *tslot;
+    pdl_wait_then_release();
+
+    if (warp == GM_EPI) {
+        int s = 0, it = 0;
+        uint32_t ph = 1;  // parity of `empty`'s last phase: the first round finds every stage free
+        bool ok = a.wait > 0;
+        const uint32_t bar0 = CG == 2 ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
+        Piece p;
+        for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
+            int mt, nt;
+            tile_of<TM>(a, p.tile, &mt, &nt);
+            const int m0 = mt * TM + (int)rank * GM_M, n0 = nt * TN + (int)rank * BN;
+            for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
+                if (!__all_sync(0xffffffffu, gm_wait<false>(&empty[s], ph, a.wait))) {
+                    *fail = 1;
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
+                    unsigned char* st = sm + s * STAGE;
+                    // parts outside the tensors are filled with zeros and count as bytes
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * STAGE);
+                    auto load = [&](unsigned char* dst, const CUtensorMap* map, int x, int y) {
+                        if constexpr (CG == 2) tma_load_2d_pair(dst, map, x, y, bar0 + 8u * s);
+                        else tma_load_2d(dst, map, x, y, &full[s]);
+                    };
+                    load(st, &amap, kb * (MXG_KB / 4), m0);  // in units of 2 bytes
+                    load(st + GM_A_BYTES, &bmap, kb * (MXG_KB / 4), n0);
+                    load(st + SFA, &asmap, kb * 256, m0 / 128);  // in words
+                    load(st + SFB, &bsmap, kb * 256, nt * TN / 128);
+                }
+                __syncwarp();
+                if (++s == ST) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+        }
+        if (lane == 0) *issued = it;
+        // the first CTA's last signals to this CTA's `empty` have landed before it leaves
+        if (CG == 2 && ok)
+            for (int k = it > ST ? it - ST : 0; k < it; ++k)
+                if (!gm_wait<false>(&empty[k % ST], (uint32_t)(k / ST) & 1u, a.wait)) {
+                    *fail = 1;
+                    break;
+                }
+    } else if (warp == GM_EPI + 1) {
+        if (rank == 0) {  // MMAs
+            int s = 0, it = 0;
+            uint32_t ph = 0;
+            bool ok = a.wait > 0;
+            const uint64_t da0 = umma_desc_sw128(smem_u32(sm)), db0 = umma_desc_sw128(smem_u32(sm) + GM_A_BYTES);
+            const uint64_t sf0 = scale_desc(smem_u32(sm) + SFA);
+            auto commit = [&](uint64_t* bar) {
+                if constexpr (CG == 2) umma_commit_pair(bar);
+                else umma_commit(bar);
+            };
+            Piece p;
+            int g = 0;  // accumulators handed over
+            for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i, ++g) {
+                int mt, nt;
+                tile_of<TM>(a, p.tile, &mt, &nt);
+                const int acc = g % ACCS;
+                if (g >= ACCS &&
+                    !__all_sync(0xffffffffu, gm_wait<CG == 2>(&tempty[acc], (uint32_t)(g / ACCS - 1) & 1u, a.wait))) {
+                    *fail = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(acc * TN);
+                // a tile of 64 columns may be the second half of its scale tile's rows: two columns on
+                const uint32_t half = TN < 128 ? (uint32_t)(nt * TN % 128) / 32 : 0u;
+                uint32_t more = 0;
+                for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
+                    if (!__all_sync(0xffffffffu, gm_wait<false>(&full[s], ph, a.wait))) {
+                        *fail = 1;
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t at = (uint32_t)s * (STAGE >> 4);  // a stage on, in units of 16
+                        const uint32_t sa = tmem + SF0 + (uint32_t)s * SFC, sb = sa + 8;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            scales_to_tmem<CG>(sa + 4 * h, sf0 + at + 32 * h);
+#pragma unroll
+                            for (int t = 0; t < BT; ++t) scales_to_tmem<CG>(sb + 4 * BT * h + 4 * t, sf0 + at + 64 + 64 * t + 32 * h);
+                        }
+#pragma unroll
+                        for (int k = 0; k < MXG_KB / 64; ++k) {  // 64 k: 32 bytes
+                            const uint32_t id = IDESC | (uint32_t)(k & 1) << 30 | (uint32_t)(k & 1) << 5;
+                            umma_mxf4<CG>(d, da0 + at + 2 * k, db0 + at + 2 * k, id, sa + 4 * (k >> 1), sb + 4 * BT * (k >> 1) + half, more);
+                            more = 1;
+                        }
+                        commit(&empty[s]);
+                        if (kb + 1 == p.kb1) commit(&tfull[acc]);
+                    }
+                    more = 1;
+                    __syncwarp();
+                    if (++s == ST) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+            }
+            if (lane == 0) *consumed = it;
+        }
+    } else {
+        Piece p;
+        int g = 0;
+        bool ok = a.wait > 0;
+        if (!ok) *fail = 1;
+        constexpr int COLS = TN / 2;
+        const int half = warp >> 2;
+        const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * COLS);
+        unsigned char* st = staging + warp * 4096;
+        // once a wait gave up the pieces that are left take NaN without waiting
+        for (int i = 0; piece_at<CG>(a, i, &p); ++i) {
+            int mt, nt;
+            tile_of<TM>(a, p.tile, &mt, &nt);
+            const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32, n0 = nt * TN + half * COLS;
+            uint32_t rq[16];
+            if (p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
+            const int acc = g % ACCS;
+            ok = ok && __all_sync(0xffffffffu, gm_wait<false>(&tfull[acc], (uint32_t)(g / ACCS) & 1u, a.wait) && !*fail);
+            if (!ok) *fail = 1;
+            tc_fence_after();
+            float v[COLS];
+#pragma unroll
+            for (int q = 0; q < COLS / 32; ++q) tmem_ld32(tm + (uint32_t)(acc * TN + 32 * q), v + 32 * q);
+            if (ok) {
+                tc_fence_before();
+                if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
+                else mbar_arrive(&tempty[acc]);
+                ++g;
+            } else {
+                fill_nan(v);
+            }
+#pragma unroll 1
+            for (int q = 0; q < COLS / 32; ++q) {
+                const int n = n0 + 32 * q;
+                if (p.slot >= 0) {
+                    store_sums<TM, TN>(a, v, row0, n, nt, p.slot, st);
+                } else {
+                    if (n >= a.N) break;
+                    residual_put(a, rq, row0, n, q + 1 < COLS / 32, st);
+                    store_block<EPI_LINEAR>(a, v, row0, n, st);
+                }
+#pragma unroll
+                for (int j = 0; j + 32 < COLS; ++j) v[j] = v[j + 32];  // the loop's body stays short
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*fail && warp == GM_EPI + 1 && rank == 0) {  // every MMA issued has completed
+        if (elect_one()) {
+            if constexpr (CG == 2) umma_commit_pair(drain);
+            else umma_commit(drain);
+        }
+        __syncwarp();
+        gm_wait<false>(drain, 0u);
+        tc_fence_before();
+    }
+    if (*fail && tid == 0) {
+        if (a.status) atomicOr(a.status, B2S_STATUS_WAIT_TIMEOUT);
+        // loads issued but not seen landing still write this CTA's shared memory: those that the first CTA counts are
+        // waited for, any other for a millisecond, a thousand times what a load takes
+        if (rank == 0)
+            for (int it = *consumed; it < *issued; ++it)
+                gm_wait<false>(&full[it % ST], (uint32_t)(it / ST) & 1u);
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000ull) {
+        }
+    }
+    if (*fail) __syncthreads();  // the same for all: nothing writes it after the barrier above
+    if constexpr (CG == 2) {  // neither CTA leaves while the other may signal it or its MMAs read its shared memory
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait();
+    }
+    if (warp == GM_EPI + 1) {
+        tc_fence_after();
+        if constexpr (CG == 2) tmem_dealloc_pair(tmem, mxg_tmem(CG, TN));
+        else tmem_dealloc(tmem, mxg_tmem(CG, TN));
+    }
+}
+
+template <int CG, int TN>
+int mx_gemm_tn(const MxOperand& A, const MxOperand& B, int64_t K, GemmArgs a, const Plan& p, void* stream) {
+    constexpr int TM = CG * GM_M;
+    a.wait = wait_limit();
+    CUtensorMap amap, bmap, asmap, bsmap;
+    const int64_t row = mx_row_bytes(K) / 2, tiles = mx_tiles(K);  // a row's codes in units of 2 bytes
+    int rc = tensor_map_2d(&amap, A.codes, row, a.M, row, MXG_KB / 4, GM_M);
+    if (rc == B2S_OK) rc = tensor_map_2d(&bmap, B.codes, row, a.N, row, MXG_KB / 4, TN / CG);
+    if (rc == B2S_OK) rc = tensor_map_words(&asmap, A.scales, tiles * 256, (a.M + 127) / 128, 256, 1);
+    if (rc == B2S_OK) rc = tensor_map_words(&bsmap, B.scales, tiles * 256, (a.N + 127) / 128, 256, mxg_btiles(TN));
+    if (rc != B2S_OK) return rc;
+    a.tiles_m = (a.M + TM - 1) / TM;
+    a.tiles_n = (a.N + TN - 1) / TN;
+    a.nkb = (int)tiles;
+    a.waves = p.waves;
+    a.rest = p.rest;
+    a.split = p.split;
+    a.chunk = p.chunk;
+    const auto kernel = mx_gemm_kernel<CG, TN>;
+    static std::atomic<bool> set[64];  // the attribute is set once per device; racing callers set the same
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_fail(e);
+    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_relaxed)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)mxg_smem(CG, TN));
+        if (e != cudaSuccess) return cuda_fail(e);
+        if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
+    }
+    e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, GM_THREADS, mxg_smem(CG, TN), stream, amap, bmap, asmap, bsmap, a);
+    if (e == cudaSuccess && p.split > 1) {
+        const int held = a.M < TM ? a.M : TM;
+        e = launch_pdl(gemm_join_kernel<TM, TN, EPI_LINEAR>,
+                       dim3((unsigned)((held * (TN / 4) + FIX_NT - 1) / FIX_NT), (unsigned)p.rest), FIX_NT, 0, stream, a, p.G);
+    }
+    return e == cudaSuccess ? B2S_OK : cuda_fail(e);
+}
+
+}  // namespace
+
+// A stage of 256 k costs what one of 64 k costs the bf16 product: the same bytes a row, the same clocks.
+Plan mx_plan(int M, int N, int64_t K) { return plan_here(M, N, mx_tiles(K) * GM_KB, EPI_LINEAR); }
+
+int mx_gemm(const MxOperand& A, const MxOperand& B, int64_t K, const GemmArgs& a, void* stream) {
+    const Plan p = mx_plan(a.M, a.N, K);
+    if (p.cg == 2) return p.tn == 256 ? mx_gemm_tn<2, 256>(A, B, K, a, p, stream) : mx_gemm_tn<2, 128>(A, B, K, a, p, stream);
+    switch (p.tn) {
+        case 256: return mx_gemm_tn<1, 256>(A, B, K, a, p, stream);
+        case 128: return mx_gemm_tn<1, 128>(A, B, K, a, p, stream);
+        default: return mx_gemm_tn<1, 64>(A, B, K, a, p, stream);
+    }
+}
+
+}  // namespace b2s

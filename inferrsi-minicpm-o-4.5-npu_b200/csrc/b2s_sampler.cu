@@ -1573,6 +1573,20 @@ int tensor_map_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t out
                ? B2S_OK
                : B2S_ERR_INVALID;
 }
+// Rows of 32-bit words, `inner` of them one after another, without a swizzle (the scale tiles of microscaled matrices).
+int tensor_map_words(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int box_inner, int box_outer) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return cuda_fail(cudaErrorNotSupported);
+    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+    const cuuint64_t strides[1] = {(cuuint64_t)inner * 4};
+    const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? B2S_OK
+               : B2S_ERR_INVALID;
+}
 }  // namespace b2s
 
 extern "C" {
