@@ -475,6 +475,26 @@ int b2s_mx_linear_workspace(int32_t rows, int32_t in_features, int32_t out_featu
 int b2s_mx_linear(const b2s_mx_linear_args* args, void* stream);
 
 /*
+ * The projection with what its gradient needs kept in microscaled 8 bits (ABI 8; OCP MX: blocks of 32 along a row, scale 2^e
+ * with e = max(floor(log2 max|x|) - 8, -127), E4M3 elements, at most 448, ties to even): out as b2s_linear gives it, x and z =
+ * x weight^T + bias at 33/32 bytes an element.  A NULL pair of codes and scales is not kept (x where the weight needs no
+ * gradient, z without an activation); args->preact is NULL.
+ *   x_codes [rows][ceil(in / 32) * 32] bytes, x_scales [ceil(in / 32)][rows] bytes; z likewise with out; codes 16-byte aligned
+ * The gradient takes x and z as they were kept: grad_weight = dz^T x^, dz = grad_out act'(z^); args' x and preact are not read.
+ * `workspace`: b2s_linear_checkpoint(_grad)_workspace bytes.
+ */
+typedef struct b2s_linear_kept {
+    void* x_codes;
+    void* x_scales;
+    void* z_codes;
+    void* z_scales;
+} b2s_linear_kept;
+int b2s_linear_checkpoint_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes);
+int b2s_linear_checkpoint(const b2s_linear_args* args, const b2s_linear_kept* kept, void* stream);
+int b2s_linear_checkpoint_grad_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes);
+int b2s_linear_checkpoint_grad(const b2s_linear_grad_args* args, const b2s_linear_kept* kept, void* stream);
+
+/*
  * The bound of each device wait inside the log-probability and projection kernels, in SM clocks: sets it for the calls
  * of this process that follow (clocks >= 0, at most the default of about a quarter of a second); a negative argument only
  * asks.  previous (optional) gets the bound before.  A wait that gives up sets B2S_STATUS_WAIT_TIMEOUT and makes what was not finished NaN

@@ -84,6 +84,12 @@ class LinearGradArgs(ctypes.Structure):
     ]
 
 
+class LinearKept(ctypes.Structure):
+    """b2s_linear_kept of include/b2s_sampler.h."""
+    _fields_ = [("x_codes", ctypes.c_void_p), ("x_scales", ctypes.c_void_p), ("z_codes", ctypes.c_void_p),
+                ("z_scales", ctypes.c_void_p)]
+
+
 class MxLinearArgs(ctypes.Structure):
     """b2s_mx_linear_args of include/b2s_sampler.h."""
     _fields_ = [
@@ -166,6 +172,13 @@ CAPI_SIGNATURES = {
     "b2s_mx_linear_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                                ctypes.POINTER(ctypes.c_int64)]),
     "b2s_mx_linear": (ctypes.c_int, [ctypes.POINTER(MxLinearArgs), ctypes.c_void_p]),
+    "b2s_linear_checkpoint_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                                       ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_linear_checkpoint": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.POINTER(LinearKept), ctypes.c_void_p]),
+    "b2s_linear_checkpoint_grad_workspace": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                                            ctypes.POINTER(ctypes.c_int64)]),
+    "b2s_linear_checkpoint_grad": (ctypes.c_int, [ctypes.POINTER(LinearGradArgs), ctypes.POINTER(LinearKept),
+                                                  ctypes.c_void_p]),
     "b2s_wait_limit": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)]),
     "b2s_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "b2s_last_cuda_error": (ctypes.c_char_p, []),

@@ -11,6 +11,9 @@
 namespace b2s {
 
 int cuda_fail(cudaError_t e);
+// x's rows in microscaled 8 bits and back in bf16 (b2s_mx.cu)
+cudaError_t mx8_quantize(const void* x, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream);
+cudaError_t mx8_dequantize(const void* codes, const void* scales, int64_t rows, int k, void* out, void* stream);
 int tensor_map_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t outer_stride, int box_inner,
                   int box_outer);
 
@@ -36,7 +39,7 @@ __device__ __forceinline__ void epilogue_rows(const GemmArgs& a, uint32_t tm, bo
     for (int q = 0; q < COLS / 32; ++q) {
         const int n = n0 + 32 * q;
         if (n >= a.N) break;
-        if (EPI == EPI_LINEAR) residual_put(a, rq, row0, n, q + 1 < COLS / 32, st);
+        if (epi_linear(EPI)) residual_put(a, rq, row0, n, q + 1 < COLS / 32, st);
         float v[32];
         if (good) tmem_ld32(tm + 32u * q, v);
         else fill_nan(v);
@@ -318,7 +321,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                 }
             } else {
                 uint32_t rq[16];
-                if (EPI == EPI_LINEAR && p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
+                if (epi_linear(EPI) && p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
                 take();
                 epilogue_rows<TM, TN, EPI>(a, tm + (uint32_t)((g & 1) * TN), ok, row0, n0, nt, p.slot, staging + warp * 4096, rq);
                 give();
@@ -500,7 +503,7 @@ int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, const Pla
         if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
     e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, GM_THREADS, gm_smem(CG, TN), stream, amap, bmap, a);
-    if constexpr (EPI == EPI_LINEAR || EPI == EPI_STORE) {
+    if constexpr (epi_linear(EPI) || EPI == EPI_STORE) {
         if (e == cudaSuccess && p.split > 1) {
             const int held = a.M < TM ? a.M : TM;
             e = launch_pdl(gemm_join_kernel<TM, TN, EPI>,
@@ -513,7 +516,7 @@ int gemm_tn(const Operand& A, const Operand& B, int64_t K, GemmArgs a, const Pla
 
 template <bool AMN, bool BMN, int EPI>
 int gemm(const Operand& A, const Operand& B, int64_t K, const GemmArgs& a, void* stream) {
-    const Plan p = plan_here(a.M, a.N, K, EPI);
+    const Plan p = plan_here(a.M, a.N, K, EPI == EPI_KEPT ? EPI_LINEAR : EPI);
     if (p.cg == 2)
         return p.tn == 256 ? gemm_tn<2, 256, AMN, BMN, EPI>(A, B, K, a, p, stream)
                            : gemm_tn<2, 128, AMN, BMN, EPI>(A, B, K, a, p, stream);
@@ -673,9 +676,10 @@ cudaError_t linear_rows(const GemmArgs& a, const void* x, int64_t xs, const void
 // cover 256 columns, the 8 warps take rows in turn; the sums (fp32, of the unrounded dz) go to part[blockIdx.y][n], or,
 // with one part, straight to the bias gradient.
 constexpr int DZ_NT = 256;
-template <bool VEC, int ACT>
+// Z8: z in microscaled 8 bits, `z_scale` its scales [blocks][rows]; else fp16.
+template <bool VEC, int ACT, bool Z8>
 __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_t dy_stride, const void* z,
-                                                          int64_t z_stride, int rows, int N, int rows_per,
+                                                          int64_t z_stride, const uint8_t* z_scale, int rows, int N, int rows_per,
                                                           void* dz, int64_t dz_stride, float* part, void* db) {
     constexpr int E = 8;
     pdl_wait_then_release();
@@ -688,7 +692,6 @@ __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_
 #pragma unroll 4
         for (int r = r0 + rl; r < r1; r += 8) {
             const unsigned short* gp = static_cast<const unsigned short*>(dy) + (int64_t)r * dy_stride + n;
-            const unsigned short* zp = static_cast<const unsigned short*>(z) + (int64_t)r * z_stride + n;
             float g[E], x[E];
             if (VEC || n + E > N) {
                 load8(gp, 0, N - n, VEC, g);
@@ -712,10 +715,23 @@ __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_
                 }
             }
             if constexpr (ACT != ACT_NONE) {
-                const uint4 q = __ldg(reinterpret_cast<const uint4*>(zp));
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                if constexpr (Z8) {
+                    const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(z) + (int64_t)r * z_stride + n));
+                    const float f = mx_scale(__ldg(z_scale + (int64_t)(n >> 5) * rows + r));
+                    float lo[4], hi[4];
+                    mx_decode4_e4m3(q.x, lo);
+                    mx_decode4_e4m3(q.y, hi);
 #pragma unroll
-                for (int j = 0; j < E; ++j) x[j] = preact_value((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+                    for (int j = 0; j < 4; ++j) {
+                        x[j] = lo[j] * f;
+                        x[4 + j] = hi[j] * f;
+                    }
+                } else {
+                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(z) + (int64_t)r * z_stride + n));
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < E; ++j) x[j] = preact_value((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+                }
 #pragma unroll
                 for (int j = 0; j < E; ++j) g[j] *= n + j < N ? act_slope<ACT>(x[j]) : 0.0f;
             }
@@ -895,8 +911,13 @@ int b2s_linear_workspace(int32_t rows, int32_t in_features, int32_t out_features
     return B2S_OK;
 }
 
-int b2s_linear(const b2s_linear_args* l, void* stream) {
-    using namespace b2s;
+}  // extern "C"
+
+namespace b2s {
+namespace {
+
+// The projection; `kept`: what b2s_linear_checkpoint keeps, or null.
+int linear_forward(const b2s_linear_args* l, const b2s_linear_kept* kept, void* stream) {
     if (!l || l->rows < 0 || l->out_features < 1 || l->in_features < 8 || l->in_features % 8 || l->activation < 0 ||
         l->activation > B2S_ACT_SILU)
         return B2S_ERR_INVALID;
@@ -909,8 +930,12 @@ int b2s_linear(const b2s_linear_args* l, void* stream) {
         (l->preact && (!aligned16(l->preact) || l->preact_row_stride < l->out_features || l->preact_row_stride % 8)) ||
         ((reinterpret_cast<uintptr_t>(l->out) | reinterpret_cast<uintptr_t>(l->residual)) & 1))
         return B2S_ERR_INVALID;
+    if (kept && (!kept->x_codes != !kept->x_scales || !kept->z_codes != !kept->z_scales || !aligned16(kept->x_codes) ||
+                 !aligned16(kept->z_codes) || l->preact))
+        return B2S_ERR_INVALID;
     int64_t need = 0;
-    b2s_linear_workspace(l->rows, l->in_features, l->out_features, &need);
+    if (kept) b2s_linear_checkpoint_workspace(l->rows, l->in_features, l->out_features, &need);
+    else b2s_linear_workspace(l->rows, l->in_features, l->out_features, &need);
     if (need && (!l->workspace || l->workspace_bytes < need || !aligned16(l->workspace))) return B2S_ERR_INVALID;
     GemmArgs a;
     memset(&a, 0, sizeof(a));
@@ -928,12 +953,38 @@ int b2s_linear(const b2s_linear_args* l, void* stream) {
     a.preact = l->preact;
     a.pre_stride = l->preact_row_stride;
     a.partial = static_cast<float*>(l->workspace);
-    if (few_rows(l->rows, l->out_features, l->in_features)) {
+    if (kept) {
+        a.z8 = static_cast<uint8_t*>(kept->z_codes);
+        a.z8_scale = static_cast<uint8_t*>(kept->z_scales);
+        if (kept->x_codes) {
+            const cudaError_t e = mx8_quantize(l->x, l->rows, l->in_features, l->x_row_stride, kept->x_codes, kept->x_scales, stream);
+            if (e != cudaSuccess) return cuda_fail(e);
+        }
+    } else if (few_rows(l->rows, l->out_features, l->in_features)) {
         const cudaError_t e = linear_rows(a, l->x, l->x_row_stride, l->weight, l->weight_row_stride, l->in_features, stream);
         return e == cudaSuccess ? B2S_OK : cuda_fail(e);
     }
-    return gemm<false, false, EPI_LINEAR>({l->x, l->x_row_stride}, {l->weight, l->weight_row_stride}, l->in_features, a,
-                                          stream);
+    const Operand x = {l->x, l->x_row_stride}, w = {l->weight, l->weight_row_stride};
+    return a.z8 ? gemm<false, false, EPI_KEPT>(x, w, l->in_features, a, stream)
+                : gemm<false, false, EPI_LINEAR>(x, w, l->in_features, a, stream);
+}
+
+}  // namespace
+}  // namespace b2s
+
+extern "C" {
+
+int b2s_linear(const b2s_linear_args* l, void* stream) { return b2s::linear_forward(l, nullptr, stream); }
+
+int b2s_linear_checkpoint_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
+    using namespace b2s;
+    if (rows < 0 || in_features < 8 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
+    *bytes = rows ? plan_here(rows, out_features, in_features, EPI_LINEAR).bytes : 0;
+    return B2S_OK;
+}
+
+int b2s_linear_checkpoint(const b2s_linear_args* l, const b2s_linear_kept* kept, void* stream) {
+    return kept ? b2s::linear_forward(l, kept, stream) : B2S_ERR_INVALID;
 }
 
 int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
@@ -947,8 +998,20 @@ int b2s_linear_grad_workspace(int32_t rows, int32_t in_features, int32_t out_fea
     return B2S_OK;
 }
 
-int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
+int b2s_linear_checkpoint_grad_workspace(int32_t rows, int32_t in_features, int32_t out_features, int64_t* bytes) {
     using namespace b2s;
+    const int rc = b2s_linear_grad_workspace(rows, in_features, out_features, bytes);
+    if (rc == B2S_OK) *bytes = up(*bytes, 256) + (int64_t)rows * in_features * 2;
+    return rc;
+}
+
+}  // extern "C"
+
+namespace b2s {
+namespace {
+
+// The projection's gradient; `kept`: from what b2s_linear_checkpoint kept, or null.
+int linear_backward(const b2s_linear_grad_args* l, const b2s_linear_kept* kept, void* stream) {
     if (!l || l->rows < 0 || l->out_features < 1 || l->in_features < 8 || l->in_features % 8 || l->activation < 0 ||
         l->activation > B2S_ACT_SILU || (l->grad_weight && !aligned16(l->grad_weight)))
         return B2S_ERR_INVALID;
@@ -961,16 +1024,29 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
             e = cudaMemsetAsync(l->grad_bias, 0, (size_t)l->out_features * 2, (cudaStream_t)stream);
         return e == cudaSuccess ? B2S_OK : cuda_fail(e);
     }
-    int64_t need = 0;
-    b2s_linear_grad_workspace(l->rows, l->in_features, l->out_features, &need);
+    int64_t need = 0, plain = 0;
+    b2s_linear_grad_workspace(l->rows, l->in_features, l->out_features, &plain);
+    if (kept) b2s_linear_checkpoint_grad_workspace(l->rows, l->in_features, l->out_features, &need);
+    else need = plain;
+    const bool z_ok = kept ? kept->z_codes && kept->z_scales && aligned16(kept->z_codes)
+                           : l->preact && aligned16(l->preact) && l->preact_row_stride >= l->out_features && l->preact_row_stride % 8 == 0;
+    const bool x_ok = kept ? kept->x_codes && kept->x_scales && aligned16(kept->x_codes)
+                           : l->x && aligned16(l->x) && l->x_row_stride >= l->in_features && l->x_row_stride % 8 == 0;
     if (!l->grad_out || l->grad_out_row_stride < l->out_features || (reinterpret_cast<uintptr_t>(l->grad_out) & 1) ||
-        !l->workspace || !aligned16(l->workspace) || l->workspace_bytes < need ||
-        (l->activation != B2S_ACT_NONE &&
-         (!l->preact || !aligned16(l->preact) || l->preact_row_stride < l->out_features || l->preact_row_stride % 8)) ||
+        !l->workspace || !aligned16(l->workspace) || l->workspace_bytes < need || (l->activation != B2S_ACT_NONE && !z_ok) ||
         (l->grad_x && (!l->weight || !aligned16(l->weight) || !aligned16(l->grad_x) ||
                        l->weight_row_stride < l->in_features || l->weight_row_stride % 8)) ||
-        (l->grad_weight && (!l->x || !aligned16(l->x) || l->x_row_stride < l->in_features || l->x_row_stride % 8)))
+        (l->grad_weight && !x_ok))
         return B2S_ERR_INVALID;
+    Operand x = {l->x, l->x_row_stride};
+    if (kept && l->grad_weight) {  // x as it was kept, in the products' type (exactly, but below bf16's normal range)
+        void* back = static_cast<unsigned char*>(l->workspace) + up(plain, 256);
+        const cudaError_t e = mx8_dequantize(kept->x_codes, kept->x_scales, l->rows, l->in_features, back, stream);
+        if (e != cudaSuccess) return cuda_fail(e);
+        x = {back, l->in_features};
+    }
+    const void* z = kept ? kept->z_codes : l->preact;
+    const int64_t z_stride = kept ? mx_blocks(l->out_features) * 32 : l->preact_row_stride;
     const int64_t ldz = up(l->out_features, 8);
     const bool dy_vec = aligned16(l->grad_out) && l->grad_out_row_stride % 8 == 0;
     // without an activation dz is dy itself, where the tensor maps can read it
@@ -983,14 +1059,19 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
     if ((products && !direct) || l->grad_bias) {
         const int per = (l->rows + parts - 1) / parts;
         const bool two = l->grad_bias && parts > 1;
-        static constexpr decltype(&linear_dz_kernel<true, ACT_NONE>) kernels[2][4] = {
-            {linear_dz_kernel<false, ACT_NONE>, linear_dz_kernel<false, ACT_RELU>, linear_dz_kernel<false, ACT_GELU>,
-             linear_dz_kernel<false, ACT_SILU>},
-            {linear_dz_kernel<true, ACT_NONE>, linear_dz_kernel<true, ACT_RELU>, linear_dz_kernel<true, ACT_GELU>,
-             linear_dz_kernel<true, ACT_SILU>}};
-        cudaError_t e = launch_pdl(kernels[dy_vec][l->activation],
+        static constexpr decltype(&linear_dz_kernel<true, ACT_NONE, false>) kernels[2][2][4] = {
+            {{linear_dz_kernel<false, ACT_NONE, false>, linear_dz_kernel<false, ACT_RELU, false>,
+              linear_dz_kernel<false, ACT_GELU, false>, linear_dz_kernel<false, ACT_SILU, false>},
+             {linear_dz_kernel<true, ACT_NONE, false>, linear_dz_kernel<true, ACT_RELU, false>,
+              linear_dz_kernel<true, ACT_GELU, false>, linear_dz_kernel<true, ACT_SILU, false>}},
+            {{linear_dz_kernel<false, ACT_NONE, false>, linear_dz_kernel<false, ACT_RELU, true>,
+              linear_dz_kernel<false, ACT_GELU, true>, linear_dz_kernel<false, ACT_SILU, true>},
+             {linear_dz_kernel<true, ACT_NONE, false>, linear_dz_kernel<true, ACT_RELU, true>,
+              linear_dz_kernel<true, ACT_GELU, true>, linear_dz_kernel<true, ACT_SILU, true>}}};
+        cudaError_t e = launch_pdl(kernels[kept != nullptr][dy_vec][l->activation],
                                    dim3((unsigned)((l->out_features + 255) / 256), (unsigned)parts), DZ_NT, 0,
-                                   stream, l->grad_out, l->grad_out_row_stride, l->preact, l->preact_row_stride,
+                                   stream, l->grad_out, l->grad_out_row_stride, z, z_stride,
+                                   kept ? static_cast<const uint8_t*>(kept->z_scales) : (const uint8_t*)nullptr,
                                    (int)l->rows, (int)l->out_features, per,
                                    products && !direct ? l->workspace : nullptr, ldz, two ? part : nullptr,
                                    two ? nullptr : l->grad_bias);
@@ -1017,9 +1098,20 @@ int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) {
     if (l->grad_weight) {
         b.M = l->out_features;
         b.out = l->grad_weight;
-        rc = gemm<true, true, EPI_STORE>(dz, {l->x, l->x_row_stride}, l->rows, b, stream);
+        rc = gemm<true, true, EPI_STORE>(dz, x, l->rows, b, stream);
     }
     return rc;
+}
+
+}  // namespace
+}  // namespace b2s
+
+extern "C" {
+
+int b2s_linear_grad(const b2s_linear_grad_args* l, void* stream) { return b2s::linear_backward(l, nullptr, stream); }
+
+int b2s_linear_checkpoint_grad(const b2s_linear_grad_args* l, const b2s_linear_kept* kept, void* stream) {
+    return kept ? b2s::linear_backward(l, kept, stream) : B2S_ERR_INVALID;
 }
 
 }  // extern "C"

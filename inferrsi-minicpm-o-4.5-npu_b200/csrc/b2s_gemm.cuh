@@ -24,6 +24,7 @@
 
 #include "b2s_head.cuh"
 #include "b2s_logprobs.cuh"
+#include "b2s_mx.cuh"
 
 namespace b2s {
 
@@ -50,7 +51,9 @@ __host__ __device__ constexpr uint32_t gm_smem(int cg, int tn) {
 // quarters a quarter of that.
 constexpr int GM_SEGMENT = 1024 / GM_KB;
 
-enum { EPI_LINEAR = 0, EPI_LSE = 1, EPI_DZ = 2, EPI_STORE = 3 };
+// EPI_KEPT: EPI_LINEAR with the pre-activation kept in microscaled 8 bits (a kernel of its own: in EPI_LINEAR's it cost registers)
+enum { EPI_LINEAR = 0, EPI_LSE = 1, EPI_DZ = 2, EPI_STORE = 3, EPI_KEPT = 4 };
+__host__ __device__ constexpr bool epi_linear(int epi) { return epi == EPI_LINEAR || epi == EPI_KEPT; }
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
 
 struct GemmArgs {
@@ -72,6 +75,9 @@ struct GemmArgs {
     int act;
     void* preact;
     int64_t pre_stride;
+    // EPI_KEPT
+    uint8_t* z8;        // the pre-activation in microscaled 8 bits: [M][N rounded up to 32]
+    uint8_t* z8_scale;  // [blocks of 32 columns][M]
     // EPI_LSE: per row and half of a column tile (m, S, U), the token's value; EPI_DZ: the gradient's inputs
     float c, inv_t;
     const int64_t* tokens;
@@ -319,6 +325,26 @@ __device__ __forceinline__ void stage_preact(unsigned char* st, const float* v) 
                                                 two(v[8 * j + 4], v[8 * j + 5]), two(v[8 * j + 6], v[8 * j + 7]));
 }
 
+// This lane's row of 32 pre-activations, a block, in microscaled 8 bits (E4M3): a fraction of 3 bits, slopes off by up to 2^-4
+// of z times the activation's curvature, for a half of fp16's memory -- what the caller asked for.  Each element is rounded
+// once, from fp32; every slope but the rectifier's is flat where small elements of a block are lost.
+__device__ __forceinline__ void keep_z8(const GemmArgs& a, const float* v, int row, int n) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+    const uint32_t code = mx_scale_code<8>(most);
+    const float inv = mx_inverse(code);
+    if (row >= a.M) return;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        w[j] = mx_encode4_e4m3(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+    uint4* p = reinterpret_cast<uint4*>(a.z8 + (int64_t)row * (mx_blocks(a.N) * 32) + n);
+    p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    a.z8_scale[(int64_t)(n >> 5) * a.M + row] = (uint8_t)code;
+}
+
 // Up to 8 bf16 of a row from column n (N columns), `vec`: the row is 16-byte aligned and n a multiple of 8.
 __device__ __forceinline__ void load8(const void* row, int n, int N, bool vec, float (&x)[8]) {
     const unsigned short* p = static_cast<const unsigned short*>(row) + n;
@@ -450,13 +476,14 @@ __device__ __forceinline__ void residual_put(const GemmArgs& a, uint32_t (&rq)[1
 template <int EPI>
 __device__ __forceinline__ void store_block(const GemmArgs& a, float* v, int row0, int n, unsigned char* st) {
     const int lane = threadIdx.x & 31, rows = min(32, a.M - row0), cols = a.N - n;
-    if constexpr (EPI == EPI_LINEAR) {
+    if constexpr (epi_linear(EPI)) {
         if (a.bias) {
             const float b = lane < cols ? bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(a.bias) + n + lane)) : 0.0f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
         }
-        if (a.preact) stage_preact(st, v);
+        if constexpr (EPI == EPI_KEPT) keep_z8(a, v, row0 + lane, n);
+        else if (a.preact) stage_preact(st, v);
         if (a.act == ACT_RELU) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = act_apply<ACT_RELU>(v[j]);
@@ -500,34 +527,57 @@ __global__ void __launch_bounds__(FIX_NT) gemm_join_kernel(const __grid_constant
     const int held = min(a.M, TM), rows = min(TM, a.M - mt * TM);
     const int i = (int)blockIdx.x * FIX_NT + (int)threadIdx.x;
     const int lr = i / (TN / 4), n = nt * TN + (i % (TN / 4)) * 4, row = mt * TM + lr;
-    if (lr >= rows || n >= a.N) return;
+    const bool live = lr < rows && n < a.N;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const float* part = a.partial + ((int64_t)blockIdx.y * held + lr) * TN + n - nt * TN;
-    const int64_t step = (int64_t)a.rest * held * TN;
+    if (live) {
+        const float* part = a.partial + ((int64_t)blockIdx.y * held + lr) * TN + n - nt * TN;
+        const int64_t step = (int64_t)a.rest * held * TN;
 #pragma unroll 4
-    for (int s = 0; s < a.split; ++s) {
-        const float4 p = *reinterpret_cast<const float4*>(part + s * step);
-        v[0] += p.x;
-        v[1] += p.y;
-        v[2] += p.z;
-        v[3] += p.w;
+        for (int s = 0; s < a.split; ++s) {
+            const float4 p = *reinterpret_cast<const float4*>(part + s * step);
+            v[0] += p.x;
+            v[1] += p.y;
+            v[2] += p.z;
+            v[3] += p.w;
+        }
     }
     unsigned short* out = static_cast<unsigned short*>(a.out) + (int64_t)row * a.out_stride + n;
     const int cols = min(4, a.N - n);
-    if (EPI == EPI_LINEAR) {
+    if constexpr (epi_linear(EPI)) {
         const unsigned short* bias = static_cast<const unsigned short*>(a.bias);
+        if (bias && live) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < cols) v[j] += bf16_bits_to_f(__ldg(bias + n + j));
+        }
+        if constexpr (EPI == EPI_KEPT) {  // a block is 8 threads' columns; those past the last one hold zeros
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const uint32_t code = mx_scale_code<8>(most);
+            const float inv = mx_inverse(code);
+            const int64_t nb = mx_blocks(a.N);
+            if (lr < rows && n < nb * 32) {
+                *reinterpret_cast<uint32_t*>(a.z8 + row * nb * 32 + n) =
+                    mx_encode4_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                if (n % 32 == 0) a.z8_scale[(int64_t)(n >> 5) * a.M + row] = (uint8_t)code;
+            }
+        }
+        if (!live) return;
         const unsigned short* res = static_cast<const unsigned short*>(a.residual) + (int64_t)row * a.res_stride + n;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j < cols) {
-                if (bias) v[j] += bf16_bits_to_f(__ldg(bias + n + j));
-                if (a.preact)
+                if (EPI == EPI_LINEAR && a.preact)
                     (static_cast<unsigned short*>(a.preact) + (int64_t)row * a.pre_stride + n)[j] = preact_bits(v[j]);
                 v[j] = act_apply(v[j], a.act);
                 if (a.residual) v[j] += bf16_bits_to_f(__ldg(res + j));
             }
         }
     }
+    if (!live) return;
     if (a.out_vec && cols == 4) {
         *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
     } else {

@@ -362,6 +362,14 @@ MxWork mx_work(int64_t rows, int64_t k) {
 }
 
 }  // namespace
+
+cudaError_t mx8_quantize(const void* x, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream) {
+    return mx_quantize<true>(x, B2S_DTYPE_BF16, rows, k, row_stride, codes, scales, stream);
+}
+cudaError_t mx8_dequantize(const void* codes, const void* scales, int64_t rows, int k, void* out, void* stream) {
+    return mx_dequantize<true>(codes, scales, rows, k, B2S_DTYPE_BF16, out, k, stream);
+}
+
 }  // namespace b2s
 
 extern "C" {

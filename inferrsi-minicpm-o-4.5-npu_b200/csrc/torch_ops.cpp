@@ -756,61 +756,71 @@ std::tuple<Tensor, Tensor> lmhead_logprobs_grad_meta(const Tensor& hidden, const
 
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
+// A projection's operands as the C entry takes them, and what keeps them alive.
+struct LinearCall {
+    Tensor x, weight, b, r, out;
+    b2s_linear_args a;
+    LinearCall(const Tensor& x_, const Tensor& weight_, const optional<Tensor>& bias, const optional<Tensor>& residual,
+               int64_t activation, const optional<Tensor>& status) {
+        TORCH_CHECK(x_.is_cuda() && x_.dim() == 2 && weight_.dim() == 2 && x_.size(1) == weight_.size(1),
+                    "x must be CUDA [rows, in] and weight [out, in]");
+        check_same(x_, x_, at::kBFloat16, "x");
+        check_same(weight_, x_, at::kBFloat16, "weight");
+        TORCH_CHECK(x_.size(1) >= 8 && x_.size(1) % 8 == 0, "in must be a multiple of 8");
+        TORCH_CHECK(x_.size(0) <= INT32_MAX && x_.size(1) <= INT32_MAX && weight_.size(0) <= INT32_MAX,
+                    "a size is beyond 2^31 - 1");
+        x = aligned_rows(x_);
+        weight = aligned_rows(weight_);
+        const int64_t R = x.size(0), N = weight.size(0);
+        if (bias.has_value() && bias->defined()) {
+            check_same(*bias, x, at::kBFloat16, "bias");
+            TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "bias must be [out]");
+            b = bias->contiguous();
+            if (reinterpret_cast<uintptr_t>(b.data_ptr()) & 15) b = b.clone();
+        }
+        if (residual.has_value() && residual->defined()) {
+            check_same(*residual, x, at::kBFloat16, "residual");
+            TORCH_CHECK(residual->dim() == 2 && residual->size(0) == R && residual->size(1) == N,
+                        "residual must be [rows, out]");
+            r = plain_rows(*residual);
+        }
+        out = fresh({R, N}, at::kBFloat16, x);
+        memset(&a, 0, sizeof(a));
+        a.x = x.data_ptr();
+        a.x_row_stride = row_stride(x);
+        a.weight = weight.data_ptr();
+        a.weight_row_stride = row_stride(weight);
+        a.rows = (int32_t)R;
+        a.in_features = (int32_t)x.size(1);
+        a.out_features = (int32_t)N;
+        a.activation = (int32_t)activation;
+        a.bias = b.defined() ? b.data_ptr() : nullptr;
+        a.residual = r.defined() ? r.data_ptr() : nullptr;
+        a.residual_row_stride = r.defined() ? row_stride(r) : 0;
+        a.out = out.data_ptr();
+        a.out_row_stride = N;
+        a.status = status_ptr(status, x);
+    }
+};
+
 // act(x weight^T + bias) + residual on [rows, in] x; the pre-activation ([rows, out rounded up to 8]) where asked for.
-std::tuple<Tensor, Tensor> linear_cuda(const Tensor& x_, const Tensor& weight_, const optional<Tensor>& bias,
+std::tuple<Tensor, Tensor> linear_cuda(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
                                        const optional<Tensor>& residual, int64_t activation, bool want_preact,
                                        const optional<Tensor>& status) {
-    c10::cuda::CUDAGuard guard(x_.device());
-    TORCH_CHECK(x_.is_cuda() && x_.dim() == 2 && weight_.dim() == 2 && x_.size(1) == weight_.size(1),
-                "x must be CUDA [rows, in] and weight [out, in]");
-    check_same(x_, x_, at::kBFloat16, "x");
-    check_same(weight_, x_, at::kBFloat16, "weight");
-    TORCH_CHECK(x_.size(1) >= 8 && x_.size(1) % 8 == 0, "in must be a multiple of 8");
-    TORCH_CHECK(x_.size(0) <= INT32_MAX && x_.size(1) <= INT32_MAX && weight_.size(0) <= INT32_MAX,
-                "a size is beyond 2^31 - 1");
-    const Tensor x = aligned_rows(x_), weight = aligned_rows(weight_);
-    const int64_t R = x.size(0), N = weight.size(0);
-    Tensor b, r;
-    if (bias.has_value() && bias->defined()) {
-        check_same(*bias, x, at::kBFloat16, "bias");
-        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "bias must be [out]");
-        b = bias->contiguous();
-        if (reinterpret_cast<uintptr_t>(b.data_ptr()) & 15) b = b.clone();
-    }
-    if (residual.has_value() && residual->defined()) {
-        check_same(*residual, x, at::kBFloat16, "residual");
-        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == R && residual->size(1) == N,
-                    "residual must be [rows, out]");
-        r = plain_rows(*residual);
-    }
-    Tensor out = fresh({R, N}, at::kBFloat16, x);
-    Tensor pre = fresh({want_preact ? R : 0, round8(N)}, at::kHalf, x);
-    b2s_linear_args a;
-    memset(&a, 0, sizeof(a));
-    a.x = x.data_ptr();
-    a.x_row_stride = row_stride(x);
-    a.weight = weight.data_ptr();
-    a.weight_row_stride = row_stride(weight);
-    a.rows = (int32_t)R;
-    a.in_features = (int32_t)x.size(1);
-    a.out_features = (int32_t)N;
-    a.activation = (int32_t)activation;
-    a.bias = b.defined() ? b.data_ptr() : nullptr;
-    a.residual = r.defined() ? r.data_ptr() : nullptr;
-    a.residual_row_stride = r.defined() ? row_stride(r) : 0;
-    a.out = out.data_ptr();
-    a.out_row_stride = N;
+    c10::cuda::CUDAGuard guard(x.device());
+    LinearCall c(x, weight, bias, residual, activation, status);
+    b2s_linear_args& a = c.a;
+    Tensor pre = fresh({want_preact ? a.rows : 0, round8(a.out_features)}, at::kHalf, c.x);
     a.preact = want_preact ? pre.data_ptr() : nullptr;
-    a.preact_row_stride = round8(N);
+    a.preact_row_stride = round8(a.out_features);
     check_rc(b2s_linear_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes), "b2s_linear_workspace");
     Tensor ws;
     if (a.workspace_bytes) {
-        ws = workspace(a.workspace_bytes, x);
+        ws = workspace(a.workspace_bytes, c.x);
         a.workspace = ws.data_ptr();
     }
-    a.status = status_ptr(status, x);
     check_rc(b2s_linear(&a, at::cuda::getCurrentCUDAStream().stream()), "b2s_linear");
-    return {out, pre};
+    return {c.out, pre};
 }
 
 std::tuple<Tensor, Tensor> linear_meta(const Tensor& x, const Tensor& weight, const optional<Tensor>&,
@@ -871,6 +881,99 @@ std::tuple<Tensor, Tensor, Tensor> linear_grad_meta(const Tensor&, const Tensor&
     const int64_t K = x.size(1), N = weight.size(0);
     return {at::empty({want_x ? x.size(0) : 0, K}, x.options()), at::empty({want_weight ? N : 0, K}, x.options()),
             at::empty({want_bias ? N : 0}, x.options())};
+}
+
+int64_t blocks32(int64_t n) { return (n + 31) / 32; }
+
+// The projection with x and the pre-activation kept in microscaled 8 bits, each where asked for.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_kept_cuda(const Tensor& x, const Tensor& weight,
+                                                                    const optional<Tensor>& bias,
+                                                                    const optional<Tensor>& residual, int64_t activation,
+                                                                    bool want_x, bool want_z, const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(x.device());
+    LinearCall c(x, weight, bias, residual, activation, status);
+    b2s_linear_args& a = c.a;
+    const int64_t R = a.rows, kb = blocks32(a.in_features), nb = blocks32(a.out_features);
+    Tensor xc = fresh({want_x ? R : 0, kb * 32}, at::kByte, c.x), xs = fresh({kb, want_x ? R : 0}, at::kByte, c.x);
+    Tensor zc = fresh({want_z ? R : 0, nb * 32}, at::kByte, c.x), zs = fresh({nb, want_z ? R : 0}, at::kByte, c.x);
+    b2s_linear_kept k = {};
+    if (want_x) k.x_codes = xc.data_ptr(), k.x_scales = xs.data_ptr();
+    if (want_z) k.z_codes = zc.data_ptr(), k.z_scales = zs.data_ptr();
+    check_rc(b2s_linear_checkpoint_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes),
+             "b2s_linear_checkpoint_workspace");
+    Tensor ws;
+    if (a.workspace_bytes) {
+        ws = workspace(a.workspace_bytes, c.x);
+        a.workspace = ws.data_ptr();
+    }
+    check_rc(b2s_linear_checkpoint(&a, &k, at::cuda::getCurrentCUDAStream().stream()), "b2s_linear_checkpoint");
+    return {c.out, xc, xs, zc, zs};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_kept_meta(const Tensor& x, const Tensor& weight,
+                                                                    const optional<Tensor>&, const optional<Tensor>&, int64_t,
+                                                                    bool want_x, bool want_z, const optional<Tensor>&) {
+    const int64_t R = x.size(0), N = weight.size(0), kb = blocks32(x.size(1)), nb = blocks32(N);
+    auto o = x.options().dtype(at::kByte);
+    return {at::empty({R, N}, x.options()), at::empty({want_x ? R : 0, kb * 32}, o), at::empty({kb, want_x ? R : 0}, o),
+            at::empty({want_z ? R : 0, nb * 32}, o), at::empty({nb, want_z ? R : 0}, o)};
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_kept_grad_cuda(const Tensor& grad_out, const Tensor& weight_, const Tensor& x_codes,
+                                                         const Tensor& x_scales, const Tensor& z_codes, const Tensor& z_scales,
+                                                         int64_t activation, bool want_x, bool want_weight, bool want_bias,
+                                                         const optional<Tensor>& status) {
+    c10::cuda::CUDAGuard guard(grad_out.device());
+    check_same(grad_out, grad_out, at::kBFloat16, "grad_out");
+    check_same(weight_, grad_out, at::kBFloat16, "weight");
+    TORCH_CHECK(grad_out.dim() == 2 && weight_.dim() == 2 && grad_out.size(1) == weight_.size(0),
+                "grad_out must be [rows, out] and weight [out, in]");
+    const int64_t R = grad_out.size(0), N = weight_.size(0), K = weight_.size(1);
+    auto check_kept = [&](const Tensor& codes, const Tensor& scales, int64_t n, const char* name) {
+        check_same(codes, grad_out, at::kByte, name);
+        check_same(scales, grad_out, at::kByte, name);
+        TORCH_CHECK(codes.dim() == 2 && codes.size(0) == R && codes.size(1) == blocks32(n) * 32 && codes.is_contiguous() &&
+                        scales.dim() == 2 && scales.size(0) == blocks32(n) && scales.size(1) == R && scales.is_contiguous(),
+                    name, " must be what linear_kept gave");
+    };
+    b2s_linear_kept k = {};
+    if (want_weight) {
+        check_kept(x_codes, x_scales, K, "x");
+        k.x_codes = x_codes.data_ptr(), k.x_scales = x_scales.data_ptr();
+    }
+    if (activation != B2S_ACT_NONE) {
+        check_kept(z_codes, z_scales, N, "z");
+        k.z_codes = z_codes.data_ptr(), k.z_scales = z_scales.data_ptr();
+    }
+    const Tensor weight = aligned_rows(weight_), g = plain_rows(grad_out);
+    Tensor dx = fresh({want_x ? R : 0, K}, at::kBFloat16, g), dw = fresh({want_weight ? N : 0, K}, at::kBFloat16, g);
+    Tensor db = fresh({want_bias ? N : 0}, at::kBFloat16, g);
+    b2s_linear_grad_args a;
+    memset(&a, 0, sizeof(a));
+    a.grad_out = g.data_ptr();
+    a.grad_out_row_stride = row_stride(g);
+    a.weight = weight.data_ptr();
+    a.weight_row_stride = row_stride(weight);
+    a.rows = (int32_t)R;
+    a.in_features = (int32_t)K;
+    a.out_features = (int32_t)N;
+    a.activation = (int32_t)activation;
+    a.grad_x = want_x ? dx.data_ptr() : nullptr;
+    a.grad_weight = want_weight ? dw.data_ptr() : nullptr;
+    a.grad_bias = want_bias ? db.data_ptr() : nullptr;
+    check_rc(b2s_linear_checkpoint_grad_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes),
+             "b2s_linear_checkpoint_grad_workspace");
+    Tensor ws = workspace(a.workspace_bytes, g);
+    a.workspace = ws.data_ptr();
+    a.status = status_ptr(status, g);
+    check_rc(b2s_linear_checkpoint_grad(&a, &k, at::cuda::getCurrentCUDAStream().stream()), "b2s_linear_checkpoint_grad");
+    return {dx, dw, db};
+}
+std::tuple<Tensor, Tensor, Tensor> linear_kept_grad_meta(const Tensor& grad_out, const Tensor& weight, const Tensor&,
+                                                         const Tensor&, const Tensor&, const Tensor&, int64_t, bool want_x,
+                                                         bool want_weight, bool want_bias, const optional<Tensor>&) {
+    const int64_t N = weight.size(0), K = weight.size(1);
+    return {at::empty({want_x ? grad_out.size(0) : 0, K}, weight.options()), at::empty({want_weight ? N : 0, K}, weight.options()),
+            at::empty({want_bias ? N : 0}, weight.options())};
 }
 
 // ------------------------------------------------------------------ embeddings and microscaled matrices
@@ -1209,6 +1312,15 @@ const auto& mx_linear_grad_op() {
     return op;
 }
 
+const auto& linear_kept_op() {
+    static const auto op = op_handle<decltype(linear_kept_cuda)>("minicpmo_sampler::linear_kept");
+    return op;
+}
+const auto& linear_kept_grad_op() {
+    static const auto op = op_handle<decltype(linear_kept_grad_cuda)>("minicpmo_sampler::linear_kept_grad");
+    return op;
+}
+
 // Under stream capture: a leaf whose gradient accumulator an eager graph on another stream keeps alive would tie the
 // captured backward pass to that stream, which invalidates the capture deep in the engine.  Said here instead, for leaves
 // that are inputs themselves and for those that inputs were made from on the capturing stream (a reshape, say).  Tracing
@@ -1381,6 +1493,59 @@ std::tuple<Tensor, Tensor> linear_autograd(const Tensor& x, const Tensor& weight
     return {o[0], o[1]};
 }
 
+struct LinearKeptNode : public torch::autograd::Function<LinearKeptNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
+                                 const optional<Tensor>& residual, int64_t activation, const optional<Tensor>& status) {
+        const bool act = activation != B2S_ACT_NONE, want_w = needs_grad(weight);
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [out, xc, xs, zc, zs] = linear_kept_op().call(x, weight, bias, residual, activation, want_w, act, status);
+        ctx->save_for_backward({weight, xc, xs, zc, zs});
+        keep_status(ctx, status);
+        ctx->saved_data["activation"] = activation;
+        // the graph's edges are numbered over the tensors that were there
+        ctx->saved_data["bias"] = bias.has_value() && bias->defined();
+        ctx->saved_data["residual"] = residual.has_value() && residual->defined();
+        ctx->mark_non_differentiable({xc, xs, zc, zs});
+        ctx->set_materialize_grads(false);
+        return {out, xc, xs, zc, zs};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(6);
+        if (!g[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        const bool want_b = has_b && ctx->needs_input_grad(2);
+        if (want_x || want_w || want_b) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            auto [dx, dw, db] = linear_kept_grad_op().call(g[0], saved[0], saved[1], saved[2], saved[3], saved[4],
+                                                           ctx->saved_data["activation"].toInt(), want_x, want_w, want_b,
+                                                           kept_status(ctx));
+            if (want_x) out[0] = dx;
+            if (want_w) out[1] = dw;
+            if (want_b) out[2] = db;
+        }
+        seal(out, "linear");
+        if (has_r && ctx->needs_input_grad(has_b ? 3 : 2)) out[3] = g[0];
+        return out;
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_kept_autograd(const Tensor& x, const Tensor& weight,
+                                                                        const optional<Tensor>& bias,
+                                                                        const optional<Tensor>& residual, int64_t activation,
+                                                                        bool want_x, bool want_z, const optional<Tensor>& status) {
+    refuse_tangents("linear", x, weight, bias, residual);
+    if (!at::GradMode::is_enabled() ||
+        !(needs_grad(x) || needs_grad(weight) || needs_grad(bias) || needs_grad(residual))) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return linear_kept_op().call(x, weight, bias, residual, activation, want_x, want_z, status);
+    }
+    check_capture({x, weight, or_none(bias), or_none(residual)});
+    variable_list o = LinearKeptNode::apply(x, weight, bias, residual, activation, status);
+    return {o[0], o[1], o[2], o[3], o[4]};
+}
+
 struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& table, double scale,
                                  const optional<Tensor>& status) {
@@ -1534,6 +1699,13 @@ TORCH_LIBRARY(minicpmo_sampler, m) {
     m.def(
         "linear_grad(Tensor grad_out, Tensor x, Tensor weight, Tensor? preact, int activation, bool want_x, "
         "bool want_weight, bool want_bias, Tensor? status) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias)");
+    m.def(
+        "linear_kept(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int activation, bool want_x, bool want_z, "
+        "Tensor? status) -> (Tensor out, Tensor x_codes, Tensor x_scales, Tensor z_codes, Tensor z_scales)");
+    m.def(
+        "linear_kept_grad(Tensor grad_out, Tensor weight, Tensor x_codes, Tensor x_scales, Tensor z_codes, Tensor z_scales, "
+        "int activation, bool want_x, bool want_weight, bool want_bias, Tensor? status) -> "
+        "(Tensor grad_x, Tensor grad_weight, Tensor grad_bias)");
     m.def("embedding(Tensor tokens, Tensor table, float scale, Tensor? status) -> Tensor");
     m.def("embedding_mx(Tensor tokens, Tensor codes, Tensor scales, int width, float scale, Tensor? status) -> Tensor");
     m.def("embedding_grad(Tensor grad_out, Tensor tokens, int vocab, float scale) -> Tensor");
@@ -1566,6 +1738,8 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, CUDA, m) {
     m.impl("lmhead_logprobs_grad", &lmhead_logprobs_grad_cuda);
     m.impl("linear", &linear_cuda);
     m.impl("linear_grad", &linear_grad_cuda);
+    m.impl("linear_kept", &linear_kept_cuda);
+    m.impl("linear_kept_grad", &linear_kept_grad_cuda);
     m.impl("embedding", &embedding_cuda);
     m.impl("embedding_mx", &embedding_mx_cuda);
     m.impl("embedding_grad", &embedding_grad_cuda);
@@ -1594,6 +1768,8 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, Meta, m) {
     m.impl("lmhead_logprobs_grad", &lmhead_logprobs_grad_meta);
     m.impl("linear", &linear_meta);
     m.impl("linear_grad", &linear_grad_meta);
+    m.impl("linear_kept", &linear_kept_meta);
+    m.impl("linear_kept_grad", &linear_kept_grad_meta);
     m.impl("embedding", &embedding_meta);
     m.impl("embedding_mx", &embedding_mx_meta);
     m.impl("embedding_grad", &embedding_grad_meta);
@@ -1607,6 +1783,7 @@ TORCH_LIBRARY_IMPL(minicpmo_sampler, Autograd, m) {
     m.impl("token_logprobs", &token_logprobs_autograd);
     m.impl("lmhead_logprobs", &lmhead_logprobs_autograd);
     m.impl("linear", &linear_autograd);
+    m.impl("linear_kept", &linear_kept_autograd);
     m.impl("embedding", &embedding_autograd);
     m.impl("mx_linear", &mx_linear_autograd);
 }

@@ -24,6 +24,8 @@ def test_python_entry_points_refuse_cpu_tensors(pkg):
         pkg.mx.linear(table.bfloat16(), table)
     with pytest.raises(ValueError):
         pkg.mx.dequantize(table)
+    with pytest.raises(ValueError):
+        pkg.projection.linear(table.bfloat16(), table.bfloat16(), checkpoint="e4m3")
 
 
 def test_embedding_arguments(pkg):
@@ -114,13 +116,42 @@ def test_product_sizes(pkg):
         assert lib.b2s_mx_linear_workspace(*bad, ctypes.byref(n)) == 1
 
 
-def test_product_argument_layout_matches_c(pkg, tmp_path):
+@pytest.mark.parametrize("bad", [dict(x_codes=None), dict(x_scales=None), dict(z_codes=None), dict(z_scales=None),
+                                 dict(x_codes=0x10008), dict(z_codes=0x10008)], ids=str)
+def test_checkpoint_arguments(pkg, bad):
+    lib, nat = pkg._native.capi(), pkg._native
+    whole = dict(x_codes=FAKE[0].value, x_scales=FAKE[1].value, z_codes=FAKE[2].value, z_scales=FAKE[3].value)
+    fwd = dict(x=FAKE[4].value, x_row_stride=64, weight=FAKE[5].value, weight_row_stride=64, rows=5, in_features=64,
+               out_features=50, activation=3, out=FAKE[6].value, out_row_stride=50, workspace=FAKE[7].value, workspace_bytes=1 << 40)
+    grad = dict(grad_out=FAKE[4].value, grad_out_row_stride=50, weight=FAKE[5].value, weight_row_stride=64, rows=5,
+                in_features=64, out_features=50, activation=3, grad_x=FAKE[6].value, grad_weight=FAKE[8].value,
+                workspace=FAKE[7].value, workspace_bytes=1 << 40)
+    kept = ctypes.byref(nat.LinearKept(**{**whole, **bad}))
+    assert lib.b2s_linear_checkpoint(ctypes.byref(nat.LinearArgs(**fwd)), kept, None) == 1
+    assert lib.b2s_linear_checkpoint_grad(ctypes.byref(nat.LinearGradArgs(**grad)), kept, None) == 1
+    good = ctypes.byref(nat.LinearKept(**whole))
+    for f, g in ((dict(x=None), dict(weight=None)), (dict(rows=-1), dict(rows=-1)), (dict(workspace=None), dict(workspace=None)),
+                 (dict(preact=FAKE[9].value, preact_row_stride=56), dict(workspace_bytes=64)),
+                 (dict(activation=4), dict(activation=4)), (dict(in_features=60), dict(in_features=60))):
+        if "workspace" not in f:
+            assert lib.b2s_linear_checkpoint(ctypes.byref(nat.LinearArgs(**{**fwd, **f})), good, None) == 1, f
+        assert lib.b2s_linear_checkpoint_grad(ctypes.byref(nat.LinearGradArgs(**{**grad, **g})), good, None) == 1, g
+    assert lib.b2s_linear_checkpoint(ctypes.byref(nat.LinearArgs(**fwd)), None, None) == 1
+    assert lib.b2s_linear_checkpoint_grad(ctypes.byref(nat.LinearGradArgs(**grad)), None, None) == 1
+    assert lib.b2s_linear_checkpoint(ctypes.byref(nat.LinearArgs(**{**fwd, "rows": 0})), good, None) == 0
+    n = ctypes.c_int64()
+    assert lib.b2s_linear_checkpoint_grad_workspace(5, 64, 50, ctypes.byref(n)) == 0 and n.value >= 5 * 64 * 2
+    assert lib.b2s_linear_checkpoint_workspace(-1, 64, 50, ctypes.byref(n)) == 1
+
+
+@pytest.mark.parametrize("name,mirror", [("b2s_mx_linear_args", "MxLinearArgs"), ("b2s_linear_kept", "LinearKept")])
+def test_argument_layout_matches_c(pkg, tmp_path, name, mirror):
     header = Path(__file__).resolve().parents[1] / "include" / "b2s_sampler.h"
-    cls = pkg._native.MxLinearArgs
+    cls = getattr(pkg._native, mirror)
     src = tmp_path / "layout.c"
     src.write_text("\n".join(["#include <stdio.h>", "#include <stddef.h>", f'#include "{header}"', "int main(void) {",
-                              'printf("%zu\\n", sizeof(b2s_mx_linear_args));',
-                              *[f'printf("%zu\\n", offsetof(b2s_mx_linear_args, {f}));' for f, _ in cls._fields_], "return 0; }"]))
+                              'printf("%zu\\n", sizeof(' + name + '));',
+                              *[f'printf("%zu\\n", offsetof({name}, {f}));' for f, _ in cls._fields_], "return 0; }"]))
     exe = tmp_path / "layout"
     subprocess.run(["gcc", "-std=c11", "-x", "c", str(src), "-o", str(exe)], check=True)
     out = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
@@ -139,6 +170,11 @@ def test_meta_kernels(pkg):
     assert ops.mx_dequantize(codes, scales, 300, torch.bfloat16).shape == (300, 300)
     assert ops.embedding_mx(t, codes, scales, 300, 1.0, None).shape == (7, 300)
     x = torch.empty(5, 300, dtype=torch.bfloat16, device="meta", requires_grad=True)
+    w = torch.empty(90, 304, dtype=torch.bfloat16, device="meta", requires_grad=True)
+    h = torch.empty(5, 304, dtype=torch.bfloat16, device="meta")
+    kept = ops.linear_kept(h, w, None, None, 3, False, False, None)
+    assert [tuple(v.shape) for v in kept] == [(5, 90), (5, 320), (10, 5), (5, 96), (3, 5)]
+    assert torch.autograd.grad(kept[0], w, torch.empty_like(kept[0]))[0].shape == (90, 304)
     y, pre = ops.mx_linear(x, None, codes, scales, 300, None, None, 3, True, None)
     d, = torch.autograd.grad(y, x, torch.empty_like(y))
     assert y.shape == (5, 300) and pre.shape == (5, 304) and d.shape == (5, 300)
