@@ -8,8 +8,10 @@
 // each 128 rows, copied in the layout of the matrix's scale tiles, and the issuing warp has the tensor cores copy them from
 // shared to tensor memory (tcgen05.cp, each 512 bytes spread over 32 lanes and 4 columns, for all four lane quarters).
 // Each stage of the ring has its own columns there: when a stage is full again, the MMAs that read its scales are done.
-// 256 columns of accumulator leave no room for a second one beside the scales, so the epilogue takes an accumulator to
-// registers at once and gives it back before it does anything else.
+// Two accumulators of 256 columns leave no room for scales beside them, so they share 128 columns: the epilogue takes those to
+// registers first (64 a thread) and lets the next tile's MMAs begin, then the other 128 from where they lie.  (Taken whole,
+// 128 a thread, the registers spilled to a first-level cache that the ring leaves nothing of: 1000 x 4096 x 151936 993 us
+// against 254, of which 33 are the epilogue; an arrival per thread instead of per warp cost 60 more.)
 #include <string.h>
 
 #include <atomic>
@@ -41,11 +43,15 @@ __host__ __device__ constexpr int mxg_stages(int cg, int tn) {
 __host__ __device__ constexpr uint32_t mxg_smem(int cg, int tn) {
     return 1024 + mxg_stages(cg, tn) * mxg_stage_bytes(cg, tn) + GM_STAGING + 256;
 }
-// Tensor memory: the accumulators, then each stage's scales: for each half of 128 k 4 columns of A's and 4 per tile of B's.
-__host__ __device__ constexpr int mxg_accs(int tn) { return tn == 256 ? 1 : 2; }
+// Tensor memory: two accumulators, then each stage's scales: for each half of 128 k 4 columns of A's and 4 per tile of B's.
+// Two times 256 columns of accumulator would leave none for the scales, so those share their middle: the second starts at
+// column 128.
+__host__ __device__ constexpr int mxg_acc_step(int tn) { return tn == 256 ? 128 : tn; }
+__host__ __device__ constexpr int mxg_acc_cols(int tn) { return mxg_acc_step(tn) + tn; }
+__host__ __device__ constexpr int mxg_free(int tn) { return tn == 256 ? 1 : 2; }  // accumulators handed back apart
 __host__ __device__ constexpr int mxg_sf_cols(int tn) { return 8 + 8 * mxg_btiles(tn); }
 __host__ __device__ constexpr uint32_t mxg_tmem(int cg, int tn) {
-    return mxg_accs(tn) * tn + mxg_stages(cg, tn) * mxg_sf_cols(tn) > 256 ? 512 : 256;
+    return mxg_acc_cols(tn) + mxg_stages(cg, tn) * mxg_sf_cols(tn) > 256 ? 512 : 256;
 }
 
 // Shared-memory descriptor of 512 bytes of scales: 32 rows of 16 bytes, 8 rows at a time (128 bytes), no swizzle.
@@ -76,14 +82,19 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, ui
             : "memory");
 }
 
+__device__ __forceinline__ void fill_nan32(float* v) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
+}
+
 template <int CG, int TN>
 __global__ void __launch_bounds__(GM_THREADS, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                    const __grid_constant__ CUtensorMap asmap, const __grid_constant__ CUtensorMap bsmap,
                    const __grid_constant__ GemmArgs a) {
-    constexpr int TM = CG * GM_M, BN = TN / CG, ST = mxg_stages(CG, TN), BT = mxg_btiles(TN), ACCS = mxg_accs(TN);
+    constexpr int TM = CG * GM_M, BN = TN / CG, ST = mxg_stages(CG, TN), BT = mxg_btiles(TN), ACCS = mxg_free(TN);
     constexpr uint32_t STAGE = mxg_stage_bytes(CG, TN), SFA = GM_A_BYTES + BN * 128, SFB = SFA + 1024;
-    constexpr uint32_t SF0 = ACCS * TN, SFC = mxg_sf_cols(TN);  // the scales' first column, columns a stage
+    constexpr uint32_t SF0 = mxg_acc_cols(TN), SFC = mxg_sf_cols(TN);  // the scales' first column, columns a stage
     // E2M1 operands (bits 7-9, 10-11 = 1), both K-major, N >> 3 at bit 17, E8M0 scales (bit 23), M >> 4 at bit 24; which two
     // of a column's four scales A and B take at bits 29 and 4
     constexpr uint32_t IDESC = (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | (1u << 23) | ((uint32_t)(TM >> 4) << 24);
@@ -114,7 +125,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         }
         for (int s = 0; s < ACCS; ++s) {
             mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], 32 * GM_EPI * CG);
+            mbar_init(&tempty[s], GM_EPI * CG);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -203,7 +214,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(acc * TN);
+                const uint32_t d = tmem + (uint32_t)((g & 1) * mxg_acc_step(TN));
                 // a tile of 64 columns may be the second half of its scale tile's rows: two columns on
                 const uint32_t half = TN < 128 ? (uint32_t)(nt * TN % 128) / 32 : 0u;
                 uint32_t more = 0;
@@ -247,41 +258,57 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         int g = 0;
         bool ok = a.wait > 0;
         if (!ok) *fail = 1;
-        constexpr int COLS = TN / 2;
+        // A warp takes its part of the accumulator's shared columns first (of all, where nothing is shared), to registers, gives
+        // the accumulator back, and then its part of the others from where they lie.
+        constexpr int COLS = TN == 256 ? 64 : TN / 2;
         const int half = warp >> 2;
-        const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * COLS);
+        const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         unsigned char* st = staging + warp * 4096;
         // once a wait gave up the pieces that are left take NaN without waiting
         for (int i = 0; piece_at<CG>(a, i, &p); ++i) {
             int mt, nt;
             tile_of<TM>(a, p.tile, &mt, &nt);
-            const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32, n0 = nt * TN + half * COLS;
+            const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32;
+            const int first = (TN == 256 && !(g & 1) ? 128 : 0) + half * COLS, n0 = nt * TN;
             uint32_t rq[16];
-            if (p.slot < 0) residual_fetch(a, rq, row0, n0);  // before the accumulator is there
+            if (p.slot < 0) residual_fetch(a, rq, row0, n0 + first);  // before the accumulator is there
             const int acc = g % ACCS;
+            const uint32_t tm = tq + (uint32_t)((g & 1) * mxg_acc_step(TN));
             ok = ok && __all_sync(0xffffffffu, gm_wait<false>(&tfull[acc], (uint32_t)(g / ACCS) & 1u, a.wait) && !*fail);
             if (!ok) *fail = 1;
             tc_fence_after();
             float v[COLS];
 #pragma unroll
-            for (int q = 0; q < COLS / 32; ++q) tmem_ld32(tm + (uint32_t)(acc * TN + 32 * q), v + 32 * q);
+            for (int q = 0; q < COLS / 32; ++q) tmem_ld32(tm + (uint32_t)(first + 32 * q), v + 32 * q);
             if (ok) {
                 tc_fence_before();
-                if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
-                else mbar_arrive(&tempty[acc]);
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
+                    else mbar_arrive(&tempty[acc]);
+                }
                 ++g;
             } else {
                 fill_nan(v);
             }
 #pragma unroll 1
-            for (int q = 0; q < COLS / 32; ++q) {
-                const int n = n0 + 32 * q;
+            for (int q = 0; q < TN / 64; ++q) {
+                int c = first + 32 * q;
+                if (TN == 256 && q >= 2) {
+                    c = (c - 64) ^ 128;  // the same part of the other half
+                    if (ok) tmem_ld32(tm + (uint32_t)c, v);
+                    else fill_nan32(v);
+                }
+                const int n = n0 + c;
                 if (p.slot >= 0) {
                     store_sums<TM, TN>(a, v, row0, n, nt, p.slot, st);
-                } else {
-                    if (n >= a.N) break;
-                    residual_put(a, rq, row0, n, q + 1 < COLS / 32, st);
+                } else if (n < a.N) {
+                    residual_put(a, rq, row0, n, false, st);
                     store_block<EPI_LINEAR>(a, v, row0, n, st);
+                }
+                if (p.slot < 0 && q + 1 < TN / 64) {  // the next block's residual
+                    const int d = TN == 256 && q >= 1 ? (first + 32 * q - 32) ^ 128 : first + 32 * q + 32;
+                    residual_fetch(a, rq, row0, n0 + d);
                 }
 #pragma unroll
                 for (int j = 0; j + 32 < COLS; ++j) v[j] = v[j + 32];  // the loop's body stays short
