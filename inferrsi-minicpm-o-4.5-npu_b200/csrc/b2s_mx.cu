@@ -2,6 +2,8 @@
 // activation and residual in its epilogue.  No counterpart in the reference.
 #include <string.h>
 
+#include <type_traits>
+
 #include "../../include/b2s_sampler.h"
 #include "b2s_gemm.cuh"
 #include "b2s_launch.cuh"
@@ -19,40 +21,135 @@ namespace {
 
 constexpr int MX_NT = 256;
 constexpr int MX_SEG = 256;  // elements of a row that a warp takes at a time: 8 a lane, the 8 blocks of a scale tile
-constexpr int MX_PER = 4;    // of those in flight
-
-// 8 elements of a row from column n (k columns) as fp32; zeros past the end.  VEC: 16-byte aligned rows.  Else the warp
-// loads a 32-element block at a time, an element a lane, and turns them round in shared memory.
+// Segments of a row in flight per warp: 16 bytes a lane each for aligned bf16 rows, 32 for fp32.  Both kernels are bound by
+// HBM; with loads unpacked to fp32 as they came and 4 in flight the Thinker's head took 547 us there and 362 back.
 template <typename T>
-__device__ __forceinline__ float mx_value(const T* p);
-template <>
+__host__ __device__ constexpr int mx_per(bool vec) { return vec && sizeof(T) == 2 ? 8 : 4; }
+
 __device__ __forceinline__ float mx_value(const float* p) { return __ldg(p); }
-template <>
 __device__ __forceinline__ float mx_value(const unsigned short* p) { return bf16_bits_to_f(__ldg(p)); }
 
-__device__ __forceinline__ void mx_load8(const float* p, float (&v)[8]) {
-    const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(p)), b = ldg_stream(reinterpret_cast<const uint4*>(p) + 1);
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
-}
-__device__ __forceinline__ void mx_load8(const unsigned short* p, float (&v)[8]) {
+// 8 elements of a row as they lie: bf16 pairs or fp32 words.
+template <typename T>
+struct MxWords {
+    uint32_t w[sizeof(T) * 2];
+};
+__device__ __forceinline__ MxWords<unsigned short> mx_words(const unsigned short* p) {
     const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    return {{a.x, a.y, a.z, a.w}};
+}
+__device__ __forceinline__ MxWords<float> mx_words(const float* p) {
+    const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(p)), b = ldg_stream(reinterpret_cast<const uint4*>(p) + 1);
+    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+// Element by element, zeros from n on.
+template <typename T>
+__device__ __forceinline__ MxWords<T> mx_words(const T* p, int64_t n) {
+    MxWords<T> r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(w[j] << 16);
-        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    for (int i = 0; i < (int)sizeof(T) * 2; ++i) {
+        if constexpr (sizeof(T) == 4) r.w[i] = i < n ? __float_as_uint(mx_value(p + i)) : 0u;
+        else r.w[i] = (2 * i < n ? (uint32_t)__ldg(p + 2 * i) : 0u) | (2 * i + 1 < n ? (uint32_t)__ldg(p + 2 * i + 1) << 16 : 0u);
+    }
+    return r;
+}
+// The largest magnitude's bits as an fp32's (NaN above everything), and the values times `inv` as fp32.
+__device__ __forceinline__ uint32_t mx_most(const MxWords<float>& x) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, x.w[i] & 0x7fffffffu);
+    return m;
+}
+__device__ __forceinline__ uint32_t mx_most(const MxWords<unsigned short>& x) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, x.w[i] & 0x7fff7fffu);
+    return max(m & 0xffff0000u, m << 16);
+}
+__device__ __forceinline__ void mx_times(const MxWords<float>& x, float inv, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x.w[i]) * inv;
+}
+__device__ __forceinline__ void mx_times(const MxWords<unsigned short>& x, float inv, float (&v)[8]) {
+    const uint32_t f = mx_twice(inv);  // what the product takes below bf16's range is far below the smallest element
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = mx_scale2(x.w[i], f);
+        v[2 * i] = __uint_as_float(w << 16);
+        v[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+}
+// A segment of an unaligned row through a warp's shared memory, coalesced on the way from global memory: 8 consecutive elements
+// of `n` a lane (zeros past them).  bf16 by whole words, but for the first element of a row that starts half a word off.
+__device__ __forceinline__ MxWords<float> mx_turn_in(const float* p, int n, uint32_t* turn) {
+    const int lane = threadIdx.x & 31;
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 32 * i + lane < n ? __float_as_uint(__ldg(p + 32 * i + lane)) : 0u;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) turn[32 * i + lane] = v[i];
+    __syncwarp();
+    const uint4 a = *reinterpret_cast<const uint4*>(turn + 8 * lane), b = *reinterpret_cast<const uint4*>(turn + 8 * lane + 4);
+    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ MxWords<unsigned short> mx_turn_in(const unsigned short* p, int n, uint32_t* turn) {
+    const int lane = threadIdx.x & 31;
+    unsigned short* t = reinterpret_cast<unsigned short*>(turn);
+    const int off = (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
+    uint32_t v[4], one = 0;
+    if (off && lane == 0 && n > 0) one = __ldg(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // the pair of elements e, e + 1: a whole aligned word
+        const int e = off + 2 * (32 * i + lane);
+        v[i] = e + 1 < n ? __ldg(reinterpret_cast<const uint32_t*>(p + e)) : e < n ? (uint32_t)__ldg(p + e) : 0u;
+    }
+    __syncwarp();
+    if (off && lane == 0) t[0] = (unsigned short)one;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = off + 2 * (32 * i + lane);
+        t[e] = (unsigned short)v[i];
+        if (e + 1 < MX_SEG) t[e + 1] = (unsigned short)(v[i] >> 16);
+    }
+    __syncwarp();
+    const uint4 a = *reinterpret_cast<const uint4*>(turn + 4 * lane);
+    return {{a.x, a.y, a.z, a.w}};
+}
+// The way back: 8 consecutive elements a lane to n elements of an unaligned row.
+__device__ __forceinline__ void mx_turn_out(float* p, int n, uint32_t* turn, const float (&v)[8]) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    *reinterpret_cast<float4*>(turn + 8 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(turn + 8 * lane + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (32 * i + lane < n) p[32 * i + lane] = __uint_as_float(turn[32 * i + lane]);
+}
+__device__ __forceinline__ void mx_turn_out(unsigned short* p, int n, uint32_t* turn, const uint32_t (&w)[4]) {
+    const int lane = threadIdx.x & 31;
+    const unsigned short* t = reinterpret_cast<const unsigned short*>(turn);
+    __syncwarp();
+    *reinterpret_cast<uint4*>(turn + 4 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
+    __syncwarp();
+    const int off = (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
+    if (off && lane == 0 && n > 0) p[0] = t[0];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = off + 2 * (32 * i + lane);
+        if (e + 1 < n) *reinterpret_cast<uint32_t*>(p + e) = t[e] | (uint32_t)t[e + 1] << 16;
+        else if (e < n) p[e] = t[e];
     }
 }
 
-// grid: (a warp per row, MX_PER segments).  EIGHT: E4M3 codes, a byte each, and scales [blocks][rows]; else the 4-bit
-// layout, whose scale tiles' rows past the matrix get zeros.
+// grid: (a warp per row, mx_per segments).  VEC: 16-byte aligned rows.  EIGHT: E4M3 codes, a byte each, and scales
+// [blocks][rows]; else the 4-bit layout, whose scale tiles' rows past the matrix get zeros.
 template <typename T, bool VEC, bool EIGHT>
 __global__ void __launch_bounds__(MX_NT) mx_quantize_kernel(const T* x, int64_t row_stride, int64_t rows, int k, uint8_t* codes,
                                                             uint8_t* scales) {
-    constexpr int E = EIGHT ? 8 : 2;
-    __shared__ float turn[VEC ? 1 : MX_NT / 32][VEC ? 1 : MX_SEG];
+    constexpr int E = EIGHT ? 8 : 2, PER = mx_per<T>(VEC);
+    __shared__ __align__(16) uint32_t turn[VEC ? 1 : MX_NT / 32][VEC ? 4 : MX_SEG * sizeof(T) / 4];
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r = (int64_t)blockIdx.x * (MX_NT / 32) + warp, tiles = mx_tiles(k);
@@ -60,53 +157,31 @@ __global__ void __launch_bounds__(MX_NT) mx_quantize_kernel(const T* x, int64_t 
     const bool live = r < rows;
     if (!live && (EIGHT || r >= (rows + 127) / 128 * 128)) return;
     const T* row = x + (live ? r : 0) * row_stride;
-    for (int64_t s0 = (int64_t)blockIdx.y * MX_PER; s0 < tiles; s0 += (int64_t)gridDim.y * MX_PER) {
-        float v[MX_PER][8];
+    for (int64_t s0 = (int64_t)blockIdx.y * PER; s0 < tiles; s0 += (int64_t)gridDim.y * PER) {
+        MxWords<T> v[PER];
 #pragma unroll
-        for (int j = 0; j < MX_PER; ++j) {
+        for (int j = 0; j < PER; ++j) {
             const int64_t n = (s0 + j) * MX_SEG + 8 * lane;
-            if (live && VEC && n + 8 <= k) {
-                mx_load8(row + n, v[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t at = VEC ? n + i : (s0 + j) * MX_SEG + 32 * i + lane;
-                    v[j][i] = live && at < k ? mx_value(row + at) : 0.0f;
-                }
-            }
+            if (VEC && live && n + 8 <= k) v[j] = mx_words(row + n);
+            else if (VEC) v[j] = mx_words(row + n, live ? k - n : 0);
         }
 #pragma unroll
-        for (int j = 0; j < MX_PER; ++j) {
+        for (int j = 0; j < PER; ++j) {
             const int64_t tile = s0 + j;
             if (tile >= tiles) break;
-            if constexpr (!VEC) {
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) turn[warp][32 * i + lane] = v[j][i];
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; i += 4) {
-                    const float4 q = *reinterpret_cast<const float4*>(&turn[warp][8 * lane + i]);
-                    v[j][i] = q.x;
-                    v[j][i + 1] = q.y;
-                    v[j][i + 2] = q.z;
-                    v[j][i + 3] = q.w;
-                }
-            }
-            uint32_t most = 0;  // of the bits without the sign: NaN above everything
-#pragma unroll
-            for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[j][i]) & 0x7fffffffu);
+            if constexpr (!VEC)
+                v[j] = mx_turn_in(row + tile * MX_SEG, live ? (int)min((int64_t)MX_SEG, k - tile * MX_SEG) : 0, turn[warp]);
+            uint32_t most = mx_most(v[j]);
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const uint32_t code = mx_scale_code<E>(most);
-            const float inv = mx_inverse(code);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[j][i] *= inv;
+            float u[8];
+            mx_times(v[j], mx_inverse(code), u);
             const int block = (int)tile * 8 + (lane >> 2);
             if constexpr (EIGHT) {
                 if (block < nb) {
                     *reinterpret_cast<uint2*>(codes + (r * nb + block) * 32 + 8 * (lane & 3)) =
-                        make_uint2(mx_encode4_e4m3(v[j][0], v[j][1], v[j][2], v[j][3]), mx_encode4_e4m3(v[j][4], v[j][5], v[j][6], v[j][7]));
+                        make_uint2(mx_encode4_e4m3(u[0], u[1], u[2], u[3]), mx_encode4_e4m3(u[4], u[5], u[6], u[7]));
                     if ((lane & 3) == 0) scales[(int64_t)block * rows + r] = (uint8_t)code;
                 }
             } else {
@@ -114,26 +189,29 @@ __global__ void __launch_bounds__(MX_NT) mx_quantize_kernel(const T* x, int64_t 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xffffffffu, code, (lane & 16) + 4 * i) << (8 * i);
                 if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(r, block, tiles)) = word;
-                if (live && block < nb) *reinterpret_cast<uint32_t*>(codes + (r * nb + block) * 16 + 4 * (lane & 3)) = mx_encode8(v[j]);
+                if (live && block < nb) *reinterpret_cast<uint32_t*>(codes + (r * nb + block) * 16 + 4 * (lane & 3)) = mx_encode8(u);
             }
         }
     }
 }
 
-template <typename T, bool EIGHT>
+// The way back, to bf16 or fp32.
+template <typename T, bool VEC, bool EIGHT>
 __global__ void __launch_bounds__(MX_NT) mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k,
-                                                              T* out, int64_t out_stride, int vec) {
+                                                              T* out, int64_t out_stride) {
+    constexpr int PER = 4;
+    __shared__ __align__(16) uint32_t turn[VEC ? 1 : MX_NT / 32][VEC ? 4 : MX_SEG * sizeof(T) / 4];
     pdl_wait_then_release();
-    const int lane = threadIdx.x & 31;
-    const int64_t r = (int64_t)blockIdx.x * (MX_NT / 32) + (threadIdx.x >> 5), tiles = mx_tiles(k);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = (int64_t)blockIdx.x * (MX_NT / 32) + warp, tiles = mx_tiles(k);
     const int nb = (int)mx_blocks(k);
     if (r >= rows) return;
-    for (int64_t s0 = (int64_t)blockIdx.y * MX_PER; s0 < tiles; s0 += (int64_t)gridDim.y * MX_PER) {
-        uint32_t c[MX_PER][2], f[MX_PER];
+    for (int64_t s0 = (int64_t)blockIdx.y * PER; s0 < tiles; s0 += (int64_t)gridDim.y * PER) {
+        uint32_t c[PER][EIGHT ? 2 : 1], f[PER];
 #pragma unroll
-        for (int j = 0; j < MX_PER; ++j) {
+        for (int j = 0; j < PER; ++j) {
             const int block = (int)(s0 + j) * 8 + (lane >> 2);
-            c[j][0] = c[j][1] = f[j] = 0;
+            c[j][0] = f[j] = 0;
             if (s0 + j < tiles && block < nb) {
                 if constexpr (EIGHT) {
                     const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + (r * nb + block) * 32 + 8 * (lane & 3)));
@@ -147,63 +225,92 @@ __global__ void __launch_bounds__(MX_NT) mx_dequantize_kernel(const uint8_t* cod
             }
         }
 #pragma unroll
-        for (int j = 0; j < MX_PER; ++j) {
-            const int64_t n = (s0 + j) * MX_SEG + 8 * lane;
-            if (n >= k) break;
+        for (int j = 0; j < PER; ++j) {
+            const int64_t n0 = (s0 + j) * MX_SEG, n = n0 + 8 * lane;
+            if (n0 >= k) break;
+            const float s = mx_scale(f[j]);
             float v[8];
+            uint32_t w[4];
             if constexpr (EIGHT) {
                 float a[4], b[4];
                 mx_decode4_e4m3(c[j][0], a);
                 mx_decode4_e4m3(c[j][1], b);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[i] = a[i];
-                    v[4 + i] = b[i];
+                    v[i] = a[i] * s;
+                    v[4 + i] = b[i] * s;
                 }
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+                }
+            } else if constexpr (sizeof(T) == 2) {
+                mx_decode8(c[j][0], w);
+                const uint32_t s2 = mx_twice(s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = mx_scale2(w[i], s2);
             } else {
                 mx_decode8(c[j][0], v);
-            }
-            const float s = mx_scale(f[j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= s;
-            mx_store8(out + r * out_stride + n, (int)min((int64_t)8, k - n), vec, v);
+                for (int i = 0; i < 8; ++i) v[i] *= s;
+            }
+            T* p = out + r * out_stride;
+            const int left = (int)min((int64_t)MX_SEG, k - n0);
+            if constexpr (!VEC) {
+                if constexpr (sizeof(T) == 2) mx_turn_out(p + n0, left, turn[warp], w);
+                else mx_turn_out(p + n0, left, turn[warp], v);
+            } else if (n + 8 <= k) {
+                if constexpr (sizeof(T) == 2) {
+                    __stcs(reinterpret_cast<uint4*>(p + n), make_uint4(w[0], w[1], w[2], w[3]));
+                } else {
+                    __stcs(reinterpret_cast<float4*>(p + n), make_float4(v[0], v[1], v[2], v[3]));
+                    __stcs(reinterpret_cast<float4*>(p + n) + 1, make_float4(v[4], v[5], v[6], v[7]));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (n + i < k) {
+                        if constexpr (sizeof(T) == 2) p[n + i] = (T)(w[i >> 1] >> (16 * (i & 1)));
+                        else p[n + i] = v[i];
+                    }
+            }
         }
     }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-dim3 mx_grid(int64_t rows, int64_t k) {
-    const int64_t y = (mx_tiles(k) + MX_PER - 1) / MX_PER;
+dim3 mx_grid(int64_t rows, int64_t k, int per) {
+    const int64_t y = (mx_tiles(k) + per - 1) / per;
     return dim3((unsigned)((rows + MX_NT / 32 - 1) / (MX_NT / 32)), (unsigned)(y < 65535 ? y : 65535));
 }
 
 template <bool EIGHT>
 cudaError_t mx_quantize(const void* x, int dtype, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream) {
-    const int e = dtype == B2S_DTYPE_F32 ? 4 : 2;
-    const bool vec = aligned16(x) && row_stride * e % 16 == 0;
-    const dim3 grid = mx_grid(EIGHT ? rows : (rows + 127) / 128 * 128, k);
-    auto go = [&](auto kernel, auto* p) {
-        return launch_pdl(kernel, grid, MX_NT, 0, stream, p, row_stride, rows, k, static_cast<uint8_t*>(codes),
+    const int64_t all = EIGHT ? rows : (rows + 127) / 128 * 128;
+    auto go = [&](auto kernel, auto* p, int per) {
+        return launch_pdl(kernel, mx_grid(all, k, per), MX_NT, 0, stream, p, row_stride, rows, k, static_cast<uint8_t*>(codes),
                           static_cast<uint8_t*>(scales));
     };
-    if (dtype == B2S_DTYPE_F32) {
-        const float* p = static_cast<const float*>(x);
-        return vec ? go(mx_quantize_kernel<float, true, EIGHT>, p) : go(mx_quantize_kernel<float, false, EIGHT>, p);
-    }
-    const unsigned short* p = static_cast<const unsigned short*>(x);
-    return vec ? go(mx_quantize_kernel<unsigned short, true, EIGHT>, p) : go(mx_quantize_kernel<unsigned short, false, EIGHT>, p);
+    auto typed = [&](auto* p) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        const bool vec = aligned16(x) && row_stride * sizeof(T) % 16 == 0;
+        return vec ? go(mx_quantize_kernel<T, true, EIGHT>, p, mx_per<T>(true)) : go(mx_quantize_kernel<T, false, EIGHT>, p, mx_per<T>(false));
+    };
+    return dtype == B2S_DTYPE_F32 ? typed(static_cast<const float*>(x)) : typed(static_cast<const unsigned short*>(x));
 }
 template <bool EIGHT>
 cudaError_t mx_dequantize(const void* codes, const void* scales, int64_t rows, int k, int dtype, void* out, int64_t out_stride,
                           void* stream) {
-    const int e = dtype == B2S_DTYPE_F32 ? 4 : 2;
-    const int vec = aligned16(out) && out_stride * e % 16 == 0;
     auto go = [&](auto kernel, auto* p) {
-        return launch_pdl(kernel, mx_grid(rows, k), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
-                          static_cast<const uint8_t*>(scales), rows, k, p, out_stride, vec);
+        return launch_pdl(kernel, mx_grid(rows, k, 4), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
+                          static_cast<const uint8_t*>(scales), rows, k, p, out_stride);
     };
-    return dtype == B2S_DTYPE_F32 ? go(mx_dequantize_kernel<float, EIGHT>, static_cast<float*>(out))
-                                  : go(mx_dequantize_kernel<__nv_bfloat16, EIGHT>, static_cast<__nv_bfloat16*>(out));
+    auto typed = [&](auto* p) {
+        using T = std::remove_pointer_t<decltype(p)>;
+        const bool vec = aligned16(out) && out_stride * sizeof(T) % 16 == 0;
+        return vec ? go(mx_dequantize_kernel<T, true, EIGHT>, p) : go(mx_dequantize_kernel<T, false, EIGHT>, p);
+    };
+    return dtype == B2S_DTYPE_F32 ? typed(static_cast<float*>(out)) : typed(static_cast<unsigned short*>(out));
 }
 
 // ------------------------------------------------------------------ the product of few rows
@@ -221,26 +328,20 @@ __device__ __forceinline__ void mx_bytes(uint32_t c, int& lo, int& hi) {
 }
 // 32 elements of x from column n as bytes, and their scale's factor (a quarter of it, for the two doubled operands).
 __device__ __forceinline__ float mx_block_bytes(const unsigned short* row, int n, int k, bool vec, int (&b)[8]) {
-    float v[4][8];
+    MxWords<unsigned short> v[4];
     uint32_t most = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        if (vec && n + 8 * q + 8 <= k) {
-            mx_load8(row + n + 8 * q, v[q]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[q][i] = n + 8 * q + i < k ? mx_value(row + n + 8 * q + i) : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[q][i]) & 0x7fffffffu);
+        v[q] = vec && n + 8 * q + 8 <= k ? mx_words(row + n + 8 * q) : mx_words(row + n + 8 * q, (int64_t)k - n - 8 * q);
+        most = max(most, mx_most(v[q]));
     }
     const uint32_t code = mx_scale_code<2>(most);
     const float inv = mx_inverse(code);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[q][i] *= inv;
-        mx_bytes(mx_encode8(v[q]), b[2 * q], b[2 * q + 1]);
+        float u[8];
+        mx_times(v[q], inv, u);
+        mx_bytes(mx_encode8(u), b[2 * q], b[2 * q + 1]);
     }
     return mx_scale(code) * 0.25f;
 }

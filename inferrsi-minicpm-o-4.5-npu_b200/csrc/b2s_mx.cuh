@@ -55,17 +55,37 @@ __device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8]) {
     }
     return r;
 }
-// The values of 8 E2M1 codes: the code's three low bits as exponent and fraction of an fp16 with bias 15, whose value is
-// 2^-14 of E2M1's (the subnormal 0.5 included), made whole by an exact product.
+// The values of 8 E2M1 codes as bf16 pairs: both bytes of a magnitude looked up by its code's low three bits, four codes at a
+// time (a byte permutation takes its selectors where the codes lie), the sign put on top.
+__device__ __forceinline__ void mx_decode8(uint32_t c, uint32_t (&w)[4]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t n = j ? c >> 16 : c;
+        const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, n & 0x7777u);
+        const uint32_t hi = __byte_perm(0x3f3f3f00u, 0x40404040u, n & 0x7777u) | __byte_perm(0x00008000u, 0u, (n >> 3) & 0x1111u);
+        w[2 * j] = __byte_perm(lo, hi, 0x5140u);
+        w[2 * j + 1] = __byte_perm(lo, hi, 0x7362u);
+    }
+}
 __device__ __forceinline__ void mx_decode8(uint32_t c, float (&v)[8]) {
+    uint32_t w[4];
+    mx_decode8(c, w);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t b = c >> (8 * j);
-        const uint32_t h = (b & 7u) << 9 | (b & 8u) << 12 | (b & 0x70u) << 21 | (b & 0x80u) << 24;
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        v[2 * j] = f.x * 16384.0f;
-        v[2 * j + 1] = f.y * 16384.0f;
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
     }
+}
+// Two bf16 times a power of two (a bf16): exact, but below the normal range.
+__device__ __forceinline__ uint32_t mx_scale2(uint32_t w, uint32_t f) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(f));
+    return r;
+}
+// 2^e, or 2^-e, twice as bf16.
+__device__ __forceinline__ uint32_t mx_twice(float f) {
+    const uint32_t b = __float_as_uint(f) >> 16;
+    return b | b << 16;
 }
 // 4 values as E4M3, and back.
 __device__ __forceinline__ uint32_t mx_encode4_e4m3(float a, float b, float c, float d) {
