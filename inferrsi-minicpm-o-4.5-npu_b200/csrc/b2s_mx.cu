@@ -21,10 +21,21 @@ namespace {
 
 constexpr int MX_NT = 256;
 constexpr int MX_SEG = 256;  // elements of a row that a warp takes at a time: 8 a lane, the 8 blocks of a scale tile
-// Segments of a row in flight per warp: 16 bytes a lane each for aligned bf16 rows, 32 for fp32.  Both kernels are bound by
-// HBM; with loads unpacked to fp32 as they came and 4 in flight the Thinker's head took 547 us there and 362 back.
+// Rows that a warp takes the same segment of, in flight together: 16 bytes a lane each of bf16, 32 of fp32.  One row after
+// another costs an addition or two for each address; segments taken as they come, with a division for each warp, were bound by
+// instruction issue (32768 x 4096 bf16 86 against 60 us there, 76 against 59 back: 5.7 TB/s).
 template <typename T>
-__host__ __device__ constexpr int mx_per(bool vec) { return vec && sizeof(T) == 2 ? 8 : 4; }
+__host__ __device__ constexpr int mx_per(bool vec) { return sizeof(T) == 2 ? 8 : 4; }
+// A CTA's 8 warps: `wide` of them (1, 2, 4, 8) on segments side by side, the others on further rows.
+struct MxGrid {
+    int64_t r0, tile, step;  // first row; first segment and the next one's distance
+    __device__ __forceinline__ MxGrid(int wide, int per) {
+        const int warp = threadIdx.x >> 5;
+        r0 = ((int64_t)blockIdx.x * ((MX_NT / 32) / wide) + warp / wide) * per;
+        tile = (int64_t)blockIdx.y * wide + warp % wide;
+        step = (int64_t)gridDim.y * wide;
+    }
+};
 
 __device__ __forceinline__ float mx_value(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float mx_value(const unsigned short* p) { return bf16_bits_to_f(__ldg(p)); }
@@ -61,9 +72,12 @@ __device__ __forceinline__ uint32_t mx_most(const MxWords<float>& x) {
     return m;
 }
 __device__ __forceinline__ uint32_t mx_most(const MxWords<unsigned short>& x) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, x.w[i] & 0x7fff7fffu);
+    auto larger = [](uint32_t a, uint32_t b) {  // of the magnitudes, NaN if one is; some sign
+        uint32_t r;
+        asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    };
+    const uint32_t m = larger(larger(x.w[0], x.w[1]), larger(x.w[2], x.w[3])) & 0x7fff7fffu;
     return max(m & 0xffff0000u, m << 16);
 }
 __device__ __forceinline__ void mx_times(const MxWords<float>& x, float inv, float (&v)[8]) {
@@ -79,61 +93,68 @@ __device__ __forceinline__ void mx_times(const MxWords<unsigned short>& x, float
         v[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
     }
 }
-// A segment of an unaligned row through a warp's shared memory, coalesced on the way from global memory: 8 consecutive elements
-// of `n` a lane (zeros past them).  bf16 by whole words, but for the first element of a row that starts half a word off.
-__device__ __forceinline__ MxWords<float> mx_turn_in(const float* p, int n, uint32_t* turn) {
+// A segment of an unaligned row, coalesced: elements (fp32) or whole words (bf16, but for the first element of a row that starts
+// half a word off), zeros from n on; and through the warp's shared memory 8 consecutive elements a lane.
+template <typename T>
+struct MxRaw {
+    uint32_t w[sizeof(T) * 2], first;
+};
+__device__ __forceinline__ MxRaw<float> mx_raw(const float* p, int n) {
     const int lane = threadIdx.x & 31;
-    uint32_t v[8];
+    MxRaw<float> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 32 * i + lane < n ? __float_as_uint(__ldg(p + 32 * i + lane)) : 0u;
+    for (int i = 0; i < 8; ++i) r.w[i] = 32 * i + lane < n ? __float_as_uint(__ldg(p + 32 * i + lane)) : 0u;
+    return r;
+}
+__device__ __forceinline__ int mx_half(const unsigned short* p) { return (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 1; }
+__device__ __forceinline__ MxRaw<unsigned short> mx_raw(const unsigned short* p, int n) {
+    const int lane = threadIdx.x & 31, off = mx_half(p);
+    MxRaw<unsigned short> r;
+    r.first = off && lane == 0 && n > 0 ? (uint32_t)__ldg(p) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = off + 2 * (32 * i + lane);
+        r.w[i] = e + 1 < n ? __ldg(reinterpret_cast<const uint32_t*>(p + e)) : e < n ? (uint32_t)__ldg(p + e) : 0u;
+    }
+    return r;
+}
+__device__ __forceinline__ MxWords<float> mx_turn_in(const MxRaw<float>& r, const float*, uint32_t* turn) {
+    const int lane = threadIdx.x & 31;
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) turn[32 * i + lane] = v[i];
+    for (int i = 0; i < 8; ++i) turn[32 * i + lane] = r.w[i];
     __syncwarp();
     const uint4 a = *reinterpret_cast<const uint4*>(turn + 8 * lane), b = *reinterpret_cast<const uint4*>(turn + 8 * lane + 4);
     return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
-__device__ __forceinline__ MxWords<unsigned short> mx_turn_in(const unsigned short* p, int n, uint32_t* turn) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ MxWords<unsigned short> mx_turn_in(const MxRaw<unsigned short>& r, const unsigned short* p, uint32_t* turn) {
+    const int lane = threadIdx.x & 31, off = mx_half(p);
     unsigned short* t = reinterpret_cast<unsigned short*>(turn);
-    const int off = (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
-    uint32_t v[4], one = 0;
-    if (off && lane == 0 && n > 0) one = __ldg(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // the pair of elements e, e + 1: a whole aligned word
-        const int e = off + 2 * (32 * i + lane);
-        v[i] = e + 1 < n ? __ldg(reinterpret_cast<const uint32_t*>(p + e)) : e < n ? (uint32_t)__ldg(p + e) : 0u;
-    }
     __syncwarp();
-    if (off && lane == 0) t[0] = (unsigned short)one;
+    if (off) {
+        if (lane == 0) t[0] = (unsigned short)r.first;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int e = off + 2 * (32 * i + lane);
-        t[e] = (unsigned short)v[i];
-        if (e + 1 < MX_SEG) t[e + 1] = (unsigned short)(v[i] >> 16);
+        for (int i = 0; i < 4; ++i) {
+            const int e = 1 + 2 * (32 * i + lane);
+            t[e] = (unsigned short)r.w[i];
+            if (e + 1 < MX_SEG) t[e + 1] = (unsigned short)(r.w[i] >> 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn[32 * i + lane] = r.w[i];
     }
     __syncwarp();
     const uint4 a = *reinterpret_cast<const uint4*>(turn + 4 * lane);
     return {{a.x, a.y, a.z, a.w}};
 }
-// The way back: 8 consecutive elements a lane to n elements of an unaligned row.
-__device__ __forceinline__ void mx_turn_out(float* p, int n, uint32_t* turn, const float (&v)[8]) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    *reinterpret_cast<float4*>(turn + 8 * lane) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(turn + 8 * lane + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (32 * i + lane < n) p[32 * i + lane] = __uint_as_float(turn[32 * i + lane]);
-}
+// The way back: 8 consecutive elements a lane, as pairs, to n elements of an unaligned row.
 __device__ __forceinline__ void mx_turn_out(unsigned short* p, int n, uint32_t* turn, const uint32_t (&w)[4]) {
     const int lane = threadIdx.x & 31;
     const unsigned short* t = reinterpret_cast<const unsigned short*>(turn);
     __syncwarp();
     *reinterpret_cast<uint4*>(turn + 4 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
     __syncwarp();
-    const int off = (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
+    const int off = mx_half(p);
     if (off && lane == 0 && n > 0) p[0] = t[0];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -143,153 +164,178 @@ __device__ __forceinline__ void mx_turn_out(unsigned short* p, int n, uint32_t* 
     }
 }
 
-// grid: (a warp per row, mx_per segments).  VEC: 16-byte aligned rows.  EIGHT: E4M3 codes, a byte each, and scales
-// [blocks][rows]; else the 4-bit layout, whose scale tiles' rows past the matrix get zeros.
+// VEC: 16-byte aligned rows.  EIGHT: E4M3 codes, a byte each, and scales [blocks][rows]; else the 4-bit layout, whose scale
+// tiles' rows past the matrix get zeros.
 template <typename T, bool VEC, bool EIGHT>
 __global__ void __launch_bounds__(MX_NT) mx_quantize_kernel(const T* x, int64_t row_stride, int64_t rows, int k, uint8_t* codes,
-                                                            uint8_t* scales) {
-    constexpr int E = EIGHT ? 8 : 2, PER = mx_per<T>(VEC);
+                                                            uint8_t* scales, int wide) {
+    constexpr int E = EIGHT ? 8 : 2, PER = mx_per<T>(VEC), BYTES = EIGHT ? 8 : 4;  // of a lane's codes
     __shared__ __align__(16) uint32_t turn[VEC ? 1 : MX_NT / 32][VEC ? 4 : MX_SEG * sizeof(T) / 4];
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t r = (int64_t)blockIdx.x * (MX_NT / 32) + warp, tiles = mx_tiles(k);
-    const int nb = (int)mx_blocks(k);
-    const bool live = r < rows;
-    if (!live && (EIGHT || r >= (rows + 127) / 128 * 128)) return;
-    const T* row = x + (live ? r : 0) * row_stride;
-    for (int64_t s0 = (int64_t)blockIdx.y * PER; s0 < tiles; s0 += (int64_t)gridDim.y * PER) {
-        MxWords<T> v[PER];
+    const int64_t tiles = mx_tiles(k), nb = mx_blocks(k);
+    const MxGrid g(wide, PER);
+    if (g.r0 >= (EIGHT ? rows : (rows + 127) / 128 * 128)) return;
+    const int live = (int)max((int64_t)0, min((int64_t)PER, rows - g.r0));  // rows of the matrix
+    for (int64_t tile = g.tile; tile < tiles; tile += g.step) {
+        const int64_t n = tile * MX_SEG + 8 * lane, block = tile * 8 + (lane >> 2);
+        const T* p = x + g.r0 * row_stride + (VEC ? n : tile * MX_SEG);
+        std::conditional_t<VEC, MxWords<T>, MxRaw<T>> in[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int64_t n = (s0 + j) * MX_SEG + 8 * lane;
-            if (VEC && live && n + 8 <= k) v[j] = mx_words(row + n);
-            else if (VEC) v[j] = mx_words(row + n, live ? k - n : 0);
+            const T* q = p + j * row_stride;
+            if constexpr (!VEC) in[j] = mx_raw(q, j < live ? (int)min((int64_t)MX_SEG, k - tile * MX_SEG) : 0);
+            else if (j < live && n + 8 <= k) in[j] = mx_words(q);
+            else in[j] = mx_words(q, j < live ? k - n : 0);
         }
+        uint8_t* c = codes + g.r0 * nb * (4 * BYTES) + block * (4 * BYTES) + BYTES * (lane & 3);
+        uint8_t* s = EIGHT ? scales + block * rows + g.r0 : scales + mx_scale_at(g.r0, tile * 8 + (lane >> 4) * 4, tiles);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int64_t tile = s0 + j;
-            if (tile >= tiles) break;
-            if constexpr (!VEC)
-                v[j] = mx_turn_in(row + tile * MX_SEG, live ? (int)min((int64_t)MX_SEG, k - tile * MX_SEG) : 0, turn[warp]);
-            uint32_t most = mx_most(v[j]);
+            MxWords<T> v;
+            if constexpr (VEC) v = in[j];
+            else v = mx_turn_in(in[j], p + j * row_stride, turn[warp]);
+            uint32_t most = mx_most(v);
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const uint32_t code = mx_scale_code<E>(most);
             float u[8];
-            mx_times(v[j], mx_inverse(code), u);
-            const int block = (int)tile * 8 + (lane >> 2);
+            mx_times(v, mx_inverse(code), u);
             if constexpr (EIGHT) {
-                if (block < nb) {
-                    *reinterpret_cast<uint2*>(codes + (r * nb + block) * 32 + 8 * (lane & 3)) =
+                if (j < live && block < nb) {
+                    *reinterpret_cast<uint2*>(c) =
                         make_uint2(mx_encode4_e4m3(u[0], u[1], u[2], u[3]), mx_encode4_e4m3(u[4], u[5], u[6], u[7]));
-                    if ((lane & 3) == 0) scales[(int64_t)block * rows + r] = (uint8_t)code;
+                    if ((lane & 3) == 0) s[j] = (uint8_t)code;
                 }
             } else {
-                uint32_t word = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xffffffffu, code, (lane & 16) + 4 * i) << (8 * i);
-                if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(r, block, tiles)) = word;
-                if (live && block < nb) *reinterpret_cast<uint32_t*>(codes + (r * nb + block) * 16 + 4 * (lane & 3)) = mx_encode8(u);
+                uint32_t word = code | __shfl_down_sync(0xffffffffu, code, 4) << 8;  // four blocks' in every 16th lane
+                word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
+                if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(s + 16 * j) = word;
+                if (j < live && block < nb) *reinterpret_cast<uint32_t*>(c) = mx_encode8(u);
             }
+            c += nb * (4 * BYTES);
         }
     }
 }
 
-// The way back, to bf16 or fp32.
+// The way back, to bf16 or fp32.  A lane takes 8 elements, 16 bytes of bf16; to fp32 4 of either half of a segment, so that a
+// store's lanes write one line after another (8 at once: 16384 x 4096 67 against 58 us).
 template <typename T, bool VEC, bool EIGHT>
 __global__ void __launch_bounds__(MX_NT) mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k,
-                                                              T* out, int64_t out_stride) {
-    constexpr int PER = 4;
+                                                              T* out, int64_t out_stride, int wide) {
+    constexpr int PER = mx_per<T>(true), H = sizeof(T) == 4 ? 2 : 1, N = 8 / H;  // rows; loads a segment, elements of each
+    static_assert(!EIGHT || H == 1, "8 bits come back as bf16");
     __shared__ __align__(16) uint32_t turn[VEC ? 1 : MX_NT / 32][VEC ? 4 : MX_SEG * sizeof(T) / 4];
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t r = (int64_t)blockIdx.x * (MX_NT / 32) + warp, tiles = mx_tiles(k);
-    const int nb = (int)mx_blocks(k);
-    if (r >= rows) return;
-    for (int64_t s0 = (int64_t)blockIdx.y * PER; s0 < tiles; s0 += (int64_t)gridDim.y * PER) {
-        uint32_t c[PER][EIGHT ? 2 : 1], f[PER];
+    const int64_t tiles = mx_tiles(k), nb = mx_blocks(k);
+    const MxGrid g(wide, PER);
+    const int live = (int)max((int64_t)0, min((int64_t)PER, rows - g.r0));
+    for (int64_t tile = g.tile; tile < tiles; tile += g.step) {
+        uint32_t c[PER][EIGHT ? 2 : H], f[PER][H];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int block = (int)(s0 + j) * 8 + (lane >> 2);
-            c[j][0] = f[j] = 0;
-            if (s0 + j < tiles && block < nb) {
-                if constexpr (EIGHT) {
-                    const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + (r * nb + block) * 32 + 8 * (lane & 3)));
-                    c[j][0] = q.x;
-                    c[j][1] = q.y;
-                    f[j] = __ldg(scales + (int64_t)block * rows + r);
-                } else {
-                    c[j][0] = __ldg(reinterpret_cast<const uint32_t*>(codes + (r * nb + block) * 16 + 4 * (lane & 3)));
-                    f[j] = __ldg(scales + mx_scale_at(r, block, tiles));
+        for (int h = 0; h < H; ++h) {
+            const int n = 128 * h + N * lane;  // in the segment
+            const int64_t block = tile * 8 + n / 32;
+            const uint8_t* pc = codes + (g.r0 * nb + block) * (EIGHT ? 32 : 16) + (EIGHT ? n % 32 : n % 32 / 2);
+            const uint8_t* ps = EIGHT ? scales + block * rows + g.r0 : scales + mx_scale_at(g.r0, block, tiles);
+#pragma unroll
+            for (int j = 0; j < PER; ++j, pc += nb * (EIGHT ? 32 : 16)) {
+                c[j][h] = f[j][h] = 0;
+                if (j < live && block < nb) {
+                    if constexpr (EIGHT) {
+                        const uint2 q = __ldg(reinterpret_cast<const uint2*>(pc));
+                        c[j][0] = q.x;
+                        c[j][1] = q.y;
+                        f[j][h] = __ldg(ps + j);
+                    } else {
+                        if constexpr (H == 2) c[j][h] = __ldg(reinterpret_cast<const unsigned short*>(pc));
+                        else c[j][h] = __ldg(reinterpret_cast<const uint32_t*>(pc));
+                        f[j][h] = __ldg(ps + 16 * j);
+                    }
                 }
             }
         }
+        T* p = out + g.r0 * out_stride + tile * MX_SEG;
+        const int left = (int)min((int64_t)MX_SEG, k - tile * MX_SEG);
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int64_t n0 = (s0 + j) * MX_SEG, n = n0 + 8 * lane;
-            if (n0 >= k) break;
-            const float s = mx_scale(f[j]);
-            float v[8];
-            uint32_t w[4];
-            if constexpr (EIGHT) {
-                float a[4], b[4];
-                mx_decode4_e4m3(c[j][0], a);
-                mx_decode4_e4m3(c[j][1], b);
+        for (int j = 0; j < PER; ++j, p += out_stride) {
+            if (j >= live) break;
+            if constexpr (sizeof(T) == 2) {
+                const float s = mx_scale(f[j][0]);
+                uint32_t w[4];
+                if constexpr (EIGHT) {
+                    float a[4], b[4];
+                    mx_decode4_e4m3(c[j][0], a);
+                    mx_decode4_e4m3(c[j][1], b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[i] = a[i] * s;
-                    v[4 + i] = b[i] * s;
+                    for (int i = 0; i < 2; ++i) {
+                        w[i] = pack_bf16(a[2 * i] * s, a[2 * i + 1] * s);
+                        w[2 + i] = pack_bf16(b[2 * i] * s, b[2 * i + 1] * s);
+                    }
+                } else {
+                    mx_decode8(c[j][0], w);
+                    const uint32_t s2 = mx_twice(s);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = mx_scale2(w[i], s2);
                 }
-                if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-                }
-            } else if constexpr (sizeof(T) == 2) {
-                mx_decode8(c[j][0], w);
-                const uint32_t s2 = mx_twice(s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = mx_scale2(w[i], s2);
-            } else {
-                mx_decode8(c[j][0], v);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= s;
-            }
-            T* p = out + r * out_stride;
-            const int left = (int)min((int64_t)MX_SEG, k - n0);
-            if constexpr (!VEC) {
-                if constexpr (sizeof(T) == 2) mx_turn_out(p + n0, left, turn[warp], w);
-                else mx_turn_out(p + n0, left, turn[warp], v);
-            } else if (n + 8 <= k) {
-                if constexpr (sizeof(T) == 2) {
+                const int n = 8 * lane;
+                if constexpr (!VEC) {
+                    mx_turn_out(p, left, turn[warp], w);
+                } else if (n + 8 <= left) {
                     __stcs(reinterpret_cast<uint4*>(p + n), make_uint4(w[0], w[1], w[2], w[3]));
                 } else {
-                    __stcs(reinterpret_cast<float4*>(p + n), make_float4(v[0], v[1], v[2], v[3]));
-                    __stcs(reinterpret_cast<float4*>(p + n) + 1, make_float4(v[4], v[5], v[6], v[7]));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (n + i < left) p[n + i] = (T)(w[i >> 1] >> (16 * (i & 1)));
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (n + i < k) {
-                        if constexpr (sizeof(T) == 2) p[n + i] = (T)(w[i >> 1] >> (16 * (i & 1)));
-                        else p[n + i] = v[i];
+                for (int h = 0; h < H; ++h) {
+                    const float s = mx_scale(f[j][h]);
+                    uint32_t w[2];
+                    mx_decode4(c[j][h], w);
+                    const float4 v = make_float4(__uint_as_float(w[0] << 16) * s, __uint_as_float(w[0] & 0xffff0000u) * s,
+                                                 __uint_as_float(w[1] << 16) * s, __uint_as_float(w[1] & 0xffff0000u) * s);
+                    const int n = 128 * h + 4 * lane;
+                    if (VEC && n + 4 <= left) {
+                        __stcs(reinterpret_cast<float4*>(p + n), v);
+                    } else if constexpr (VEC) {
+                        if (n < left) p[n] = v.x;
+                        if (n + 1 < left) p[n + 1] = v.y;
+                        if (n + 2 < left) p[n + 2] = v.z;
+                    } else {
+                        *reinterpret_cast<float4*>(turn[warp] + n) = v;
                     }
+                }
+                if constexpr (!VEC) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (32 * i + lane < left) p[32 * i + lane] = __uint_as_float(turn[warp][32 * i + lane]);
+                    __syncwarp();
+                }
             }
         }
     }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-dim3 mx_grid(int64_t rows, int64_t k, int per) {
-    const int64_t y = (mx_tiles(k) + per - 1) / per;
-    return dim3((unsigned)((rows + MX_NT / 32 - 1) / (MX_NT / 32)), (unsigned)(y < 65535 ? y : 65535));
+int mx_wide(int64_t k) {
+    const int64_t t = mx_tiles(k);
+    return t > 4 ? 8 : t > 2 ? 4 : t > 1 ? 2 : 1;
 }
-
+dim3 mx_grid(int64_t rows, int64_t k, int per) {
+    const int wide = mx_wide(k);
+    const int64_t each = (int64_t)per * (MX_NT / 32 / wide), y = (mx_tiles(k) + wide - 1) / wide;
+    return dim3((unsigned)((rows + each - 1) / each), (unsigned)(y < 65535 ? y : 65535));
+}
 template <bool EIGHT>
 cudaError_t mx_quantize(const void* x, int dtype, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream) {
     const int64_t all = EIGHT ? rows : (rows + 127) / 128 * 128;
     auto go = [&](auto kernel, auto* p, int per) {
         return launch_pdl(kernel, mx_grid(all, k, per), MX_NT, 0, stream, p, row_stride, rows, k, static_cast<uint8_t*>(codes),
-                          static_cast<uint8_t*>(scales));
+                          static_cast<uint8_t*>(scales), mx_wide(k));
     };
     auto typed = [&](auto* p) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
@@ -302,15 +348,18 @@ template <bool EIGHT>
 cudaError_t mx_dequantize(const void* codes, const void* scales, int64_t rows, int k, int dtype, void* out, int64_t out_stride,
                           void* stream) {
     auto go = [&](auto kernel, auto* p) {
-        return launch_pdl(kernel, mx_grid(rows, k, 4), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
-                          static_cast<const uint8_t*>(scales), rows, k, p, out_stride);
+        using T = std::remove_pointer_t<decltype(p)>;
+        return launch_pdl(kernel, mx_grid(rows, k, mx_per<T>(true)), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
+                          static_cast<const uint8_t*>(scales), rows, k, p, out_stride, mx_wide(k));
     };
     auto typed = [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
         const bool vec = aligned16(out) && out_stride * sizeof(T) % 16 == 0;
         return vec ? go(mx_dequantize_kernel<T, true, EIGHT>, p) : go(mx_dequantize_kernel<T, false, EIGHT>, p);
     };
-    return dtype == B2S_DTYPE_F32 ? typed(static_cast<float*>(out)) : typed(static_cast<unsigned short*>(out));
+    if constexpr (!EIGHT)
+        if (dtype == B2S_DTYPE_F32) return typed(static_cast<float*>(out));
+    return typed(static_cast<unsigned short*>(out));
 }
 
 // ------------------------------------------------------------------ the product of few rows

@@ -55,17 +55,17 @@ __device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8]) {
     }
     return r;
 }
-// The values of 8 E2M1 codes as bf16 pairs: both bytes of a magnitude looked up by its code's low three bits, four codes at a
+// The values of E2M1 codes as bf16 pairs: both bytes of a magnitude looked up by its code's low three bits, four codes at a
 // time (a byte permutation takes its selectors where the codes lie), the sign put on top.
+__device__ __forceinline__ void mx_decode4(uint32_t n, uint32_t* w) {
+    const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, n & 0x7777u);
+    const uint32_t hi = __byte_perm(0x3f3f3f00u, 0x40404040u, n & 0x7777u) | __byte_perm(0x00008000u, 0u, (n >> 3) & 0x1111u);
+    w[0] = __byte_perm(lo, hi, 0x5140u);
+    w[1] = __byte_perm(lo, hi, 0x7362u);
+}
 __device__ __forceinline__ void mx_decode8(uint32_t c, uint32_t (&w)[4]) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint32_t n = j ? c >> 16 : c;
-        const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, n & 0x7777u);
-        const uint32_t hi = __byte_perm(0x3f3f3f00u, 0x40404040u, n & 0x7777u) | __byte_perm(0x00008000u, 0u, (n >> 3) & 0x1111u);
-        w[2 * j] = __byte_perm(lo, hi, 0x5140u);
-        w[2 * j + 1] = __byte_perm(lo, hi, 0x7362u);
-    }
+    mx_decode4(c, w);
+    mx_decode4(c >> 16, w + 2);
 }
 __device__ __forceinline__ void mx_decode8(uint32_t c, float (&v)[8]) {
     uint32_t w[4];
