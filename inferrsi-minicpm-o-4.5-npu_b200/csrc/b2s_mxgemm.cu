@@ -31,6 +31,10 @@ int tensor_map_words(CUtensorMap* map, const void* base, int64_t inner, int64_t 
 namespace {
 
 constexpr int MXG_KB = 256;  // k per stage: one 128-byte row of the swizzle
+constexpr int MXG_EPI = 16;  // epilogue warps: warp w has tensor-memory quarter w % 4 and part w / 4 of the columns
+constexpr int MXG_THREADS = 32 * MXG_EPI + 64;
+constexpr uint32_t MXG_STAGING = MXG_EPI * 2048;  // per epilogue warp: 32 rows of 32 bf16, or of 16 fp32
+__host__ __device__ constexpr int mxg_parts(int tn) { return tn < 128 ? tn / 32 : 4; }  // of 32 columns, and again 32 of 256
 // 128-row scale tiles of B that a tile of TN columns touches
 __host__ __device__ constexpr int mxg_btiles(int tn) { return tn > 128 ? tn / 128 : 1; }
 // A stage of one CTA: 128 rows of A, its share of B, A's scales (1 KB) and all of the tile's B's.
@@ -41,7 +45,7 @@ __host__ __device__ constexpr int mxg_stages(int cg, int tn) {
     return (int)(184u * 1024u / mxg_stage_bytes(cg, tn)) > 7 ? 7 : (int)(184u * 1024u / mxg_stage_bytes(cg, tn));
 }
 __host__ __device__ constexpr uint32_t mxg_smem(int cg, int tn) {
-    return 1024 + mxg_stages(cg, tn) * mxg_stage_bytes(cg, tn) + GM_STAGING + 256;
+    return 1024 + mxg_stages(cg, tn) * mxg_stage_bytes(cg, tn) + MXG_STAGING + 256;
 }
 // Tensor memory: two accumulators, then each stage's scales: for each half of 128 k 4 columns of A's and 4 per tile of B's.
 // Two times 256 columns of accumulator would leave none for the scales, so those share their middle: the second starts at
@@ -82,13 +86,206 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, ui
             : "memory");
 }
 
-__device__ __forceinline__ void fill_nan32(float* v) {
+// An arrival on the first CTA's mbarrier that orders nothing but this CTA's: what it tells of, tensor memory read, is ordered by
+// the tcgen05 fences.  (With the cluster's scope it waits for the warp's stores of the tile before: 1100 clocks a tile.)
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// ------------------------------------------------------------------ the epilogue's blocks of 32 rows x 32 columns
+// b2s_gemm.cuh's, but for twice as many warps: 64-byte rows of staging, two blocks' worth of which a 5th stage of the ring
+// takes, the bias from broadcast loads and packed arithmetic.
+
+// 16-byte chunk j of row r: conflict-free for a lane per row, and for 4 lanes a row.
+__device__ __forceinline__ uint4* row_at(unsigned char* st, int r, int j) {
+    return reinterpret_cast<uint4*>(st + r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+}
+// Pairs of 16-bit values, 32 of this lane's row, to global memory: rows `stride` elements apart.
+__device__ __forceinline__ void put_rows(unsigned char* st, const uint32_t (&w)[16], unsigned short* out, int64_t stride, int rows,
+                                         int cols, bool vec) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
+    for (int j = 0; j < 4; ++j) *row_at(st, lane, j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    __syncwarp();
+    if (vec) {
+        const int r = lane >> 2, c = lane & 3;
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *row_at(st, 8 * i + r, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (8 * i + r < rows) *reinterpret_cast<uint4*>(out + (8 * i + r) * stride + 8 * c) = v[i];
+    } else if (lane < cols) {
+        out += lane;
+#pragma unroll 1
+        for (int r = 0; r < 32; r += 8) {
+            unsigned short v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = reinterpret_cast<const unsigned short*>(row_at(st, r + k, lane >> 3))[lane & 7];
+#pragma unroll
+            for (int k = 0; k < 8; ++k, out += stride)
+                if (r + k < rows) *out = v[k];
+        }
+    }
+    __syncwarp();
+}
+// A block of the residual into registers, in flight until it is wanted, and its row for this lane.
+__device__ __forceinline__ void fetch_rows(const GemmArgs& a, uint32_t (&q)[16], int row0, int n) {
+    if (!a.residual || n >= a.N) return;
+    const int lane = threadIdx.x & 31, rows = a.M - row0, left = a.N - n;
+    const unsigned short* p = static_cast<const unsigned short*>(a.residual) + (int64_t)row0 * a.res_stride + n;
+    if (vec_block(a, n, a.res_vec)) {
+        const int r = lane >> 2, c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (8 * i + r < rows) u = __ldg(reinterpret_cast<const uint4*>(p + (8 * i + r) * a.res_stride + 8 * c));
+            q[4 * i] = u.x;
+            q[4 * i + 1] = u.y;
+            q[4 * i + 2] = u.z;
+            q[4 * i + 3] = u.w;
+        }
+    } else {
+        const int w = 2 * (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = 2 * i + (lane >> 4);
+            const unsigned short* g = p + r * a.res_stride + w;
+            const uint32_t lo = r < rows && w < left ? __ldg(g) : 0, hi = r < rows && w + 1 < left ? __ldg(g + 1) : 0;
+            q[i] = lo | hi << 16;
+        }
+    }
+}
+__device__ __forceinline__ void turn_rows(unsigned char* st, uint32_t (&q)[16], bool vec) {
+    const int lane = threadIdx.x & 31;
+    if (vec) {
+        const int r = lane >> 2, c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *row_at(st, 8 * i + r, c) = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+    } else {
+        const int w = lane & 15;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) reinterpret_cast<uint32_t*>(row_at(st, 2 * i + (lane >> 4), w >> 2))[w & 3] = q[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint4 u = *row_at(st, lane, j);
+        q[4 * j] = u.x;
+        q[4 * j + 1] = u.y;
+        q[4 * j + 2] = u.z;
+        q[4 * j + 3] = u.w;
+    }
+    __syncwarp();
+}
+
+// The activations of pairs, in packed arithmetic: the operations of act_apply, one for one.
+template <int ACT>
+__device__ __forceinline__ float2 act_pair(float2 z) {
+    auto both = [](float x) { return make_float2(x, x); };
+    const float2 m = make_float2(fabsf(z.x), fabsf(z.y));
+    if (ACT == ACT_RELU) return make_float2(fmax_nan(z.x, 0.0f), fmax_nan(z.y, 0.0f));
+    if (ACT == ACT_GELU) {
+        const float2 d = __ffma2_rn(both(0.363f), m, both(1.0f));
+        const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+        const float2 x = __fmul2_rn(__fmul2_rn(both(-0.72134752044448170f), m), m);
+        float2 p = both(0.096218183507f);
+        p = __ffma2_rn(p, t, both(-0.358431707466f));
+        p = __ffma2_rn(p, t, both(0.346512311336f));
+        p = __ffma2_rn(p, t, both(0.061501895887f));
+        p = __ffma2_rn(p, t, both(0.278014403086f));
+        p = __ffma2_rn(p, t, both(0.286393762026f));
+        p = __ffma2_rn(p, t, both(0.289791861116f));
+        const float2 q = __fmul2_rn(both(0.5f), __fmul2_rn(__fmul2_rn(p, t), make_float2(ex2(x.x), ex2(x.y))));
+        const float2 o = __fadd2_rn(both(1.0f), make_float2(-q.x, -q.y));
+        return __fmul2_rn(z, make_float2(z.x > 0.0f ? o.x : q.x, z.y > 0.0f ? o.y : q.y));
+    }
+    if (ACT == ACT_SILU) {
+        const float2 x = __fmul2_rn(both(-0.72134752044448170f), m), h = make_float2(ex2(x.x), ex2(x.y));
+        const float2 w = __fmul2_rn(__fmul2_rn(z, h), h), d = __ffma2_rn(h, h, both(1.0f));
+        return make_float2(__fdividef(z.x < 0.0f ? w.x : z.x, d.x), __fdividef(z.y < 0.0f ? w.y : z.y, d.y));
+    }
+    return z;
+}
+template <int ACT>
+__device__ __forceinline__ void act_row(float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const float2 y = act_pair<ACT>(make_float2(v[j], v[j + 1]));
+        v[j] = y.x;
+        v[j + 1] = y.y;
+    }
+}
+
+// This lane's row of 32 accumulated columns from n through the epilogue and to the output; rq: the residual's block.
+__device__ __forceinline__ void finish_block(const GemmArgs& a, float (&v)[32], uint32_t (&rq)[16], int row0, int n, unsigned char* st) {
+    const int lane = threadIdx.x & 31, rows = a.M - row0, cols = a.N - n;
+    const unsigned short* bias = static_cast<const unsigned short*>(a.bias);
+    if (bias) {
+        if (cols >= 32 && (reinterpret_cast<uintptr_t>(bias) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(bias + n) + j);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[8 * j + 2 * k] += __uint_as_float(w[k] << 16);
+                    v[8 * j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+                }
+            }
+        } else {
+            const float b = lane < cols ? bf16_bits_to_f(__ldg(bias + n + lane)) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
+        }
+    }
+    uint32_t w[16];
+    if (a.preact) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = (uint32_t)preact_bits(v[2 * j]) | (uint32_t)preact_bits(v[2 * j + 1]) << 16;
+        put_rows(st, w, static_cast<unsigned short*>(a.preact) + (int64_t)row0 * a.pre_stride + n, a.pre_stride, rows, cols,
+                 vec_block(a, n, 1));
+    }
+    if (a.act == ACT_RELU) act_row<ACT_RELU>(v);
+    else if (a.act == ACT_GELU) act_row<ACT_GELU>(v);
+    else if (a.act == ACT_SILU) act_row<ACT_SILU>(v);
+    if (a.residual) {
+        turn_rows(st, rq, vec_block(a, n, a.res_vec));
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            v[2 * j] += __uint_as_float(rq[j] << 16);
+            v[2 * j + 1] += __uint_as_float(rq[j] & 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);  // the output's one rounding
+    put_rows(st, w, static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride + n, a.out_stride, rows, cols,
+             vec_block(a, n, a.out_vec));
+}
+// A chunk of a split tile: 32 columns of its fp32 sums as they are, 16 at a time.
+template <int TM, int TN>
+__device__ __forceinline__ void keep_sums(const GemmArgs& a, const float (&v)[32], int row0, int n, int nt, int slot, unsigned char* st) {
+    const int lane = threadIdx.x & 31, rows = a.M - row0, r = lane >> 2, c = lane & 3;
+    float* dst = a.partial + ((int64_t)slot * min(a.M, TM) + row0 % TM) * TN + n - nt * TN + 4 * c;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16, dst += 16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(row_at(st, lane, j)) = make_float4(v[h + 4 * j], v[h + 4 * j + 1], v[h + 4 * j + 2], v[h + 4 * j + 3]);
+        __syncwarp();
+        uint4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = *row_at(st, 8 * i + r, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (8 * i + r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)(8 * i + r) * TN) = u[i];
+        __syncwarp();
+    }
 }
 
 template <int CG, int TN>
-__global__ void __launch_bounds__(GM_THREADS, 1)
+__global__ void __launch_bounds__(MXG_THREADS, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                    const __grid_constant__ CUtensorMap asmap, const __grid_constant__ CUtensorMap bsmap,
                    const __grid_constant__ GemmArgs a) {
@@ -104,7 +301,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
     const uint32_t base_u = smem_u32(smem_raw);
     unsigned char* sm = smem_raw + (((base_u + 1023u) & ~1023u) - base_u);
     unsigned char* staging = sm + ST * STAGE;
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + GM_STAGING);  // the first CTA's serves both
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + MXG_STAGING);  // the first CTA's serves both
     uint64_t* empty = full + ST;
     uint64_t* tfull = empty + ST;      // [ACCS] an accumulator is complete
     uint64_t* tempty = tfull + ACCS;   // [ACCS] an accumulator has been read (the first CTA's, by both)
@@ -125,7 +322,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         }
         for (int s = 0; s < ACCS; ++s) {
             mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], GM_EPI * CG);
+            mbar_init(&tempty[s], 4 * mxg_parts(TN) * CG);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -133,7 +330,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         *issued = 0;
         *consumed = 0;
     }
-    if (warp == GM_EPI + 1) {
+    if (warp == MXG_EPI + 1) {
         if constexpr (CG == 2) tmem_alloc_pair(tslot, mxg_tmem(CG, TN));
         else tmem_alloc(tslot, mxg_tmem(CG, TN));
     }
@@ -147,7 +344,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
     const uint32_t tmem = *tslot;
     pdl_wait_then_release();
 
-    if (warp == GM_EPI) {
+    if (warp == MXG_EPI) {
         int s = 0, it = 0;
         uint32_t ph = 1;  // parity of `empty`'s last phase: the first round finds every stage free
         bool ok = a.wait > 0;
@@ -191,7 +388,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
                     *fail = 1;
                     break;
                 }
-    } else if (warp == GM_EPI + 1) {
+    } else if (warp == MXG_EPI + 1) {
         if (rank == 0) {  // MMAs
             int s = 0, it = 0;
             uint32_t ph = 0;
@@ -253,72 +450,57 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
             }
             if (lane == 0) *consumed = it;
         }
-    } else {
+    } else if (warp < 4 * mxg_parts(TN)) {
         Piece p;
         int g = 0;
         bool ok = a.wait > 0;
         if (!ok) *fail = 1;
         // A warp takes its part of the accumulator's shared columns first (of all, where nothing is shared), to registers, gives
         // the accumulator back, and then its part of the others from where they lie.
-        constexpr int COLS = TN == 256 ? 64 : TN / 2;
-        const int half = warp >> 2;
         const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        unsigned char* st = staging + warp * 4096;
+        unsigned char* st = staging + warp * 2048;
         // once a wait gave up the pieces that are left take NaN without waiting
         for (int i = 0; piece_at<CG>(a, i, &p); ++i) {
             int mt, nt;
             tile_of<TM>(a, p.tile, &mt, &nt);
-            const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32;
-            const int first = (TN == 256 && !(g & 1) ? 128 : 0) + half * COLS, n0 = nt * TN;
+            const int row0 = mt * TM + (int)rank * GM_M + (warp & 3) * 32, n0 = nt * TN;
+            int c = (TN == 256 && !(g & 1) ? 128 : 0) + (warp >> 2) * 32;
             uint32_t rq[16];
-            if (p.slot < 0) residual_fetch(a, rq, row0, n0 + first);  // before the accumulator is there
+            if (p.slot < 0) fetch_rows(a, rq, row0, n0 + c);  // before the accumulator is there
             const int acc = g % ACCS;
             const uint32_t tm = tq + (uint32_t)((g & 1) * mxg_acc_step(TN));
             ok = ok && __all_sync(0xffffffffu, gm_wait<false>(&tfull[acc], (uint32_t)(g / ACCS) & 1u, a.wait) && !*fail);
             if (!ok) *fail = 1;
             tc_fence_after();
-            float v[COLS];
-#pragma unroll
-            for (int q = 0; q < COLS / 32; ++q) tmem_ld32(tm + (uint32_t)(first + 32 * q), v + 32 * q);
-            if (ok) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CG == 2) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
-                    else mbar_arrive(&tempty[acc]);
-                }
-                ++g;
-            } else {
-                fill_nan(v);
-            }
 #pragma unroll 1
-            for (int q = 0; q < TN / 64; ++q) {
-                int c = first + 32 * q;
-                if (TN == 256 && q >= 2) {
-                    c = (c - 64) ^ 128;  // the same part of the other half
-                    if (ok) tmem_ld32(tm + (uint32_t)c, v);
-                    else fill_nan32(v);
+            for (int q = 0; q < (TN == 256 ? 2 : 1); ++q) {
+                float v[32];
+                if (ok) tmem_ld32(tm + (uint32_t)c, v);
+                else fill_nan(v);
+                if (q == 0 && ok) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (CG == 2) arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
+                        else mbar_arrive(&tempty[acc]);
+                    }
+                    ++g;
                 }
                 const int n = n0 + c;
+                c ^= 128;
                 if (p.slot >= 0) {
-                    store_sums<TM, TN>(a, v, row0, n, nt, p.slot, st);
-                } else if (n < a.N) {
-                    residual_put(a, rq, row0, n, false, st);
-                    store_block<EPI_LINEAR>(a, v, row0, n, st);
+                    keep_sums<TM, TN>(a, v, row0, n, nt, p.slot, st);
+                } else {
+                    if (n < a.N) finish_block(a, v, rq, row0, n, st);
+                    if (TN == 256 && q == 0) fetch_rows(a, rq, row0, n0 + c);
                 }
-                if (p.slot < 0 && q + 1 < TN / 64) {  // the next block's residual
-                    const int d = TN == 256 && q >= 1 ? (first + 32 * q - 32) ^ 128 : first + 32 * q + 32;
-                    residual_fetch(a, rq, row0, n0 + d);
-                }
-#pragma unroll
-                for (int j = 0; j + 32 < COLS; ++j) v[j] = v[j + 32];  // the loop's body stays short
             }
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (*fail && warp == GM_EPI + 1 && rank == 0) {  // every MMA issued has completed
+    if (*fail && warp == MXG_EPI + 1 && rank == 0) {  // every MMA issued has completed
         if (elect_one()) {
             if constexpr (CG == 2) umma_commit_pair(drain);
             else umma_commit(drain);
@@ -344,7 +526,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         cluster_arrive_release();
         cluster_wait();
     }
-    if (warp == GM_EPI + 1) {
+    if (warp == MXG_EPI + 1) {
         tc_fence_after();
         if constexpr (CG == 2) tmem_dealloc_pair(tmem, mxg_tmem(CG, TN));
         else tmem_dealloc(tmem, mxg_tmem(CG, TN));
@@ -379,7 +561,7 @@ int mx_gemm_tn(const MxOperand& A, const MxOperand& B, int64_t K, GemmArgs a, co
         if (e != cudaSuccess) return cuda_fail(e);
         if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
-    e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, GM_THREADS, mxg_smem(CG, TN), stream, amap, bmap, asmap, bsmap, a);
+    e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, MXG_THREADS, mxg_smem(CG, TN), stream, amap, bmap, asmap, bsmap, a);
     if (e == cudaSuccess && p.split > 1) {
         const int held = a.M < TM ? a.M : TM;
         e = launch_pdl(gemm_join_kernel<TM, TN, EPI_LINEAR>,
