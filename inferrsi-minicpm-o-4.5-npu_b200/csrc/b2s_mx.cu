@@ -628,6 +628,8 @@ int b2s_mx_linear(const b2s_mx_linear_args* l, void* stream) {
     a.preact = l->preact;
     a.pre_stride = l->preact_row_stride;
     a.partial = reinterpret_cast<float*>(ws + w.partial);
+    // The kernel in front of the product is the quantisation, which waits for everything before it: the weight is there.
+    a.early = l->x != nullptr;
     return mx_gemm(x, {l->weight_codes, l->weight_scales}, l->in_features, a, stream);
 }
 

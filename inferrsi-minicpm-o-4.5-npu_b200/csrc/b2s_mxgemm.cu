@@ -342,18 +342,41 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
     }
     tc_fence_after();
     const uint32_t tmem = *tslot;
-    pdl_wait_then_release();
+    if (warp != MXG_EPI) pdl_wait_then_release();
 
     if (warp == MXG_EPI) {
         int s = 0, it = 0;
         uint32_t ph = 1;  // parity of `empty`'s last phase: the first round finds every stage free
         bool ok = a.wait > 0;
         const uint32_t bar0 = CG == 2 ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
+        const uint32_t bytes = CG * (STAGE - (uint32_t)(GM_M - a.a_rows) * 128u);
+        auto load = [&](int stage, uint32_t to, const CUtensorMap* map, int x, int y) {
+            unsigned char* dst = sm + stage * STAGE + to;
+            if constexpr (CG == 2) tma_load_2d_pair(dst, map, x, y, bar0 + 8u * stage);
+            else tma_load_2d(dst, map, x, y, &full[stage]);
+        };
+        // parts outside the tensors are filled with zeros and count as bytes
+        auto load_b = [&](int stage, int nt, int kb) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+            load(stage, GM_A_BYTES, &bmap, kb * (MXG_KB / 4), nt * TN + (int)rank * BN);  // in units of 2 bytes
+            load(stage, SFB, &bsmap, kb * 256, nt * TN / 128);                            // in words
+        };
         Piece p;
+        int early = 0;  // stages whose B is on its way before the wait for the kernel that makes A
+        if (ok && a.early) {
+            for (int i = 0; early < ST && piece_at<CG>(a, i, &p); ++i) {
+                int mt, nt;
+                tile_of<TM>(a, p.tile, &mt, &nt);
+                for (int kb = p.kb0; kb < p.kb1 && early < ST; ++kb, ++early)
+                    if (elect_one()) load_b(early, nt, kb);
+            }
+            __syncwarp();
+        }
+        pdl_wait_then_release();
         for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
             int mt, nt;
             tile_of<TM>(a, p.tile, &mt, &nt);
-            const int m0 = mt * TM + (int)rank * GM_M, n0 = nt * TN + (int)rank * BN;
+            const int m0 = mt * TM + (int)rank * GM_M;
             for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
                 if (!__all_sync(0xffffffffu, gm_wait<false>(&empty[s], ph, a.wait))) {
                     *fail = 1;
@@ -361,17 +384,9 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
                     break;
                 }
                 if (elect_one()) {
-                    unsigned char* st = sm + s * STAGE;
-                    // parts outside the tensors are filled with zeros and count as bytes
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * STAGE);
-                    auto load = [&](unsigned char* dst, const CUtensorMap* map, int x, int y) {
-                        if constexpr (CG == 2) tma_load_2d_pair(dst, map, x, y, bar0 + 8u * s);
-                        else tma_load_2d(dst, map, x, y, &full[s]);
-                    };
-                    load(st, &amap, kb * (MXG_KB / 4), m0);  // in units of 2 bytes
-                    load(st + GM_A_BYTES, &bmap, kb * (MXG_KB / 4), n0);
-                    load(st + SFA, &asmap, kb * 256, m0 / 128);  // in words
-                    load(st + SFB, &bsmap, kb * 256, nt * TN / 128);
+                    if (it >= early) load_b(s, nt, kb);
+                    load(s, 0, &amap, kb * (MXG_KB / 4), m0);
+                    load(s, SFA, &asmap, kb * 256, m0 / 128);
                 }
                 __syncwarp();
                 if (++s == ST) {
@@ -539,7 +554,9 @@ int mx_gemm_tn(const MxOperand& A, const MxOperand& B, int64_t K, GemmArgs a, co
     a.wait = wait_limit();
     CUtensorMap amap, bmap, asmap, bsmap;
     const int64_t row = mx_row_bytes(K) / 2, tiles = mx_tiles(K);  // a row's codes in units of 2 bytes
-    int rc = tensor_map_2d(&amap, A.codes, row, a.M, row, MXG_KB / 4, GM_M);
+    // rows past the end cost a load as much as others: a tile of 16 rows that loads 128 takes 16 x 4096 x 151936 from 69 to 78 us
+    a.a_rows = CG == 1 && a.M < GM_M ? (a.M + 7) / 8 * 8 : GM_M;
+    int rc = tensor_map_2d(&amap, A.codes, row, a.M, row, MXG_KB / 4, a.a_rows);
     if (rc == B2S_OK) rc = tensor_map_2d(&bmap, B.codes, row, a.N, row, MXG_KB / 4, TN / CG);
     if (rc == B2S_OK) rc = tensor_map_words(&asmap, A.scales, tiles * 256, (a.M + 127) / 128, 256, 1);
     if (rc == B2S_OK) rc = tensor_map_words(&bsmap, B.scales, tiles * 256, (a.N + 127) / 128, 256, mxg_btiles(TN));
