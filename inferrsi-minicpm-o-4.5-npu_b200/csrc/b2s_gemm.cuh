@@ -78,9 +78,7 @@ struct GemmArgs {
     // EPI_KEPT
     uint8_t* z8;        // the pre-activation in microscaled 8 bits: [M][N rounded up to 32]
     uint8_t* z8_scale;  // [blocks of 32 columns][M]
-    // the microscaled product: rows of A a tile loads (all 128, or M rounded up to 8 where that is less), and whether its B may
-    // be read before the kernel in front has completed
-    int a_rows, early;
+    int early;  // the microscaled product: its B may be read before the kernel in front has completed
     // EPI_LSE: per row and half of a column tile (m, S, U), the token's value; EPI_DZ: the gradient's inputs
     float c, inv_t;
     const int64_t* tokens;

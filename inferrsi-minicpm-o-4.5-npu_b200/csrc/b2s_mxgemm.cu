@@ -286,7 +286,8 @@ __device__ __forceinline__ void keep_sums(const GemmArgs& a, const float (&v)[32
 
 template <int CG, int TN>
 __global__ void __launch_bounds__(MXG_THREADS, 1)
-    mx_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap atail,
+                   const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap btail,
                    const __grid_constant__ CUtensorMap asmap, const __grid_constant__ CUtensorMap bsmap,
                    const __grid_constant__ GemmArgs a) {
     constexpr int TM = CG * GM_M, BN = TN / CG, ST = mxg_stages(CG, TN), BT = mxg_btiles(TN), ACCS = mxg_free(TN);
@@ -314,6 +315,8 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
     if (tid == 0) {
         prefetch_tensormap(&amap);
         prefetch_tensormap(&bmap);
+        prefetch_tensormap(&atail);
+        prefetch_tensormap(&btail);
         prefetch_tensormap(&asmap);
         prefetch_tensormap(&bsmap);
         for (int s = 0; s < ST; ++s) {
@@ -349,34 +352,47 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
         uint32_t ph = 1;  // parity of `empty`'s last phase: the first round finds every stage free
         bool ok = a.wait > 0;
         const uint32_t bar0 = CG == 2 ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
-        const uint32_t bytes = CG * (STAGE - (uint32_t)(GM_M - a.a_rows) * 128u);
         auto load = [&](int stage, uint32_t to, const CUtensorMap* map, int x, int y) {
             unsigned char* dst = sm + stage * STAGE + to;
             if constexpr (CG == 2) tma_load_2d_pair(dst, map, x, y, bar0 + 8u * stage);
             else tma_load_2d(dst, map, x, y, &full[stage]);
         };
-        // parts outside the tensors are filled with zeros and count as bytes
-        auto load_b = [&](int stage, int nt, int kb) {
+        // A CTA's parts of a tile's operands, the rows that are there (by a map of the last part's height, rounded up to 8): rows
+        // past the end cost a load as much as others (a tile of 16 rows that loads 128 takes 16 x 4096 x 151936 from 69 to 78
+        // us).  What is not loaded is left as it was and not stored.
+        const CUtensorMap *ma, *mb;  // null: no rows
+        int m0, n0, nt;
+        uint32_t bytes;
+        auto tile = [&](int64_t t) {
+            auto held = [](int first, int part, int end) { return end - first >= part ? part : end > first ? (end - first + 7) / 8 * 8 : 0; };
+            int mt;
+            tile_of<TM>(a, t, &mt, &nt);
+            m0 = mt * TM + (int)rank * GM_M;
+            n0 = nt * TN + (int)rank * BN;
+            const int ra = held(m0, GM_M, a.M), rb = held(n0, BN, a.N);
+            ma = ra == GM_M ? &amap : ra ? &atail : nullptr;
+            mb = rb == BN ? &bmap : rb ? &btail : nullptr;
+            bytes = CG * (STAGE - SFA) + 128u * (uint32_t)(ra + rb);
+            if (CG == 2) bytes += 128u * (uint32_t)(held(m0 + GM_M, GM_M, a.M) + held(n0 + BN, BN, a.N));  // the first CTA counts both
+        };
+        auto load_b = [&](int stage, int kb) {
             if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
-            load(stage, GM_A_BYTES, &bmap, kb * (MXG_KB / 4), nt * TN + (int)rank * BN);  // in units of 2 bytes
-            load(stage, SFB, &bsmap, kb * 256, nt * TN / 128);                            // in words
+            if (mb) load(stage, GM_A_BYTES, mb, kb * (MXG_KB / 4), n0);  // in units of 2 bytes
+            load(stage, SFB, &bsmap, kb * 256, nt * TN / 128);           // in words; tiles past the end are zeros and count as bytes
         };
         Piece p;
         int early = 0;  // stages whose B is on its way before the wait for the kernel that makes A
         if (ok && a.early) {
             for (int i = 0; early < ST && piece_at<CG>(a, i, &p); ++i) {
-                int mt, nt;
-                tile_of<TM>(a, p.tile, &mt, &nt);
+                tile(p.tile);
                 for (int kb = p.kb0; kb < p.kb1 && early < ST; ++kb, ++early)
-                    if (elect_one()) load_b(early, nt, kb);
+                    if (elect_one()) load_b(early, kb);
             }
             __syncwarp();
         }
         pdl_wait_then_release();
         for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i) {
-            int mt, nt;
-            tile_of<TM>(a, p.tile, &mt, &nt);
-            const int m0 = mt * TM + (int)rank * GM_M;
+            tile(p.tile);
             for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
                 if (!__all_sync(0xffffffffu, gm_wait<false>(&empty[s], ph, a.wait))) {
                     *fail = 1;
@@ -384,8 +400,8 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
                     break;
                 }
                 if (elect_one()) {
-                    if (it >= early) load_b(s, nt, kb);
-                    load(s, 0, &amap, kb * (MXG_KB / 4), m0);
+                    if (it >= early) load_b(s, kb);
+                    if (ma) load(s, 0, ma, kb * (MXG_KB / 4), m0);
                     load(s, SFA, &asmap, kb * 256, m0 / 128);
                 }
                 __syncwarp();
@@ -552,12 +568,14 @@ template <int CG, int TN>
 int mx_gemm_tn(const MxOperand& A, const MxOperand& B, int64_t K, GemmArgs a, const Plan& p, void* stream) {
     constexpr int TM = CG * GM_M;
     a.wait = wait_limit();
-    CUtensorMap amap, bmap, asmap, bsmap;
+    CUtensorMap amap, atail, bmap, btail, asmap, bsmap;
     const int64_t row = mx_row_bytes(K) / 2, tiles = mx_tiles(K);  // a row's codes in units of 2 bytes
-    // rows past the end cost a load as much as others: a tile of 16 rows that loads 128 takes 16 x 4096 x 151936 from 69 to 78 us
-    a.a_rows = CG == 1 && a.M < GM_M ? (a.M + 7) / 8 * 8 : GM_M;
-    int rc = tensor_map_2d(&amap, A.codes, row, a.M, row, MXG_KB / 4, a.a_rows);
-    if (rc == B2S_OK) rc = tensor_map_2d(&bmap, B.codes, row, a.N, row, MXG_KB / 4, TN / CG);
+    constexpr int BN = TN / CG;
+    auto tail = [](int all, int part) { return all % part ? (all % part + 7) / 8 * 8 : 8; };
+    int rc = tensor_map_2d(&amap, A.codes, row, a.M, row, MXG_KB / 4, GM_M);
+    if (rc == B2S_OK) rc = tensor_map_2d(&atail, A.codes, row, a.M, row, MXG_KB / 4, tail(a.M, GM_M));
+    if (rc == B2S_OK) rc = tensor_map_2d(&bmap, B.codes, row, a.N, row, MXG_KB / 4, BN);
+    if (rc == B2S_OK) rc = tensor_map_2d(&btail, B.codes, row, a.N, row, MXG_KB / 4, tail(a.N, BN));
     if (rc == B2S_OK) rc = tensor_map_words(&asmap, A.scales, tiles * 256, (a.M + 127) / 128, 256, 1);
     if (rc == B2S_OK) rc = tensor_map_words(&bsmap, B.scales, tiles * 256, (a.N + 127) / 128, 256, mxg_btiles(TN));
     if (rc != B2S_OK) return rc;
@@ -578,7 +596,8 @@ int mx_gemm_tn(const MxOperand& A, const MxOperand& B, int64_t K, GemmArgs a, co
         if (e != cudaSuccess) return cuda_fail(e);
         if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
-    e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, MXG_THREADS, mxg_smem(CG, TN), stream, amap, bmap, asmap, bsmap, a);
+    e = launch_cluster(kernel, dim3((unsigned)(p.G * CG)), CG, MXG_THREADS, mxg_smem(CG, TN), stream, amap, atail, bmap, btail,
+                       asmap, bsmap, a);
     if (e == cudaSuccess && p.split > 1) {
         const int held = a.M < TM ? a.M : TM;
         e = launch_pdl(gemm_join_kernel<TM, TN, EPI_LINEAR>,
