@@ -2,16 +2,20 @@
 // tcgen05.mma kind::mxf4, whose blocks of 32 k carry their scales into the multiplication, at four times bf16's rate; fp32
 // accumulation in tensor memory; bias, activation and residual in the epilogue.
 //
-// The shape is b2s_gemm.cuh's: persistent CTAs or pairs of them, a TMA ring, one loading and one issuing warp and eight
-// epilogue warps, tiles cut by the same plan (a stage of 256 k holds the same 128 bytes a row and takes the same clocks as
-// one of 64 k in bf16), chunks along k joined by a second kernel.  What is added: a stage brings 1 KB of scales for
-// each 128 rows, copied in the layout of the matrix's scale tiles, and the issuing warp has the tensor cores copy them from
-// shared to tensor memory (tcgen05.cp, each 512 bytes spread over 32 lanes and 4 columns, for all four lane quarters).
-// Each stage of the ring has its own columns there: when a stage is full again, the MMAs that read its scales are done.
-// Two accumulators of 256 columns leave no room for scales beside them, so they share 128 columns: the epilogue takes those to
-// registers first (64 a thread) and lets the next tile's MMAs begin, then the other 128 from where they lie.  (Taken whole,
-// 128 a thread, the registers spilled to a first-level cache that the ring leaves nothing of: 1000 x 4096 x 151936 993 us
-// against 254, of which 33 are the epilogue; an arrival per thread instead of per warp cost 60 more.)
+// The shape is b2s_gemm.cuh's: persistent CTAs or pairs of them, a TMA ring (a stage of 256 k holds the 128 bytes a row that 64 k
+// are in bf16), a loading and an issuing warp, tiles that do not fill a round split along k and joined by a second kernel.
+// What is different:
+// * A stage brings 1 KB of scales for each 128 rows, as the matrix's scale tiles lie, and the issuing warp has the tensor cores
+//   copy them to tensor memory (tcgen05.cp: 512 bytes to 32 lanes x 4 columns, the same in all four lane quarters).  Each
+//   stage of the ring has its own columns there: when a stage is full again, the MMAs that read its scales are done.
+// * Two accumulators of 256 columns leave no room for scales beside them, so they share 128 columns: the epilogue takes those to
+//   registers first and lets the next tile's MMAs begin, then the other 128 from where they lie.  (Taken whole, 128 columns a
+//   thread, the registers spilled to a first-level cache that the ring leaves nothing of: 1000 x 4096 x 151936 993 us against
+//   254 with shared columns.)
+// * Sixteen epilogue warps instead of eight: the MMAs are four times as fast, the epilogue is what is left (8192 x 4096 x 4096
+//   with gelu 105 against 84 us).
+// A large product is bound by the way from L2 to the SMs: a pair's stage asks for 70 KB in 530 clocks, 66 bytes a clock and SM,
+// and the output's way out comes on top (1000 x 4096 x 151936: 5.0 PFLOP/s; 5.7 without the epilogue, 6.6 without loads too).
 #include <string.h>
 
 #include <atomic>
@@ -34,9 +38,8 @@ constexpr int MXG_KB = 256;  // k per stage: one 128-byte row of the swizzle
 constexpr int MXG_EPI = 16;  // epilogue warps: warp w has tensor-memory quarter w % 4 and part w / 4 of the columns
 constexpr int MXG_THREADS = 32 * MXG_EPI + 64;
 constexpr uint32_t MXG_STAGING = MXG_EPI * 2048;  // per epilogue warp: 32 rows of 32 bf16, or of 16 fp32
-__host__ __device__ constexpr int mxg_parts(int tn) { return tn < 128 ? tn / 32 : 4; }  // of 32 columns, and again 32 of 256
-// 128-row scale tiles of B that a tile of TN columns touches
-__host__ __device__ constexpr int mxg_btiles(int tn) { return tn > 128 ? tn / 128 : 1; }
+constexpr int MXG_PARTS = 4;  // of 32 columns, and again 32 of 256
+__host__ __device__ constexpr int mxg_btiles(int tn) { return tn / 128; }  // scale tiles of B
 // A stage of one CTA: 128 rows of A, its share of B, A's scales (1 KB) and all of the tile's B's.
 __host__ __device__ constexpr uint32_t mxg_stage_bytes(int cg, int tn) {
     return GM_A_BYTES + (uint32_t)(tn / cg) * 128 + 1024 + 1024 * mxg_btiles(tn);
@@ -54,9 +57,10 @@ __host__ __device__ constexpr int mxg_acc_step(int tn) { return tn == 256 ? 128 
 __host__ __device__ constexpr int mxg_acc_cols(int tn) { return mxg_acc_step(tn) + tn; }
 __host__ __device__ constexpr int mxg_free(int tn) { return tn == 256 ? 1 : 2; }  // accumulators handed back apart
 __host__ __device__ constexpr int mxg_sf_cols(int tn) { return 8 + 8 * mxg_btiles(tn); }
-__host__ __device__ constexpr uint32_t mxg_tmem(int cg, int tn) {
-    return mxg_acc_cols(tn) + mxg_stages(cg, tn) * mxg_sf_cols(tn) > 256 ? 512 : 256;
-}
+constexpr uint32_t MXG_TMEM = 512;
+static_assert(mxg_acc_cols(128) + mxg_stages(1, 128) * mxg_sf_cols(128) <= (int)MXG_TMEM &&
+                  mxg_acc_cols(256) + mxg_stages(2, 256) * mxg_sf_cols(256) <= (int)MXG_TMEM,
+              "accumulators and scales fit tensor memory");
 
 // Shared-memory descriptor of 512 bytes of scales: 32 rows of 16 bytes, 8 rows at a time (128 bytes), no swizzle.
 __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
         }
         for (int s = 0; s < ACCS; ++s) {
             mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], 4 * mxg_parts(TN) * CG);
+            mbar_init(&tempty[s], 4 * MXG_PARTS * CG);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -334,8 +338,8 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
         *consumed = 0;
     }
     if (warp == MXG_EPI + 1) {
-        if constexpr (CG == 2) tmem_alloc_pair(tslot, mxg_tmem(CG, TN));
-        else tmem_alloc(tslot, mxg_tmem(CG, TN));
+        if constexpr (CG == 2) tmem_alloc_pair(tslot, MXG_TMEM);
+        else tmem_alloc(tslot, MXG_TMEM);
     }
     tc_fence_before();
     __syncthreads();
@@ -433,8 +437,6 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
             Piece p;
             int g = 0;  // accumulators handed over
             for (int i = 0; ok && piece_at<CG>(a, i, &p); ++i, ++g) {
-                int mt, nt;
-                tile_of<TM>(a, p.tile, &mt, &nt);
                 const int acc = g % ACCS;
                 if (g >= ACCS &&
                     !__all_sync(0xffffffffu, gm_wait<CG == 2>(&tempty[acc], (uint32_t)(g / ACCS - 1) & 1u, a.wait))) {
@@ -443,8 +445,6 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)((g & 1) * mxg_acc_step(TN));
-                // a tile of 64 columns may be the second half of its scale tile's rows: two columns on
-                const uint32_t half = TN < 128 ? (uint32_t)(nt * TN % 128) / 32 : 0u;
                 uint32_t more = 0;
                 for (int kb = p.kb0; kb < p.kb1; ++kb, ++it) {
                     if (!__all_sync(0xffffffffu, gm_wait<false>(&full[s], ph, a.wait))) {
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
 #pragma unroll
                         for (int k = 0; k < MXG_KB / 64; ++k) {  // 64 k: 32 bytes
                             const uint32_t id = IDESC | (uint32_t)(k & 1) << 30 | (uint32_t)(k & 1) << 5;
-                            umma_mxf4<CG>(d, da0 + at + 2 * k, db0 + at + 2 * k, id, sa + 4 * (k >> 1), sb + 4 * BT * (k >> 1) + half, more);
+                            umma_mxf4<CG>(d, da0 + at + 2 * k, db0 + at + 2 * k, id, sa + 4 * (k >> 1), sb + 4 * BT * (k >> 1), more);
                             more = 1;
                         }
                         commit(&empty[s]);
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
             }
             if (lane == 0) *consumed = it;
         }
-    } else if (warp < 4 * mxg_parts(TN)) {
+    } else if (warp < 4 * MXG_PARTS) {
         Piece p;
         int g = 0;
         bool ok = a.wait > 0;
@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(MXG_THREADS, 1)
     }
     if (warp == MXG_EPI + 1) {
         tc_fence_after();
-        if constexpr (CG == 2) tmem_dealloc_pair(tmem, mxg_tmem(CG, TN));
-        else tmem_dealloc(tmem, mxg_tmem(CG, TN));
+        if constexpr (CG == 2) tmem_dealloc_pair(tmem, MXG_TMEM);
+        else tmem_dealloc(tmem, MXG_TMEM);
     }
 }
 
@@ -608,17 +608,67 @@ int mx_gemm_tn(const MxOperand& A, const MxOperand& B, int64_t K, GemmArgs a, co
 
 }  // namespace
 
-// A stage of 256 k costs what one of 64 k costs the bf16 product: the same bytes a row, the same clocks.
-Plan mx_plan(int M, int N, int64_t K) { return plan_here(M, N, mx_tiles(K) * GM_KB, EPI_LINEAR); }
+// The cheaper of two cuts by estimated clocks: tiles of 128 x 128 by one CTA, 256 x 256 by a pair (128 x 64 was up to 1 us
+// better for a few short products, 128 x 256 or a pair with 128 columns up to 4 % for a few others).  A stage costs its MMAs
+// (530 clocks for 256 columns; 480 for 128, the issuing warp's pace) or its way from L2 (62 bytes a clock; rows outside A are
+// not fetched), with a single tile of rows its weights' way from HBM (26 bytes a clock for each of all CTAs).  A pair's
+// accumulators share columns, and its MMAs wait 1500 clocks a tile for the epilogue to take them.  The epilogue costs 4000
+// clocks for 128 columns, hidden under the next tile's stages except the last one's.  Tiles that do not fill a round may be
+// split along k, where the saving passes the second launch, 6000 clocks, and the sums' way there and back.
+// Measured, us, 128 x 128 / 256 x 256: 300 x 4096 x 4096 13.8 / 15.9, 2000 x 4096 x 4096 33 / 28, 1000 x 4096 x 151936 345 / 248,
+// 8192 x 768 x 768 15.9 / 18.7; 16 x 16384 x 256 23.7 whole, 14.3 in four.
+Plan mx_plan(int M, int N, int64_t K) {
+    auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    const int sms = sms_here();
+    const int64_t nkb = mx_tiles(K);
+    Plan best = {};
+    int64_t best_cost = INT64_MAX;
+    for (int cg = 1; cg <= 2; ++cg) {
+        const int tn = 128 * cg, tm = GM_M * cg, U = sms / cg;
+        if (cg == 2 && M <= GM_M) continue;  // half of the pair would have no rows
+        const int64_t tiles = ceil_div(M, tm) * ceil_div(N, tn);
+        const int64_t busy = tiles < U ? tiles : U, hbm = M <= GM_M ? tn * 136 * busy / (26 * U) : 0;
+        int64_t stage = cg == 2 ? 530 : 480;
+        const int64_t fill = ((M < GM_M ? M : GM_M) + tn / cg) * 136 / 62;
+        if (stage < fill) stage = fill;
+        if (stage < hbm) stage = hbm;
+        const int64_t wait = cg == 2 ? 1500 : 300, tail = tn == 256 ? 8000 : 4000;
+        Plan p = {};
+        p.cg = cg;
+        p.tn = tn;
+        p.G = (int)busy;
+        p.waves = (int)(tiles / U);
+        p.rest = (int)(tiles % U);
+        p.split = 1;
+        p.chunk = (int)nkb;
+        auto rounds_cost = [&](int64_t rounds) {
+            const int64_t mine = nkb * stage + wait;
+            return rounds ? mine + (rounds - 1) * (mine > tail ? mine : tail) + tail : 0;
+        };
+        int64_t cost = rounds_cost(p.waves + (p.rest ? 1 : 0));
+        for (int64_t want = 2; p.rest && want <= nkb && want <= 64; want += want < 4 ? 1 : want / 2) {  // 2 3 4 6 9 13 19 28 42 63
+            const int64_t chunk = ceil_div(nkb, want), split = ceil_div(nkb, chunk);
+            const int64_t bytes = split * p.rest * (M < tm ? M : tm) * tn * 4;
+            const int64_t c = rounds_cost(p.waves) + ceil_div(p.rest * split, U) * chunk * stage + tail + 6000 + 2 * bytes / 3000;
+            if (split > 1 && c < cost) {
+                cost = c;
+                p.split = (int)split;
+                p.chunk = (int)chunk;
+                p.bytes = bytes;
+                p.G = (int)(p.waves || p.rest * split >= U ? U : p.rest * split);
+            }
+        }
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = p;
+        }
+    }
+    return best;
+}
 
 int mx_gemm(const MxOperand& A, const MxOperand& B, int64_t K, const GemmArgs& a, void* stream) {
     const Plan p = mx_plan(a.M, a.N, K);
-    if (p.cg == 2) return p.tn == 256 ? mx_gemm_tn<2, 256>(A, B, K, a, p, stream) : mx_gemm_tn<2, 128>(A, B, K, a, p, stream);
-    switch (p.tn) {
-        case 256: return mx_gemm_tn<1, 256>(A, B, K, a, p, stream);
-        case 128: return mx_gemm_tn<1, 128>(A, B, K, a, p, stream);
-        default: return mx_gemm_tn<1, 64>(A, B, K, a, p, stream);
-    }
+    return p.cg == 2 ? mx_gemm_tn<2, 256>(A, B, K, a, p, stream) : mx_gemm_tn<1, 128>(A, B, K, a, p, stream);
 }
 
 }  // namespace b2s
