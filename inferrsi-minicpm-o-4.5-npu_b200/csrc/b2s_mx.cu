@@ -375,32 +375,12 @@ __device__ __forceinline__ void mx_bytes(uint32_t c, int& lo, int& hi) {
     lo = four(c);
     hi = four(c >> 16);
 }
-// 32 elements of x from column n as bytes, and their scale's factor (a quarter of it, for the two doubled operands).
-__device__ __forceinline__ float mx_block_bytes(const unsigned short* row, int n, int k, bool vec, int (&b)[8]) {
-    MxWords<unsigned short> v[4];
-    uint32_t most = 0;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        v[q] = vec && n + 8 * q + 8 <= k ? mx_words(row + n + 8 * q) : mx_words(row + n + 8 * q, (int64_t)k - n - 8 * q);
-        most = max(most, mx_most(v[q]));
-    }
-    const uint32_t code = mx_scale_code<2>(most);
-    const float inv = mx_inverse(code);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        float u[8];
-        mx_times(v[q], inv, u);
-        mx_bytes(mx_encode8(u), b[2 * q], b[2 * q + 1]);
-    }
-    return mx_scale(code) * 0.25f;
-}
-
 struct MxRowsArgs {
     const unsigned short* x;  // bf16 rows, or null and the codes and scales of a quantised x
     int64_t x_stride;
     const uint8_t *xc, *xs;
     const uint8_t *wc, *ws;
-    int M, N, K, act, x_vec, tpr;
+    int M, N, K, act, x_vec;
     const unsigned short *bias, *residual;
     int64_t res_stride;
     __half* preact;
@@ -409,97 +389,161 @@ struct MxRowsArgs {
     int64_t out_stride;
 };
 
-// out = act(x^ w^T + b) + r for groups of at most R rows (grid.y), F features per group of `tpr` threads.  A thread takes
-// the blocks tpr apart: x's block as bytes in registers (quantised here: no launch of its own), a feature's 16 bytes of
-// codes as bytes, and integer dot products, exact within a block; blocks are added in fp32.
-constexpr int MXR_NT = 128;
+// out = act(x^ w^T + b) + r for at most R rows.  A CTA quantises x itself (no launch of its own), to bytes in shared memory; then its
+// warps take F features at a time: a lane has the blocks 32 apart, 16 bytes of codes each, turned to bytes, and integer dot
+// products with x's, exact within a block; blocks are added in fp32.  With x's blocks in registers and a group of threads per
+// feature, x was quantised once for every four features: 1 x 4096 x 4096 MXROWS.
+constexpr int MXR_NT = 256;
+constexpr int MXR_SMEM = 36 * 1024;  // of x: 32 bytes and a factor a block and row
 template <int R, int F>
 __global__ void __launch_bounds__(MXR_NT) mx_rows_kernel(const __grid_constant__ MxRowsArgs a) {
-    __shared__ float red[MXR_NT / 32][R * F];
+    constexpr int W = MXR_NT / 32, U = 4;  // warps; blocks of a lane in flight
+    extern __shared__ __align__(16) unsigned char xsm[];
     pdl_wait_then_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int group = tid / a.tpr, n0 = ((int)blockIdx.x * (MXR_NT / a.tpr) + group) * F, r0 = (int)blockIdx.y * R;
     const int nb = (int)mx_blocks(a.K);
-    const int64_t tiles = mx_tiles(a.K);
-    float acc[R][F];
+    const int64_t tiles = mx_tiles(a.K), step = (int64_t)gridDim.x * W * F;
+    const uint4* wp[F];
+    const uint8_t* sp[F];
+    auto at = [&](int64_t n0) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int f = 0; f < F; ++f) acc[r][f] = 0.0f;
-    for (int b = tid % a.tpr; b < nb; b += a.tpr) {
-        uint4 w[F];
-        uint32_t ws[F];
-#pragma unroll
-        for (int f = 0; f < F; ++f) {  // features and rows past the end repeat the last one; they are not stored
-            const int64_t n = min(n0 + f, a.N - 1);
-            w[f] = ldg_stream(reinterpret_cast<const uint4*>(a.wc) + n * nb + b);
-            ws[f] = __ldg(a.ws + mx_scale_at(n, b, tiles));
+        for (int f = 0; f < F; ++f) {  // a feature past the end repeats the last one
+            const int64_t n = min(n0 + f, (int64_t)a.N - 1);
+            wp[f] = reinterpret_cast<const uint4*>(a.wc) + n * nb;
+            sp[f] = a.ws + mx_scale_at(n, 0, tiles);
         }
-        int xb[R][8];
-        float xs[R];
+    };
+    uint4 w[U][F];
+    uint32_t ws[U][F];
+    auto load = [&](int b0) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t m = min(r0 + r, a.M - 1);
-            if (a.x) {
-                xs[r] = mx_block_bytes(a.x + m * a.x_stride, 32 * b, a.K, a.x_vec, xb[r]);
-            } else {
-                const uint4 q = __ldg(reinterpret_cast<const uint4*>(a.xc) + m * nb + b);
-                mx_bytes(q.x, xb[r][0], xb[r][1]);
-                mx_bytes(q.y, xb[r][2], xb[r][3]);
-                mx_bytes(q.z, xb[r][4], xb[r][5]);
-                mx_bytes(q.w, xb[r][6], xb[r][7]);
-                xs[r] = mx_scale(__ldg(a.xs + mx_scale_at(m, b, tiles))) * 0.25f;
-            }
-        }
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            int wb[8];
-            mx_bytes(w[f].x, wb[0], wb[1]);
-            mx_bytes(w[f].y, wb[2], wb[3]);
-            mx_bytes(w[f].z, wb[4], wb[5]);
-            mx_bytes(w[f].w, wb[6], wb[7]);
-            const float s = mx_scale(ws[f]);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                int d = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) d = __dp4a(wb[j], xb[r][j], d);
-                acc[r][f] = __fmaf_rn((float)d, xs[r] * s, acc[r][f]);
-            }
-        }
+            for (int f = 0; f < F; ++f)
+                if (b0 + 32 * u < nb) {
+                    w[u][f] = ldg_stream(wp[f] + b0 + 32 * u);
+                    ws[u][f] = __ldg(sp[f] + mx_scale_at(0, b0 + 32 * u, tiles));
+                }
+    };
+    int64_t n0 = ((int64_t)blockIdx.x * W + warp) * F;
+    if (n0 < a.N) {  // on their way while x is quantised
+        at(n0);
+        load(lane);
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int f = 0; f < F; ++f) {
-            float t = acc[r][f];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            if (lane == 0) red[warp][r * F + f] = t;
+    uint2* xb = reinterpret_cast<uint2*>(xsm);  // [R][nb][4]: a lane's 8 elements as bytes; the lanes' 16-byte reads are 32 apart
+    float* xf = reinterpret_cast<float*>(xsm + (size_t)R * nb * 32);  // [R][nb]
+    for (int i0 = warp * 32; i0 < 4 * R * nb; i0 += MXR_NT) {         // 8 elements a lane, a block four lanes
+        const int i = i0 + lane, r = i / (4 * nb), e = i % (4 * nb);
+        const bool in = i < 4 * R * nb;
+        const int64_t m = min(r, a.M - 1);  // rows past the end repeat the last one; they are not stored
+        uint32_t c = 0;
+        float f = 0.0f;
+        if (a.x) {
+            const unsigned short* row = a.x + m * a.x_stride + 8 * e;
+            const int left = in ? a.K - 8 * e : 0;
+            const MxWords<unsigned short> v = a.x_vec && left >= 8 ? mx_words(row) : mx_words(row, left);
+            uint32_t most = mx_most(v);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const uint32_t code = mx_scale_code<2>(most);
+            float u[8];
+            mx_times(v, mx_inverse(code), u);
+            c = mx_encode8(u);
+            f = mx_scale(code);
+        } else if (in) {
+            c = __ldg(reinterpret_cast<const uint32_t*>(a.xc) + m * nb * 4 + e);
+            f = mx_scale(__ldg(a.xs + mx_scale_at(m, e >> 2, tiles)));
         }
+        if (!in) continue;
+        int lo, hi;
+        mx_bytes(c, lo, hi);
+        xb[i] = make_uint2((uint32_t)lo, (uint32_t)hi);
+        if ((e & 3) == 0) xf[i >> 2] = f * 0.25f;  // both operands' bytes are doubled
+    }
     __syncthreads();
-    const int per = a.tpr / 32;  // warps of a group
-    for (int i = tid; i < R * F * (MXR_NT / a.tpr); i += MXR_NT) {
-        const int g = i / (R * F), j = i % (R * F), m = r0 + j / F, n = ((int)blockIdx.x * (MXR_NT / a.tpr) + g) * F + j % F;
-        if (m >= a.M || n >= a.N) continue;
-        float t = red[g * per][j];
-        for (int k = 1; k < per; ++k) t += red[g * per + k][j];
-        if (a.bias) t += bf16_bits_to_f(__ldg(a.bias + n));
-        if (a.preact) a.preact[(int64_t)m * a.pre_stride + n] = __ushort_as_half(preact_bits(t));
-        t = act_apply(t, a.act);
-        if (a.residual) t += bf16_bits_to_f(__ldg(a.residual + (int64_t)m * a.res_stride + n));
-        a.out[(int64_t)m * a.out_stride + n] = __float2bfloat16_rn(t);
+    for (; n0 < a.N; n0 += step) {
+        float acc[R][F] = {};
+        for (int b0 = lane; b0 < nb; b0 += 32 * U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int b = b0 + 32 * u;
+                if (b >= nb) break;
+                int wb[F][8];
+                float s[F];
+#pragma unroll
+                for (int f = 0; f < F; ++f) {
+                    mx_bytes(w[u][f].x, wb[f][0], wb[f][1]);
+                    mx_bytes(w[u][f].y, wb[f][2], wb[f][3]);
+                    mx_bytes(w[u][f].z, wb[f][4], wb[f][5]);
+                    mx_bytes(w[u][f].w, wb[f][6], wb[f][7]);
+                    s[f] = mx_scale(ws[u][f]);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const int4* x = reinterpret_cast<const int4*>(xb) + 2 * (r * nb + b);
+                    const int4 p = x[0], q = x[1];
+                    const float xs = xf[r * nb + b];
+#pragma unroll
+                    for (int f = 0; f < F; ++f) {
+                        int d = __dp4a(wb[f][0], p.x, 0);
+                        d = __dp4a(wb[f][1], p.y, d);
+                        d = __dp4a(wb[f][2], p.z, d);
+                        d = __dp4a(wb[f][3], p.w, d);
+                        d = __dp4a(wb[f][4], q.x, d);
+                        d = __dp4a(wb[f][5], q.y, d);
+                        d = __dp4a(wb[f][6], q.z, d);
+                        d = __dp4a(wb[f][7], q.w, d);
+                        acc[r][f] = __fmaf_rn((float)d, xs * s[f], acc[r][f]);
+                    }
+                }
+            }
+            if (b0 + 32 * U < nb) load(b0 + 32 * U);
+        }
+        const int64_t done = n0;
+        if (n0 + step < a.N) {  // the next features' on their way under the sums
+            at(n0 + step);
+            load(lane);
+        }
+        float mine = 0.0f;  // lane r F + f: the row's and feature's sum
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                float t = acc[r][f];
+#pragma unroll
+                for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+                mine = lane == r * F + f ? t : mine;
+            }
+        const int m = lane / F;
+        const int64_t n = done + lane % F;
+        if (lane < R * F && m < a.M && n < a.N) {
+            float t = mine;
+            if (a.bias) t += bf16_bits_to_f(__ldg(a.bias + n));
+            if (a.preact) a.preact[(int64_t)m * a.pre_stride + n] = __ushort_as_half(preact_bits(t));
+            t = act_apply(t, a.act);
+            if (a.residual) t += bf16_bits_to_f(__ldg(a.residual + (int64_t)m * a.res_stride + n));
+            a.out[(int64_t)m * a.out_stride + n] = __float2bfloat16_rn(t);
+        }
     }
 }
 
+template <int R>
 cudaError_t mx_rows(const MxRowsArgs& a, void* stream) {
-    auto go = [&](auto kernel, int R, int F) {
-        const int64_t per = (int64_t)(MXR_NT / a.tpr) * F;
-        return launch_pdl(kernel, dim3((unsigned)((a.N + per - 1) / per), (unsigned)((a.M + R - 1) / R)), MXR_NT, 0, stream, a);
+    const int64_t most = 3 * (int64_t)sms_here(), one = ((int64_t)a.N + 7) / 8;  // blocks with a feature a warp
+    auto go = [&](auto kernel, int64_t want) {
+        return launch_pdl(kernel, dim3((unsigned)(want < most ? want : most)), MXR_NT, (uint32_t)(R * mx_blocks(a.K) * 36), stream, a);
     };
-    return a.M == 1 ? go(mx_rows_kernel<1, 4>, 1, 4) : a.M == 2 ? go(mx_rows_kernel<2, 4>, 2, 4) : go(mx_rows_kernel<4, 4>, 4, 4);
+    return one <= most ? go(mx_rows_kernel<R, 1>, one) : go(mx_rows_kernel<R, 2>, (one + 1) / 2);
 }
-bool mx_few_rows(int rows) { return rows <= 4; }
+cudaError_t mx_rows(const MxRowsArgs& a, void* stream) {
+    return a.M == 1 ? mx_rows<1>(a, stream) : a.M == 2 ? mx_rows<2>(a, stream) : mx_rows<4>(a, stream);
+}
+// Which products take it.  Against the tensor cores' path, us: 1 x 4096 x 768 3.7 : 11.0, 4 x 768 x 6562 6.1 : 8.4, 1 x 4096 x 4096
+// 6.2 : 11.7, 4 rows of it 9.9 : 11.9, but 1 x 4096 x 8192 11.9 : 12.3 and 4 rows 20.5 : 12.3, 1 x 768 x 30000 14.0 : 11.3, 1 x
+// 4096 x 151936 106 : 63 (turning codes to bytes takes two operations an element).
+bool mx_few_rows(int rows, int N, int64_t K) {
+    return rows <= 4 && N * K <= 1 << 24 && (rows < 3 ? rows : 4) * mx_blocks(K) * 36 <= MXR_SMEM;
+}
 
 // The workspace of the tensor cores' path: x's codes and scales, then the sums of tiles that are split.
 struct MxWork {
@@ -554,7 +598,7 @@ int b2s_mx_linear_workspace(int32_t rows, int32_t in_features, int32_t out_featu
     using namespace b2s;
     if (rows < 0 || in_features < 1 || out_features < 1 || !bytes) return B2S_ERR_INVALID;
     *bytes = 0;
-    if (rows && !mx_few_rows(rows)) {
+    if (rows && !mx_few_rows(rows, out_features, in_features)) {
         const MxWork w = mx_work(rows, in_features);
         *bytes = w.partial + mx_plan(rows, out_features, in_features).bytes;
     }
@@ -578,7 +622,7 @@ int b2s_mx_linear(const b2s_mx_linear_args* l, void* stream) {
     int64_t need = 0;
     b2s_mx_linear_workspace(l->rows, l->in_features, l->out_features, &need);
     if (need && (!l->workspace || l->workspace_bytes < need || !aligned16(l->workspace))) return B2S_ERR_INVALID;
-    if (mx_few_rows(l->rows)) {
+    if (mx_few_rows(l->rows, l->out_features, l->in_features)) {
         MxRowsArgs a;
         memset(&a, 0, sizeof(a));
         a.x = static_cast<const unsigned short*>(l->x);
@@ -599,8 +643,6 @@ int b2s_mx_linear(const b2s_mx_linear_args* l, void* stream) {
         a.pre_stride = l->preact_row_stride;
         a.out = static_cast<__nv_bfloat16*>(l->out);
         a.out_stride = l->out_row_stride;
-        const int64_t nb = mx_blocks(a.K);
-        a.tpr = nb > 64 ? 128 : nb > 32 ? 64 : 32;
         const cudaError_t e = mx_rows(a, stream);
         return e == cudaSuccess ? B2S_OK : cuda_fail(e);
     }
