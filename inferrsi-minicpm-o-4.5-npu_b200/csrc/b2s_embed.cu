@@ -7,14 +7,15 @@
 //
 // Gradient: the whole table's gradient is written once, so what bounds it is that write (1.24 GB for the Thinker's table)
 // and one read of the rows' gradients.  The positions are sorted by id without a sort of keys: a count per id (the atomic's
-// old value is the position's place among its id's, in order of arrival), ranges handed out to the ids that occur, and
-// then each id's positions put in ascending order, so that sums do not depend on who arrived first.  An id's positions
-// are summed in pieces of EM_PIECE, in order, in fp32; an id with several pieces leaves their sums in a workspace, and a
-// last kernel adds them in order.
+// old value is the position's place among its id's, in order of arrival), the counts' prefix sums, and then each id's
+// positions put in ascending order, so that sums do not depend on who arrived first.  The sorted positions are summed in
+// chunks of EM_CHUNK, whatever ids they hold, one chunk a warp and part of a row, in order, in fp32: an id inside a chunk is
+// written at once, of one that goes on the sums are joined by whoever completes them, in order.
 #include <string.h>
 
 #include "../../include/b2s_sampler.h"
 #include "b2s_device.cuh"
+#include "b2s_gemm.cuh"
 #include "b2s_launch.cuh"
 #include "b2s_logprobs.cuh"
 #include "b2s_mx.cuh"
@@ -26,32 +27,48 @@ int cuda_fail(cudaError_t e);
 namespace {
 
 constexpr int EM_NT = 256;
-constexpr int EM_PIECE = 32;   // positions summed by one warp
-constexpr int EM_UNITS = 128;  // 16-byte units (or elements) of a row that a warp takes
+constexpr int EM_CHUNK = 32;   // sorted positions that a warp sums
+constexpr int EM_JOIN = 16;    // sums joined at a time
+constexpr int EM_BINS = 4096;  // at most, of ids counted together
+constexpr int EM_UNITS = 64;   // 16-byte units (or elements) of a row that a warp takes
 constexpr int EM_WINDOW = 1 << 17;  // positions that a CTA's bitmap covers (16 KB)
 
-// E: 4 (fp32) or 2 (bf16) bytes an element; a unit is 16 bytes of them (VEC) or a single one.
+// E: 4 (fp32) or 2 (bf16) bytes an element; a unit is 16 bytes of them (VEC) or a single one, as it lies and as fp32.
+template <int E, bool VEC>
+struct RawUnit {
+    uint32_t w[VEC ? 4 : 1];
+    __device__ __forceinline__ void load(const void* row, int64_t u) {
+        if constexpr (VEC) {
+            const uint4 q = ldg_stream(reinterpret_cast<const uint4*>(row) + u);
+            w[0] = q.x;
+            w[1] = q.y;
+            w[2] = q.z;
+            w[3] = q.w;
+        } else if constexpr (E == 4) {
+            w[0] = __ldg(static_cast<const uint32_t*>(row) + u);
+        } else {
+            w[0] = (uint32_t)__ldg(static_cast<const unsigned short*>(row) + u) << 16;
+        }
+    }
+};
 template <int E, bool VEC>
 struct Unit {
     static constexpr int N = VEC ? 16 / E : 1;
     float v[N];
-    __device__ __forceinline__ void load(const void* row, int64_t u) {
-        if constexpr (VEC) {
-            const uint4 q = ldg_stream(reinterpret_cast<const uint4*>(row) + u);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = 0.0f;
+    }
+    __device__ __forceinline__ void add(const RawUnit<E, VEC>& o) {
+        if constexpr (VEC && E == 2) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (E == 4) {
-                    v[j] = __uint_as_float(w[j]);
-                } else {
-                    v[2 * j] = __uint_as_float(w[j] << 16);
-                    v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                }
+                v[2 * j] += __uint_as_float(o.w[j] << 16);
+                v[2 * j + 1] += __uint_as_float(o.w[j] & 0xffff0000u);
             }
-        } else if constexpr (E == 4) {
-            v[0] = __ldg(static_cast<const float*>(row) + u);
         } else {
-            v[0] = bf16_bits_to_f(__ldg(static_cast<const unsigned short*>(row) + u));
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] += __uint_as_float(o.w[j]);
         }
     }
     // each value times s, rounded to the element's type
@@ -73,14 +90,6 @@ struct Unit {
         } else {
             static_cast<__nv_bfloat16*>(row)[u] = __float2bfloat16_rn(v[0] * s);
         }
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = 0.0f;
-    }
-    __device__ __forceinline__ void add(const Unit& o) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] += o.v[j];
     }
 };
 
@@ -106,15 +115,17 @@ __global__ void __launch_bounds__(EM_NT) embed_kernel(const int64_t* tokens, int
     const int64_t t = token_at(tokens, i, vocab, lane == 0 && u0 == 0 ? status : nullptr);
     const unsigned char* src = static_cast<const unsigned char*>(table) + (t < 0 ? 0 : t) * row_bytes;
     unsigned char* dst = static_cast<unsigned char*>(out) + i * units * Unit<E, VEC>::N * E;
-    Unit<E, VEC> v[EM_UNITS / 32];
-#pragma unroll
-    for (int j = 0; j < EM_UNITS / 32; ++j) {
-        v[j].zero();
-        if (t >= 0 && u0 + 32 * j < units) v[j].load(src, u0 + 32 * j);
-    }
+    RawUnit<E, VEC> q[EM_UNITS / 32];
 #pragma unroll
     for (int j = 0; j < EM_UNITS / 32; ++j)
-        if (u0 + 32 * j < units) v[j].store(dst, u0 + 32 * j, s);
+        if (t >= 0 && u0 + 32 * j < units) q[j].load(src, u0 + 32 * j);
+#pragma unroll
+    for (int j = 0; j < EM_UNITS / 32; ++j) {
+        Unit<E, VEC> v;
+        v.zero();
+        if (t >= 0) v.add(q[j]);
+        if (u0 + 32 * j < units) v.store(dst, u0 + 32 * j, s);
+    }
 }
 
 // The same from a microscaled table: a unit is 8 elements, 4 bytes of codes.
@@ -154,17 +165,19 @@ __global__ void __launch_bounds__(EM_NT) embed_mx_kernel(const int64_t* tokens, 
 
 // ------------------------------------------------------------------ gradient
 
-// The words that start as zero, then the arrays that the kernels fill.
+// The workspace: words that start as zero, then the arrays that the kernels fill.
 struct EmbedSort {
-    int* next;    // [4]: places, pieces, ids with several pieces, their sums
-    int* count;   // [vocab] positions of an id
-    int* base;    // [vocab] where they start, for the ids that occur
-    int* place;   // [n] among the id's positions in order of arrival; -1: none
-    int* loose;   // [n] positions by id, in order of arrival
-    int* order;   // [n] positions by id, ascending
-    int4* piece;  // [n] (id, start, length, sum's place or -1)
-    int4* split;  // [n / EM_PIECE + 1] (id, first sum, sums)
-    float* sums;  // [2 n / EM_PIECE][width]
+    int* count;    // [vocab] positions of an id
+    int* bin;      // [bins] positions of 1 << shift ids
+    int* arrived;  // [2][slots][parts] sums that are there, of a group (at its first) and groups of an id (at its first)
+    int* total;    // positions that are not padding
+    int* base;     // [vocab] where an id's positions start, sorted
+    int* place;    // [n] among the id's positions in order of arrival; -1: none
+    int* loose;    // [n] positions by id, in order of arrival
+    int* order;    // [n] positions by id, ascending
+    int* id;       // [n] their ids
+    float* sums;   // [slots][width]: two for each chunk, of the id that came from the one before and of the last one, that goes on
+    int slots, shift, bins;
 };
 
 __global__ void __launch_bounds__(EM_NT) embed_count_kernel(const int64_t* tokens, int n, int64_t vocab, EmbedSort e) {
@@ -176,39 +189,50 @@ __global__ void __launch_bounds__(EM_NT) embed_count_kernel(const int64_t* token
     int at = 0;
     if (t >= 0 && lane == leader) at = atomicAdd(e.count + t, __popc(same));
     at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
+    const uint32_t near = __match_any_sync(0xffffffffu, t < 0 ? -1 : t >> e.shift);
+    if (t >= 0 && lane == __ffs(near) - 1) atomicAdd(e.bin + (t >> e.shift), __popc(near));
     if (i < n) e.place[i] = t < 0 ? -1 : at;
 }
 
-// The first arrival of each id takes a range of places and its pieces; which range an id gets does not matter.
-__global__ void __launch_bounds__(EM_NT) embed_range_kernel(const int64_t* tokens, int n, EmbedSort e) {
-    pdl_wait_then_release();
-    const int i = blockIdx.x * EM_NT + threadIdx.x, lane = threadIdx.x & 31;
-    const bool first = i < n && e.place[i] == 0;
-    const int t = first ? (int)tokens[i] : 0, c = first ? e.count[t] : 0, p = (c + EM_PIECE - 1) / EM_PIECE;
-    const int s = p > 1 ? p : 0;
-    auto take = [&](int k, int want) {  // a warp's wants from a counter with one atomic
-        int incl = want;
+// Exclusive prefix of v over the CTA's threads, and the sum.
+__device__ __forceinline__ int em_scan(int v, int* total) {
+    __shared__ int sums[EM_NT / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = v;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += u;
-        }
-        int at = 0;
-        if (lane == 31 && incl) at = atomicAdd(e.next + k, incl);
-        return __shfl_sync(0xffffffffu, at, 31) + incl - want;
-    };
-    const int base = take(0, c), piece = take(1, p), split = take(2, s ? 1 : 0), sum = take(3, s);
-    if (first) e.base[t] = base;
-    if (s) e.split[split] = make_int4(t, sum, s, 0);
-    uint32_t todo = __ballot_sync(0xffffffffu, first);
-    if (first && p == 1) e.piece[piece] = make_int4(t, base, c, -1);
-    for (todo = __ballot_sync(0xffffffffu, p > 1); todo; todo &= todo - 1) {  // long ones by the whole warp
-        const int l = __ffs(todo) - 1;
-        const int lt = __shfl_sync(0xffffffffu, t, l), lb = __shfl_sync(0xffffffffu, base, l), lc = __shfl_sync(0xffffffffu, c, l);
-        const int lp = __shfl_sync(0xffffffffu, piece, l), ls = __shfl_sync(0xffffffffu, sum, l);
-        for (int k = lane; k * EM_PIECE < lc; k += 32)
-            e.piece[lp + k] = make_int4(lt, lb + k * EM_PIECE, min(EM_PIECE, lc - k * EM_PIECE), ls + k);
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
     }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    int at = incl - v, all = 0;
+#pragma unroll
+    for (int j = 0; j < EM_NT / 32; ++j) {
+        if (j < warp) at += sums[j];
+        all += sums[j];
+    }
+    __syncthreads();
+    *total = all;
+    return at;
+}
+// A CTA per bin: where its ids' positions start.
+__global__ void __launch_bounds__(EM_NT) embed_scan_kernel(int64_t vocab, EmbedSort e) {
+    pdl_wait_then_release();
+    int mine = 0, start;
+    for (int j = threadIdx.x; j < (int)blockIdx.x; j += EM_NT) mine += e.bin[j];
+    em_scan(mine, &start);
+    const int64_t first = (int64_t)blockIdx.x << e.shift, end = min(vocab, first + ((int64_t)1 << e.shift));
+    for (int64_t v0 = first; v0 < end; v0 += 4 * EM_NT) {
+        const int64_t v = v0 + 4 * threadIdx.x;  // count and base are padded to whole vectors
+        int4 c = make_int4(0, 0, 0, 0);
+        if (v < end) c = *reinterpret_cast<const int4*>(e.count + v);
+        int all;
+        const int at = start + em_scan(c.x + c.y + c.z + c.w, &all);
+        if (v < end) *reinterpret_cast<int4*>(e.base + v) = make_int4(at, at + c.x, at + c.x + c.y, at + c.x + c.y + c.z);
+        start += all;
+    }
+    if ((int)blockIdx.x == e.bins - 1 && threadIdx.x == 0) *e.total = start;
 }
 
 __global__ void __launch_bounds__(EM_NT) embed_scatter_kernel(const int64_t* tokens, int n, EmbedSort e) {
@@ -218,21 +242,49 @@ __global__ void __launch_bounds__(EM_NT) embed_scatter_kernel(const int64_t* tok
     e.loose[e.base[tokens[i]] + e.place[i]] = i;
 }
 
-// Each id's positions in ascending order.  Up to EM_SHORT of them: a place's rank by comparison with the others.  More: the
-// CTA that has the range's first place marks them in a bitmap, EM_WINDOW positions at a time, and reads it in order.
-constexpr int EM_SHORT = 64;
-__global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* tokens, int n, EmbedSort e) {
+// The first `orders` CTAs put each id's positions in ascending order.  Up to EM_SHORT of them: a place's rank by comparison with
+// the others.  More: the CTA that has the first place marks them in a bitmap, EM_WINDOW positions at a time, and reads it in
+// order.  The other CTAs write zeros for the ids that do not occur, a warp per EM_ZERO bytes of a row.
+constexpr int EM_SHORT = 64, EM_ZERO = 8192;
+__global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* tokens, int n, int64_t vocab, int64_t row_bytes,
+                                                            int64_t zeros, int orders, unsigned char* out, int e_bytes,
+                                                            EmbedSort e) {
     __shared__ uint32_t bits[EM_WINDOW / 32];
-    __shared__ int warp_sum[EM_NT / 32], longs[EM_NT / EM_SHORT + 1], found;
+    __shared__ int longs[EM_NT / EM_SHORT + 1], found;
     pdl_wait_then_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int k = blockIdx.x * EM_NT + tid, all = e.next[0];
+    if ((int)blockIdx.x >= orders) {
+        const int64_t w = (int64_t)(blockIdx.x - orders) * (EM_NT / 32) + warp, v = w / zeros;
+        if (v >= vocab || e.count[v]) return;
+        unsigned char* p = out + v * row_bytes + w % zeros * EM_ZERO;
+        unsigned char* end = out + v * row_bytes + min(row_bytes, (w % zeros + 1) * EM_ZERO);
+        unsigned char* a = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p) + 15) & ~(uintptr_t)15);
+        unsigned char* z = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(end) & ~(uintptr_t)15);
+        const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+        if (a < z) {
+#pragma unroll 4
+            for (unsigned char* q = a + 16 * lane; q < z; q += 512) __stcs(reinterpret_cast<uint4*>(q), none);
+        } else {
+            a = z = end;
+        }
+        // the ends that are not whole vectors, in elements
+        for (unsigned char* q = p + (int64_t)lane * e_bytes; q < a; q += 32 * e_bytes)
+            if (e_bytes == 4) *reinterpret_cast<uint32_t*>(q) = 0;
+            else *reinterpret_cast<unsigned short*>(q) = 0;
+        for (unsigned char* q = z + (int64_t)lane * e_bytes; q < end; q += 32 * e_bytes)
+            if (e_bytes == 4) *reinterpret_cast<uint32_t*>(q) = 0;
+            else *reinterpret_cast<unsigned short*>(q) = 0;
+        return;
+    }
+    const int64_t k = (int64_t)blockIdx.x * EM_NT + tid;
     if (tid == 0) found = 0;
     __syncthreads();
-    if (k < all) {
+    if (k < *e.total) {
         const int i = e.loose[k], t = (int)tokens[i], c = e.count[t], b = e.base[t];
+        e.id[k] = t;
         if (c <= EM_SHORT) {
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < c; ++j) rank += e.loose[b + j] < i;
             e.order[b + rank] = i;
         } else if (b == k) {
@@ -252,102 +304,143 @@ __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* token
                 if (i >= 0 && i < EM_WINDOW) atomicOr(&bits[i >> 5], 1u << (i & 31));
             }
             __syncthreads();
-            int mine = 0;
+            int mine = 0, all;
             for (int j = tid * per; j < min(words, (tid + 1) * per); ++j) mine += __popc(bits[j]);
-            int incl = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += u;
-            }
-            if (lane == 31) warp_sum[warp] = incl;
-            __syncthreads();
-            int at = b + done + incl - mine, total = 0;
-            for (int j = 0; j < EM_NT / 32; ++j) {
-                if (j < warp) at += warp_sum[j];
-                total += warp_sum[j];
-            }
+            int at = b + done + em_scan(mine, &all);
             for (int j = tid * per; j < min(words, (tid + 1) * per); ++j)
                 for (uint32_t m = bits[j]; m; m &= m - 1) e.order[at++] = (int)w0 + 32 * j + __ffs(m) - 1;
-            done += total;
+            done += all;
             __syncthreads();
         }
     }
 }
 
-// grid: first a warp per piece and part of a row (`warps` of them), then a warp per id and part that writes zeros for the
-// ids that do not occur.
+// A warp per chunk and part of a row.
+constexpr int EM_ROWS = 4;  // rows in flight
 template <int E, bool VEC>
-__global__ void __launch_bounds__(EM_NT) embed_sum_kernel(const void* grad, int64_t row_bytes, int n, int64_t vocab,
-                                                          int64_t units, int64_t pieces, float s, void* out, EmbedSort e) {
+__global__ void __launch_bounds__(EM_NT) embed_sum_kernel(const void* grad, int64_t row_bytes, int64_t units, int parts, float s,
+                                                          void* out, EmbedSort e) {
     constexpr int N = Unit<E, VEC>::N, W = EM_UNITS / 32;
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31;
-    int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5);
-    const int64_t i = w / pieces, u0 = (w % pieces) * EM_UNITS + lane;
+    const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), chunk = w / parts;
+    const int part = (int)(w % parts), total = *e.total;
+    const int64_t u0 = (int64_t)part * EM_UNITS + lane, width = units * N, k0 = chunk * EM_CHUNK;
+    if (k0 >= total) return;
+    const int held = (int)min((int64_t)EM_CHUNK, total - k0);
+    const int pos = lane < held ? e.order[k0 + lane] : 0, id = lane < held ? e.id[k0 + lane] : -1;
+    const int before = k0 ? e.id[k0 - 1] : -1, after = k0 + held < total ? e.id[k0 + held] : -1;
+    const int next = __shfl_down_sync(0xffffffffu, id, 1);
+    const uint32_t ends = __ballot_sync(0xffffffffu, lane < held && (lane == held - 1 || next != id));  // last rows of ids
+    const int first_id = __shfl_sync(0xffffffffu, id, 0), last_id = __shfl_sync(0xffffffffu, id, held - 1);
+    const bool from = first_id == before, on = last_id == after;  // an id from the chunk before, one that goes on
     Unit<E, VEC> sum[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) sum[j].zero();
-    if (i >= n) {
-        const int64_t v = i - n;
-        if (v >= vocab || e.count[v]) return;
-        unsigned char* dst = static_cast<unsigned char*>(out) + v * units * N * E;
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-            if (u0 + 32 * j < units) sum[j].store(dst, u0 + 32 * j, 0.0f);
-        return;
-    }
-    if (i >= e.next[1]) return;
-    const int4 p = e.piece[i];
-    const int mine = lane < p.z ? e.order[p.y + lane] : 0;
-#pragma unroll 2
-    for (int k = 0; k < p.z; ++k) {
-        const unsigned char* src = static_cast<const unsigned char*>(grad) + __shfl_sync(0xffffffffu, mine, k) * row_bytes;
-        Unit<E, VEC> g[W];
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            g[j].zero();
-            if (u0 + 32 * j < units) g[j].load(src, u0 + 32 * j);
-        }
-#pragma unroll
-        for (int j = 0; j < W; ++j) sum[j].add(g[j]);
-    }
-    if (p.w < 0) {
-        unsigned char* dst = static_cast<unsigned char*>(out) + p.x * units * N * E;
+    auto write = [&](int64_t to) {
+        unsigned char* dst = static_cast<unsigned char*>(out) + to * width * E;
 #pragma unroll
         for (int j = 0; j < W; ++j)
             if (u0 + 32 * j < units) sum[j].store(dst, u0 + 32 * j, s);
-    } else {
-        float* dst = e.sums + p.w * units * N;
+    };
+    auto keep = [&](int64_t slot) {
 #pragma unroll
         for (int j = 0; j < W; ++j)
-            if (u0 + 32 * j < units)
+            if (u0 + 32 * j < units) {
+                float* q = e.sums + slot * width + (u0 + 32 * j) * N;
+                if constexpr (VEC) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) dst[(u0 + 32 * j) * N + k] = sum[j].v[k];
+                    for (int k = 0; k < N; k += 4)
+                        __stcg(reinterpret_cast<float4*>(q + k), make_float4(sum[j].v[k], sum[j].v[k + 1], sum[j].v[k + 2], sum[j].v[k + 3]));
+                } else {
+                    __stcg(q, sum[j].v[0]);
+                }
+            }
+    };
+    int start = 0;  // of the id being summed
+#pragma unroll 1
+    for (int k = 0; k < held; k += EM_ROWS) {
+        RawUnit<E, VEC> g[EM_ROWS][W];
+#pragma unroll
+        for (int r = 0; r < EM_ROWS; ++r) {
+            const unsigned char* src = static_cast<const unsigned char*>(grad) + __shfl_sync(0xffffffffu, pos, (k + r) & 31) * row_bytes;
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (k + r < held && u0 + 32 * j < units) g[r][j].load(src, u0 + 32 * j);
+        }
+#pragma unroll
+        for (int r = 0; r < EM_ROWS; ++r) {
+            if (k + r >= held) break;
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (u0 + 32 * j < units) sum[j].add(g[r][j]);
+            if (ends >> (k + r) & 1) {
+                const bool goes = on && k + r == held - 1, came = from && start == 0;
+                if (goes || came) keep(2 * chunk + (came ? 0 : 1));
+                else write(__shfl_sync(0xffffffffu, id, k + r));
+#pragma unroll
+                for (int j = 0; j < W; ++j) sum[j].zero();
+                start = k + r + 1;
+            }
+        }
     }
-}
-
-// The ids with several pieces: their sums added in order.  grid: (parts of a row of EM_NT columns, ids).
-template <int E>
-__global__ void __launch_bounds__(EM_NT) embed_join_kernel(int64_t width, float s, void* out, EmbedSort e) {
-    pdl_wait_then_release();
-    const int64_t col = (int64_t)blockIdx.x * EM_NT + threadIdx.x;
-    const int ids = e.next[2];
-    if (col >= width) return;
-    for (int k = blockIdx.y; k < ids; k += gridDim.y) {
-        const int4 p = e.split[k];
-        float v = 0.0f;
-#pragma unroll 8
-        for (int j = 0; j < p.z; ++j) v += e.sums[(int64_t)(p.y + j) * width + col];
-        const int64_t at = p.x * width + col;
-        if (E == 4) static_cast<float*>(out)[at] = v * s;
-        else static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v * s);
+    if (!from && !on) return;
+    auto last = [&](int64_t counter, int of) {  // whether this warp is the last of `of` to get here
+        __threadfence();
+        __syncwarp();
+        int there = 0;
+        if (lane == 0) there = atomicAdd(e.arrived + counter * parts + part, 1);
+        there = __shfl_sync(0xffffffffu, there, 0);
+        __threadfence();
+        return there == of - 1;
+    };
+    // An id's sums lie with its chunks from c0 on, in the first one's second place and the others' first.  They are added in
+    // order, EM_JOIN at a time and then the groups', so that which warp it is that completes them does not matter.
+#pragma unroll 1
+    for (int both = 0; both < 2; ++both) {
+        if (both ? !on || (from && first_id == last_id) : !from) continue;  // a chunk of one id has one sum
+        const int t = both ? last_id : first_id, b = e.base[t], c0 = b / EM_CHUNK, of = (b + e.count[t] - 1) / EM_CHUNK - c0 + 1;
+        auto slot = [&](int j) { return 2 * (int64_t)(c0 + j) + (j ? 0 : 1); };
+        auto join = [&](int j0, int count, int apart) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum[j].zero();
+#pragma unroll 4
+            for (int k = 0; k < count; ++k) {
+                const float* q = e.sums + slot(j0 + k * apart) * width;
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (u0 + 32 * j < units) {
+                        if constexpr (VEC) {
+#pragma unroll
+                            for (int c = 0; c < N; c += 4) {
+                                const float4 v = __ldcg(reinterpret_cast<const float4*>(q + (u0 + 32 * j) * N + c));
+                                sum[j].v[c] += v.x;
+                                sum[j].v[c + 1] += v.y;
+                                sum[j].v[c + 2] += v.z;
+                                sum[j].v[c + 3] += v.w;
+                            }
+                        } else {
+                            sum[j].v[0] += __ldcg(q + u0 + 32 * j);
+                        }
+                    }
+            }
+        };
+        const int group = ((int)chunk - c0) / EM_JOIN * EM_JOIN, groups = (of + EM_JOIN - 1) / EM_JOIN, in = min(EM_JOIN, of - group);
+        if (!last(slot(group), in)) continue;
+        join(group, in, 1);
+        if (groups > 1) {
+            keep(slot(group));  // in the first one's place, which nobody reads again
+            if (!last(e.slots + slot(0), groups)) continue;
+            join(0, groups, EM_JOIN);
+        }
+        write(t);
     }
 }
 
 int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
-
-// The workspace's arrays, and its bytes.
+int64_t parts_of(int64_t units) { return (units + EM_UNITS - 1) / EM_UNITS; }
+// The workspace's arrays, and its bytes, `zeroed` of them to be zero; the parts of a row are those of single elements, where rows
+// may be unaligned.
 int64_t embed_layout(int64_t n, int64_t vocab, int64_t width, unsigned char* at, EmbedSort* e, int64_t* zeroed) {
     int64_t used = 0;
     auto take = [&](int64_t bytes) {
@@ -355,16 +448,21 @@ int64_t embed_layout(int64_t n, int64_t vocab, int64_t width, unsigned char* at,
         used += up(bytes, 256);
         return p;
     };
-    e->next = reinterpret_cast<int*>(take(16));
-    e->count = reinterpret_cast<int*>(take(vocab * 4));
+    e->slots = (int)(2 * ((n + EM_CHUNK - 1) / EM_CHUNK));
+    e->shift = 10;  // bins of 1024 ids, or as many as make EM_BINS
+    while ((vocab - 1) >> e->shift >= EM_BINS) ++e->shift;
+    e->bins = (int)(((vocab - 1) >> e->shift) + 1);
+    e->count = reinterpret_cast<int*>(take(up(vocab, 4) * 4));
+    e->bin = reinterpret_cast<int*>(take((int64_t)e->bins * 4));
+    e->arrived = reinterpret_cast<int*>(take(2 * (int64_t)e->slots * parts_of(width) * 4));
     *zeroed = used;
-    e->base = reinterpret_cast<int*>(take(vocab * 4));
+    e->total = reinterpret_cast<int*>(take(4));
+    e->base = reinterpret_cast<int*>(take(up(vocab, 4) * 4));
     e->place = reinterpret_cast<int*>(take(n * 4));
     e->loose = reinterpret_cast<int*>(take(n * 4));
     e->order = reinterpret_cast<int*>(take(n * 4));
-    e->piece = reinterpret_cast<int4*>(take(n * 16));
-    e->split = reinterpret_cast<int4*>(take((n / EM_PIECE + 1) * 16));
-    e->sums = reinterpret_cast<float*>(take(2 * (n / EM_PIECE) * width * 4));
+    e->id = reinterpret_cast<int*>(take(n * 4));
+    e->sums = reinterpret_cast<float*>(take((int64_t)e->slots * width * 4));
     return used;
 }
 
@@ -455,26 +553,25 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
         workspace_bytes < embed_layout(n, vocab, width, static_cast<unsigned char*>(workspace), &s, &zeroed))
         return B2S_ERR_INVALID;
     const bool vec = aligned16(grad_out) && aligned16(grad_table) && (int64_t)width * e % 16 == 0 && grad_row_stride * e % 16 == 0;
-    const int64_t units = vec ? (int64_t)width * e / 16 : width, pieces = (units + EM_UNITS - 1) / EM_UNITS;
-    const unsigned blocks = blocks_of(((int64_t)n + vocab) * pieces), per = (unsigned)(((int64_t)n + EM_NT - 1) / EM_NT);
-    if (!blocks) return B2S_ERR_UNSUPPORTED;
+    const int64_t units = vec ? (int64_t)width * e / 16 : width, parts = parts_of(units);
+    const int64_t row_bytes = (int64_t)width * e, zeros = (row_bytes + EM_ZERO - 1) / EM_ZERO;
+    const unsigned per = (unsigned)(((int64_t)n + EM_NT - 1) / EM_NT);
+    const unsigned blocks = blocks_of(((int64_t)n + EM_CHUNK - 1) / EM_CHUNK * parts), zero_blocks = blocks_of(vocab * zeros);
+    if (!blocks || !zero_blocks || (int64_t)zero_blocks + per > 0x7fffffff) return B2S_ERR_UNSUPPORTED;
     cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
     if (r == cudaSuccess) r = launch_pdl(embed_count_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s);
-    if (r == cudaSuccess) r = launch_pdl(embed_range_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, s);
+    if (r == cudaSuccess) r = launch_pdl(embed_scan_kernel, dim3((unsigned)s.bins), EM_NT, 0, stream, (int64_t)vocab, s);
     if (r == cudaSuccess) r = launch_pdl(embed_scatter_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, s);
-    if (r == cudaSuccess) r = launch_pdl(embed_order_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, s);
+    if (r == cudaSuccess)
+        r = launch_pdl(embed_order_kernel, dim3(zero_blocks + per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, row_bytes, zeros,
+                       (int)per, static_cast<unsigned char*>(grad_table), e, s);
     if (r != cudaSuccess) return cuda_fail(r);
     auto sum = [&](auto kernel) {
-        return launch_pdl(kernel, dim3(blocks), EM_NT, 0, stream, grad_out, grad_row_stride * e, (int)n, (int64_t)vocab, units,
-                          pieces, scale, grad_table, s);
+        return launch_pdl(kernel, dim3(blocks), EM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts, scale,
+                          grad_table, s);
     };
     r = e == 4 ? (vec ? sum(embed_sum_kernel<4, true>) : sum(embed_sum_kernel<4, false>))
                : (vec ? sum(embed_sum_kernel<2, true>) : sum(embed_sum_kernel<2, false>));
-    if (r == cudaSuccess && n > EM_PIECE) {
-        const dim3 grid((unsigned)((width + EM_NT - 1) / EM_NT), (unsigned)(n / EM_PIECE < 64 ? n / EM_PIECE : 64));
-        auto join = [&](auto kernel) { return launch_pdl(kernel, grid, EM_NT, 0, stream, (int64_t)width, scale, grad_table, s); };
-        r = e == 4 ? join(embed_join_kernel<4>) : join(embed_join_kernel<2>);
-    }
     return r == cudaSuccess ? B2S_OK : cuda_fail(r);
 }
 
