@@ -9,7 +9,7 @@
 // and one read of the rows' gradients.  The positions are sorted by id without a sort of keys: a count per id (the atomic's
 // old value is the position's place among its id's, in order of arrival), the counts' prefix sums, and then each id's
 // positions put in ascending order, so that sums do not depend on who arrived first.  The sorted positions are summed in
-// chunks of EM_CHUNK, whatever ids they hold, one chunk a warp and part of a row, in order, in fp32: an id inside a chunk is
+// chunks of 8 to 32, whatever ids they hold, one chunk a warp and part of a row, in order, in fp32: an id inside a chunk is
 // written at once, of one that goes on the sums are joined by whoever completes them, in order.
 #include <string.h>
 
@@ -27,8 +27,8 @@ int cuda_fail(cudaError_t e);
 namespace {
 
 constexpr int EM_NT = 256;
-constexpr int EM_CHUNK = 32;   // sorted positions that a warp sums
 constexpr int EM_JOIN = 16;    // sums joined at a time
+constexpr int EM_SHORT = 64;   // positions of an id that are put in order by comparison
 constexpr int EM_BINS = 4096;  // at most, of ids counted together
 constexpr int EM_UNITS = 64;   // 16-byte units (or elements) of a row that a warp takes
 constexpr int EM_WINDOW = 1 << 17;  // positions that a CTA's bitmap covers (16 KB)
@@ -103,16 +103,16 @@ __device__ __forceinline__ int64_t token_at(const int64_t* tokens, int64_t i, in
     return t < 0 ? -1 : t;
 }
 
-// grid: a warp per row and piece of EM_UNITS units
+// grid: a warp per row and part of EM_UNITS units (128 units a warp: 30001 x 768 fp32 21 us either way; 32: 26)
 template <int E, bool VEC>
 __global__ void __launch_bounds__(EM_NT) embed_kernel(const int64_t* tokens, int64_t n, const void* table,
-                                                      int64_t row_bytes, int64_t vocab, int64_t units, int64_t pieces, float s,
+                                                      int64_t row_bytes, int64_t vocab, int64_t units, int64_t parts, float s,
                                                       void* out, uint32_t* status) {
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), i = w / pieces, u0 = (w % pieces) * EM_UNITS + lane;
+    const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), i = w / parts, u0 = (w % parts) * EM_UNITS + lane;
     if (i >= n) return;
-    const int64_t t = token_at(tokens, i, vocab, lane == 0 && u0 == 0 ? status : nullptr);
+    const int64_t t = token_at(tokens, i, vocab, u0 == 0 ? status : nullptr);
     const unsigned char* src = static_cast<const unsigned char*>(table) + (t < 0 ? 0 : t) * row_bytes;
     unsigned char* dst = static_cast<unsigned char*>(out) + i * units * Unit<E, VEC>::N * E;
     RawUnit<E, VEC> q[EM_UNITS / 32];
@@ -170,7 +170,9 @@ struct EmbedSort {
     int* count;    // [vocab] positions of an id
     int* bin;      // [bins] positions of 1 << shift ids
     int* arrived;  // [2][slots][parts] sums that are there, of a group (at its first) and groups of an id (at its first)
+    int* longs;    // how many ids have more than EM_SHORT positions
     int* total;    // positions that are not padding
+    int* long_id;  // [n / EM_SHORT] which
     int* base;     // [vocab] where an id's positions start, sorted
     int* place;    // [n] among the id's positions in order of arrival; -1: none
     int* loose;    // [n] positions by id, in order of arrival
@@ -178,6 +180,7 @@ struct EmbedSort {
     int* id;       // [n] their ids
     float* sums;   // [slots][width]: two for each chunk, of the id that came from the one before and of the last one, that goes on
     int slots, shift, bins;
+    int chunk;     // sorted positions that a warp sums, as a power of two: 8, 16 or 32
 };
 
 __global__ void __launch_bounds__(EM_NT) embed_count_kernel(const int64_t* tokens, int n, int64_t vocab, EmbedSort e) {
@@ -230,6 +233,12 @@ __global__ void __launch_bounds__(EM_NT) embed_scan_kernel(int64_t vocab, EmbedS
         int all;
         const int at = start + em_scan(c.x + c.y + c.z + c.w, &all);
         if (v < end) *reinterpret_cast<int4*>(e.base + v) = make_int4(at, at + c.x, at + c.x + c.y, at + c.x + c.y + c.z);
+        if (max(max(c.x, c.y), max(c.z, c.w)) > EM_SHORT) {  // in any order: each is put in order by itself
+            if (c.x > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v;
+            if (c.y > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v + 1;
+            if (c.z > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v + 2;
+            if (c.w > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v + 3;
+        }
         start += all;
     }
     if ((int)blockIdx.x == e.bins - 1 && threadIdx.x == 0) *e.total = start;
@@ -242,19 +251,56 @@ __global__ void __launch_bounds__(EM_NT) embed_scatter_kernel(const int64_t* tok
     e.loose[e.base[tokens[i]] + e.place[i]] = i;
 }
 
-// The first `orders` CTAs put each id's positions in ascending order.  Up to EM_SHORT of them: a place's rank by comparison with
-// the others.  More: the CTA that has the first place marks them in a bitmap, EM_WINDOW positions at a time, and reads it in
-// order.  The other CTAs write zeros for the ids that do not occur, a warp per EM_ZERO bytes of a row.
-constexpr int EM_SHORT = 64, EM_ZERO = 8192;
+// All of that for up to EM_FEW positions in one launch: a position's place is how many come before it by (id, position), found by
+// comparison with all, 8 lanes a position (four launches instead of six).
+constexpr int EM_FEW = 4096;
+__global__ void __launch_bounds__(EM_NT) embed_rank_kernel(const int64_t* tokens, int n, int64_t vocab, EmbedSort e) {
+    __shared__ int ids[EM_FEW];
+    pdl_wait_then_release();
+    int real = 0;
+    for (int j = threadIdx.x; j < n; j += EM_NT) {
+        const int t = (int)token_at(tokens, j, vocab, nullptr);
+        ids[j] = t < 0 ? 0x7fffffff : t;  // behind all others, equal to none
+        real += t >= 0;
+    }
+    int all;
+    em_scan(real, &all);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *e.total = all;
+    const int i = blockIdx.x * (EM_NT / 8) + (threadIdx.x >> 3), t = i < n ? ids[i] : 0x7fffffff;
+    int before = 0, lower = 0, same = 0;
+    for (int j = threadIdx.x & 7; j < n; j += 8) {
+        const int o = ids[j];
+        lower += o < t;
+        same += o == t;
+        before += o == t && j < i;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        lower += __shfl_xor_sync(0xffffffffu, lower, o);
+        same += __shfl_xor_sync(0xffffffffu, same, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if ((threadIdx.x & 7) || t == 0x7fffffff) return;
+    e.order[lower + before] = i;
+    e.id[lower + before] = t;
+    if (before == 0) {
+        e.base[t] = lower;
+        e.count[t] = same;
+    }
+}
+
+// The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order: marked in a bitmap,
+// EM_WINDOW positions at a time, and read from it.  The next `orders` CTAs do the others', a place's rank by comparison with the
+// id's other places.  The last ones write zeros for the ids that do not occur, a warp per EM_ZERO bytes of a row.
+constexpr int EM_ZERO = 8192;
 __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* tokens, int n, int64_t vocab, int64_t row_bytes,
-                                                            int64_t zeros, int orders, unsigned char* out, int e_bytes,
+                                                            int64_t zeros, int longs, int orders, unsigned char* out, int e_bytes,
                                                             EmbedSort e) {
     __shared__ uint32_t bits[EM_WINDOW / 32];
-    __shared__ int longs[EM_NT / EM_SHORT + 1], found;
     pdl_wait_then_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if ((int)blockIdx.x >= orders) {
-        const int64_t w = (int64_t)(blockIdx.x - orders) * (EM_NT / 32) + warp, v = w / zeros;
+    if ((int)blockIdx.x >= longs + orders) {
+        const int64_t w = (int64_t)(blockIdx.x - longs - orders) * (EM_NT / 32) + warp, v = w / zeros;
         if (v >= vocab || e.count[v]) return;
         unsigned char* p = out + v * row_bytes + w % zeros * EM_ZERO;
         unsigned char* end = out + v * row_bytes + min(row_bytes, (w % zeros + 1) * EM_ZERO);
@@ -276,24 +322,20 @@ __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* token
             else *reinterpret_cast<unsigned short*>(q) = 0;
         return;
     }
-    const int64_t k = (int64_t)blockIdx.x * EM_NT + tid;
-    if (tid == 0) found = 0;
-    __syncthreads();
-    if (k < *e.total) {
+    if ((int)blockIdx.x >= longs) {
+        const int64_t k = (int64_t)(blockIdx.x - longs) * EM_NT + tid;
+        if (k >= *e.total) return;
         const int i = e.loose[k], t = (int)tokens[i], c = e.count[t], b = e.base[t];
         e.id[k] = t;
-        if (c <= EM_SHORT) {
-            int rank = 0;
-#pragma unroll 4
-            for (int j = 0; j < c; ++j) rank += e.loose[b + j] < i;
-            e.order[b + rank] = i;
-        } else if (b == k) {
-            longs[atomicAdd(&found, 1)] = t;
-        }
+        if (c > EM_SHORT) return;
+        int rank = 0;
+#pragma unroll 16
+        for (int j = 0; j < c; ++j) rank += e.loose[b + j] < i;
+        e.order[b + rank] = i;
+        return;
     }
-    __syncthreads();
-    for (int f = 0; f < found; ++f) {
-        const int t = longs[f], c = e.count[t], b = e.base[t];
+    for (int f = blockIdx.x; f < *e.longs; f += longs) {
+        const int t = e.long_id[f], c = e.count[t], b = e.base[t];
         int done = 0;
         for (int64_t w0 = 0; w0 < n && done < c; w0 += EM_WINDOW) {
             const int words = ((int)min((int64_t)EM_WINDOW, n - w0) + 31) / 32, per = (words + EM_NT - 1) / EM_NT;
@@ -325,9 +367,9 @@ __global__ void __launch_bounds__(EM_NT) embed_sum_kernel(const void* grad, int6
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), chunk = w / parts;
     const int part = (int)(w % parts), total = *e.total;
-    const int64_t u0 = (int64_t)part * EM_UNITS + lane, width = units * N, k0 = chunk * EM_CHUNK;
+    const int64_t u0 = (int64_t)part * EM_UNITS + lane, width = units * N, k0 = chunk << e.chunk;
     if (k0 >= total) return;
-    const int held = (int)min((int64_t)EM_CHUNK, total - k0);
+    const int held = (int)min((int64_t)1 << e.chunk, total - k0);
     const int pos = lane < held ? e.order[k0 + lane] : 0, id = lane < held ? e.id[k0 + lane] : -1;
     const int before = k0 ? e.id[k0 - 1] : -1, after = k0 + held < total ? e.id[k0 + held] : -1;
     const int next = __shfl_down_sync(0xffffffffu, id, 1);
@@ -399,7 +441,7 @@ __global__ void __launch_bounds__(EM_NT) embed_sum_kernel(const void* grad, int6
 #pragma unroll 1
     for (int both = 0; both < 2; ++both) {
         if (both ? !on || (from && first_id == last_id) : !from) continue;  // a chunk of one id has one sum
-        const int t = both ? last_id : first_id, b = e.base[t], c0 = b / EM_CHUNK, of = (b + e.count[t] - 1) / EM_CHUNK - c0 + 1;
+        const int t = both ? last_id : first_id, b = e.base[t], c0 = b >> e.chunk, of = ((b + e.count[t] - 1) >> e.chunk) - c0 + 1;
         auto slot = [&](int j) { return 2 * (int64_t)(c0 + j) + (j ? 0 : 1); };
         auto join = [&](int j0, int count, int apart) {
 #pragma unroll
@@ -448,15 +490,19 @@ int64_t embed_layout(int64_t n, int64_t vocab, int64_t width, unsigned char* at,
         used += up(bytes, 256);
         return p;
     };
-    e->slots = (int)(2 * ((n + EM_CHUNK - 1) / EM_CHUNK));
+    // 32 positions a warp, fewer where there would be few warps (2048 x 768 of 6562 ids: 26 against 21 us)
+    e->chunk = n * width <= 1 << 22 ? 3 : n * width <= 1 << 24 ? 4 : 5;
+    e->slots = (int)(2 * (((n - 1) >> e->chunk) + 1));
     e->shift = 10;  // bins of 1024 ids, or as many as make EM_BINS
     while ((vocab - 1) >> e->shift >= EM_BINS) ++e->shift;
     e->bins = (int)(((vocab - 1) >> e->shift) + 1);
     e->count = reinterpret_cast<int*>(take(up(vocab, 4) * 4));
     e->bin = reinterpret_cast<int*>(take((int64_t)e->bins * 4));
     e->arrived = reinterpret_cast<int*>(take(2 * (int64_t)e->slots * parts_of(width) * 4));
+    e->longs = reinterpret_cast<int*>(take(4));
     *zeroed = used;
     e->total = reinterpret_cast<int*>(take(4));
+    e->long_id = reinterpret_cast<int*>(take(n / EM_SHORT * 4));
     e->base = reinterpret_cast<int*>(take(up(vocab, 4) * 4));
     e->place = reinterpret_cast<int*>(take(n * 4));
     e->loose = reinterpret_cast<int*>(take(n * 4));
@@ -556,15 +602,23 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
     const int64_t units = vec ? (int64_t)width * e / 16 : width, parts = parts_of(units);
     const int64_t row_bytes = (int64_t)width * e, zeros = (row_bytes + EM_ZERO - 1) / EM_ZERO;
     const unsigned per = (unsigned)(((int64_t)n + EM_NT - 1) / EM_NT);
-    const unsigned blocks = blocks_of(((int64_t)n + EM_CHUNK - 1) / EM_CHUNK * parts), zero_blocks = blocks_of(vocab * zeros);
-    if (!blocks || !zero_blocks || (int64_t)zero_blocks + per > 0x7fffffff) return B2S_ERR_UNSUPPORTED;
+    const unsigned blocks = blocks_of((((int64_t)n - 1 >> s.chunk) + 1) * parts), zero_blocks = blocks_of(vocab * zeros);
+    if (!blocks || !zero_blocks || (int64_t)zero_blocks + per + 1024 > 0x7fffffff) return B2S_ERR_UNSUPPORTED;
     cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
-    if (r == cudaSuccess) r = launch_pdl(embed_count_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s);
-    if (r == cudaSuccess) r = launch_pdl(embed_scan_kernel, dim3((unsigned)s.bins), EM_NT, 0, stream, (int64_t)vocab, s);
-    if (r == cudaSuccess) r = launch_pdl(embed_scatter_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, s);
+    const bool few = n <= EM_FEW;
+    if (few) {
+        if (r == cudaSuccess)
+            r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / 8 - 1) / (EM_NT / 8))), EM_NT, 0, stream, tokens, (int)n,
+                           (int64_t)vocab, s);
+    } else {
+        if (r == cudaSuccess) r = launch_pdl(embed_count_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s);
+        if (r == cudaSuccess) r = launch_pdl(embed_scan_kernel, dim3((unsigned)s.bins), EM_NT, 0, stream, (int64_t)vocab, s);
+        if (r == cudaSuccess) r = launch_pdl(embed_scatter_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, s);
+    }
+    const unsigned orders = few ? 0 : per, most = 2 * (unsigned)sms_here(), longs = few ? 0 : n / EM_SHORT < (int)most ? n / EM_SHORT : most;
     if (r == cudaSuccess)
-        r = launch_pdl(embed_order_kernel, dim3(zero_blocks + per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, row_bytes, zeros,
-                       (int)per, static_cast<unsigned char*>(grad_table), e, s);
+        r = launch_pdl(embed_order_kernel, dim3(zero_blocks + orders + longs), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, row_bytes,
+                       zeros, (int)longs, (int)orders, static_cast<unsigned char*>(grad_table), e, s);
     if (r != cudaSuccess) return cuda_fail(r);
     auto sum = [&](auto kernel) {
         return launch_pdl(kernel, dim3(blocks), EM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts, scale,
