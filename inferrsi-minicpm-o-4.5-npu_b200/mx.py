@@ -40,20 +40,25 @@ class MXTensor:
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
-        ts._need_cuda(codes, scales)
-        shape = tuple(int(s) for s in shape)
+        shape = torch.Size(shape)
         if not shape or shape[-1] < 1 or min(shape) < 0:
-            raise ValueError(f"shape must be [..., k] with k at least 1, got {shape}")
-        rows, k = 1, shape[-1]
-        for s in shape[:-1]:
-            rows *= s
+            raise ValueError(f"shape must be [..., k] with k at least 1, got {tuple(shape)}")
+        k, rows = shape[-1], shape[:-1].numel()
         for name, t, want in (("codes", codes, (rows, 16 * -(-k // BLOCK))),
                               ("scales", scales, (-(-rows // 128), -(-k // 256), 1024))):
-            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous() or t.data_ptr() % 16:
+            if not t.is_cuda:
+                ts._need_cuda(t)
+            if t.dtype is not torch.uint8 or t.shape != want or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} must be contiguous 16-byte aligned uint8 {list(want)}, got {t.dtype} {list(t.shape)}")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on one device")
-        self.codes, self.scales, self.shape = codes, scales, torch.Size(shape)
+        self.codes, self.scales, self.shape = codes, scales, shape
+
+    @classmethod
+    def _made(cls, codes: torch.Tensor, scales: torch.Tensor, shape: torch.Size) -> "MXTensor":
+        q = cls.__new__(cls)
+        q.codes, q.scales, q.shape = codes, scales, shape
+        return q
 
     @property
     def device(self) -> torch.device:
@@ -71,10 +76,9 @@ def quantize(x: torch.Tensor) -> MXTensor:
         raise ValueError(f"x must be float32 or bfloat16, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be [..., k] with k at least 1, got {tuple(x.shape)}")
-    x2 = x.detach()
+    x2 = x.detach() if x.requires_grad else x
     x2 = x2 if x2.dim() == 2 else x2.reshape(x.shape[:-1].numel(), x.shape[-1])
-    codes, scales = _native.ops().mx_quantize(x2)
-    return MXTensor(codes, scales, x.shape)
+    return MXTensor._made(*_native.ops().mx_quantize(x2), x.shape)
 
 
 def dequantize(q: MXTensor, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -83,7 +87,8 @@ def dequantize(q: MXTensor, *, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
         raise ValueError(f"q must be an MXTensor, got {type(q).__name__}")
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
-    return _native.ops().mx_dequantize(q.codes, q.scales, q.shape[-1], dtype).reshape(q.shape)
+    x = _native.ops().mx_dequantize(q.codes, q.scales, q.shape[-1], dtype)
+    return x if len(q.shape) == 2 else x.reshape(q.shape)
 
 
 def linear(x: Union[torch.Tensor, MXTensor], weight: MXTensor, bias: Optional[torch.Tensor] = None, *,
