@@ -678,7 +678,7 @@ cudaError_t linear_rows(const GemmArgs& a, const void* x, int64_t xs, const void
 constexpr int DZ_NT = 256;
 // Z8: z in microscaled 8 bits, `z_scale` its scales [blocks][rows]; else fp16.
 template <bool VEC, int ACT, bool Z8>
-__global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_t dy_stride, const void* z,
+__global__ void __launch_bounds__(DZ_NT, 4) linear_dz_kernel(const void* dy, int64_t dy_stride, const void* z,
                                                           int64_t z_stride, const uint8_t* z_scale, int rows, int N, int rows_per,
                                                           void* dz, int64_t dz_stride, float* part, void* db) {
     constexpr int E = 8;
@@ -733,7 +733,11 @@ __global__ void __launch_bounds__(DZ_NT) linear_dz_kernel(const void* dy, int64_
                     for (int j = 0; j < E; ++j) x[j] = preact_value((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
                 }
 #pragma unroll
-                for (int j = 0; j < E; ++j) g[j] *= n + j < N ? act_slope<ACT>(x[j]) : 0.0f;
+                for (int j = 0; j < E; j += 2) {
+                    const float2 d = act_slope_pair<ACT, Z8>(make_float2(x[j], x[j + 1]));
+                    g[j] *= n + j < N ? d.x : 0.0f;
+                    g[j + 1] *= n + j + 1 < N ? d.y : 0.0f;
+                }
             }
             if (dz) store8(static_cast<unsigned short*>(dz) + (int64_t)r * dz_stride + n, 0, N - n, true, g);
 #pragma unroll

@@ -141,6 +141,40 @@ __device__ __forceinline__ float act_slope(float z) {
     return 1.0f;
 }
 
+// The slopes of a pair, in packed arithmetic: act_slope's operations, one for one.  BOUNDED: finite pre-activations, of any size.
+template <int ACT, bool BOUNDED>
+__device__ __forceinline__ float2 act_slope_pair(float2 z) {
+    auto both = [](float x) { return make_float2(x, x); };
+    if constexpr (!BOUNDED) {
+        z.x = fabsf(z.x) > 6.0e4f ? copysignf(6.0e4f, z.x) : z.x;
+        z.y = fabsf(z.y) > 6.0e4f ? copysignf(6.0e4f, z.y) : z.y;
+    }
+    if (ACT == ACT_GELU) {
+        const float2 m = make_float2(fabsf(z.x), fabsf(z.y));
+        const float2 d = __ffma2_rn(both(0.363f), m, both(1.0f));
+        const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+        const float2 x = __fmul2_rn(__fmul2_rn(both(-0.72134752044448170f), m), m);
+        const float2 e = make_float2(ex2(x.x), ex2(x.y));
+        float2 p = both(0.096218183507f);
+        p = __ffma2_rn(p, t, both(-0.358431707466f));
+        p = __ffma2_rn(p, t, both(0.346512311336f));
+        p = __ffma2_rn(p, t, both(0.061501895887f));
+        p = __ffma2_rn(p, t, both(0.278014403086f));
+        p = __ffma2_rn(p, t, both(0.286393762026f));
+        p = __ffma2_rn(p, t, both(0.289791861116f));
+        const float2 q = __fmul2_rn(both(0.5f), __fmul2_rn(__fmul2_rn(p, t), e));
+        const float2 o = __fadd2_rn(both(1.0f), make_float2(-q.x, -q.y));
+        return __ffma2_rn(__fmul2_rn(both(0.398942280401432678f), z), e, make_float2(z.x > 0.0f ? o.x : q.x, z.y > 0.0f ? o.y : q.y));
+    }
+    if (ACT == ACT_SILU) {
+        const float2 x = __fmul2_rn(both(-1.44269504088896341f), z);
+        const float2 d = __fadd2_rn(both(1.0f), make_float2(ex2(x.x), ex2(x.y)));
+        const float2 s = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+        return __fmul2_rn(s, __ffma2_rn(z, __fadd2_rn(both(1.0f), make_float2(-s.x, -s.y)), both(1.0f)));
+    }
+    return make_float2(act_slope<ACT>(z.x), act_slope<ACT>(z.y));
+}
+
 // Shared-memory matrix descriptor of an operand with m (or n) contiguous, 128-byte swizzle: blocks of [64 k rows x 64
 // m], 8 KB each; leading offset = the next block of 64 m (bits 16-29), stride offset = the next 8 k rows (bits 32-45).
 __device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t saddr) {
