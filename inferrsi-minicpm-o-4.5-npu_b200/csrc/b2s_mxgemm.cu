@@ -184,70 +184,85 @@ __device__ __forceinline__ void turn_rows(unsigned char* st, uint32_t (&q)[16], 
     __syncwarp();
 }
 
-// The activations of pairs, in packed arithmetic: the operations of act_apply, one for one.
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The activations of pairs, in packed arithmetic, in as few operations as they take: with gelu, bias and residual the epilogue's
+// instructions are what a tile of 4096 k waits for.  gelu(z) = max(z, 0) - |z| q with act_apply's tail q = 1 - Phi(|z|) (its
+// polynomial halved); silu as there, e^z by halves.
 template <int ACT>
 __device__ __forceinline__ float2 act_pair(float2 z) {
-    auto both = [](float x) { return make_float2(x, x); };
-    const float2 m = make_float2(fabsf(z.x), fabsf(z.y));
+    // finite, so that infinity times the tail's zero is no NaN; NaN comes through z itself
+    const float2 m = make_float2(fminf(fabsf(z.x), 3.0e38f), fminf(fabsf(z.y), 3.0e38f));
     if (ACT == ACT_RELU) return make_float2(fmax_nan(z.x, 0.0f), fmax_nan(z.y, 0.0f));
     if (ACT == ACT_GELU) {
-        const float2 d = __ffma2_rn(both(0.363f), m, both(1.0f));
-        const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+        const float2 d = __ffma2_rn(both(0.363f), m, both(1.0f)), t = make_float2(rcp(d.x), rcp(d.y));
         const float2 x = __fmul2_rn(__fmul2_rn(both(-0.72134752044448170f), m), m);
-        float2 p = both(0.096218183507f);
-        p = __ffma2_rn(p, t, both(-0.358431707466f));
-        p = __ffma2_rn(p, t, both(0.346512311336f));
-        p = __ffma2_rn(p, t, both(0.061501895887f));
-        p = __ffma2_rn(p, t, both(0.278014403086f));
-        p = __ffma2_rn(p, t, both(0.286393762026f));
-        p = __ffma2_rn(p, t, both(0.289791861116f));
-        const float2 q = __fmul2_rn(both(0.5f), __fmul2_rn(__fmul2_rn(p, t), make_float2(ex2(x.x), ex2(x.y))));
-        const float2 o = __fadd2_rn(both(1.0f), make_float2(-q.x, -q.y));
-        return __fmul2_rn(z, make_float2(z.x > 0.0f ? o.x : q.x, z.y > 0.0f ? o.y : q.y));
+        float2 p = both(0.5f * 0.096218183507f);
+        p = __ffma2_rn(p, t, both(0.5f * -0.358431707466f));
+        p = __ffma2_rn(p, t, both(0.5f * 0.346512311336f));
+        p = __ffma2_rn(p, t, both(0.5f * 0.061501895887f));
+        p = __ffma2_rn(p, t, both(0.5f * 0.278014403086f));
+        p = __ffma2_rn(p, t, both(0.5f * 0.286393762026f));
+        p = __ffma2_rn(p, t, both(0.5f * 0.289791861116f));
+        const float2 q = __fmul2_rn(__fmul2_rn(p, t), make_float2(ex2(x.x), ex2(x.y)));
+        return __ffma2_rn(make_float2(-m.x, -m.y), q, make_float2(fmax_nan(z.x, 0.0f), fmax_nan(z.y, 0.0f)));
     }
     if (ACT == ACT_SILU) {
         const float2 x = __fmul2_rn(both(-0.72134752044448170f), m), h = make_float2(ex2(x.x), ex2(x.y));
         const float2 w = __fmul2_rn(__fmul2_rn(z, h), h), d = __ffma2_rn(h, h, both(1.0f));
-        return make_float2(__fdividef(z.x < 0.0f ? w.x : z.x, d.x), __fdividef(z.y < 0.0f ? w.y : z.y, d.y));
+        return __fmul2_rn(make_float2(z.x < 0.0f ? w.x : z.x, z.y < 0.0f ? w.y : z.y), make_float2(rcp(d.x), rcp(d.y)));
     }
     return z;
 }
 template <int ACT>
-__device__ __forceinline__ void act_row(float (&v)[32]) {
+__device__ __forceinline__ void act_row(float2 (&v)[16]) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-        const float2 y = act_pair<ACT>(make_float2(v[j], v[j + 1]));
-        v[j] = y.x;
-        v[j + 1] = y.y;
-    }
+    for (int j = 0; j < 16; ++j) v[j] = act_pair<ACT>(v[j]);
 }
+__device__ __forceinline__ float2 wide2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
 // This lane's row of 32 accumulated columns from n through the epilogue and to the output; rq: the residual's block.
-__device__ __forceinline__ void finish_block(const GemmArgs& a, float (&v)[32], uint32_t (&rq)[16], int row0, int n, unsigned char* st) {
+__device__ __forceinline__ void finish_block(const GemmArgs& a, const float (&acc)[32], uint32_t (&rq)[16], int row0, int n,
+                                             unsigned char* st) {
     const int lane = threadIdx.x & 31, rows = a.M - row0, cols = a.N - n;
     const unsigned short* bias = static_cast<const unsigned short*>(a.bias);
+    float2 v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = make_float2(acc[2 * j], acc[2 * j + 1]);
     if (bias) {
         if (cols >= 32 && (reinterpret_cast<uintptr_t>(bias) & 15) == 0) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint4 u = __ldg(reinterpret_cast<const uint4*>(bias + n) + j);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[8 * j + 2 * k] += __uint_as_float(w[k] << 16);
-                    v[8 * j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
-                }
+                v[4 * j] = __fadd2_rn(v[4 * j], wide2(u.x));
+                v[4 * j + 1] = __fadd2_rn(v[4 * j + 1], wide2(u.y));
+                v[4 * j + 2] = __fadd2_rn(v[4 * j + 2], wide2(u.z));
+                v[4 * j + 3] = __fadd2_rn(v[4 * j + 3], wide2(u.w));
             }
         } else {
             const float b = lane < cols ? bf16_bits_to_f(__ldg(bias + n + lane)) : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
+            for (int j = 0; j < 16; ++j)
+                v[j] = __fadd2_rn(v[j], make_float2(__shfl_sync(0xffffffffu, b, 2 * j), __shfl_sync(0xffffffffu, b, 2 * j + 1)));
         }
     }
     uint32_t w[16];
     if (a.preact) {
+        // as preact_bits, whose smallest positive value is asked for by the rectifier's slope alone
+        if (a.act == ACT_RELU) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = (uint32_t)preact_bits(v[2 * j]) | (uint32_t)preact_bits(v[2 * j + 1]) << 16;
+            for (int j = 0; j < 16; ++j) w[j] = (uint32_t)preact_bits(v[j].x) | (uint32_t)preact_bits(v[j].y) << 16;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const __half2 h = __floats2half2_rn(v[j].x, v[j].y);
+                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
         put_rows(st, w, static_cast<unsigned short*>(a.preact) + (int64_t)row0 * a.pre_stride + n, a.pre_stride, rows, cols,
                  vec_block(a, n, 1));
     }
@@ -257,13 +272,10 @@ __device__ __forceinline__ void finish_block(const GemmArgs& a, float (&v)[32], 
     if (a.residual) {
         turn_rows(st, rq, vec_block(a, n, a.res_vec));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            v[2 * j] += __uint_as_float(rq[j] << 16);
-            v[2 * j + 1] += __uint_as_float(rq[j] & 0xffff0000u);
-        }
+        for (int j = 0; j < 16; ++j) v[j] = __fadd2_rn(v[j], wide2(rq[j]));
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);  // the output's one rounding
+    for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[j].x, v[j].y);  // the output's one rounding
     put_rows(st, w, static_cast<unsigned short*>(a.out) + (int64_t)row0 * a.out_stride + n, a.out_stride, rows, cols,
              vec_block(a, n, a.out_vec));
 }

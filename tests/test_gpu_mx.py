@@ -67,6 +67,18 @@ def test_every_value_of_a_block(pkg):
     assert torch.equal(pkg.mx.dequantize(q, dtype=torch.float32).double(), _mx.four(x))
 
 
+def test_small_bf16_blocks(pkg):
+    """Blocks down to bf16's smallest numbers, whose scale is the smallest there is."""
+    g = gen(2)
+    x = torch.randn(300, 32, device=DEV, generator=g) * torch.exp2(torch.randint(-133, -115, (300, 1), device=DEV, generator=g).double()).float()
+    for v in (x, x.bfloat16()):
+        q = pkg.mx.quantize(v)
+        want = _mx.four(v)
+        assert torch.equal(_mx.unpack(q.codes, q.scales, 32), want)
+        assert torch.equal(pkg.mx.dequantize(q, dtype=torch.float32).double(), want)
+        assert torch.equal(pkg.mx.dequantize(q), want.float().bfloat16())
+
+
 def test_not_finite_blocks(pkg):
     x = torch.randn(4, 96, device=DEV)
     x[0, 3], x[1, 40], x[2, 95] = float("nan"), float("inf"), -float("inf")
@@ -157,6 +169,25 @@ def test_not_finite_rows(pkg, n):
     bad = torch.zeros(n, 300, dtype=torch.bool, device=DEV)
     bad[n // 2] = bad[:, 7] = True
     assert bool(torch.isnan(y[bad]).all()) and torch.equal(y[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("n", [1, 40, 300])
+@pytest.mark.parametrize("activation", [None, "relu", "gelu", "silu"])
+def test_infinite_and_far_preactivations(pkg, n, activation):
+    """Columns whose bias is far out: what the activation is there, NaN for NaN, the others as they were."""
+    x, w, b, _, _ = operands(pkg, n, 64, 200, 3)
+    q = pkg.mx.quantize(w)
+    clean = pkg.mx.linear(x, q, b, activation=activation)
+    far = b.clone()
+    far[5], far[100], far[101], far[130], far[199] = float("inf"), 3e38, -3e38, float("nan"), 1e4
+    y = pkg.mx.linear(x, q, far, activation=activation)
+    keep = torch.ones(200, dtype=torch.bool, device=DEV)
+    keep[[5, 100, 101, 130, 199]] = False
+    assert torch.equal(y[:, keep], clean[:, keep])
+    assert bool((y[:, 5] == float("inf")).all()) and bool(torch.isnan(y[:, 130]).all())
+    assert torch.equal(y[:, 100], far[100].expand(n))  # the sums are far below a step of 3e38
+    assert torch.equal(y[:, 101], far[101].expand(n) if activation is None else torch.zeros_like(y[:, 101]))
+    assert bool(((y[:, 199].double() - 1e4).abs() <= 2.0 ** -8 * 1e4 + 64 * 12 * 12 * 2).all())
 
 
 @pytest.mark.parametrize("activation", [None, "relu", "gelu", "silu"])
