@@ -106,7 +106,7 @@ def test_quantize_strides_and_shapes(pkg, dtype):
     assert torch.equal(pkg.mx.dequantize(pkg.mx.quantize(x.t().contiguous().t())).double(), _mx.four(x))
 
 
-SIZES = [(1, 1, 1), (1, 30, 7), (1, 4096, 768), (2, 768, 768), (3, 72, 5), (4, 2049, 100), (5, 64, 40), (16, 4096, 777), (17, 641, 333),
+SIZES = [(1, 1, 1), (9, 1, 1), (130, 1, 300), (5, 32, 127), (1, 30, 7), (1, 4096, 768), (2, 768, 768), (3, 72, 5), (4, 2049, 100), (5, 64, 40), (16, 4096, 777), (17, 641, 333),
          (64, 768, 6562), (100, 200, 129), (128, 64, 256), (129, 1000, 257), (513, 768, 1537), (1000, 256, 4096),
          (2050, 80, 64), (31, 8192, 40), (1300, 2048, 1024), (300, 33, 4000), (257, 515, 513)]
 
