@@ -375,6 +375,12 @@ __device__ __forceinline__ void mx_bytes(uint32_t c, int& lo, int& hi) {
     lo = four(c);
     hi = four(c >> 16);
 }
+// The product of two scales: finite unless one is NaN, so that a block whose products are all zero adds zero.
+__device__ __forceinline__ float mx_factor(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, 0f7F7FFFFF;" : "=f"(r) : "f"(a * b));
+    return r;
+}
 struct MxRowsArgs {
     const unsigned short* x;  // bf16 rows, or null and the codes and scales of a quantised x
     int64_t x_stride;
@@ -391,8 +397,8 @@ struct MxRowsArgs {
 
 // out = act(x^ w^T + b) + r for at most R rows.  A CTA quantises x itself (no launch of its own), to bytes in shared memory; then its
 // warps take F features at a time: a lane has the blocks 32 apart, 16 bytes of codes each, turned to bytes, and integer dot
-// products with x's, exact within a block; blocks are added in fp32.  With x's blocks in registers and a group of threads per
-// feature, x was quantised once for every four features: 1 x 4096 x 4096 MXROWS.
+// products with x's, exact within a block; blocks are added in fp32.  (With x's blocks in registers and a group of threads per
+// feature x was quantised once for every four features: 1 x 4096 x 4096 9.5 us against 6.2.)
 constexpr int MXR_NT = 256;
 constexpr int MXR_SMEM = 36 * 1024;  // of x: 32 bytes and a factor a block and row
 template <int R, int F>
@@ -493,7 +499,7 @@ __global__ void __launch_bounds__(MXR_NT) mx_rows_kernel(const __grid_constant__
                         d = __dp4a(wb[f][5], q.y, d);
                         d = __dp4a(wb[f][6], q.z, d);
                         d = __dp4a(wb[f][7], q.w, d);
-                        acc[r][f] = __fmaf_rn((float)d, xs * s[f], acc[r][f]);
+                        acc[r][f] = __fmaf_rn((float)d, mx_factor(xs, s[f]), acc[r][f]);
                     }
                 }
             }

@@ -190,6 +190,22 @@ def test_infinite_and_far_preactivations(pkg, n, activation):
     assert bool(((y[:, 199].double() - 1e4).abs() <= 2.0 ** -8 * 1e4 + 64 * 12 * 12 * 2).all())
 
 
+@pytest.mark.parametrize("n", [1, 3, 40, 300])
+@pytest.mark.parametrize("far", [100, 120])
+def test_scales_whose_product_passes_fp32(pkg, n, far):
+    """Exact in any order: powers of two in one block, a small product in another."""
+    def product(a, b):
+        x, w = torch.zeros(n, 256, device="cuda", dtype=torch.bfloat16), torch.zeros(320, 256, device="cuda", dtype=torch.bfloat16)
+        x[:, 0], x[:, 40], w[:, 40] = 2.0 ** a, 1.0, 3.0
+        for at, value in b.items():
+            w[:, at] = 2.0 ** value
+        return pkg.mx.linear(x, pkg.mx.quantize(w)).float().unique().tolist()
+    assert product(far, {1: far}) == [3.0]  # zeros met by 2^far on either side
+    assert product(far, {0: -far}) == [4.0]
+    assert product(far, {0: far}) == [float("inf")]
+    assert product(-far, {0: -far}) == [3.0]
+
+
 @pytest.mark.parametrize("activation", [None, "relu", "gelu", "silu"])
 @pytest.mark.parametrize("n,k,m", [(1, 30, 7), (3, 72, 5), (17, 641, 333), (129, 1000, 257), (513, 768, 1537), (64, 768, 6562)])
 def test_gradient(pkg, n, k, m, activation):
