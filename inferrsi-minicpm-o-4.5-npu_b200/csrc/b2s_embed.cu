@@ -37,13 +37,15 @@ constexpr int EM_WINDOW = 1 << 17;  // positions that a CTA's bitmap covers (16 
 template <int E, bool VEC>
 struct RawUnit {
     uint32_t w[VEC ? 4 : 1];
+    __device__ __forceinline__ void take(const uint4& q) {
+        w[0] = q.x;
+        w[1] = q.y;
+        w[2] = q.z;
+        w[3] = q.w;
+    }
     __device__ __forceinline__ void load(const void* row, int64_t u) {
         if constexpr (VEC) {
-            const uint4 q = ldg_stream(reinterpret_cast<const uint4*>(row) + u);
-            w[0] = q.x;
-            w[1] = q.y;
-            w[2] = q.z;
-            w[3] = q.w;
+            take(ldg_stream(reinterpret_cast<const uint4*>(row) + u));
         } else if constexpr (E == 4) {
             w[0] = __ldg(static_cast<const uint32_t*>(row) + u);
         } else {
@@ -357,15 +359,20 @@ __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* token
     }
 }
 
-// A warp per chunk and part of a row.
-constexpr int EM_ROWS = 4;  // rows in flight
+// A warp per chunk and part of a row.  Whole 16-byte units come by asynchronous copies, EM_AHEAD rows ahead of the sums and each
+// lane its own: what bounds this is bytes in flight, and loads to registers, four rows at a time, left too few (30001 x 768 fp32
+// of 6562 ids, with the sort, 45 us against 38.5, 32768 x 1024 bf16 of 20000 49 against 40; 8 rows ahead 40 and 46).  CTAs of two
+// warps: their shares end more evenly than four warps' (38.5 against 42).
+constexpr int EM_SUM_NT = 64;
+constexpr int EM_ROWS = 4;    // rows taken together
+constexpr int EM_AHEAD = 12;  // rows in flight
 template <int E, bool VEC>
-__global__ void __launch_bounds__(EM_NT) embed_sum_kernel(const void* grad, int64_t row_bytes, int64_t units, int parts, float s,
-                                                          void* out, EmbedSort e) {
+__global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* grad, int64_t row_bytes, int64_t units, int parts,
+                                                                 float s, void* out, EmbedSort e) {
     constexpr int N = Unit<E, VEC>::N, W = EM_UNITS / 32;
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), chunk = w / parts;
+    const int64_t w = (int64_t)blockIdx.x * (EM_SUM_NT / 32) + (threadIdx.x >> 5), chunk = w / parts;
     const int part = (int)(w % parts), total = *e.total;
     const int64_t u0 = (int64_t)part * EM_UNITS + lane, width = units * N, k0 = chunk << e.chunk;
     if (k0 >= total) return;
@@ -400,16 +407,9 @@ __global__ void __launch_bounds__(EM_NT) embed_sum_kernel(const void* grad, int6
             }
     };
     int start = 0;  // of the id being summed
-#pragma unroll 1
-    for (int k = 0; k < held; k += EM_ROWS) {
-        RawUnit<E, VEC> g[EM_ROWS][W];
-#pragma unroll
-        for (int r = 0; r < EM_ROWS; ++r) {
-            const unsigned char* src = static_cast<const unsigned char*>(grad) + __shfl_sync(0xffffffffu, pos, (k + r) & 31) * row_bytes;
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (k + r < held && u0 + 32 * j < units) g[r][j].load(src, u0 + 32 * j);
-        }
+    RawUnit<E, VEC> g[EM_ROWS][W];
+    auto row = [&](int k) { return static_cast<const unsigned char*>(grad) + __shfl_sync(0xffffffffu, pos, k & 31) * row_bytes; };
+    auto add_rows = [&](int k) {
 #pragma unroll
         for (int r = 0; r < EM_ROWS; ++r) {
             if (k + r >= held) break;
@@ -424,6 +424,48 @@ __global__ void __launch_bounds__(EM_NT) embed_sum_kernel(const void* grad, int6
                 for (int j = 0; j < W; ++j) sum[j].zero();
                 start = k + r + 1;
             }
+        }
+    };
+    if constexpr (VEC) {
+        __shared__ uint4 ring[EM_SUM_NT / 32][EM_AHEAD][EM_UNITS];
+        uint4(*mine)[EM_UNITS] = ring[threadIdx.x >> 5];
+        auto fetch = [&](int k, int slot) {
+#pragma unroll
+            for (int r = 0; r < EM_ROWS; ++r) {
+                const uint4* src = reinterpret_cast<const uint4*>(row(k + r));
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (k + r < held && u0 + 32 * j < units) cp_async16(&mine[slot + r][32 * j + lane], src + u0 + 32 * j);
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < EM_AHEAD; k += EM_ROWS) fetch(k, k);
+        int slot = 0;
+#pragma unroll 1
+        for (int k = 0; k < held; k += EM_ROWS) {
+            cp_async_wait<EM_AHEAD / EM_ROWS - 1>();
+#pragma unroll
+            for (int r = 0; r < EM_ROWS; ++r)
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (k + r < held && u0 + 32 * j < units) g[r][j].take(mine[slot + r][32 * j + lane]);
+            __syncwarp();  // read, before the next rows are written there
+            fetch(k + EM_AHEAD, slot);
+            slot = slot + EM_ROWS == EM_AHEAD ? 0 : slot + EM_ROWS;
+            add_rows(k);
+        }
+    } else {
+#pragma unroll 1
+        for (int k = 0; k < held; k += EM_ROWS) {
+#pragma unroll
+            for (int r = 0; r < EM_ROWS; ++r) {
+                const unsigned char* src = row(k + r);
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (k + r < held && u0 + 32 * j < units) g[r][j].load(src, u0 + 32 * j);
+            }
+            add_rows(k);
         }
     }
     if (!from && !on) return;
@@ -517,8 +559,8 @@ bool embed_sizes_ok(int64_t n, int64_t vocab, int64_t width) {
     return n <= LP_MAX_SIZE && vocab <= LP_MAX_SIZE && width <= LP_MAX_SIZE;
 }
 // Blocks of a launch with `warps` warps, 0 where those are more than a grid holds.
-unsigned blocks_of(int64_t warps) {
-    const int64_t b = (warps + EM_NT / 32 - 1) / (EM_NT / 32);
+unsigned blocks_of(int64_t warps, int threads = EM_NT) {
+    const int64_t each = threads / 32, b = (warps + each - 1) / each;
     return b > 0x7fffffff ? 0u : (unsigned)b;
 }
 
@@ -602,7 +644,7 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
     const int64_t units = vec ? (int64_t)width * e / 16 : width, parts = parts_of(units);
     const int64_t row_bytes = (int64_t)width * e, zeros = (row_bytes + EM_ZERO - 1) / EM_ZERO;
     const unsigned per = (unsigned)(((int64_t)n + EM_NT - 1) / EM_NT);
-    const unsigned blocks = blocks_of((((int64_t)n - 1 >> s.chunk) + 1) * parts), zero_blocks = blocks_of(vocab * zeros);
+    const unsigned blocks = blocks_of((((int64_t)n - 1 >> s.chunk) + 1) * parts, EM_SUM_NT), zero_blocks = blocks_of(vocab * zeros);
     if (!blocks || !zero_blocks || (int64_t)zero_blocks + per + 1024 > 0x7fffffff) return B2S_ERR_UNSUPPORTED;
     cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
     const bool few = n <= EM_FEW;
@@ -621,7 +663,7 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
                        zeros, (int)longs, (int)orders, static_cast<unsigned char*>(grad_table), e, s);
     if (r != cudaSuccess) return cuda_fail(r);
     auto sum = [&](auto kernel) {
-        return launch_pdl(kernel, dim3(blocks), EM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts, scale,
+        return launch_pdl(kernel, dim3(blocks), EM_SUM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts, scale,
                           grad_table, s);
     };
     r = e == 4 ? (vec ? sum(embed_sum_kernel<4, true>) : sum(embed_sum_kernel<4, false>))
