@@ -421,7 +421,7 @@ int b2s_embedding_mx(const int64_t* tokens, int32_t n, const void* codes, const 
 
 /*
  * The lookup's gradient (ABI 8): grad_table[v] = scale * the sum of grad_out's rows i with tokens[i] = v, in ascending
- * order of i in fp32 (pieces of 32, those in order), rounded once; zeros for ids that do not occur.  grad_table [vocab,
+ * order of i in fp32 (in pieces of up to 32, those in order), rounded once; zeros for ids that do not occur.  grad_table [vocab,
  * width] contiguous, `dtype` its and grad_out's.  The same call gives the same bits.
  */
 int b2s_embedding_grad_workspace(int32_t n, int32_t vocab, int32_t width, int64_t* bytes);
@@ -495,9 +495,9 @@ int b2s_linear_checkpoint_grad_workspace(int32_t rows, int32_t in_features, int3
 int b2s_linear_checkpoint_grad(const b2s_linear_grad_args* args, const b2s_linear_kept* kept, void* stream);
 
 /*
- * The bound of each device wait inside the log-probability and projection kernels, in SM clocks: sets it for the calls
- * of this process that follow (clocks >= 0, at most the default of about a quarter of a second); a negative argument only
- * asks.  previous (optional) gets the bound before.  A wait that gives up sets B2S_STATUS_WAIT_TIMEOUT and makes what was not finished NaN
+ * The bound of each device wait inside the log-probability, projection and microscaled product kernels, in SM clocks: sets it
+ * for the calls of this process that follow (clocks >= 0, at most the default of about a quarter of a second); a negative
+ * argument only asks.  previous (optional) gets the bound before.  A wait that gives up sets B2S_STATUS_WAIT_TIMEOUT and makes what was not finished NaN
  * (ranks and ids of alternatives -1).  0: calls start no copies and no products and give up at once, which shows a caller
  * what that looks like.  A captured call keeps the bound it was captured with.  (ABI 7)
  */

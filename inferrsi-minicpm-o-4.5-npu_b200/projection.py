@@ -6,7 +6,8 @@ the layers that feed a head -- as one tensor-core product with everything in its
 ``checkpoint="e4m3"`` keeps what the backward pass needs, x and the pre-activation, in microscaled 8 bits (OCP MX: blocks of
 32 along a row, each with a power-of-two scale, elements rounded to E4M3): about 2 bytes for each pair of input and output
 elements instead of 4, at 3 fraction bits, so that the weight's gradient is 2 to 3 % off and slopes are those of the rounded
-pre-activation.  The output, and the gradients of x (but for its slopes) and residual, are as without.
+pre-activation; a block that holds NaN or an infinity comes back as NaN.  The output, and the gradients of x (but for its
+slopes) and residual, are as without.
 
 bf16 in and out, fp32 in between, rounded once.  Differentiable in x, weight, bias and residual (once).  Like the head
 products of this engine it takes CUDA tensors only, runs on the current stream, never synchronises, keeps no state
