@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(DZ_NT, 4) linear_dz_kernel(const void* dy, int
 #pragma unroll 4
         for (int r = r0 + rl; r < r1; r += 8) {
             const unsigned short* gp = static_cast<const unsigned short*>(dy) + (int64_t)r * dy_stride + n;
-            float g[E], x[E];
+            float g[E];
             if (VEC || n + E > N) {
                 load8(gp, 0, N - n, VEC, g);
             } else {
@@ -714,7 +714,8 @@ __global__ void __launch_bounds__(DZ_NT, 4) linear_dz_kernel(const void* dy, int
                     g[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
                 }
             }
-            if constexpr (ACT != ACT_NONE) {
+            if constexpr (ACT != ACT_NONE) {  // columns past N come out as anything: neither stored nor summed below
+                float2 x[E / 2];
                 if constexpr (Z8) {
                     const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(z) + (int64_t)r * z_stride + n));
                     const float f = mx_scale(__ldg(z_scale + (int64_t)(n >> 5) * rows + r));
@@ -722,26 +723,31 @@ __global__ void __launch_bounds__(DZ_NT, 4) linear_dz_kernel(const void* dy, int
                     mx_decode4_e4m3(q.x, lo);
                     mx_decode4_e4m3(q.y, hi);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        x[j] = lo[j] * f;
-                        x[4 + j] = hi[j] * f;
+                    for (int j = 0; j < 2; ++j) {
+                        x[j] = __fmul2_rn(make_float2(lo[2 * j], lo[2 * j + 1]), make_float2(f, f));
+                        x[2 + j] = __fmul2_rn(make_float2(hi[2 * j], hi[2 * j + 1]), make_float2(f, f));
                     }
                 } else {
                     const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(z) + (int64_t)r * z_stride + n));
                     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                    for (int j = 0; j < E; ++j) x[j] = preact_value((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+                    for (int j = 0; j < 4; ++j)
+                        x[j] = make_float2(preact_value((unsigned short)w[j]), preact_value((unsigned short)(w[j] >> 16)));
                 }
 #pragma unroll
-                for (int j = 0; j < E; j += 2) {
-                    const float2 d = act_slope_pair<ACT, Z8>(make_float2(x[j], x[j + 1]));
-                    g[j] *= n + j < N ? d.x : 0.0f;
-                    g[j + 1] *= n + j + 1 < N ? d.y : 0.0f;
+                for (int j = 0; j < 4; ++j) {
+                    const float2 d = __fmul2_rn(make_float2(g[2 * j], g[2 * j + 1]), act_slope_pair<ACT, Z8>(x[j]));
+                    g[2 * j] = d.x;
+                    g[2 * j + 1] = d.y;
                 }
             }
             if (dz) store8(static_cast<unsigned short*>(dz) + (int64_t)r * dz_stride + n, 0, N - n, true, g);
 #pragma unroll
-            for (int j = 0; j < E; ++j) sum[j] += g[j];
+            for (int j = 0; j < E; j += 2) {
+                const float2 s = __fadd2_rn(make_float2(sum[j], sum[j + 1]), make_float2(g[j], g[j + 1]));
+                sum[j] = s.x;
+                sum[j + 1] = s.y;
+            }
         }
     }
     if (!part && !db) return;

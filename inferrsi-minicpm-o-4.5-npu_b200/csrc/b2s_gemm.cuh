@@ -141,6 +141,12 @@ __device__ __forceinline__ float act_slope(float z) {
     return 1.0f;
 }
 
+// 1 / x as __fdividef(1, x) gives it for x of at least 1, without its way for small x.
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // The slopes of a pair, in packed arithmetic: act_slope's operations, one for one.  BOUNDED: finite pre-activations, of any size.
 template <int ACT, bool BOUNDED>
 __device__ __forceinline__ float2 act_slope_pair(float2 z) {
@@ -152,7 +158,7 @@ __device__ __forceinline__ float2 act_slope_pair(float2 z) {
     if (ACT == ACT_GELU) {
         const float2 m = make_float2(fabsf(z.x), fabsf(z.y));
         const float2 d = __ffma2_rn(both(0.363f), m, both(1.0f));
-        const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+        const float2 t = make_float2(rcp(d.x), rcp(d.y));
         const float2 x = __fmul2_rn(__fmul2_rn(both(-0.72134752044448170f), m), m);
         const float2 e = make_float2(ex2(x.x), ex2(x.y));
         float2 p = both(0.096218183507f);
@@ -163,14 +169,14 @@ __device__ __forceinline__ float2 act_slope_pair(float2 z) {
         p = __ffma2_rn(p, t, both(0.286393762026f));
         p = __ffma2_rn(p, t, both(0.289791861116f));
         const float2 q = __fmul2_rn(both(0.5f), __fmul2_rn(__fmul2_rn(p, t), e));
-        const float2 o = __fadd2_rn(both(1.0f), make_float2(-q.x, -q.y));
+        const float2 o = __ffma2_rn(both(-1.0f), q, both(1.0f));
         return __ffma2_rn(__fmul2_rn(both(0.398942280401432678f), z), e, make_float2(z.x > 0.0f ? o.x : q.x, z.y > 0.0f ? o.y : q.y));
     }
     if (ACT == ACT_SILU) {
         const float2 x = __fmul2_rn(both(-1.44269504088896341f), z);
         const float2 d = __fadd2_rn(both(1.0f), make_float2(ex2(x.x), ex2(x.y)));
-        const float2 s = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
-        return __fmul2_rn(s, __ffma2_rn(z, __fadd2_rn(both(1.0f), make_float2(-s.x, -s.y)), both(1.0f)));
+        const float2 s = make_float2(rcp(d.x), rcp(d.y));
+        return __fmul2_rn(s, __ffma2_rn(z, __ffma2_rn(both(-1.0f), s, both(1.0f)), both(1.0f)));
     }
     return make_float2(act_slope<ACT>(z.x), act_slope<ACT>(z.y));
 }

@@ -185,11 +185,6 @@ __device__ __forceinline__ void turn_rows(unsigned char* st, uint32_t (&q)[16], 
 }
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // The activations of pairs, in packed arithmetic, in as few operations as they take: with gelu, bias and residual the epilogue's
 // instructions are what a tile of 4096 k waits for.  gelu(z) = max(z, 0) - |z| q with act_apply's tail q = 1 - Phi(|z|) (its
 // polynomial halved); silu as there, e^z by halves.
