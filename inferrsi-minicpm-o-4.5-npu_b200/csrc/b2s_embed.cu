@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(EM_NT) embed_scatter_kernel(const int64_t* tok
 }
 
 // All of that for up to EM_FEW positions in one launch: a position's place is how many come before it by (id, position), found by
-// comparison with all, 8 lanes a position (four launches instead of six).
+// comparison with all, 8 lanes a position (three launches instead of six).
 constexpr int EM_FEW = 4096;
 __global__ void __launch_bounds__(EM_NT) embed_rank_kernel(const int64_t* tokens, int n, int64_t vocab, EmbedSort e) {
     __shared__ int ids[EM_FEW];
@@ -291,37 +291,44 @@ __global__ void __launch_bounds__(EM_NT) embed_rank_kernel(const int64_t* tokens
     }
 }
 
+// Warp w of those that write zeros for the ids that do not occur: EM_ZERO bytes of a row each, `zeros` of them a row.
+constexpr int EM_ZERO = 8192;
+__device__ __forceinline__ void em_zero(int64_t w, int64_t vocab, int64_t row_bytes, int64_t zeros, unsigned char* out, int e_bytes,
+                                        const EmbedSort& e) {
+    const int lane = threadIdx.x & 31;
+    const int64_t v = w / zeros;
+    if (v >= vocab || e.count[v]) return;
+    unsigned char* p = out + v * row_bytes + w % zeros * EM_ZERO;
+    unsigned char* end = out + v * row_bytes + min(row_bytes, (w % zeros + 1) * EM_ZERO);
+    unsigned char* a = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p) + 15) & ~(uintptr_t)15);
+    unsigned char* z = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(end) & ~(uintptr_t)15);
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    if (a < z) {
+#pragma unroll 4
+        for (unsigned char* q = a + 16 * lane; q < z; q += 512) __stcs(reinterpret_cast<uint4*>(q), none);
+    } else {
+        a = z = end;
+    }
+    // the ends that are not whole vectors, in elements
+    for (unsigned char* q = p + (int64_t)lane * e_bytes; q < a; q += 32 * e_bytes)
+        if (e_bytes == 4) *reinterpret_cast<uint32_t*>(q) = 0;
+        else *reinterpret_cast<unsigned short*>(q) = 0;
+    for (unsigned char* q = z + (int64_t)lane * e_bytes; q < end; q += 32 * e_bytes)
+        if (e_bytes == 4) *reinterpret_cast<uint32_t*>(q) = 0;
+        else *reinterpret_cast<unsigned short*>(q) = 0;
+}
+
 // The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order: marked in a bitmap,
 // EM_WINDOW positions at a time, and read from it.  The next `orders` CTAs do the others', a place's rank by comparison with the
-// id's other places.  The last ones write zeros for the ids that do not occur, a warp per EM_ZERO bytes of a row.
-constexpr int EM_ZERO = 8192;
+// id's other places.  The last ones write zeros for the ids that do not occur.
 __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* tokens, int n, int64_t vocab, int64_t row_bytes,
                                                             int64_t zeros, int longs, int orders, unsigned char* out, int e_bytes,
                                                             EmbedSort e) {
     __shared__ uint32_t bits[EM_WINDOW / 32];
     pdl_wait_then_release();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, warp = tid >> 5;
     if ((int)blockIdx.x >= longs + orders) {
-        const int64_t w = (int64_t)(blockIdx.x - longs - orders) * (EM_NT / 32) + warp, v = w / zeros;
-        if (v >= vocab || e.count[v]) return;
-        unsigned char* p = out + v * row_bytes + w % zeros * EM_ZERO;
-        unsigned char* end = out + v * row_bytes + min(row_bytes, (w % zeros + 1) * EM_ZERO);
-        unsigned char* a = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p) + 15) & ~(uintptr_t)15);
-        unsigned char* z = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(end) & ~(uintptr_t)15);
-        const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-        if (a < z) {
-#pragma unroll 4
-            for (unsigned char* q = a + 16 * lane; q < z; q += 512) __stcs(reinterpret_cast<uint4*>(q), none);
-        } else {
-            a = z = end;
-        }
-        // the ends that are not whole vectors, in elements
-        for (unsigned char* q = p + (int64_t)lane * e_bytes; q < a; q += 32 * e_bytes)
-            if (e_bytes == 4) *reinterpret_cast<uint32_t*>(q) = 0;
-            else *reinterpret_cast<unsigned short*>(q) = 0;
-        for (unsigned char* q = z + (int64_t)lane * e_bytes; q < end; q += 32 * e_bytes)
-            if (e_bytes == 4) *reinterpret_cast<uint32_t*>(q) = 0;
-            else *reinterpret_cast<unsigned short*>(q) = 0;
+        em_zero((int64_t)(blockIdx.x - longs - orders) * (EM_NT / 32) + warp, vocab, row_bytes, zeros, out, e_bytes, e);
         return;
     }
     if ((int)blockIdx.x >= longs) {
@@ -362,15 +369,21 @@ __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* token
 // A warp per chunk and part of a row.  Whole 16-byte units come by asynchronous copies, EM_AHEAD rows ahead of the sums and each
 // lane its own: what bounds this is bytes in flight, and loads to registers, four rows at a time, left too few (30001 x 768 fp32
 // of 6562 ids, with the sort, 45 us against 38.5, 32768 x 1024 bf16 of 20000 49 against 40; 8 rows ahead 40 and 46).  CTAs of two
-// warps: their shares end more evenly than four warps' (38.5 against 42).
+// warps: their shares end more evenly than four warps' (38.5 against 42).  CTAs from `sums` on write zeros (em_zero).
 constexpr int EM_SUM_NT = 64;
 constexpr int EM_ROWS = 4;    // rows taken together
 constexpr int EM_AHEAD = 12;  // rows in flight
 template <int E, bool VEC>
 __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* grad, int64_t row_bytes, int64_t units, int parts,
-                                                                 float s, void* out, EmbedSort e) {
+                                                                 float s, void* out, EmbedSort e, unsigned sums, int64_t vocab,
+                                                                 int64_t zeros) {
     constexpr int N = Unit<E, VEC>::N, W = EM_UNITS / 32;
     pdl_wait_then_release();
+    if (blockIdx.x >= sums) {
+        em_zero((int64_t)(blockIdx.x - sums) * (EM_SUM_NT / 32) + (threadIdx.x >> 5), vocab, units * N * E, zeros,
+                static_cast<unsigned char*>(out), E, e);
+        return;
+    }
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * (EM_SUM_NT / 32) + (threadIdx.x >> 5), chunk = w / parts;
     const int part = (int)(w % parts), total = *e.total;
@@ -646,8 +659,10 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
     const unsigned per = (unsigned)(((int64_t)n + EM_NT - 1) / EM_NT);
     const unsigned blocks = blocks_of((((int64_t)n - 1 >> s.chunk) + 1) * parts, EM_SUM_NT), zero_blocks = blocks_of(vocab * zeros);
     if (!blocks || !zero_blocks || (int64_t)zero_blocks + per + 1024 > 0x7fffffff) return B2S_ERR_UNSUPPORTED;
-    cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
     const bool few = n <= EM_FEW;
+    const unsigned late = few ? blocks_of(vocab * zeros, EM_SUM_NT) : 0u;  // CTAs of the last launch that write zeros then
+    if (few && (!late || (int64_t)late + blocks > 0x7fffffff)) return B2S_ERR_UNSUPPORTED;
+    cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
     if (few) {
         if (r == cudaSuccess)
             r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / 8 - 1) / (EM_NT / 8))), EM_NT, 0, stream, tokens, (int)n,
@@ -657,14 +672,15 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
         if (r == cudaSuccess) r = launch_pdl(embed_scan_kernel, dim3((unsigned)s.bins), EM_NT, 0, stream, (int64_t)vocab, s);
         if (r == cudaSuccess) r = launch_pdl(embed_scatter_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, s);
     }
-    const unsigned orders = few ? 0 : per, most = 2 * (unsigned)sms_here(), longs = few ? 0 : n / EM_SHORT < (int)most ? n / EM_SHORT : most;
-    if (r == cudaSuccess)
-        r = launch_pdl(embed_order_kernel, dim3(zero_blocks + orders + longs), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, row_bytes,
-                       zeros, (int)longs, (int)orders, static_cast<unsigned char*>(grad_table), e, s);
+    if (r == cudaSuccess && !few) {
+        const unsigned most = 2 * (unsigned)sms_here(), longs = n / EM_SHORT < (int)most ? n / EM_SHORT : most;
+        r = launch_pdl(embed_order_kernel, dim3(zero_blocks + per + longs), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, row_bytes,
+                       zeros, (int)longs, (int)per, static_cast<unsigned char*>(grad_table), e, s);
+    }
     if (r != cudaSuccess) return cuda_fail(r);
     auto sum = [&](auto kernel) {
-        return launch_pdl(kernel, dim3(blocks), EM_SUM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts, scale,
-                          grad_table, s);
+        return launch_pdl(kernel, dim3(blocks + late), EM_SUM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts, scale,
+                          grad_table, s, blocks, (int64_t)vocab, zeros);
     };
     r = e == 4 ? (vec ? sum(embed_sum_kernel<4, true>) : sum(embed_sum_kernel<4, false>))
                : (vec ? sum(embed_sum_kernel<2, true>) : sum(embed_sum_kernel<2, false>));
