@@ -254,10 +254,12 @@ __global__ void __launch_bounds__(EM_NT) embed_scatter_kernel(const int64_t* tok
 }
 
 // All of that for up to EM_FEW positions in one launch: a position's place is how many come before it by (id, position), found by
-// comparison with all, 8 lanes a position (three launches instead of six).
+// comparison with all, EM_RANK lanes a position (three launches instead of six: 1024 of 1000 x 256 12.4 us against 17.4, 2048 14.5
+// against 17.2, 4096 20.8 against 18.5, but of 30,000 x 2048 33.6 against 37.6; with 8 lanes and an id at a time 14.4, 16.4, 22.3).
 constexpr int EM_FEW = 4096;
+constexpr int EM_RANK = 16;
 __global__ void __launch_bounds__(EM_NT) embed_rank_kernel(const int64_t* tokens, int n, int64_t vocab, EmbedSort e) {
-    __shared__ int ids[EM_FEW];
+    __shared__ __align__(16) int ids[EM_FEW];
     pdl_wait_then_release();
     int real = 0;
     for (int j = threadIdx.x; j < n; j += EM_NT) {
@@ -265,24 +267,30 @@ __global__ void __launch_bounds__(EM_NT) embed_rank_kernel(const int64_t* tokens
         ids[j] = t < 0 ? 0x7fffffff : t;  // behind all others, equal to none
         real += t >= 0;
     }
+    for (int j = n + threadIdx.x; j < (n + 3) / 4 * 4; j += EM_NT) ids[j] = 0x7fffffff;
     int all;
     em_scan(real, &all);
     if (blockIdx.x == 0 && threadIdx.x == 0) *e.total = all;
-    const int i = blockIdx.x * (EM_NT / 8) + (threadIdx.x >> 3), t = i < n ? ids[i] : 0x7fffffff;
+    const int i = blockIdx.x * (EM_NT / EM_RANK) + threadIdx.x / EM_RANK, t = i < n ? ids[i] : 0x7fffffff;
     int before = 0, lower = 0, same = 0;
-    for (int j = threadIdx.x & 7; j < n; j += 8) {
-        const int o = ids[j];
-        lower += o < t;
-        same += o == t;
-        before += o == t && j < i;
+#pragma unroll 4
+    for (int j = 4 * (threadIdx.x % EM_RANK); j < n; j += 4 * EM_RANK) {
+        const int4 q = *reinterpret_cast<const int4*>(ids + j);
+        const int o[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            lower += o[k] < t;
+            same += o[k] == t;
+            before += o[k] == t && j + k < i;
+        }
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < EM_RANK; o <<= 1) {
         lower += __shfl_xor_sync(0xffffffffu, lower, o);
         same += __shfl_xor_sync(0xffffffffu, same, o);
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
-    if ((threadIdx.x & 7) || t == 0x7fffffff) return;
+    if (threadIdx.x % EM_RANK || t == 0x7fffffff) return;
     e.order[lower + before] = i;
     e.id[lower + before] = t;
     if (before == 0) {
@@ -665,7 +673,7 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
     cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
     if (few) {
         if (r == cudaSuccess)
-            r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / 8 - 1) / (EM_NT / 8))), EM_NT, 0, stream, tokens, (int)n,
+            r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / EM_RANK - 1) / (EM_NT / EM_RANK))), EM_NT, 0, stream, tokens, (int)n,
                            (int64_t)vocab, s);
     } else {
         if (r == cudaSuccess) r = launch_pdl(embed_count_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s);

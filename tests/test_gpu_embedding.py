@@ -142,6 +142,21 @@ def test_gradient(pkg, n, vocab, width, kind, dtype):
     assert torch.equal(d, want_grad(tokens, whole, vocab, 0.5).float().to(dtype))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [2, 3, 7, 8, 9, 12, 13, 31, 47, 1021, 4094, 4096, 4097])
+@pytest.mark.parametrize("vocab,width", [(1, 520), (5, 264), (900, 40), (3000, 7)])
+def test_gradient_at_changes_of_path(pkg, n, vocab, width, dtype):
+    """Whole numbers, exact in any order below 2^24 and rounded once: positions by rank or by counts, chunks that end in a row of an
+    id or between two, absent ids in the last rows."""
+    g = gen(n * 7 + vocab)
+    tokens = torch.randint(-1, vocab, (n,), device=DEV, generator=g)
+    tokens[tokens == vocab - 2] = -1
+    table = torch.zeros(vocab, width, device=DEV, dtype=dtype, requires_grad=True)
+    dy = torch.randint(-3, 4, (n, width), device=DEV, generator=g).to(dtype)
+    d, = torch.autograd.grad(pkg.embedding.lookup(tokens, table), table, dy)
+    assert torch.equal(d, want_grad(tokens, dy, vocab, 1.0).float().to(dtype))
+
+
 def test_gradient_ignores_what_padding_and_lost_ids_receive(pkg):
     tokens = torch.tensor([2, -1, 9, 2, 500, -7], device=DEV)
     table = torch.zeros(10, 16, device=DEV, requires_grad=True)
