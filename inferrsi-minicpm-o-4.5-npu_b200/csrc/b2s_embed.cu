@@ -27,10 +27,13 @@ int cuda_fail(cudaError_t e);
 namespace {
 
 constexpr int EM_NT = 256;
-constexpr int EM_JOIN = 16;    // sums joined at a time
+constexpr int EM_JOIN = 4;     // 2^4 sums joined at a time
 constexpr int EM_SHORT = 64;   // positions of an id that are put in order by comparison
 constexpr int EM_BINS = 4096;  // at most, of ids counted together
 constexpr int EM_UNITS = 64;   // 16-byte units (or elements) of a row that a warp takes
+constexpr int EM_MID = 512;    // ... by a CTA in shared memory; beyond, by bitmaps
+constexpr int EM_HUGE = 4096;  // ... by several CTAs, at most EM_PARTS
+constexpr int EM_PARTS = 64;
 constexpr int EM_WINDOW = 1 << 17;  // positions that a CTA's bitmap covers (16 KB)
 
 // E: 4 (fp32) or 2 (bf16) bytes an element; a unit is 16 bytes of them (VEC) or a single one, as it lies and as fp32.
@@ -171,31 +174,72 @@ __global__ void __launch_bounds__(EM_NT) embed_mx_kernel(const int64_t* tokens, 
 struct EmbedSort {
     int* count;    // [vocab] positions of an id
     int* bin;      // [bins] positions of 1 << shift ids
-    int* arrived;  // [2][slots][parts] sums that are there, of a group (at its first) and groups of an id (at its first)
-    int* longs;    // how many ids have more than EM_SHORT positions
+    int* arrived;  // [slots][parts] sums that are there, of those that are joined
+    int* longs;    // how many parts the ids with more than EM_SHORT positions have
     int* total;    // positions that are not padding
-    int* long_id;  // [n / EM_SHORT] which
+    int2* long_id; // [2 n / EM_SHORT] which, and which part of its positions
     int* base;     // [vocab] where an id's positions start, sorted
     int* place;    // [n] among the id's positions in order of arrival; -1: none
     int* loose;    // [n] positions by id, in order of arrival
     int* order;    // [n] positions by id, ascending
     int* id;       // [n] their ids
     float* sums;   // [slots][width]: two for each chunk, of the id that came from the one before and of the last one, that goes on
-    int slots, shift, bins;
+    int slots, shift, bins, windows;
     int chunk;     // sorted positions that a warp sums, as a power of two: 8, 16 or 32
+    // CTAs that put an id's positions in order, each in its share of the windows
+    __device__ __forceinline__ int parts_of(int positions) const { return positions > EM_HUGE ? min(windows, EM_PARTS) : 1; }
 };
 
+// Counts per id and bin, an atomic for a warp's equal ids.  TABLE: a CTA's positions are counted in shared memory first, ids in a
+// table (open addressing, never more than half full), so that an id or a bin that is much of the input costs an atomic a CTA: the
+// gradient of 300,000 positions of 151,936 ids, 8 wide, takes 96 us against 125, a million Zipf-distributed 340 against 450, but
+// 30001 of 6562 768 wide 30.9 against 28.8.
+constexpr int EM_TABLE = 2 * EM_NT;
+constexpr int EM_MANY = 1 << 16;  // positions from which on
+template <bool TABLE>
 __global__ void __launch_bounds__(EM_NT) embed_count_kernel(const int64_t* tokens, int n, int64_t vocab, EmbedSort e) {
+    __shared__ int key[TABLE ? EM_TABLE : 1], num[TABLE ? EM_TABLE : 1], bin[TABLE ? EM_BINS : 1];
+    const int tid = threadIdx.x, lane = tid & 31;
+    if constexpr (TABLE) {
+        for (int j = tid; j < EM_TABLE; j += EM_NT) {
+            key[j] = -1;
+            num[j] = 0;
+        }
+        for (int j = tid; j < e.bins; j += EM_NT) bin[j] = 0;
+    }
     pdl_wait_then_release();
-    const int i = blockIdx.x * EM_NT + threadIdx.x, lane = threadIdx.x & 31;
+    const int i = blockIdx.x * EM_NT + tid;
     const int t = i < n ? (int)token_at(tokens, i, vocab, nullptr) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, t);  // one atomic for a warp's equal ids
+    const uint32_t same = __match_any_sync(0xffffffffu, t);
     const int leader = __ffs(same) - 1;
+    const bool leads = t >= 0 && lane == leader;
     int at = 0;
-    if (t >= 0 && lane == leader) at = atomicAdd(e.count + t, __popc(same));
+    if constexpr (TABLE) {
+        int slot = 0;
+        bool first = false;  // of the CTA with this id
+        __syncthreads();
+        if (leads) {
+            slot = (int)((uint32_t)t * 2654435761u >> 16) & (EM_TABLE - 1);
+            for (;; slot = (slot + 1) & (EM_TABLE - 1)) {
+                const int was = atomicCAS(&key[slot], -1, t);
+                first = was == -1;
+                if (first || was == t) break;
+            }
+            at = atomicAdd(&num[slot], __popc(same));
+            atomicAdd(&bin[t >> e.shift], __popc(same));
+        }
+        __syncthreads();
+        if (first) num[slot] = atomicAdd(e.count + t, num[slot]);
+        for (int j = tid; j < e.bins; j += EM_NT)
+            if (bin[j]) atomicAdd(e.bin + j, bin[j]);
+        __syncthreads();
+        if (leads) at += num[slot];
+    } else {
+        if (leads) at = atomicAdd(e.count + t, __popc(same));
+        const uint32_t near = __match_any_sync(0xffffffffu, t < 0 ? -1 : t >> e.shift);
+        if (t >= 0 && lane == __ffs(near) - 1) atomicAdd(e.bin + (t >> e.shift), __popc(near));
+    }
     at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
-    const uint32_t near = __match_any_sync(0xffffffffu, t < 0 ? -1 : t >> e.shift);
-    if (t >= 0 && lane == __ffs(near) - 1) atomicAdd(e.bin + (t >> e.shift), __popc(near));
     if (i < n) e.place[i] = t < 0 ? -1 : at;
 }
 
@@ -236,10 +280,13 @@ __global__ void __launch_bounds__(EM_NT) embed_scan_kernel(int64_t vocab, EmbedS
         const int at = start + em_scan(c.x + c.y + c.z + c.w, &all);
         if (v < end) *reinterpret_cast<int4*>(e.base + v) = make_int4(at, at + c.x, at + c.x + c.y, at + c.x + c.y + c.z);
         if (max(max(c.x, c.y), max(c.z, c.w)) > EM_SHORT) {  // in any order: each is put in order by itself
-            if (c.x > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v;
-            if (c.y > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v + 1;
-            if (c.z > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v + 2;
-            if (c.w > EM_SHORT) e.long_id[atomicAdd(e.longs, 1)] = (int)v + 3;
+            const int k[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (k[j] <= EM_SHORT) continue;
+                const int parts = e.parts_of(k[j]), f = atomicAdd(e.longs, parts);
+                for (int p = 0; p < parts; ++p) e.long_id[f + p] = make_int2((int)v + j, p);
+            }
         }
         start += all;
     }
@@ -326,13 +373,15 @@ __device__ __forceinline__ void em_zero(int64_t w, int64_t vocab, int64_t row_by
         else *reinterpret_cast<unsigned short*>(q) = 0;
 }
 
-// The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order: marked in a bitmap,
-// EM_WINDOW positions at a time, and read from it.  The next `orders` CTAs do the others', a place's rank by comparison with the
-// id's other places.  The last ones write zeros for the ids that do not occur.
+// The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order: up to EM_MID by comparison
+// in shared memory, more by marking them in a bitmap of EM_WINDOW positions and reading it, behind as many as come before it;
+// of an id with more than EM_HUGE several CTAs each do some of the windows (300,000 equal ids 8 wide 226 us against 483 by one CTA;
+// a million Zipf-distributed 340 against 425, and 732 with bitmaps for the short ones too).  The next `orders` CTAs do the others', a place's rank by comparison with the id's other places.
+// The last ones write zeros for the ids that do not occur.
 __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* tokens, int n, int64_t vocab, int64_t row_bytes,
                                                             int64_t zeros, int longs, int orders, unsigned char* out, int e_bytes,
                                                             EmbedSort e) {
-    __shared__ uint32_t bits[EM_WINDOW / 32];
+    __shared__ __align__(16) uint32_t bits[EM_WINDOW / 32];
     pdl_wait_then_release();
     const int tid = threadIdx.x, warp = tid >> 5;
     if ((int)blockIdx.x >= longs + orders) {
@@ -352,24 +401,45 @@ __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* token
         return;
     }
     for (int f = blockIdx.x; f < *e.longs; f += longs) {
-        const int t = e.long_id[f], c = e.count[t], b = e.base[t];
-        int done = 0;
-        for (int64_t w0 = 0; w0 < n && done < c; w0 += EM_WINDOW) {
-            const int words = ((int)min((int64_t)EM_WINDOW, n - w0) + 31) / 32, per = (words + EM_NT - 1) / EM_NT;
-            for (int j = tid; j < words; j += EM_NT) bits[j] = 0;
+        const int t = e.long_id[f].x, c = e.count[t], b = e.base[t], parts = e.parts_of(c);
+        const int* loose = e.loose + b;
+        if (c <= EM_MID && e.windows > 1) {
+            int* at = reinterpret_cast<int*>(bits);
+            for (int j = tid; j < EM_MID; j += EM_NT) at[j] = j < c ? loose[j] : 0x7fffffff;
             __syncthreads();
             for (int j = tid; j < c; j += EM_NT) {
-                const int64_t i = e.loose[b + j] - w0;
-                if (i >= 0 && i < EM_WINDOW) atomicOr(&bits[i >> 5], 1u << (i & 31));
+                const int i = at[j];
+                int rank = 0;
+#pragma unroll 4
+                for (int k = 0; k < c; k += 4) {
+                    const int4 q = *reinterpret_cast<const int4*>(at + k);
+                    rank += (q.x < i) + (q.y < i) + (q.z < i) + (q.w < i);
+                }
+                e.order[b + rank] = i;
             }
             __syncthreads();
-            int mine = 0, all;
-            for (int j = tid * per; j < min(words, (tid + 1) * per); ++j) mine += __popc(bits[j]);
-            int at = b + done + em_scan(mine, &all);
-            for (int j = tid * per; j < min(words, (tid + 1) * per); ++j)
-                for (uint32_t m = bits[j]; m; m &= m - 1) e.order[at++] = (int)w0 + 32 * j + __ffs(m) - 1;
-            done += all;
+            continue;
+        }
+        for (int w = e.long_id[f].y; w < e.windows; w += parts) {
+            const int w0 = w * EM_WINDOW, held = min(EM_WINDOW, n - w0), words = (held + 31) / 32, per = (words + EM_NT - 1) / EM_NT;
+            for (int j = tid; j < words; j += EM_NT) bits[j] = 0;
             __syncthreads();
+            int before = 0, mine = 0, start, all;
+#pragma unroll 8
+            for (int j = tid; j < c; j += EM_NT) {
+                const int i = loose[j] - w0;
+                before += i < 0;
+                if (i >= 0 && i < held) atomicOr(&bits[i >> 5], 1u << (i & 31));
+            }
+            __syncthreads();
+            if (e.windows > 1) em_scan(before, &start);
+            else start = 0;
+            for (int j = tid * per; j < min(words, (tid + 1) * per); ++j) mine += __popc(bits[j]);
+            int at = b + start + em_scan(mine, &all);
+            for (int j = tid * per; j < min(words, (tid + 1) * per); ++j)
+                for (uint32_t m = bits[j]; m; m &= m - 1) e.order[at++] = w0 + 32 * j + __ffs(m) - 1;
+            __syncthreads();
+            if (start + all == c) break;
         }
     }
 }
@@ -500,7 +570,8 @@ __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* gra
         return there == of - 1;
     };
     // An id's sums lie with its chunks from c0 on, in the first one's second place and the others' first.  They are added in
-    // order, EM_JOIN at a time and then the groups', so that which warp it is that completes them does not matter.
+    // order, 2^EM_JOIN neighbours at a time, then as many of those sums, and so on, so that which warp it is that completes them does
+    // not matter.  A sum replaces its first part; level l counts arrivals at its first part's l-th neighbour.
 #pragma unroll 1
     for (int both = 0; both < 2; ++both) {
         if (both ? !on || (from && first_id == last_id) : !from) continue;  // a chunk of one id has one sum
@@ -530,15 +601,19 @@ __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* gra
                     }
             }
         };
-        const int group = ((int)chunk - c0) / EM_JOIN * EM_JOIN, groups = (of + EM_JOIN - 1) / EM_JOIN, in = min(EM_JOIN, of - group);
-        if (!last(slot(group), in)) continue;
-        join(group, in, 1);
-        if (groups > 1) {
-            keep(slot(group));  // in the first one's place, which nobody reads again
-            if (!last(e.slots + slot(0), groups)) continue;
-            join(0, groups, EM_JOIN);
+        bool whole = true;
+        for (int level = 0, span = 0; (of - 1) >> span; ++level, span += EM_JOIN) {  // 2^span chunks in a sum
+            const int group = ((int)chunk - c0) >> (span + EM_JOIN) << (span + EM_JOIN);
+            const int in = min(1 << EM_JOIN, ((of - group - 1) >> span) + 1);
+            if (in == 1) continue;  // the last sum of its level, as it is
+            if (!last(slot(group + level), in)) {
+                whole = false;
+                break;
+            }
+            join(group, in, 1 << span);
+            if ((of - 1) >> (span + EM_JOIN)) keep(slot(group));
         }
-        write(t);
+        if (whole) write(t);
     }
 }
 
@@ -554,18 +629,20 @@ int64_t embed_layout(int64_t n, int64_t vocab, int64_t width, unsigned char* at,
         return p;
     };
     // 32 positions a warp, fewer where there would be few warps (2048 x 768 of 6562 ids: 26 against 21 us)
-    e->chunk = n * width <= 1 << 22 ? 3 : n * width <= 1 << 24 ? 4 : 5;
+    const int64_t shares = n * ((width + 511) / 512);
+    e->chunk = shares <= 1 << 13 ? 3 : shares <= 1 << 15 ? 4 : 5;
     e->slots = (int)(2 * (((n - 1) >> e->chunk) + 1));
     e->shift = 10;  // bins of 1024 ids, or as many as make EM_BINS
     while ((vocab - 1) >> e->shift >= EM_BINS) ++e->shift;
     e->bins = (int)(((vocab - 1) >> e->shift) + 1);
+    e->windows = (int)((n - 1) / EM_WINDOW + 1);
     e->count = reinterpret_cast<int*>(take(up(vocab, 4) * 4));
     e->bin = reinterpret_cast<int*>(take((int64_t)e->bins * 4));
-    e->arrived = reinterpret_cast<int*>(take(2 * (int64_t)e->slots * parts_of(width) * 4));
+    e->arrived = reinterpret_cast<int*>(take((int64_t)e->slots * parts_of(width) * 4));
     e->longs = reinterpret_cast<int*>(take(4));
     *zeroed = used;
     e->total = reinterpret_cast<int*>(take(4));
-    e->long_id = reinterpret_cast<int*>(take(n / EM_SHORT * 4));
+    e->long_id = reinterpret_cast<int2*>(take(2 * (n / EM_SHORT) * 8));
     e->base = reinterpret_cast<int*>(take(up(vocab, 4) * 4));
     e->place = reinterpret_cast<int*>(take(n * 4));
     e->loose = reinterpret_cast<int*>(take(n * 4));
@@ -676,12 +753,14 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
             r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / EM_RANK - 1) / (EM_NT / EM_RANK))), EM_NT, 0, stream, tokens, (int)n,
                            (int64_t)vocab, s);
     } else {
-        if (r == cudaSuccess) r = launch_pdl(embed_count_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s);
+        if (r == cudaSuccess)
+            r = n < EM_MANY ? launch_pdl(embed_count_kernel<false>, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s)
+                            : launch_pdl(embed_count_kernel<true>, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s);
         if (r == cudaSuccess) r = launch_pdl(embed_scan_kernel, dim3((unsigned)s.bins), EM_NT, 0, stream, (int64_t)vocab, s);
         if (r == cudaSuccess) r = launch_pdl(embed_scatter_kernel, dim3(per), EM_NT, 0, stream, tokens, (int)n, s);
     }
     if (r == cudaSuccess && !few) {
-        const unsigned most = 2 * (unsigned)sms_here(), longs = n / EM_SHORT < (int)most ? n / EM_SHORT : most;
+        const unsigned most = 2 * (unsigned)sms_here(), longs = 2 * (n / EM_SHORT) < (int)most ? 2 * (n / EM_SHORT) : most;
         r = launch_pdl(embed_order_kernel, dim3(zero_blocks + per + longs), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, row_bytes,
                        zeros, (int)longs, (int)per, static_cast<unsigned char*>(grad_table), e, s);
     }

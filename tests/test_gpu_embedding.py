@@ -157,6 +157,24 @@ def test_gradient_at_changes_of_path(pkg, n, vocab, width, dtype):
     assert torch.equal(d, want_grad(tokens, dy, vocab, 1.0).float().to(dtype))
 
 
+@pytest.mark.parametrize("n,vocab,width,kind", [(65_535, 40_000, 5, "uniform"), (65_536, 40_000, 8, "uniform"), (65_537, 5_000_000, 4, "zipf"),
+                                                (200_000, 3000, 16, "zipf"), (600_000, 9000, 8, "zipf"), (400_000, 3, 8, "uniform"),
+                                                (131_073, 1, 8, "equal"), (300_000, 600, 1, "uniform")])
+def test_gradient_of_many_positions(pkg, n, vocab, width, kind):
+    """Whole numbers, exact in any order and rounded once: ids with a few positions, hundreds, thousands and most of them, on either
+    side of a bitmap's end, joined over several levels."""
+    g = gen(n + width)
+    tokens = draw_tokens(kind, n, vocab, g)
+    dy = torch.randint(-3, 4, (n, width), device=DEV, generator=g).bfloat16()
+    table = torch.zeros(vocab, width, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    d, = torch.autograd.grad(pkg.embedding.lookup(tokens, table), table, dy)
+    assert torch.equal(d, want_grad(tokens, dy, vocab, 1.0).float().bfloat16())
+    loud = torch.randn(n, width, device=DEV, generator=g).bfloat16()  # the same bits each time
+    first, = torch.autograd.grad(pkg.embedding.lookup(tokens, table), table, loud)
+    again, = torch.autograd.grad(pkg.embedding.lookup(tokens, table), table, loud)
+    assert torch.equal(first, again)
+
+
 def test_gradient_ignores_what_padding_and_lost_ids_receive(pkg):
     tokens = torch.tensor([2, -1, 9, 2, 500, -7], device=DEV)
     table = torch.zeros(10, 16, device=DEV, requires_grad=True)
