@@ -373,11 +373,12 @@ __device__ __forceinline__ void em_zero(int64_t w, int64_t vocab, int64_t row_by
         else *reinterpret_cast<unsigned short*>(q) = 0;
 }
 
-// The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order: up to EM_MID by comparison
-// in shared memory, more by marking them in a bitmap of EM_WINDOW positions and reading it, behind as many as come before it;
-// of an id with more than EM_HUGE several CTAs each do some of the windows (300,000 equal ids 8 wide 226 us against 483 by one CTA;
-// a million Zipf-distributed 340 against 425, and 732 with bitmaps for the short ones too).  The next `orders` CTAs do the others', a place's rank by comparison with the id's other places.
-// The last ones write zeros for the ids that do not occur.
+// The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order.  Where one bitmap covers all
+// positions they are marked in it and read back.  Of longer inputs, up to EM_MID by comparison in shared memory, more by bitmaps
+// of EM_WINDOW positions, each behind as many as come before it; of an id with more than EM_HUGE several CTAs each do some of the
+// windows (300,000 equal ids 8 wide 226 us against 483 by one CTA; a million Zipf-distributed 340 against 425, and 732 with
+// bitmaps for up to EM_MID too; with one bitmap comparisons cost 30001 of 6562 40 against 37).  The next `orders` CTAs do the
+// others', a place's rank by comparison with the id's other places.  The last ones write zeros for the ids that do not occur.
 __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* tokens, int n, int64_t vocab, int64_t row_bytes,
                                                             int64_t zeros, int longs, int orders, unsigned char* out, int e_bytes,
                                                             EmbedSort e) {
@@ -421,7 +422,8 @@ __global__ void __launch_bounds__(EM_NT) embed_order_kernel(const int64_t* token
             continue;
         }
         for (int w = e.long_id[f].y; w < e.windows; w += parts) {
-            const int w0 = w * EM_WINDOW, held = min(EM_WINDOW, n - w0), words = (held + 31) / 32, per = (words + EM_NT - 1) / EM_NT;
+            const int w0 = w * EM_WINDOW, held = min(EM_WINDOW, n - w0);
+            const int words = (held + 31) / 32, per = (words + EM_NT - 1) / EM_NT;
             for (int j = tid; j < words; j += EM_NT) bits[j] = 0;
             __syncthreads();
             int before = 0, mine = 0, start, all;
@@ -491,7 +493,8 @@ __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* gra
                 if constexpr (VEC) {
 #pragma unroll
                     for (int k = 0; k < N; k += 4)
-                        __stcg(reinterpret_cast<float4*>(q + k), make_float4(sum[j].v[k], sum[j].v[k + 1], sum[j].v[k + 2], sum[j].v[k + 3]));
+                        __stcg(reinterpret_cast<float4*>(q + k),
+                               make_float4(sum[j].v[k], sum[j].v[k + 1], sum[j].v[k + 2], sum[j].v[k + 3]));
                 } else {
                     __stcg(q, sum[j].v[0]);
                 }
@@ -570,8 +573,8 @@ __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* gra
         return there == of - 1;
     };
     // An id's sums lie with its chunks from c0 on, in the first one's second place and the others' first.  They are added in
-    // order, 2^EM_JOIN neighbours at a time, then as many of those sums, and so on, so that which warp it is that completes them does
-    // not matter.  A sum replaces its first part; level l counts arrivals at its first part's l-th neighbour.
+    // order, 2^EM_JOIN neighbours at a time, then as many of those sums, and so on, so that which warp it is that completes
+    // them does not matter.  A sum replaces its first part; level l counts arrivals at its first part's l-th neighbour.
 #pragma unroll 1
     for (int both = 0; both < 2; ++both) {
         if (both ? !on || (from && first_id == last_id) : !from) continue;  // a chunk of one id has one sum
@@ -750,8 +753,8 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
     cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
     if (few) {
         if (r == cudaSuccess)
-            r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / EM_RANK - 1) / (EM_NT / EM_RANK))), EM_NT, 0, stream, tokens, (int)n,
-                           (int64_t)vocab, s);
+            r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / EM_RANK - 1) / (EM_NT / EM_RANK))), EM_NT, 0, stream,
+                           tokens, (int)n, (int64_t)vocab, s);
     } else {
         if (r == cudaSuccess)
             r = n < EM_MANY ? launch_pdl(embed_count_kernel<false>, dim3(per), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, s)
@@ -761,13 +764,13 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
     }
     if (r == cudaSuccess && !few) {
         const unsigned most = 2 * (unsigned)sms_here(), longs = 2 * (n / EM_SHORT) < (int)most ? 2 * (n / EM_SHORT) : most;
-        r = launch_pdl(embed_order_kernel, dim3(zero_blocks + per + longs), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab, row_bytes,
-                       zeros, (int)longs, (int)per, static_cast<unsigned char*>(grad_table), e, s);
+        r = launch_pdl(embed_order_kernel, dim3(zero_blocks + per + longs), EM_NT, 0, stream, tokens, (int)n, (int64_t)vocab,
+                       row_bytes, zeros, (int)longs, (int)per, static_cast<unsigned char*>(grad_table), e, s);
     }
     if (r != cudaSuccess) return cuda_fail(r);
     auto sum = [&](auto kernel) {
-        return launch_pdl(kernel, dim3(blocks + late), EM_SUM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts, scale,
-                          grad_table, s, blocks, (int64_t)vocab, zeros);
+        return launch_pdl(kernel, dim3(blocks + late), EM_SUM_NT, 0, stream, grad_out, grad_row_stride * e, units, (int)parts,
+                          scale, grad_table, s, blocks, (int64_t)vocab, zeros);
     };
     r = e == 4 ? (vec ? sum(embed_sum_kernel<4, true>) : sum(embed_sum_kernel<4, false>))
                : (vec ? sum(embed_sum_kernel<2, true>) : sum(embed_sum_kernel<2, false>));
