@@ -190,6 +190,14 @@ struct EmbedSort {
     __device__ __forceinline__ int parts_of(int positions) const { return positions > EM_HUGE ? min(windows, EM_PARTS) : 1; }
 };
 
+// Zeros, as a kernel that starts under the end of the one before and lets the next one start (a memset does neither: the gradient of
+// 30001 of 6562 x 768 36.4 us against 34.5, of 16 of 1000 x 256 8.2 against 6.6).
+__global__ void __launch_bounds__(EM_NT) embed_clear_kernel(uint4* p, int64_t units) {
+    pdl_wait_then_release();
+    const int64_t step = (int64_t)gridDim.x * EM_NT;
+    for (int64_t i = (int64_t)blockIdx.x * EM_NT + threadIdx.x; i < units; i += step) p[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 // Counts per id and bin, an atomic for a warp's equal ids.  TABLE: a CTA's positions are counted in shared memory first, ids in a
 // table (open addressing, never more than half full), so that an id or a bin that is much of the input costs an atomic a CTA: the
 // gradient of 300,000 positions of 151,936 ids, 8 wide, takes 96 us against 125, a million Zipf-distributed 340 against 450, but
@@ -750,7 +758,9 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
     const bool few = n <= EM_FEW;
     const unsigned late = few ? blocks_of(vocab * zeros, EM_SUM_NT) : 0u;  // CTAs of the last launch that write zeros then
     if (few && (!late || (int64_t)late + blocks > 0x7fffffff)) return B2S_ERR_UNSUPPORTED;
-    cudaError_t r = cudaMemsetAsync(workspace, 0, (size_t)zeroed, (cudaStream_t)stream);
+    const int64_t clear = zeroed / 16, clears = (clear + EM_NT - 1) / EM_NT, room = 8 * (int64_t)sms_here();
+    cudaError_t r = launch_pdl(embed_clear_kernel, dim3((unsigned)(clears < room ? clears : room)), EM_NT, 0, stream,
+                               static_cast<uint4*>(workspace), clear);
     if (few) {
         if (r == cudaSuccess)
             r = launch_pdl(embed_rank_kernel, dim3((unsigned)((n + EM_NT / EM_RANK - 1) / (EM_NT / EM_RANK))), EM_NT, 0, stream,
