@@ -253,6 +253,10 @@ __device__ __forceinline__ void pdl_wait_then_release() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// A kernel that runs beside its predecessor starts without a wait and ends with this one (in one thread of its grid): what follows it
+// in the stream then finds the predecessor complete too.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- warp / CTA primitives
 
 __device__ __forceinline__ float warp_max(float v) {

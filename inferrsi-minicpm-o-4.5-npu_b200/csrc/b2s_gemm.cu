@@ -12,8 +12,8 @@ namespace b2s {
 
 int cuda_fail(cudaError_t e);
 // x's rows in microscaled 8 bits and back in bf16 (b2s_mx.cu)
-cudaError_t mx8_quantize(const void* x, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream);
-cudaError_t mx8_dequantize(const void* codes, const void* scales, int64_t rows, int k, void* out, void* stream);
+cudaError_t mx8_quantize(const void* x, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, bool beside, void* stream);
+cudaError_t mx8_dequantize(const void* codes, const void* scales, int64_t rows, int k, void* out, bool beside, void* stream);
 int tensor_map_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t outer_stride, int box_inner,
                   int box_outer);
 
@@ -999,17 +999,19 @@ int linear_forward(const b2s_linear_args* l, const b2s_linear_kept* kept, void* 
     if (kept) {
         a.z8 = static_cast<uint8_t*>(kept->z_codes);
         a.z8_scale = static_cast<uint8_t*>(kept->z_scales);
-        if (kept->x_codes) {
-            const cudaError_t e = mx8_quantize(l->x, l->rows, l->in_features, l->x_row_stride, kept->x_codes, kept->x_scales, stream);
-            if (e != cudaSuccess) return cuda_fail(e);
-        }
     } else if (few_rows(l->rows, l->out_features, l->in_features)) {
         const cudaError_t e = linear_rows(a, l->x, l->x_row_stride, l->weight, l->weight_row_stride, l->in_features, stream);
         return e == cudaSuccess ? B2S_OK : cuda_fail(e);
     }
     const Operand x = {l->x, l->x_row_stride}, w = {l->weight, l->weight_row_stride};
-    return a.z8 ? gemm<false, false, EPI_KEPT>(x, w, l->in_features, a, stream)
-                : gemm<false, false, EPI_LINEAR>(x, w, l->in_features, a, stream);
+    int rc = a.z8 ? gemm<false, false, EPI_KEPT>(x, w, l->in_features, a, stream)
+                  : gemm<false, false, EPI_LINEAR>(x, w, l->in_features, a, stream);
+    if (rc == B2S_OK && kept && kept->x_codes) {  // on the SMs' spare threads while the product runs
+        const cudaError_t e =
+            mx8_quantize(l->x, l->rows, l->in_features, l->x_row_stride, kept->x_codes, kept->x_scales, true, stream);
+        if (e != cudaSuccess) rc = cuda_fail(e);
+    }
+    return rc;
 }
 
 }  // namespace
@@ -1082,12 +1084,6 @@ int linear_backward(const b2s_linear_grad_args* l, const b2s_linear_kept* kept, 
         (l->grad_weight && !x_ok))
         return B2S_ERR_INVALID;
     Operand x = {l->x, l->x_row_stride};
-    if (kept && l->grad_weight) {  // x as it was kept, in the products' type (exactly, but below bf16's normal range)
-        void* back = static_cast<unsigned char*>(l->workspace) + up(plain, 256);
-        const cudaError_t e = mx8_dequantize(kept->x_codes, kept->x_scales, l->rows, l->in_features, back, stream);
-        if (e != cudaSuccess) return cuda_fail(e);
-        x = {back, l->in_features};
-    }
     const void* z = kept ? kept->z_codes : l->preact;
     const int64_t z_stride = kept ? mx_blocks(l->out_features) * 32 : l->preact_row_stride;
     const int64_t ldz = up(l->out_features, 8);
@@ -1139,6 +1135,13 @@ int linear_backward(const b2s_linear_grad_args* l, const b2s_linear_kept* kept, 
         if (rc != B2S_OK) return rc;
     }
     if (l->grad_weight) {
+        if (kept) {  // x as it was kept, in the products' type (exactly, but below bf16's normal range), beside what runs already
+            void* back = static_cast<unsigned char*>(l->workspace) + up(plain, 256);
+            const bool beside = l->grad_x || !direct || l->grad_bias;
+            const cudaError_t e = mx8_dequantize(kept->x_codes, kept->x_scales, l->rows, l->in_features, back, beside, stream);
+            if (e != cudaSuccess) return cuda_fail(e);
+            x = {back, l->in_features};
+        }
         b.M = l->out_features;
         b.out = l->grad_weight;
         rc = gemm<true, true, EPI_STORE>(dz, x, l->rows, b, stream);

@@ -45,6 +45,33 @@ def test_gradient(pkg, n, k, m, activation):
             assert bool(((got.double() - ref).abs() <= tol * (1 + 2.0 ** -8) + 2.0 ** -8 * ref.abs() + 2.0 ** -60).all())
 
 
+@pytest.mark.parametrize("n,k,m", [(4099, 768, 1537), (2000, 8192, 200), (300, 4096, 64), (64, 768, 6562), (1, 8, 8)])
+def test_what_is_kept_runs_beside_the_products(pkg, n, k, m):
+    """x is quantised beside the product and brought back beside the rows' gradient: from an x that the kernel in front has just
+    written, before the kernel behind writes it anew, every time the same, also with no other kernel in the call."""
+    ops = torch.ops.minicpmo_sampler
+    x, w, b, _, dy = operands(n, k, m, n + k)
+    none = torch.empty(0, (m + 31) // 32 * 32, device=DEV, dtype=torch.uint8), torch.empty((m + 31) // 32, 0, device=DEV, dtype=torch.uint8)
+    work = x.clone()
+
+    def run(again):
+        if again:
+            work.fill_(float("nan"))
+            work.copy_(x)
+        kept = ops.linear_kept(work, w, b, None, 3, True, True, None)
+        if again:
+            work.fill_(0.5)
+        plain = ops.linear_kept_grad(dy, w, *kept[1:3], *none, 0, False, True, False, None)[1]
+        return (*kept, plain, *ops.linear_kept_grad(dy, w, *kept[1:], 3, True, True, True, None),
+                ops.linear_kept_grad(dy, w, *kept[1:], 3, False, True, False, None)[1])
+    want = run(False)
+    torch.cuda.synchronize()
+    assert torch.equal(_mx.eight(x), (want[1][:, :k].view(torch.float8_e4m3fn).double()
+                                      * torch.exp2(want[2].double() - 127).t().repeat_interleave(32, 1)[:, :k]))
+    for _ in range(10):
+        assert all(torch.equal(p, q) for p, q in zip(run(True), want))
+
+
 @pytest.mark.parametrize("activation", [None, "silu"])
 def test_each_gradient_alone_and_twice(pkg, activation):
     x, w, b, r, dy = operands(70, 96, 130, 3)
