@@ -79,6 +79,7 @@ struct GemmArgs {
     uint8_t* z8;        // the pre-activation in microscaled 8 bits: [M][N rounded up to 32]
     uint8_t* z8_scale;  // [blocks of 32 columns][M]
     int early;  // the microscaled product: its B may be read before the kernel in front has completed
+    int group;  // row tiles taken together, 0: GM_GROUP x 128 rows
     // EPI_LSE: per row and half of a column tile (m, S, U), the token's value; EPI_DZ: the gradient's inputs
     float c, inv_t;
     const int64_t* tokens;
@@ -431,15 +432,23 @@ Plan plan_here(int M, int N, int64_t K, int epi);
 
 namespace {
 
-// Tile t (TM rows each) of the order that takes GM_GROUP x 128 rows at a time.
+// Tile t (TM rows each) of the order that takes GM_GROUP x 128 rows at a time, or `group` tiles.  In 32 bits where they hold it: each
+// role of a CTA asks for every tile, and a 64-bit division is some hundred instructions.
 template <int TM>
 __device__ __forceinline__ void tile_of(const GemmArgs& a, int64_t t, int* mt, int* nt) {
-    constexpr int GROUP = GM_GROUP * GM_M / TM;
-    const int64_t per = (int64_t)GROUP * a.tiles_n;
-    const int g = (int)(t / per), in = (int)(t % per);
-    const int gm = min(GROUP, a.tiles_m - g * GROUP);
-    *mt = g * GROUP + in % gm;
-    *nt = in / gm;
+    const int group = a.group ? a.group : GM_GROUP * GM_M / TM;
+    const int64_t per = (int64_t)group * a.tiles_n;
+    int g, in;
+    if ((((uint64_t)t | (uint64_t)per) >> 32) == 0) {
+        g = (int)((uint32_t)t / (uint32_t)per);
+        in = (int)((uint32_t)t - (uint32_t)g * (uint32_t)per);
+    } else {
+        g = (int)(t / per);
+        in = (int)(t % per);
+    }
+    const int gm = min(group, a.tiles_m - g * group);
+    *nt = gm == 1 ? in : (int)((uint32_t)in / (uint32_t)gm);
+    *mt = g * group + in - *nt * gm;
 }
 
 // The i-th piece of work of CTA (or pair) c of G: a tile and its k blocks [kb0, kb1); slot: where its sums go, -1 for a whole tile.
@@ -459,9 +468,11 @@ __device__ __forceinline__ bool piece_at(const GemmArgs& a, int i, Piece* p) {
     }
     const int64_t u = (int64_t)(i - a.waves) * G + c;
     if (u >= (int64_t)a.rest * a.split) return false;
-    p->tile = (int64_t)a.waves * G + u % a.rest;
+    p->tile = (int64_t)a.waves * G + u;
     if (a.split > 1) {
-        p->kb0 = (int)(u / a.rest) * a.chunk;
+        const int k = (int)u / a.rest;
+        p->tile -= (int64_t)k * a.rest;
+        p->kb0 = k * a.chunk;
         p->kb1 = min(a.nkb, p->kb0 + a.chunk);
         p->slot = (int)u;
     }
