@@ -27,11 +27,12 @@ constexpr int MX_NT = 256;
 constexpr int MX8_NT = 128;
 __host__ __device__ constexpr int mx_threads(bool eight) { return eight ? MX8_NT : MX_NT; }
 constexpr int MX_SEG = 256;  // elements of a row that a warp takes at a time: 8 a lane, the 8 blocks of a scale tile
-// Rows that a warp takes the same segment of, in flight together: 16 bytes a lane each of bf16, 32 of fp32.  One row after
-// another costs an addition or two for each address; segments taken as they come, with a division for each warp, were bound by
-// instruction issue (32768 x 4096 bf16 86 against 60 us there, 76 against 59 back: 5.7 TB/s).
-template <typename T>
-__host__ __device__ constexpr int mx_per(bool vec) { return sizeof(T) == 2 ? 8 : 4; }
+// A warp takes the same segment of PER rows, in flight together: of fp32 4, 32 bytes a lane each (2: 2000 x 4096 8.2 us against 7.4);
+// of bf16 8, 16 bytes each, where that makes more warps than the SMs hold at once, 4 where they are fewer (4 against 8: 300 x 4096
+// 2.9 us to 3.3, 2000 x 4095 7.5 to 8.9, but 4099 x 4096 10.4 to 9.9 and 32768 x 4096 67 to 60).  One row after another costs an
+// addition or two for each address; segments taken as they come, with a division for each warp, were bound by instruction issue
+// (32768 x 4096 bf16 86 against 60 us there, 76 against 59 back: 5.7 TB/s).
+bool mx_many(int64_t rows, int64_t k) { return (rows + 7) / 8 * mx_tiles(k) > 32 * (int64_t)sms_here(); }
 // A CTA's warps: `wide` of them (1, 2, 4, 8) on segments side by side, the others on further rows.
 struct MxGrid {
     int64_t r0, tile, step;  // first row; first segment and the next one's distance
@@ -186,11 +187,11 @@ __device__ __forceinline__ void mx_turn_out(unsigned short* p, int n, uint32_t* 
 
 // VEC: 16-byte aligned rows.  EIGHT: E4M3 codes, a byte each, and scales [blocks][rows]; else the 4-bit layout, whose scale
 // tiles' rows past the matrix get zeros.
-template <typename T, bool VEC, bool EIGHT>
+template <typename T, bool VEC, bool EIGHT, int PER>
 __global__ void __launch_bounds__(mx_threads(EIGHT)) mx_quantize_kernel(const T* x, int64_t row_stride, int64_t rows, int k,
                                                                         uint8_t* codes, uint8_t* scales, int wide, int beside) {
     static_assert(!EIGHT || (VEC && sizeof(T) == 2), "8 bits are a projection's x");
-    constexpr int E = EIGHT ? 8 : 2, PER = mx_per<T>(VEC), BYTES = EIGHT ? 8 : 4;  // of a lane's codes
+    constexpr int E = EIGHT ? 8 : 2, BYTES = EIGHT ? 8 : 4;  // of a lane's codes
     __shared__ __align__(16) uint32_t turn[VEC ? 1 : MX_NT / 32][VEC ? 4 : MX_SEG * sizeof(T) / 4];
     if (!EIGHT || !beside) pdl_wait_then_release();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -242,11 +243,11 @@ __global__ void __launch_bounds__(mx_threads(EIGHT)) mx_quantize_kernel(const T*
 
 // The way back, to bf16 or fp32.  A lane takes 8 elements, 16 bytes of bf16; to fp32 4 of either half of a segment, so that a
 // store's lanes write one line after another (8 at once: 16384 x 4096 67 against 58 us).
-template <typename T, bool VEC, bool EIGHT>
+template <typename T, bool VEC, bool EIGHT, int PER>
 __global__ void __launch_bounds__(mx_threads(EIGHT)) mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows,
                                                                           int k, T* out, int64_t out_stride, int wide, int beside) {
     static_assert(!EIGHT || VEC, "8 bits are a projection's x");
-    constexpr int PER = mx_per<T>(true), H = sizeof(T) == 4 ? 2 : 1, N = 8 / H;  // rows; loads a segment, elements of each
+    constexpr int H = sizeof(T) == 4 ? 2 : 1, N = 8 / H;  // loads a segment, elements of each
     static_assert(!EIGHT || H == 1, "8 bits come back as bf16");
     __shared__ __align__(16) uint32_t turn[VEC ? 1 : MX_NT / 32][VEC ? 4 : MX_SEG * sizeof(T) / 4];
     if (!EIGHT || !beside) pdl_wait_then_release();
@@ -356,28 +357,36 @@ dim3 mx_grid(int64_t rows, int64_t k, int per, int warps) {
     return dim3((unsigned)((rows + each - 1) / each), (unsigned)(y < 65535 ? y : 65535));
 }
 cudaError_t mx_quantize(const void* x, int dtype, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream) {
+    const int64_t all = (rows + 127) / 128 * 128;
     auto go = [&](auto kernel, auto* p, int per) {
-        return launch_pdl(kernel, mx_grid((rows + 127) / 128 * 128, k, per, MX_NT / 32), MX_NT, 0, stream, p, row_stride, rows, k,
+        return launch_pdl(kernel, mx_grid(all, k, per, MX_NT / 32), MX_NT, 0, stream, p, row_stride, rows, k,
                           static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), mx_wide(k, MX_NT / 32), 0);
     };
-    auto typed = [&](auto* p) {
-        using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-        const bool vec = aligned16(x) && row_stride * sizeof(T) % 16 == 0;
-        return vec ? go(mx_quantize_kernel<T, true, false>, p, mx_per<T>(true))
-                   : go(mx_quantize_kernel<T, false, false>, p, mx_per<T>(false));
-    };
-    return dtype == B2S_DTYPE_F32 ? typed(static_cast<const float*>(x)) : typed(static_cast<const unsigned short*>(x));
+    const bool vec = aligned16(x) && row_stride * (dtype == B2S_DTYPE_F32 ? 4 : 2) % 16 == 0;
+    if (dtype == B2S_DTYPE_F32) {
+        const float* p = static_cast<const float*>(x);
+        return go(vec ? mx_quantize_kernel<float, true, false, 4> : mx_quantize_kernel<float, false, false, 4>, p, 4);
+    }
+    using T = unsigned short;
+    const T* p = static_cast<const T*>(x);
+    return mx_many(all, k) ? go(vec ? mx_quantize_kernel<T, true, false, 8> : mx_quantize_kernel<T, false, false, 8>, p, 8)
+                           : go(vec ? mx_quantize_kernel<T, true, false, 4> : mx_quantize_kernel<T, false, false, 4>, p, 4);
 }
 cudaError_t mx_dequantize(const void* codes, const void* scales, int64_t rows, int k, int dtype, void* out, int64_t out_stride,
                           void* stream) {
-    auto typed = [&](auto* p) {
-        using T = std::remove_pointer_t<decltype(p)>;
-        const bool vec = aligned16(out) && out_stride * sizeof(T) % 16 == 0;
-        return launch_pdl(vec ? mx_dequantize_kernel<T, true, false> : mx_dequantize_kernel<T, false, false>,
-                          mx_grid(rows, k, mx_per<T>(true), MX_NT / 32), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
+    auto go = [&](auto kernel, auto* p, int per) {
+        return launch_pdl(kernel, mx_grid(rows, k, per, MX_NT / 32), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
                           static_cast<const uint8_t*>(scales), rows, k, p, out_stride, mx_wide(k, MX_NT / 32), 0);
     };
-    return dtype == B2S_DTYPE_F32 ? typed(static_cast<float*>(out)) : typed(static_cast<unsigned short*>(out));
+    const bool vec = aligned16(out) && out_stride * (dtype == B2S_DTYPE_F32 ? 4 : 2) % 16 == 0;
+    if (dtype == B2S_DTYPE_F32) {
+        float* p = static_cast<float*>(out);
+        return go(vec ? mx_dequantize_kernel<float, true, false, 4> : mx_dequantize_kernel<float, false, false, 4>, p, 4);
+    }
+    using T = unsigned short;
+    T* p = static_cast<T*>(out);
+    return mx_many(rows, k) ? go(vec ? mx_dequantize_kernel<T, true, false, 8> : mx_dequantize_kernel<T, false, false, 8>, p, 8)
+                            : go(vec ? mx_dequantize_kernel<T, true, false, 4> : mx_dequantize_kernel<T, false, false, 4>, p, 4);
 }
 
 // ------------------------------------------------------------------ the product of few rows
@@ -585,13 +594,13 @@ MxWork mx_work(int64_t rows, int64_t k) {
 // waited for what came before it.
 cudaError_t mx8_quantize(const void* x, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, bool beside, void* stream) {
     using T = unsigned short;
-    return launch_pdl(mx_quantize_kernel<T, true, true>, mx_grid(rows, k, mx_per<T>(true), MX8_NT / 32), MX8_NT, 0, stream,
+    return launch_pdl(mx_quantize_kernel<T, true, true, 8>, mx_grid(rows, k, 8, MX8_NT / 32), MX8_NT, 0, stream,
                       static_cast<const T*>(x), row_stride, rows, k, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
                       mx_wide(k, MX8_NT / 32), (int)beside);
 }
 cudaError_t mx8_dequantize(const void* codes, const void* scales, int64_t rows, int k, void* out, bool beside, void* stream) {
     using T = unsigned short;
-    return launch_pdl(mx_dequantize_kernel<T, true, true>, mx_grid(rows, k, mx_per<T>(true), MX8_NT / 32), MX8_NT, 0, stream,
+    return launch_pdl(mx_dequantize_kernel<T, true, true, 8>, mx_grid(rows, k, 8, MX8_NT / 32), MX8_NT, 0, stream,
                       static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, k, static_cast<T*>(out),
                       (int64_t)k, mx_wide(k, MX8_NT / 32), (int)beside);
 }
