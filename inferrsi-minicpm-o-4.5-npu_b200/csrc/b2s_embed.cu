@@ -13,6 +13,8 @@
 // written at once, of one that goes on the sums are joined by whoever completes them, in order.
 #include <string.h>
 
+#include <type_traits>
+
 #include "../../include/b2s_sampler.h"
 #include "b2s_device.cuh"
 #include "b2s_gemm.cuh"
@@ -30,7 +32,12 @@ constexpr int EM_NT = 256;
 constexpr int EM_JOIN = 4;     // 2^4 sums joined at a time
 constexpr int EM_SHORT = 64;   // positions of an id that are put in order by comparison
 constexpr int EM_BINS = 4096;  // at most, of ids counted together
-constexpr int EM_UNITS = 64;   // 16-byte units (or elements) of a row that a warp takes
+constexpr int EM_UNITS = 64;   // 16-byte units of a row that a warp takes
+constexpr int EM_ELEMENTS = 256;  // or single elements, of rows that are not aligned
+// Where rows are summed, of single fp32 elements EM_WIDE (30001 x 1001 81 us with 64, 56 with 128, 52 with 256, but 300 x 33 9.9,
+// 10.3 and 11.6), of bf16 64 (61; 77 with 256).
+constexpr int EM_WIDE = 128;
+__host__ __device__ constexpr int em_units(bool vec, int e) { return vec || e == 2 ? EM_UNITS : EM_WIDE; }
 constexpr int EM_MID = 512;    // ... by a CTA in shared memory; beyond, by bitmaps
 constexpr int EM_HUGE = 4096;  // ... by several CTAs, at most EM_PARTS
 constexpr int EM_PARTS = 64;
@@ -108,24 +115,26 @@ __device__ __forceinline__ int64_t token_at(const int64_t* tokens, int64_t i, in
     return t < 0 ? -1 : t;
 }
 
-// grid: a warp per row and part of EM_UNITS units (128 units a warp: 30001 x 768 fp32 21 us either way; 32: 26)
-template <int E, bool VEC>
+// grid: a warp per row and part of U units, all in flight together.  U is the least that holds a row, up to 128 (131,072 x 768
+// fp32 83 us against 98 with 64; 200,000 x 256 bf16 29.6 with 32 against 34 with 64 and 48 with 128), of unaligned rows 256
+// elements (30001 x 1001 bf16 30 us; 64 with 64).
+template <int E, bool VEC, int U>
 __global__ void __launch_bounds__(EM_NT) embed_kernel(const int64_t* tokens, int64_t n, const void* table,
                                                       int64_t row_bytes, int64_t vocab, int64_t units, int64_t parts, float s,
                                                       void* out, uint32_t* status) {
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), i = w / parts, u0 = (w % parts) * EM_UNITS + lane;
+    const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), i = w / parts, u0 = (w % parts) * U + lane;
     if (i >= n) return;
     const int64_t t = token_at(tokens, i, vocab, u0 == 0 ? status : nullptr);
     const unsigned char* src = static_cast<const unsigned char*>(table) + (t < 0 ? 0 : t) * row_bytes;
     unsigned char* dst = static_cast<unsigned char*>(out) + i * units * Unit<E, VEC>::N * E;
-    RawUnit<E, VEC> q[EM_UNITS / 32];
+    RawUnit<E, VEC> q[U / 32];
 #pragma unroll
-    for (int j = 0; j < EM_UNITS / 32; ++j)
+    for (int j = 0; j < U / 32; ++j)
         if (t >= 0 && u0 + 32 * j < units) q[j].load(src, u0 + 32 * j);
 #pragma unroll
-    for (int j = 0; j < EM_UNITS / 32; ++j) {
+    for (int j = 0; j < U / 32; ++j) {
         Unit<E, VEC> v;
         v.zero();
         if (t >= 0) v.add(q[j]);
@@ -133,21 +142,24 @@ __global__ void __launch_bounds__(EM_NT) embed_kernel(const int64_t* tokens, int
     }
 }
 
-// The same from a microscaled table: a unit is 8 elements, 4 bytes of codes.
+// The same from a microscaled table: a unit is 8 elements, 4 bytes of codes.  U: 128 where that takes an aligned row at once
+// (131,072 x 768 62.6 us against 72.6 with 64; 16000 x 1001 51 against 48), 64 of longer ones (2000 x 4096 7.5; 128: 7.8), 32 of
+// short ones (100,000 x 256 22.0; 64: 23.5).
+template <int U>
 __global__ void __launch_bounds__(EM_NT) embed_mx_kernel(const int64_t* tokens, int64_t n, const uint8_t* codes,
                                                          const uint8_t* scales, int64_t vocab, int width, int64_t pieces, float s,
                                                          __nv_bfloat16* out, int vec, uint32_t* status) {
     pdl_wait_then_release();
     const int lane = threadIdx.x & 31, units = (width + 7) / 8;
     const int64_t w = (int64_t)blockIdx.x * (EM_NT / 32) + (threadIdx.x >> 5), i = w / pieces;
-    const int u0 = (int)(w % pieces) * EM_UNITS + lane;
+    const int u0 = (int)(w % pieces) * U + lane;
     if (i >= n) return;
     const int64_t t = token_at(tokens, i, vocab, lane == 0 && u0 == 0 ? status : nullptr);
     const int64_t bytes = mx_row_bytes(width), tiles = mx_tiles(width);
-    uint32_t c[EM_UNITS / 32];
-    float f[EM_UNITS / 32];
+    uint32_t c[U / 32];
+    float f[U / 32];
 #pragma unroll
-    for (int j = 0; j < EM_UNITS / 32; ++j) {
+    for (int j = 0; j < U / 32; ++j) {
         const int u = u0 + 32 * j;
         c[j] = 0;
         f[j] = 0.0f;
@@ -157,7 +169,7 @@ __global__ void __launch_bounds__(EM_NT) embed_mx_kernel(const int64_t* tokens, 
         }
     }
 #pragma unroll
-    for (int j = 0; j < EM_UNITS / 32; ++j) {
+    for (int j = 0; j < U / 32; ++j) {
         const int u = u0 + 32 * j;
         if (u >= units) break;
         float v[8];
@@ -190,8 +202,8 @@ struct EmbedSort {
     __device__ __forceinline__ int parts_of(int positions) const { return positions > EM_HUGE ? min(windows, EM_PARTS) : 1; }
 };
 
-// Zeros, as a kernel that starts under the end of the one before and lets the next one start (a memset does neither: the gradient of
-// 30001 of 6562 x 768 36.4 us against 34.5, of 16 of 1000 x 256 8.2 against 6.6).
+// Zeros, as a kernel that starts under the end of the one before and lets the next one start (a memset does neither: the gradient
+// of 30001 of 6562 x 768 36.4 us against 34.5, of 16 of 1000 x 256 8.2 against 6.6).
 __global__ void __launch_bounds__(EM_NT) embed_clear_kernel(uint4* p, int64_t units) {
     pdl_wait_then_release();
     const int64_t step = (int64_t)gridDim.x * EM_NT;
@@ -381,8 +393,8 @@ __device__ __forceinline__ void em_zero(int64_t w, int64_t vocab, int64_t row_by
         else *reinterpret_cast<unsigned short*>(q) = 0;
 }
 
-// The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order.  Where one bitmap covers all
-// positions they are marked in it and read back.  Of longer inputs, up to EM_MID by comparison in shared memory, more by bitmaps
+// The first `longs` CTAs put the positions of the ids with more than EM_SHORT of them in ascending order.  Where one bitmap covers
+// all positions they are marked in it and read back.  Of longer inputs, up to EM_MID by comparison in shared memory, more by bitmaps
 // of EM_WINDOW positions, each behind as many as come before it; of an id with more than EM_HUGE several CTAs each do some of the
 // windows (300,000 equal ids 8 wide 226 us against 483 by one CTA; a million Zipf-distributed 340 against 425, and 732 with
 // bitmaps for up to EM_MID too; with one bitmap comparisons cost 30001 of 6562 40 against 37).  The next `orders` CTAs do the
@@ -465,7 +477,7 @@ template <int E, bool VEC>
 __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* grad, int64_t row_bytes, int64_t units, int parts,
                                                                  float s, void* out, EmbedSort e, unsigned sums, int64_t vocab,
                                                                  int64_t zeros) {
-    constexpr int N = Unit<E, VEC>::N, W = EM_UNITS / 32;
+    constexpr int N = Unit<E, VEC>::N, W = em_units(VEC, E) / 32;
     pdl_wait_then_release();
     if (blockIdx.x >= sums) {
         em_zero((int64_t)(blockIdx.x - sums) * (EM_SUM_NT / 32) + (threadIdx.x >> 5), vocab, units * N * E, zeros,
@@ -475,7 +487,7 @@ __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* gra
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * (EM_SUM_NT / 32) + (threadIdx.x >> 5), chunk = w / parts;
     const int part = (int)(w % parts), total = *e.total;
-    const int64_t u0 = (int64_t)part * EM_UNITS + lane, width = units * N, k0 = chunk << e.chunk;
+    const int64_t u0 = (int64_t)part * em_units(VEC, E) + lane, width = units * N, k0 = chunk << e.chunk;
     if (k0 >= total) return;
     const int held = (int)min((int64_t)1 << e.chunk, total - k0);
     const int pos = lane < held ? e.order[k0 + lane] : 0, id = lane < held ? e.id[k0 + lane] : -1;
@@ -629,7 +641,7 @@ __global__ void __launch_bounds__(EM_SUM_NT, 8) embed_sum_kernel(const void* gra
 }
 
 int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
-int64_t parts_of(int64_t units) { return (units + EM_UNITS - 1) / EM_UNITS; }
+int64_t parts_of(int64_t units, bool vec, int e) { return (units + em_units(vec, e) - 1) / em_units(vec, e); }
 // The workspace's arrays, and its bytes, `zeroed` of them to be zero; the parts of a row are those of single elements, where rows
 // may be unaligned.
 int64_t embed_layout(int64_t n, int64_t vocab, int64_t width, unsigned char* at, EmbedSort* e, int64_t* zeroed) {
@@ -649,7 +661,7 @@ int64_t embed_layout(int64_t n, int64_t vocab, int64_t width, unsigned char* at,
     e->windows = (int)((n - 1) / EM_WINDOW + 1);
     e->count = reinterpret_cast<int*>(take(up(vocab, 4) * 4));
     e->bin = reinterpret_cast<int*>(take((int64_t)e->bins * 4));
-    e->arrived = reinterpret_cast<int*>(take((int64_t)e->slots * parts_of(width) * 4));
+    e->arrived = reinterpret_cast<int*>(take((int64_t)e->slots * parts_of(width, false, 2) * 4));
     e->longs = reinterpret_cast<int*>(take(4));
     *zeroed = used;
     e->total = reinterpret_cast<int*>(take(4));
@@ -690,15 +702,23 @@ int b2s_embedding(const int64_t* tokens, int32_t n, const void* table, int32_t d
     if (!tokens || !table || !out || ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) & (e - 1)))
         return B2S_ERR_INVALID;
     const bool vec = aligned16(table) && aligned16(out) && (int64_t)width * e % 16 == 0 && row_stride * e % 16 == 0;
-    const int64_t units = vec ? (int64_t)width * e / 16 : width, pieces = (units + EM_UNITS - 1) / EM_UNITS;
+    const int64_t units = vec ? (int64_t)width * e / 16 : width;
+    const int64_t each = !vec ? EM_ELEMENTS : units <= 32 ? 32 : units <= 64 ? 64 : 128;
+    const int64_t pieces = (units + each - 1) / each;
     const unsigned blocks = blocks_of(n * pieces);
     if (!blocks) return B2S_ERR_UNSUPPORTED;
     auto go = [&](auto kernel) {
         return launch_pdl(kernel, dim3(blocks), EM_NT, 0, stream, tokens, (int64_t)n, table, row_stride * e, (int64_t)vocab,
                           units, pieces, scale, out, status);
     };
-    const cudaError_t r = e == 4 ? (vec ? go(embed_kernel<4, true>) : go(embed_kernel<4, false>))
-                                 : (vec ? go(embed_kernel<2, true>) : go(embed_kernel<2, false>));
+    auto typed = [&](auto bytes) {
+        constexpr int E = decltype(bytes)::value;
+        if (!vec) return go(embed_kernel<E, false, EM_ELEMENTS>);
+        return each == 32   ? go(embed_kernel<E, true, 32>)
+               : each == 64 ? go(embed_kernel<E, true, 64>)
+                            : go(embed_kernel<E, true, 128>);
+    };
+    const cudaError_t r = e == 4 ? typed(std::integral_constant<int, 4>()) : typed(std::integral_constant<int, 2>());
     return r == cudaSuccess ? B2S_OK : cuda_fail(r);
 }
 
@@ -710,13 +730,17 @@ int b2s_embedding_mx(const int64_t* tokens, int32_t n, const void* codes, const 
     if (n == 0) return B2S_OK;
     if (!tokens || !codes || !scales || !out || !aligned16(codes) || !aligned16(scales) || (reinterpret_cast<uintptr_t>(out) & 1))
         return B2S_ERR_INVALID;
-    const int64_t pieces = ((width + 7) / 8 + EM_UNITS - 1) / EM_UNITS;
+    const bool vec = aligned16(out) && width % 8 == 0;
+    const int64_t units = (width + 7) / 8, each = units <= 32 ? 32 : vec && units > 64 && units <= 128 ? 128 : 64;
+    const int64_t pieces = (units + each - 1) / each;
     const unsigned blocks = blocks_of(n * pieces);
     if (!blocks) return B2S_ERR_UNSUPPORTED;
-    const cudaError_t r = launch_pdl(embed_mx_kernel, dim3(blocks), EM_NT, 0, stream, tokens, (int64_t)n,
-                                     static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), (int64_t)vocab,
-                                     (int)width, pieces, scale, static_cast<__nv_bfloat16*>(out),
-                                     (int)(aligned16(out) && width % 8 == 0), status);
+    auto go = [&](auto kernel) {
+        return launch_pdl(kernel, dim3(blocks), EM_NT, 0, stream, tokens, (int64_t)n, static_cast<const uint8_t*>(codes),
+                          static_cast<const uint8_t*>(scales), (int64_t)vocab, (int)width, pieces, scale,
+                          static_cast<__nv_bfloat16*>(out), (int)vec, status);
+    };
+    const cudaError_t r = each == 32 ? go(embed_mx_kernel<32>) : each == 64 ? go(embed_mx_kernel<64>) : go(embed_mx_kernel<128>);
     return r == cudaSuccess ? B2S_OK : cuda_fail(r);
 }
 
@@ -750,7 +774,7 @@ int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, i
         workspace_bytes < embed_layout(n, vocab, width, static_cast<unsigned char*>(workspace), &s, &zeroed))
         return B2S_ERR_INVALID;
     const bool vec = aligned16(grad_out) && aligned16(grad_table) && (int64_t)width * e % 16 == 0 && grad_row_stride * e % 16 == 0;
-    const int64_t units = vec ? (int64_t)width * e / 16 : width, parts = parts_of(units);
+    const int64_t units = vec ? (int64_t)width * e / 16 : width, parts = parts_of(units, vec, e);
     const int64_t row_bytes = (int64_t)width * e, zeros = (row_bytes + EM_ZERO - 1) / EM_ZERO;
     const unsigned per = (unsigned)(((int64_t)n + EM_NT - 1) / EM_NT);
     const unsigned blocks = blocks_of((((int64_t)n - 1 >> s.chunk) + 1) * parts, EM_SUM_NT), zero_blocks = blocks_of(vocab * zeros);

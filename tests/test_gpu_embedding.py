@@ -97,6 +97,18 @@ def test_lookup_of_a_4_bit_table(pkg, width):
         assert torch.equal(y.double(), want.bfloat16().double())  # 12 times two bits is exact before the rounding
 
 
+@pytest.mark.parametrize("width", [8, 120, 128, 136, 248, 256, 264, 512, 520, 768, 1001, 1016, 1024, 1032, 2056])
+def test_rows_of_every_length(pkg, width):
+    """Rows that a warp takes at once or in pieces of each size, of every kind of table, and into outputs of 4-bit tables that are not
+    aligned."""
+    g = gen(width)
+    tokens = torch.randint(-1, 90, (301,), device=DEV, generator=g)
+    table = torch.randn(90, width, device=DEV, generator=g)
+    for t in (table, table.bfloat16()):
+        assert torch.equal(pkg.embedding.lookup(tokens, t, scale=2.0).double(), want_rows(tokens, t, 2.0))
+    assert torch.equal(pkg.embedding.lookup(tokens, pkg.mx.quantize(table)).double(), want_rows(tokens, _mx.four(table), 1.0))
+
+
 def cases():
     yield 1, 1, 8, "equal"
     yield 33, 5, 24, "equal"          # one id in two pieces
