@@ -27,7 +27,7 @@ constexpr int MX_NT = 256;
 constexpr int MX8_NT = 128;
 __host__ __device__ constexpr int mx_threads(bool eight) { return eight ? MX8_NT : MX_NT; }
 constexpr int MX_SEG = 256;  // elements of a row that a warp takes at a time: 8 a lane, the 8 blocks of a scale tile
-// A warp takes the same segment of PER rows, in flight together: of fp32 4, 32 bytes a lane each (2: 2000 x 4096 8.2 us against 7.4);
+// A warp takes the same segment of PER rows, in flight together: of fp32 4, 32 bytes a lane each (2: 2000 x 4096 8.2 us, 4 7.4);
 // of bf16 8, 16 bytes each, where that makes more warps than the SMs hold at once, 4 where they are fewer (4 against 8: 300 x 4096
 // 2.9 us to 3.3, 2000 x 4095 7.5 to 8.9, but 4099 x 4096 10.4 to 9.9 and 32768 x 4096 67 to 60).  One row after another costs an
 // addition or two for each address; segments taken as they come, with a division for each warp, were bound by instruction issue
@@ -345,48 +345,163 @@ __global__ void __launch_bounds__(mx_threads(EIGHT)) mx_dequantize_kernel(const 
     if (EIGHT && beside && blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-int mx_wide(int64_t k, int warps) {
-    const int64_t t = mx_tiles(k);
-    const int w = t > 4 ? 8 : t > 2 ? 4 : t > 1 ? 2 : 1;
-    return w < warps ? w : warps;
+// Rows of up to 128 elements, R of them side by side in a warp's 32 lanes (8 of up to 32 elements, 4 of 64, 2), MXN_PER times:
+// 262,144 x 128 bf16 17.6 us there and 17.0 back, x 64 9.3, where the kernels above, a row a warp, take 43 and 34, 42 and 34.  Not
+// back to unaligned rows, whose stores those put together (65536 x 100 23 against 11).
+constexpr int MXN_PER = 4;
+constexpr int MX_NARROW = 128;
+template <typename T, bool VEC, int R>
+__global__ void __launch_bounds__(MX_NT) mx_quantize_narrow_kernel(const T* x, int64_t row_stride, int64_t rows, int k,
+                                                                   uint8_t* codes, uint8_t* scales) {
+    constexpr int L = 32 / R;  // lanes of a row
+    pdl_wait_then_release();
+    const int lane = threadIdx.x & 31, col = lane % L, n = 8 * col, block = col >> 2, nb = (int)mx_blocks(k);
+    const int64_t all = (rows + 127) / 128 * 128;  // the scale tiles' rows past the matrix get zeros
+    const int64_t r0 = ((int64_t)blockIdx.x * (MX_NT / 32) + (threadIdx.x >> 5)) * (R * MXN_PER) + lane / L;
+    MxWords<T> in[MXN_PER];
+#pragma unroll
+    for (int j = 0; j < MXN_PER; ++j) {
+        const int64_t r = r0 + j * R;
+        const T* q = x + r * row_stride + n;
+        if (VEC && r < rows && n + 8 <= k) in[j] = mx_words(q);
+        else in[j] = mx_words(q, r < rows ? k - n : 0);
+    }
+#pragma unroll
+    for (int j = 0; j < MXN_PER; ++j) {
+        const int64_t r = r0 + j * R;
+        uint32_t most = mx_most(in[j]);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const uint32_t code = mx_scale_code<2>(most);
+        float u[8];
+        mx_times(in[j], mx_inverse(code), u);
+        uint32_t word = code;  // the row's blocks in its first lane
+        if (L >= 8) word |= __shfl_down_sync(0xffffffffu, word, 4) << 8;
+        if (L >= 16) word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
+        if (col == 0 && r < all) {
+            uint32_t* s = reinterpret_cast<uint32_t*>(scales + mx_scale_at(r, 0, 1));
+            s[0] = word;
+            s[128] = 0;  // blocks 4 to 7
+        }
+        if (r < rows && block < nb) *reinterpret_cast<uint32_t*>(codes + (r * nb + block) * 16 + 4 * (col & 3)) = mx_encode8(u);
+    }
 }
-dim3 mx_grid(int64_t rows, int64_t k, int per, int warps) {
-    const int wide = mx_wide(k, warps);
+// 8 elements a lane to bf16, 4 to fp32, 16 bytes each.
+template <typename T, int R>
+__global__ void __launch_bounds__(MX_NT) mx_dequantize_narrow_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                                                     int k, T* out, int64_t out_stride) {
+    constexpr int L = 32 / R, N = 16 / sizeof(T);
+    pdl_wait_then_release();
+    const int lane = threadIdx.x & 31, n = N * (lane % L), block = n >> 5, nb = (int)mx_blocks(k);
+    const int64_t r0 = ((int64_t)blockIdx.x * (MX_NT / 32) + (threadIdx.x >> 5)) * (R * MXN_PER) + lane / L;
+    uint32_t c[MXN_PER], f[MXN_PER];
+#pragma unroll
+    for (int j = 0; j < MXN_PER; ++j) {
+        const int64_t r = r0 + j * R;
+        c[j] = f[j] = 0;
+        if (r < rows && block < nb) {
+            const uint8_t* p = codes + (r * nb + block) * 16 + n % 32 / 2;
+            if constexpr (N == 8) c[j] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            else c[j] = __ldg(reinterpret_cast<const unsigned short*>(p));
+            f[j] = __ldg(scales + mx_scale_at(r, block, 1));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MXN_PER; ++j) {
+        const int64_t r = r0 + j * R;
+        if (r >= rows || n >= k) continue;
+        float v[8];
+        mx_decode8(c[j], v);
+        const float s = mx_scale(f[j]);
+        T* p = out + r * out_stride + n;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= s;
+        if constexpr (N == 8) {
+            mx_store8(p, min(8, k - n), true, v);
+        } else if (n + 4 <= k) {
+            __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < k) p[i] = v[i];
+        }
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Segments that a CTA's warps take side by side: as many as leave no warp without one where there are many (65536 x 768 bf16 24.2
+// us against 26.2, x 576 27.6 against 30.8), else as many as leave each one (4099 x 768 3.9 against 4.3).
+int mx_wide(int64_t k, int warps, bool many) {
+    const int64_t t = mx_tiles(k), w = many ? t & -t : t > 4 ? 8 : t > 2 ? 4 : t;
+    return w < warps ? (int)w : warps;
+}
+dim3 mx_grid(int64_t rows, int64_t k, int per, int warps, int wide) {
     const int64_t each = (int64_t)per * (warps / wide), y = (mx_tiles(k) + wide - 1) / wide;
     return dim3((unsigned)((rows + each - 1) / each), (unsigned)(y < 65535 ? y : 65535));
 }
-cudaError_t mx_quantize(const void* x, int dtype, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, void* stream) {
+cudaError_t mx_quantize(const void* x, int dtype, int64_t rows, int k, int64_t row_stride, void* codes, void* scales,
+                        void* stream) {
     const int64_t all = (rows + 127) / 128 * 128;
+    const bool many = mx_many(all, k);
+    const int wide = mx_wide(k, MX_NT / 32, many);
+    auto narrow = [&](auto* p, bool vec) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        auto run = [&](auto kernel, int r) {
+            const int64_t each = r * MXN_PER * (MX_NT / 32);
+            return launch_pdl(kernel, dim3((unsigned)((all + each - 1) / each)), MX_NT, 0, stream, p, row_stride, rows, k,
+                              static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
+        };
+        return k <= 32   ? run(vec ? mx_quantize_narrow_kernel<T, true, 8> : mx_quantize_narrow_kernel<T, false, 8>, 8)
+               : k <= 64 ? run(vec ? mx_quantize_narrow_kernel<T, true, 4> : mx_quantize_narrow_kernel<T, false, 4>, 4)
+                         : run(vec ? mx_quantize_narrow_kernel<T, true, 2> : mx_quantize_narrow_kernel<T, false, 2>, 2);
+    };
     auto go = [&](auto kernel, auto* p, int per) {
-        return launch_pdl(kernel, mx_grid(all, k, per, MX_NT / 32), MX_NT, 0, stream, p, row_stride, rows, k,
-                          static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), mx_wide(k, MX_NT / 32), 0);
+        return launch_pdl(kernel, mx_grid(all, k, per, MX_NT / 32, wide), MX_NT, 0, stream, p, row_stride, rows, k,
+                          static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), wide, 0);
     };
     const bool vec = aligned16(x) && row_stride * (dtype == B2S_DTYPE_F32 ? 4 : 2) % 16 == 0;
     if (dtype == B2S_DTYPE_F32) {
         const float* p = static_cast<const float*>(x);
+        if (k <= MX_NARROW) return narrow(p, vec);
         return go(vec ? mx_quantize_kernel<float, true, false, 4> : mx_quantize_kernel<float, false, false, 4>, p, 4);
     }
     using T = unsigned short;
     const T* p = static_cast<const T*>(x);
-    return mx_many(all, k) ? go(vec ? mx_quantize_kernel<T, true, false, 8> : mx_quantize_kernel<T, false, false, 8>, p, 8)
-                           : go(vec ? mx_quantize_kernel<T, true, false, 4> : mx_quantize_kernel<T, false, false, 4>, p, 4);
+    if (k <= MX_NARROW) return narrow(p, vec);
+    return many ? go(vec ? mx_quantize_kernel<T, true, false, 8> : mx_quantize_kernel<T, false, false, 8>, p, 8)
+                : go(vec ? mx_quantize_kernel<T, true, false, 4> : mx_quantize_kernel<T, false, false, 4>, p, 4);
 }
 cudaError_t mx_dequantize(const void* codes, const void* scales, int64_t rows, int k, int dtype, void* out, int64_t out_stride,
                           void* stream) {
+    const bool many = mx_many(rows, k);
+    const int wide = mx_wide(k, MX_NT / 32, many);
+    auto narrow = [&](auto* p) {
+        using T = std::remove_pointer_t<decltype(p)>;
+        auto run = [&](auto kernel, int r) {
+            const int64_t each = r * MXN_PER * (MX_NT / 32);
+            return launch_pdl(kernel, dim3((unsigned)((rows + each - 1) / each)), MX_NT, 0, stream,
+                              static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, k, p, out_stride);
+        };
+        constexpr int R = sizeof(T) == 2 ? 8 : 4;  // of rows of 32 elements
+        return k <= 32   ? run(mx_dequantize_narrow_kernel<T, R>, R)
+               : k <= 64 ? run(mx_dequantize_narrow_kernel<T, R / 2>, R / 2)
+                         : run(mx_dequantize_narrow_kernel<T, R / 4>, R / 4);
+    };
     auto go = [&](auto kernel, auto* p, int per) {
-        return launch_pdl(kernel, mx_grid(rows, k, per, MX_NT / 32), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
-                          static_cast<const uint8_t*>(scales), rows, k, p, out_stride, mx_wide(k, MX_NT / 32), 0);
+        return launch_pdl(kernel, mx_grid(rows, k, per, MX_NT / 32, wide), MX_NT, 0, stream, static_cast<const uint8_t*>(codes),
+                          static_cast<const uint8_t*>(scales), rows, k, p, out_stride, wide, 0);
     };
     const bool vec = aligned16(out) && out_stride * (dtype == B2S_DTYPE_F32 ? 4 : 2) % 16 == 0;
     if (dtype == B2S_DTYPE_F32) {
         float* p = static_cast<float*>(out);
+        if (k <= MX_NARROW && vec) return narrow(p);
         return go(vec ? mx_dequantize_kernel<float, true, false, 4> : mx_dequantize_kernel<float, false, false, 4>, p, 4);
     }
     using T = unsigned short;
     T* p = static_cast<T*>(out);
-    return mx_many(rows, k) ? go(vec ? mx_dequantize_kernel<T, true, false, 8> : mx_dequantize_kernel<T, false, false, 8>, p, 8)
-                            : go(vec ? mx_dequantize_kernel<T, true, false, 4> : mx_dequantize_kernel<T, false, false, 4>, p, 4);
+    if (k <= MX_NARROW && vec) return narrow(static_cast<__nv_bfloat16*>(out));
+    return many ? go(vec ? mx_dequantize_kernel<T, true, false, 8> : mx_dequantize_kernel<T, false, false, 8>, p, 8)
+                : go(vec ? mx_dequantize_kernel<T, true, false, 4> : mx_dequantize_kernel<T, false, false, 4>, p, 4);
 }
 
 // ------------------------------------------------------------------ the product of few rows
@@ -594,15 +709,17 @@ MxWork mx_work(int64_t rows, int64_t k) {
 // waited for what came before it.
 cudaError_t mx8_quantize(const void* x, int64_t rows, int k, int64_t row_stride, void* codes, void* scales, bool beside, void* stream) {
     using T = unsigned short;
-    return launch_pdl(mx_quantize_kernel<T, true, true, 8>, mx_grid(rows, k, 8, MX8_NT / 32), MX8_NT, 0, stream,
+    const int wide = mx_wide(k, MX8_NT / 32, false);
+    return launch_pdl(mx_quantize_kernel<T, true, true, 8>, mx_grid(rows, k, 8, MX8_NT / 32, wide), MX8_NT, 0, stream,
                       static_cast<const T*>(x), row_stride, rows, k, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
-                      mx_wide(k, MX8_NT / 32), (int)beside);
+                      wide, (int)beside);
 }
 cudaError_t mx8_dequantize(const void* codes, const void* scales, int64_t rows, int k, void* out, bool beside, void* stream) {
     using T = unsigned short;
-    return launch_pdl(mx_dequantize_kernel<T, true, true, 8>, mx_grid(rows, k, 8, MX8_NT / 32), MX8_NT, 0, stream,
+    const int wide = mx_wide(k, MX8_NT / 32, false);
+    return launch_pdl(mx_dequantize_kernel<T, true, true, 8>, mx_grid(rows, k, 8, MX8_NT / 32, wide), MX8_NT, 0, stream,
                       static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, k, static_cast<T*>(out),
-                      (int64_t)k, mx_wide(k, MX8_NT / 32), (int)beside);
+                      (int64_t)k, wide, (int)beside);
 }
 
 }  // namespace b2s

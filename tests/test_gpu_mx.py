@@ -45,6 +45,23 @@ def test_quantize(pkg, rows, k, dtype):
     assert torch.equal(full[:rows, :nb].int() - 127, e.int()) and not bool(full[rows:].any()) and not bool(full[:, nb:].any())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 5, 129, 1000])
+@pytest.mark.parametrize("k", [1, 8, 32, 40, 60, 64, 72, 96, 100, 120, 128, 136, 576, 768])
+def test_short_rows(pkg, rows, k, dtype):
+    """Several rows a warp, aligned or not, from strided rows too; the layout's padding is zero."""
+    x = (torch.randn(rows, k + 8, device=DEV, generator=gen(rows + k)) * 3).to(dtype)
+    for part in (x[:, :k], x[:, :k].contiguous(), x[:, 3:3 + k]):
+        q = pkg.mx.quantize(part)
+        want = _mx.four(part)
+        assert torch.equal(_mx.unpack(q.codes, q.scales, k)[:, :k], want)
+        for out in (torch.float32, torch.bfloat16):
+            assert torch.equal(pkg.mx.dequantize(q, dtype=out).double(), want)
+        blocks = -(-k // 32)
+        tiles = q.scales.view(q.scales.shape[0], q.scales.shape[1], 2, 32, 4, 4).permute(0, 4, 3, 1, 2, 5).reshape(q.scales.shape[0] * 128, -1)
+        assert int(tiles[rows:].sum()) == 0 and int(tiles[:, blocks:].sum()) == 0
+
+
 def test_every_value_of_a_block(pkg):
     """Every fp32 magnitude near a rounding border of the grid, of either sign, at scales over the whole range."""
     grid = torch.tensor(_mx.E2M1, dtype=torch.float64)
