@@ -125,30 +125,14 @@ __device__ __forceinline__ float act_apply(float z, int act) {
     return act == ACT_RELU ? act_apply<ACT_RELU>(z)
                            : act == ACT_GELU ? act_apply<ACT_GELU>(z) : act == ACT_SILU ? act_apply<ACT_SILU>(z) : z;
 }
-// The slope of a pre-activation that came back from fp16: past 65504 (infinite there) it is what it is at 6e4.
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-    z = fabsf(z) > 6.0e4f ? copysignf(6.0e4f, z) : z;
-    if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (ACT == ACT_GELU) {
-        float e;
-        const float q = 0.5f * gelu_tail(z, &e);
-        return __fmaf_rn(0.398942280401432678f * z, e, z > 0.0f ? 1.0f - q : q);
-    }
-    if (ACT == ACT_SILU) {
-        const float s = __fdividef(1.0f, 1.0f + ex2(-1.44269504088896341f * z));
-        return s * (1.0f + z * (1.0f - s));
-    }
-    return 1.0f;
-}
-
 // 1 / x as __fdividef(1, x) gives it for x of at least 1, without its way for small x.
 __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The slopes of a pair, in packed arithmetic: act_slope's operations, one for one.  BOUNDED: finite pre-activations, of any size.
+// The slopes of a pair of pre-activations, in packed arithmetic.  BOUNDED: finite ones of any size; else ones that came back from
+// fp16: past 65504 (infinite there) they are what they are at 6e4.
 template <int ACT, bool BOUNDED>
 __device__ __forceinline__ float2 act_slope_pair(float2 z) {
     auto both = [](float x) { return make_float2(x, x); };
@@ -179,7 +163,8 @@ __device__ __forceinline__ float2 act_slope_pair(float2 z) {
         const float2 s = make_float2(rcp(d.x), rcp(d.y));
         return __fmul2_rn(s, __ffma2_rn(z, __ffma2_rn(both(-1.0f), s, both(1.0f)), both(1.0f)));
     }
-    return make_float2(act_slope<ACT>(z.x), act_slope<ACT>(z.y));
+    auto rectifier = [](float x) { return x > 0.0f ? 1.0f : (x != x ? x : 0.0f); };
+    return make_float2(rectifier(z.x), rectifier(z.y));
 }
 
 // Shared-memory matrix descriptor of an operand with m (or n) contiguous, 128-byte swizzle: blocks of [64 k rows x 64
@@ -387,23 +372,8 @@ __device__ __forceinline__ void keep_z8(const GemmArgs& a, const float* v, int r
     a.z8_scale[(int64_t)(n >> 5) * a.M + row] = (uint8_t)code;
 }
 
-// Up to 8 bf16 of a row from column n (N columns), `vec`: the row is 16-byte aligned and n a multiple of 8.
-__device__ __forceinline__ void load8(const void* row, int n, int N, bool vec, float (&x)[8]) {
-    const unsigned short* p = static_cast<const unsigned short*>(row) + n;
-    if (vec && n + 8 <= N) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[2 * j] = __uint_as_float(w[j] << 16);
-            x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = n + j < N ? bf16_bits_to_f(__ldg(p + j)) : 0.0f;
-    }
-}
-// The same stored, each value rounded once to bf16 (the output's type).
+// Up to 8 values of a row from column n (N columns), each rounded once to bf16 (the output's type); `vec`: the row is 16-byte
+// aligned and n a multiple of 8.
 __device__ __forceinline__ void store8(void* row, int n, int N, bool vec, const float* x) {
     __nv_bfloat16* p = static_cast<__nv_bfloat16*>(row) + n;
     if (vec && n + 8 <= N) {

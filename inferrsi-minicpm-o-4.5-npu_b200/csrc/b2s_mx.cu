@@ -44,9 +44,6 @@ struct MxGrid {
     }
 };
 
-__device__ __forceinline__ float mx_value(const float* p) { return __ldg(p); }
-__device__ __forceinline__ float mx_value(const unsigned short* p) { return bf16_bits_to_f(__ldg(p)); }
-
 // 8 elements of a row as they lie: bf16 pairs or fp32 words.
 template <typename T>
 struct MxWords {
@@ -80,7 +77,7 @@ __device__ __forceinline__ MxWords<T> mx_words(const T* p, int64_t n) {
     MxWords<T> r;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) * 2; ++i) {
-        if constexpr (sizeof(T) == 4) r.w[i] = i < n ? __float_as_uint(mx_value(p + i)) : 0u;
+        if constexpr (sizeof(T) == 4) r.w[i] = i < n ? __float_as_uint(__ldg(p + i)) : 0u;
         else r.w[i] = (2 * i < n ? (uint32_t)__ldg(p + 2 * i) : 0u) | (2 * i + 1 < n ? (uint32_t)__ldg(p + 2 * i + 1) << 16 : 0u);
     }
     return r;
