@@ -90,29 +90,43 @@ struct GemmArgs {
     const float* g_h;
 };
 
-// 2 (1 - Phi(|z|)) = erfc(|z| / sqrt 2), and e^(-z^2 / 2), which the slope needs too: the tail is t P(t) e^(-z^2 / 2) with
+__device__ __forceinline__ float fma_rn(float a, float b, float c) { return __fmaf_rn(a, b, c); }
+__device__ __forceinline__ float2 fma_rn(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ void spread(float x, float& v) { v = x; }
+__device__ __forceinline__ void spread(float x, float2& v) { v = make_float2(x, x); }
+// gelu's tail, 2 (1 - Phi(|z|)) = erfc(|z| / sqrt 2), is t P(t) e^(-z^2 / 2) with
 // t = 1 / (1 + 0.363 |z|) and P the polynomial of degree 6 whose largest relative error over |z| <= 14.5 is least (a linear
 // program over a grid: 8e-7).  For negative z the result is z times the tail, so that the error has to be relative: with
 // fp32's arithmetic it is below 2e-6 down to z = -5 and 8e-6 at -13 (the exponent's own rounding), where the result leaves
 // fp32's normal range; a half step of bf16 is 2e-3 at least.
-__device__ __forceinline__ float gelu_tail(float z, float* e) {
-    const float a = fabsf(z), t = __fdividef(1.0f, __fmaf_rn(0.363f, a, 1.0f));
-    *e = ex2(-0.72134752044448170f * a * a);
-    float p = 0.096218183507f;
-    p = __fmaf_rn(p, t, -0.358431707466f);
-    p = __fmaf_rn(p, t, 0.346512311336f);
-    p = __fmaf_rn(p, t, 0.061501895887f);
-    p = __fmaf_rn(p, t, 0.278014403086f);
-    p = __fmaf_rn(p, t, 0.286393762026f);
-    p = __fmaf_rn(p, t, 0.289791861116f);
-    return p * t * *e;
+constexpr float GELU_T = 0.363f, GELU_E = -0.72134752044448170f;  // t's factor; of z^2, the exponent of 2
+// s P(t) of a value or a pair, s a power of two.
+template <typename V>
+__device__ __forceinline__ V gelu_poly(V t, float s) {
+    constexpr float C[7] = {0.096218183507f, -0.358431707466f, 0.346512311336f, 0.061501895887f,
+                            0.278014403086f, 0.286393762026f,  0.289791861116f};
+    V p, c;
+    spread(s * C[0], p);
+#pragma unroll
+    for (int j = 1; j < 7; ++j) {
+        spread(s * C[j], c);
+        p = fma_rn(p, t, c);
+    }
+    return p;
 }
+__device__ __forceinline__ float gelu_tail(float z) {
+    const float a = fabsf(z), t = __fdividef(1.0f, __fmaf_rn(GELU_T, a, 1.0f));
+    return gelu_poly(t, 1.0f) * t * ex2(GELU_E * a * a);
+}
+// The activations, which all epilogues take alike: act(-infinity) is the limit, 0, as is the slope there, so that the infinity is
+// taken for a value whose tail is zero (infinity times that zero would be NaN); act(infinity) is infinity.
+constexpr float ACT_FAR = 3.0e38f;
 template <int ACT>
 __device__ __forceinline__ float act_apply(float z) {
     if (ACT == ACT_RELU) return fmax_nan(z, 0.0f);
+    if (ACT == ACT_GELU || ACT == ACT_SILU) z = fmax_nan(z, -ACT_FAR);
     if (ACT == ACT_GELU) {
-        float e;
-        const float q = 0.5f * gelu_tail(z, &e);
+        const float q = 0.5f * gelu_tail(z);
         return z * (z > 0.0f ? 1.0f - q : q);
     }
     if (ACT == ACT_SILU) {  // z / (1 + e^-z); below zero z e^z / (1 + e^z), e^z by halves, as it leaves the range before z e^z does
@@ -142,17 +156,11 @@ __device__ __forceinline__ float2 act_slope_pair(float2 z) {
     }
     if (ACT == ACT_GELU) {
         const float2 m = make_float2(fabsf(z.x), fabsf(z.y));
-        const float2 d = __ffma2_rn(both(0.363f), m, both(1.0f));
+        const float2 d = __ffma2_rn(both(GELU_T), m, both(1.0f));
         const float2 t = make_float2(rcp(d.x), rcp(d.y));
-        const float2 x = __fmul2_rn(__fmul2_rn(both(-0.72134752044448170f), m), m);
+        const float2 x = __fmul2_rn(__fmul2_rn(both(GELU_E), m), m);
         const float2 e = make_float2(ex2(x.x), ex2(x.y));
-        float2 p = both(0.096218183507f);
-        p = __ffma2_rn(p, t, both(-0.358431707466f));
-        p = __ffma2_rn(p, t, both(0.346512311336f));
-        p = __ffma2_rn(p, t, both(0.061501895887f));
-        p = __ffma2_rn(p, t, both(0.278014403086f));
-        p = __ffma2_rn(p, t, both(0.286393762026f));
-        p = __ffma2_rn(p, t, both(0.289791861116f));
+        const float2 p = gelu_poly(t, 1.0f);
         const float2 q = __fmul2_rn(both(0.5f), __fmul2_rn(__fmul2_rn(p, t), e));
         const float2 o = __ffma2_rn(both(-1.0f), q, both(1.0f));
         return __ffma2_rn(__fmul2_rn(both(0.398942280401432678f), z), e, make_float2(z.x > 0.0f ? o.x : q.x, z.y > 0.0f ? o.y : q.y));

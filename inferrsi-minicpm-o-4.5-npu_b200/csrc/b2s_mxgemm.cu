@@ -185,28 +185,22 @@ __device__ __forceinline__ void turn_rows(unsigned char* st, uint32_t (&q)[16], 
 }
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-// The activations of pairs, in packed arithmetic, in as few operations as they take: with gelu, bias and residual the epilogue's
-// instructions are what a tile of 4096 k waits for.  gelu(z) = max(z, 0) - |z| q with act_apply's tail q = 1 - Phi(|z|) (its
-// polynomial halved); silu as there, e^z by halves.
+// The activations of pairs, act_apply's in packed arithmetic, in as few operations as they take: with gelu, bias and residual the
+// epilogue's instructions are what a tile of 4096 k waits for.  gelu(z) = max(z, 0) - |z| q with act_apply's tail q = 1 - Phi(|z|)
+// (its polynomial halved); silu as there, e^z by halves.
 template <int ACT>
 __device__ __forceinline__ float2 act_pair(float2 z) {
     // finite, so that infinity times the tail's zero is no NaN; NaN comes through z itself
-    const float2 m = make_float2(fminf(fabsf(z.x), 3.0e38f), fminf(fabsf(z.y), 3.0e38f));
+    const float2 m = make_float2(fminf(fabsf(z.x), ACT_FAR), fminf(fabsf(z.y), ACT_FAR));
     if (ACT == ACT_RELU) return make_float2(fmax_nan(z.x, 0.0f), fmax_nan(z.y, 0.0f));
     if (ACT == ACT_GELU) {
-        const float2 d = __ffma2_rn(both(0.363f), m, both(1.0f)), t = make_float2(rcp(d.x), rcp(d.y));
-        const float2 x = __fmul2_rn(__fmul2_rn(both(-0.72134752044448170f), m), m);
-        float2 p = both(0.5f * 0.096218183507f);
-        p = __ffma2_rn(p, t, both(0.5f * -0.358431707466f));
-        p = __ffma2_rn(p, t, both(0.5f * 0.346512311336f));
-        p = __ffma2_rn(p, t, both(0.5f * 0.061501895887f));
-        p = __ffma2_rn(p, t, both(0.5f * 0.278014403086f));
-        p = __ffma2_rn(p, t, both(0.5f * 0.286393762026f));
-        p = __ffma2_rn(p, t, both(0.5f * 0.289791861116f));
-        const float2 q = __fmul2_rn(__fmul2_rn(p, t), make_float2(ex2(x.x), ex2(x.y)));
+        const float2 d = __ffma2_rn(both(GELU_T), m, both(1.0f)), t = make_float2(rcp(d.x), rcp(d.y));
+        const float2 x = __fmul2_rn(__fmul2_rn(both(GELU_E), m), m);
+        const float2 q = __fmul2_rn(__fmul2_rn(gelu_poly(t, 0.5f), t), make_float2(ex2(x.x), ex2(x.y)));
         return __ffma2_rn(make_float2(-m.x, -m.y), q, make_float2(fmax_nan(z.x, 0.0f), fmax_nan(z.y, 0.0f)));
     }
     if (ACT == ACT_SILU) {
+        z = make_float2(fmax_nan(z.x, -ACT_FAR), fmax_nan(z.y, -ACT_FAR));
         const float2 x = __fmul2_rn(both(-0.72134752044448170f), m), h = make_float2(ex2(x.x), ex2(x.y));
         const float2 w = __fmul2_rn(__fmul2_rn(z, h), h), d = __ffma2_rn(h, h, both(1.0f));
         return __fmul2_rn(make_float2(z.x < 0.0f ? w.x : z.x, z.y < 0.0f ? w.y : z.y), make_float2(rcp(d.x), rcp(d.y)));

@@ -96,8 +96,8 @@ def linear(x: Union[torch.Tensor, MXTensor], weight: MXTensor, bias: Optional[to
            status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(x^ weight^T + bias) + residual``: x [..., in] bfloat16 (rounded to 4 bits within the call) or an ``MXTensor``,
     weight an ``MXTensor`` [out, in], bias [out] and residual [..., out] bfloat16; any in and out.  ``activation``: None,
-    "relu", "gelu" or "silu".  Differentiable once, in x, bias and residual; the gradient of x takes the weight in bfloat16,
-    out * in * 2 bytes of workspace."""
+    "relu", "gelu" or "silu" (0 at -infinity).  Differentiable once, in x, bias and residual; the gradient of x takes
+    the weight in bfloat16, out * in * 2 bytes of workspace."""
     ts._need_cuda(x, bias, residual, status)
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation: {activation!r}")

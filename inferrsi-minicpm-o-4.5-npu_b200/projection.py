@@ -32,8 +32,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
            status: Optional[torch.Tensor] = None, checkpoint: Optional[str] = None) -> torch.Tensor:
     """``act(x weight^T + bias) + residual``: x [..., in], weight [out, in], bias [out], residual [..., out], all bf16;
-    in a multiple of 8, any out.  ``activation``: None, "relu", "gelu" or "silu".  ``checkpoint``: None, or "e4m3" to keep
-    8 bits of x and of the pre-activation for the backward pass."""
+    in a multiple of 8, any out.  ``activation``: None, "relu", "gelu" or "silu" (0 at -infinity).  ``checkpoint``: None, or
+    "e4m3" to keep 8 bits of x and of the pre-activation for the backward pass."""
     ts._need_cuda(x, weight, bias, residual, status)
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation: {activation!r}")
