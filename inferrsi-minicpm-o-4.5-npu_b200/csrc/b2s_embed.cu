@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(EM_NT) embed_kernel(const int64_t* tokens, int
         Unit<E, VEC> v;
         v.zero();
         if (t >= 0) v.add(q[j]);
-        if (u0 + 32 * j < units) v.store(dst, u0 + 32 * j, s);
+        if (u0 + 32 * j < units) v.store(dst, u0 + 32 * j, t < 0 ? 1.0f : s);  // padding is +0 whatever the scale's sign
     }
 }
 
