@@ -481,7 +481,7 @@ int b2s_mx_linear(const b2s_mx_linear_args* args, void* stream);
  * gradient, z without an activation); args->preact is NULL.
  *   x_codes [rows][ceil(in / 32) * 32] bytes, x_scales [ceil(in / 32)][rows] bytes; z likewise with out; codes 16-byte aligned
  * The gradient takes x and z as they were kept: grad_weight = dz^T x^, dz = grad_out act'(z^); args' x and preact are not read.
- * `workspace`: b2s_linear_checkpoint(_grad)_workspace bytes.
+ * `workspace`: b2s_linear_checkpoint(_grad)_workspace bytes; b2s_linear_grad_workspace's where args->grad_weight is NULL.
  */
 typedef struct b2s_linear_kept {
     void* x_codes;

@@ -1071,8 +1071,8 @@ int linear_backward(const b2s_linear_grad_args* l, const b2s_linear_kept* kept, 
     }
     int64_t need = 0, plain = 0;
     b2s_linear_grad_workspace(l->rows, l->in_features, l->out_features, &plain);
-    if (kept) b2s_linear_checkpoint_grad_workspace(l->rows, l->in_features, l->out_features, &need);
-    else need = plain;
+    if (kept && l->grad_weight) b2s_linear_checkpoint_grad_workspace(l->rows, l->in_features, l->out_features, &need);
+    else need = plain;  // x comes back to bf16 for the weight's gradient alone
     const bool z_ok = kept ? kept->z_codes && kept->z_scales && aligned16(kept->z_codes)
                            : l->preact && aligned16(l->preact) && l->preact_row_stride >= l->out_features && l->preact_row_stride % 8 == 0;
     const bool x_ok = kept ? kept->x_codes && kept->x_scales && aligned16(kept->x_codes)

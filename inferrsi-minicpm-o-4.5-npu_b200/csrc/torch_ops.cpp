@@ -960,8 +960,8 @@ std::tuple<Tensor, Tensor, Tensor> linear_kept_grad_cuda(const Tensor& grad_out,
     a.grad_x = want_x ? dx.data_ptr() : nullptr;
     a.grad_weight = want_weight ? dw.data_ptr() : nullptr;
     a.grad_bias = want_bias ? db.data_ptr() : nullptr;
-    check_rc(b2s_linear_checkpoint_grad_workspace(a.rows, a.in_features, a.out_features, &a.workspace_bytes),
-             "b2s_linear_checkpoint_grad_workspace");
+    const auto bytes = want_weight ? b2s_linear_checkpoint_grad_workspace : b2s_linear_grad_workspace;
+    check_rc(bytes(a.rows, a.in_features, a.out_features, &a.workspace_bytes), "b2s_linear_checkpoint_grad_workspace");
     Tensor ws = workspace(a.workspace_bytes, g);
     a.workspace = ws.data_ptr();
     a.status = status_ptr(status, g);
