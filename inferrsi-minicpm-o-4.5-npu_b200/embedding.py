@@ -14,7 +14,6 @@ graph.  Differentiable once, in the table.
 
 from __future__ import annotations
 
-import math
 from typing import Optional, Union
 
 import torch
@@ -23,6 +22,8 @@ from . import _native
 from . import mx
 from . import talker_sampler as ts
 
+_F32_MAX = torch.finfo(torch.float32).max
+
 
 def lookup(tokens: torch.Tensor, table: Union[torch.Tensor, "mx.MXTensor"], *, scale: float = 1.0,
            status: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -30,8 +31,8 @@ def lookup(tokens: torch.Tensor, table: Union[torch.Tensor, "mx.MXTensor"], *, s
     [*tokens.shape, width] in the table's type (bfloat16 from a 4-bit table)."""
     ts._need_cuda(tokens, table, status)
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale!r}")
+    if not abs(scale) <= _F32_MAX:
+        raise ValueError(f"scale must be finite in float32, got {scale!r}")
     if tokens.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"tokens must be int64 or int32, got {tokens.dtype}")
     t = tokens if tokens.dim() == 1 else tokens.reshape(-1)
