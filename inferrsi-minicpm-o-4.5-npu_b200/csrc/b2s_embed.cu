@@ -2,15 +2,17 @@
 // t_i = v, in ascending order of i.  Ids below 0 are padding: zeros, and no part in the gradient.  Ids past the table are
 // taken as padding too and set B2S_STATUS_TOKEN_RANGE.  No counterpart in the reference, whose models call torch's own.
 //
-// Forward: a copy of rows.  A warp takes a piece of one row, 16 bytes a lane and four loads in flight.  From a
-// microscaled table a lane decodes 8 elements.
+// Forward: a copy of rows.  A warp takes a piece of one row, 16 bytes a lane and load, as many loads in flight as the row's length
+// wants (one, two or four; eight of single elements).  From a microscaled table a lane decodes 8 elements a load.
 //
 // Gradient: the whole table's gradient is written once, so what bounds it is that write (1.24 GB for the Thinker's table)
 // and one read of the rows' gradients.  The positions are sorted by id without a sort of keys: a count per id (the atomic's
 // old value is the position's place among its id's, in order of arrival), the counts' prefix sums, and then each id's
 // positions put in ascending order, so that sums do not depend on who arrived first.  The sorted positions are summed in
 // chunks of 8 to 32, whatever ids they hold, one chunk a warp and part of a row, in order, in fp32: an id inside a chunk is
-// written at once, of one that goes on the sums are joined by whoever completes them, in order.
+// written at once, of one that goes on the sums are joined by whoever completes them, 16 neighbours at a time in a fixed tree.  Where
+// chunks cut an id's positions depends on how many positions lower ids have: the same call gives the same bits, another list
+// of tokens may add the same rows in another grouping.
 #include <string.h>
 
 #include <type_traits>
@@ -30,7 +32,9 @@ namespace {
 
 constexpr int EM_NT = 256;
 constexpr int EM_JOIN = 4;     // 2^4 sums joined at a time
-constexpr int EM_SHORT = 64;   // positions of an id that are put in order by comparison
+constexpr int EM_SHORT = 64;   // positions of an id that are put in order by comparison with all of its others
+constexpr int EM_MID = 512;    // ... that a CTA puts in order in shared memory; beyond, by bitmaps
+constexpr int EM_HUGE = 4096;  // ... beyond which several CTAs do, EM_PARTS at most
 constexpr int EM_BINS = 4096;  // at most, of ids counted together
 constexpr int EM_UNITS = 64;   // 16-byte units of a row that a warp takes
 constexpr int EM_ELEMENTS = 256;  // or single elements, of rows that are not aligned
@@ -38,8 +42,6 @@ constexpr int EM_ELEMENTS = 256;  // or single elements, of rows that are not al
 // 10.3 and 11.6), of bf16 64 (61; 77 with 256).
 constexpr int EM_WIDE = 128;
 __host__ __device__ constexpr int em_units(bool vec, int e) { return vec || e == 2 ? EM_UNITS : EM_WIDE; }
-constexpr int EM_MID = 512;    // ... by a CTA in shared memory; beyond, by bitmaps
-constexpr int EM_HUGE = 4096;  // ... by several CTAs, at most EM_PARTS
 constexpr int EM_PARTS = 64;
 constexpr int EM_WINDOW = 1 << 17;  // positions that a CTA's bitmap covers (16 KB)
 

@@ -108,7 +108,7 @@ __device__ __forceinline__ void mx_decode4_e4m3(uint32_t c, float (&v)[4]) {
     v[3] = y.y;
 }
 
-// Up to 8 values to bf16 or fp32, each rounded once to the output's type; `vec`: p is 16-byte aligned.
+// Up to 8 values to bf16, each rounded once; `vec`: p is 16-byte aligned.
 __device__ __forceinline__ void mx_store8(__nv_bfloat16* p, int n, bool vec, const float (&v)[8]) {
     if (vec && n == 8) {
         uint32_t w[4];
@@ -122,16 +122,6 @@ __device__ __forceinline__ void mx_store8(__nv_bfloat16* p, int n, bool vec, con
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < n) p[j] = __float2bfloat16_rn(v[j]);
-    }
-}
-__device__ __forceinline__ void mx_store8(float* p, int n, bool vec, const float (&v)[8]) {
-    if (vec && n == 8) {
-        __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
-        __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < n) p[j] = v[j];
     }
 }
 
