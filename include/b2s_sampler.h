@@ -420,9 +420,10 @@ int b2s_embedding_mx(const int64_t* tokens, int32_t n, const void* codes, const 
                      float scale, void* out, uint32_t* status, void* stream);
 
 /*
- * The lookup's gradient (ABI 8): grad_table[v] = scale * the sum of grad_out's rows i with tokens[i] = v, in ascending
- * order of i in fp32 (in pieces of up to 32, those in order), rounded once; zeros for ids that do not occur.  grad_table [vocab,
- * width] contiguous, `dtype` its and grad_out's.  The same call gives the same bits.
+ * The lookup's gradient (ABI 8): grad_table[v] = scale * the sum of grad_out's rows i with tokens[i] = v in fp32, rounded
+ * once; zeros for ids that do not occur.  Sums are of pieces of 8 to 32 positions, cut at fixed places of the list of all positions
+ * ordered by id, in ascending order of i within a piece, the pieces joined in a fixed tree.  grad_table [vocab, width] contiguous,
+ * `dtype` its and grad_out's.  The same call gives the same bits; an id's last bits depend on the other tokens of the call.
  */
 int b2s_embedding_grad_workspace(int32_t n, int32_t vocab, int32_t width, int64_t* bytes);
 int b2s_embedding_grad(const int64_t* tokens, int32_t n, const void* grad_out, int64_t grad_row_stride, int32_t dtype,

@@ -6,7 +6,9 @@ of training a head.  No counterpart in the reference, whose models call torch's 
 A token of ``PAD`` (any id below 0: what inactive rows sample) gives zeros and has no part in the gradient; an id past the
 table is taken the same way and sets 32 in ``status``.  The table is float32, bfloat16 or a microscaled 4-bit matrix
 (``mx.MXTensor``, no gradient; bfloat16 rows).  The gradient is the whole table's, in its type: every id's rows summed in
-fp32 in the order of their positions and rounded once, the same bits each time.
+fp32 and rounded once.  The sums are of pieces of 8 to 32 positions, cut at fixed places of the list of all positions ordered by
+id, in ascending order within a piece; an id's pieces are joined in a fixed tree.  The same call gives the same bits; where an id's
+pieces are cut, and with that its last bits, depends on the other tokens of the call.
 
 CUDA tensors only; on the current stream, without synchronising, keeping no state between calls; can be captured in a CUDA
 graph.  Differentiable once, in the table.
